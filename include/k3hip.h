@@ -454,6 +454,76 @@ int k3_mla_step_decode(const void *x, int x_dtype, const void *q_a, const float 
                        int64_t rope_dim, int64_t v_dim, int64_t kv_lora_rank, void *workspace,
                        int64_t workspace_bytes, void *stream);
 
+/* ---- latent attention over a 4-bit cache ------------------------------------------------ */
+
+/* A cached position is 512 latent values as MXFP4 -- packed uint8 [256] (element 2i in the low
+ * nibble of byte i), scales uint8 [16], one E8M0 byte per 32 values, as k3_mxfp4_decode reads
+ * them -- and rot, 64 rotary values in bf16: 400 bytes for the bf16 cache's 1152.  Buffers are
+ * [B, cap, .] with batch and row pitches in elements and contiguous rows.  Counterpart of the
+ * reference's optional quantised latent (air_llm/models/kimi_k3/mla_quant.py:64-116, group-affine
+ * there), which keeps the rotary part unquantised too.
+ *
+ * k3_mla_q4_append rounds new latents c [B, T, 512] and rotary rows r [B, T, 64] (each bf16 or fp32,
+ * pitches in elements) into positions start[b] + i, i < counts[b] <= T, of sequence b.
+ * start: int32 [B] on the device, or null: start0 for all (then start0 + T <= cap is checked here);
+ * counts: int32 [B] on the device, or null: T.  Positions outside 0 .. cap - 1 are left out.
+ * A group of 32 with largest magnitude m gets the scale 2^e, e = floor(log2 m) - 2, one more if
+ * m > 7 * 2^e, its byte e + 127 held to 2..252; codes round to nearest, ties to even.  A group with
+ * a NaN or an infinity gets byte 255: the position is NaN to every query that sees it.
+ * c 16-byte aligned with pitches of whole 16 bytes; packed 4-byte aligned, pitches multiples of 4. */
+int k3_mla_q4_append(const void *c, int64_t c_batch, int64_t c_row, int c_dtype, const void *r, int64_t r_batch,
+                     int64_t r_row, int r_dtype, void *packed, int64_t p_batch, int64_t p_row, void *scales,
+                     int64_t s_batch, int64_t s_row, void *rot, int64_t rot_batch, int64_t rot_row,
+                     const int32_t *start, int64_t start0, const int32_t *counts, int64_t B, int64_t T, int64_t cap,
+                     int64_t kv_lora_rank, int64_t rope_dim, void *stream);
+
+/* Workspace bytes of k3_mla_q4_attention for the same sizes (weights: whether it is given a weight
+ * buffer).  No initialisation. */
+int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim, int64_t max_length, int out_dtype,
+                                 int weights);
+
+/* The absorbed attention of T queries of each of B sequences over the 4-bit cache, causal: query t of
+ * sequence b's first counts[b] sees positions 0 .. lengths[b] - counts[b] + t, so the last one sees the whole
+ * sequence.
+ *   o[b,t,h] = W_UV[h] (softmax_j(scale (q_nope[b,t,h] W_UK[h] . lat[b,j] + q_rot[b,t,h] . rot[b,j])) lat[b])
+ *   weight[b,j] += the sum over t and h of those probabilities    (weight null: not formed)
+ * q_nope [B, T, H, nope], q_rot [B, T, H, 64]: bf16 or fp32 (both the same), pitches in elements, multiples
+ *   of 4; w_uk [H, nope, 512], w_uv [H, v, 512] bf16;
+ * lengths int32 [B] on the device (taken as 0 .. max_length) or null: max_length for all; counts int32 [B] on
+ *   the device (taken as 0 .. T) or null: T.  Every sequence has max_length readable rows;
+ * gate [B, T, H, v] fp32 logits or null: o times sigmoid(gate);
+ * out [B, T, H, v] contiguous, out_dtype; weight fp32 rows w_batch floats apart, positions past lengths[b] left as
+ *   they are.
+ * A query that sees nothing (also: t >= counts[b]) gets zeros and adds nothing to weight.  Deterministic.  The cache's
+ * values enter exactly; queries and probabilities to about 2^-17 of their group's largest for a bf16 out without
+ * weight, else (queries) 2^-22 and, for an fp32 out, (probabilities) 2^-25; sums and softmax in fp32.
+ * nope a multiple of 8 up to 256, v one up to 1024, H <= 4096, B H <= 65536, max_length <= 2^24.  Pointers 16-byte
+ * aligned; p_row and p_batch multiples of 16, rot pitches of 8.
+ * Counterpart of MLAAttention.__call__ over a QuantLatent cache (air_llm/models/kimi_k3/attention_mla.py:193-212). */
+int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t qn_token, int64_t qn_head, const void *q_rot,
+                        int64_t qr_batch, int64_t qr_token, int64_t qr_head, int q_dtype, const void *w_uk,
+                        const void *w_uv, const void *packed, int64_t p_batch, int64_t p_row, const void *scales,
+                        int64_t s_batch, int64_t s_row, const void *rot, int64_t rot_batch, int64_t rot_row,
+                        const int32_t *lengths, const int32_t *counts, int64_t max_length, int64_t B, int64_t T, int64_t H,
+                        int64_t kv_lora_rank, int64_t rope_dim, int64_t nope_dim, int64_t v_dim, float scale,
+                        const float *gate, void *out, int out_dtype, float *weight, int64_t w_batch, void *workspace,
+                        int64_t workspace_bytes, void *stream);
+
+/* ---- eviction by accumulated attention weight --------------------------------------------- */
+
+/* Of sequence b's n = lengths[b] positions (0 .. max_length; lengths null: max_length for all) the first
+ * `sink`, the last `recent` and, of those between, the ones with the largest weight[b] stay, min(n, keep) in all (sink + recent
+ * <= keep; ties: the lowest position; NaN counts below all).  index [B, keep] int32: the kept positions in ascending order, then -1;
+ * kept [B] int32: how many.  Then row i of every dst buffer is row index[i] of its src, and rows kept[b] .. dst_rows - 1
+ * are zeroed.  buffers <= 8; the six arrays are host arrays of one entry per buffer: pointers, and batch and row pitches and row
+ * sizes in bytes.  weight rows are w_batch floats apart.  src and dst must not overlap.  No counterpart in the
+ * reference, whose cache only grows. */
+int k3_cache_evict(const float *weight, int64_t w_batch, const int32_t *lengths, int64_t max_length, int64_t B,
+                   int64_t keep, int64_t sink, int64_t recent, int32_t *index, int32_t *kept, int64_t buffers,
+                   const void *const *src, const int64_t *src_batch, const int64_t *src_row, void *const *dst,
+                   const int64_t *dst_batch, const int64_t *dst_row, const int64_t *row_bytes, int64_t dst_rows,
+                   void *stream);
+
 /* ---- Kimi Delta Attention recurrent step (one token) -------------------------------------- */
 
 /* For every value head h (q/k head h / (v_heads / qk_heads)), on the fp32 state

@@ -1,0 +1,209 @@
+// Eviction from a cache by accumulated attention weight: of a sequence's n positions the first `sink`, the last `recent` and,
+// of those between, the ones with the largest weights stay, `keep` in all (all n where n <= keep), and move to the
+// front of new buffers in their order.
+//
+// Two launches.  select (a block per sequence): the weights become keys that order as whole numbers do (NaN below
+// all, -0 as 0); the key of the last one to stay is found 11, 11 and 10 bits at a time from a histogram of the keys
+// that still match, kept in LDS; of the positions with exactly that key the lowest stay.  Every thread owns a
+// contiguous run of positions, so two counts per thread and one scan give each kept position its place, in order, with no
+// atomics on the result.  gather: rows of every buffer, 16 bytes a thread.
+// Bound by the latency of the histogram passes over LDS (select), by HBM (gather).
+#include <algorithm>
+
+#include "k3_common.h"
+
+namespace k3 {
+namespace {
+
+constexpr int kThreads = 1024, kBins = 2048, kCopies = 4, kMaxBuffers = 8;
+
+struct SelectArgs {
+    const float *weight;
+    int64_t ld;
+    const int32_t *lengths;
+    int length, cap, keep, sink, recent;
+    int32_t *index, *kept;
+};
+
+__device__ __forceinline__ uint32_t order_key(float f) {
+    const uint32_t u = __float_as_uint(f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;               // NaN
+    if (u == 0x80000000u) return 0x80000000u;                     // -0 as 0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// exclusive prefix of v over the block's threads, and the total
+__device__ __forceinline__ int block_prefix(int v, int *sums, int &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(s, o);
+        if (lane >= o) s += x;
+    }
+    if (lane == 63) sums[wave] = s;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+        const int x = sums[w];
+        before += w < wave ? x : 0;
+        total += x;
+    }
+    __syncthreads();
+    return before + s - v;
+}
+
+__global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
+    __shared__ int hist[kBins * kCopies];
+    __shared__ int sums[kThreads / 64];
+    __shared__ int found[2];
+    const int tid = threadIdx.x, b = blockIdx.x;
+    const int n = a.lengths ? min(max(a.lengths[b], 0), a.cap) : a.length;
+    int32_t *index = a.index + static_cast<int64_t>(b) * a.keep;
+    const float *w = a.weight + b * a.ld;
+    const int nk = min(n, a.keep);
+    if (tid == 0) a.kept[b] = nk;
+    for (int i = nk + tid; i < a.keep; i += kThreads) index[i] = -1;
+    if (n <= a.keep) {
+        for (int i = tid; i < n; i += kThreads) index[i] = i;
+        return;
+    }
+    // the middle positions lo .. hi - 1, `need` of them stay
+    const int lo = a.sink, hi = n - a.recent;
+    int need = a.keep - a.sink - a.recent;
+    for (int i = tid; i < a.sink; i += kThreads) index[i] = i;
+    for (int i = tid; i < a.recent; i += kThreads) index[a.keep - a.recent + i] = hi + i;
+    if (need == 0) return;
+    uint32_t prefix = 0;     // the bits of the threshold key found so far
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
+        for (int i = tid; i < kBins * kCopies; i += kThreads) hist[i] = 0;
+        __syncthreads();
+        for (int i = lo + tid; i < hi; i += kThreads) {
+            const uint32_t k = order_key(w[i]);
+            if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[((k >> shift) & (bins - 1)) * kCopies + (tid & (kCopies - 1))], 1);
+        }
+        __syncthreads();
+        // thread t counts bins 2 t' and 2 t' + 1 from the top: t' = 1023 - t
+        const int top = kThreads - 1 - tid;
+        int c[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            c[x] = 0;
+#pragma unroll
+            for (int k = 0; k < kCopies; ++k) c[x] += hist[(2 * top + x) * kCopies + k];
+        }
+        int total;
+        const int above = block_prefix(c[0] + c[1], sums, total);   // keys in higher bins
+        if (above < need && above + c[1] >= need) found[0] = 2 * top + 1, found[1] = need - above;
+        if (above + c[1] < need && above + c[1] + c[0] >= need) found[0] = 2 * top, found[1] = need - above - c[1];
+        __syncthreads();
+        prefix = (prefix << bits) | static_cast<uint32_t>(found[0]);
+        need = found[1];
+        __syncthreads();
+    }
+    // keys above the threshold stay, and the first `need` at it
+    const int run = (hi - lo + kThreads - 1) / kThreads, i0 = min(hi, lo + tid * run), i1 = min(hi, i0 + run);
+    int more = 0, same = 0, total;
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t k = order_key(w[i]);
+        more += k > prefix;
+        same += k == prefix;
+    }
+    const int same_before = block_prefix(same, sums, total);
+    const int take = min(max(need - same_before, 0), same);
+    int at = a.sink + block_prefix(more + take, sums, total), left = take;
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t k = order_key(w[i]);
+        bool stay = k > prefix;
+        if (k == prefix && left > 0) stay = true, --left;
+        if (stay) index[at++] = i;
+    }
+}
+
+struct GatherArgs {
+    const char *src[kMaxBuffers];
+    char *dst[kMaxBuffers];
+    int64_t src_b[kMaxBuffers], src_r[kMaxBuffers], dst_b[kMaxBuffers], dst_r[kMaxBuffers];   // bytes
+    int units[kMaxBuffers], unit[kMaxBuffers];                                                // of a row; bytes of a unit: 16, 4 or 1
+    const int32_t *index;
+    int buffers, keep, rows;
+};
+constexpr int kGatherRows = 64;
+
+template <typename U>
+__device__ __forceinline__ void copy_rows(const GatherArgs &a, int x, int b, int r0, int nrows, const int *at) {
+    const int units = a.units[x];
+    const char *src = a.src[x] + b * a.src_b[x];
+    char *dst = a.dst[x] + b * a.dst_b[x] + r0 * a.dst_r[x];
+    for (int i = threadIdx.x; i < nrows * units; i += 256) {
+        const int r = i / units, u = i % units, s = at[r];
+        U v{};
+        if (s >= 0) v = *reinterpret_cast<const U *>(src + s * a.src_r[x] + u * static_cast<int>(sizeof(U)));
+        *reinterpret_cast<U *>(dst + r * a.dst_r[x] + u * static_cast<int>(sizeof(U))) = v;
+    }
+}
+
+__global__ __launch_bounds__(256) void gather_kernel(GatherArgs a) {
+    __shared__ int at[kGatherRows];
+    const int b = blockIdx.y, r0 = blockIdx.x * kGatherRows, nrows = min(kGatherRows, a.rows - r0);
+    if (static_cast<int>(threadIdx.x) < nrows) {
+        const int r = r0 + threadIdx.x;
+        at[threadIdx.x] = r < a.keep ? a.index[static_cast<int64_t>(b) * a.keep + r] : -1;
+    }
+    __syncthreads();
+    for (int x = 0; x < a.buffers; ++x) {
+        if (a.unit[x] == 16)
+            copy_rows<uint4>(a, x, b, r0, nrows, at);
+        else if (a.unit[x] == 4)
+            copy_rows<uint32_t>(a, x, b, r0, nrows, at);
+        else
+            copy_rows<uint8_t>(a, x, b, r0, nrows, at);
+    }
+}
+
+}  // namespace
+}  // namespace k3
+
+using namespace k3;
+
+extern "C" int k3_cache_evict(const float *weight, int64_t w_batch, const int32_t *lengths, int64_t max_length, int64_t B, int64_t keep,
+                              int64_t sink, int64_t recent, int32_t *index, int32_t *kept, int64_t buffers, const void *const *src,
+                              const int64_t *src_batch, const int64_t *src_row, void *const *dst, const int64_t *dst_batch,
+                              const int64_t *dst_row, const int64_t *row_bytes, int64_t dst_rows, void *stream) {
+    if (B == 0) return K3_OK;
+    if (!kept || (keep > 0 && !index) || (max_length > 0 && !weight) ||
+        (buffers > 0 && (!src || !src_batch || !src_row || !dst || !dst_batch || !dst_row || !row_bytes)))
+        return set_error(K3_ERR_NULL, "cache evict: null pointer");
+    if (B < 0 || B > 65535 || max_length < 0 || max_length > (1 << 30) || keep < 0 || keep > (1 << 30) || sink < 0 || recent < 0 ||
+        sink + recent > keep || w_batch < 0)
+        return set_error(K3_ERR_SHAPE, "cache evict: B=%lld, length=%lld, keep=%lld with sink=%lld and recent=%lld", (long long)B,
+                         (long long)max_length, (long long)keep, (long long)sink, (long long)recent);
+    if (buffers < 0 || buffers > kMaxBuffers || dst_rows < (buffers > 0 ? keep : 0) || dst_rows > (1 << 30))
+        return set_error(K3_ERR_SHAPE, "cache evict: %lld buffers (at most %d) of %lld rows for %lld kept", (long long)buffers, kMaxBuffers,
+                         (long long)dst_rows, (long long)keep);
+    GatherArgs g{};
+    for (int64_t x = 0; x < buffers; ++x) {
+        if (row_bytes[x] < 0 || row_bytes[x] > (1 << 20) || (row_bytes[x] > 0 && dst_rows > 0 && (!dst[x] || (max_length > 0 && !src[x]))))
+            return set_error(K3_ERR_SHAPE, "cache evict: buffer %lld", (long long)x);
+        if (src_row[x] < row_bytes[x] || dst_row[x] < row_bytes[x])
+            return set_error(K3_ERR_SHAPE, "cache evict: rows of buffer %lld overlap", (long long)x);
+        const int64_t all = row_bytes[x] | src_batch[x] | src_row[x] | dst_batch[x] | dst_row[x] |
+                            static_cast<int64_t>(reinterpret_cast<uintptr_t>(src[x]) | reinterpret_cast<uintptr_t>(dst[x]));
+        g.unit[x] = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+        g.units[x] = static_cast<int>(row_bytes[x] / g.unit[x]);
+        g.src[x] = static_cast<const char *>(src[x]), g.dst[x] = static_cast<char *>(dst[x]);
+        g.src_b[x] = src_batch[x], g.src_r[x] = src_row[x], g.dst_b[x] = dst_batch[x], g.dst_r[x] = dst_row[x];
+    }
+    auto st = static_cast<hipStream_t>(stream);
+    const SelectArgs s{weight, w_batch, lengths, static_cast<int>(max_length), static_cast<int>(max_length), static_cast<int>(keep),
+                       static_cast<int>(sink), static_cast<int>(recent), index, kept};
+    select_kernel<<<dim3(static_cast<unsigned>(B)), kThreads, 0, st>>>(s);
+    int rc = check_hip(hipGetLastError(), "cache evict: select launch");
+    if (rc || buffers == 0 || dst_rows == 0) return rc;
+    g.index = index, g.buffers = static_cast<int>(buffers), g.keep = static_cast<int>(keep), g.rows = static_cast<int>(dst_rows);
+    gather_kernel<<<dim3(static_cast<unsigned>(cdiv(dst_rows, kGatherRows)), static_cast<unsigned>(B)), 256, 0, st>>>(g);
+    return check_hip(hipGetLastError(), "cache evict: gather launch");
+}

@@ -1,0 +1,88 @@
+// The 4-bit latent cache's queries and rows, as the attention and the weight-sum kernels take them.
+//
+// A cached position is 512 latent values as MXFP4 (256 bytes of E2M1 codes, element 2i in the low
+// nibble of byte i, and 16 E8M0 scale bytes, one per 32 values) and 64 rotary values in bf16.
+//
+// Scores.  The matrix cores take the codes as they are: v_mfma_scale_f32_16x16x128_f8f6f4 reads an
+// E2M1 operand with one E8M0 byte per row and 32 columns, which is the cache's own layout: lane
+// (row r, quarter q) holds 16 bytes, group 4 q + s in step s of four (the order of a sum's columns is free, and
+// in this one the lane's four scale bytes are one dword of the row).  The absorbed query qa (fp32) enters as a sum of E2M3 terms (6 bits: 1 + 2 + 3) that share the other
+// operand's place, each with an E8M0 byte per 32 columns:
+//     qa = t1 + t2 + t3 + t4 (+ t5),   |t1| <= 7.5 s, the next terms' units s / 16, s / 2^9, s / 2^14, s / 2^19
+// Each term rounds what is left to nearest; E2M3's step below 4 is at most 1/4, so a term leaves at most
+// 1/8 of its unit (the first, up to 7.5: 1/4): 2^-17 s after four terms, 2^-22 s after five, where the group's
+// largest magnitude is above 3.75 s.  E2M1 x E2M3 products run at four times bf16's rate (measured: 4128 against
+// 1107 TFLOP/s), so five terms cost 1.25 bf16 products and need no decoded keys; two bf16 terms (2^-17) would cost
+// two products and the decoding.  The rotary columns are bf16 on both sides, the query in two or three terms.
+//
+// Query operands of 16 rows (a row: one head of one query), `terms` latent and `rterms` rotary terms:
+//     [term][step]                  64 lanes x 16 bytes, then 64 x 8: the lane's 32 codes, 192 bits
+//     [term]                        64 lanes x 4 bytes: the lane's scale byte of every step
+//     [rotary term][step of 32]     64 lanes x 16 bytes: 8 bf16 columns
+// where lane (q, r) = 16 q + r holds row r, columns 32 (4 q + step) .. +32 (rotary: 32 step + 8 q .. +8).
+#pragma once
+
+#include "k3_common.h"
+
+namespace k3 {
+namespace {
+
+constexpr int kQ4Lat = 512, kQ4Rope = 64, kQ4Steps = kQ4Lat / 128;
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef float f32x32_t __attribute__((ext_vector_type(32)));
+
+__host__ __device__ constexpr int q4_tile_bytes(int terms, int rterms) { return terms * 6400 + rterms * 2048; }
+__host__ __device__ constexpr int q4_code_at(int term, int step) { return (term * kQ4Steps + step) * 1536; }
+__host__ __device__ constexpr int q4_scale_at(int terms, int term) { return terms * 6144 + term * 256; }
+__host__ __device__ constexpr int q4_rope_at(int terms, int rterm, int step) {
+    return terms * 6400 + (rterm * 2 + step) * 1024;
+}
+
+// Where sequence b's query t (of its first `count`, the last of them at position length - 1) may look: positions
+// 0 .. sees - 1.
+__device__ __forceinline__ int q4_sees(int t, int count, int length) {
+    return t < count ? max(0, length - count + t + 1) : 0;
+}
+
+// scores of 16 positions (rows of A: codes and scale bytes) against 16 query rows, 128 columns
+template <int STEP>
+__device__ __forceinline__ f32x4 q4_mfma(u32x4 k, int kscale, u32x4 qlo, u32x2 qhi, int qscale, f32x4 c) {
+    const i32x8 a = {static_cast<int>(k.x), static_cast<int>(k.y), static_cast<int>(k.z), static_cast<int>(k.w), 0, 0, 0, 0};
+    const i32x8 b = {static_cast<int>(qlo.x), static_cast<int>(qlo.y), static_cast<int>(qlo.z), static_cast<int>(qlo.w),
+                     static_cast<int>(qhi.x), static_cast<int>(qhi.y), 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4 /* E2M1 */, 2 /* E2M3 */, STEP, kscale, STEP, qscale);
+}
+
+__device__ __forceinline__ f32x4 q4_mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Sum / max over the four 16-lane rows of the wave (lanes l, l^16, l^32, l^48), in every lane.
+__device__ __forceinline__ float q4_rows_sum(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float q4_rows_max(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// bf16 pair (RNE, hardware conversion) of (a, b): low half a
+__device__ __forceinline__ uint32_t q4_pack_bf16(float a, float b) {
+    const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ float q4_lo(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float q4_hi(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+
+}  // namespace
+}  // namespace k3

@@ -1,6 +1,8 @@
 """Torch tensor plumbing for the C-ABI: device pointers, dtype enums and streams."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 from torch.autograd import forward_ad
 
@@ -38,6 +40,14 @@ def stream(t: torch.Tensor) -> int:
 def stream_of(device: torch.device) -> int:
     """The current HIP stream of a device (the current device where it has no index)."""
     return _raw_stream(torch.cuda.current_device() if device.index is None else device.index)
+
+
+_here = contextlib.nullcontext()
+
+
+def current(device: torch.device):
+    """A context in which device is the current one (nothing to do where it already is)."""
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def require_device(*ts: torch.Tensor) -> None:

@@ -1,0 +1,163 @@
+"""The 4-bit latent cache: writing it and attending over it.
+
+A cached position holds its 512 latent values as MXFP4 -- ``packed`` [256] u8 E2M1 codes and
+``scales`` [16] u8 E8M0 bytes, the format of ``k3hip.mxfp4`` -- and its 64 rotary values in bf16:
+400 bytes where the bf16 cache takes 1152.  The counterpart of the reference's optional quantised
+latent (``air_llm/models/kimi_k3/mla_quant.py:64-116``; group-affine there), which keeps the rotary
+part unquantised as well.
+
+``mla_q4_append`` rounds new latents into a batch of such caches, ``mla_q4_attention`` is the absorbed
+latent attention of one token or several of each sequence over them (``attention_mla.py:193-212``),
+and sums, if asked to, the attention weight that every position received, by which
+``k3hip.evict.cache_evict`` chooses what stays.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib, _workspace
+from . import _torch as T
+
+LATENT, ROPE, GROUP = 512, 64, 32
+# Scratch up to this size is kept per stream (a decode step's); larger scratch, a prompt's, is the call's own.
+KEPT_WORKSPACE = 1 << 26
+
+
+def _buffers(packed, scales, rot):
+    """The cache's three buffers as [B, cap, .]: dtypes, shapes and row layout."""
+    for t, name, width, dtype in ((packed, "packed", LATENT // 2, torch.uint8), (scales, "scales", LATENT // GROUP, torch.uint8),
+                                  (rot, "rot", ROPE, torch.bfloat16)):
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}; got {t.dtype}")
+        if t.dim() != 3 or t.shape[2] != width:
+            raise ValueError(f"{name} must be [B, cap, {width}]; got {tuple(t.shape)}")
+        if t.shape[1] and t.stride(2) != 1:
+            raise ValueError(f"{name}: the values of a position must be contiguous")
+    if packed.shape[:2] != scales.shape[:2] or packed.shape[:2] != rot.shape[:2]:
+        raise ValueError(f"packed {tuple(packed.shape)}, scales {tuple(scales.shape)} and rot {tuple(rot.shape)} differ in batch "
+                         "or capacity")
+    return packed.shape[:2]
+
+
+def _per_sequence(v, B: int, name: str, device) -> torch.Tensor | None:
+    """An int32 [B] device tensor as it is, None as None."""
+    if v is None:
+        return None
+    if v.dtype != torch.int32:
+        raise TypeError(f"{name} must be an int32 tensor; got {v.dtype}")
+    if tuple(v.shape) != (B,):
+        raise ValueError(f"{name} must be [{B}]; got {tuple(v.shape)}")
+    if v.device != device:
+        raise ValueError(f"{name} is on {v.device}, the cache on {device}")
+    return v.contiguous()
+
+
+def _pitches(t: torch.Tensor) -> tuple[int, int]:
+    """Batch and row pitch in elements; a pitch that is never used may be anything."""
+    return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else max(t.stride(1), t.shape[2]))
+
+
+def _row_input(t: torch.Tensor, per: int) -> torch.Tensor:
+    """Contiguous rows, pitches of whole 16 bytes (``per`` elements), a 16-byte aligned base; else a copy."""
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % per for s in t.stride()[:-1]):
+        t = T.contiguous_aligned(t)
+    return t
+
+
+def mla_q4_append(c_new: torch.Tensor, r_new: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, rot: torch.Tensor,
+                  start: int | torch.Tensor = 0, counts: torch.Tensor | None = None) -> None:
+    """Round c_new [B, T, 512] and r_new [B, T, 64] (bf16 or fp32) into positions start .. start + T - 1 of the cache,
+    in place.
+
+    ``start``: a whole number (positions past the capacity are a ValueError), or an int32 [B] device tensor, every
+    sequence its own; ``counts`` int32 [B]: only sequence b's first counts[b] tokens are written.  Positions
+    that a tensor puts outside the capacity are left out.  A group's scale is the power of two that puts its
+    largest magnitude at 4 to 7 times itself (above 7 the next one); codes round to nearest even.  A position with a NaN or an
+    infinity is NaN to every query that sees it.
+    """
+    B, cap = _buffers(packed, scales, rot)
+    if c_new.dim() != 3 or r_new.dim() != 3 or c_new.shape[2] != LATENT or r_new.shape[2] != ROPE or \
+            c_new.shape[:2] != r_new.shape[:2] or c_new.shape[0] != B:
+        raise ValueError(f"c_new [B, T, {LATENT}] and r_new [B, T, {ROPE}] with B = {B} expected; got {tuple(c_new.shape)}, "
+                         f"{tuple(r_new.shape)}")
+    n = c_new.shape[1]
+    T.require_device(c_new, r_new, packed, scales, rot)
+    cdt, rdt = T.dtype_code(c_new.dtype), T.dtype_code(r_new.dtype)
+    starts, start0 = (start, 0) if isinstance(start, torch.Tensor) else (None, int(start))
+    starts = _per_sequence(starts, B, "start", packed.device)
+    counts = _per_sequence(counts, B, "counts", packed.device)
+    if starts is None and not 0 <= start0 <= start0 + n <= cap:
+        raise ValueError(f"{n} tokens at position {start0} do not fit a capacity of {cap}")
+    if B == 0 or n == 0 or cap == 0:
+        return
+    c_new = _row_input(c_new, 16 // c_new.element_size())
+    if r_new.stride(2) != 1:
+        r_new = r_new.contiguous()
+    with T.current(packed.device):
+        _lib.call("k3_mla_q4_append", c_new.data_ptr(), c_new.stride(0), c_new.stride(1), cdt, r_new.data_ptr(), r_new.stride(0),
+                  r_new.stride(1), rdt, packed.data_ptr(), *_pitches(packed), scales.data_ptr(), *_pitches(scales), rot.data_ptr(),
+                  *_pitches(rot), T.ptr(starts), start0, T.ptr(counts), B, n, cap, LATENT, ROPE, T.stream(packed))
+
+
+def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor, wv: torch.Tensor, packed: torch.Tensor,
+                     scales: torch.Tensor, rot: torch.Tensor, scale: float, lengths: torch.Tensor | int | None = None,
+                     counts: torch.Tensor | None = None, weight: torch.Tensor | None = None,
+                     gate: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Absorbed latent attention of T queries of each of B sequences over the 4-bit cache -> [B, T, H, v] in out_dtype.
+
+    q_nope [B, T, H, nope], q_rot [B, T, H, 64] (bf16 or fp32); wk [H, nope, 512], wv [H, v, 512] bf16; packed, scales,
+    rot [B, cap, .].  Causal: the queries are each sequence's last T positions, query t sees positions 0 ..
+    length - T + t.  ``lengths``: the sequences' lengths, a whole number for all or an int32 [B] device tensor (default: the
+    capacity); ``counts`` int32 [B]: sequence b has only counts[b] queries, the first ones of its T.  A query that
+    sees nothing gives zeros.
+
+    ``weight`` fp32 [B, cap], changed in place: every position's attention weight, summed over the queries and heads, is
+    added to it.  ``gate`` [B, T, H * v] fp32: the output times sigmoid(gate).
+    """
+    B, cap = _buffers(packed, scales, rot)
+    if q_nope.dim() != 4 or q_rot.dim() != 4 or q_nope.shape[:3] != q_rot.shape[:3] or q_nope.shape[0] != B or q_rot.shape[3] != ROPE:
+        raise ValueError(f"q_nope [B, T, H, nope] and q_rot [B, T, H, {ROPE}] with B = {B} expected; got {tuple(q_nope.shape)}, "
+                         f"{tuple(q_rot.shape)}")
+    Tq, H, nope = q_nope.shape[1:]
+    if wk.dim() != 3 or wv.dim() != 3 or tuple(wk.shape) != (H, nope, LATENT) or wv.shape[0] != H or wv.shape[2] != LATENT:
+        raise ValueError(f"wk [{H}, {nope}, {LATENT}] and wv [{H}, v, {LATENT}] expected; got {tuple(wk.shape)}, {tuple(wv.shape)}")
+    if wk.dtype != torch.bfloat16 or wv.dtype != torch.bfloat16:
+        raise TypeError("wk and wv must be bfloat16 (the checkpoint dtype)")
+    V = wv.shape[1]
+    T.require_device(q_nope, q_rot, wk, wv, packed, scales, rot, weight, gate)
+    if T.tracked(q_nope, q_rot, wk, wv, rot, gate):
+        raise ValueError("mla_q4_attention carries no gradient: call it under no_grad or on detached tensors")
+    device = packed.device
+    most = cap
+    if lengths is not None and not isinstance(lengths, torch.Tensor):
+        most, lengths = int(lengths), None
+        if not 0 <= most <= cap:
+            raise ValueError(f"length {most} outside the capacity {cap}")
+    lengths = _per_sequence(lengths, B, "lengths", device)
+    counts = _per_sequence(counts, B, "counts", device)
+    if weight is not None:
+        if weight.dtype != torch.float32:
+            raise TypeError(f"weight must be float32; got {weight.dtype}")
+        if tuple(weight.shape) != (B, cap) or (cap > 1 and weight.stride(1) != 1):
+            raise ValueError(f"weight must be [{B}, {cap}] with contiguous rows; got {tuple(weight.shape)}")
+    if gate is not None:
+        if gate.numel() != B * Tq * H * V or gate.shape[:2] != (B, Tq):
+            raise ValueError(f"gate must be [{B}, {Tq}, {H * V}]; got {tuple(gate.shape)}")
+        gate = T.contiguous_aligned(gate.to(torch.float32))
+    out_code = T.dtype_code(out_dtype)
+    out = torch.empty((B, Tq, H, V), dtype=out_dtype, device=device)
+    if out.numel() == 0:
+        return out
+    qdt = torch.bfloat16 if q_nope.dtype == torch.bfloat16 and q_rot.dtype == torch.bfloat16 else torch.float32
+    q_nope, q_rot = _row_input(q_nope.to(qdt), 4), _row_input(q_rot.to(qdt), 4)
+    wk, wv = T.contiguous_aligned(wk), T.contiguous_aligned(wv)
+    nbytes = _lib.size("k3_mla_q4_workspace_size", B, Tq, H, V, most, out_code, 0 if weight is None else 1)
+    with T.current(device):
+        ws = (_workspace.get(device, nbytes, "mla_q4") if nbytes <= KEPT_WORKSPACE
+              else torch.empty(nbytes, dtype=torch.uint8, device=device))
+        _lib.call("k3_mla_q4_attention", q_nope.data_ptr(), *q_nope.stride()[:3], q_rot.data_ptr(), *q_rot.stride()[:3],
+                  T.dtype_code(qdt), wk.data_ptr(), wv.data_ptr(), packed.data_ptr(), *_pitches(packed), scales.data_ptr(),
+                  *_pitches(scales), rot.data_ptr(), *_pitches(rot), T.ptr(lengths), T.ptr(counts), most, B, Tq, H, LATENT, ROPE,
+                  nope, V, float(scale), T.ptr(gate), out.data_ptr(), out_code, T.ptr(weight),
+                  0 if weight is None else weight.stride(0), ws.data_ptr(), ws.numel(), T.stream(packed))
+    return out

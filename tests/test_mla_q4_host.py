@@ -1,0 +1,220 @@
+"""What the 4-bit cache's calls refuse before anything is launched (no GPU: the check for device tensors comes after the
+shapes', and the C entry points check on the host)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import _q4_oracle as oracle
+
+BF16, U8 = torch.bfloat16, torch.uint8
+
+
+def _cache(B=2, cap=8):
+    return torch.zeros(B, cap, 256, dtype=U8), torch.zeros(B, cap, 16, dtype=U8), torch.zeros(B, cap, 64, dtype=BF16)
+
+
+def _launches(monkeypatch):
+    """The Python layer without a GPU: device checks pass, launches are recorded."""
+    import contextlib
+
+    from k3hip import _lib, _workspace
+    from k3hip import _torch as T
+    calls = []
+    monkeypatch.setattr(T, "require_device", lambda *ts: None)
+    monkeypatch.setattr(T, "stream", lambda t: 0)
+    monkeypatch.setattr(T, "current", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(_workspace, "get", lambda d, n, tag="": torch.empty(n, dtype=U8))
+    monkeypatch.setattr(_lib, "call", lambda name, *a: calls.append((name, a)))
+    return calls
+
+
+# ------------------------------------------------------------------------------- append
+@pytest.mark.parametrize("c,r,start,error", [
+    ((2, 3, 511), (2, 3, 64), 0, ValueError), ((2, 3, 512), (2, 3, 63), 0, ValueError), ((2, 3, 512), (2, 4, 64), 0, ValueError),
+    ((1, 3, 512), (1, 3, 64), 0, ValueError), ((3, 512), (3, 64), 0, ValueError), ((2, 3, 512), (2, 3, 64), 6, ValueError),
+    ((2, 3, 512), (2, 3, 64), -1, ValueError), ((2, 9, 512), (2, 9, 64), 0, ValueError),
+])
+def test_append_refuses(monkeypatch, c, r, start, error):
+    from k3hip.mla_q4 import mla_q4_append
+    calls = _launches(monkeypatch)
+    with pytest.raises(error):
+        mla_q4_append(torch.zeros(*c), torch.zeros(*r), *_cache(), start=start)
+    assert not calls
+
+
+@pytest.mark.parametrize("which,change", [
+    (0, lambda t: t.to(torch.int8)), (1, lambda t: t.float()), (2, lambda t: t.float()), (0, lambda t: t[..., :128]),
+    (1, lambda t: t[:, :5]), (2, lambda t: t[:1]), (0, lambda t: t[0]), (0, lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)),
+])
+def test_both_refuse_buffers_of_another_form(monkeypatch, which, change):
+    from k3hip.mla_q4 import mla_q4_append, mla_q4_attention
+    calls = _launches(monkeypatch)
+    cache = list(_cache())
+    cache[which] = change(cache[which])
+    with pytest.raises((ValueError, TypeError)):
+        mla_q4_append(torch.zeros(2, 1, 512), torch.zeros(2, 1, 64), *cache)
+    with pytest.raises((ValueError, TypeError)):
+        mla_q4_attention(torch.zeros(2, 1, 4, 128), torch.zeros(2, 1, 4, 64), torch.zeros(4, 128, 512, dtype=BF16),
+                         torch.zeros(4, 128, 512, dtype=BF16), *cache, 0.1)
+    assert not calls
+
+
+@pytest.mark.parametrize("bad", [torch.zeros(2, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), torch.zeros(2, 1, dtype=torch.int32)])
+def test_lengths_of_another_form(monkeypatch, bad):
+    from k3hip.evict import cache_evict
+    from k3hip.mla_q4 import mla_q4_append, mla_q4_attention
+    calls = _launches(monkeypatch)
+    q = (torch.zeros(2, 1, 4, 128), torch.zeros(2, 1, 4, 64), torch.zeros(4, 128, 512, dtype=BF16), torch.zeros(4, 128, 512, dtype=BF16))
+    for f in (lambda: mla_q4_append(torch.zeros(2, 1, 512), torch.zeros(2, 1, 64), *_cache(), start=bad),
+              lambda: mla_q4_append(torch.zeros(2, 1, 512), torch.zeros(2, 1, 64), *_cache(), counts=bad),
+              lambda: mla_q4_attention(*q, *_cache(), 0.1, lengths=bad), lambda: mla_q4_attention(*q, *_cache(), 0.1, counts=bad),
+              lambda: cache_evict(torch.zeros(2, 8), [], 4, lengths=bad)):
+        with pytest.raises((ValueError, TypeError)):
+            f()
+    assert not calls
+
+
+# ------------------------------------------------------------------------------- attention
+def _attend(**kw):
+    from k3hip.mla_q4 import mla_q4_attention
+    a = {"q_nope": torch.zeros(2, 3, 4, 128), "q_rot": torch.zeros(2, 3, 4, 64), "wk": torch.zeros(4, 128, 512, dtype=BF16),
+         "wv": torch.zeros(4, 96, 512, dtype=BF16)}
+    a.update({k: kw.pop(k) for k in list(kw) if k in a})
+    return mla_q4_attention(*a.values(), *_cache(), 0.1, **kw)
+
+
+@pytest.mark.parametrize("kw,error", [
+    ({"q_nope": torch.zeros(2, 3, 4, 120)}, ValueError), ({"q_rot": torch.zeros(2, 3, 4, 32)}, ValueError),
+    ({"q_rot": torch.zeros(2, 2, 4, 64)}, ValueError), ({"q_nope": torch.zeros(3, 4, 128)}, ValueError),
+    ({"wk": torch.zeros(4, 128, 512)}, TypeError), ({"wv": torch.zeros(3, 96, 512, dtype=BF16)}, ValueError),
+    ({"wv": torch.zeros(4, 96, 256, dtype=BF16)}, ValueError), ({"lengths": 9}, ValueError), ({"lengths": -1}, ValueError),
+    ({"weight": torch.zeros(2, 8, dtype=BF16)}, TypeError), ({"weight": torch.zeros(2, 7)}, ValueError),
+    ({"weight": torch.zeros(8, 2).t()}, ValueError), ({"gate": torch.zeros(2, 3, 4 * 95)}, ValueError),
+    ({"gate": torch.zeros(3, 2, 4 * 96)}, ValueError), ({"out_dtype": torch.float16}, TypeError),
+    ({"q_nope": torch.zeros(2, 3, 4, 128, requires_grad=True)}, ValueError), ({"q_nope": torch.zeros(2, 3, 4, 128, dtype=torch.float16),
+                                                                              "out_dtype": torch.int32}, TypeError),
+])
+def test_attention_refuses(monkeypatch, kw, error):
+    calls = _launches(monkeypatch)
+    with pytest.raises(error):
+        _attend(**kw)
+    assert not calls
+
+
+def test_attention_passes_views_and_copies_what_it_cannot_read(monkeypatch):
+    calls = _launches(monkeypatch)
+    q = torch.zeros(2, 3, 4, 192)
+    _attend(q_nope=q[..., :128], q_rot=q[..., 128:])
+    (name, a), = calls
+    assert name == "k3_mla_q4_attention" and a[:4] == (q.data_ptr(), 2304, 768, 192) and a[4] == q.data_ptr() + 512
+    odd = torch.zeros(2, 3, 4, 193)
+    _attend(q_nope=odd[..., :128], q_rot=odd[..., 128:192])
+    assert calls[1][1][1:4] == (1536, 512, 128) and calls[1][1][5:8] == (768, 256, 64)
+
+
+def test_entry_points_check_their_arguments():
+    """Every refusal of the C entry points comes from the host, before a launch."""
+    from k3hip import _lib
+    lib = _lib.lib()
+    p, n = ctypes.c_void_p(4096), None
+    app = [p, 1536, 512, 0, p, 192, 64, 0, p, 2048, 256, p, 128, 16, p, 512, 64, n, 0, n, 2, 3, 8, 512, 64, n]
+
+    def append(**at):
+        args = list(app)
+        for k, v in at.items():
+            args[int(k[1:])] = v
+        return lib.k3_mla_q4_append(*args)
+    assert append(_0=n) == _lib.K3_ERR_NULL and append(_8=n) == _lib.K3_ERR_NULL
+    assert append(_3=5) == _lib.K3_ERR_DTYPE and append(_7=2) == _lib.K3_ERR_DTYPE
+    assert append(_18=6) == _lib.K3_ERR_SHAPE and b"do not fit" in lib.k3_last_error()
+    for at in ({"_23": 256}, {"_24": 32}, {"_20": -1}, {"_20": 70000}, {"_2": 510}, {"_10": 255}, {"_13": 15}, {"_16": 63}, {"_22": 2}):
+        assert append(**at) == _lib.K3_ERR_SHAPE, at
+    assert append(_0=ctypes.c_void_p(4104)) == _lib.K3_ERR_ALIGN and append(_8=ctypes.c_void_p(4097)) == _lib.K3_ERR_ALIGN
+    assert append(_21=0) == _lib.K3_OK and append(_20=0) == _lib.K3_OK
+
+    size = lib.k3_mla_q4_workspace_size(2, 3, 4, 96, 8, 0, 1)
+    assert size > 0 and lib.k3_mla_q4_workspace_size(0, 3, 4, 96, 8, 0, 1) == 0
+    att = [p, 1536, 512, 128, p, 768, 256, 64, 0, p, p, p, 2048, 256, p, 128, 16, p, 512, 64, n, n, 8, 2, 3, 4, 512, 64, 128, 96,
+           0.1, n, p, 0, p, 8, p, size, n]
+
+    def attend(**at):
+        args = list(att)
+        for k, v in at.items():
+            args[int(k[1:])] = v
+        return lib.k3_mla_q4_attention(*args)
+    for i in (0, 4, 9, 10, 11, 14, 17, 32, 36):
+        assert attend(**{f"_{i}": n}) == _lib.K3_ERR_NULL, i
+    assert attend(_8=4) == _lib.K3_ERR_DTYPE and attend(_33=9) == _lib.K3_ERR_DTYPE
+    for at in ({"_26": 256}, {"_27": 32}, {"_28": 120 + 4}, {"_28": 264}, {"_28": 0}, {"_29": 1032}, {"_29": 92}, {"_25": 0}, {"_25": 5000},
+               {"_23": 40000}, {"_22": -1}, {"_22": (1 << 24) + 1}, {"_1": 1538}, {"_7": 63}, {"_13": 248}, {"_13": 264}, {"_16": 8},
+               {"_19": 60}, {"_24": 1 << 25}):
+        assert attend(**at) == _lib.K3_ERR_SHAPE, at
+    for i in (0, 4, 9, 10, 11, 17, 32, 36):
+        assert attend(**{f"_{i}": ctypes.c_void_p(4104)}) == _lib.K3_ERR_ALIGN, i
+    assert attend(_37=size - 1) == _lib.K3_ERR_WORKSPACE
+    assert attend(_23=0) == _lib.K3_OK and attend(_24=0) == _lib.K3_OK
+
+
+# ------------------------------------------------------------------------------- eviction
+@pytest.mark.parametrize("kw", [
+    {"keep": -1}, {"sink": -1}, {"recent": -1}, {"sink": 3, "recent": 2}, {"capacity": 3}, {"lengths": 9}, {"lengths": -2},
+    {"weight": torch.zeros(8)}, {"buffers": [torch.zeros(2, 7, 4)]}, {"buffers": [torch.zeros(2, 8)] * 9},
+    {"buffers": [torch.zeros(8)]}, {"buffers": [torch.zeros(2, 8, 3, requires_grad=True)]},
+])
+def test_evict_refuses(monkeypatch, kw):
+    from k3hip.evict import cache_evict
+    calls = _launches(monkeypatch)
+    a = {"weight": torch.zeros(2, 8), "buffers": [torch.zeros(2, 8, 4)], "keep": 4}
+    a.update(kw)
+    with pytest.raises(ValueError):
+        cache_evict(**a)
+    with pytest.raises(TypeError):
+        cache_evict(torch.zeros(2, 8, dtype=torch.float64), [], 4)
+    assert not calls
+
+
+def test_evict_entry_point_checks_its_arguments():
+    from k3hip import _lib
+    lib = _lib.lib()
+    p, n = ctypes.c_void_p(4096), None
+    longs, ptrs = (ctypes.c_int64 * 2), (ctypes.c_void_p * 2)
+    one, big = longs(64, 16), longs(512, 128)
+    base = [p, 8, n, 8, 2, 4, 1, 2, p, p, 2, ptrs(4096, 8192), big, one, ptrs(16384, 32768), big, one, one, 4, n]
+
+    def evict(**at):
+        args = list(base)
+        for k, v in at.items():
+            args[int(k[1:])] = v
+        return lib.k3_cache_evict(*args)
+    for i in (0, 8, 9, 11, 12, 13, 14, 15, 16, 17):
+        assert evict(**{f"_{i}": n}) == _lib.K3_ERR_NULL, i
+    for at in ({"_4": -1}, {"_4": 70000}, {"_3": -1}, {"_5": 2}, {"_6": -1}, {"_7": -1}, {"_10": 9}, {"_18": 3}, {"_13": longs(63, 16)},
+               {"_16": longs(64, 15)}, {"_17": longs(-1, 4)}, {"_11": ptrs(4096, 0)}, {"_14": ptrs(0, 4096)}):
+        assert evict(**at) == _lib.K3_ERR_SHAPE, at
+    assert evict(_4=0) == _lib.K3_OK
+
+
+# ------------------------------------------------------------------------------- the oracle itself
+def test_oracle_rounds_to_the_nearest_value():
+    g = torch.Generator().manual_seed(0)
+    for _ in range(40):
+        x = (torch.randn(32, generator=g, dtype=torch.float64) * 3).float().double().tolist()
+        codes, byte = oracle.round_group(x)
+        s = 2.0 ** (byte - 127)
+        top = max(map(abs, x)) / s
+        assert 3.5 < top <= 7
+        for v, c in zip(x, codes):
+            got = oracle.E2M1[c & 7] * s
+            assert all(abs(abs(v) - got) <= abs(abs(v) - e * s) for e in oracle.E2M1)
+    assert oracle.round_group([7.0] * 32)[1] == 127 and oracle.round_group([7.01] * 32)[1] == 128
+    assert oracle.round_group([2.5, 3.5, 5.0, 0.25, 0.75, 6.0] + [0.0] * 26)[0][:6] == [4, 6, 6, 0, 2, 7]
+
+
+def test_oracle_evicts():
+    assert oracle.evict([5, 1, 3, 3, 3, 2, 9], 7, 5, 1, 1) == [0, 2, 3, 4, 6]
+    assert oracle.evict([5, 1, 3, 3, 3, 2, 9], 7, 4, 0, 2) == [0, 2, 5, 6]
+    assert oracle.evict([1.0, float("nan"), -1.0], 3, 2, 0, 0) == [0, 2]
+    assert oracle.evict([1.0, 2.0], 2, 3, 0, 0) == [0, 1]
