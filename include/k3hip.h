@@ -478,9 +478,9 @@ int k3_mla_q4_append(const void *c, int64_t c_batch, int64_t c_row, int c_dtype,
                      int64_t kv_lora_rank, int64_t rope_dim, void *stream);
 
 /* Workspace bytes of k3_mla_q4_attention for the same sizes (weights: whether it is given a weight
- * buffer).  No initialisation. */
-int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim, int64_t max_length, int out_dtype,
-                                 int weights);
+ * buffer; varied: whether it is given lengths).  No initialisation. */
+int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim, int64_t max_length, int q_dtype,
+                                 int out_dtype, int weights, int varied);
 
 /* The absorbed attention of T queries of each of B sequences over the 4-bit cache, causal: query t of
  * sequence b's first counts[b] sees positions 0 .. lengths[b] - counts[b] + t, so the last one sees the whole
@@ -495,8 +495,8 @@ int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim,
  * out [B, T, H, v] contiguous, out_dtype; weight fp32 rows w_batch floats apart, positions past lengths[b] left as
  *   they are.
  * A query that sees nothing (also: t >= counts[b]) gets zeros and adds nothing to weight.  Deterministic.  The cache's
- * values enter exactly; queries and probabilities to about 2^-17 of their group's largest for a bf16 out without
- * weight, else (queries) 2^-22 and, for an fp32 out, (probabilities) 2^-25; sums and softmax in fp32.
+ * values enter exactly; the absorbed queries to 2^-12 of a unit under their group's largest for a bf16 out without weight,
+ * else 2^-22; the probabilities to 2^-11 for a bf16 out, 2^-22 for fp32; sums and softmax in fp32.
  * nope a multiple of 8 up to 256, v one up to 1024, H <= 4096, B H <= 65536, max_length <= 2^24.  Pointers 16-byte
  * aligned; p_row and p_batch multiples of 16, rot pitches of 8.
  * Counterpart of MLAAttention.__call__ over a QuantLatent cache (air_llm/models/kimi_k3/attention_mla.py:193-212). */

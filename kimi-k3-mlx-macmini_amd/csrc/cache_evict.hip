@@ -3,11 +3,12 @@
 // front of new buffers in their order.
 //
 // Two launches.  select (a block per sequence): the weights become keys that order as whole numbers do (NaN below
-// all, -0 as 0); the key of the last one to stay is found 11, 11 and 10 bits at a time from a histogram of the keys
-// that still match, kept in LDS; of the positions with exactly that key the lowest stay.  Every thread owns a
-// contiguous run of positions, so two counts per thread and one scan give each kept position its place, in order, with no
-// atomics on the result.  gather: rows of every buffer, 16 bytes a thread.
-// Bound by the latency of the histogram passes over LDS (select), by HBM (gather).
+// all, -0 as 0) and stay in registers (up to 32,768 positions; beyond that every pass reads them again); the key of the
+// last one to stay is found 11, 11 and 10 bits at a time from a histogram of the keys that still match, in LDS (four
+// copies, by lane, for weights that are alike), and no further than a bin that stays whole.  Of the positions with exactly
+// that key the lowest stay.  A wave's ballot over 64 neighbours counts them in order, and one scan over those
+// counts gives each kept position its place: no atomics on the result.  gather: rows of every buffer, 16 bytes a thread.
+// Bound by the latency of a block's passes (select), by HBM or the launch (gather).
 #include <algorithm>
 
 #include "k3_common.h"
@@ -15,7 +16,7 @@
 namespace k3 {
 namespace {
 
-constexpr int kThreads = 1024, kBins = 2048, kCopies = 4, kMaxBuffers = 8;
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048, kCopies = 4, kMaxBuffers = 8;
 
 struct SelectArgs {
     const float *weight;
@@ -55,14 +56,17 @@ __device__ __forceinline__ int block_prefix(int v, int *sums, int &total) {
     return before + s - v;
 }
 
+// VPT keys a thread, position (j * kWaves + wave) * 64 + lane of a chunk of kThreads * VPT
+template <int VPT>
 __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
     __shared__ int hist[kBins * kCopies];
-    __shared__ int sums[kThreads / 64];
-    __shared__ int found[2];
-    const int tid = threadIdx.x, b = blockIdx.x;
+    __shared__ int2 counts[VPT * kWaves];   // of 64 neighbours: keys above the threshold, keys at it
+    __shared__ int sums[kWaves];
+    __shared__ int found[3];
+    constexpr int kChunk = kThreads * VPT;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
     const int n = a.lengths ? min(max(a.lengths[b], 0), a.cap) : a.length;
     int32_t *index = a.index + static_cast<int64_t>(b) * a.keep;
-    const float *w = a.weight + b * a.ld;
     const int nk = min(n, a.keep);
     if (tid == 0) a.kept[b] = nk;
     for (int i = nk + tid; i < a.keep; i += kThreads) index[i] = -1;
@@ -70,56 +74,93 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
         for (int i = tid; i < n; i += kThreads) index[i] = i;
         return;
     }
-    // the middle positions lo .. hi - 1, `need` of them stay
-    const int lo = a.sink, hi = n - a.recent;
+    // the middle positions sink .. sink + mid - 1, `need` of them stay
+    const int mid = n - a.recent - a.sink;
     int need = a.keep - a.sink - a.recent;
     for (int i = tid; i < a.sink; i += kThreads) index[i] = i;
-    for (int i = tid; i < a.recent; i += kThreads) index[a.keep - a.recent + i] = hi + i;
+    for (int i = tid; i < a.recent; i += kThreads) index[a.keep - a.recent + i] = n - a.recent + i;
     if (need == 0) return;
+    const float *w = a.weight + b * a.ld + a.sink;
+    uint32_t key[VPT];
+    auto load = [&](int c0) {
+        float f[VPT];
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int i = c0 + j * kThreads + tid;
+            f[j] = i < mid ? w[i] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) key[j] = order_key(f[j]);
+    };
+    if (mid <= kChunk) load(0);
     uint32_t prefix = 0;     // the bits of the threshold key found so far
+    int shift = 32;
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
-        for (int i = tid; i < kBins * kCopies; i += kThreads) hist[i] = 0;
+        const int bits = pass == 2 ? 10 : 11;
+        shift -= bits;
+#pragma unroll
+        for (int i = 0; i < kBins * kCopies / kThreads; ++i) hist[i * kThreads + tid] = 0;
         __syncthreads();
-        for (int i = lo + tid; i < hi; i += kThreads) {
-            const uint32_t k = order_key(w[i]);
-            if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[((k >> shift) & (bins - 1)) * kCopies + (tid & (kCopies - 1))], 1);
+        for (int c0 = 0; c0 < mid; c0 += kChunk) {
+            if (mid > kChunk) load(c0);
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const uint32_t k = key[j];
+                if (c0 + j * kThreads + tid < mid && (pass == 0 || (k >> (shift + bits)) == prefix))
+                    atomicAdd(&hist[((k >> shift) & ((1 << bits) - 1)) * kCopies + (tid & (kCopies - 1))], 1);
+            }
         }
         __syncthreads();
-        // thread t counts bins 2 t' and 2 t' + 1 from the top: t' = 1023 - t
+        // thread t counts bins 2 t' and 2 t' + 1, t' = 1023 - t: from the top down
         const int top = kThreads - 1 - tid;
         int c[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            c[x] = 0;
-#pragma unroll
-            for (int k = 0; k < kCopies; ++k) c[x] += hist[(2 * top + x) * kCopies + k];
+            const int4 v = *reinterpret_cast<const int4 *>(&hist[(2 * top + x) * kCopies]);
+            c[x] = (v.x + v.y) + (v.z + v.w);
         }
         int total;
         const int above = block_prefix(c[0] + c[1], sums, total);   // keys in higher bins
-        if (above < need && above + c[1] >= need) found[0] = 2 * top + 1, found[1] = need - above;
-        if (above + c[1] < need && above + c[1] + c[0] >= need) found[0] = 2 * top, found[1] = need - above - c[1];
+#pragma unroll
+        for (int x = 1, over = above; x >= 0; over += c[x], --x)
+            if (over < need && over + c[x] >= need) found[0] = 2 * top + x, found[1] = need - over, found[2] = c[x];
         __syncthreads();
         prefix = (prefix << bits) | static_cast<uint32_t>(found[0]);
         need = found[1];
+        const bool whole = found[1] == found[2];
         __syncthreads();
+        if (whole) break;
     }
-    // keys above the threshold stay, and the first `need` at it
-    const int run = (hi - lo + kThreads - 1) / kThreads, i0 = min(hi, lo + tid * run), i1 = min(hi, i0 + run);
-    int more = 0, same = 0, total;
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t k = order_key(w[i]);
-        more += k > prefix;
-        same += k == prefix;
-    }
-    const int same_before = block_prefix(same, sums, total);
-    const int take = min(max(need - same_before, 0), same);
-    int at = a.sink + block_prefix(more + take, sums, total), left = take;
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t k = order_key(w[i]);
-        bool stay = k > prefix;
-        if (k == prefix && left > 0) stay = true, --left;
-        if (stay) index[at++] = i;
+    // keys whose leading bits are above the prefix stay, and the first `need` of those that match
+    int at = a.sink, same_seen = 0;
+    for (int c0 = 0; c0 < mid; c0 += kChunk) {
+        if (mid > kChunk) load(c0);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const bool there = c0 + j * kThreads + tid < mid;
+            const uint64_t more = __ballot(there && (key[j] >> shift) > prefix), same = __ballot(there && (key[j] >> shift) == prefix);
+            if (lane == 0) counts[j * kWaves + wave] = make_int2(__popcll(more), __popcll(same));
+        }
+        __syncthreads();
+        const int2 v = tid < VPT * kWaves ? counts[tid] : make_int2(0, 0);
+        int total, all;
+        const int same_before = same_seen + block_prefix(v.y, sums, all);
+        const int place = at + block_prefix(v.x + min(max(need - same_before, 0), v.y), sums, total);
+        if (tid < VPT * kWaves) counts[tid] = make_int2(place, same_before);
+        __syncthreads();
+        const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int i = c0 + j * kThreads + tid;
+            const bool same = i < mid && (key[j] >> shift) == prefix;
+            const uint64_t sames = __ballot(same);
+            const int2 o = counts[j * kWaves + wave];
+            const bool stay = (i < mid && (key[j] >> shift) > prefix) || (same && o.y + __popcll(sames & below) < need);
+            const uint64_t stays = __ballot(stay);
+            if (stay) index[o.x + __popcll(stays & below)] = a.sink + i;
+        }
+        at += total, same_seen += all;
+        __syncthreads();
     }
 }
 
@@ -129,7 +170,7 @@ struct GatherArgs {
     int64_t src_b[kMaxBuffers], src_r[kMaxBuffers], dst_b[kMaxBuffers], dst_r[kMaxBuffers];   // bytes
     int units[kMaxBuffers], unit[kMaxBuffers];                                                // of a row; bytes of a unit: 16, 4 or 1
     const int32_t *index;
-    int buffers, keep, rows;
+    int buffers, keep, rows, per;   // rows a block takes
 };
 constexpr int kGatherRows = 64;
 
@@ -148,7 +189,7 @@ __device__ __forceinline__ void copy_rows(const GatherArgs &a, int x, int b, int
 
 __global__ __launch_bounds__(256) void gather_kernel(GatherArgs a) {
     __shared__ int at[kGatherRows];
-    const int b = blockIdx.y, r0 = blockIdx.x * kGatherRows, nrows = min(kGatherRows, a.rows - r0);
+    const int b = blockIdx.y, r0 = blockIdx.x * a.per, nrows = min(a.per, a.rows - r0);
     if (static_cast<int>(threadIdx.x) < nrows) {
         const int r = r0 + threadIdx.x;
         at[threadIdx.x] = r < a.keep ? a.index[static_cast<int64_t>(b) * a.keep + r] : -1;
@@ -200,10 +241,18 @@ extern "C" int k3_cache_evict(const float *weight, int64_t w_batch, const int32_
     auto st = static_cast<hipStream_t>(stream);
     const SelectArgs s{weight, w_batch, lengths, static_cast<int>(max_length), static_cast<int>(max_length), static_cast<int>(keep),
                        static_cast<int>(sink), static_cast<int>(recent), index, kept};
-    select_kernel<<<dim3(static_cast<unsigned>(B)), kThreads, 0, st>>>(s);
+    const dim3 grid(static_cast<unsigned>(B));
+    if (max_length <= 4 * kThreads)
+        select_kernel<4><<<grid, kThreads, 0, st>>>(s);
+    else if (max_length <= 16 * kThreads)
+        select_kernel<16><<<grid, kThreads, 0, st>>>(s);
+    else
+        select_kernel<32><<<grid, kThreads, 0, st>>>(s);
     int rc = check_hip(hipGetLastError(), "cache evict: select launch");
     if (rc || buffers == 0 || dst_rows == 0) return rc;
     g.index = index, g.buffers = static_cast<int>(buffers), g.keep = static_cast<int>(keep), g.rows = static_cast<int>(dst_rows);
-    gather_kernel<<<dim3(static_cast<unsigned>(cdiv(dst_rows, kGatherRows)), static_cast<unsigned>(B)), 256, 0, st>>>(g);
+    g.per = kGatherRows;      // fewer rows to a block until there are two blocks a CU
+    while (g.per > 4 && cdiv(dst_rows, g.per) * B < 512) g.per /= 2;
+    gather_kernel<<<dim3(static_cast<unsigned>(cdiv(dst_rows, g.per)), static_cast<unsigned>(B)), 256, 0, st>>>(g);
     return check_hip(hipGetLastError(), "cache evict: gather launch");
 }

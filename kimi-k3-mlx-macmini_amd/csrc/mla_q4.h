@@ -8,12 +8,20 @@
 // (row r, quarter q) holds 16 bytes, group 4 q + s in step s of four (the order of a sum's columns is free, and
 // in this one the lane's four scale bytes are one dword of the row).  The absorbed query qa (fp32) enters as a sum of E2M3 terms (6 bits: 1 + 2 + 3) that share the other
 // operand's place, each with an E8M0 byte per 32 columns:
-//     qa = t1 + t2 + t3 + t4 (+ t5),   |t1| <= 7.5 s, the next terms' units s / 16, s / 2^9, s / 2^14, s / 2^19
+//     qa = t1 + t2 + t3 (+ t4 + t5),   |t1| <= 7.5 s, the next terms' units s / 16, s / 2^9, s / 2^14, s / 2^19
 // Each term rounds what is left to nearest; E2M3's step below 4 is at most 1/4, so a term leaves at most
-// 1/8 of its unit (the first, up to 7.5: 1/4): 2^-17 s after four terms, 2^-22 s after five, where the group's
-// largest magnitude is above 3.75 s.  E2M1 x E2M3 products run at four times bf16's rate (measured: 4128 against
+// 1/8 of its unit (the first, up to 7.5: 1/4): 2^-12 s after three terms, 2^-22 s after five, where the group's
+// largest magnitude is above 3.75 s.  Three (2^-14 of the largest at worst) are taken where the result is rounded to
+// bf16 (2^-8), five where it is fp32 or the weights are summed.  E2M1 x E2M3 products run at four times bf16's rate (measured: 4128 against
 // 1107 TFLOP/s), so five terms cost 1.25 bf16 products and need no decoded keys; two bf16 terms (2^-17) would cost
-// two products and the decoding.  The rotary columns are bf16 on both sides, the query in two or three terms.
+// two products and the decoding.  The rotary columns are bf16 on both sides: bf16 queries are one term, fp32 ones two or three.
+//
+// Values.  The second product's operands are fp16: E2M1 times 2^-23 .. 2^13 (scale bytes 104 .. 140) is exact in it,
+// and its 11 bits make one term of a probability enough for a bf16 result (2^-11 each, independent, below the
+// result's own 2^-8) and two for fp32 (2^-22), where bf16 would need two and three.  Probabilities are 2^kLift times those of the
+// row's reference maximum, so fp16's last bit, 2^-24, is 2^-34 of the largest.  A block that has come upon a scale
+// byte outside that range (of a group that is not all zeros) goes over its positions again with bf16 operands, exact for every byte, and one
+// term more.
 //
 // Query operands of 16 rows (a row: one head of one query), `terms` latent and `rterms` rotary terms:
 //     [term][step]                  64 lanes x 16 bytes, then 64 x 8: the lane's 32 codes, 192 bits
@@ -28,6 +36,10 @@ namespace k3 {
 namespace {
 
 constexpr int kQ4Lat = 512, kQ4Rope = 64, kQ4Steps = kQ4Lat / 128;
+constexpr float kLift = 10.f, kSlack = 5.f;              // log2: probabilities stay under 2^15, fp16's largest is 2^16 - 32
+constexpr uint32_t kHalfLow = 104, kHalfHigh = 140;      // scale bytes whose values are exact in fp16
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -62,6 +74,10 @@ __device__ __forceinline__ f32x4 q4_mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 q4_mfma_f16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
 // Sum / max over the four 16-lane rows of the wave (lanes l, l^16, l^32, l^48), in every lane.
 __device__ __forceinline__ float q4_rows_sum(float v) {
     auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -79,6 +95,10 @@ __device__ __forceinline__ float q4_rows_max(float v) {
 // bf16 pair (RNE, hardware conversion) of (a, b): low half a
 __device__ __forceinline__ uint32_t q4_pack_bf16(float a, float b) {
     const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ uint32_t q4_pack_f16(float a, float b) {
+    const f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
     return __builtin_bit_cast(uint32_t, v);
 }
 __device__ __forceinline__ float q4_lo(uint32_t pair) { return __uint_as_float(pair << 16); }

@@ -14,16 +14,16 @@
 //   weights  (if asked for) p once more from the rows' final maxima and sums, added over the rows
 //
 // attend, per round of 32 positions: a thread stages one group (16 bytes of codes and their scale byte); the codes go to
-// LDS as they are, where the score waves (0..3) read them as matrix operands; the same thread decodes its group to bf16
-// (exact: E2M1 times a power of two) into the value tile, which the context waves (4..7, 128 columns each) read
-// transposed.  The probabilities enter the second product as two bf16 terms (bf16 results, 2^-17) or three (fp32
-// results).  In iteration i the score waves take round i's scores and turn round i - 1's into probabilities, and the
-// context waves take round i - 2's products, one barrier per iteration.  A row's reference maximum moves only when a score exceeds it
-// by kSlack (log2), so the accumulators are seldom rescaled.
+// LDS as they are, where the score waves (0..3) read them as matrix operands; the same thread decodes its group
+// (exactly: E2M1 times a power of two) into the value tile, which the context waves (4..7, 128 columns each) read
+// transposed (fp16, see mla_q4.h).  In iteration i the score waves take round i's scores and turn round i - 1's into
+// probabilities, and the context waves take round i - 2's products, one barrier per iteration.  A row's reference maximum moves
+// only when a score exceeds it by kSlack (log2), so the accumulators are seldom rescaled.
 //
 // A position whose scale byte is 255 (NaN) makes its scores NaN by the matrix product itself, so every row that sees it is NaN; its
 // values are staged as zeros, so a row that does not see it (weight zero) stays clean.
 #include <algorithm>
+#include <type_traits>
 
 #include "mla_q4.h"
 
@@ -59,7 +59,7 @@ __device__ __forceinline__ void terms8(const float (&v)[8], u32x4 (&f)[3]) {
 // grid (H, ceil(M / 16), 4): queries 16 y .. +16 of head x, latent columns 128 z .. +128
 template <typename QT, int NT, int RT>
 __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
-    extern __shared__ char lds[];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     float *fs = reinterpret_cast<float *>(lds);                         // [16][kFLd], after the products
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
     const int h = blockIdx.x, m0 = blockIdx.y * 16, quarter = blockIdx.z;
@@ -190,25 +190,26 @@ constexpr int kKLd = 272;                       // LDS bytes of a staged row of 
 constexpr int kRLd = 144;                       // .. of a rotary row: 128 + 16
 constexpr int kVLd = 1056;                      // .. of a value row: 1024 + 32
 constexpr int kKBytes = kRound * kKLd, kRBytes = kRound * kRLd, kVBytes = kRound * kVLd;
-constexpr float kSlack = 64.f;
 
 constexpr int kKSlots = 3;
 
-constexpr int attend_lds(int RG, int RT, int PT) {
-    return kKSlots * kKBytes + 2 * kRBytes + 2 * kVBytes + 2 * RG * PT * 1024 + RG * RT * 2048;
+constexpr int attend_lds(int RG, int RT, int PT) {   // PT fp16 terms of the probabilities (bf16: one more)
+    return kKSlots * kKBytes + 2 * kRBytes + 2 * kVBytes + 2 * RG * (PT + 1) * 1024 + RG * RT * 2048;
 }
 
 // RG: groups of 16 rows (2: two score waves to a group, one tile of 16 positions each; 4: one, two tiles);
-// NT latent and RT rotary terms of the queries, PT terms of the probabilities
+// NT latent and RT rotary terms of the queries, PT fp16 terms of the probabilities
 template <int RG, int NT, int RT, int PT>
 __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     constexpr int TG = 4 / RG, NTILE = 2 / TG;   // score waves of a row group; tiles of 16 positions per score wave
-    extern __shared__ char lds[];
+    constexpr int kPLd = (PT + 1) * 1024;        // LDS bytes of a row group's probabilities
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ float xm[2][TG][RG * 16];         // tile maxima [parity][score wave of the group][row]
     __shared__ float xf[2][RG * 16];             // rescale factors [parity][row]
     __shared__ float xl[TG][RG * 16];
+    __shared__ int wide;                         // a staged scale byte needs bf16's range
     char *const kbuf = lds, *const rbuf = lds + kKSlots * kKBytes, *const vbuf = rbuf + 2 * kRBytes, *const pbuf = vbuf + 2 * kVBytes;
-    char *const qbuf = pbuf + 2 * RG * PT * 1024;   // the queries' rotary operands
+    char *const qbuf = pbuf + 2 * RG * kPLd;     // the queries' rotary operands
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, q4 = lane >> 4;
     const int nb = gridDim.x;
@@ -228,58 +229,72 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     }
     const int n = t_end - t_begin, nr = (n + kRound - 1) / kRound;
 
-    // ---- staging: thread = (position tid / 16, group tid % 16); the first four waves also a 16-byte rotary chunk
+    // ---- staging, by the context waves: thread = (positions st / 16 and 16 more, group st % 16) and a 16-byte rotary chunk
     const auto rp = make_rsrc(a.packed + b * a.p_b + t_begin * a.p_t, static_cast<uint32_t>((n - 1) * a.p_t + 256));
     const auto rs = make_rsrc(a.scales + b * a.s_b + t_begin * a.s_t, static_cast<uint32_t>((n - 1) * a.s_t + 16));
     const auto rr = make_rsrc(a.rot + b * a.r_b + t_begin * a.r_t, static_cast<uint32_t>((n - 1) * a.r_t + 128));
-    const int srow = tid >> 4, sgrp = tid & 15, orow = (tid >> 3) & 31, ochunk = tid & 7;
+    const int st = tid & 255, srow = st >> 4, sgrp = st & 15, orow = st >> 3, ochunk = st & 7;
     struct Stage {
-        u32x4 k, o;
-        uint32_t s;
+        u32x4 k[2], o;
+        uint32_t s[2];
     };
-    auto load = [&](Stage &g, int rd) {
-        const int i = rd * kRound + srow, j = rd * kRound + orow;
-        const bool ok = i < n;
-        g.k = __builtin_bit_cast(u32x4, buf_load16(rp, ok ? static_cast<uint32_t>(i) * static_cast<uint32_t>(a.p_t) + sgrp * 16u : kOobOffset));
-        g.s = __builtin_amdgcn_raw_buffer_load_b8(rs, ok ? static_cast<uint32_t>(i) * static_cast<uint32_t>(a.s_t) + sgrp : kOobOffset, 0, 0);
-        if (wave < 4)
-            g.o = __builtin_bit_cast(u32x4, buf_load16(rr, j < n ? static_cast<uint32_t>(j) * static_cast<uint32_t>(a.r_t) + ochunk * 16u : kOobOffset));
+    auto load = [&](Stage &g, int rd) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int i = rd * kRound + 16 * u + srow;
+            const bool ok = i < n;
+            g.k[u] = __builtin_bit_cast(u32x4, buf_load16(rp, ok ? static_cast<uint32_t>(i) * static_cast<uint32_t>(a.p_t) + sgrp * 16u : kOobOffset));
+            g.s[u] = __builtin_amdgcn_raw_buffer_load_b8(rs, ok ? static_cast<uint32_t>(i) * static_cast<uint32_t>(a.s_t) + sgrp : kOobOffset, 0, 0);
+        }
+        const int j = rd * kRound + orow;
+        g.o = __builtin_bit_cast(u32x4, buf_load16(rr, j < n ? static_cast<uint32_t>(j) * static_cast<uint32_t>(a.r_t) + ochunk * 16u : kOobOffset));
     };
-    auto store_k = [&](const Stage &g, int rd) {
-        char *k = kbuf + (rd % kKSlots) * kKBytes + srow * kKLd;
-        *reinterpret_cast<u32x4 *>(k + sgrp * 16) = g.k;
-        reinterpret_cast<uint8_t *>(k)[256 + sgrp] = static_cast<uint8_t>(g.s);
-        if (wave < 4) *reinterpret_cast<u32x4 *>(rbuf + (rd & 1) * kRBytes + orow * kRLd + ochunk * 16) = g.o;
+    auto store_k = [&](const Stage &g, int rd, bool look) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            char *k = kbuf + (rd % kKSlots) * kKBytes + (16 * u + srow) * kKLd;
+            *reinterpret_cast<u32x4 *>(k + sgrp * 16) = g.k[u];
+            reinterpret_cast<uint8_t *>(k)[256 + sgrp] = static_cast<uint8_t>(g.s[u]);
+            // (a NaN's values are staged as zeros; -0 codes count as values)
+            if (look && g.s[u] - kHalfLow > kHalfHigh - kHalfLow && g.s[u] != 255u && (g.k[u].x | g.k[u].y | g.k[u].z | g.k[u].w) != 0u)
+                wide = 1;
+        }
+        *reinterpret_cast<u32x4 *>(rbuf + (rd & 1) * kRBytes + orow * kRLd + ochunk * 16) = g.o;
     };
-    // this thread's group (which it staged itself) as bf16, 64 bytes; lanes 4..7, 8..11, 12..15 of a 16-lane row start at
-    // another 16 bytes, so a store instruction's lanes spread over the banks
-    auto store_v = [&](int rd) {
-        const char *ks = kbuf + (rd % kKSlots) * kKBytes + srow * kKLd;
+    // this thread's group (which it staged itself) as fp16 or bf16, 64 bytes; lanes 4..7, 8..11, 12..15 of a 16-lane row
+    // start at another 16 bytes, so a store instruction's lanes spread over the banks
+    auto store_v = [&](int rd, int u, auto bf) __attribute__((always_inline)) {
+        const char *ks = kbuf + (rd % kKSlots) * kKBytes + (16 * u + srow) * kKLd;
         const u32x4 k = *reinterpret_cast<const u32x4 *>(ks + sgrp * 16);
         const uint32_t s = reinterpret_cast<const uint8_t *>(ks)[256 + sgrp];
-        char *v = vbuf + (rd & 1) * kVBytes + srow * kVLd + sgrp * 64;
-        const float f = e8m0_to_f32(s);
+        char *v = vbuf + (rd & 1) * kVBytes + (16 * u + srow) * kVLd + sgrp * 64;
         const int x = (lane >> 2) & 3;
         const u32x4 y = (x & 1) ? u32x4{k.y, k.x, k.w, k.z} : k;
         u32x4 z = (x & 2) ? u32x4{y.z, y.w, y.x, y.y} : y;
         if (s == 255u) z = u32x4{0u, 0u, 0u, 0u};
-        const float fz = s == 255u ? 0.f : f;
+        const float f = s == 255u ? 0.f : e8m0_to_f32(s);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const u32x4 o = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], fz, 0)),
-                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], fz, 1)),
-                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], fz, 2)),
-                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], fz, 3))};
+            u32x4 o;
+            if constexpr (decltype(bf)::value)
+                o = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], f, 0)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], f, 1)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], f, 2)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], f, 3))};
+            else
+                o = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(z[j], f, 0)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(z[j], f, 1)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(z[j], f, 2)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(z[j], f, 3))};
             *reinterpret_cast<u32x4 *>(v + ((j ^ x) << 4)) = o;
         }
     };
 
-    // Iteration i (all waves): store round i + 1's codes (loaded two iterations before), load round i + 3, decode
-    // round i - 1.
-    Stage g[2];
-    load(g[0], 0);
-    load(g[1], 1);
-    const int iters = nr + 2;
+    // iterations 0 .. nr + 1, an even number of them (rounds past the last are zeros that no row sees)
+    const int iters = (nr + 3) & ~1;
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, 1> odd{};
+    if (tid == 0) wide = 0;
     if (wave < 4) {
         // ================= score waves
         const int rg = TG == 1 ? wave : wave % RG, tg = TG == 1 ? 0 : wave / RG;
@@ -303,10 +318,10 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         const int row = row0 + rg * 16 + r16;
         const int sees = row < a.rows ? q4_sees(a.t0 + row / a.H, cnt, len) : 0;
         const int limit = min(sees, t_end) - t_begin;       // positions of this split that the row sees
-        float m_ref = -INFINITY, l_run = 0.f;
+        float m_ref, l_run, mt[2];
         f32x4 sc[2][NTILE];                                 // scores of round i (parity)
 
-        auto scores = [&](int rd, f32x4 (&out)[NTILE]) {
+        auto scores = [&](int rd, f32x4 (&out)[NTILE]) __attribute__((always_inline)) {
             f32x4 hr[NTILE];
 #pragma unroll
             for (int u = 0; u < NTILE; ++u) hr[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -338,10 +353,11 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                     d = q4_mfma<3>(kc[3], ks, qlo[x][3], qhi[x][3], qs[x], d);
                 }
                 out[u] = hi + (lo + hr[u]);
+                __builtin_amdgcn_sched_barrier(0);   // (hoisting the next tile's operands costs the registers of a query term)
             }
         };
         // scores -> scaled (log2 units), hidden positions -infinity; the tile maxima are published
-        auto publish = [&](int rd, f32x4 (&s)[NTILE]) {
+        auto publish = [&](int rd, f32x4 (&s)[NTILE]) __attribute__((always_inline)) {
             float mt = -INFINITY;
 #pragma unroll
             for (int u = 0; u < NTILE; ++u)
@@ -355,7 +371,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
             if (TG > 1 && q4 == 0) xm[rd & 1][tg][rg * 16 + r16] = mt;
             return mt;
         };
-        auto probs = [&](int rd, const f32x4 (&s)[NTILE], float mt) {
+        auto probs = [&](int rd, const f32x4 (&s)[NTILE], float mt, auto bf) __attribute__((always_inline)) {
             if constexpr (TG > 1) mt = fmaxf(xm[rd & 1][0][rg * 16 + r16], xm[rd & 1][TG - 1][rg * 16 + r16]);
             float f = 1.f;
             if (mt > m_ref + kSlack || m_ref == -INFINITY) {
@@ -364,46 +380,62 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 l_run *= f;
                 m_ref = mt;
             }
-            const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-            char *p = pbuf + (rd & 1) * RG * PT * 1024 + rg * PT * 1024 + lane * 16;
+            const float ref = m_ref == -INFINITY ? 0.f : m_ref - kLift;
+            char *p = pbuf + ((rd & 1) * RG + rg) * kPLd + lane * 16;
 #pragma unroll
             for (int u = 0; u < NTILE; ++u) {
-                uint32_t e[3][2];
+                float e[4];
 #pragma unroll
-                for (int v = 0; v < 4; v += 2) {
-                    float p0 = __builtin_amdgcn_exp2f(s[u][v] - ref), p1 = __builtin_amdgcn_exp2f(s[u][v + 1] - ref);
-                    l_run += p0 + p1;
+                for (int v = 0; v < 4; ++v) {
+                    e[v] = __builtin_amdgcn_exp2f(s[u][v] - ref);
+                    l_run += e[v];
+                }
+                char *pu = p + (tg * NTILE + u) * 8;
+                if constexpr (!decltype(bf)::value) {
 #pragma unroll
                     for (int x = 0; x < PT; ++x) {
-                        e[x][v / 2] = q4_pack_bf16(p0, p1);
-                        p0 -= q4_lo(e[x][v / 2]), p1 -= q4_hi(e[x][v / 2]);
+                        const uint32_t a0 = q4_pack_f16(e[0], e[1]), a1 = q4_pack_f16(e[2], e[3]);
+                        *reinterpret_cast<u32x2 *>(pu + x * 1024) = u32x2{a0, a1};
+                        if (x + 1 < PT) {
+                            const f16x2 h0 = __builtin_bit_cast(f16x2, a0), h1 = __builtin_bit_cast(f16x2, a1);
+                            e[0] -= static_cast<float>(h0[0]), e[1] -= static_cast<float>(h0[1]);
+                            e[2] -= static_cast<float>(h1[0]), e[3] -= static_cast<float>(h1[1]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < PT + 1; ++x) {
+                        const uint32_t a0 = q4_pack_bf16(e[0], e[1]), a1 = q4_pack_bf16(e[2], e[3]);
+                        *reinterpret_cast<u32x2 *>(pu + x * 1024) = u32x2{a0, a1};
+                        e[0] -= q4_lo(a0), e[1] -= q4_hi(a0), e[2] -= q4_lo(a1), e[3] -= q4_hi(a1);
                     }
                 }
-#pragma unroll
-                for (int x = 0; x < PT; ++x) *reinterpret_cast<u32x2 *>(p + x * 1024 + (tg * NTILE + u) * 8) = u32x2{e[x][0], e[x][1]};
             }
             if (tg == 0 && q4 == 0) xf[rd & 1][rg * 16 + r16] = f;
         };
 
-        store_k(g[0], 0);
-        load(g[0], 2);
-        __syncthreads();
-        float mt[2] = {-INFINITY, -INFINITY};
-        for (int i0 = 0; i0 < iters; i0 += 2) {
-#pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                const int i = i0 + d;
-                if (i < iters) {
-                    store_k(g[(d + 1) & 1], i + 1);
-                    load(g[(d + 1) & 1], i + 3);
-                    if (i > 0) store_v(i - 1);
-                    scores(i, sc[d & 1]);
-                    if (i > 0) probs(i - 1, sc[(d + 1) & 1], mt[(d + 1) & 1]);
-                    mt[d & 1] = publish(i, sc[d & 1]);
-                    __syncthreads();
-                }
+        auto all = [&](auto bf) __attribute__((always_inline)) {
+            m_ref = -INFINITY, l_run = 0.f;
+            __syncthreads();   // wide is clear
+            __syncthreads();   // round 0 is staged
+            auto part = [&](int i, auto par) __attribute__((always_inline)) {
+                constexpr int d = decltype(par)::value;
+                scores(i, sc[d]);
+                probs(i - 1, sc[1 - d], mt[1 - d], bf);
+                mt[d] = publish(i, sc[d]);
+                __syncthreads();
+            };
+            scores(0, sc[0]);
+            mt[0] = publish(0, sc[0]);
+            __syncthreads();
+            part(1, odd);
+            for (int i = 2; i < iters; i += 2) {
+                part(i, even);
+                part(i + 1, odd);
             }
-        }
+        };
+        all(std::false_type{});
+        if (__builtin_amdgcn_readfirstlane(wide)) all(std::true_type{});
         const float l = q4_rows_sum(l_run);
         if (TG > 1 && q4 == 0) xl[tg][rg * 16 + r16] = l;
         __syncthreads();
@@ -412,19 +444,15 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         // ================= context waves: columns 128 (wave - 4) .. +128
         const int col0 = (wave - 4) * 128;
         f32x4 acc[8][RG];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-#pragma unroll
-            for (int r = 0; r < RG; ++r) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-        auto context = [&](int rd) {
-            const char *p = pbuf + (rd & 1) * RG * PT * 1024 + lane * 16;
-            u32x4 pf[RG][PT];
+        auto context = [&](int rd, auto bf) __attribute__((always_inline)) {
+            constexpr bool kBf = decltype(bf)::value;
+            constexpr int N = PT + kBf;
+            const char *p = pbuf + (rd & 1) * RG * kPLd + lane * 16;
+            const char *v = vbuf + (rd & 1) * kVBytes + (4 * q4 + (r16 >> 2)) * kVLd + (col0 + (r16 & 3) * 4) * 2;
             float f[RG];
             bool any = false;
 #pragma unroll
             for (int r = 0; r < RG; ++r) {
-#pragma unroll
-                for (int x = 0; x < PT; ++x) pf[r][x] = *reinterpret_cast<const u32x4 *>(p + (r * PT + x) * 1024);
                 f[r] = xf[rd & 1][r * 16 + r16];
                 any = any || f[r] != 1.f;
             }
@@ -434,34 +462,68 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int r = 0; r < RG; ++r) acc[c][r] *= f[r];
             }
-            const char *v = vbuf + (rd & 1) * kVBytes + (4 * q4 + (r16 >> 2)) * kVLd + (col0 + (r16 & 3) * 4) * 2;
+            u32x4 pf[RG][N];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
+            for (int r = 0; r < RG; ++r)
+#pragma unroll
+                for (int x = 0; x < N; ++x) pf[r][x] = *reinterpret_cast<const u32x4 *>(p + r * kPLd + x * 1024);
+            // the columns' operands are read two tiles ahead; nothing moves across a tile (that costs registers)
+            auto column = [&](int c) __attribute__((always_inline)) {
                 const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(v + c * 32));
                 const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(v + c * 32 + 16 * kVLd));
-                const u32x4 vf = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                return __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            u32x4 vf[2] = {column(0), column(1)};
 #pragma unroll
-                for (int t = PT - 1; t >= 0; --t)
+            for (int c = 0; c < 8; ++c) {
 #pragma unroll
-                    for (int r = 0; r < RG; ++r) acc[c][r] = q4_mfma_bf16(vf, pf[r][t], acc[c][r]);
+                for (int t = N - 1; t >= 0; --t)
+#pragma unroll
+                    for (int r = 0; r < RG; ++r)
+                        acc[c][r] = kBf ? q4_mfma_bf16(vf[c & 1], pf[r][t], acc[c][r]) : q4_mfma_f16(vf[c & 1], pf[r][t], acc[c][r]);
+                if (c + 2 < 8) vf[c & 1] = column(c + 2);
+                // the next round's values are decoded while the matrix cores work on this one's
+                if (c == 1 || c == 4) store_v(rd + 1, c / 4, bf);
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
-        store_k(g[0], 0);
-        load(g[0], 2);
-        __syncthreads();
-        for (int i0 = 0; i0 < iters; i0 += 2) {
+        auto all = [&](auto bf) __attribute__((always_inline)) {
 #pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                const int i = i0 + d;
-                if (i < iters) {
-                    store_k(g[(d + 1) & 1], i + 1);
-                    load(g[(d + 1) & 1], i + 3);
-                    if (i > 0) store_v(i - 1);
-                    if (i > 1) context(i - 2);
-                    __syncthreads();
-                }
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int r = 0; r < RG; ++r) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+            constexpr bool kLook = !decltype(bf)::value;
+            Stage g[2];
+            load(g[0], 0);
+            load(g[1], 1);
+            __syncthreads();
+            store_k(g[0], 0, kLook);
+            load(g[0], 2);
+            __syncthreads();
+            // store round i + 1's codes (loaded two iterations before), load round i + 3, decode round i - 1, take round
+            // i - 2's products
+            auto stage = [&](int i, auto par) __attribute__((always_inline)) {
+                constexpr int d = decltype(par)::value;
+                store_k(g[1 - d], i + 1, kLook);
+                load(g[1 - d], i + 3);
+            };
+            stage(0, even);
+            __syncthreads();
+            stage(1, odd);
+            store_v(0, 0, bf);
+            store_v(0, 1, bf);
+            __syncthreads();
+            for (int i = 2; i < iters; i += 2) {
+                stage(i, even);
+                context(i - 2, bf);
+                __syncthreads();
+                stage(i + 1, odd);
+                context(i - 1, bf);
+                __syncthreads();
             }
-        }
+        };
+        all(std::false_type{});
+        if (__builtin_amdgcn_readfirstlane(wide)) all(std::true_type{});
         __syncthreads();
         float *part = a.part + ((static_cast<int64_t>(b) * a.NS + split) * a.rows + row0) * kQ4Lat + col0 + 4 * q4;
 #pragma unroll
@@ -483,7 +545,7 @@ struct UvArgs {
     void *out;               // [B, Tall, H, V]
     int out_bf16;
     const float *gate;       // [B, Tall, H, V] or null
-    float2 *stats;           // [B][rows]: maximum, 1 / sum; or null
+    float2 *stats;           // [B][rows]: maximum less kLift, 1 / sum (which is lifted); or null
     int H, T, M, V, rows, NS, Tall, t0;
 };
 constexpr int kMaxSplits = 256;
@@ -507,7 +569,7 @@ __device__ __forceinline__ void store_out4(void *out, int bf16, const float *gat
 template <int CP>
 __global__ __launch_bounds__(256) void uv_kernel(UvArgs a) {
     constexpr int kLd = CP + 4;
-    extern __shared__ float sm[];
+    extern __shared__ __attribute__((aligned(16))) float sm[];
     float *const ctx = sm, *const wsp = sm + 16 * kLd, *const red = wsp + 16 * a.NS;   // red: 8 x CP, few queries
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
     const int h = blockIdx.x, m0 = blockIdx.y * 16, col0 = blockIdx.z * CP;
@@ -538,7 +600,7 @@ __global__ __launch_bounds__(256) void uv_kernel(UvArgs a) {
             const int s = lane + 64 * u;
             if (s < a.NS) wsp[i * a.NS + s] = v[u].y == 0.f ? 0.f : e[u] * inv;
         }
-        if (a.stats && blockIdx.z == 0 && lane == 0) a.stats[static_cast<int64_t>(b) * a.rows + row] = make_float2(mx, inv);
+        if (a.stats && blockIdx.z == 0 && lane == 0) a.stats[static_cast<int64_t>(b) * a.rows + row] = make_float2(mx - kLift, inv);
     }
     __syncthreads();
     constexpr int kC4 = CP / 4, kG = 256 / kC4;     // threads across the columns; groups of threads
@@ -751,18 +813,19 @@ struct Plan {
 
 constexpr int64_t kChunkRows = 1 << 16;   // rows (heads x queries, all sequences) of one pass over the queries
 
-// What the launches are cut into; a function of its arguments alone.  queries: of one pass (<= 0: as many as a pass takes)
-Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int out_bf16, int weights) {
+// What the launches are cut into; a function of its arguments alone.
+Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf16, int out_bf16, int weights, int varied) {
     Plan p{};
     const bool fine = !out_bf16 || weights;
-    p.NT = fine ? 5 : 4, p.RT = fine ? 3 : 2, p.PT = out_bf16 ? 2 : 3;
+    p.NT = fine ? 5 : 3, p.RT = q_bf16 ? 1 : fine ? 3 : 2, p.PT = out_bf16 ? 1 : 2;
     p.T = static_cast<int>(std::max<int64_t>(1, std::min(T, kChunkRows / (B * H))));
     p.rows = static_cast<int>(p.T * H);
     p.RG = p.rows > 64 ? 4 : 2;
     p.rblocks = static_cast<int>(cdiv(p.rows, 16 * p.RG));
     p.tiles = p.rblocks * p.RG;
     const int64_t base = B * p.rblocks;
-    int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, 256 / base));
+    // one block a CU; sequences of their own lengths: four, so the longest one's blocks are not what all wait for
+    int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (varied && B > 1 ? 1024 : 256) / base));
     int64_t ts = cdiv(cdiv(std::max<int64_t>(npos, 1), ns), kRound) * kRound;
     p.Ts = static_cast<int>(ts);
     p.NS = static_cast<int>(cdiv(std::max<int64_t>(npos, 1), ts));
@@ -795,6 +858,13 @@ int launch_attend(const AttendArgs &a, hipStream_t st) {
     return check_hip(hipGetLastError(), "mla q4: attention launch");
 }
 
+template <int RG>
+int launch_attend_of(const AttendArgs &a, const Plan &p, hipStream_t st) {
+    if (p.NT == 3) return p.RT == 1 ? launch_attend<RG, 3, 1, 1>(a, st) : launch_attend<RG, 3, 2, 1>(a, st);
+    if (p.PT == 1) return p.RT == 1 ? launch_attend<RG, 5, 1, 1>(a, st) : launch_attend<RG, 5, 3, 1>(a, st);
+    return p.RT == 1 ? launch_attend<RG, 5, 1, 2>(a, st) : launch_attend<RG, 5, 3, 2>(a, st);
+}
+
 template <typename QT, int NT, int RT>
 int launch_qa(const QaArgs &a, hipStream_t st) {
     const int bytes = std::max(((a.nope + 31) / 32) * 32 * kWLd, 16 * kFLd * 4);
@@ -822,10 +892,10 @@ int launch_uv(const UvArgs &a, hipStream_t st) {
 
 using namespace k3;
 
-extern "C" int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim, int64_t max_length, int out_dtype,
-                                            int weights) {
+extern "C" int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim, int64_t max_length, int q_dtype,
+                                            int out_dtype, int weights, int varied) {
     if (B <= 0 || T <= 0 || H <= 0 || v_dim <= 0 || max_length < 0) return 0;
-    return plan_of(B, T, H, v_dim, max_length, out_dtype == K3_BF16, weights != 0).total;
+    return plan_of(B, T, H, v_dim, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weights != 0, varied != 0).total;
 }
 
 extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t qn_token, int64_t qn_head, const void *q_rot,
@@ -858,7 +928,7 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
     if (!aligned16(q_nope) || !aligned16(q_rot) || !aligned16(w_uk) || !aligned16(w_uv) || !aligned16(out) || !aligned16(workspace) ||
         !aligned16(packed) || !aligned16(rot) || (gate && !aligned16(gate)))
         return set_error(K3_ERR_ALIGN, "mla q4: queries, weights, cache, output and workspace must be 16-byte aligned");
-    const Plan p = plan_of(B, T, H, v_dim, max_length, out_dtype == K3_BF16, weight != nullptr);
+    const Plan p = plan_of(B, T, H, v_dim, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weight != nullptr, lengths != nullptr);
     if (workspace_bytes < p.total)
         return set_error(K3_ERR_WORKSPACE, "mla q4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.total);
     if (static_cast<int64_t>(p.Ts) * std::max(p_row, 2 * rot_row) >= (1ll << 31))
@@ -872,10 +942,10 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         QaArgs qa{q_nope, q_rot, qn_batch, qn_token, qn_head, qr_batch, qr_token, qr_head, static_cast<const uint16_t *>(w_uk),
                   ws + p.qop, q_seq, static_cast<int>(H), static_cast<int>(nope_dim), Tc, static_cast<int>(B * Tc), static_cast<int>(t0)};
         int rc;
-        if (p.NT == 5)
-            rc = q_dtype == K3_F32 ? launch_qa<float, 5, 3>(qa, st) : launch_qa<uint16_t, 5, 3>(qa, st);
+        if (q_dtype == K3_BF16)
+            rc = p.NT == 5 ? launch_qa<uint16_t, 5, 1>(qa, st) : launch_qa<uint16_t, 3, 1>(qa, st);
         else
-            rc = q_dtype == K3_F32 ? launch_qa<float, 4, 2>(qa, st) : launch_qa<uint16_t, 4, 2>(qa, st);
+            rc = p.NT == 5 ? launch_qa<float, 5, 3>(qa, st) : launch_qa<float, 3, 2>(qa, st);
         if (rc) return rc;
         AttendArgs a{};
         a.qop = ws + p.qop, a.q_seq = q_seq;
@@ -888,14 +958,7 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         a.H = static_cast<int>(H), a.T = Tc, a.t0 = static_cast<int>(t0), a.rows = rows, a.Ts = p.Ts, a.NS = p.NS, a.rblocks = rblocks;
         a.B = static_cast<int>(B), a.c = scale * 1.4426950408889634f;
         a.swizzle = (a.B * a.NS * rblocks) % 8 == 0;
-        if (p.RG == 4)
-            rc = p.NT == 4   ? launch_attend<4, 4, 2, 2>(a, st)
-                 : p.PT == 2 ? launch_attend<4, 5, 3, 2>(a, st)
-                             : launch_attend<4, 5, 3, 3>(a, st);
-        else
-            rc = p.NT == 4   ? launch_attend<2, 4, 2, 2>(a, st)
-                 : p.PT == 2 ? launch_attend<2, 5, 3, 2>(a, st)
-                             : launch_attend<2, 5, 3, 3>(a, st);
+        rc = p.RG == 4 ? launch_attend_of<4>(a, p, st) : launch_attend_of<2>(a, p, st);
         if (rc) return rc;
         UvArgs u{};
         u.part = a.part, u.ml = a.ml, u.w_uv = static_cast<const uint16_t *>(w_uv);
@@ -916,7 +979,10 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
                           0, static_cast<int>(max_length)};
             wa.chunks = static_cast<int>(cdiv(wa.tiles, wa.chunk));
             const dim3 grid(static_cast<unsigned>(cdiv(max_length, 128 * kWTiles)), static_cast<unsigned>(wa.chunks), static_cast<unsigned>(B));
-            weights_kernel<5, 3><<<grid, 512, 0, st>>>(wa);
+            if (p.RT == 1)
+                weights_kernel<5, 1><<<grid, 512, 0, st>>>(wa);
+            else
+                weights_kernel<5, 3><<<grid, 512, 0, st>>>(wa);
             rc = check_hip(hipGetLastError(), "mla q4: weights launch");
             if (rc) return rc;
             weights_add_kernel<<<dim3(static_cast<unsigned>(cdiv(max_length, 256)), static_cast<unsigned>(B)), 256, 0, st>>>(wa);

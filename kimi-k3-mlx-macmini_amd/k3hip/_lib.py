@@ -59,7 +59,7 @@ SIGNATURES: dict[str, list] = {
                            _F32, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P],
     "k3_mla_q4_append": [_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64,
                          _P, _I64, _I64, _I64, _I64, _I64, _P],
-    "k3_mla_q4_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I32, _I32],
+    "k3_mla_q4_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32],
     "k3_mla_q4_attention": [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I32, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64,
                             _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F32, _P, _P, _I32, _P, _I64, _P,
                             _I64, _P],

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from . import _torch as T
-from .mla_q4 import _per_sequence
+from .mla_q4 import _keep_plan, _layout, _per_sequence, _plans
 
 MAX_BUFFERS = 8
 
@@ -29,12 +29,40 @@ def cache_evict(weight: torch.Tensor, buffers, keep: int, lengths: torch.Tensor 
     <= keep): ties go to the lowest position, a NaN weight counts below all others.  index: the positions that stayed, ascending, then -1.
     Rows past a sequence's new length are zero.  ``capacity``: rows of the new buffers (default: keep).
     """
+    buffers = list(buffers)
+    length = lengths if not isinstance(lengths, torch.Tensor) else None
+    if length is not None:
+        lengths = None
+    key = (weight.shape, weight.stride(), weight.dtype, keep, length, _layout(lengths), sink, recent, capacity,
+           *[(x.shape, x.stride(), x.dtype) for x in buffers])
+    (B, cap, keep, sink, recent, rows, most, w_pitch, direct, shapes, arrays, ptrs) = _plans.get(key) or _keep_plan(
+        key, _evict_plan(weight, buffers, keep, length, lengths, sink, recent, capacity))
+    T.require_device(weight, lengths, *buffers)
+    if T.tracked(*buffers):
+        raise ValueError("cache_evict carries no gradient: call it under no_grad or on detached buffers")
+    if w_pitch is None:
+        weight, w_pitch = weight.contiguous(), cap
+    if not all(direct):
+        # (their layout is the key's: a copy's pitches are those of a contiguous buffer, which the plan holds)
+        buffers = [x if ok else x.contiguous() for x, ok in zip(buffers, direct)]
+    new = [x.new_empty(s) for x, s in zip(buffers, shapes)]
+    index, kept = weight.new_empty((B, keep), dtype=torch.int32), weight.new_empty(B, dtype=torch.int32)
+    if B == 0:
+        return new, index, kept
+    src_b, src_r, dst_b, dst_r, size = arrays
+    with T.current(weight.device):
+        _lib.call("k3_cache_evict", weight.data_ptr(), w_pitch, T.ptr(lengths), most, B, keep, sink, recent, index.data_ptr(),
+                  kept.data_ptr(), len(new), ptrs(*[x.data_ptr() for x in buffers]), src_b, src_r, ptrs(*[x.data_ptr() for x in new]),
+                  dst_b, dst_r, size, rows, T.stream(weight))
+    return new, index, kept
+
+
+def _evict_plan(weight, buffers, keep, length, lengths, sink, recent, capacity) -> tuple:
     if weight.dim() != 2:
         raise ValueError(f"weight must be [B, cap]; got {tuple(weight.shape)}")
     if weight.dtype != torch.float32:
         raise TypeError(f"weight must be float32; got {weight.dtype}")
     B, cap = weight.shape
-    buffers = list(buffers)
     if len(buffers) > MAX_BUFFERS:
         raise ValueError(f"at most {MAX_BUFFERS} buffers; got {len(buffers)}")
     keep, sink, recent = int(keep), int(sink), int(recent)
@@ -46,32 +74,23 @@ def cache_evict(weight: torch.Tensor, buffers, keep: int, lengths: torch.Tensor 
     for x in buffers:
         if x.dim() < 2 or tuple(x.shape[:2]) != (B, cap):
             raise ValueError(f"buffers must be [{B}, {cap}, ...]; got {tuple(x.shape)}")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise ValueError("cache_evict carries no gradient: call it under no_grad or on detached buffers")
-    T.require_device(weight, *buffers)
-    device, most = weight.device, cap
-    if lengths is not None and not isinstance(lengths, torch.Tensor):
-        most, lengths = int(lengths), None
+    most = cap
+    if length is not None:
+        most = int(length)
         if not 0 <= most <= cap:
             raise ValueError(f"length {most} outside the capacity {cap}")
-    lengths = _per_sequence(lengths, B, "lengths", device)
-    if cap > 1 and weight.stride(1) != 1:
-        weight = weight.contiguous()
-    src = [x if x[0, :1].is_contiguous() and (cap < 2 or x.stride(1) >= math.prod(x.shape[2:])) else x.contiguous()
-           for x in buffers] if B else buffers
-    new = [torch.empty((B, rows, *x.shape[2:]), dtype=x.dtype, device=device) for x in buffers]
-    index = torch.empty((B, keep), dtype=torch.int32, device=device)
-    kept = torch.empty(B, dtype=torch.int32, device=device)
-    if B == 0:
-        return new, index, kept
-    n = len(src)
-    size = [math.prod(x.shape[2:]) * x.element_size() for x in src]
-    longs, ptrs = ctypes.c_int64 * max(n, 1), ctypes.c_void_p * max(n, 1)
-    src_b = longs(*[x.stride(0) * x.element_size() if B > 1 else 0 for x in src])
-    src_r = longs(*[x.stride(1) * x.element_size() if cap > 1 else s for x, s in zip(src, size)])
-    dst_b, dst_r = longs(*[rows * s for s in size]), longs(*size)
-    with T.current(device):
-        _lib.call("k3_cache_evict", T.ptr(weight), weight.stride(0) if B > 1 else 0, T.ptr(lengths), most, B, keep, sink, recent,
-                  T.ptr(index), T.ptr(kept), n, ptrs(*[x.data_ptr() for x in src]), src_b, src_r,
-                  ptrs(*[x.data_ptr() for x in new]), dst_b, dst_r, longs(*size), rows, T.stream(weight))
-    return new, index, kept
+    _per_sequence(lengths, B, "lengths")
+    width = [math.prod(x.shape[2:]) for x in buffers]
+    size = [n * x.element_size() for n, x in zip(width, buffers)]
+    direct, src_b, src_r = [], [], []
+    for x, n in zip(buffers, width):
+        ok = B == 0 or cap == 0 or (x[0, 0].is_contiguous() and (cap < 2 or x.stride(1) >= n) and (B < 2 or x.stride(0) >= 0))
+        e = x.element_size()
+        direct.append(ok)
+        src_b.append((x.stride(0) if ok else cap * n) * e if B > 1 else 0)
+        src_r.append((x.stride(1) if ok else n) * e if cap > 1 else n * e)
+    longs = ctypes.c_int64 * max(len(buffers), 1)
+    return (B, cap, keep, sink, recent, rows, most, None if cap > 1 and weight.stride(1) != 1 else weight.stride(0) if B > 1 else 0,
+            tuple(direct), tuple((B, rows, *x.shape[2:]) for x in buffers),
+            (longs(*src_b), longs(*src_r), longs(*[rows * s for s in size]), longs(*size), longs(*size)),
+            ctypes.c_void_p * max(len(buffers), 1))

@@ -23,6 +23,19 @@ LATENT, ROPE, GROUP = 512, 64, 32
 KEPT_WORKSPACE = 1 << 26
 
 
+# What a call's layout (shapes, strides, dtypes; no addresses) comes to, once its checks are passed: the checks cost
+# more than a short call's kernels.
+_plans: dict[tuple, tuple] = {}
+MAX_PLANS = 4096
+
+
+def _keep_plan(key: tuple, plan: tuple) -> tuple:
+    if len(_plans) >= MAX_PLANS:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
 def _buffers(packed, scales, rot):
     """The cache's three buffers as [B, cap, .]: dtypes, shapes and row layout."""
     for t, name, width, dtype in ((packed, "packed", LATENT // 2, torch.uint8), (scales, "scales", LATENT // GROUP, torch.uint8),
@@ -39,17 +52,18 @@ def _buffers(packed, scales, rot):
     return packed.shape[:2]
 
 
-def _per_sequence(v, B: int, name: str, device) -> torch.Tensor | None:
-    """An int32 [B] device tensor as it is, None as None."""
+def _per_sequence(v: torch.Tensor | None, B: int, name: str) -> None:
+    """Refuses what is neither None nor a contiguous int32 [B] tensor."""
     if v is None:
-        return None
+        return
     if v.dtype != torch.int32:
         raise TypeError(f"{name} must be an int32 tensor; got {v.dtype}")
-    if tuple(v.shape) != (B,):
-        raise ValueError(f"{name} must be [{B}]; got {tuple(v.shape)}")
-    if v.device != device:
-        raise ValueError(f"{name} is on {v.device}, the cache on {device}")
-    return v.contiguous()
+    if tuple(v.shape) != (B,) or not v.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{B}]; got {tuple(v.shape)}")
+
+
+def _layout(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
 
 
 def _pitches(t: torch.Tensor) -> tuple[int, int]:
@@ -57,11 +71,9 @@ def _pitches(t: torch.Tensor) -> tuple[int, int]:
     return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else max(t.stride(1), t.shape[2]))
 
 
-def _row_input(t: torch.Tensor, per: int) -> torch.Tensor:
-    """Contiguous rows, pitches of whole 16 bytes (``per`` elements), a 16-byte aligned base; else a copy."""
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % per for s in t.stride()[:-1]):
-        t = T.contiguous_aligned(t)
-    return t
+def _rows_ok(t: torch.Tensor, per: int) -> bool:
+    """Contiguous rows, pitches of whole 16 bytes (``per`` elements): read as they are where the base is aligned too."""
+    return t.stride(-1) == 1 and not any(s % per for s in t.stride()[:-1])
 
 
 def mla_q4_append(c_new: torch.Tensor, r_new: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, rot: torch.Tensor,
@@ -75,28 +87,39 @@ def mla_q4_append(c_new: torch.Tensor, r_new: torch.Tensor, packed: torch.Tensor
     largest magnitude at 4 to 7 times itself (above 7 the next one); codes round to nearest even.  A position with a NaN or an
     infinity is NaN to every query that sees it.
     """
+    starts = start if isinstance(start, torch.Tensor) else None
+    key = (c_new.shape, c_new.stride(), c_new.dtype, r_new.shape, r_new.stride(), r_new.dtype, packed.shape, packed.stride(),
+           packed.dtype, scales.shape, scales.stride(), scales.dtype, rot.shape, rot.stride(), rot.dtype, _layout(starts), _layout(counts))
+    B, n, cap, c_ok, r_ok, cdt, rdt, pp, sp, rp = _plans.get(key) or _keep_plan(
+        key, _append_plan(c_new, r_new, packed, scales, rot, starts, counts))
+    start0 = 0 if starts is not None else int(start)
+    if starts is None and not 0 <= start0 <= start0 + n <= cap:
+        raise ValueError(f"{n} tokens at position {start0} do not fit a capacity of {cap}")
+    T.require_device(c_new, r_new, packed, scales, rot, starts, counts)
+    if B == 0 or n == 0 or cap == 0:
+        return
+    if not c_ok or c_new.data_ptr() % 16:
+        c_new = T.contiguous_aligned(c_new)
+    if not r_ok:
+        r_new = r_new.contiguous()
+    cs, rs = c_new.stride(), r_new.stride()
+    with T.current(packed.device):
+        _lib.call("k3_mla_q4_append", c_new.data_ptr(), cs[0], cs[1], cdt, r_new.data_ptr(), rs[0], rs[1], rdt, packed.data_ptr(),
+                  *pp, scales.data_ptr(), *sp, rot.data_ptr(), *rp, 0 if starts is None else starts.data_ptr(), start0,
+                  0 if counts is None else counts.data_ptr(), B, n, cap, LATENT, ROPE, T.stream(packed))
+
+
+def _append_plan(c_new, r_new, packed, scales, rot, starts, counts) -> tuple:
     B, cap = _buffers(packed, scales, rot)
     if c_new.dim() != 3 or r_new.dim() != 3 or c_new.shape[2] != LATENT or r_new.shape[2] != ROPE or \
             c_new.shape[:2] != r_new.shape[:2] or c_new.shape[0] != B:
         raise ValueError(f"c_new [B, T, {LATENT}] and r_new [B, T, {ROPE}] with B = {B} expected; got {tuple(c_new.shape)}, "
                          f"{tuple(r_new.shape)}")
-    n = c_new.shape[1]
-    T.require_device(c_new, r_new, packed, scales, rot)
     cdt, rdt = T.dtype_code(c_new.dtype), T.dtype_code(r_new.dtype)
-    starts, start0 = (start, 0) if isinstance(start, torch.Tensor) else (None, int(start))
-    starts = _per_sequence(starts, B, "start", packed.device)
-    counts = _per_sequence(counts, B, "counts", packed.device)
-    if starts is None and not 0 <= start0 <= start0 + n <= cap:
-        raise ValueError(f"{n} tokens at position {start0} do not fit a capacity of {cap}")
-    if B == 0 or n == 0 or cap == 0:
-        return
-    c_new = _row_input(c_new, 16 // c_new.element_size())
-    if r_new.stride(2) != 1:
-        r_new = r_new.contiguous()
-    with T.current(packed.device):
-        _lib.call("k3_mla_q4_append", c_new.data_ptr(), c_new.stride(0), c_new.stride(1), cdt, r_new.data_ptr(), r_new.stride(0),
-                  r_new.stride(1), rdt, packed.data_ptr(), *_pitches(packed), scales.data_ptr(), *_pitches(scales), rot.data_ptr(),
-                  *_pitches(rot), T.ptr(starts), start0, T.ptr(counts), B, n, cap, LATENT, ROPE, T.stream(packed))
+    _per_sequence(starts, B, "start")
+    _per_sequence(counts, B, "counts")
+    return (B, c_new.shape[1], cap, _rows_ok(c_new, 16 // c_new.element_size()), r_new.stride(2) == 1, cdt, rdt, _pitches(packed),
+            _pitches(scales), _pitches(rot))
 
 
 def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor, wv: torch.Tensor, packed: torch.Tensor,
@@ -114,6 +137,40 @@ def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor
     ``weight`` fp32 [B, cap], changed in place: every position's attention weight, summed over the queries and heads, is
     added to it.  ``gate`` [B, T, H * v] fp32: the output times sigmoid(gate).
     """
+    length = lengths if not isinstance(lengths, torch.Tensor) else None
+    if length is not None:
+        lengths = None
+    key = (q_nope.shape, q_nope.stride(), q_nope.dtype, q_rot.shape, q_rot.stride(), q_rot.dtype, wk.shape, wk.dtype, wv.shape, wv.dtype,
+           packed.shape, packed.stride(), packed.dtype, scales.shape, scales.stride(), scales.dtype, rot.shape, rot.stride(), rot.dtype,
+           length, _layout(lengths), _layout(counts), _layout(weight), None if gate is None else gate.shape, out_dtype)
+    (B, Tq, H, V, nope, most, qdt, code, out_code, n_ok, r_ok, pp, sp, rp, w_pitch, nbytes) = _plans.get(key) or _keep_plan(
+        key, _attention_plan(q_nope, q_rot, wk, wv, packed, scales, rot, length, lengths, counts, weight, gate, out_dtype))
+    T.require_device(q_nope, q_rot, wk, wv, packed, scales, rot, weight, gate, lengths, counts)
+    if T.tracked(q_nope, q_rot, wk, wv, rot, gate):
+        raise ValueError("mla_q4_attention carries no gradient: call it under no_grad or on detached tensors")
+    device = packed.device
+    out = torch.empty((B, Tq, H, V), dtype=out_dtype, device=device)
+    if B == 0 or Tq == 0:
+        return out
+    if gate is not None:
+        gate = T.contiguous_aligned(gate.to(torch.float32))
+    if not n_ok or q_nope.data_ptr() % 16:
+        q_nope = T.contiguous_aligned(q_nope.to(qdt))
+    if not r_ok or q_rot.data_ptr() % 16:
+        q_rot = T.contiguous_aligned(q_rot.to(qdt))
+    wk, wv = T.contiguous_aligned(wk), T.contiguous_aligned(wv)
+    ns, rs = q_nope.stride(), q_rot.stride()
+    with T.current(device):
+        ws = (_workspace.get(device, nbytes, "mla_q4") if nbytes <= KEPT_WORKSPACE
+              else torch.empty(nbytes, dtype=torch.uint8, device=device))
+        _lib.call("k3_mla_q4_attention", q_nope.data_ptr(), ns[0], ns[1], ns[2], q_rot.data_ptr(), rs[0], rs[1], rs[2], code,
+                  wk.data_ptr(), wv.data_ptr(), packed.data_ptr(), *pp, scales.data_ptr(), *sp, rot.data_ptr(), *rp, T.ptr(lengths),
+                  T.ptr(counts), most, B, Tq, H, LATENT, ROPE, nope, V, scale, T.ptr(gate), out.data_ptr(), out_code, T.ptr(weight),
+                  w_pitch, ws.data_ptr(), ws.numel(), T.stream(packed))
+    return out
+
+
+def _attention_plan(q_nope, q_rot, wk, wv, packed, scales, rot, length, lengths, counts, weight, gate, out_dtype) -> tuple:
     B, cap = _buffers(packed, scales, rot)
     if q_nope.dim() != 4 or q_rot.dim() != 4 or q_nope.shape[:3] != q_rot.shape[:3] or q_nope.shape[0] != B or q_rot.shape[3] != ROPE:
         raise ValueError(f"q_nope [B, T, H, nope] and q_rot [B, T, H, {ROPE}] with B = {B} expected; got {tuple(q_nope.shape)}, "
@@ -124,40 +181,24 @@ def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor
     if wk.dtype != torch.bfloat16 or wv.dtype != torch.bfloat16:
         raise TypeError("wk and wv must be bfloat16 (the checkpoint dtype)")
     V = wv.shape[1]
-    T.require_device(q_nope, q_rot, wk, wv, packed, scales, rot, weight, gate)
-    if T.tracked(q_nope, q_rot, wk, wv, rot, gate):
-        raise ValueError("mla_q4_attention carries no gradient: call it under no_grad or on detached tensors")
-    device = packed.device
     most = cap
-    if lengths is not None and not isinstance(lengths, torch.Tensor):
-        most, lengths = int(lengths), None
+    if length is not None:
+        most = int(length)
         if not 0 <= most <= cap:
             raise ValueError(f"length {most} outside the capacity {cap}")
-    lengths = _per_sequence(lengths, B, "lengths", device)
-    counts = _per_sequence(counts, B, "counts", device)
+    _per_sequence(lengths, B, "lengths")
+    _per_sequence(counts, B, "counts")
     if weight is not None:
         if weight.dtype != torch.float32:
             raise TypeError(f"weight must be float32; got {weight.dtype}")
         if tuple(weight.shape) != (B, cap) or (cap > 1 and weight.stride(1) != 1):
             raise ValueError(f"weight must be [{B}, {cap}] with contiguous rows; got {tuple(weight.shape)}")
-    if gate is not None:
-        if gate.numel() != B * Tq * H * V or gate.shape[:2] != (B, Tq):
-            raise ValueError(f"gate must be [{B}, {Tq}, {H * V}]; got {tuple(gate.shape)}")
-        gate = T.contiguous_aligned(gate.to(torch.float32))
+    if gate is not None and (gate.numel() != B * Tq * H * V or gate.shape[:2] != (B, Tq)):
+        raise ValueError(f"gate must be [{B}, {Tq}, {H * V}]; got {tuple(gate.shape)}")
     out_code = T.dtype_code(out_dtype)
-    out = torch.empty((B, Tq, H, V), dtype=out_dtype, device=device)
-    if out.numel() == 0:
-        return out
     qdt = torch.bfloat16 if q_nope.dtype == torch.bfloat16 and q_rot.dtype == torch.bfloat16 else torch.float32
-    q_nope, q_rot = _row_input(q_nope.to(qdt), 4), _row_input(q_rot.to(qdt), 4)
-    wk, wv = T.contiguous_aligned(wk), T.contiguous_aligned(wv)
-    nbytes = _lib.size("k3_mla_q4_workspace_size", B, Tq, H, V, most, out_code, 0 if weight is None else 1)
-    with T.current(device):
-        ws = (_workspace.get(device, nbytes, "mla_q4") if nbytes <= KEPT_WORKSPACE
-              else torch.empty(nbytes, dtype=torch.uint8, device=device))
-        _lib.call("k3_mla_q4_attention", q_nope.data_ptr(), *q_nope.stride()[:3], q_rot.data_ptr(), *q_rot.stride()[:3],
-                  T.dtype_code(qdt), wk.data_ptr(), wv.data_ptr(), packed.data_ptr(), *_pitches(packed), scales.data_ptr(),
-                  *_pitches(scales), rot.data_ptr(), *_pitches(rot), T.ptr(lengths), T.ptr(counts), most, B, Tq, H, LATENT, ROPE,
-                  nope, V, float(scale), T.ptr(gate), out.data_ptr(), out_code, T.ptr(weight),
-                  0 if weight is None else weight.stride(0), ws.data_ptr(), ws.numel(), T.stream(packed))
-    return out
+    nbytes = _lib.size("k3_mla_q4_workspace_size", B, Tq, H, V, most, T.dtype_code(qdt), out_code, 0 if weight is None else 1,
+                       0 if lengths is None else 1)
+    return (B, Tq, H, V, nope, most, qdt, T.dtype_code(qdt), out_code, q_nope.dtype == qdt and _rows_ok(q_nope, 4),
+            q_rot.dtype == qdt and _rows_ok(q_rot, 4), _pitches(packed), _pitches(scales), _pitches(rot),
+            0 if weight is None or B == 1 else weight.stride(0), nbytes)

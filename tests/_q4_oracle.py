@@ -52,12 +52,12 @@ def attention(q_nope, q_rot, wk, wv, packed, scales, rot, scale, lengths, counts
     """-> (o, bound on |error of o|, weight sums, bound on theirs), float64.  lengths, counts: lists.
 
     The bounds, u = 2^-24 (half a step of fp32):
-    * qa: fp32 sums of nope products, the fp32 query split exactly: (nope + 4) u of sum |q W|; its terms leave at most 2^-22 (fine) or
-      2^-17 of a unit that is at most the group's largest / 3.75;
+    * qa: fp32 sums of nope products, the fp32 query split exactly: (nope + 4) u of sum |q W|; its terms leave at most 2^-22 (fine, five terms) or
+      2^-12 (three) of a unit that is at most the group's largest / 3.75;
     * a score: that, times |lat|; its sum of at most 26 matrix instructions in a row and four joins, each
       rounding once and adding its products exactly to 2u: 64 u of the sum of magnitudes; the rotary query's two terms leave 2^-17 (fine: 2^-25);
       the scaling to log2 units and the subtraction of the maximum: 4 u of |s| and of the maximum;
-    * a probability: the score errors of itself and of the normaliser (2 E), exp2 2 u, its terms 2^-17 (fine 2^-25), a rescale per round;
+    * a probability: the score errors of itself and of the normaliser (2 E), exp2 2 u, its terms 2^-11 (one fp16) or 2^-22 (fine, two), a rescale per round;
     * sums over n positions: n / 32 rounds of up to 3 products, the joins of splits: (n / 8 + 300) u;
     * W_UV: three terms, 512 products: 64 u and 2^-24; then the rounding of the output, out_eps.
     """
@@ -81,12 +81,12 @@ def attention(q_nope, q_rot, wk, wv, packed, scales, rot, scale, lengths, counts
             qa = torch.einsum("hn,hnr->hr", q, wk64)
             s = (qa @ L.T + qr @ R.T) * scale                                       # [H, v]
             top = qa.abs().reshape(H, 16, 32).amax(2, keepdim=True).expand(H, 16, 32).reshape(H, 512)
-            left = torch.einsum("hn,hnr->hr", q.abs(), wk64.abs()) * (nope + 4) * u + top * (2.0 ** -22 if fine_q else 2.0 ** -17) / 3.75
+            left = torch.einsum("hn,hnr->hr", q.abs(), wk64.abs()) * (nope + 4) * u + top * (2.0 ** -22 if fine_q else 2.0 ** -12) / 3.75
             left_r = qr.abs() * (2.0 ** -25 if fine_q else 2.0 ** -17)
             E = (left @ L.abs().T + left_r @ R.abs().T + 64 * u * (qa.abs() @ L.abs().T + qr.abs() @ R.abs().T)) * abs(scale)
             E = (E + 4 * u * (s.abs() + s.abs().amax(1, keepdim=True))).amax(1, keepdim=True)
             p = torch.softmax(s, -1)
-            rel_p = torch.expm1(2 * E) + 4 * u + (2.0 ** -25 if fine_p else 2.0 ** -17) + v / 16 * u
+            rel_p = torch.expm1(2 * E) + 4 * u + (2.0 ** -22 if fine_p else 2.0 ** -11) + v / 16 * u
             ctx, mag = p @ L, p @ L.abs()
             e_ctx = mag * (rel_p + (v / 8 + 300) * u)
             o[b, t] = torch.einsum("hr,hvr->hv", ctx, wv64)

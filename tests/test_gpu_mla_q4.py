@@ -247,7 +247,7 @@ def test_queries_of_any_size(std):
         _check(args, weight=True)
 
 
-@pytest.mark.parametrize("byte", [2, 30, 200, 225])
+@pytest.mark.parametrize("byte", [2, 30, 102, 106, 108, 136, 138, 142, 200, 225])
 def test_cache_values_of_any_size(byte):
     """Latents far from one: the scale bytes' exponent goes through the products as it is (225: values of 2^100, with
     queries small enough for finite scores)."""
@@ -255,6 +255,21 @@ def test_cache_values_of_any_size(byte):
     scales = scales - 126 + byte if byte > 4 else torch.full_like(scales, 2)
     q = q_nope * 2.0 ** -(byte - 126) if byte > 126 else q_nope
     _check((q, q_rot, wk, wv, packed, scales, rot))
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("H", [20, 80])
+@pytest.mark.parametrize("at,byte", [(0, 90), (33, 150), (64, 60), (127, 103), (100, 141)])
+def test_a_single_group_past_half_precision(at, byte, H, out):
+    """One group of one position whose values fp16 does not hold, early or late in the sequence; the query is small there, so the
+    scores stay finite."""
+    q_nope, q_rot, wk, wv, packed, scales, rot = _problem(1, 2, H, 128, 105, x=out)
+    scales[0, at, 5] = byte
+    wk = wk.clone()
+    if byte > 127:
+        wk[:, :, 160:192] *= 2.0 ** (126 - byte)
+    _check((q_nope, q_rot, wk, wv, packed, scales, rot), out=out)
+    _check((q_nope, q_rot, wk, wv, packed, scales, rot), [at], out=out)     # behind the end: no reason to care
 
 
 def test_growing_scores_move_the_reference():

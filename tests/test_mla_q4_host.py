@@ -135,8 +135,8 @@ def test_entry_points_check_their_arguments():
     assert append(_0=ctypes.c_void_p(4104)) == _lib.K3_ERR_ALIGN and append(_8=ctypes.c_void_p(4097)) == _lib.K3_ERR_ALIGN
     assert append(_21=0) == _lib.K3_OK and append(_20=0) == _lib.K3_OK
 
-    size = lib.k3_mla_q4_workspace_size(2, 3, 4, 96, 8, 0, 1)
-    assert size > 0 and lib.k3_mla_q4_workspace_size(0, 3, 4, 96, 8, 0, 1) == 0
+    size = lib.k3_mla_q4_workspace_size(2, 3, 4, 96, 8, 0, 0, 1, 0)
+    assert size > 0 and lib.k3_mla_q4_workspace_size(0, 3, 4, 96, 8, 0, 0, 1, 0) == 0
     att = [p, 1536, 512, 128, p, 768, 256, 64, 0, p, p, p, 2048, 256, p, 128, 16, p, 512, 64, n, n, 8, 2, 3, 4, 512, 64, 128, 96,
            0.1, n, p, 0, p, 8, p, size, n]
 
