@@ -33,6 +33,21 @@ namespace {
 typedef short s4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4_t *lds_s4;
 
+// The order of a sequence's rows: by query (row = t H + h: the heads of one query are neighbours, few queries fill the tiles)
+// or by head (row = h Tp + t, Tp = T rounded up to 16: a tile is 16 queries of one head, so a block of the query and output
+// launches, which takes one head's matrix, writes and reads whole tiles).
+struct Rows {
+    int T, H, Tp;                           // Tp 0: by query
+    __host__ __device__ int count() const { return Tp ? H * Tp : T * H; }
+    __device__ int of(int t, int h) const { return Tp ? h * Tp + t : t * H + h; }
+    __device__ int query(int row) const { return Tp ? row % Tp : row / H; }       // may be >= T: no row
+    // the last query of rows row0 .. row1
+    __device__ int last_query(int row0, int row1) const {
+        if (!Tp) return row1 / H;
+        return row0 / Tp != row1 / Tp ? T - 1 : min(row1 % Tp, T - 1);
+    }
+};
+
 // ------------------------------------------------------------------ qa
 struct QaArgs {
     const void *q_nope, *q_rot;
@@ -40,7 +55,8 @@ struct QaArgs {
     const uint16_t *w_uk;                   // [H, nope, 512]
     char *qop;                              // [B][tiles] operand tiles
     int64_t q_seq;                          // bytes of a sequence's tiles
-    int H, nope, T, M, t0;                  // T queries from t0 on; M = B T
+    int H, nope, M, t0;                     // rows.T queries from t0 on; M = B T
+    Rows rows;
 };
 
 constexpr int kWLd = 272;                   // LDS bytes per staged weight row (128 columns + 16 bytes)
@@ -56,78 +72,115 @@ __device__ __forceinline__ void terms8(const float (&v)[8], u32x4 (&f)[3]) {
         f[x] = u32x4{hi16x2(t[x][0], t[x][1]), hi16x2(t[x][2], t[x][3]), hi16x2(t[x][4], t[x][5]), hi16x2(t[x][6], t[x][7])};
 }
 
-// grid (H, ceil(M / 16), 4): queries 16 y .. +16 of head x, latent columns 128 z .. +128
-template <typename QT, int NT, int RT>
+// 8 query values of a lane: slots 8 q4 .. +8 of a step of 32 hold n = 4 q4 + {0..3} and 16 + 4 q4 + {0..3}, the order in which
+// the transposed reads of the weights give theirs
+template <typename QT>
+struct QueryRaw {
+    typedef typename std::conditional<std::is_same<QT, float>::value, f32x4, u32x2>::type V;
+    V x[2];
+    __device__ __forceinline__ void load(const QT *q, int n, int nope, bool live) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[i] = live && n + 16 * i < nope ? *reinterpret_cast<const V *>(q + n + 16 * i) : V{};
+    }
+    __device__ __forceinline__ void terms(u32x4 (&f)[3]) const {
+        if constexpr (std::is_same<QT, float>::value) {
+            const float v[8] = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+            terms8(v, f);
+        } else {
+            f[0] = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
+        }
+    }
+};
+
+// grid (H, ceil(M / (16 MT)), 4): queries 16 MT y .. of head x, latent columns 128 z .. +128
+// MT 1: few queries, bound by the latency of reading W_UK once (every load in flight at once); MT 4: 64 queries to a
+// block's 32 KB of W_UK, bound by the terms' rounding (VALU) and by writing them.
+template <typename QT, int NT, int RT, int MT>
 __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    float *fs = reinterpret_cast<float *>(lds);                         // [16][kFLd], after the products
+    float *fs = reinterpret_cast<float *>(lds);                         // [16 MT][kFLd], after the products
+    constexpr int kTerms = std::is_same<QT, float>::value ? 3 : 1, kAhead = MT == 1 ? 4 : 0;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
-    const int h = blockIdx.x, m0 = blockIdx.y * 16, quarter = blockIdx.z;
-    const int steps = (a.nope + 31) >> 5;
+    const int h = blockIdx.x, m0 = blockIdx.y * 16 * MT, quarter = blockIdx.z;
+    const int steps = (a.nope + 31) >> 5, T = a.rows.T;
     const uint16_t *w = a.w_uk + static_cast<int64_t>(h) * a.nope * kQ4Lat + quarter * 128;
-    for (int i = tid; i < steps * 32 * 16; i += 256) {
-        const int n = i >> 4, c = i & 15;
-        const uint4 v = n < a.nope ? *reinterpret_cast<const uint4 *>(w + static_cast<int64_t>(n) * kQ4Lat + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4 *>(lds + n * kWLd + c * 16) = v;
+    const QT *q[MT];
+    bool live[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int m = m0 + 16 * i + r16;
+        live[i] = m < a.M;
+        const int b = live[i] ? m / T : 0, t = live[i] ? a.t0 + m % T : 0;
+        q[i] = static_cast<const QT *>(a.q_nope) + b * a.n_b + t * a.n_t + h * a.n_h + 4 * q4;
     }
-    // this lane's query values: slots 8 q4 .. +8 of a step hold n = 4 q4 + {0..3} and 16 + 4 q4 + {0..3}, as the
-    // transposed reads of the weights give them
-    const int m = m0 + r16;
-    const bool live = m < a.M;
-    const int b = live ? m / a.T : 0, t = live ? a.t0 + m % a.T : 0;
-    const QT *q = static_cast<const QT *>(a.q_nope) + b * a.n_b + t * a.n_t + h * a.n_h;
-    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        u32x4 qf[3];
-        constexpr int kTerms = std::is_same<QT, float>::value ? 3 : 1;
-        if constexpr (kTerms == 3) {
-            float v[8];
+    QueryRaw<QT> ahead[kAhead ? kAhead : 1];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int n = 32 * s + 16 * x + 4 * q4;
-                const float4 g = live && n < a.nope ? *reinterpret_cast<const float4 *>(q + n) : make_float4(0.f, 0.f, 0.f, 0.f);
-                v[4 * x] = g.x, v[4 * x + 1] = g.y, v[4 * x + 2] = g.z, v[4 * x + 3] = g.w;
-            }
-            terms8(v, qf);
-        } else {
-            uint2 g[2];
+    for (int s = 0; s < kAhead; ++s) ahead[s].load(q[0], 32 * s, a.nope - 4 * q4, live[0]);
+    for (int i0 = 0; i0 < 2 * steps; i0 += 8) {
+        uint4 v[8];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int n = 32 * s + 16 * x + 4 * q4;
-                g[x] = live && n < a.nope ? *reinterpret_cast<const uint2 *>(q + n) : make_uint2(0u, 0u);
-            }
-            qf[0] = u32x4{g[0].x, g[0].y, g[1].x, g[1].y};
+        for (int u = 0; u < 8; ++u) {
+            const int i = (i0 + u) * 256 + tid, n = i >> 4;
+            v[u] = n < a.nope ? *reinterpret_cast<const uint4 *>(w + static_cast<int64_t>(n) * kQ4Lat + (i & 15) * 8) : make_uint4(0u, 0u, 0u, 0u);
         }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = (i0 + u) * 256 + tid, n = i >> 4;
+            if (n < 32 * steps) *reinterpret_cast<uint4 *>(lds + n * kWLd + (i & 15) * 16) = v[u];
+        }
+    }
+    f32x4 acc[2][MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[0][i] = acc[1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+    auto step = [&](int s, const QueryRaw<QT> (&raw)[MT]) __attribute__((always_inline)) {
         const char *wr = lds + (32 * s + 4 * q4 + (r16 >> 2)) * kWLd + (r16 & 3) * 8 + wave * 64;
+        u32x4 wf[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + j * 32));
             const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + j * 32 + 16 * kWLd));
-            const u32x4 wf = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-            for (int k = kTerms - 1; k >= 0; --k) acc[j] = q4_mfma_bf16(wf, qf[k], acc[j]);
+            wf[j] = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            u32x4 qf[3];
+            raw[i].terms(qf);
+#pragma unroll
+            for (int k = kTerms - 1; k >= 0; --k)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[j][i] = q4_mfma_bf16(wf[j], qf[k], acc[j][i]);
+        }
+    };
+    if constexpr (MT == 1) {
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s)
+            if (s < steps) step(s, {ahead[s]});
+    }
+    for (int s = kAhead; s < steps; ++s) {
+        QueryRaw<QT> raw[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) raw[i].load(q[i], 32 * s, a.nope - 4 * q4, live[i]);
+        step(s, raw);
     }
     __syncthreads();   // the weights are read
 #pragma unroll
-    for (int j = 0; j < 2; ++j) *reinterpret_cast<f32x4 *>(fs + r16 * kFLd + wave * 32 + j * 16 + 4 * q4) = acc[j];
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) *reinterpret_cast<f32x4 *>(fs + (16 * i + r16) * kFLd + wave * 32 + j * 16 + 4 * q4) = acc[j][i];
     __syncthreads();
-    const int part = tid < 64 ? 0 : 1;
-    const int i = part == 0 ? tid >> 2 : (tid - 64) >> 3;       // query of the tile
-    if (m0 + i >= a.M || i >= 16) return;
-    const int mi = m0 + i, bi = mi / a.T, row = (mi % a.T) * a.H + h;
-    char *tile = a.qop + bi * a.q_seq + static_cast<int64_t>(row >> 4) * q4_tile_bytes(NT, RT);
-    if (part == 0) {
-        // one group of 32 columns: its terms
-        const int g = tid & 3, at = quarter * 16 + (row & 15);
+    if (tid < 64 * MT && m0 + (tid >> 2) < a.M) {
+        // one group of 32 columns of one query: its terms
+        const int i = tid >> 2, g = tid & 3, m = m0 + i, row = a.rows.of(m % T, h), at = quarter * 16 + (row & 15);
+        char *tile = a.qop + m / T * a.q_seq + static_cast<int64_t>(row >> 4) * q4_tile_bytes(NT, RT);
         const float *src = fs + i * kFLd + g * 32;
         float v[32];
         uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            v[j] = src[j];
-            top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+        for (int j = 0; j < 32; j += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(src + j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j + k] = x[k], top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
         }
         int byte = static_cast<int>(top >> 23) - 2 + ((top & 0x7fffffu) > 0x700000u ? 1 : 0);   // top / 2^(byte - 127) <= 7.5
         byte = min(max(byte, 1), 253);
@@ -151,18 +204,22 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
             reinterpret_cast<uint8_t *>(tile + q4_scale_at(NT, x))[at * 4 + g] = static_cast<uint8_t>(bad ? 255 : byte);
             byte = max(byte - (x == 0 ? 4 : 5), 1);
         }
-    } else if (quarter == 0) {
-        // rotary columns 8 c .. +8 of query i
-        const int c = (tid - 64) & 7, at = (c & 3) * 16 + (row & 15);
-        const QT *qr = static_cast<const QT *>(a.q_rot) + bi * a.r_b + (a.t0 + mi % a.T) * a.r_t + h * a.r_h + c * 8;
+    }
+    if (quarter != 0) return;
+    // rotary columns 8 c .. +8 of a query (one query tile: by the threads that had no group)
+    for (int j = MT == 1 ? tid - 64 : tid; j < 128 * MT; j += 256) {
+        const int i = j >> 3, m = m0 + i, c = j & 7;
+        if (j < 0 || m >= a.M) continue;
+        const int row = a.rows.of(m % T, h), at = (c & 3) * 16 + (row & 15);
+        char *tile = a.qop + m / T * a.q_seq + static_cast<int64_t>(row >> 4) * q4_tile_bytes(NT, RT);
+        const QT *qr = static_cast<const QT *>(a.q_rot) + m / T * a.r_b + (a.t0 + m % T) * a.r_t + h * a.r_h + c * 8;
         u32x4 f[3] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
         if constexpr (std::is_same<QT, float>::value) {
-            float v[8];
-            const float4 x = *reinterpret_cast<const float4 *>(qr), y = *reinterpret_cast<const float4 *>(qr + 4);
-            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(qr), y = *reinterpret_cast<const f32x4 *>(qr + 4);
+            const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
             terms8(v, f);
         } else {
-            const uint2 x = *reinterpret_cast<const uint2 *>(qr), y = *reinterpret_cast<const uint2 *>(qr + 4);
+            const u32x2 x = *reinterpret_cast<const u32x2 *>(qr), y = *reinterpret_cast<const u32x2 *>(qr + 4);
             f[0] = u32x4{x.x, x.y, y.x, y.y};
         }
 #pragma unroll
@@ -180,7 +237,8 @@ struct AttendArgs {
     int length, cap, count;                     // where those are null
     float *part;                                // [B][NS][rows][512]
     float2 *ml;                                 // [B][NS][rows]
-    int H, T, t0, rows, Ts, NS, rblocks, B;
+    Rows order;
+    int t0, rows, Ts, NS, rblocks, B;           // rows: order.count()
     float c;                                    // scale * log2(e)
     int swizzle;
 };
@@ -192,6 +250,8 @@ constexpr int kVLd = 1056;                      // .. of a value row: 1024 + 32
 constexpr int kKBytes = kRound * kKLd, kRBytes = kRound * kRLd, kVBytes = kRound * kVLd;
 
 constexpr int kKSlots = 3;
+constexpr int kCLd = 132;                       // floats of a context row on its way out: 128 + 4
+static_assert(4 * 16 * kCLd * 4 <= 2 * kVBytes, "the contexts' way out fits the value tiles");
 
 constexpr int attend_lds(int RG, int RT, int PT) {   // PT fp16 terms of the probabilities (bf16: one more)
     return kKSlots * kKBytes + 2 * kRBytes + 2 * kVBytes + 2 * RG * (PT + 1) * 1024 + RG * RT * 2048;
@@ -214,13 +274,16 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     const int r16 = lane & 15, q4 = lane >> 4;
     const int nb = gridDim.x;
     const int w = a.swizzle ? (blockIdx.x & 7) * (nb >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-    const int rb = w % a.rblocks, split = (w / a.rblocks) % a.NS, b = w / (a.rblocks * a.NS);
+    int rb = w % a.rblocks;
+    const int split = (w / a.rblocks) % a.NS, b = w / (a.rblocks * a.NS);
+    // whole blocks of one head: the last queries, which see most, first
+    if (a.order.Tp && a.order.Tp % (16 * RG) == 0) rb = rb % a.order.H * (a.order.Tp / (16 * RG)) + (a.order.Tp / (16 * RG) - 1 - rb / a.order.H);
     const int row0 = rb * 16 * RG;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.cap) : a.length;
     const int cnt = a.counts ? min(max(a.counts[b], 0), a.count) : a.count;
     // the last query of the block that is there sees most
-    const int tlast = min(a.t0 + (min(row0 + 16 * RG, a.rows) - 1) / a.H, cnt - 1);
-    const int most = tlast >= a.t0 + row0 / a.H ? q4_sees(tlast, cnt, len) : 0;
+    const int tlast = min(a.t0 + a.order.last_query(row0, min(row0 + 16 * RG, a.rows) - 1), cnt - 1);
+    const int most = tlast >= a.t0 ? q4_sees(tlast, cnt, len) : 0;
     const int t_begin = split * a.Ts, t_end = min(most, t_begin + a.Ts);
     float2 *ml = a.ml + (static_cast<int64_t>(b) * a.NS + split) * a.rows;
     if (t_end <= t_begin) {
@@ -316,7 +379,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int x = 0; x < 2 * RT; ++x) *reinterpret_cast<u32x4 *>(qr + x * 1024) = *reinterpret_cast<const u32x4 *>(tile + q4_rope_at(NT, 0, x) + lane * 16);
         const int row = row0 + rg * 16 + r16;
-        const int sees = row < a.rows ? q4_sees(a.t0 + row / a.H, cnt, len) : 0;
+        const int tq = a.order.query(row), sees = row < a.rows && tq < a.order.T ? q4_sees(a.t0 + tq, cnt, len) : 0;
         const int limit = min(sees, t_end) - t_begin;       // positions of this split that the row sees
         float m_ref, l_run, mt[2];
         f32x4 sc[2][NTILE];                                 // scores of round i (parity)
@@ -525,13 +588,20 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         all(std::false_type{});
         if (__builtin_amdgcn_readfirstlane(wide)) all(std::true_type{});
         __syncthreads();
-        float *part = a.part + ((static_cast<int64_t>(b) * a.NS + split) * a.rows + row0) * kQ4Lat + col0 + 4 * q4;
+        // the records through LDS (the value tiles are done with), so that a store writes 512 contiguous bytes of two rows: as the
+        // accumulators lie, 64 bytes of sixteen rows, the 256 blocks of a short split took 7 us to write them
+        float *part = a.part + ((static_cast<int64_t>(b) * a.NS + split) * a.rows + row0) * kQ4Lat + col0;
+        float *const x = reinterpret_cast<float *>(vbuf) + (wave - 4) * 16 * kCLd;
 #pragma unroll
         for (int r = 0; r < RG; ++r) {
-            if (row0 + r * 16 + r16 >= a.rows) continue;
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<f32x4 *>(part + static_cast<int64_t>(r * 16 + r16) * kQ4Lat + c * 16) = acc[c][r];
+            for (int c = 0; c < 8; ++c) *reinterpret_cast<f32x4 *>(x + r16 * kCLd + c * 16 + 4 * q4) = acc[c][r];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int j = 2 * i + (lane >> 5);
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(x + j * kCLd + (lane & 31) * 4);
+                if (row0 + r * 16 + j < a.rows) *reinterpret_cast<f32x4 *>(part + static_cast<int64_t>(r * 16 + j) * kQ4Lat + (lane & 31) * 4) = v;
+            }
         }
     }
 }
@@ -541,148 +611,227 @@ struct UvArgs {
     const float *part;
     const float2 *ml;
     const uint16_t *w_uv;    // [H, V, 512]
-    float *opart;            // [4][M][H][V], or null: out
     void *out;               // [B, Tall, H, V]
     int out_bf16;
     const float *gate;       // [B, Tall, H, V] or null
     float2 *stats;           // [B][rows]: maximum less kLift, 1 / sum (which is lifted); or null
-    int H, T, M, V, rows, NS, Tall, t0;
+    Rows order;
+    int M, V, rows, NS, Tall, t0;
 };
 constexpr int kMaxSplits = 256;
 
-__device__ __forceinline__ void store_out4(void *out, int bf16, const float *gate, int64_t at, f32x4 v) {
-    if (gate) {
-        const f32x4 g = *reinterpret_cast<const f32x4 *>(gate + at);
+__device__ __forceinline__ void store_out4(const UvArgs &a, int m, int h, int v, f32x4 o) {
+    const int64_t at = ((static_cast<int64_t>(m / a.order.T) * a.Tall + a.t0 + m % a.order.T) * a.order.H + h) * a.V + v;
+    if (a.gate) {
+        const f32x4 g = *reinterpret_cast<const f32x4 *>(a.gate + at);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = v[i] / (1.0f + expf(-g[i]));
+        for (int i = 0; i < 4; ++i) o[i] = o[i] / (1.0f + expf(-g[i]));
     }
-    if (bf16)
-        *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(out) + at) = u32x2{q4_pack_bf16(v[0], v[1]), q4_pack_bf16(v[2], v[3])};
+    if (a.out_bf16)
+        *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + at) = u32x2{q4_pack_bf16(o[0], o[1]), q4_pack_bf16(o[2], o[3])};
     else
-        *reinterpret_cast<f32x4 *>(static_cast<float *>(out) + at) = v;
+        *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + at) = o;
 }
 
-// grid (H, ceil(M / 16), 512 / CP): queries 16 y .. +16 of head x over the latent columns CP z .. +CP
-//   join    ctx = sum_s 2^(m_s - M) ctx_s / L, the splits in a fixed order (few queries: eight groups of splits, added
-//           in group order)
-//   W_UV    fp32 contexts as three bf16 terms
-template <int CP>
-__global__ __launch_bounds__(256) void uv_kernel(UvArgs a) {
-    constexpr int kLd = CP + 4;
+// The weights of a row's records, 2^(m_s - M) / L with M = max m_s, L = sum 2^(m_s - M) l_s, by a wave; a split the row sees
+// nothing of has no record (its sum is exactly 0), and its weight is zero whatever the others are.
+__device__ __forceinline__ void record_weights(const UvArgs &a, int b, int row, float *wsp) {
+    const int lane = threadIdx.x & 63;
+    const float2 *ml = a.ml + static_cast<int64_t>(b) * a.NS * a.rows + row;
+    float2 v[kMaxSplits / 64];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kMaxSplits / 64; ++u) {
+        const int s = lane + 64 * u;
+        v[u] = s < a.NS ? ml[static_cast<int64_t>(s) * a.rows] : make_float2(-INFINITY, 0.f);
+        mx = fmaxf(mx, v[u].x);
+    }
+    mx = wave_max_all(mx);
+    float l = 0.f, e[kMaxSplits / 64];
+#pragma unroll
+    for (int u = 0; u < kMaxSplits / 64; ++u) {
+        e[u] = v[u].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v[u].x - mx);
+        l = fmaf(e[u], v[u].y, l);
+    }
+    l = wave_sum_all(l);
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int u = 0; u < kMaxSplits / 64; ++u) {
+        const int s = lane + 64 * u;
+        if (s < a.NS) wsp[s] = v[u].y == 0.f ? 0.f : e[u] * inv;
+    }
+    if (a.stats && lane == 0) a.stats[static_cast<int64_t>(b) * a.rows + row] = make_float2(mx - kLift, inv);
+}
+
+// Few queries: grid (H, ceil(M / 16)), eight waves, queries 16 y .. +16 of head x.  A wave joins the records of its 64 latent columns
+// (16 lanes x 4 columns, four splits at a time) and multiplies them with its columns of W_UV (loaded first of all); the
+// waves' products are added in order.  Bound by the latency of the records (NS x 2 KB a query) and of W_UV, 128 KB a head.
+// One launch: blocks of 128 columns each and a launch that added their products took 14 us at 64 heads and 128 ranges, this takes 16 (and 9 for 12.5 with one range).
+constexpr int kXLd = 68, kDLd = 132;        // floats of a staged context row (64 columns), of a product row (128)
+constexpr int few_lds(int NS) { return (8 * 16 * kXLd + 8 * 16 * kDLd + 16 * NS) * 4; }
+
+__global__ __launch_bounds__(512, 1) void uv_few_kernel(UvArgs a) {
     extern __shared__ __attribute__((aligned(16))) float sm[];
-    float *const ctx = sm, *const wsp = sm + 16 * kLd, *const red = wsp + 16 * a.NS;   // red: 8 x CP, few queries
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
-    const int h = blockIdx.x, m0 = blockIdx.y * 16, col0 = blockIdx.z * CP;
-    const int nv = min(16, a.M - m0);
-    for (int i = wave; i < nv; i += 4) {
-        const int m = m0 + i, b = m / a.T, row = (m % a.T) * a.H + h;
-        const float2 *ml = a.ml + static_cast<int64_t>(b) * a.NS * a.rows + row;
-        float2 v[kMaxSplits / 64];
-        float mx = -INFINITY;
+    float *const x = sm + wave * 16 * kXLd, *const d = sm + 8 * 16 * kXLd, *const wsp = d + 8 * 16 * kDLd;
+    const int h = blockIdx.x, m0 = blockIdx.y * 16, col0 = wave * 64, nv = min(16, a.M - m0);
+    auto weights_of = [&](int v0, u32x4 (&w)[8][2]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kMaxSplits / 64; ++u) {
-            const int s = lane + 64 * u;
-            v[u] = s < a.NS ? ml[static_cast<int64_t>(s) * a.rows] : make_float2(-INFINITY, 0.f);
-            mx = fmaxf(mx, v[u].x);
-        }
-        mx = wave_max_all(mx);
-        float l = 0.f, e[kMaxSplits / 64];
+        for (int t = 0; t < 8; ++t) {
+            const int v = v0 + t * 16 + r16;
+            const uint16_t *wr = a.w_uv + (static_cast<int64_t>(h) * a.V + v) * kQ4Lat + col0 + 8 * q4;
 #pragma unroll
-        for (int u = 0; u < kMaxSplits / 64; ++u) {
-            // (a split the row sees nothing of has no record: its weight is zero, whatever the maximum is)
-            e[u] = v[u].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v[u].x - mx);
-            l = fmaf(e[u], v[u].y == 0.f ? 0.f : v[u].y, l);
+            for (int k = 0; k < 2; ++k) w[t][k] = v < a.V ? *reinterpret_cast<const u32x4 *>(wr + k * 32) : u32x4{0u, 0u, 0u, 0u};
         }
-        l = wave_sum_all(l);
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
+    };
+    u32x4 w[8][2];
+    weights_of(0, w);
+    constexpr int kBatch = 8;
+    auto record = [&](int i) __attribute__((always_inline)) {
+        const int m = m0 + i, b = m / a.order.T, row = a.order.of(m % a.order.T, h);
+        return a.part + (static_cast<int64_t>(b) * a.NS * a.rows + row) * kQ4Lat + col0 + 4 * r16;
+    };
+    const int64_t pitch = static_cast<int64_t>(a.rows) * kQ4Lat;
+    f32x4 first[kBatch];                    // the first query's first records: in bounds, whether there is one or not
 #pragma unroll
-        for (int u = 0; u < kMaxSplits / 64; ++u) {
-            const int s = lane + 64 * u;
-            if (s < a.NS) wsp[i * a.NS + s] = v[u].y == 0.f ? 0.f : e[u] * inv;
-        }
-        if (a.stats && blockIdx.z == 0 && lane == 0) a.stats[static_cast<int64_t>(b) * a.rows + row] = make_float2(mx - kLift, inv);
+    for (int u = 0; u < kBatch; ++u) first[u] = *reinterpret_cast<const f32x4 *>(record(0) + min(q4 + 4 * u, a.NS - 1) * pitch);
+    for (int i = wave; i < nv; i += 8) {
+        const int m = m0 + i;
+        record_weights(a, m / a.order.T, a.order.of(m % a.order.T, h), wsp + i * a.NS);
     }
     __syncthreads();
-    constexpr int kC4 = CP / 4, kG = 256 / kC4;     // threads across the columns; groups of threads
-    const int c4 = tid % kC4, gr = tid / kC4;
-    int np = 1;                                     // groups that take different queries
-    while (np < nv && np < kG) np *= 2;
-    const int sg = gr / np, ns = kG / np;
-    for (int i0 = 0; i0 < nv; i0 += np) {
-        const int i = i0 + gr % np;
+    for (int i = 0; i < nv; ++i) {
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
-        if (i < nv) {
-            const int m = m0 + i, b = m / a.T, row = (m % a.T) * a.H + h;
-            const float *src = a.part + (static_cast<int64_t>(b) * a.NS * a.rows + row) * kQ4Lat + col0 + 4 * c4;
-            for (int j = sg; j < a.NS; j += 4 * ns) {
-                f32x4 x[4];
-                float wgt[4];
+        const float *src = record(i), *ws = wsp + i * a.NS;
+        for (int j = q4; j < a.NS; j += 4 * kBatch) {
+            f32x4 y[kBatch];
+            float f[kBatch];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int k = j + u * ns;
-                    wgt[u] = k < a.NS ? wsp[i * a.NS + k] : 0.f;
-                    x[u] = wgt[u] != 0.f ? *reinterpret_cast<const f32x4 *>(src + static_cast<int64_t>(k) * a.rows * kQ4Lat)
-                                         : f32x4{0.f, 0.f, 0.f, 0.f};
-                }
+            for (int u = 0; u < kBatch; ++u) {
+                const int k = j + 4 * u;
+                f[u] = k < a.NS ? ws[k] : 0.f;
+                if (i == 0 && j < 4)
+                    y[u] = first[u];
+                else if (f[u] != 0.f)
+                    y[u] = *reinterpret_cast<const f32x4 *>(src + k * pitch);
+                if (f[u] == 0.f) y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) s += x[u] * wgt[u];
-            }
+            for (int u = 0; u < kBatch; ++u) s += y[u] * f[u];
         }
-        if (ns == 1) {
-            if (i < nv) *reinterpret_cast<f32x4 *>(ctx + i * kLd + 4 * c4) = s;
-        } else {
-            *reinterpret_cast<f32x4 *>(red + gr * CP + 4 * c4) = s;
-            __syncthreads();
-            if (gr < np && i0 + gr < nv) {
-                f32x4 t = *reinterpret_cast<const f32x4 *>(red + gr * CP + 4 * c4);
-                for (int k = 1; k < ns; ++k) t += *reinterpret_cast<const f32x4 *>(red + (k * np + gr) * CP + 4 * c4);
-                *reinterpret_cast<f32x4 *>(ctx + (i0 + gr) * kLd + 4 * c4) = t;
-            }
-            __syncthreads();
-        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] = q4_rows_sum(s[k]);
+        if (q4 == 0) *reinterpret_cast<f32x4 *>(x + i * kXLd + 4 * r16) = s;
     }
-    for (int i = tid; i < (16 - nv) * CP; i += 256) ctx[(nv + i / CP) * kLd + i % CP] = 0.f;   // queries past the last
-    __syncthreads();
-    u32x4 cf[CP / 32][3];
+    for (int i = nv + q4; i < 16; i += 4) *reinterpret_cast<f32x4 *>(x + i * kXLd + 4 * r16) = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 cf[2][3];                         // (a wave's own rows: its LDS accesses are in order)
 #pragma unroll
-    for (int k = 0; k < CP / 32; ++k) {
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(ctx + r16 * kLd + k * 32 + 8 * q4);
-        const f32x4 y = *reinterpret_cast<const f32x4 *>(ctx + r16 * kLd + k * 32 + 8 * q4 + 4);
-        const float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    for (int k = 0; k < 2; ++k) {
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(x + r16 * kXLd + k * 32 + 8 * q4);
+        const f32x4 z = *reinterpret_cast<const f32x4 *>(x + r16 * kXLd + k * 32 + 8 * q4 + 4);
+        const float v[8] = {y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]};
         terms8(v, cf[k]);
     }
-    const int m = m0 + r16;
-    const int64_t at = m < a.M ? ((static_cast<int64_t>(m / a.T) * a.Tall + a.t0 + m % a.T) * a.H + h) * a.V : 0;
-    for (int vt = wave; vt * 16 < a.V; vt += 4) {
-        const int v = vt * 16 + r16;
-        const uint16_t *wr = a.w_uv + (static_cast<int64_t>(h) * a.V + v) * kQ4Lat + col0 + 8 * q4;
-        f32x4 d = {0.f, 0.f, 0.f, 0.f}, dl = d;
-#pragma unroll
-        for (int k = 0; k < CP / 32; ++k) {
-            const u32x4 wf = v < a.V ? *reinterpret_cast<const u32x4 *>(wr + k * 32) : u32x4{0u, 0u, 0u, 0u};
-            dl = q4_mfma_bf16(wf, cf[k][2], dl);
-            dl = q4_mfma_bf16(wf, cf[k][1], dl);
-            d = q4_mfma_bf16(wf, cf[k][0], d);
+    for (int v0 = 0; v0 < a.V; v0 += 128) {
+        if (v0) {
+            weights_of(v0, w);
+            __syncthreads();                // the last products are added up
         }
-        d += dl;
-        if (m >= a.M || vt * 16 + 4 * q4 >= a.V) continue;
-        if (a.opart)
-            *reinterpret_cast<f32x4 *>(a.opart + ((static_cast<int64_t>(blockIdx.z) * a.M + m) * a.H + h) * a.V + vt * 16 + 4 * q4) = d;
-        else
-            store_out4(a.out, a.out_bf16, a.gate, at + vt * 16 + 4 * q4, d);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int y = 2; y >= 0; --y)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) o = q4_mfma_bf16(w[t][k], cf[k][y], o);
+            *reinterpret_cast<f32x4 *>(d + (wave * 16 + r16) * kDLd + t * 16 + 4 * q4) = o;
+        }
+        __syncthreads();
+        const int i = tid >> 5, v = (tid & 31) * 4;
+        if (i < nv && v0 + v < a.V) {
+            f32x4 o = *reinterpret_cast<const f32x4 *>(d + i * kDLd + v);
+#pragma unroll
+            for (int u = 1; u < 8; ++u) o += *reinterpret_cast<const f32x4 *>(d + (u * 16 + i) * kDLd + v);
+            store_out4(a, m0 + i, h, v0 + v, o);
+        }
     }
 }
 
-// o = the four column quarters' products in order (then the output gate); four values a thread
-__global__ __launch_bounds__(256) void out_kernel(UvArgs a) {
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
-    const int64_t hv = static_cast<int64_t>(a.H) * a.V, n = a.M * hv;
-    if (i >= n) return;
-    f32x4 o = *reinterpret_cast<const f32x4 *>(a.opart + i);
+// Many queries: grid (H, ceil(M / 64)), four waves, queries 64 y .. +64 of head x, 128 latent columns at a time: a thread joins
+// the records of 4 columns of 8 queries and leaves them in LDS as TERMS bf16 terms (two, 2^-17, for a bf16 result); a wave
+// takes 32 of 128 output columns for all 64 queries.  Bound by reading the records.
+template <int TERMS>
+__global__ __launch_bounds__(256) void uv_many_kernel(UvArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int kLd = 272, kTerm = 64 * kLd;      // bytes: 128 columns + 16
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
+    float *const wsp = reinterpret_cast<float *>(lds + TERMS * kTerm);
+    const int h = blockIdx.x, m0 = blockIdx.y * 64, nv = min(64, a.M - m0);
+    for (int i = wave; i < nv; i += 4) {
+        const int m = m0 + i;
+        record_weights(a, m / a.order.T, a.order.of(m % a.order.T, h), wsp + i * a.NS);
+    }
+    __syncthreads();
+    const int64_t pitch = static_cast<int64_t>(a.rows) * kQ4Lat;
+    const int c4 = tid & 31, i8 = tid >> 5;
+    for (int v0 = 0; v0 < a.V; v0 += 128) {
+        f32x4 acc[2][4];
 #pragma unroll
-    for (int q = 1; q < 4; ++q) o += *reinterpret_cast<const f32x4 *>(a.opart + q * n + i);
-    const int64_t m = i / hv;
-    store_out4(a.out, a.out_bf16, a.gate, ((m / a.T) * a.Tall + a.t0 + m % a.T) * hv + i % hv, o);
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int col0 = 0; col0 < kQ4Lat; col0 += 128) {
+            u32x4 w[2][4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int v = v0 + (2 * wave + t) * 16 + r16;
+                const uint16_t *wr = a.w_uv + (static_cast<int64_t>(h) * a.V + v) * kQ4Lat + col0 + 8 * q4;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[t][k] = v < a.V ? *reinterpret_cast<const u32x4 *>(wr + k * 32) : u32x4{0u, 0u, 0u, 0u};
+            }
+            f32x4 s[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < a.NS; ++k) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int i = 8 * u + i8, m = m0 + i;
+                    const float f = i < nv ? wsp[i * a.NS + k] : 0.f;
+                    if (f != 0.f)
+                        s[u] += f * *reinterpret_cast<const f32x4 *>(a.part + (static_cast<int64_t>(m / a.order.T) * a.NS + k) * pitch +
+                                                                    static_cast<int64_t>(a.order.of(m % a.order.T, h)) * kQ4Lat + col0 + 4 * c4);
+                }
+            }
+            __syncthreads();    // the last columns' operands are read
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int y = 0; y < TERMS; ++y) {
+                    const u32x2 p = {q4_pack_bf16(s[u][0], s[u][1]), q4_pack_bf16(s[u][2], s[u][3])};
+                    *reinterpret_cast<u32x2 *>(lds + y * kTerm + (8 * u + i8) * kLd + c4 * 8) = p;
+                    s[u] -= f32x4{q4_lo(p.x), q4_hi(p.x), q4_lo(p.y), q4_hi(p.y)};
+                }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int y = TERMS - 1; y >= 0; --y)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const u32x4 c = *reinterpret_cast<const u32x4 *>(lds + y * kTerm + (16 * r + r16) * kLd + k * 64 + q4 * 16);
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) acc[t][r] = q4_mfma_bf16(w[t][k], c, acc[t][r]);
+                    }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int i = 16 * r + r16, v = v0 + (2 * wave + t) * 16 + 4 * q4;
+                if (i < nv && v < a.V) store_out4(a, m0 + i, h, v, acc[t][r]);
+            }
+    }
 }
 
 // ------------------------------------------------------------------ weights
@@ -696,27 +845,52 @@ struct WeightArgs {
 };
 constexpr int kWTiles = 4;   // tiles of 16 positions per wave
 
-// grid (ceil(npos / 512), chunks, B): a wave keeps 64 positions' codes in registers and takes the row tiles
-// chunk y .. of its sequence, adding their probabilities; part[chunk][b][position]
+// grid (ceil(npos / 512), chunks, B): a wave keeps 64 positions' codes in registers; the block takes the row tiles
+// chunk y .. of its sequence one after the other, each staged in LDS for its eight waves while the last one is worked on, and adds
+// their probabilities; part[chunk][b][position].  Bound by the matrix cores and, with few rows, by the first loads.
 template <int NT, int RT>
 __global__ __launch_bounds__(512, 1) void weights_kernel(WeightArgs wa) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int kBytes = q4_tile_bytes(NT, RT), kLoads = (kBytes + 8191) / 8192;
     const AttendArgs &a = wa.a;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, q4 = lane >> 4;
-    const int b = blockIdx.z, j0 = (blockIdx.x * 8 + wave) * (16 * kWTiles);
-    if (j0 >= wa.npos) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
+    const int b = blockIdx.z, jb = blockIdx.x * (8 * 16 * kWTiles), j0 = jb + wave * (16 * kWTiles);
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.cap) : a.length;
     const int cnt = a.counts ? min(max(a.counts[b], 0), a.count) : a.count;
-    const int n = len - j0;                        // positions there are from j0 on
+    const int n = min(len - j0, 16 * kWTiles);     // positions there are from j0 on
     f32x4 sum[kWTiles];
 #pragma unroll
     for (int u = 0; u < kWTiles; ++u) sum[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int first = blockIdx.y * wa.chunk, last = min(wa.tiles, first + wa.chunk);
+    const int last = min(wa.tiles, (static_cast<int>(blockIdx.y) + 1) * wa.chunk);
+    // positions that the rows of tile i see
+    auto seen = [&](int i) __attribute__((always_inline)) {
+        const int t = min(a.t0 + a.order.last_query(16 * i, min(16 * i + 16, a.rows) - 1), cnt - 1);
+        return t >= a.t0 ? q4_sees(t, cnt, len) : 0;
+    };
+    auto next = [&](int i) __attribute__((always_inline)) {   // the first tile from i on that sees any of the block's positions
+        while (i < last && seen(i) <= jb) ++i;
+        return i;
+    };
+    u32x4 stage[kLoads];
+    auto load = [&](int i) __attribute__((always_inline)) {
+        const char *tile = a.qop + b * a.q_seq + static_cast<int64_t>(min(i, wa.tiles - 1)) * kBytes;
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+            stage[u] = *reinterpret_cast<const u32x4 *>(tile + min(u * 8192 + tid * 16, kBytes - 16));
+    };
+    auto store = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+            if (u * 8192 + tid * 16 < kBytes) *reinterpret_cast<u32x4 *>(lds + buf * kBytes + u * 8192 + tid * 16) = stage[u];
+    };
+    int i = next(blockIdx.y * wa.chunk);
+    load(i);
+    u32x4 kc[kWTiles][kQ4Steps], ro[kWTiles][2];
+    int ks[kWTiles];
     if (n > 0) {
-        const auto rp = make_rsrc(a.packed + b * a.p_b + j0 * a.p_t, static_cast<uint32_t>(min(n - 1, 16 * kWTiles - 1) * a.p_t + 256));
-        const auto rs = make_rsrc(a.scales + b * a.s_b + j0 * a.s_t, static_cast<uint32_t>(min(n - 1, 16 * kWTiles - 1) * a.s_t + 16));
-        const auto rr = make_rsrc(a.rot + b * a.r_b + j0 * a.r_t, static_cast<uint32_t>(min(n - 1, 16 * kWTiles - 1) * a.r_t + 128));
-        u32x4 kc[kWTiles][kQ4Steps], ro[kWTiles][2];
-        int ks[kWTiles];
+        const auto rp = make_rsrc(a.packed + b * a.p_b + j0 * a.p_t, static_cast<uint32_t>((n - 1) * a.p_t + 256));
+        const auto rs = make_rsrc(a.scales + b * a.s_b + j0 * a.s_t, static_cast<uint32_t>((n - 1) * a.s_t + 16));
+        const auto rr = make_rsrc(a.rot + b * a.r_b + j0 * a.r_t, static_cast<uint32_t>((n - 1) * a.r_t + 128));
 #pragma unroll
         for (int u = 0; u < kWTiles; ++u) {
             const int j = u * 16 + r16;
@@ -734,13 +908,27 @@ __global__ __launch_bounds__(512, 1) void weights_kernel(WeightArgs wa) {
                           rs, ok ? static_cast<uint32_t>(j) * static_cast<uint32_t>(a.s_t) + q4 * 4u + s : kOobOffset, 0, 0)) << (8 * s);
             ks[u] = static_cast<int>(k4);
         }
-        for (int i = first; i < last; ++i) {
-            const int tlast = min(a.t0 + (min(i * 16 + 16, a.rows) - 1) / a.H, cnt - 1);
-            if (q4_sees(tlast, cnt, len) <= j0) continue;    // (tlast < t0: no query of the tile is there, and its rows see nothing)
-            const int row = i * 16 + r16;
-            const int limit = (row < a.rows ? q4_sees(a.t0 + row / a.H, cnt, len) : 0) - j0;
-            const float2 st = row < a.rows ? wa.stats[static_cast<int64_t>(b) * a.rows + row] : make_float2(0.f, 0.f);
-            const char *tile = a.qop + b * a.q_seq + static_cast<int64_t>(i) * q4_tile_bytes(NT, RT);
+    } else {
+#pragma unroll
+        for (int u = 0; u < kWTiles; ++u) {
+            ks[u] = 0;
+#pragma unroll
+            for (int s = 0; s < kQ4Steps; ++s) kc[u][s] = u32x4{0u, 0u, 0u, 0u};
+            ro[u][0] = ro[u][1] = u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    int buf = 0;
+    store(0);
+    __syncthreads();
+    while (i < last) {
+        const int following = next(i + 1);
+        if (following < last) load(following);
+        const char *tile = lds + buf * kBytes + lane * 16;
+        if (n > 0 && seen(i) > j0) {
+            const int row = i * 16 + r16, tq = a.order.query(row);
+            const bool there = row < a.rows && tq < a.order.T;
+            const int limit = (there ? q4_sees(a.t0 + tq, cnt, len) : 0) - j0;
+            const float2 st = there ? wa.stats[static_cast<int64_t>(b) * a.rows + row] : make_float2(0.f, 0.f);
             f32x4 hi[kWTiles], lo[kWTiles];
 #pragma unroll
             for (int u = 0; u < kWTiles; ++u) hi[u] = lo[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -748,19 +936,19 @@ __global__ __launch_bounds__(512, 1) void weights_kernel(WeightArgs wa) {
             for (int x = RT - 1; x >= 0; --x)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const u32x4 qr = *reinterpret_cast<const u32x4 *>(tile + q4_rope_at(NT, x, s) + lane * 16);
+                    const u32x4 qr = *reinterpret_cast<const u32x4 *>(tile + q4_rope_at(NT, x, s));
 #pragma unroll
                     for (int u = 0; u < kWTiles; ++u) lo[u] = q4_mfma_bf16(ro[u][s], qr, lo[u]);
                 }
 #pragma unroll
             for (int x = NT - 1; x >= 0; --x) {
-                const int qs = *reinterpret_cast<const int *>(tile + q4_scale_at(NT, x) + lane * 4);
+                const int qs = *reinterpret_cast<const int *>(tile + q4_scale_at(NT, x) - lane * 12);
                 u32x4 qlo[kQ4Steps];
                 u32x2 qhi[kQ4Steps];
 #pragma unroll
                 for (int s = 0; s < kQ4Steps; ++s) {
-                    qlo[s] = *reinterpret_cast<const u32x4 *>(tile + q4_code_at(x, s) + lane * 16);
-                    qhi[s] = *reinterpret_cast<const u32x2 *>(tile + q4_code_at(x, s) + 1024 + lane * 8);
+                    qlo[s] = *reinterpret_cast<const u32x4 *>(tile + q4_code_at(x, s));
+                    qhi[s] = *reinterpret_cast<const u32x2 *>(tile + q4_code_at(x, s) + 1024 - lane * 8);
                 }
 #pragma unroll
                 for (int u = 0; u < kWTiles; ++u) {
@@ -779,8 +967,12 @@ __global__ __launch_bounds__(512, 1) void weights_kernel(WeightArgs wa) {
                     sum[u][v] += u * 16 + 4 * q4 + v < limit ? p : 0.f;
                 }
         }
+        if (following < last) store(buf ^ 1);
+        __syncthreads();
+        buf ^= 1, i = following;
     }
     // over the 16 rows of the tiles (lanes of a DPP row), in a fixed order
+    if (j0 >= wa.npos) return;
     float *out = wa.part + (static_cast<int64_t>(blockIdx.y) * a.B + b) * wa.npos + j0;
 #pragma unroll
     for (int u = 0; u < kWTiles; ++u)
@@ -794,34 +986,47 @@ __global__ __launch_bounds__(512, 1) void weights_kernel(WeightArgs wa) {
         }
 }
 
-// weight[b][j] += the chunks' sums in order
+// weight[b][j] += the chunks' sums: four threads a position, each every fourth chunk, added in order
 __global__ __launch_bounds__(256) void weights_add_kernel(WeightArgs wa) {
-    const int j = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
-    if (j >= wa.npos) return;
+    __shared__ float part[4][64];
+    const int c = threadIdx.x & 63, g = threadIdx.x >> 6, j = blockIdx.x * 64 + c, b = blockIdx.y;
     const int len = wa.a.lengths ? min(max(wa.a.lengths[b], 0), wa.a.cap) : wa.a.length;
-    if (j >= len) return;
+    const float *src = wa.part + static_cast<int64_t>(b) * wa.npos + j;
+    const int64_t pitch = static_cast<int64_t>(wa.a.B) * wa.npos;
     float s = 0.f;
-    for (int k = 0; k < wa.chunks; ++k) s += wa.part[(static_cast<int64_t>(k) * wa.a.B + b) * wa.npos + j];
-    wa.weight[b * wa.w_b + j] += s;
+    if (j < len) {
+#pragma unroll 8
+        for (int k = g; k < wa.chunks; k += 4) s += src[k * pitch];
+    }
+    part[g][c] = s;
+    __syncthreads();
+    if (g == 0 && j < len) wa.weight[b * wa.w_b + j] += (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
 }
 
 // ------------------------------------------------------------------ host side
 struct Plan {
-    int NT, RT, PT, RG, T, rows, tiles, rblocks, Ts, NS, uv_quarters, chunk, chunks;
-    int64_t qop, ml, part, stats, opart, wpart, total;
+    int NT, RT, PT, RG, tiles, rblocks, Ts, NS, many, chunk, chunks;
+    Rows order;
+    int64_t qop, ml, part, stats, wpart, total;
 };
 
 constexpr int64_t kChunkRows = 1 << 16;   // rows (heads x queries, all sequences) of one pass over the queries
+constexpr int kByHead = 32;               // queries of a sequence from which rows go by head
+constexpr int kManyQueries = 48;          // queries (all sequences) from which uv_many takes less than uv_few
+
+Rows rows_of(int64_t T, int64_t H) {
+    return Rows{static_cast<int>(T), static_cast<int>(H), T >= kByHead ? static_cast<int>(cdiv(T, 16) * 16) : 0};
+}
 
 // What the launches are cut into; a function of its arguments alone.
 Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf16, int out_bf16, int weights, int varied) {
     Plan p{};
     const bool fine = !out_bf16 || weights;
     p.NT = fine ? 5 : 3, p.RT = q_bf16 ? 1 : fine ? 3 : 2, p.PT = out_bf16 ? 1 : 2;
-    p.T = static_cast<int>(std::max<int64_t>(1, std::min(T, kChunkRows / (B * H))));
-    p.rows = static_cast<int>(p.T * H);
-    p.RG = p.rows > 64 ? 4 : 2;
-    p.rblocks = static_cast<int>(cdiv(p.rows, 16 * p.RG));
+    p.order = rows_of(std::max<int64_t>(1, std::min(T, kChunkRows / (B * H))), H);
+    const int64_t rows = p.order.count();
+    p.RG = rows > 64 ? 4 : 2;
+    p.rblocks = static_cast<int>(cdiv(rows, 16 * p.RG));
     p.tiles = p.rblocks * p.RG;
     const int64_t base = B * p.rblocks;
     // one block a CU; sequences of their own lengths: four, so the longest one's blocks are not what all wait for
@@ -829,8 +1034,7 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
     int64_t ts = cdiv(cdiv(std::max<int64_t>(npos, 1), ns), kRound) * kRound;
     p.Ts = static_cast<int>(ts);
     p.NS = static_cast<int>(cdiv(std::max<int64_t>(npos, 1), ts));
-    const int64_t M = B * p.T;
-    p.uv_quarters = H * cdiv(M, 16) < 512;
+    p.many = B * p.order.T >= kManyQueries;
     const int64_t pos_blocks = std::max<int64_t>(1, cdiv(npos, 128 * kWTiles));
     p.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.tiles, 512 / (pos_blocks * B))));
     p.chunk = static_cast<int>(cdiv(p.tiles, p.chunks));
@@ -838,10 +1042,9 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
     auto up = [](int64_t v) { return (v + 255) & ~int64_t(255); };
     int64_t o = 0;
     p.qop = o, o += up(B * p.tiles * q4_tile_bytes(p.NT, p.RT));
-    p.ml = o, o += up(B * p.NS * p.rows * 8);
-    p.part = o, o += up(B * p.NS * p.rows * kQ4Lat * 4);
-    p.stats = o, o += weights ? up(B * p.rows * 8) : 0;
-    p.opart = o, o += p.uv_quarters ? up(4 * M * H * V * 4) : 0;
+    p.ml = o, o += up(B * p.NS * rows * 8);
+    p.part = o, o += up(B * p.NS * rows * kQ4Lat * 4);
+    p.stats = o, o += weights ? up(B * rows * 8) : 0;
     p.wpart = o, o += weights ? up(static_cast<int64_t>(p.chunks) * B * npos * 4) : 0;
     p.total = o;
     return p;
@@ -865,26 +1068,54 @@ int launch_attend_of(const AttendArgs &a, const Plan &p, hipStream_t st) {
     return p.RT == 1 ? launch_attend<RG, 5, 1, 2>(a, st) : launch_attend<RG, 5, 3, 2>(a, st);
 }
 
-template <typename QT, int NT, int RT>
-int launch_qa(const QaArgs &a, hipStream_t st) {
-    const int bytes = std::max(((a.nope + 31) / 32) * 32 * kWLd, 16 * kFLd * 4);
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(qa_kernel<QT, NT, RT>),
+template <typename QT, int NT, int RT, int MT>
+int launch_qa_of(const QaArgs &a, hipStream_t st) {
+    const int bytes = std::max(((a.nope + 31) / 32) * 32 * kWLd, 16 * MT * kFLd * 4);
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(qa_kernel<QT, NT, RT, MT>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 256 * kWLd);
     const int rc = check_hip(attr, "mla q4: query LDS size");
     if (rc) return rc;
-    qa_kernel<QT, NT, RT><<<dim3(a.H, static_cast<unsigned>(cdiv(a.M, 16)), 4), 256, bytes, st>>>(a);
+    qa_kernel<QT, NT, RT, MT><<<dim3(a.H, static_cast<unsigned>(cdiv(a.M, 16 * MT)), 4), 256, bytes, st>>>(a);
     return check_hip(hipGetLastError(), "mla q4: query launch");
 }
 
-template <int CP>
-int launch_uv(const UvArgs &a, hipStream_t st) {
-    const int bytes = (16 * (CP + 4) + 16 * a.NS + 8 * CP) * 4;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_kernel<CP>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (24 * (CP + 4) + 16 * kMaxSplits) * 4);
-    const int rc = check_hip(attr, "mla q4: output LDS size");
+template <typename QT, int NT, int RT>
+int launch_qa(const QaArgs &a, hipStream_t st) {
+    return a.M > 32 ? launch_qa_of<QT, NT, RT, 4>(a, st) : launch_qa_of<QT, NT, RT, 1>(a, st);
+}
+
+int launch_uv(const UvArgs &a, int many, hipStream_t st) {
+    static const hipError_t few = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_few_kernel),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, few_lds(kMaxSplits));
+    static const hipError_t many2 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_many_kernel<2>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 64 * 272 + 64 * kMaxSplits * 4);
+    static const hipError_t many3 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_many_kernel<3>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 3 * 64 * 272 + 64 * kMaxSplits * 4);
+    const int rc = check_hip(!many ? few : a.out_bf16 ? many2 : many3, "mla q4: output LDS size");
     if (rc) return rc;
-    uv_kernel<CP><<<dim3(a.H, static_cast<unsigned>(cdiv(a.M, 16)), kQ4Lat / CP), 256, bytes, st>>>(a);
+    const unsigned H = static_cast<unsigned>(a.order.H);
+    if (!many)
+        uv_few_kernel<<<dim3(H, static_cast<unsigned>(cdiv(a.M, 16))), 512, few_lds(a.NS), st>>>(a);
+    else if (a.out_bf16)
+        uv_many_kernel<2><<<dim3(H, static_cast<unsigned>(cdiv(a.M, 64))), 256, 2 * 64 * 272 + 64 * a.NS * 4, st>>>(a);
+    else
+        uv_many_kernel<3><<<dim3(H, static_cast<unsigned>(cdiv(a.M, 64))), 256, 3 * 64 * 272 + 64 * a.NS * 4, st>>>(a);
     return check_hip(hipGetLastError(), "mla q4: join and W_UV launch");
+}
+
+template <int RT>
+int launch_weights(const WeightArgs &wa, hipStream_t st) {
+    constexpr int bytes = 2 * q4_tile_bytes(5, RT);
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(weights_kernel<5, RT>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    int rc = check_hip(attr, "mla q4: weights LDS size");
+    if (rc) return rc;
+    const unsigned B = static_cast<unsigned>(wa.a.B);
+    weights_kernel<5, RT><<<dim3(static_cast<unsigned>(cdiv(wa.npos, 128 * kWTiles)), static_cast<unsigned>(wa.chunks), B), 512, bytes, st>>>(wa);
+    rc = check_hip(hipGetLastError(), "mla q4: weights launch");
+    if (rc) return rc;
+    weights_add_kernel<<<dim3(static_cast<unsigned>(cdiv(wa.npos, 64)), B), 256, 0, st>>>(wa);
+    return check_hip(hipGetLastError(), "mla q4: weight sum launch");
 }
 
 }  // namespace
@@ -935,12 +1166,13 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         return set_error(K3_ERR_SHAPE, "mla q4: a split of %d positions spans 2 GiB", p.Ts);
     auto st = static_cast<hipStream_t>(stream);
     char *ws = static_cast<char *>(workspace);
-    for (int64_t t0 = 0; t0 < T; t0 += p.T) {
-        const int Tc = static_cast<int>(std::min<int64_t>(p.T, T - t0));
-        const int rows = static_cast<int>(Tc * H), rblocks = static_cast<int>(cdiv(rows, 16 * p.RG));
+    for (int64_t t0 = 0; t0 < T; t0 += p.order.T) {
+        // (the last pass may have fewer queries; its order stays that of the others, whose room it has)
+        Rows order = rows_of(std::min<int64_t>(p.order.T, T - t0), H);
+        const int rows = order.count(), M = static_cast<int>(B * order.T);
         const int64_t q_seq = static_cast<int64_t>(p.tiles) * q4_tile_bytes(p.NT, p.RT);
         QaArgs qa{q_nope, q_rot, qn_batch, qn_token, qn_head, qr_batch, qr_token, qr_head, static_cast<const uint16_t *>(w_uk),
-                  ws + p.qop, q_seq, static_cast<int>(H), static_cast<int>(nope_dim), Tc, static_cast<int>(B * Tc), static_cast<int>(t0)};
+                  ws + p.qop, q_seq, static_cast<int>(H), static_cast<int>(nope_dim), M, static_cast<int>(t0), order};
         int rc;
         if (q_dtype == K3_BF16)
             rc = p.NT == 5 ? launch_qa<uint16_t, 5, 1>(qa, st) : launch_qa<uint16_t, 3, 1>(qa, st);
@@ -955,38 +1187,26 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         a.lengths = lengths, a.counts = counts;
         a.length = static_cast<int>(max_length), a.cap = a.length, a.count = static_cast<int>(T);
         a.part = reinterpret_cast<float *>(ws + p.part), a.ml = reinterpret_cast<float2 *>(ws + p.ml);
-        a.H = static_cast<int>(H), a.T = Tc, a.t0 = static_cast<int>(t0), a.rows = rows, a.Ts = p.Ts, a.NS = p.NS, a.rblocks = rblocks;
-        a.B = static_cast<int>(B), a.c = scale * 1.4426950408889634f;
-        a.swizzle = (a.B * a.NS * rblocks) % 8 == 0;
+        a.order = order, a.t0 = static_cast<int>(t0), a.rows = rows, a.Ts = p.Ts, a.NS = p.NS;
+        a.rblocks = static_cast<int>(cdiv(rows, 16 * p.RG)), a.B = static_cast<int>(B), a.c = scale * 1.4426950408889634f;
+        // blocks b % 8 run on one XCD: with several ranges its blocks get neighbouring ones (one L2 reads them); with one range the blocks
+        // that see most, which come first, are to be spread
+        a.swizzle = p.NS > 1 && (a.B * a.NS * a.rblocks) % 8 == 0;
         rc = p.RG == 4 ? launch_attend_of<4>(a, p, st) : launch_attend_of<2>(a, p, st);
         if (rc) return rc;
         UvArgs u{};
         u.part = a.part, u.ml = a.ml, u.w_uv = static_cast<const uint16_t *>(w_uv);
-        u.opart = p.uv_quarters ? reinterpret_cast<float *>(ws + p.opart) : nullptr;
         u.out = out, u.out_bf16 = out_dtype == K3_BF16, u.gate = gate;
         u.stats = weight ? reinterpret_cast<float2 *>(ws + p.stats) : nullptr;
-        u.H = a.H, u.T = Tc, u.M = static_cast<int>(B * Tc), u.V = static_cast<int>(v_dim), u.rows = rows, u.NS = p.NS;
+        u.order = order, u.M = M, u.V = static_cast<int>(v_dim), u.rows = rows, u.NS = p.NS;
         u.Tall = static_cast<int>(T), u.t0 = a.t0;
-        rc = p.uv_quarters ? launch_uv<128>(u, st) : launch_uv<512>(u, st);
+        rc = launch_uv(u, p.many, st);
         if (rc) return rc;
-        if (p.uv_quarters) {
-            out_kernel<<<dim3(static_cast<unsigned>(cdiv(static_cast<int64_t>(u.M) * H * v_dim, 1024))), 256, 0, st>>>(u);
-            rc = check_hip(hipGetLastError(), "mla q4: output launch");
-            if (rc) return rc;
-        }
         if (weight && max_length > 0) {
             WeightArgs wa{a, u.stats, reinterpret_cast<float *>(ws + p.wpart), weight, w_batch, static_cast<int>(cdiv(rows, 16)), p.chunk,
                           0, static_cast<int>(max_length)};
             wa.chunks = static_cast<int>(cdiv(wa.tiles, wa.chunk));
-            const dim3 grid(static_cast<unsigned>(cdiv(max_length, 128 * kWTiles)), static_cast<unsigned>(wa.chunks), static_cast<unsigned>(B));
-            if (p.RT == 1)
-                weights_kernel<5, 1><<<grid, 512, 0, st>>>(wa);
-            else
-                weights_kernel<5, 3><<<grid, 512, 0, st>>>(wa);
-            rc = check_hip(hipGetLastError(), "mla q4: weights launch");
-            if (rc) return rc;
-            weights_add_kernel<<<dim3(static_cast<unsigned>(cdiv(max_length, 256)), static_cast<unsigned>(B)), 256, 0, st>>>(wa);
-            rc = check_hip(hipGetLastError(), "mla q4: weight sum launch");
+            rc = p.RT == 1 ? launch_weights<1>(wa, st) : launch_weights<3>(wa, st);
             if (rc) return rc;
         }
     }
