@@ -468,8 +468,8 @@ int k3_mla_step_decode(const void *x, int x_dtype, const void *q_a, const float 
  * start: int32 [B] on the device, or null: start0 for all (then start0 + T <= cap is checked here);
  * counts: int32 [B] on the device, or null: T.  Positions outside 0 .. cap - 1 are left out.
  * A group of 32 with largest magnitude m gets the scale 2^e, e = floor(log2 m) - 2, one more if
- * m > 7 * 2^e, its byte e + 127 held to 2..252; codes round to nearest, ties to even.  A group with
- * a NaN or an infinity gets byte 255: the position is NaN to every query that sees it.
+ * m > 7 * 2^e, its byte e + 127 held to 2..252; codes round to nearest, ties to even.  A group of
+ * zeros gets byte 127, one with a NaN or an infinity 255: the position is NaN to every query that sees it.
  * c 16-byte aligned with pitches of whole 16 bytes; packed 4-byte aligned, pitches multiples of 4. */
 int k3_mla_q4_append(const void *c, int64_t c_batch, int64_t c_row, int c_dtype, const void *r, int64_t r_batch,
                      int64_t r_row, int r_dtype, void *packed, int64_t p_batch, int64_t p_row, void *scales,

@@ -20,8 +20,7 @@
 // and its 11 bits make one term of a probability enough for a bf16 result (2^-11 each, independent, below the
 // result's own 2^-8) and two for fp32 (2^-22), where bf16 would need two and three.  Probabilities are 2^kLift times those of the
 // row's reference maximum, so fp16's last bit, 2^-24, is 2^-34 of the largest.  A block that has come upon a scale
-// byte outside that range (of a group that is not all zeros) goes over its positions again with bf16 operands, exact for every byte, and one
-// term more.
+// byte outside that range goes over its positions again with bf16 operands, exact for every byte, and one term more.
 //
 // Query operands of 16 rows (a row: one head of one query), `terms` latent and `rterms` rotary terms:
 //     [term][step]                  64 lanes x 16 bytes, then 64 x 8: the lane's 32 codes, 192 bits
@@ -101,8 +100,29 @@ __device__ __forceinline__ uint32_t q4_pack_f16(float a, float b) {
     const f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
     return __builtin_bit_cast(uint32_t, v);
 }
+// eight E2M1 codes (of eight positions) times their scales, eight fp16 powers of two: exact
+__device__ __forceinline__ u32x4 q4_values_f16(uint32_t codes, u32x4 scales) {
+    // (as scalars: a bit cast of a vector's element reads its first one)
+    const uint32_t h[4] = {scales.x, scales.y, scales.z, scales.w};
+    const f16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 1),
+                        __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 3)};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __builtin_bit_cast(uint32_t, v[i] * __builtin_bit_cast(f16x2, h[i]));
+    return u32x4{o[0], o[1], o[2], o[3]};
+}
 __device__ __forceinline__ float q4_lo(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float q4_hi(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+// the same in bf16
+__device__ __forceinline__ u32x4 q4_values_bf16(uint32_t codes, u32x4 scales) {
+    const f32x2 c[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1),
+                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 3)};
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = hi16x2(__float_as_uint(c[i].x * q4_lo(scales[i])), __float_as_uint(c[i].y * q4_hi(scales[i])));
+    return v;
+}
 
 }  // namespace
 }  // namespace k3

@@ -13,15 +13,16 @@
 //   out      (few rows) the four column quarters of that product added, and the output gate
 //   weights  (if asked for) p once more from the rows' final maxima and sums, added over the rows
 //
-// attend, per round of 32 positions: a thread stages one group (16 bytes of codes and their scale byte); the codes go to
-// LDS as they are, where the score waves (0..3) read them as matrix operands; the same thread decodes its group
-// (exactly: E2M1 times a power of two) into the value tile, which the context waves (4..7, 128 columns each) read
-// transposed (fp16, see mla_q4.h).  In iteration i the score waves take round i's scores and turn round i - 1's into
-// probabilities, and the context waves take round i - 2's products, one barrier per iteration.  A row's reference maximum moves
-// only when a score exceeds it by kSlack (log2), so the accumulators are seldom rescaled.
+// attend, per round of 64 positions: the codes go to LDS as they are, 256 bytes and 16 scale bytes a position, and both products
+// take them from there: the score waves (0..3) as operands of the scaled product, the context waves (4..7, 128 columns each)
+// transposed, 4 bits at a time (ds_read_b64_tr_b4), decoded in registers to fp16 and multiplied with the positions' scales, which the
+// score waves leave in LDS as fp16 (exact, see mla_q4.h).  (Decoding into a value tile in LDS, 1 KB a position written and read, held
+// rounds of 32 positions only and took 0.86 us for each at 32 rows, 1.15 at 64.)  One barrier an iteration: round i + 1 is stored, round
+// i's scores and the last round's probabilities are formed, the context waves take the products of the round before.  A row's reference
+// maximum moves only when a score exceeds it by kSlack (log2), so the accumulators are seldom rescaled.
 //
 // A position whose scale byte is 255 (NaN) makes its scores NaN by the matrix product itself, so every row that sees it is NaN; its
-// values are staged as zeros, so a row that does not see it (weight zero) stays clean.
+// scale for the second product is zero, so a row that does not see it (weight zero) stays clean.
 #include <algorithm>
 #include <type_traits>
 
@@ -31,7 +32,9 @@ namespace k3 {
 namespace {
 
 typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s4_t *lds_s4;
+typedef __attribute__((address_space(3))) i32x2 *lds_i2;
 
 // The order of a sequence's rows: by query (row = t H + h: the heads of one query are neighbours, few queries fill the tiles)
 // or by head (row = h Tp + t, Tp = T rounded up to 16: a tile is 16 queries of one head, so a block of the query and output
@@ -243,33 +246,33 @@ struct AttendArgs {
     int swizzle;
 };
 
-constexpr int kRound = 32;                      // positions per round
+constexpr int kRound = 64;                      // positions per round: four tiles of 16
 constexpr int kKLd = 272;                       // LDS bytes of a staged row of codes: 256 + 16 scale bytes
 constexpr int kRLd = 144;                       // .. of a rotary row: 128 + 16
-constexpr int kVLd = 1056;                      // .. of a value row: 1024 + 32
-constexpr int kKBytes = kRound * kKLd, kRBytes = kRound * kRLd, kVBytes = kRound * kVLd;
-
-constexpr int kKSlots = 3;
+constexpr int kKBytes = kRound * kKLd, kRBytes = kRound * kRLd, kTBytes = kRound * 32;
 constexpr int kCLd = 132;                       // floats of a context row on its way out: 128 + 4
-static_assert(4 * 16 * kCLd * 4 <= 2 * kVBytes, "the contexts' way out fits the value tiles");
 
+// RG: groups of 16 rows.  1, 2: 4 / RG score waves to a group, which tell each other their tiles' maxima through LDS and a
+// barrier, so a round's probabilities are formed one iteration after its scores (kLag 2); 4: a wave to a group, in the same one.
+constexpr int attend_lag(int RG) { return RG == 4 ? 1 : 2; }
 constexpr int attend_lds(int RG, int RT, int PT) {   // PT fp16 terms of the probabilities (bf16: one more)
-    return kKSlots * kKBytes + 2 * kRBytes + 2 * kVBytes + 2 * RG * (PT + 1) * 1024 + RG * RT * 2048;
+    const int slots = attend_lag(RG) + 2;
+    return slots * (kKBytes + kTBytes) + 2 * kRBytes + 2 * RG * (PT + 1) * 2048 + RG * RT * 2048;
 }
 
-// RG: groups of 16 rows (2: two score waves to a group, one tile of 16 positions each; 4: one, two tiles);
 // NT latent and RT rotary terms of the queries, PT fp16 terms of the probabilities
 template <int RG, int NT, int RT, int PT>
 __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
-    constexpr int TG = 4 / RG, NTILE = 2 / TG;   // score waves of a row group; tiles of 16 positions per score wave
-    constexpr int kPLd = (PT + 1) * 1024;        // LDS bytes of a row group's probabilities
+    constexpr int TG = 4 / RG, NTILE = RG;       // score waves of a row group; tiles of 16 positions per score wave
+    constexpr int kLag = attend_lag(RG), kSlots = kLag + 2;
+    constexpr int kPLd = (PT + 1) * 2048;        // LDS bytes of a row group's probabilities
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ float xm[2][TG][RG * 16];         // tile maxima [parity][score wave of the group][row]
     __shared__ float xf[2][RG * 16];             // rescale factors [parity][row]
     __shared__ float xl[TG][RG * 16];
     __shared__ int wide;                         // a staged scale byte needs bf16's range
-    char *const kbuf = lds, *const rbuf = lds + kKSlots * kKBytes, *const vbuf = rbuf + 2 * kRBytes, *const pbuf = vbuf + 2 * kVBytes;
-    char *const qbuf = pbuf + 2 * RG * kPLd;     // the queries' rotary operands
+    char *const kbuf = lds, *const tbuf = kbuf + kSlots * kKBytes, *const rbuf = tbuf + kSlots * kTBytes;
+    char *const pbuf = rbuf + 2 * kRBytes, *const qbuf = pbuf + 2 * RG * kPLd;   // qbuf: the queries' rotary operands
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, q4 = lane >> 4;
     const int nb = gridDim.x;
@@ -292,75 +295,94 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     }
     const int n = t_end - t_begin, nr = (n + kRound - 1) / kRound;
 
-    // ---- staging, by the context waves: thread = (positions st / 16 and 16 more, group st % 16) and a 16-byte rotary chunk
-    const auto rp = make_rsrc(a.packed + b * a.p_b + t_begin * a.p_t, static_cast<uint32_t>((n - 1) * a.p_t + 256));
-    const auto rs = make_rsrc(a.scales + b * a.s_b + t_begin * a.s_t, static_cast<uint32_t>((n - 1) * a.s_t + 16));
-    const auto rr = make_rsrc(a.rot + b * a.r_b + t_begin * a.r_t, static_cast<uint32_t>((n - 1) * a.r_t + 128));
-    const int st = tid & 255, srow = st >> 4, sgrp = st & 15, orow = st >> 3, ochunk = st & 7;
+    // ---- staging: a thread takes two groups of codes (positions tid / 16 and 32 more) and a 16-byte rotary chunk; the score
+    // waves also four scale bytes each (position tid / 4)
+    const uint8_t *const kp = a.packed + b * a.p_b + t_begin * a.p_t, *const sp = a.scales + b * a.s_b + t_begin * a.s_t;
+    const uint8_t *const op = a.rot + b * a.r_b + t_begin * a.r_t;
+    const int srow = tid >> 4, sgrp = tid & 15, orow = tid >> 3, ochunk = tid & 7, brow = (tid & 255) >> 2, bquad = tid & 3;
+    const uint32_t ko = static_cast<uint32_t>(srow) * static_cast<uint32_t>(a.p_t) + sgrp * 16u, k32 = 32u * static_cast<uint32_t>(a.p_t);
+    const uint32_t oo = static_cast<uint32_t>(orow) * static_cast<uint32_t>(a.r_t) + ochunk * 16u;
+    const uint32_t so = static_cast<uint32_t>(brow) * static_cast<uint32_t>(a.s_t) + bquad * 4u;
     struct Stage {
         u32x4 k[2], o;
-        uint32_t s[2];
+        uint32_t s;
     };
+    // (a resource of the round's own rows: those past the last are outside it and load zeros)
     auto load = [&](Stage &g, int rd) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int i = rd * kRound + 16 * u + srow;
-            const bool ok = i < n;
-            g.k[u] = __builtin_bit_cast(u32x4, buf_load16(rp, ok ? static_cast<uint32_t>(i) * static_cast<uint32_t>(a.p_t) + sgrp * 16u : kOobOffset));
-            g.s[u] = __builtin_amdgcn_raw_buffer_load_b8(rs, ok ? static_cast<uint32_t>(i) * static_cast<uint32_t>(a.s_t) + sgrp : kOobOffset, 0, 0);
-        }
-        const int j = rd * kRound + orow;
-        g.o = __builtin_bit_cast(u32x4, buf_load16(rr, j < n ? static_cast<uint32_t>(j) * static_cast<uint32_t>(a.r_t) + ochunk * 16u : kOobOffset));
+        const int64_t at = static_cast<int64_t>(rd) * kRound;
+        const int last = n - 1 - rd * kRound;
+        const auto rk = make_rsrc(kp + at * a.p_t, last < 0 ? 0u : static_cast<uint32_t>(last) * static_cast<uint32_t>(a.p_t) + 256u);
+        const auto ro = make_rsrc(op + at * a.r_t, last < 0 ? 0u : static_cast<uint32_t>(last) * static_cast<uint32_t>(a.r_t) + 128u);
+        g.k[0] = __builtin_bit_cast(u32x4, buf_load16(rk, ko));
+        g.k[1] = __builtin_bit_cast(u32x4, buf_load16(rk, ko + k32));
+        g.o = __builtin_bit_cast(u32x4, buf_load16(ro, oo));
+        if (wave < 4) g.s = buf_load4(make_rsrc(sp + at * a.s_t, last < 0 ? 0u : static_cast<uint32_t>(last) * static_cast<uint32_t>(a.s_t) + 16u), so);
     };
-    auto store_k = [&](const Stage &g, int rd, bool look) __attribute__((always_inline)) {
+    // codes and rotary rows as they are; of the scale bytes a second form, 2^(byte - 127) in 16 bits, [group][position], for the
+    // context waves (a NaN's is zero)
+    auto store = [&](const Stage &g, int rd, auto bf) __attribute__((always_inline)) {
+        char *k = kbuf + rd % kSlots * kKBytes;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            char *k = kbuf + (rd % kKSlots) * kKBytes + (16 * u + srow) * kKLd;
-            *reinterpret_cast<u32x4 *>(k + sgrp * 16) = g.k[u];
-            reinterpret_cast<uint8_t *>(k)[256 + sgrp] = static_cast<uint8_t>(g.s[u]);
-            // (a NaN's values are staged as zeros; -0 codes count as values)
-            if (look && g.s[u] - kHalfLow > kHalfHigh - kHalfLow && g.s[u] != 255u && (g.k[u].x | g.k[u].y | g.k[u].z | g.k[u].w) != 0u)
-                wide = 1;
-        }
+        for (int u = 0; u < 2; ++u) *reinterpret_cast<u32x4 *>(k + (32 * u + srow) * kKLd + sgrp * 16) = g.k[u];
         *reinterpret_cast<u32x4 *>(rbuf + (rd & 1) * kRBytes + orow * kRLd + ochunk * 16) = g.o;
-    };
-    // this thread's group (which it staged itself) as fp16 or bf16, 64 bytes; lanes 4..7, 8..11, 12..15 of a 16-lane row
-    // start at another 16 bytes, so a store instruction's lanes spread over the banks
-    auto store_v = [&](int rd, int u, auto bf) __attribute__((always_inline)) {
-        const char *ks = kbuf + (rd % kKSlots) * kKBytes + (16 * u + srow) * kKLd;
-        const u32x4 k = *reinterpret_cast<const u32x4 *>(ks + sgrp * 16);
-        const uint32_t s = reinterpret_cast<const uint8_t *>(ks)[256 + sgrp];
-        char *v = vbuf + (rd & 1) * kVBytes + (16 * u + srow) * kVLd + sgrp * 64;
-        const int x = (lane >> 2) & 3;
-        const u32x4 y = (x & 1) ? u32x4{k.y, k.x, k.w, k.z} : k;
-        u32x4 z = (x & 2) ? u32x4{y.z, y.w, y.x, y.y} : y;
-        if (s == 255u) z = u32x4{0u, 0u, 0u, 0u};
-        const float f = s == 255u ? 0.f : e8m0_to_f32(s);
+        if (wave < 4) {
+            *reinterpret_cast<uint32_t *>(k + brow * kKLd + 256 + bquad * 4) = g.s;
+            char *t = tbuf + rd % kSlots * kTBytes + bquad * 4 * (2 * kRound) + 2 * brow;
+            bool out = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            u32x4 o;
-            if constexpr (decltype(bf)::value)
-                o = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], f, 0)),
-                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], f, 1)),
-                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], f, 2)),
-                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(z[j], f, 3))};
-            else
-                o = u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(z[j], f, 0)),
-                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(z[j], f, 1)),
-                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(z[j], f, 2)),
-                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(z[j], f, 3))};
-            *reinterpret_cast<u32x4 *>(v + ((j ^ x) << 4)) = o;
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t e = (g.s >> (8 * x)) & 255u;
+                uint32_t h;
+                if constexpr (decltype(bf)::value) {
+                    h = e == 255u ? 0u : e == 0u ? 64u : e << 7;          // bf16; 2^-127 is a subnormal
+                } else {
+                    h = e >= 113u ? (e - 112u) << 10 : 1u << (e - 103u);  // fp16; below 2^-14 a subnormal
+                    const bool in = e - kHalfLow <= kHalfHigh - kHalfLow;
+                    h = in ? h : 0u;
+                    out = out || !(in || e == 255u);
+                }
+                *reinterpret_cast<uint16_t *>(t + x * (2 * kRound)) = static_cast<uint16_t>(h);
+            }
+            if (out && rd * kRound + brow < n) wide = 1;
         }
     };
-
-    // iterations 0 .. nr + 1, an even number of them (rounds past the last are zeros that no row sees)
-    const int iters = (nr + 3) & ~1;
+    if (tid == 0) wide = 0;
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
-    if (tid == 0) wide = 0;
+    // Iterations 0 .. nr - 1 + kLag: store round i + 1 (loaded two iterations before; 64 rows, whose accumulators leave few registers
+    // and whose iterations are long: one), load the one after next, and the role's part.  With two rounds in registers their
+    // number is even (rounds past the last are zeros that no row sees).
+    auto rounds = [&](auto bf, auto part) __attribute__((always_inline)) {
+        Stage g[kLag];
+        load(g[0], 0);
+        if (kLag > 1) load(g[kLag - 1], 1);
+        __syncthreads();        // wide is clear; every wave is done with a first pass
+        store(g[0], 0, bf);
+        load(g[0], kLag);
+        __syncthreads();
+        if constexpr (kLag == 1) {
+            for (int i = 0; i < nr + 1; ++i) {
+                store(g[0], i + 1, bf);
+                load(g[0], i + 2);
+                part(i, even);
+                __syncthreads();
+            }
+        } else {
+            for (int i = 0; i < nr + 2; i += 2) {
+                store(g[1], i + 1, bf);
+                load(g[1], i + 3);
+                part(i, even);
+                __syncthreads();
+                store(g[0], i + 2, bf);
+                load(g[0], i + 4);
+                part(i + 1, odd);
+                __syncthreads();
+            }
+        }
+    };
     if (wave < 4) {
         // ================= score waves
-        const int rg = TG == 1 ? wave : wave % RG, tg = TG == 1 ? 0 : wave / RG;
+        const int rg = wave % RG, tg = wave / RG;
         const char *tile = a.qop + b * a.q_seq + static_cast<int64_t>((row0 >> 4) + rg) * q4_tile_bytes(NT, RT);
         u32x4 qlo[NT][kQ4Steps];
         u32x2 qhi[NT][kQ4Steps];
@@ -374,7 +396,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 qhi[x][k] = *reinterpret_cast<const u32x2 *>(tile + q4_code_at(x, k) + 1024 + lane * 8);
             }
         }
-        // (the two score waves of a row group write the same)
+        // (the score waves of a row group write the same)
         char *const qr = qbuf + rg * RT * 2048 + lane * 16;
 #pragma unroll
         for (int x = 0; x < 2 * RT; ++x) *reinterpret_cast<u32x4 *>(qr + x * 1024) = *reinterpret_cast<const u32x4 *>(tile + q4_rope_at(NT, 0, x) + lane * 16);
@@ -382,69 +404,56 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         const int tq = a.order.query(row), sees = row < a.rows && tq < a.order.T ? q4_sees(a.t0 + tq, cnt, len) : 0;
         const int limit = min(sees, t_end) - t_begin;       // positions of this split that the row sees
         float m_ref, l_run, mt[2];
-        f32x4 sc[2][NTILE];                                 // scores of round i (parity)
+        f32x4 sc[kLag][NTILE];                              // scaled scores of round i (log2 units; hidden: -infinity)
 
+        // round rd's scores; their maximum over the wave's tiles
         auto scores = [&](int rd, f32x4 (&out)[NTILE]) __attribute__((always_inline)) {
-            f32x4 hr[NTILE];
-#pragma unroll
-            for (int u = 0; u < NTILE; ++u) hr[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int x = RT - 1; x >= 0; --x) {
-                    const u32x4 qv = *reinterpret_cast<const u32x4 *>(qr + (2 * x + s) * 1024);
-#pragma unroll
-                    for (int u = 0; u < NTILE; ++u) {
-                        const char *o = rbuf + (rd & 1) * kRBytes + ((tg * NTILE + u) * 16 + r16) * kRLd + s * 64 + q4 * 16;
-                        hr[u] = q4_mfma_bf16(*reinterpret_cast<const u32x4 *>(o), qv, hr[u]);
-                    }
-                }
+            float top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < NTILE; ++u) {
-                const char *k = kbuf + (rd % kKSlots) * kKBytes + ((tg * NTILE + u) * 16 + r16) * kKLd;
+                const int at = (tg * NTILE + u) * 16;
+                const char *k = kbuf + rd % kSlots * kKBytes + (at + r16) * kKLd, *o = rbuf + (rd & 1) * kRBytes + (at + r16) * kRLd + q4 * 16;
                 const int ks = *reinterpret_cast<const int *>(k + 256 + q4 * 4);
                 u32x4 kc[kQ4Steps];
 #pragma unroll
                 for (int s = 0; s < kQ4Steps; ++s) kc[s] = *reinterpret_cast<const u32x4 *>(k + q4 * 64 + s * 16);
-                f32x4 hi = {0.f, 0.f, 0.f, 0.f}, lo = hi;
+                f32x4 d[4];                                 // the terms in chains of their own
+#pragma unroll
+                for (int x = 0; x < 4; ++x) d[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int x = RT - 1; x >= 0; --x)
+                        d[3] = q4_mfma_bf16(*reinterpret_cast<const u32x4 *>(o + s * 64), *reinterpret_cast<const u32x4 *>(qr + (2 * x + s) * 1024), d[3]);
 #pragma unroll
                 for (int x = NT - 1; x >= 0; --x) {
-                    f32x4 &d = x < 2 ? hi : lo;
-                    d = q4_mfma<0>(kc[0], ks, qlo[x][0], qhi[x][0], qs[x], d);
-                    d = q4_mfma<1>(kc[1], ks, qlo[x][1], qhi[x][1], qs[x], d);
-                    d = q4_mfma<2>(kc[2], ks, qlo[x][2], qhi[x][2], qs[x], d);
-                    d = q4_mfma<3>(kc[3], ks, qlo[x][3], qhi[x][3], qs[x], d);
+                    f32x4 &c = d[x < 3 ? x : 3];
+                    c = q4_mfma<0>(kc[0], ks, qlo[x][0], qhi[x][0], qs[x], c);
+                    c = q4_mfma<1>(kc[1], ks, qlo[x][1], qhi[x][1], qs[x], c);
+                    c = q4_mfma<2>(kc[2], ks, qlo[x][2], qhi[x][2], qs[x], c);
+                    c = q4_mfma<3>(kc[3], ks, qlo[x][3], qhi[x][3], qs[x], c);
                 }
-                out[u] = hi + (lo + hr[u]);
-                __builtin_amdgcn_sched_barrier(0);   // (hoisting the next tile's operands costs the registers of a query term)
-            }
-        };
-        // scores -> scaled (log2 units), hidden positions -infinity; the tile maxima are published
-        auto publish = [&](int rd, f32x4 (&s)[NTILE]) __attribute__((always_inline)) {
-            float mt = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < NTILE; ++u)
+                const f32x4 s = d[0] + ((d[3] + d[2]) + d[1]);
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
-                    const int j = rd * kRound + (tg * NTILE + u) * 16 + 4 * q4 + v;
-                    s[u][v] = j < limit ? s[u][v] * a.c : -INFINITY;
-                    mt = fmaxf(mt, s[u][v]);
+                    out[u][v] = rd * kRound + at + 4 * q4 + v < limit ? s[v] * a.c : -INFINITY;
+                    top = fmaxf(top, out[u][v]);
                 }
-            mt = q4_rows_max(mt);
-            if (TG > 1 && q4 == 0) xm[rd & 1][tg][rg * 16 + r16] = mt;
-            return mt;
+                if (RG == 4 || NT == 5) __builtin_amdgcn_sched_barrier(0);   // (the next tile's operands are more than the registers hold)
+            }
+            return q4_rows_max(top);
         };
+        // round rd's probabilities, lifted by kLift over the row's reference, with the maximum mt over all of the round's tiles
         auto probs = [&](int rd, const f32x4 (&s)[NTILE], float mt, auto bf) __attribute__((always_inline)) {
-            if constexpr (TG > 1) mt = fmaxf(xm[rd & 1][0][rg * 16 + r16], xm[rd & 1][TG - 1][rg * 16 + r16]);
             float f = 1.f;
-            if (mt > m_ref + kSlack || m_ref == -INFINITY) {
+            if (mt > m_ref + kSlack || (m_ref == -INFINITY && mt != -INFINITY)) {
                 f = m_ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref - mt);
-                if (mt == -INFINITY) f = 1.f;
                 l_run *= f;
                 m_ref = mt;
             }
             const float ref = m_ref == -INFINITY ? 0.f : m_ref - kLift;
-            char *p = pbuf + ((rd & 1) * RG + rg) * kPLd + lane * 16;
+            // slot [tile][half][row][8 positions]: what lane (row, tile) of the second product takes in its two steps
+            char *p = pbuf + ((rd & 1) * RG + rg) * kPLd + ((q4 >> 1) * 16 + r16) * 16 + (q4 & 1) * 8;
 #pragma unroll
             for (int u = 0; u < NTILE; ++u) {
                 float e[4];
@@ -453,12 +462,12 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                     e[v] = __builtin_amdgcn_exp2f(s[u][v] - ref);
                     l_run += e[v];
                 }
-                char *pu = p + (tg * NTILE + u) * 8;
+                char *pu = p + (tg * NTILE + u) * 512;
                 if constexpr (!decltype(bf)::value) {
 #pragma unroll
                     for (int x = 0; x < PT; ++x) {
                         const uint32_t a0 = q4_pack_f16(e[0], e[1]), a1 = q4_pack_f16(e[2], e[3]);
-                        *reinterpret_cast<u32x2 *>(pu + x * 1024) = u32x2{a0, a1};
+                        *reinterpret_cast<u32x2 *>(pu + x * 2048) = u32x2{a0, a1};
                         if (x + 1 < PT) {
                             const f16x2 h0 = __builtin_bit_cast(f16x2, a0), h1 = __builtin_bit_cast(f16x2, a1);
                             e[0] -= static_cast<float>(h0[0]), e[1] -= static_cast<float>(h0[1]);
@@ -469,40 +478,43 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int x = 0; x < PT + 1; ++x) {
                         const uint32_t a0 = q4_pack_bf16(e[0], e[1]), a1 = q4_pack_bf16(e[2], e[3]);
-                        *reinterpret_cast<u32x2 *>(pu + x * 1024) = u32x2{a0, a1};
+                        *reinterpret_cast<u32x2 *>(pu + x * 2048) = u32x2{a0, a1};
                         e[0] -= q4_lo(a0), e[1] -= q4_hi(a0), e[2] -= q4_lo(a1), e[3] -= q4_hi(a1);
                     }
                 }
             }
             if (tg == 0 && q4 == 0) xf[rd & 1][rg * 16 + r16] = f;
         };
-
         auto all = [&](auto bf) __attribute__((always_inline)) {
             m_ref = -INFINITY, l_run = 0.f;
-            __syncthreads();   // wide is clear
-            __syncthreads();   // round 0 is staged
-            auto part = [&](int i, auto par) __attribute__((always_inline)) {
+            rounds(bf, [&](int i, auto par) __attribute__((always_inline)) {
                 constexpr int d = decltype(par)::value;
-                scores(i, sc[d]);
-                probs(i - 1, sc[1 - d], mt[1 - d], bf);
-                mt[d] = publish(i, sc[d]);
-                __syncthreads();
-            };
-            scores(0, sc[0]);
-            mt[0] = publish(0, sc[0]);
-            __syncthreads();
-            part(1, odd);
-            for (int i = 2; i < iters; i += 2) {
-                part(i, even);
-                part(i + 1, odd);
-            }
+                if constexpr (kLag == 1) {
+                    mt[0] = scores(i, sc[0]);
+                    probs(i, sc[0], mt[0], bf);
+                } else {
+                    mt[d] = scores(i, sc[d]);
+                    if (q4 == 0) xm[i & 1][tg][rg * 16 + r16] = mt[d];
+                    if (i > 0) {
+                        float m = xm[(i - 1) & 1][0][rg * 16 + r16];
+#pragma unroll
+                        for (int x = 1; x < TG; ++x) m = fmaxf(m, xm[(i - 1) & 1][x][rg * 16 + r16]);
+                        probs(i - 1, sc[kLag - 1 - d], m, bf);
+                    }
+                }
+            });
         };
         all(std::false_type{});
         if (__builtin_amdgcn_readfirstlane(wide)) all(std::true_type{});
         const float l = q4_rows_sum(l_run);
-        if (TG > 1 && q4 == 0) xl[tg][rg * 16 + r16] = l;
+        if (q4 == 0) xl[tg][rg * 16 + r16] = l;
         __syncthreads();
-        if (tg == 0 && q4 == 0 && row < a.rows) ml[row] = make_float2(m_ref, TG > 1 ? xl[0][rg * 16 + r16] + xl[TG - 1][rg * 16 + r16] : l);
+        if (tg == 0 && q4 == 0 && row < a.rows) {
+            float sum = xl[0][rg * 16 + r16];
+#pragma unroll
+            for (int x = 1; x < TG; ++x) sum += xl[x][rg * 16 + r16];
+            ml[row] = make_float2(m_ref, sum);
+        }
     } else {
         // ================= context waves: columns 128 (wave - 4) .. +128
         const int col0 = (wave - 4) * 128;
@@ -510,8 +522,14 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         auto context = [&](int rd, auto bf) __attribute__((always_inline)) {
             constexpr bool kBf = decltype(bf)::value;
             constexpr int N = PT + kBf;
-            const char *p = pbuf + (rd & 1) * RG * kPLd + lane * 16;
-            const char *v = vbuf + (rd & 1) * kVBytes + (4 * q4 + (r16 >> 2)) * kVLd + (col0 + (r16 & 3) * 4) * 2;
+            // lane (column r16, positions 16 q4 .. +16): the codes of a tile of 16 columns, transposed, as they lie in the rows
+            const char *k = kbuf + rd % kSlots * kKBytes + (16 * q4 + r16) * kKLd + col0 / 2;
+            const char *t = tbuf + rd % kSlots * kTBytes + (col0 / 32) * (2 * kRound) + 32 * q4;
+            const char *p = pbuf + (rd & 1) * RG * kPLd + (q4 * 32 + r16) * 16;
+            u32x2 code[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                code[c] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i2)(k + c * 8)));
             float f[RG];
             bool any = false;
 #pragma unroll
@@ -525,29 +543,26 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
 #pragma unroll
                     for (int r = 0; r < RG; ++r) acc[c][r] *= f[r];
             }
-            u32x4 pf[RG][N];
 #pragma unroll
-            for (int r = 0; r < RG; ++r)
+            for (int s = 0; s < 2; ++s) {                   // 8 of the lane's 16 positions
+                u32x4 pf[RG][N];
 #pragma unroll
-                for (int x = 0; x < N; ++x) pf[r][x] = *reinterpret_cast<const u32x4 *>(p + r * kPLd + x * 1024);
-            // the columns' operands are read two tiles ahead; nothing moves across a tile (that costs registers)
-            auto column = [&](int c) __attribute__((always_inline)) {
-                const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(v + c * 32));
-                const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(v + c * 32 + 16 * kVLd));
-                return __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-            };
-            u32x4 vf[2] = {column(0), column(1)};
+                for (int r = 0; r < RG; ++r)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
+                    for (int x = 0; x < N; ++x) pf[r][x] = *reinterpret_cast<const u32x4 *>(p + r * kPLd + x * 2048 + s * 256);
 #pragma unroll
-                for (int t = N - 1; t >= 0; --t)
+                for (int g = 0; g < 4; ++g) {               // 32 columns: one scale a position
+                    const u32x4 h = *reinterpret_cast<const u32x4 *>(t + g * (2 * kRound) + s * 16);
 #pragma unroll
-                    for (int r = 0; r < RG; ++r)
-                        acc[c][r] = kBf ? q4_mfma_bf16(vf[c & 1], pf[r][t], acc[c][r]) : q4_mfma_f16(vf[c & 1], pf[r][t], acc[c][r]);
-                if (c + 2 < 8) vf[c & 1] = column(c + 2);
-                // the next round's values are decoded while the matrix cores work on this one's
-                if (c == 1 || c == 4) store_v(rd + 1, c / 4, bf);
-                __builtin_amdgcn_sched_barrier(0);
+                    for (int c = 2 * g; c < 2 * g + 2; ++c) {
+                        const u32x4 v = kBf ? q4_values_bf16(code[c][s], h) : q4_values_f16(code[c][s], h);
+#pragma unroll
+                        for (int x = N - 1; x >= 0; --x)
+#pragma unroll
+                            for (int r = 0; r < RG; ++r) acc[c][r] = kBf ? q4_mfma_bf16(v, pf[r][x], acc[c][r]) : q4_mfma_f16(v, pf[r][x], acc[c][r]);
+                    }
+                    if (RG == 4) __builtin_amdgcn_sched_barrier(0);
+                }
             }
         };
         auto all = [&](auto bf) __attribute__((always_inline)) {
@@ -555,43 +570,18 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
             for (int c = 0; c < 8; ++c)
 #pragma unroll
                 for (int r = 0; r < RG; ++r) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-            constexpr bool kLook = !decltype(bf)::value;
-            Stage g[2];
-            load(g[0], 0);
-            load(g[1], 1);
-            __syncthreads();
-            store_k(g[0], 0, kLook);
-            load(g[0], 2);
-            __syncthreads();
-            // store round i + 1's codes (loaded two iterations before), load round i + 3, decode round i - 1, take round
-            // i - 2's products
-            auto stage = [&](int i, auto par) __attribute__((always_inline)) {
-                constexpr int d = decltype(par)::value;
-                store_k(g[1 - d], i + 1, kLook);
-                load(g[1 - d], i + 3);
-            };
-            stage(0, even);
-            __syncthreads();
-            stage(1, odd);
-            store_v(0, 0, bf);
-            store_v(0, 1, bf);
-            __syncthreads();
-            for (int i = 2; i < iters; i += 2) {
-                stage(i, even);
-                context(i - 2, bf);
-                __syncthreads();
-                stage(i + 1, odd);
-                context(i - 1, bf);
-                __syncthreads();
-            }
+            rounds(bf, [&](int i, auto) __attribute__((always_inline)) {
+                if (i >= kLag) context(i - kLag, bf);
+            });
         };
         all(std::false_type{});
         if (__builtin_amdgcn_readfirstlane(wide)) all(std::true_type{});
         __syncthreads();
-        // the records through LDS (the value tiles are done with), so that a store writes 512 contiguous bytes of two rows: as the
+        // the records through LDS (the codes are done with), so that a store writes 512 contiguous bytes of two rows: as the
         // accumulators lie, 64 bytes of sixteen rows, the 256 blocks of a short split took 7 us to write them
         float *part = a.part + ((static_cast<int64_t>(b) * a.NS + split) * a.rows + row0) * kQ4Lat + col0;
-        float *const x = reinterpret_cast<float *>(vbuf) + (wave - 4) * 16 * kCLd;
+        float *const x = reinterpret_cast<float *>(kbuf) + (wave - 4) * 16 * kCLd;
+        static_assert(4 * 16 * kCLd * 4 <= kSlots * kKBytes, "the contexts' way out fits the code tiles");
 #pragma unroll
         for (int r = 0; r < RG; ++r) {
 #pragma unroll
@@ -1025,7 +1015,7 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
     p.NT = fine ? 5 : 3, p.RT = q_bf16 ? 1 : fine ? 3 : 2, p.PT = out_bf16 ? 1 : 2;
     p.order = rows_of(std::max<int64_t>(1, std::min(T, kChunkRows / (B * H))), H);
     const int64_t rows = p.order.count();
-    p.RG = rows > 64 ? 4 : 2;
+    p.RG = rows > 64 ? 4 : rows > 16 ? 2 : 1;
     p.rblocks = static_cast<int>(cdiv(rows, 16 * p.RG));
     p.tiles = p.rblocks * p.RG;
     const int64_t base = B * p.rblocks;
@@ -1192,7 +1182,7 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         // blocks b % 8 run on one XCD: with several ranges its blocks get neighbouring ones (one L2 reads them); with one range the blocks
         // that see most, which come first, are to be spread
         a.swizzle = p.NS > 1 && (a.B * a.NS * a.rblocks) % 8 == 0;
-        rc = p.RG == 4 ? launch_attend_of<4>(a, p, st) : launch_attend_of<2>(a, p, st);
+        rc = p.RG == 4 ? launch_attend_of<4>(a, p, st) : p.RG == 2 ? launch_attend_of<2>(a, p, st) : launch_attend_of<1>(a, p, st);
         if (rc) return rc;
         UvArgs u{};
         u.part = a.part, u.ml = a.ml, u.w_uv = static_cast<const uint16_t *>(w_uv);

@@ -4,8 +4,8 @@
 // A group of 32 values x with largest magnitude m gets the scale 2^e, e = floor(log2 m) - 2, one more where
 // m > 7 * 2^e: the magnitudes then end at 7, which rounds to 6, the format's largest, and is as far from it as the
 // midpoint of 4 and 6 from either; the usual rule (never one more) would clip up to 8.  The byte is e + 127 held to 2..252, the
-// range the rest of the library takes; codes round to nearest, ties to even.  A group with a NaN or an infinity
-// gets byte 255, which makes the position NaN to every query that sees it.
+// range the rest of the library takes; codes round to nearest, ties to even.  A group of zeros gets
+// byte 127, one with a NaN or an infinity 255, which makes the position NaN to every query that sees it.
 //
 // With norm weights the row is RMS-normalised first, in fp32 (the decode step's latent).
 //
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     top = umax_dpp<0x4e>(top);   // quad_perm [2,3,0,1]
     // biased exponent of m, less two, one more above 7/8 of the next power of two (1.75 x 2^floor(log2 m))
     int byte = static_cast<int>(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-    byte = top >= 0x7f800000u ? 255 : min(max(byte, 2), 252);
+    byte = top >= 0x7f800000u ? 255 : top == 0u ? 127 : min(max(byte, 2), 252);
     uint32_t code = 0;
     if (byte < 255) {
         const float s = __uint_as_float(static_cast<uint32_t>(byte) << 23);

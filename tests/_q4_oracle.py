@@ -15,7 +15,7 @@ def round_group(x):
         return [0] * 32, 255
     top = max(abs(v) for v in x)
     if top == 0:
-        return [0] * 32, 2
+        return [0] * 32, 127
     e = math.frexp(top)[1] - 3                     # floor(log2 top) - 2
     if top > 7.0 * 2.0 ** e:
         e += 1
