@@ -295,91 +295,75 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     }
     const int n = t_end - t_begin, nr = (n + kRound - 1) / kRound;
 
-    // ---- staging: a thread takes two groups of codes (positions tid / 16 and 32 more) and a 16-byte rotary chunk; the score
-    // waves also four scale bytes each (position tid / 4)
+    // ---- staging, by the context waves: a thread takes four groups of codes (positions st / 16 and every 16th from there), two
+    // 16-byte rotary chunks (st / 8 and 32 more) and four scale bytes (st / 4)
     const uint8_t *const kp = a.packed + b * a.p_b + t_begin * a.p_t, *const sp = a.scales + b * a.s_b + t_begin * a.s_t;
     const uint8_t *const op = a.rot + b * a.r_b + t_begin * a.r_t;
-    const int srow = tid >> 4, sgrp = tid & 15, orow = tid >> 3, ochunk = tid & 7, brow = (tid & 255) >> 2, bquad = tid & 3;
-    const uint32_t ko = static_cast<uint32_t>(srow) * static_cast<uint32_t>(a.p_t) + sgrp * 16u, k32 = 32u * static_cast<uint32_t>(a.p_t);
-    const uint32_t oo = static_cast<uint32_t>(orow) * static_cast<uint32_t>(a.r_t) + ochunk * 16u;
-    const uint32_t so = static_cast<uint32_t>(brow) * static_cast<uint32_t>(a.s_t) + bquad * 4u;
+    const int st = tid & 255, srow = st >> 4, sgrp = st & 15, orow = st >> 3, ochunk = st & 7, brow = st >> 2, bquad = st & 3;
     struct Stage {
-        u32x4 k[2], o;
+        u32x4 k[4], o[2];
         uint32_t s;
     };
-    // (a resource of the round's own rows: those past the last are outside it and load zeros)
-    auto load = [&](Stage &g, int rd) __attribute__((always_inline)) {
-        const int64_t at = static_cast<int64_t>(rd) * kRound;
-        const int last = n - 1 - rd * kRound;
-        const auto rk = make_rsrc(kp + at * a.p_t, last < 0 ? 0u : static_cast<uint32_t>(last) * static_cast<uint32_t>(a.p_t) + 256u);
-        const auto ro = make_rsrc(op + at * a.r_t, last < 0 ? 0u : static_cast<uint32_t>(last) * static_cast<uint32_t>(a.r_t) + 128u);
-        g.k[0] = __builtin_bit_cast(u32x4, buf_load16(rk, ko));
-        g.k[1] = __builtin_bit_cast(u32x4, buf_load16(rk, ko + k32));
-        g.o = __builtin_bit_cast(u32x4, buf_load16(ro, oo));
-        if (wave < 4) g.s = buf_load4(make_rsrc(sp + at * a.s_t, last < 0 ? 0u : static_cast<uint32_t>(last) * static_cast<uint32_t>(a.s_t) + 16u), so);
+    // The next round to load: its rows' addresses and the bytes there are from them on (rows past the last are outside and load
+    // zeros), moved on by a round's rows.
+    struct Next {
+        const uint8_t *k, *o, *s;
+        int kb, ob, sb;
+    } nx;
+    const int64_t kstep = kRound * a.p_t, ostep = kRound * a.r_t, sstep = kRound * a.s_t;
+    const uint32_t ko = static_cast<uint32_t>(srow) * static_cast<uint32_t>(a.p_t) + sgrp * 16u, k16 = 16u * static_cast<uint32_t>(a.p_t);
+    const uint32_t oo = static_cast<uint32_t>(orow) * static_cast<uint32_t>(a.r_t) + ochunk * 16u, o32 = 32u * static_cast<uint32_t>(a.r_t);
+    const uint32_t so = static_cast<uint32_t>(brow) * static_cast<uint32_t>(a.s_t) + bquad * 4u;
+    auto rewind = [&]() __attribute__((always_inline)) {
+        nx = Next{kp, op, sp, static_cast<int>((n - 1) * a.p_t + 256), static_cast<int>((n - 1) * a.r_t + 128), static_cast<int>((n - 1) * a.s_t + 16)};
     };
-    // codes and rotary rows as they are; of the scale bytes a second form, 2^(byte - 127) in 16 bits, [group][position], for the
-    // context waves (a NaN's is zero)
-    auto store = [&](const Stage &g, int rd, auto bf) __attribute__((always_inline)) {
-        char *k = kbuf + rd % kSlots * kKBytes;
+    auto load = [&](Stage &g) __attribute__((always_inline)) {
+        const auto rk = make_rsrc(nx.k, static_cast<uint32_t>(nx.kb)), ro = make_rsrc(nx.o, static_cast<uint32_t>(nx.ob));
 #pragma unroll
-        for (int u = 0; u < 2; ++u) *reinterpret_cast<u32x4 *>(k + (32 * u + srow) * kKLd + sgrp * 16) = g.k[u];
-        *reinterpret_cast<u32x4 *>(rbuf + (rd & 1) * kRBytes + orow * kRLd + ochunk * 16) = g.o;
-        if (wave < 4) {
-            *reinterpret_cast<uint32_t *>(k + brow * kKLd + 256 + bquad * 4) = g.s;
-            char *t = tbuf + rd % kSlots * kTBytes + bquad * 4 * (2 * kRound) + 2 * brow;
-            bool out = false;
+        for (int u = 0; u < 4; ++u) g.k[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, ko + u * k16, 0, 0));
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint32_t e = (g.s >> (8 * x)) & 255u;
-                uint32_t h;
-                if constexpr (decltype(bf)::value) {
-                    h = e == 255u ? 0u : e == 0u ? 64u : e << 7;          // bf16; 2^-127 is a subnormal
-                } else {
-                    h = e >= 113u ? (e - 112u) << 10 : 1u << (e - 103u);  // fp16; below 2^-14 a subnormal
-                    const bool in = e - kHalfLow <= kHalfHigh - kHalfLow;
-                    h = in ? h : 0u;
-                    out = out || !(in || e == 255u);
-                }
-                *reinterpret_cast<uint16_t *>(t + x * (2 * kRound)) = static_cast<uint16_t>(h);
+        for (int u = 0; u < 2; ++u) g.o[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ro, oo + u * o32, 0, 0));
+        g.s = buf_load4(make_rsrc(nx.s, static_cast<uint32_t>(nx.sb)), so);
+        nx.k += kstep, nx.o += ostep, nx.s += sstep;
+        nx.kb = max(nx.kb - static_cast<int>(kstep), 0), nx.ob = max(nx.ob - static_cast<int>(ostep), 0), nx.sb = max(nx.sb - static_cast<int>(sstep), 0);
+    };
+    auto store = [&](const Stage &g, int rd) __attribute__((always_inline)) {
+        char *k = kbuf + rd % kSlots * kKBytes, *o = rbuf + (rd & 1) * kRBytes + orow * kRLd + ochunk * 16;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) *reinterpret_cast<u32x4 *>(k + (16 * u + srow) * kKLd + sgrp * 16) = g.k[u];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) *reinterpret_cast<u32x4 *>(o + 32 * u * kRLd) = g.o[u];
+        *reinterpret_cast<uint32_t *>(k + brow * kKLd + 256 + bquad * 4) = g.s;
+    };
+    // Of round rd's scale bytes a second form, by the score waves: 2^(byte - 127) in 16 bits, [group][position], for the context
+    // waves (a NaN's is zero).
+    auto scales = [&](int rd, auto bf) __attribute__((always_inline)) {
+        const uint32_t four = *reinterpret_cast<const uint32_t *>(kbuf + rd % kSlots * kKBytes + brow * kKLd + 256 + bquad * 4);
+        char *t = tbuf + rd % kSlots * kTBytes + bquad * 4 * (2 * kRound) + 2 * brow;
+        bool out = false;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const uint32_t e = (four >> (8 * x)) & 255u;
+            uint32_t h;
+            if constexpr (decltype(bf)::value) {
+                h = e == 255u ? 0u : e == 0u ? 64u : e << 7;          // bf16; 2^-127 is a subnormal
+            } else {
+                const bool in = e - kHalfLow <= kHalfHigh - kHalfLow;
+                h = in ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(__uint_as_float(e << 23))) : 0u;
+                out = out || !(in || e == 255u);
             }
-            if (out && rd * kRound + brow < n) wide = 1;
+            *reinterpret_cast<uint16_t *>(t + x * (2 * kRound)) = static_cast<uint16_t>(h);
         }
+        if (out && rd * kRound + brow < n) wide = 1;
     };
     if (tid == 0) wide = 0;
+    // Iterations 0 .. nr - 1 + kLag, a multiple of kAhead (rounds past the last are zeros that no row sees).  A round is loaded kAhead
+    // iterations before it is stored: its rows take about 2 us to come, two rounds ahead held a 16-row block to 0.92 us a round.
+    // (More rows: their accumulators leave the registers for fewer, and their iterations are longer.)
+    constexpr int kAhead = RG == 4 ? 1 : RG == 2 ? 2 : 4;
+    const int iters = (nr + kLag + kAhead - 1) / kAhead * kAhead;
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
-    // Iterations 0 .. nr - 1 + kLag: store round i + 1 (loaded two iterations before; 64 rows, whose accumulators leave few registers
-    // and whose iterations are long: one), load the one after next, and the role's part.  With two rounds in registers their
-    // number is even (rounds past the last are zeros that no row sees).
-    auto rounds = [&](auto bf, auto part) __attribute__((always_inline)) {
-        Stage g[kLag];
-        load(g[0], 0);
-        if (kLag > 1) load(g[kLag - 1], 1);
-        __syncthreads();        // wide is clear; every wave is done with a first pass
-        store(g[0], 0, bf);
-        load(g[0], kLag);
-        __syncthreads();
-        if constexpr (kLag == 1) {
-            for (int i = 0; i < nr + 1; ++i) {
-                store(g[0], i + 1, bf);
-                load(g[0], i + 2);
-                part(i, even);
-                __syncthreads();
-            }
-        } else {
-            for (int i = 0; i < nr + 2; i += 2) {
-                store(g[1], i + 1, bf);
-                load(g[1], i + 3);
-                part(i, even);
-                __syncthreads();
-                store(g[0], i + 2, bf);
-                load(g[0], i + 4);
-                part(i + 1, odd);
-                __syncthreads();
-            }
-        }
-    };
     if (wave < 4) {
         // ================= score waves
         const int rg = wave % RG, tg = wave / RG;
@@ -417,6 +401,9 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 u32x4 kc[kQ4Steps];
 #pragma unroll
                 for (int s = 0; s < kQ4Steps; ++s) kc[s] = *reinterpret_cast<const u32x4 *>(k + q4 * 64 + s * 16);
+                u32x4 oc[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) oc[x] = *reinterpret_cast<const u32x4 *>(o + x * 64);
                 f32x4 d[4];                                 // the terms in chains of their own
 #pragma unroll
                 for (int x = 0; x < 4; ++x) d[x] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -424,7 +411,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
                     for (int x = RT - 1; x >= 0; --x)
-                        d[3] = q4_mfma_bf16(*reinterpret_cast<const u32x4 *>(o + s * 64), *reinterpret_cast<const u32x4 *>(qr + (2 * x + s) * 1024), d[3]);
+                        d[3] = q4_mfma_bf16(oc[s], *reinterpret_cast<const u32x4 *>(qr + (2 * x + s) * 1024), d[3]);
 #pragma unroll
                 for (int x = NT - 1; x >= 0; --x) {
                     f32x4 &c = d[x < 3 ? x : 3];
@@ -487,7 +474,14 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         };
         auto all = [&](auto bf) __attribute__((always_inline)) {
             m_ref = -INFINITY, l_run = 0.f;
-            rounds(bf, [&](int i, auto par) __attribute__((always_inline)) {
+            // the context waves' first kLag iterations, before there is a round for them, take zero scales and zero probabilities (a
+            // branch around the products would cost a copy of the accumulators)
+            for (int i = tid * 16; i < 2 * RG * kPLd; i += 256 * 16) *reinterpret_cast<u32x4 *>(pbuf + i) = u32x4{0u, 0u, 0u, 0u};
+            for (int i = tid * 16; i < kLag * kTBytes; i += 256 * 16) *reinterpret_cast<u32x4 *>(tbuf + (kSlots - kLag) * kTBytes + i) = u32x4{0u, 0u, 0u, 0u};
+            if (tid < 2 * RG * 16) xf[tid / (RG * 16)][tid % (RG * 16)] = 1.f;
+            __syncthreads();        // all this and wide are set; every wave is done with a first pass
+            __syncthreads();        // round 0 is staged
+            auto part = [&](int i, auto par) __attribute__((always_inline)) {
                 constexpr int d = decltype(par)::value;
                 if constexpr (kLag == 1) {
                     mt[0] = scores(i, sc[0]);
@@ -502,7 +496,17 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                         probs(i - 1, sc[kLag - 1 - d], m, bf);
                     }
                 }
-            });
+                scales(i, bf);
+                __syncthreads();
+            };
+            if constexpr (kLag == 1) {
+                for (int i = 0; i < iters; ++i) part(i, even);
+            } else {
+                for (int i = 0; i < iters; i += 2) {
+                    part(i, even);
+                    part(i + 1, odd);
+                }
+            }
         };
         all(std::false_type{});
         if (__builtin_amdgcn_readfirstlane(wide)) all(std::true_type{});
@@ -519,12 +523,13 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         // ================= context waves: columns 128 (wave - 4) .. +128
         const int col0 = (wave - 4) * 128;
         f32x4 acc[8][RG];
-        auto context = [&](int rd, auto bf) __attribute__((always_inline)) {
+        auto context = [&](int rd, auto bf, auto stage) __attribute__((always_inline)) {
             constexpr bool kBf = decltype(bf)::value;
             constexpr int N = PT + kBf;
             // lane (column r16, positions 16 q4 .. +16): the codes of a tile of 16 columns, transposed, as they lie in the rows
-            const char *k = kbuf + rd % kSlots * kKBytes + (16 * q4 + r16) * kKLd + col0 / 2;
-            const char *t = tbuf + rd % kSlots * kTBytes + (col0 / 32) * (2 * kRound) + 32 * q4;
+            const int slot = (rd + kSlots) % kSlots;
+            const char *k = kbuf + slot * kKBytes + (16 * q4 + r16) * kKLd + col0 / 2;
+            const char *t = tbuf + slot * kTBytes + (col0 / 32) * (2 * kRound) + 32 * q4;
             const char *p = pbuf + (rd & 1) * RG * kPLd + (q4 * 32 + r16) * 16;
             u32x2 code[8];
 #pragma unroll
@@ -532,6 +537,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 code[c] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i2)(k + c * 8)));
             float f[RG];
             bool any = false;
+            stage();
 #pragma unroll
             for (int r = 0; r < RG; ++r) {
                 f[r] = xf[rd & 1][r * 16 + r16];
@@ -570,9 +576,24 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
             for (int c = 0; c < 8; ++c)
 #pragma unroll
                 for (int r = 0; r < RG; ++r) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-            rounds(bf, [&](int i, auto) __attribute__((always_inline)) {
-                if (i >= kLag) context(i - kLag, bf);
-            });
+            Stage g[kAhead];
+            rewind();
+#pragma unroll
+            for (int d = 0; d < kAhead; ++d) load(g[d]);
+            __syncthreads();
+            store(g[0], 0);
+            load(g[0]);
+            __syncthreads();
+            for (int i = 0; i < iters; i += kAhead) {
+#pragma unroll
+                for (int d = 0; d < kAhead; ++d) {
+                    context(i + d - kLag, bf, [&]() __attribute__((always_inline)) {
+                        store(g[(d + 1) % kAhead], i + d + 1);
+                        load(g[(d + 1) % kAhead]);
+                    });
+                    __syncthreads();
+                }
+            }
         };
         all(std::false_type{});
         if (__builtin_amdgcn_readfirstlane(wide)) all(std::true_type{});
@@ -1152,7 +1173,7 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
     const Plan p = plan_of(B, T, H, v_dim, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weight != nullptr, lengths != nullptr);
     if (workspace_bytes < p.total)
         return set_error(K3_ERR_WORKSPACE, "mla q4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.total);
-    if (static_cast<int64_t>(p.Ts) * std::max(p_row, 2 * rot_row) >= (1ll << 31))
+    if (static_cast<int64_t>(p.Ts) * std::max({p_row, s_row, 2 * rot_row}) >= (1ll << 31))
         return set_error(K3_ERR_SHAPE, "mla q4: a split of %d positions spans 2 GiB", p.Ts);
     auto st = static_cast<hipStream_t>(stream);
     char *ws = static_cast<char *>(workspace);
