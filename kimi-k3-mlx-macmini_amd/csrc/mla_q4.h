@@ -12,9 +12,9 @@
 // Each term rounds what is left to nearest; E2M3's step below 4 is at most 1/4, so a term leaves at most
 // 1/8 of its unit (the first, up to 7.5: 1/4): 2^-12 s after three terms, 2^-22 s after five, where the group's
 // largest magnitude is above 3.75 s.  Three (2^-14 of the largest at worst) are taken where the result is rounded to
-// bf16 (2^-8), five where it is fp32 or the weights are summed.  E2M1 x E2M3 products run at four times bf16's rate (measured: 4128 against
-// 1107 TFLOP/s), so five terms cost 1.25 bf16 products and need no decoded keys; two bf16 terms (2^-17) would cost
-// two products and the decoding.  The rotary columns are bf16 on both sides: bf16 queries are one term, fp32 ones two or three.
+// bf16 (2^-8), five where it is fp32 or the weights are summed.  An E2M1 x E2M3 product
+// of 16 x 16 x 128 takes the time of a bf16 one of 16 x 16 x 32 (19.5 against 18 cycles in a dependent chain), so five terms cost
+// 1.25 bf16 products and need no decoded keys; two bf16 terms (2^-17) would cost two products and the decoding.  The rotary columns are bf16 on both sides: bf16 queries are one term, fp32 ones two or three.
 //
 // Values.  The second product's operands are fp16: E2M1 times 2^-23 .. 2^13 (scale bytes 104 .. 140) is exact in it,
 // and its 11 bits make one term of a probability enough for a bf16 result (2^-11 each, independent, below the

@@ -358,9 +358,8 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     };
     if (tid == 0) wide = 0;
     // Iterations 0 .. nr - 1 + kLag, a multiple of kAhead (rounds past the last are zeros that no row sees).  A round is loaded kAhead
-    // iterations before it is stored: its rows take about 2 us to come, two rounds ahead held a 16-row block to 0.92 us a round.
-    // (More rows: their accumulators leave the registers for fewer, and their iterations are longer.)
-    constexpr int kAhead = RG == 4 ? 1 : RG == 2 ? 2 : 4;
+    // iterations before it is stored (four measured no better than two; 64 rows leave the registers for one).
+    constexpr int kAhead = RG == 4 ? 1 : 2;
     const int iters = (nr + kLag + kAhead - 1) / kAhead * kAhead;
     constexpr std::integral_constant<int, 0> even{};
     constexpr std::integral_constant<int, 1> odd{};
@@ -674,96 +673,129 @@ __device__ __forceinline__ void record_weights(const UvArgs &a, int b, int row, 
     if (a.stats && lane == 0) a.stats[static_cast<int64_t>(b) * a.rows + row] = make_float2(mx - kLift, inv);
 }
 
-// Few queries: grid (H, ceil(M / 16)), eight waves, queries 16 y .. +16 of head x.  A wave joins the records of its 64 latent columns
-// (16 lanes x 4 columns, four splits at a time) and multiplies them with its columns of W_UV (loaded first of all); the
-// waves' products are added in order.  Bound by the latency of the records (NS x 2 KB a query) and of W_UV, 128 KB a head.
-// One launch: blocks of 128 columns each and a launch that added their products took 14 us at 64 heads and 128 ranges, this takes 16 (and 9 for 12.5 with one range).
-constexpr int kXLd = 68, kDLd = 132;        // floats of a staged context row (64 columns), of a product row (128)
-constexpr int few_lds(int NS) { return (8 * 16 * kXLd + 8 * 16 * kDLd + 16 * NS) * 4; }
+// Few queries: grid (H, ceil(M / per), Z), WAVES waves, queries per y .. +per (at most 16) of head x, VT tiles of 16 output columns
+// (z).  A wave joins the records of its 512 / WAVES latent columns (4 to a lane, 64 / kLanes splits at a time) and multiplies them with
+// its columns of W_UV (loaded first of all); the waves' products are added in order.  Bound by the latency of the records (NS x 2 KB a
+// query) and of W_UV, 128 KB a head.
+//   many records: 16 waves have 128 KB of them on the way (10.0 us at 128 splits of 64 heads; 8 waves, 64 KB: 16)
+//   up to kFewSplits: 8 waves with half of the output columns each (6.5 us at 6 splits of 96 heads; 16 waves, all columns: 10.0)
+constexpr int kDLd = 132;                   // floats of a product row (128)
+constexpr int kFewSplits = 8;
+constexpr int few_lds(int waves, int NS) { return (16 * (512 + 4 * waves) + 8 * 16 * kDLd + 16 * NS) * 4; }
 
-__global__ __launch_bounds__(512, 1) void uv_few_kernel(UvArgs a) {
+template <int WAVES, int VT>
+__global__ __launch_bounds__(64 * WAVES, 1) void uv_few_kernel(UvArgs a, int per) {
+    constexpr int kCols = 512 / WAVES, kLanes = kCols / 4, kPar = 64 / kLanes, kSteps = kCols / 32, kXLd = kCols + 4;
     extern __shared__ __attribute__((aligned(16))) float sm[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
-    float *const x = sm + wave * 16 * kXLd, *const d = sm + 8 * 16 * kXLd, *const wsp = d + 8 * 16 * kDLd;
-    const int h = blockIdx.x, m0 = blockIdx.y * 16, col0 = wave * 64, nv = min(16, a.M - m0);
-    auto weights_of = [&](int v0, u32x4 (&w)[8][2]) __attribute__((always_inline)) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
+    const int cl = lane % kLanes, sl = lane / kLanes;
+    float *const x = sm + wave * 16 * kXLd, *const d = sm + WAVES * 16 * kXLd, *const wsp = d + 8 * 16 * kDLd;
+    const int h = blockIdx.x, m0 = blockIdx.y * per, col0 = wave * kCols, nv = min(per, a.M - m0);
+    auto weights_of = [&](int v0, u32x4 (&w)[VT][kSteps]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
+        for (int t = 0; t < VT; ++t) {
             const int v = v0 + t * 16 + r16;
             const uint16_t *wr = a.w_uv + (static_cast<int64_t>(h) * a.V + v) * kQ4Lat + col0 + 8 * q4;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) w[t][k] = v < a.V ? *reinterpret_cast<const u32x4 *>(wr + k * 32) : u32x4{0u, 0u, 0u, 0u};
+            for (int k = 0; k < kSteps; ++k) w[t][k] = v < a.V ? *reinterpret_cast<const u32x4 *>(wr + 32 * k) : u32x4{0u, 0u, 0u, 0u};
         }
     };
-    u32x4 w[8][2];
-    weights_of(0, w);
-    constexpr int kBatch = 8;
+    u32x4 w[VT][kSteps];
+    const int vz = blockIdx.z * 16 * VT;
+    weights_of(vz, w);
+    constexpr int kBatch = WAVES == 16 ? 7 : 8;     // (in registers, beside the weights)
+    // (a pass's records are at most 2^16 rows, so 2^27 bytes)
+    const uint32_t pitch = static_cast<uint32_t>(a.rows) * kQ4Lat;
     auto record = [&](int i) __attribute__((always_inline)) {
         const int m = m0 + i, b = m / a.order.T, row = a.order.of(m % a.order.T, h);
-        return a.part + (static_cast<int64_t>(b) * a.NS * a.rows + row) * kQ4Lat + col0 + 4 * r16;
+        return static_cast<uint32_t>(b * a.NS) * pitch + static_cast<uint32_t>(row * kQ4Lat + col0);
     };
-    const int64_t pitch = static_cast<int64_t>(a.rows) * kQ4Lat;
-    f32x4 first[kBatch];                    // the first query's first records: in bounds, whether there is one or not
+    // the next records to add: in bounds, whether they were written or not (a split that the row sees nothing of has none)
+    auto load = [&](int i, int j, f32x4 (&y)[kBatch]) __attribute__((always_inline)) {
+        const float *src = a.part + record(min(i, nv - 1));
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) first[u] = *reinterpret_cast<const f32x4 *>(record(0) + min(q4 + 4 * u, a.NS - 1) * pitch);
-    for (int i = wave; i < nv; i += 8) {
+        for (int u = 0; u < kBatch; ++u) {
+            if (u > 0 && j + kPar * u >= a.NS) break;       // (the same for all lanes)
+            y[u] = *reinterpret_cast<const f32x4 *>(src + (static_cast<uint32_t>(min(j + kPar * u + sl, a.NS - 1)) * pitch + 4u * cl));
+        }
+    };
+    f32x4 y[kBatch];
+    load(0, 0, y);
+    for (int i = wave; i < nv; i += WAVES) {
         const int m = m0 + i;
         record_weights(a, m / a.order.T, a.order.of(m % a.order.T, h), wsp + i * a.NS);
     }
     __syncthreads();
     for (int i = 0; i < nv; ++i) {
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
-        const float *src = record(i), *ws = wsp + i * a.NS;
-        for (int j = q4; j < a.NS; j += 4 * kBatch) {
-            f32x4 y[kBatch];
-            float f[kBatch];
+        for (int j = 0; j < a.NS; j += kPar * kBatch) {
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
-                const int k = j + 4 * u;
-                f[u] = k < a.NS ? ws[k] : 0.f;
-                if (i == 0 && j < 4)
-                    y[u] = first[u];
-                else if (f[u] != 0.f)
-                    y[u] = *reinterpret_cast<const f32x4 *>(src + k * pitch);
-                if (f[u] == 0.f) y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (u > 0 && j + kPar * u >= a.NS) break;
+                const int k = j + kPar * u + sl;
+                const float f = k < a.NS ? wsp[i * a.NS + k] : 0.f;
+                if (f == 0.f) y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                s += y[u] * f;
             }
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) s += y[u] * f[u];
+            if (j + kPar * kBatch < a.NS)
+                load(i, j + kPar * kBatch, y);
+            else if (i + 1 < nv)
+                load(i + 1, 0, y);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] = q4_rows_sum(s[k]);
-        if (q4 == 0) *reinterpret_cast<f32x4 *>(x + i * kXLd + 4 * r16) = s;
+        for (int k = 0; k < 4; ++k) {       // the lanes of a column group, in a fixed order
+            s[k] = q4_rows_sum(s[k]);
+            if (kLanes == 8) s[k] += __shfl_xor(s[k], 8);
+        }
+        if (sl == 0) *reinterpret_cast<f32x4 *>(x + i * kXLd + 4 * cl) = s;
     }
-    for (int i = nv + q4; i < 16; i += 4) *reinterpret_cast<f32x4 *>(x + i * kXLd + 4 * r16) = f32x4{0.f, 0.f, 0.f, 0.f};
-    u32x4 cf[2][3];                         // (a wave's own rows: its LDS accesses are in order)
+    for (int i = nv + sl; i < 16; i += kPar) *reinterpret_cast<f32x4 *>(x + i * kXLd + 4 * cl) = f32x4{0.f, 0.f, 0.f, 0.f};
+    u32x4 cf[kSteps][3];                    // (a wave's own rows: its LDS accesses are in order)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const f32x4 y = *reinterpret_cast<const f32x4 *>(x + r16 * kXLd + k * 32 + 8 * q4);
-        const f32x4 z = *reinterpret_cast<const f32x4 *>(x + r16 * kXLd + k * 32 + 8 * q4 + 4);
-        const float v[8] = {y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]};
+    for (int k = 0; k < kSteps; ++k) {
+        const float *xr = x + r16 * kXLd + 32 * k + 8 * q4;
+        const f32x4 u = *reinterpret_cast<const f32x4 *>(xr), z = *reinterpret_cast<const f32x4 *>(xr + 4);
+        const float v[8] = {u[0], u[1], u[2], u[3], z[0], z[1], z[2], z[3]};
         terms8(v, cf[k]);
     }
-    for (int v0 = 0; v0 < a.V; v0 += 128) {
-        if (v0) {
+    float *const dw = d + ((wave & 7) * 16 + r16) * kDLd + 4 * q4;
+    for (int v0 = vz; v0 < a.V; v0 += 16 * VT * gridDim.z) {
+        if (v0 != vz) {
             weights_of(v0, w);
             __syncthreads();                // the last products are added up
         }
+        f32x4 o[VT];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < VT; ++t) {
+            o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int y = 2; y >= 0; --y)
+            for (int k = 2; k >= 0; --k)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) o = q4_mfma_bf16(w[t][k], cf[k][y], o);
-            *reinterpret_cast<f32x4 *>(d + (wave * 16 + r16) * kDLd + t * 16 + 4 * q4) = o;
+                for (int c = 0; c < kSteps; ++c) o[t] = q4_mfma_bf16(w[t][c], cf[c][k], o[t]);
+        }
+        if (WAVES == 16) {
+            if (wave >= 8) {
+#pragma unroll
+                for (int t = 0; t < VT; ++t) *reinterpret_cast<f32x4 *>(dw + t * 16) = o[t];
+            }
+            __syncthreads();
+            if (wave < 8) {
+#pragma unroll
+                for (int t = 0; t < VT; ++t) *reinterpret_cast<f32x4 *>(dw + t * 16) = o[t] + *reinterpret_cast<const f32x4 *>(dw + t * 16);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < VT; ++t) *reinterpret_cast<f32x4 *>(dw + t * 16) = o[t];
         }
         __syncthreads();
-        const int i = tid >> 5, v = (tid & 31) * 4;
-        if (i < nv && v0 + v < a.V) {
-            f32x4 o = *reinterpret_cast<const f32x4 *>(d + i * kDLd + v);
+        for (int j = tid; j < 16 * 4 * VT; j += 64 * WAVES) {
+            const int i = j / (4 * VT), v = j % (4 * VT) * 4;
+            if (i < nv && v0 + v < a.V) {
+                f32x4 t = *reinterpret_cast<const f32x4 *>(d + i * kDLd + v);
 #pragma unroll
-            for (int u = 1; u < 8; ++u) o += *reinterpret_cast<const f32x4 *>(d + (u * 16 + i) * kDLd + v);
-            store_out4(a, m0 + i, h, v0 + v, o);
+                for (int u = 1; u < 8; ++u) t += *reinterpret_cast<const f32x4 *>(d + (u * 16 + i) * kDLd + v);
+                store_out4(a, m0 + i, h, v0 + v, t);
+            }
         }
     }
 }
@@ -772,7 +804,7 @@ __global__ __launch_bounds__(512, 1) void uv_few_kernel(UvArgs a) {
 // the records of 4 columns of 8 queries and leaves them in LDS as TERMS bf16 terms (two, 2^-17, for a bf16 result); a wave
 // takes 32 of 128 output columns for all 64 queries.  Bound by reading the records.
 template <int TERMS>
-__global__ __launch_bounds__(256) void uv_many_kernel(UvArgs a) {
+__global__ __launch_bounds__(256, 2) void uv_many_kernel(UvArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int kLd = 272, kTerm = 64 * kLd;      // bytes: 128 columns + 16
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
@@ -783,8 +815,14 @@ __global__ __launch_bounds__(256) void uv_many_kernel(UvArgs a) {
         record_weights(a, m / a.order.T, a.order.of(m % a.order.T, h), wsp + i * a.NS);
     }
     __syncthreads();
-    const int64_t pitch = static_cast<int64_t>(a.rows) * kQ4Lat;
+    const uint32_t pitch = static_cast<uint32_t>(a.rows) * kQ4Lat;
     const int c4 = tid & 31, i8 = tid >> 5;
+    uint32_t at[8];     // (a pass's records are at most 2^16 rows, so 2^27 bytes)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int m = m0 + min(8 * u + i8, nv - 1);
+        at[u] = static_cast<uint32_t>(m / a.order.T * a.NS) * pitch + static_cast<uint32_t>(a.order.of(m % a.order.T, h) * kQ4Lat + 4 * c4);
+    }
     for (int v0 = 0; v0 < a.V; v0 += 128) {
         f32x4 acc[2][4];
 #pragma unroll
@@ -804,14 +842,18 @@ __global__ __launch_bounds__(256) void uv_many_kernel(UvArgs a) {
             f32x4 s[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
             for (int k = 0; k < a.NS; ++k) {
+                // (in bounds, whether the record was written or not: its weight is zero where it was not)
+                f32x4 y[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) y[u] = *reinterpret_cast<const f32x4 *>(a.part + (at[u] + k * pitch + col0));
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
-                    const int i = 8 * u + i8, m = m0 + i;
+                    const int i = 8 * u + i8;
                     const float f = i < nv ? wsp[i * a.NS + k] : 0.f;
-                    if (f != 0.f)
-                        s[u] += f * *reinterpret_cast<const f32x4 *>(a.part + (static_cast<int64_t>(m / a.order.T) * a.NS + k) * pitch +
-                                                                    static_cast<int64_t>(a.order.of(m % a.order.T, h)) * kQ4Lat + col0 + 4 * c4);
+                    if (f == 0.f) y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    s[u] += f * y[u];
                 }
             }
             __syncthreads();    // the last columns' operands are read
@@ -1036,13 +1078,18 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
     p.NT = fine ? 5 : 3, p.RT = q_bf16 ? 1 : fine ? 3 : 2, p.PT = out_bf16 ? 1 : 2;
     p.order = rows_of(std::max<int64_t>(1, std::min(T, kChunkRows / (B * H))), H);
     const int64_t rows = p.order.count();
-    p.RG = rows > 64 ? 4 : rows > 16 ? 2 : 1;
+    // Rows of a block.  A round costs 0.9 us at 16 rows, 1.1 at 32 and 1.8 at 64 (bf16 results; fp32 1.2, 1.6, 2.5), so more rows cost less
+    // each; but one block a CU is wanted, and a row's record of each range (2 KB) is written and read again, so few rows
+    // over a short cache take small blocks.  Measured, 64 heads, one token, us at 16 / 32 / 64 rows: 4096 positions 27.0 / 28.4 / 30.4,
+    // 32,768 34.1 / 35.8 / 38.2; 32 such sequences of up to 8192: 92 / 81 / 71; five tokens of 96 heads over 7001: 50 / 48 / 48.
+    p.RG = rows > 32 && B * cdiv(rows, 64) >= 8 ? 4 : rows > 16 && (npos > 32768 || B * cdiv(rows, 32) >= 8) ? 2 : 1;
     p.rblocks = static_cast<int>(cdiv(rows, 16 * p.RG));
     p.tiles = p.rblocks * p.RG;
     const int64_t base = B * p.rblocks;
-    // one block a CU; sequences of their own lengths: four, so the longest one's blocks are not what all wait for
-    int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (varied && B > 1 ? 1024 : 256) / base));
-    int64_t ts = cdiv(cdiv(std::max<int64_t>(npos, 1), ns), kRound) * kRound;
+    // One block a CU (sequences of their own lengths: half as many again, so the longest one's blocks are not what all wait
+    // for), and at least two rounds to a block: 4096 positions in ranges of 64 took 29.2 us for 27.0.
+    int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (varied && B > 1 ? 384 : 256) / base));
+    int64_t ts = std::max<int64_t>(2 * kRound, cdiv(cdiv(std::max<int64_t>(npos, 1), ns), kRound) * kRound);
     p.Ts = static_cast<int>(ts);
     p.NS = static_cast<int>(cdiv(std::max<int64_t>(npos, 1), ts));
     p.many = B * p.order.T >= kManyQueries;
@@ -1096,20 +1143,29 @@ int launch_qa(const QaArgs &a, hipStream_t st) {
 }
 
 int launch_uv(const UvArgs &a, int many, hipStream_t st) {
-    static const hipError_t few = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_few_kernel),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, few_lds(kMaxSplits));
+    static const hipError_t few16 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_few_kernel<16, 8>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, few_lds(16, kMaxSplits));
+    static const hipError_t few8 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_few_kernel<8, 4>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, few_lds(8, kFewSplits));
     static const hipError_t many2 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_many_kernel<2>),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 64 * 272 + 64 * kMaxSplits * 4);
     static const hipError_t many3 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_many_kernel<3>),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 3 * 64 * 272 + 64 * kMaxSplits * 4);
-    const int rc = check_hip(!many ? few : a.out_bf16 ? many2 : many3, "mla q4: output LDS size");
+    const int rc = check_hip(!many ? (few8 != hipSuccess ? few8 : few16) : a.out_bf16 ? many2 : many3, "mla q4: output LDS size");
     if (rc) return rc;
     const unsigned H = static_cast<unsigned>(a.order.H);
-    if (!many)
-        uv_few_kernel<<<dim3(H, static_cast<unsigned>(cdiv(a.M, 16))), 512, few_lds(a.NS), st>>>(a);
-    else if (a.out_bf16)
+    if (!many) {
+        int per = static_cast<int>(std::min<int64_t>(16, a.M));     // fewer queries to a block until there are two blocks a CU
+        while (per > 1 && H * cdiv(a.M, per) < 512) per = (per + 1) / 2;
+        const unsigned tiles = static_cast<unsigned>(cdiv(a.M, per));
+        if (a.NS <= kFewSplits)
+            uv_few_kernel<8, 4><<<dim3(H, tiles, 2), 512, few_lds(8, a.NS), st>>>(a, per);
+        else
+            uv_few_kernel<16, 8><<<dim3(H, tiles), 1024, few_lds(16, a.NS), st>>>(a, per);
+    }
+    if (many && a.out_bf16)
         uv_many_kernel<2><<<dim3(H, static_cast<unsigned>(cdiv(a.M, 64))), 256, 2 * 64 * 272 + 64 * a.NS * 4, st>>>(a);
-    else
+    else if (many)
         uv_many_kernel<3><<<dim3(H, static_cast<unsigned>(cdiv(a.M, 64))), 256, 3 * 64 * 272 + 64 * a.NS * 4, st>>>(a);
     return check_hip(hipGetLastError(), "mla q4: join and W_UV launch");
 }
