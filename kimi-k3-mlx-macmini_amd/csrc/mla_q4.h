@@ -6,15 +6,16 @@
 // Scores.  The matrix cores take the codes as they are: v_mfma_scale_f32_16x16x128_f8f6f4 reads an
 // E2M1 operand with one E8M0 byte per row and 32 columns, which is the cache's own layout: lane
 // (row r, quarter q) holds 16 bytes, group 4 q + s in step s of four (the order of a sum's columns is free, and
-// in this one the lane's four scale bytes are one dword of the row).  The absorbed query qa (fp32) enters as a sum of E2M3 terms (6 bits: 1 + 2 + 3) that share the other
-// operand's place, each with an E8M0 byte per 32 columns:
+// in this one the lane's four scale bytes are one dword of the row).  The absorbed query qa (fp32) enters as a sum of E2M3
+// terms (6 bits: 1 + 2 + 3) that share the other operand's place, each with an E8M0 byte per 32 columns:
 //     qa = t1 + t2 + t3 (+ t4 + t5),   |t1| <= 7.5 s, the next terms' units s / 16, s / 2^9, s / 2^14, s / 2^19
 // Each term rounds what is left to nearest; E2M3's step below 4 is at most 1/4, so a term leaves at most
 // 1/8 of its unit (the first, up to 7.5: 1/4): 2^-12 s after three terms, 2^-22 s after five, where the group's
 // largest magnitude is above 3.75 s.  Three (2^-14 of the largest at worst) are taken where the result is rounded to
-// bf16 (2^-8), five where it is fp32 or the weights are summed.  An E2M1 x E2M3 product
-// of 16 x 16 x 128 takes the time of a bf16 one of 16 x 16 x 32 (19.5 against 18 cycles in a dependent chain), so five terms cost
-// 1.25 bf16 products and need no decoded keys; two bf16 terms (2^-17) would cost two products and the decoding.  The rotary columns are bf16 on both sides: bf16 queries are one term, fp32 ones two or three.
+// bf16 (2^-8), five where it is fp32 or the weights are summed.  An E2M1 x E2M3 product of 16 x 16 x 128 takes the time of a bf16
+// one of 16 x 16 x 32 (19.5 against 18 cycles in a dependent chain), so five terms cost 1.25 bf16 products and need no decoded keys;
+// two bf16 terms (2^-17) would cost two products and the decoding.  The rotary columns are bf16 on both sides: bf16 queries are
+// one term, fp32 ones two or three.
 //
 // Values.  The second product's operands are fp16: E2M1 times 2^-23 .. 2^13 (scale bytes 104 .. 140) is exact in it,
 // and its 11 bits make one term of a probability enough for a bf16 result (2^-11 each, independent, below the

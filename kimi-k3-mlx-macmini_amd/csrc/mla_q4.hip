@@ -96,29 +96,26 @@ struct QueryRaw {
 };
 
 // grid (H, ceil(M / (16 MT)), 4): queries 16 MT y .. of head x, latent columns 128 z .. +128
-// MT 1: few queries, bound by the latency of reading W_UK once (every load in flight at once); MT 4: 64 queries to a
-// block's 32 KB of W_UK, bound by the terms' rounding (VALU) and by writing them.
+// MT 1: few queries, a wave to 32 of the columns; bound by the latency of reading W_UK once (every load in flight at once).
+// MT 4: 64 queries to a block's 32 KB of W_UK, a wave to 16 of them, whose bf16 terms it forms once for all columns; bound by the
+// 6-bit terms' rounding and by writing them.  (A wave to 32 columns of all 64 formed each query's terms four times: 87 us for
+// 1024 fp32 queries of 64 heads, 64 for 512; this: 56 and 44.)
 template <typename QT, int NT, int RT, int MT>
 __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float *fs = reinterpret_cast<float *>(lds);                         // [16 MT][kFLd], after the products
-    constexpr int kTerms = std::is_same<QT, float>::value ? 3 : 1, kAhead = MT == 1 ? 4 : 0;
+    constexpr int kTerms = std::is_same<QT, float>::value ? 3 : 1, kAhead = 4, kTiles = MT == 1 ? 2 : 8;    // column tiles of a wave
+    static_assert(MT == 1 || MT == 4, "a wave to 32 columns, or to a tile of queries");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
     const int h = blockIdx.x, m0 = blockIdx.y * 16 * MT, quarter = blockIdx.z;
     const int steps = (a.nope + 31) >> 5, T = a.rows.T;
     const uint16_t *w = a.w_uk + static_cast<int64_t>(h) * a.nope * kQ4Lat + quarter * 128;
-    const QT *q[MT];
-    bool live[MT];
+    const int qt = MT == 1 ? 0 : wave, col = MT == 1 ? wave * 32 : 0, mine = m0 + 16 * qt + r16;   // the wave's queries and columns
+    const bool live = mine < a.M;
+    const QT *q = static_cast<const QT *>(a.q_nope) + (live ? mine / T : 0) * a.n_b + (live ? a.t0 + mine % T : 0) * a.n_t + h * a.n_h + 4 * q4;
+    QueryRaw<QT> ahead[kAhead];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int m = m0 + 16 * i + r16;
-        live[i] = m < a.M;
-        const int b = live[i] ? m / T : 0, t = live[i] ? a.t0 + m % T : 0;
-        q[i] = static_cast<const QT *>(a.q_nope) + b * a.n_b + t * a.n_t + h * a.n_h + 4 * q4;
-    }
-    QueryRaw<QT> ahead[kAhead ? kAhead : 1];
-#pragma unroll
-    for (int s = 0; s < kAhead; ++s) ahead[s].load(q[0], 32 * s, a.nope - 4 * q4, live[0]);
+    for (int s = 0; s < kAhead; ++s) ahead[s].load(q, 32 * s, a.nope - 4 * q4, live);
     for (int i0 = 0; i0 < 2 * steps; i0 += 8) {
         uint4 v[8];
 #pragma unroll
@@ -132,45 +129,40 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
             if (n < 32 * steps) *reinterpret_cast<uint4 *>(lds + n * kWLd + (i & 15) * 16) = v[u];
         }
     }
-    f32x4 acc[2][MT];
+    f32x4 acc[kTiles];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[0][i] = acc[1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < kTiles; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     __syncthreads();
-    auto step = [&](int s, const QueryRaw<QT> (&raw)[MT]) __attribute__((always_inline)) {
-        const char *wr = lds + (32 * s + 4 * q4 + (r16 >> 2)) * kWLd + (r16 & 3) * 8 + wave * 64;
-        u32x4 wf[2];
+    auto step = [&](int s, const QueryRaw<QT> &raw) __attribute__((always_inline)) {
+        const char *wr = lds + (32 * s + 4 * q4 + (r16 >> 2)) * kWLd + (r16 & 3) * 8 + col * 2;
+        u32x4 qf[3];
+        raw.terms(qf);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + j * 32));
-            const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + j * 32 + 16 * kWLd));
-            wf[j] = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-        }
+        for (int j0 = 0; j0 < kTiles; j0 += 2) {
+            u32x4 wf[2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            u32x4 qf[3];
-            raw[i].terms(qf);
+            for (int j = 0; j < 2; ++j) {
+                const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + (j0 + j) * 32));
+                const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + (j0 + j) * 32 + 16 * kWLd));
+                wf[j] = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
 #pragma unroll
             for (int k = kTerms - 1; k >= 0; --k)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[j][i] = q4_mfma_bf16(wf[j], qf[k], acc[j][i]);
+                for (int j = 0; j < 2; ++j) acc[j0 + j] = q4_mfma_bf16(wf[j], qf[k], acc[j0 + j]);
         }
     };
-    if constexpr (MT == 1) {
 #pragma unroll
-        for (int s = 0; s < kAhead; ++s)
-            if (s < steps) step(s, {ahead[s]});
-    }
+    for (int s = 0; s < kAhead; ++s)
+        if (s < steps) step(s, ahead[s]);
     for (int s = kAhead; s < steps; ++s) {
-        QueryRaw<QT> raw[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) raw[i].load(q[i], 32 * s, a.nope - 4 * q4, live[i]);
+        QueryRaw<QT> raw;
+        raw.load(q, 32 * s, a.nope - 4 * q4, live);
         step(s, raw);
     }
     __syncthreads();   // the weights are read
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) *reinterpret_cast<f32x4 *>(fs + (16 * i + r16) * kFLd + wave * 32 + j * 16 + 4 * q4) = acc[j][i];
+    for (int j = 0; j < kTiles; ++j) *reinterpret_cast<f32x4 *>(fs + (16 * qt + r16) * kFLd + col + j * 16 + 4 * q4) = acc[j];
     __syncthreads();
     if (tid < 64 * MT && m0 + (tid >> 2) < a.M) {
         // one group of 32 columns of one query: its terms
