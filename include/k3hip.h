@@ -466,7 +466,8 @@ int k3_mla_step_decode(const void *x, int x_dtype, const void *q_a, const float 
  * k3_mla_q4_append rounds new latents c [B, T, 512] and rotary rows r [B, T, 64] (each bf16 or fp32,
  * pitches in elements) into positions start[b] + i, i < counts[b] <= T, of sequence b.
  * start: int32 [B] on the device, or null: start0 for all (then start0 + T <= cap is checked here);
- * counts: int32 [B] on the device, or null: T.  Positions outside 0 .. cap - 1 are left out.
+ * counts: int32 [B] on the device, or null: T.  Positions outside 0 .. cap - 1 are left out.  weight, if not null: fp32
+ * rows w_batch floats apart, the attention that positions have received, zeroed where a position is written.
  * A group of 32 with largest magnitude m gets the scale 2^e, e = floor(log2 m) - 2, one more if
  * m > 7 * 2^e, its byte e + 127 held to 2..252; codes round to nearest, ties to even.  A group of
  * zeros gets byte 127, one with a NaN or an infinity 255: the position is NaN to every query that sees it.
@@ -474,8 +475,8 @@ int k3_mla_step_decode(const void *x, int x_dtype, const void *q_a, const float 
 int k3_mla_q4_append(const void *c, int64_t c_batch, int64_t c_row, int c_dtype, const void *r, int64_t r_batch,
                      int64_t r_row, int r_dtype, void *packed, int64_t p_batch, int64_t p_row, void *scales,
                      int64_t s_batch, int64_t s_row, void *rot, int64_t rot_batch, int64_t rot_row,
-                     const int32_t *start, int64_t start0, const int32_t *counts, int64_t B, int64_t T, int64_t cap,
-                     int64_t kv_lora_rank, int64_t rope_dim, void *stream);
+                     const int32_t *start, int64_t start0, const int32_t *counts, float *weight, int64_t w_batch,
+                     int64_t B, int64_t T, int64_t cap, int64_t kv_lora_rank, int64_t rope_dim, void *stream);
 
 /* Workspace bytes of k3_mla_q4_attention for the same sizes (weights: whether it is given a weight
  * buffer; varied: whether it is given lengths).  No initialisation. */
@@ -508,6 +509,22 @@ int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t qn_token, 
                         int64_t kv_lora_rank, int64_t rope_dim, int64_t nope_dim, int64_t v_dim, float scale,
                         const float *gate, void *out, int out_dtype, float *weight, int64_t w_batch, void *workspace,
                         int64_t workspace_bytes, void *stream);
+
+/* Workspace bytes k3_mla_step_decode_q4 needs for T = pos + 1 cache rows (weights: 1 if they are summed). */
+int64_t k3_mla_step_q4_workspace_size(int64_t q_lora_rank, int64_t heads, int64_t nope_dim, int64_t rope_dim, int64_t v_dim,
+                                      int64_t kv_lora_rank, int64_t T, int weights);
+
+/* k3_mla_step_decode over the 4-bit cache: row pos gets rmsnorm(ckv[:r], kv_a_norm) as k3_mla_q4_append rounds it
+ * and bf16(ckv[r:]); the core is k3_mla_q4_attention's over rows 0..pos.  packed, scales, rot: one sequence's
+ * cache_rows rows, pitches in elements (packed and rot rows whole 16 bytes); weight: fp32 [cache_rows], to which the step's
+ * attention weights are added (row pos starts at zero), or null.  kv_lora_rank 512, rope_dim 64, nope_dim and v_dim multiples of 8 up to 256 and 1024; the
+ * rest as there. */
+int k3_mla_step_decode_q4(const void *x, int x_dtype, const void *q_a, const float *q_a_norm, const void *q_b, const void *kv_a,
+                          const float *kv_a_norm, const void *w_uk, const void *w_uv, const void *g_proj, const void *o_proj,
+                          void *packed, int64_t p_row, void *scales, int64_t s_row, void *rot, int64_t rot_row, float *weight,
+                          int64_t cache_rows, int64_t pos, float eps, float scale, void *out, int out_dtype, int64_t hidden,
+                          int64_t q_lora_rank, int64_t heads, int64_t nope_dim, int64_t rope_dim, int64_t v_dim,
+                          int64_t kv_lora_rank, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* ---- eviction by accumulated attention weight --------------------------------------------- */
 

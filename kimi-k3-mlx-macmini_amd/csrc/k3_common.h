@@ -30,6 +30,12 @@ int mla_decode_core(const void *q_nope, const void *q_rot, int64_t ld_q, int64_t
                     int64_t v_dim, float scale, void *out, int out_dtype, int64_t ld_out, const float *gate,
                     void *workspace, int64_t workspace_bytes, void *stream, int cache_dtype = K3_BF16);
 
+// The launch of k3_mla_q4_append, arguments checked by the caller; with norm weights [512] the latents are RMS-normalised first.
+int mla_q4_append(const void *c, int64_t c_b, int64_t c_t, int c_dtype, const void *r, int64_t r_b, int64_t r_t, int r_dtype,
+                  const float *norm, float eps, void *packed, int64_t p_b, int64_t p_t, void *scales, int64_t s_b, int64_t s_t,
+                  void *rot, int64_t o_b, int64_t o_t, const int32_t *start, int64_t start0, const int32_t *counts,
+                  float *weight, int64_t w_b, int64_t B, int64_t T, int64_t cap, hipStream_t st);
+
 // The multi-token MLA attention's keys and values: every head's expansion of the latent cache,
 // as three bf16 terms.  tpad: the tokens rounded up to 32 (the added ones are zero).
 //   keys    [heads][tpad][3][128]

@@ -24,6 +24,8 @@ struct AppendArgs {
     int64_t p_b, p_t, s_b, s_t, o_b, o_t;  // elements of each buffer
     const int32_t *start, *counts;       // [B] or null
     int64_t start0;
+    float *weight;                       // [B] rows of w_b floats, or null: the written positions' is zeroed
+    int64_t w_b;
     const float *norm;                   // [512] or null
     float eps;
     int64_t T, cap;
@@ -81,6 +83,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[6], v[7], s, 3);
     }
     *reinterpret_cast<uint32_t *>(a.packed + b * a.p_b + at * a.p_t + lane * 4) = code;
+    if (a.weight && lane == 0) a.weight[b * a.w_b + at] = 0.f;
     if ((lane & 3) == 0) a.scales[b * a.s_b + at * a.s_t + (lane >> 2)] = static_cast<uint8_t>(byte);
     const RT *r = static_cast<const RT *>(a.r) + b * a.r_b + i * a.r_t + lane;
     uint16_t o;
@@ -95,10 +98,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 
 int mla_q4_append(const void *c, int64_t c_b, int64_t c_t, int c_dtype, const void *r, int64_t r_b, int64_t r_t, int r_dtype,
                   const float *norm, float eps, void *packed, int64_t p_b, int64_t p_t, void *scales, int64_t s_b, int64_t s_t,
-                  void *rot, int64_t o_b, int64_t o_t, const int32_t *start, int64_t start0, const int32_t *counts, int64_t B,
-                  int64_t T, int64_t cap, hipStream_t st) {
+                  void *rot, int64_t o_b, int64_t o_t, const int32_t *start, int64_t start0, const int32_t *counts,
+                  float *weight, int64_t w_b, int64_t B, int64_t T, int64_t cap, hipStream_t st) {
     const AppendArgs a{c,   r,   c_b, c_t, r_b, r_t,   static_cast<uint8_t *>(packed), static_cast<uint8_t *>(scales),
-                       static_cast<uint16_t *>(rot), p_b, p_t, s_b, s_t, o_b, o_t, start, counts, start0, norm, eps, T, cap};
+                       static_cast<uint16_t *>(rot), p_b, p_t, s_b, s_t, o_b, o_t, start, counts, start0, weight, w_b, norm, eps, T, cap};
     const dim3 grid(static_cast<unsigned>(cdiv(T, 4)), static_cast<unsigned>(B));
     if (c_dtype == K3_F32)
         r_dtype == K3_F32 ? append_kernel<float, float><<<grid, 256, 0, st>>>(a) : append_kernel<float, uint16_t><<<grid, 256, 0, st>>>(a);
@@ -115,8 +118,8 @@ using namespace k3;
 extern "C" int k3_mla_q4_append(const void *c, int64_t c_batch, int64_t c_row, int c_dtype, const void *r, int64_t r_batch,
                                 int64_t r_row, int r_dtype, void *packed, int64_t p_batch, int64_t p_row, void *scales,
                                 int64_t s_batch, int64_t s_row, void *rot, int64_t rot_batch, int64_t rot_row,
-                                const int32_t *start, int64_t start0, const int32_t *counts, int64_t B, int64_t T, int64_t cap,
-                                int64_t kv_lora_rank, int64_t rope_dim, void *stream) {
+                                const int32_t *start, int64_t start0, const int32_t *counts, float *weight, int64_t w_batch,
+                                int64_t B, int64_t T, int64_t cap, int64_t kv_lora_rank, int64_t rope_dim, void *stream) {
     if (B == 0 || T == 0) return K3_OK;
     if (!c || !r || !packed || !scales || !rot) return set_error(K3_ERR_NULL, "mla q4 append: null pointer");
     if ((c_dtype != K3_F32 && c_dtype != K3_BF16) || (r_dtype != K3_F32 && r_dtype != K3_BF16))
@@ -134,5 +137,5 @@ extern "C" int k3_mla_q4_append(const void *c, int64_t c_batch, int64_t c_row, i
     if (!aligned16(c) || (reinterpret_cast<uintptr_t>(packed) & 3u))
         return set_error(K3_ERR_ALIGN, "mla q4 append: c must be 16-byte and packed 4-byte aligned");
     return mla_q4_append(c, c_batch, c_row, c_dtype, r, r_batch, r_row, r_dtype, nullptr, 0.f, packed, p_batch, p_row, scales, s_batch,
-                         s_row, rot, rot_batch, rot_row, start, start0, counts, B, T, cap, static_cast<hipStream_t>(stream));
+                         s_row, rot, rot_batch, rot_row, start, start0, counts, weight, w_batch, B, T, cap, static_cast<hipStream_t>(stream));
 }

@@ -57,8 +57,11 @@ SIGNATURES: dict[str, list] = {
     "k3_mla_step_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64],
     "k3_mla_step_decode": [_P, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _F32,
                            _F32, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P],
+    "k3_mla_step_q4_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I32],
+    "k3_mla_step_decode_q4": [_P, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _F32, _F32,
+                              _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P],
     "k3_mla_q4_append": [_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64,
-                         _P, _I64, _I64, _I64, _I64, _I64, _P],
+                         _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P],
     "k3_mla_q4_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32],
     "k3_mla_q4_attention": [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I32, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64,
                             _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F32, _P, _P, _I32, _P, _I64, _P,
@@ -102,6 +105,7 @@ _RESTYPE = {"k3_last_error": ctypes.c_char_p, "k3_version": ctypes.c_char_p,
             "k3_mla_workspace_size": ctypes.c_int64,
             "k3_mla_step_workspace_size": ctypes.c_int64,
             "k3_mla_q4_workspace_size": ctypes.c_int64,
+            "k3_mla_step_q4_workspace_size": ctypes.c_int64,
             "k3_kda_step_workspace_size": ctypes.c_int64,
             "k3_mxfp4_matvec_launches": ctypes.c_int64,
             "k3_stream_capture_id": ctypes.c_int64,

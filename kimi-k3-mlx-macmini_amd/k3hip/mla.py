@@ -30,6 +30,13 @@ accepted: a decode token on it runs the HIP core on the fp32 rows
 (``k3_mla_decode_absorbed_f32``; with bf16 ``kv_b``, the checkpoint dtype, whose halves the
 core takes as they are), the projections around it in fp32; fp32 ``kv_b`` (validation mode)
 runs the fp32 masked form.
+
+``cfg.mla_cache_bits = 4`` (the reference's option, ``attention_mla.py:164-166``), or a caller's
+``k3hip.mla_q4.MLACacheQ4``, keeps the latents as MXFP4: a decode token runs ``k3_mla_step_decode_q4``, any
+other call ``k3_mla_q4_attention`` on the codes, for all sequences of a batch at once; fp32 ``kv_b`` takes the fp32
+masked form over the decoded latents, and calls that a gradient is asked of are refused.  ``cfg.mla_cache_weights``
+(not the reference's) makes a new cache of this kind sum the attention its positions receive, which ``MLACacheQ4.evict``
+goes by.
 """
 from __future__ import annotations
 
@@ -39,6 +46,7 @@ import torch
 
 from . import _blas, _lib, _workspace
 from . import _torch as T
+from .mla_q4 import MLACacheQ4, new_cache_q4
 
 CACHE_STEP = 256
 KV_LORA_RANK = 512
@@ -47,6 +55,11 @@ ROPE_DIM = 64
 
 def _round_up(n: int, step: int) -> int:
     return ((n + step - 1) // step) * step
+
+
+def grown_capacity(need: int, capacity: int) -> int:
+    """A full cache's next capacity: doubled, at least CACHE_STEP (attention_mla.py:93-101)."""
+    return _round_up(max(need, 2 * capacity, CACHE_STEP), CACHE_STEP)
 
 
 @dataclass
@@ -70,7 +83,7 @@ class MLACache:
         (attention_mla.py:93-101)."""
         need = self.length + n
         if need > self.capacity:
-            cap = _round_up(max(need, 2 * self.capacity, CACHE_STEP), CACHE_STEP)
+            cap = grown_capacity(need, self.capacity)
             self.latent = _grown(self.latent, cap, self.length)
             self.rot = _grown(self.rot, cap, self.length)
         return self
@@ -103,7 +116,7 @@ def _grown(buf: torch.Tensor, cap: int, keep: int) -> torch.Tensor:
 
 def new_cache(B: int, kv_lora_rank: int, rope: int, T: int, dtype=torch.bfloat16,
               device="cuda") -> MLACache:
-    """``_new_cache`` (attention_mla.py:127-134) without the quantised option."""
+    """``_new_cache`` (attention_mla.py:127-134); ``k3hip.mla_q4.new_cache_q4`` is its quantised option."""
     cap = _round_up(max(T, CACHE_STEP), CACHE_STEP)
     return MLACache(torch.zeros((B, cap, kv_lora_rank), dtype=dtype, device=device),
                     torch.zeros((B, cap, rope), dtype=dtype, device=device), 0)
@@ -227,9 +240,17 @@ class MLAAttention:
         kb32 = self.kv_b.to(torch.float32).reshape(nh, nope + cfg.v_head_dim, cfg.kv_lora_rank)
         self._wk32, self._wv32 = kb32[:, :nope, :], kb32[:, nope:, :]   # the fp32 form uses kv_b as given
         self.cache_dtype = getattr(cfg, "mla_cache_dtype", torch.bfloat16)
+        self.cache_bits = getattr(cfg, "mla_cache_bits", None)
+        if self.cache_bits not in (None, 0, 4, 16):
+            raise ValueError(f"mla_cache_bits {self.cache_bits}: the latent cache is held in 4 bits, or in mla_cache_dtype (None)")
+        if self.cache_bits == 4 and getattr(cfg, "mla_cache_group_size", None) not in (None, 32):
+            raise ValueError(f"mla_cache_group_size {cfg.mla_cache_group_size}: the 4-bit cache has a scale for every 32 values")
+        if self.cache_bits == 4 and (cfg.kv_lora_rank, cfg.qk_rope_head_dim) != (KV_LORA_RANK, ROPE_DIM):
+            raise ValueError(f"the 4-bit cache takes kv_lora_rank {KV_LORA_RANK} and qk_rope_head_dim {ROPE_DIM}; got "
+                             f"{cfg.kv_lora_rank}, {cfg.qk_rope_head_dim}")
         mats = [self.q_a, self.q_b, self.kv_a, self.o_w] + ([self.g_w] if self.g_w is not None else [])
         self.fused_step = (all(m.dtype == torch.bfloat16 and m.is_cuda for m in mats)
-                           and self.cache_dtype == torch.bfloat16
+                           and (self.cache_dtype == torch.bfloat16 or self.cache_bits == 4)
                            and cfg.kv_lora_rank == KV_LORA_RANK and cfg.qk_rope_head_dim == ROPE_DIM)
         if self.fused_step:
             self._mats = {k: T.contiguous_aligned(m) for k, m in
@@ -254,7 +275,14 @@ class MLAAttention:
     def __call__(self, x: torch.Tensor, cache: MLACache | None = None):
         c = self.cfg
         B, Tn, _ = x.shape
-        if self.fused_step and B == 1 and Tn == 1 and (cache is None or cache.latent.dtype == torch.bfloat16):
+        if cache is None and self.cache_bits == 4:
+            cache = new_cache_q4(B, Tn, bool(getattr(c, "mla_cache_weights", False)), x.device)
+        q4 = isinstance(cache, MLACacheQ4)
+        if q4 and T.tracked(x, self.q_a, self.q_an, self.q_b, self.kv_a, self.kv_an, self.kv_b, self.g_w, self.o_w):
+            raise ValueError("the 4-bit cache carries no gradient: call the layer under no_grad or on detached tensors")
+        if q4 and cache.weight is not None and self.kv_b.dtype != torch.bfloat16:
+            raise ValueError("the masked form (fp32 kv_b) sums no attention weights: the cache must keep none")
+        if self.fused_step and B == 1 and Tn == 1 and (cache is None or q4 or cache.latent.dtype == torch.bfloat16):
             return self.decode_step(x, cache)
         nh, qhd, vhd = c.num_attention_heads, c.q_head_dim, c.v_head_dim
         nope, rope, klr = c.qk_nope_head_dim, c.qk_rope_head_dim, c.kv_lora_rank
@@ -263,7 +291,7 @@ class MLAAttention:
         mats = [self.q_a, self.kv_a] + ([self.g_w] if gated else [])
         xf = x.reshape(B * Tn, x.shape[-1])
         # (a gradient or tangent of anything the call reads takes the tensor form throughout)
-        rest = [self.q_an, self.kv_an, self.kv_b] + ([] if cache is None else [cache.latent, cache.rot])
+        rest = [self.q_an, self.kv_an, self.kv_b] + ([] if cache is None else [cache.rot] if q4 else [cache.latent, cache.rot])
         if (B * Tn > 1 and _blas.dense_ok(xf, *mats) and _blas.weights_ok(self.q_b, self.o_w)
                 and not T.tracked(*rest)):
             qa, ckv, *g = _blas.project(xf, mats, checked=True)
@@ -282,8 +310,11 @@ class MLAAttention:
         if cache is None:
             cache = new_cache(B, klr, rope, Tn, self.cache_dtype, x.device)
         cache.append(c_new, r_new)
-        lat, rot = cache.view()
         scale = qhd ** -0.5
+        if q4 and self.kv_b.dtype == torch.bfloat16:
+            o = cache.attend(q[..., :nope], q[..., nope:], self.wk, self.wv, scale, gate)
+            return mm(o.reshape(B, Tn, nh * vhd), self.o_w), cache
+        lat, rot = cache.view()
         # one query token: the HIP core, over a bf16 cache or the reference's default fp32
         # cache; an fp32 cache with fp32 kv_b (validation mode) keeps the exact fp32 form,
         # since the core takes W_UK / W_UV in bf16
@@ -362,31 +393,42 @@ class MLAAttention:
                   c.qk_rope_head_dim, c.qk_nope_head_dim, vhd, float(scale), T.ptr(ws), ws.numel(), T.stream(q))
         return out
 
-    def decode_step(self, x: torch.Tensor, cache: MLACache | None = None):
-        """One token at batch 1 through k3_mla_step_decode (attention_mla.py:168-216): the
-        new latent row is written into the cache at position ``cache.length``."""
+    def decode_step(self, x: torch.Tensor, cache: MLACache | MLACacheQ4 | None = None):
+        """One token at batch 1 through k3_mla_step_decode, or k3_mla_step_decode_q4 on a 4-bit cache
+        (attention_mla.py:168-216): the new latent row is written into the cache at position ``cache.length``."""
         c = self.cfg
         nh, nope, rope, vhd, klr = (c.num_attention_heads, c.qk_nope_head_dim, c.qk_rope_head_dim,
                                     c.v_head_dim, c.kv_lora_rank)
         hidden, ql = x.shape[-1], self.q_a.shape[0]
-        if cache is None:
+        if cache is None and self.cache_bits == 4:
+            cache = new_cache_q4(1, 1, bool(getattr(c, "mla_cache_weights", False)), x.device)
+        elif cache is None:
             cache = new_cache(1, klr, rope, 1, self.cache_dtype, x.device)
         cache.reserve(1)
         pos = cache.length
         xin = T.contiguous_aligned(x.reshape(hidden))
         if xin.dtype not in (torch.float32, torch.bfloat16):
             xin = xin.to(torch.float32)
-        lat, rot = cache.latent[0], cache.rot[0]
-        nbytes = int(_lib.lib().k3_mla_step_workspace_size(hidden, ql, nh, nope, rope, vhd, klr, pos + 1))
-        ws = _workspace.get(x.device, nbytes, "mla_step")
         out = torch.empty(hidden, dtype=torch.float32, device=x.device)
         m = self._mats
-        _lib.call("k3_mla_step_decode", T.ptr(xin), T.dtype_code(xin.dtype), T.ptr(m["q_a"]), T.ptr(self._q_an32),
-                  T.ptr(m["q_b"]), T.ptr(m["kv_a"]), T.ptr(self._kv_an32), T.ptr(self.wk), T.ptr(self.wv),
-                  T.ptr(m["g"] if getattr(c, "mla_use_output_gate", False) else None), T.ptr(m["o"]), T.ptr(lat),
-                  lat.stride(0), T.ptr(rot), rot.stride(0), cache.capacity, pos, float(c.rms_norm_eps),
-                  float(c.q_head_dim ** -0.5), T.ptr(out), _lib.K3_F32, hidden, ql, nh, nope, rope, vhd, klr,
-                  T.ptr(ws), ws.numel(), T.stream(xin))
+        gate = m["g"] if getattr(c, "mla_use_output_gate", False) else None
+        front = (T.ptr(xin), T.dtype_code(xin.dtype), T.ptr(m["q_a"]), T.ptr(self._q_an32), T.ptr(m["q_b"]), T.ptr(m["kv_a"]),
+                 T.ptr(self._kv_an32), T.ptr(self.wk), T.ptr(self.wv), T.ptr(gate), T.ptr(m["o"]))
+        back = (cache.capacity, pos, float(c.rms_norm_eps), float(c.q_head_dim ** -0.5), T.ptr(out), _lib.K3_F32, hidden, ql, nh,
+                nope, rope, vhd, klr)
+        if isinstance(cache, MLACacheQ4):
+            packed, scales, rot, weight = cache.packed, cache.scales, cache.rot, cache.weight
+            T.require_device(xin, packed, scales, rot, weight)
+            nbytes = _lib.size("k3_mla_step_q4_workspace_size", ql, nh, nope, rope, vhd, klr, pos + 1, int(weight is not None))
+            ws = _workspace.get(x.device, nbytes, "mla_step")
+            _lib.call("k3_mla_step_decode_q4", *front, T.ptr(packed), packed.stride(1), T.ptr(scales), scales.stride(1), T.ptr(rot),
+                      rot.stride(1), T.ptr(weight), *back, T.ptr(ws), ws.numel(), T.stream(xin))
+        else:
+            lat, rot = cache.latent[0], cache.rot[0]
+            nbytes = int(_lib.lib().k3_mla_step_workspace_size(hidden, ql, nh, nope, rope, vhd, klr, pos + 1))
+            ws = _workspace.get(x.device, nbytes, "mla_step")
+            _lib.call("k3_mla_step_decode", *front, T.ptr(lat), lat.stride(0), T.ptr(rot), rot.stride(0), *back, T.ptr(ws),
+                      ws.numel(), T.stream(xin))
         cache.length = pos + 1
         return out.reshape(1, 1, hidden), cache
 

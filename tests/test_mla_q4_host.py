@@ -120,7 +120,7 @@ def test_entry_points_check_their_arguments():
     from k3hip import _lib
     lib = _lib.lib()
     p, n = ctypes.c_void_p(4096), None
-    app = [p, 1536, 512, 0, p, 192, 64, 0, p, 2048, 256, p, 128, 16, p, 512, 64, n, 0, n, 2, 3, 8, 512, 64, n]
+    app = [p, 1536, 512, 0, p, 192, 64, 0, p, 2048, 256, p, 128, 16, p, 512, 64, n, 0, n, n, 0, 2, 3, 8, 512, 64, n]
 
     def append(**at):
         args = list(app)
@@ -130,10 +130,10 @@ def test_entry_points_check_their_arguments():
     assert append(_0=n) == _lib.K3_ERR_NULL and append(_8=n) == _lib.K3_ERR_NULL
     assert append(_3=5) == _lib.K3_ERR_DTYPE and append(_7=2) == _lib.K3_ERR_DTYPE
     assert append(_18=6) == _lib.K3_ERR_SHAPE and b"do not fit" in lib.k3_last_error()
-    for at in ({"_23": 256}, {"_24": 32}, {"_20": -1}, {"_20": 70000}, {"_2": 510}, {"_10": 255}, {"_13": 15}, {"_16": 63}, {"_22": 2}):
+    for at in ({"_25": 256}, {"_26": 32}, {"_22": -1}, {"_22": 70000}, {"_2": 510}, {"_10": 255}, {"_13": 15}, {"_16": 63}, {"_24": 2}):
         assert append(**at) == _lib.K3_ERR_SHAPE, at
     assert append(_0=ctypes.c_void_p(4104)) == _lib.K3_ERR_ALIGN and append(_8=ctypes.c_void_p(4097)) == _lib.K3_ERR_ALIGN
-    assert append(_21=0) == _lib.K3_OK and append(_20=0) == _lib.K3_OK
+    assert append(_23=0) == _lib.K3_OK and append(_22=0) == _lib.K3_OK
 
     size = lib.k3_mla_q4_workspace_size(2, 3, 4, 96, 8, 0, 0, 1, 0)
     assert size > 0 and lib.k3_mla_q4_workspace_size(0, 3, 4, 96, 8, 0, 0, 1, 0) == 0
@@ -218,3 +218,97 @@ def test_oracle_evicts():
     assert oracle.evict([5, 1, 3, 3, 3, 2, 9], 7, 4, 0, 2) == [0, 2, 5, 6]
     assert oracle.evict([1.0, float("nan"), -1.0], 3, 2, 0, 0) == [0, 2]
     assert oracle.evict([1.0, 2.0], 2, 3, 0, 0) == [0, 1]
+
+
+# ------------------------------------------------------------------------------- the cache and the layer
+def _cfg(**kw):
+    from types import SimpleNamespace
+    return SimpleNamespace(**{**dict(hidden_size=64, num_attention_heads=2, q_lora_rank=64, kv_lora_rank=512, qk_nope_head_dim=128,
+                                     qk_rope_head_dim=64, v_head_dim=128, q_head_dim=192, rms_norm_eps=1e-5, mla_cache_bits=4), **kw})
+
+
+def _layer(cfg):
+    from k3hip.mla import MLAAttention
+    z = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
+    klr, rope = cfg.kv_lora_rank, cfg.qk_rope_head_dim
+    return MLAAttention(cfg, {"q_a_proj.weight": z(64, 64), "q_a_layernorm.weight": z(64), "q_b_proj.weight": z(2 * 192, 64),
+                              "kv_a_proj_with_mqa.weight": z(klr + rope, 64), "kv_a_layernorm.weight": z(klr),
+                              "kv_b_proj.weight": z(2 * 256, klr), "o_proj.weight": z(64, 256)})
+
+
+@pytest.mark.parametrize("kw", [{"mla_cache_bits": 8}, {"mla_cache_bits": 3}, {"mla_cache_group_size": 64}, {"kv_lora_rank": 256},
+                                {"qk_rope_head_dim": 32}])
+def test_layer_refuses_other_quantised_caches(kw):
+    with pytest.raises(ValueError):
+        _layer(_cfg(**kw))
+    if "mla_cache_bits" not in kw:
+        _layer(_cfg(**{**kw, "mla_cache_bits": None}))
+
+
+@pytest.mark.parametrize("bits", [None, 0, 16])
+def test_layer_without_the_option_keeps_its_cache(bits):
+    layer = _layer(_cfg(mla_cache_bits=bits))
+    assert layer.cache_bits != 4 and layer.cache_dtype == BF16
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_cache_grows_by_doubling(weights):
+    from k3hip.mla_q4 import new_cache_q4
+    cache = new_cache_q4(2, 1, weights, "cpu")
+    assert cache.capacity == 256 and cache.bytes_per_token() == 400 and cache.nbytes_used() == 0
+    for x in cache._buffers():
+        x.copy_(torch.randint(1, 100, x.shape).to(x.dtype))
+    before = [x.clone() for x in cache._buffers()]
+    cache.length = 250
+    assert cache.reserve(6).capacity == 256 and cache.packed is not None
+    cache.reserve(7)
+    assert cache.capacity == 512 and cache.length == 250 and cache.nbytes_used() == 2 * 250 * 400
+    for x, y in zip(cache._buffers(), before):
+        assert torch.equal(x[:, :250], y[:, :250]) and not x[:, 250:].any() and x.dtype == y.dtype
+    cache.length = 512
+    assert cache.reserve(1000).capacity == 1536
+    assert (cache.weight is not None) == weights
+
+
+def test_cache_without_weights_cannot_evict():
+    from k3hip.mla_q4 import new_cache_q4
+    with pytest.raises(ValueError, match="no attention weights"):
+        new_cache_q4(1, 1, device="cpu").evict(4)
+
+
+def test_cache_passes_its_buffers_and_length(monkeypatch):
+    from k3hip.mla_q4 import new_cache_q4
+    calls = _launches(monkeypatch)
+    cache = new_cache_q4(1, 1, True, "cpu")
+    cache.append(torch.zeros(1, 300, 512), torch.zeros(1, 300, 64))
+    cache.attend(torch.zeros(1, 2, 4, 128), torch.zeros(1, 2, 4, 64), torch.zeros(4, 128, 512, dtype=BF16), torch.zeros(4, 128, 512, dtype=BF16),
+                 0.1)
+    cache.evict(40, 4, 20)
+    assert cache.length == 40 and cache.capacity == 512
+    (a, append), (b, attend), (c, evict) = calls
+    assert (a, b, c) == ("k3_mla_q4_append", "k3_mla_q4_attention", "k3_cache_evict")
+    assert append[18] == 0 and append[20] != 0 and append[23:25] == (300, 512) and attend[22] == 300 and evict[3:8] == (300, 1, 40, 4, 20)
+
+
+def test_step_entry_point_checks_its_arguments():
+    from k3hip import _lib
+    lib = _lib.lib()
+    p, n = ctypes.c_void_p(4096), None
+    size = lib.k3_mla_step_q4_workspace_size(64, 2, 128, 64, 128, 512, 6, 1)
+    assert size > lib.k3_mla_step_q4_workspace_size(64, 2, 128, 64, 128, 512, 6, 0) > 0
+    args = [p, 0, p, p, p, p, p, p, p, n, p, p, 256, p, 16, p, 64, p, 8, 5, 1e-5, 0.1, p, 0, 64, 64, 2, 128, 64, 128, 512, p, size, n]
+
+    def step(**at):
+        a = list(args)
+        for k, v in at.items():
+            a[int(k[1:])] = v
+        return lib.k3_mla_step_decode_q4(*a)
+    for i in (0, 2, 3, 4, 5, 6, 7, 8, 10, 11, 13, 15, 22, 31):
+        assert step(**{f"_{i}": n}) == _lib.K3_ERR_NULL, i
+    assert step(_1=3) == _lib.K3_ERR_DTYPE and step(_23=3) == _lib.K3_ERR_DTYPE
+    for at in ({"_12": 255}, {"_12": 264}, {"_14": 15}, {"_16": 63}, {"_16": 68}, {"_18": 5}, {"_19": -1}, {"_19": 8}, {"_24": 60}, {"_25": 0},
+               {"_27": 264}, {"_28": 32}, {"_29": 1032}, {"_30": 256}, {"_18": (1 << 24) + 1}):
+        assert step(**at) == _lib.K3_ERR_SHAPE, at
+    for i in (0, 2, 3, 4, 5, 6, 7, 8, 10, 11, 15, 31):
+        assert step(**{f"_{i}": ctypes.c_void_p(4104)}) == _lib.K3_ERR_ALIGN, i
+    assert step(_32=size - 1) == _lib.K3_ERR_WORKSPACE
