@@ -51,6 +51,76 @@ struct Rows {
     }
 };
 
+// ------------------------------------------------------------------ ranges
+// What the blocks of the attention take, a range of positions of a sequence each ("slot", with a record of its own for every row).
+// Sequences of one length, or with rows enough for the card: range `slot % NS` of sequence `slot / NS`.  Sequences of lengths of their
+// own that are few blocks: a list made on the device, by a block of the query launch, with ranges of one length that fills the card
+// with what there is rather than with the capacity.  (32 sequences of up to 8192 positions, 1028 on average: NS ranges of the capacity
+// each took 68 us in all, the list 54.)
+struct Ranges {
+    const int32_t *lengths;     // [B]
+    int4 *slot;                 // [slots]: sequence (-1: none), first position, last + 1, the sequence's length
+    int2 *seq;                  // [B]: first slot, number of slots; null: no list
+    int B, cap, slots, spread, least;   // spread: slots less one a sequence; least: shortest range
+};
+constexpr int kMaxListed = 512;         // sequences of a list
+
+// by 256 threads
+__device__ __forceinline__ void list_ranges(const Ranges &a, int *lds) {
+    int *const first = lds, *const len = lds + kMaxListed, *const part = lds + 2 * kMaxListed;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int n[2], own = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {       // sequences 2 tid, 2 tid + 1
+        const int b = 2 * tid + u;
+        n[u] = b < a.B ? min(max(a.lengths[b], 0), a.cap) : 0;
+        len[b] = n[u], own += n[u];
+    }
+    float total = static_cast<float>(own);      // (the ranges' length need not be exact, but the same everywhere: one thread sets it)
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+    if (lane == 0) part[wave] = __float_as_int(total);
+    __syncthreads();
+    if (tid == 0) {
+        float t = 0.f;
+        for (int i = 0; i < 4; ++i) t += __int_as_float(part[i]);
+        part[4] = max(a.least, (static_cast<int>(t * 1.001f / static_cast<float>(a.spread)) + 64) & ~63);
+    }
+    __syncthreads();
+    const int Ts = part[4];
+    int c[2], sum = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) c[u] = (n[u] + Ts - 1) / Ts, sum += c[u];
+    int before = sum;                   // inclusive over the wave's threads
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(before, o);
+        if (lane >= o) before += x;
+    }
+    if (lane == 63) part[8 + wave] = before;
+    __syncthreads();
+    before -= sum;
+    for (int i = 0; i < wave; ++i) before += part[8 + i];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int b = 2 * tid + u;
+        first[b] = before;
+        if (b < a.B) a.seq[b] = make_int2(min(before, a.slots - 1), min(c[u], a.slots - before));
+        before += c[u];
+    }
+    if (tid == 255) part[12] = before;
+    __syncthreads();
+    const int used = part[12];
+    for (int s = tid; s < a.slots; s += 256) {
+        int b = 0;                      // the last sequence that starts at or before s (one of several that start there has ranges: the last)
+#pragma unroll
+        for (int o = kMaxListed / 2; o; o >>= 1)
+            if (first[b + o] <= s) b += o;
+        const int at = (s - first[b]) * Ts;
+        a.slot[s] = s < used ? make_int4(b, at, min(at + Ts, len[b]), len[b]) : make_int4(-1, 0, 0, 0);
+    }
+}
+
 // ------------------------------------------------------------------ qa
 struct QaArgs {
     const void *q_nope, *q_rot;
@@ -60,6 +130,7 @@ struct QaArgs {
     int64_t q_seq;                          // bytes of a sequence's tiles
     int H, nope, M, t0;                     // rows.T queries from t0 on; M = B T
     Rows rows;
+    Ranges ranges;
 };
 
 constexpr int kWLd = 272;                   // LDS bytes per staged weight row (128 columns + 16 bytes)
@@ -95,7 +166,7 @@ struct QueryRaw {
     }
 };
 
-// grid (H, ceil(M / (16 MT)), 4): queries 16 MT y .. of head x, latent columns 128 z .. +128
+// grid (H, ceil(M / (16 MT)), 4): queries 16 MT y .. of head x, latent columns 128 z .. +128; z = 4, if there: the list of ranges
 // MT 1: few queries, a wave to 32 of the columns; bound by the latency of reading W_UK once (every load in flight at once).
 // MT 4: 64 queries to a block's 32 KB of W_UK, a wave to 16 of them, whose bf16 terms it forms once for all columns; bound by the
 // 6-bit terms' rounding and by writing them.  (A wave to 32 columns of all 64 formed each query's terms four times: 87 us for
@@ -108,6 +179,10 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     static_assert(MT == 1 || MT == 4, "a wave to 32 columns, or to a tile of queries");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
     const int h = blockIdx.x, m0 = blockIdx.y * 16 * MT, quarter = blockIdx.z;
+    if (quarter == 4) {
+        if (h == 0 && m0 == 0) list_ranges(a.ranges, reinterpret_cast<int *>(lds));
+        return;
+    }
     const int steps = (a.nope + 31) >> 5, T = a.rows.T;
     const uint16_t *w = a.w_uk + static_cast<int64_t>(h) * a.nope * kQ4Lat + quarter * 128;
     const int qt = MT == 1 ? 0 : wave, col = MT == 1 ? wave * 32 : 0, mine = m0 + 16 * qt + r16;   // the wave's queries and columns
@@ -230,8 +305,9 @@ struct AttendArgs {
     int64_t p_b, p_t, s_b, s_t, r_b, r_t;       // bytes
     const int32_t *lengths, *counts;            // [B] or null
     int length, cap, count;                     // where those are null
-    float *part;                                // [B][NS][rows][512]
-    float2 *ml;                                 // [B][NS][rows]
+    const int4 *slot;                           // the list of ranges, or null
+    float *part;                                // [slots][rows][512]
+    float2 *ml;                                 // [slots][rows]
     Rows order;
     int t0, rows, Ts, NS, rblocks, B;           // rows: order.count()
     float c;                                    // scale * log2(e)
@@ -270,17 +346,27 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     const int nb = gridDim.x;
     const int w = a.swizzle ? (blockIdx.x & 7) * (nb >> 3) + (blockIdx.x >> 3) : blockIdx.x;
     int rb = w % a.rblocks;
-    const int split = (w / a.rblocks) % a.NS, b = w / (a.rblocks * a.NS);
+    const int slot = w / a.rblocks;
+    int4 range;                                 // sequence, first position, last + 1, length
+    if (a.slot) {
+        const int4 r = a.slot[slot];
+        range = make_int4(__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y), __builtin_amdgcn_readfirstlane(r.z),
+                          __builtin_amdgcn_readfirstlane(r.w));
+        if (range.x < 0) return;
+    } else {
+        range.x = slot / a.NS, range.y = slot % a.NS * a.Ts, range.z = range.y + a.Ts;
+        range.w = a.lengths ? min(max(a.lengths[range.x], 0), a.cap) : a.length;
+    }
+    const int b = range.x, len = range.w;
     // whole blocks of one head: the last queries, which see most, first
     if (a.order.Tp && a.order.Tp % (16 * RG) == 0) rb = rb % a.order.H * (a.order.Tp / (16 * RG)) + (a.order.Tp / (16 * RG) - 1 - rb / a.order.H);
     const int row0 = rb * 16 * RG;
-    const int len = a.lengths ? min(max(a.lengths[b], 0), a.cap) : a.length;
     const int cnt = a.counts ? min(max(a.counts[b], 0), a.count) : a.count;
     // the last query of the block that is there sees most
     const int tlast = min(a.t0 + a.order.last_query(row0, min(row0 + 16 * RG, a.rows) - 1), cnt - 1);
     const int most = tlast >= a.t0 ? q4_sees(tlast, cnt, len) : 0;
-    const int t_begin = split * a.Ts, t_end = min(most, t_begin + a.Ts);
-    float2 *ml = a.ml + (static_cast<int64_t>(b) * a.NS + split) * a.rows;
+    const int t_begin = range.y, t_end = min(most, range.z);
+    float2 *ml = a.ml + static_cast<int64_t>(slot) * a.rows;
     if (t_end <= t_begin) {
         if (tid < 16 * RG && row0 + tid < a.rows) ml[row0 + tid] = make_float2(-INFINITY, 0.f);
         return;
@@ -591,7 +677,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         __syncthreads();
         // the records through LDS (the codes are done with), so that a store writes 512 contiguous bytes of two rows: as the
         // accumulators lie, 64 bytes of sixteen rows, the 256 blocks of a short split took 7 us to write them
-        float *part = a.part + ((static_cast<int64_t>(b) * a.NS + split) * a.rows + row0) * kQ4Lat + col0;
+        float *part = a.part + (static_cast<int64_t>(slot) * a.rows + row0) * kQ4Lat + col0;
         float *const x = reinterpret_cast<float *>(kbuf) + (wave - 4) * 16 * kCLd;
         static_assert(4 * 16 * kCLd * 4 <= kSlots * kKBytes, "the contexts' way out fits the code tiles");
 #pragma unroll
@@ -617,8 +703,10 @@ struct UvArgs {
     int out_bf16;
     const float *gate;       // [B, Tall, H, V] or null
     float2 *stats;           // [B][rows]: maximum less kLift, 1 / sum (which is lifted); or null
+    const int2 *seq;         // the sequences' records, or null: NS each
     Rows order;
     int M, V, rows, NS, Tall, t0;
+    __device__ __forceinline__ int2 records(int b) const { return seq ? seq[b] : make_int2(b * NS, NS); }  // first, number (at most NS)
 };
 constexpr int kMaxSplits = 256;
 
@@ -635,53 +723,51 @@ __device__ __forceinline__ void store_out4(const UvArgs &a, int m, int h, int v,
         *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + at) = o;
 }
 
-// The weights of a row's records, 2^(m_s - M) / L with M = max m_s, L = sum 2^(m_s - M) l_s, by a wave; a split the row sees
-// nothing of has no record (its sum is exactly 0), and its weight is zero whatever the others are.
-__device__ __forceinline__ void record_weights(const UvArgs &a, int b, int row, float *wsp) {
+// The weights of a row's records, 2^(m_s - M) / L with M = max m_s, L = sum 2^(m_s - M) l_s, by a wave, record 64 u + lane in
+// w[u]; a split the row sees nothing of has no record (its sum is exactly 0), and its weight is zero whatever the others are.
+__device__ __forceinline__ void record_weights(const UvArgs &a, int b, int row, int2 there, bool stats, float (&w)[kMaxSplits / 64]) {
     const int lane = threadIdx.x & 63;
-    const float2 *ml = a.ml + static_cast<int64_t>(b) * a.NS * a.rows + row;
+    const float2 *ml = a.ml + static_cast<int64_t>(there.x) * a.rows + row;
     float2 v[kMaxSplits / 64];
     float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kMaxSplits / 64; ++u) {
         const int s = lane + 64 * u;
-        v[u] = s < a.NS ? ml[static_cast<int64_t>(s) * a.rows] : make_float2(-INFINITY, 0.f);
+        v[u] = s < there.y ? ml[static_cast<int64_t>(s) * a.rows] : make_float2(-INFINITY, 0.f);
         mx = fmaxf(mx, v[u].x);
     }
     mx = wave_max_all(mx);
-    float l = 0.f, e[kMaxSplits / 64];
+    float l = 0.f;
 #pragma unroll
     for (int u = 0; u < kMaxSplits / 64; ++u) {
-        e[u] = v[u].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v[u].x - mx);
-        l = fmaf(e[u], v[u].y, l);
+        w[u] = v[u].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v[u].x - mx);
+        l = fmaf(w[u], v[u].y, l);
     }
     l = wave_sum_all(l);
     const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int u = 0; u < kMaxSplits / 64; ++u) {
-        const int s = lane + 64 * u;
-        if (s < a.NS) wsp[s] = v[u].y == 0.f ? 0.f : e[u] * inv;
-    }
-    if (a.stats && lane == 0) a.stats[static_cast<int64_t>(b) * a.rows + row] = make_float2(mx - kLift, inv);
+    for (int u = 0; u < kMaxSplits / 64; ++u) w[u] = v[u].y == 0.f ? 0.f : w[u] * inv;
+    if (stats && a.stats && lane == 0) a.stats[static_cast<int64_t>(b) * a.rows + row] = make_float2(mx - kLift, inv);
 }
 
 // Few queries: grid (H, ceil(M / per), Z), WAVES waves, queries per y .. +per (at most 16) of head x, VT tiles of 16 output columns
-// (z).  A wave joins the records of its 512 / WAVES latent columns (4 to a lane, 64 / kLanes splits at a time) and multiplies them with
-// its columns of W_UV (loaded first of all); the waves' products are added in order.  Bound by the latency of the records (NS x 2 KB a
-// query) and of W_UV, 128 KB a head.
-//   many records: 16 waves have 128 KB of them on the way (10.0 us at 128 splits of 64 heads; 8 waves, 64 KB: 16)
-//   up to kFewSplits: 8 waves with half of the output columns each (6.5 us at 6 splits of 96 heads; 16 waves, all columns: 10.0)
-constexpr int kDLd = 132;                   // floats of a product row (128)
+// (z).  Two waves join a query's records, 256 columns each, four to a lane (with fewer queries than pairs of waves, 2, 4 or 8 pairs
+// every 2nd, 4th, 8th record); then a wave multiplies 512 / WAVES columns of all queries with its columns of W_UV (loaded
+// first of all), and the waves' products are added in order.  Bound by the latency of the records (NS x 2 KB a query) and of W_UV,
+// 128 KB a head.  (A wave that joined its columns of every query, eight records side by side in its lanes, spent more on adding up the
+// lanes than on the records: 17 us for 32 queries of 64 heads with 1 to 43 records each, this: 13.)
+//   many records: 16 waves have 128 KB of them on the way
+//   up to kFewSplits: 8 waves with half of the output columns each (6 records of 96 heads: 6.1 us; 16 waves, all columns: 10.0)
+constexpr int kXLd = kQ4Lat + 4, kDLd = 132;        // floats of a context row (512), of a product row (128)
 constexpr int kFewSplits = 8;
-constexpr int few_lds(int waves, int NS) { return (16 * (512 + 4 * waves) + 8 * 16 * kDLd + 16 * NS) * 4; }
+constexpr int kFewLds = (16 * kXLd + 8 * 16 * kDLd) * 4;
 
 template <int WAVES, int VT>
 __global__ __launch_bounds__(64 * WAVES, 1) void uv_few_kernel(UvArgs a, int per) {
-    constexpr int kCols = 512 / WAVES, kLanes = kCols / 4, kPar = 64 / kLanes, kSteps = kCols / 32, kXLd = kCols + 4;
+    constexpr int kCols = 512 / WAVES, kSteps = kCols / 32, kPairs = WAVES / 2;
     extern __shared__ __attribute__((aligned(16))) float sm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
-    const int cl = lane % kLanes, sl = lane / kLanes;
-    float *const x = sm + wave * 16 * kXLd, *const d = sm + WAVES * 16 * kXLd, *const wsp = d + 8 * 16 * kDLd;
+    float *const x = sm, *const d = sm + 16 * kXLd;
     const int h = blockIdx.x, m0 = blockIdx.y * per, col0 = wave * kCols, nv = min(per, a.M - m0);
     auto weights_of = [&](int v0, u32x4 (&w)[VT][kSteps]) __attribute__((always_inline)) {
 #pragma unroll
@@ -695,58 +781,50 @@ __global__ __launch_bounds__(64 * WAVES, 1) void uv_few_kernel(UvArgs a, int per
     u32x4 w[VT][kSteps];
     const int vz = blockIdx.z * 16 * VT;
     weights_of(vz, w);
-    constexpr int kBatch = WAVES == 16 ? 7 : 8;     // (in registers, beside the weights)
-    // (a pass's records are at most 2^16 rows, so 2^27 bytes)
-    const uint32_t pitch = static_cast<uint32_t>(a.rows) * kQ4Lat;
-    auto record = [&](int i) __attribute__((always_inline)) {
+    int pairs = 1;                          // of a query
+    while (2 * pairs * nv <= kPairs) pairs *= 2;
+    const int g = (wave >> 1) & (pairs - 1);
+    constexpr int kBatch = 8;
+    for (int i = (wave >> 1) / pairs; i < nv; i += kPairs / pairs) {
         const int m = m0 + i, b = m / a.order.T, row = a.order.of(m % a.order.T, h);
-        return static_cast<uint32_t>(b * a.NS) * pitch + static_cast<uint32_t>(row * kQ4Lat + col0);
-    };
-    // the next records to add: in bounds, whether they were written or not (a split that the row sees nothing of has none)
-    auto load = [&](int i, int j, f32x4 (&y)[kBatch]) __attribute__((always_inline)) {
-        const float *src = a.part + record(min(i, nv - 1));
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            if (u > 0 && j + kPar * u >= a.NS) break;       // (the same for all lanes)
-            y[u] = *reinterpret_cast<const f32x4 *>(src + (static_cast<uint32_t>(min(j + kPar * u + sl, a.NS - 1)) * pitch + 4u * cl));
-        }
-    };
-    f32x4 y[kBatch];
-    load(0, 0, y);
-    for (int i = wave; i < nv; i += WAVES) {
-        const int m = m0 + i;
-        record_weights(a, m / a.order.T, a.order.of(m % a.order.T, h), wsp + i * a.NS);
-    }
-    __syncthreads();
-    for (int i = 0; i < nv; ++i) {
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
-        for (int j = 0; j < a.NS; j += kPar * kBatch) {
+        int2 there = a.records(b);
+        there.x = __builtin_amdgcn_readfirstlane(there.x), there.y = __builtin_amdgcn_readfirstlane(there.y);
+        const int n = there.y;
+        const int64_t pitch = static_cast<int64_t>(a.rows) * kQ4Lat;
+        const float *src = a.part + there.x * pitch + row * kQ4Lat + (wave & 1) * 256 + lane * 4;
+        f32x4 y[kBatch];
+        auto load = [&](int k) __attribute__((always_inline)) {     // (written or not: where not, the weight is zero)
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
-                if (u > 0 && j + kPar * u >= a.NS) break;
-                const int k = j + kPar * u + sl;
-                const float f = k < a.NS ? wsp[i * a.NS + k] : 0.f;
-                if (f == 0.f) y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-                s += y[u] * f;
+                if (k + pairs * u >= n) break;
+                y[u] = *reinterpret_cast<const f32x4 *>(src + (k + pairs * u) * pitch);
             }
-            if (j + kPar * kBatch < a.NS)
-                load(i, j + kPar * kBatch, y);
-            else if (i + 1 < nv)
-                load(i + 1, 0, y);
-        }
+        };
+        load(g);
+        float f[kMaxSplits / 64];
+        record_weights(a, b, row, there, g == 0 && (wave & 1) == 0, f);
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        for (int k = g; k < n; k += pairs * kBatch) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {       // the lanes of a column group, in a fixed order
-            s[k] = q4_rows_sum(s[k]);
-            if (kLanes == 8) s[k] += __shfl_xor(s[k], 8);
+            for (int u = 0; u < kBatch; ++u) {
+                const int c = k + pairs * u;
+                if (c >= n) break;
+                const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c < 64 ? f[0] : c < 128 ? f[1] : c < 192 ? f[2] : f[3]), c & 63));
+                if (v != 0.f) s += y[u] * v;
+            }
+            if (k + pairs * kBatch < n) load(k + pairs * kBatch);
         }
-        if (sl == 0) *reinterpret_cast<f32x4 *>(x + i * kXLd + 4 * cl) = s;
+        *reinterpret_cast<f32x4 *>(x + (i * pairs + g) * kXLd + (wave & 1) * 256 + lane * 4) = s;
     }
-    for (int i = nv + sl; i < 16; i += kPar) *reinterpret_cast<f32x4 *>(x + i * kXLd + 4 * cl) = f32x4{0.f, 0.f, 0.f, 0.f};
-    u32x4 cf[kSteps][3];                    // (a wave's own rows: its LDS accesses are in order)
+    __syncthreads();
+    u32x4 cf[kSteps][3];
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
-        const float *xr = x + r16 * kXLd + 32 * k + 8 * q4;
-        const f32x4 u = *reinterpret_cast<const f32x4 *>(xr), z = *reinterpret_cast<const f32x4 *>(xr + 4);
+        f32x4 u = {0.f, 0.f, 0.f, 0.f}, z = u;
+        if (r16 < nv) {
+            const float *xr = x + r16 * pairs * kXLd + col0 + 32 * k + 8 * q4;
+            for (int c = 0; c < pairs; ++c) u += *reinterpret_cast<const f32x4 *>(xr + c * kXLd), z += *reinterpret_cast<const f32x4 *>(xr + c * kXLd + 4);
+        }
         const float v[8] = {u[0], u[1], u[2], u[3], z[0], z[1], z[2], z[3]};
         terms8(v, cf[k]);
     }
@@ -794,7 +872,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void uv_few_kernel(UvArgs a, int per
 
 // Many queries: grid (H, ceil(M / 64)), four waves, queries 64 y .. +64 of head x, 128 latent columns at a time: a thread joins
 // the records of 4 columns of 8 queries and leaves them in LDS as TERMS bf16 terms (two, 2^-17, for a bf16 result); a wave
-// takes 32 of 128 output columns for all 64 queries.  Bound by reading the records.
+// takes 32 of 128 output columns for all 64 queries.  Bound by reading the records.  (Not with a list of ranges.)
 template <int TERMS>
 __global__ __launch_bounds__(256, 2) void uv_many_kernel(UvArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -804,7 +882,12 @@ __global__ __launch_bounds__(256, 2) void uv_many_kernel(UvArgs a) {
     const int h = blockIdx.x, m0 = blockIdx.y * 64, nv = min(64, a.M - m0);
     for (int i = wave; i < nv; i += 4) {
         const int m = m0 + i;
-        record_weights(a, m / a.order.T, a.order.of(m % a.order.T, h), wsp + i * a.NS);
+        const int b = m / a.order.T;
+        float f[kMaxSplits / 64];
+        record_weights(a, b, a.order.of(m % a.order.T, h), a.records(b), true, f);
+#pragma unroll
+        for (int u = 0; u < kMaxSplits / 64; ++u)
+            if (64 * u + lane < a.NS) wsp[i * a.NS + 64 * u + lane] = f[u];
     }
     __syncthreads();
     const uint32_t pitch = static_cast<uint32_t>(a.rows) * kQ4Lat;
@@ -1050,9 +1133,9 @@ __global__ __launch_bounds__(256) void weights_add_kernel(WeightArgs wa) {
 
 // ------------------------------------------------------------------ host side
 struct Plan {
-    int NT, RT, PT, RG, tiles, rblocks, Ts, NS, many, chunk, chunks;
+    int NT, RT, PT, RG, tiles, rblocks, Ts, NS, slots, spread, listed, many, chunk, chunks;     // listed: Ts is the shortest range
     Rows order;
-    int64_t qop, ml, part, stats, wpart, total;
+    int64_t qop, ml, part, stats, wpart, slot, seq, total;
 };
 
 constexpr int64_t kChunkRows = 1 << 16;   // rows (heads x queries, all sequences) of one pass over the queries
@@ -1071,20 +1154,34 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
     p.order = rows_of(std::max<int64_t>(1, std::min(T, kChunkRows / (B * H))), H);
     const int64_t rows = p.order.count();
     // Rows of a block.  A round costs 0.9 us at 16 rows, 1.1 at 32 and 1.8 at 64 (bf16 results; fp32 1.2, 1.6, 2.5), so more rows cost less
-    // each; but one block a CU is wanted, and a row's record of each range (2 KB) is written and read again, so few rows
-    // over a short cache take small blocks.  Measured, 64 heads, one token, us at 16 / 32 / 64 rows: 4096 positions 27.0 / 28.4 / 30.4,
-    // 32,768 34.1 / 35.8 / 38.2; 32 such sequences of up to 8192: 92 / 81 / 71; five tokens of 96 heads over 7001: 50 / 48 / 48.
-    p.RG = rows > 32 && B * cdiv(rows, 64) >= 8 ? 4 : rows > 16 && (npos > 32768 || B * cdiv(rows, 32) >= 8) ? 2 : 1;
+    // each; but they fill the card with shorter ranges, and every range begins (two rounds' worth) and leaves records (2 KB a row),
+    // and a batch of small blocks is cut into fewer ranges of unequal length.  Measured, us at 16 / 32 / 64 rows and bf16, by the rounds a CU would
+    // have with 16 (r; sequences of their own lengths: half the capacity's):
+    //   r 6 (5 tokens of 96 heads over 3500) 33.2 / 33.2 / 37.4;  8 (1 of 64 over 32,768) 34.7 / 38.1 / 43.4;  13 (5 of 96 over
+    //   7001) 39.1 / 40.7 / 41.1;  16 (1 of 64 over 65,536) 41.7 / 42.2 / 47.1, (2 over 32,768) 41.5 / 40.6 / 43.4;  26 (5 of 96 over
+    //   14,000) 52.9 / 47.4 / 48.8;  32 (1 of 64 over 131,072) 58.4 / 53.2 / 56.1;  51 (5 of 96 over 28,000) 80.7 / 64.0 / 63.0
+    //   batches of 64 heads: 8 of up to 8192 31.7 / 35.1 / 35.8, 32 of them 49.5 / 41.7 / 44.2, 64 of up to 1024 53.2 / 49.2 / 48.9
+    const int64_t r = B * cdiv(rows, 16) * cdiv(npos, kRound) / (varied && B > 1 ? 512 : 256);
+    p.RG = rows <= 16 || (B * cdiv(rows, 16) < 128 && r <= 14) ? 1 : rows <= 32 || (B * cdiv(rows, 32) < 128 && r <= 48) ? 2 : 4;
     p.rblocks = static_cast<int>(cdiv(rows, 16 * p.RG));
     p.tiles = p.rblocks * p.RG;
     const int64_t base = B * p.rblocks;
-    // One block a CU (sequences of their own lengths: half as many again, so the longest one's blocks are not what all wait
-    // for), and at least two rounds to a block: 4096 positions in ranges of 64 took 29.2 us for 27.0.
-    int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (varied && B > 1 ? 384 : 256) / base));
+    // One block a CU, and at least two rounds to a block: 4096 positions in ranges of 64 took 29.2 us for 27.0.
+    int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, 256 / base));
     int64_t ts = std::max<int64_t>(2 * kRound, cdiv(cdiv(std::max<int64_t>(npos, 1), ns), kRound) * kRound);
-    p.Ts = static_cast<int>(ts);
     p.NS = static_cast<int>(cdiv(std::max<int64_t>(npos, 1), ts));
-    p.many = B * p.order.T >= kManyQueries;
+    p.listed = varied && B > 1 && base < 512;
+    if (p.listed) {
+        // a range that is not full for every sequence, so that many fewer for the rest, but as many as there are sequences at least
+        const int64_t spread = std::max<int64_t>(256 / p.rblocks - B, B);
+        ts = std::max<int64_t>(2 * kRound, cdiv(cdiv(npos, kMaxSplits), kRound) * kRound);
+        p.NS = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(cdiv(npos, ts), spread + 1)));
+        p.spread = static_cast<int>(spread), p.slots = static_cast<int>(spread + B);
+    } else {
+        p.slots = static_cast<int>(B * p.NS);
+    }
+    p.Ts = static_cast<int>(ts);
+    p.many = !p.listed && B * p.order.T >= kManyQueries;
     const int64_t pos_blocks = std::max<int64_t>(1, cdiv(npos, 128 * kWTiles));
     p.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.tiles, 512 / (pos_blocks * B))));
     p.chunk = static_cast<int>(cdiv(p.tiles, p.chunks));
@@ -1092,8 +1189,10 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
     auto up = [](int64_t v) { return (v + 255) & ~int64_t(255); };
     int64_t o = 0;
     p.qop = o, o += up(B * p.tiles * q4_tile_bytes(p.NT, p.RT));
-    p.ml = o, o += up(B * p.NS * rows * 8);
-    p.part = o, o += up(B * p.NS * rows * kQ4Lat * 4);
+    p.ml = o, o += up(p.slots * rows * 8);
+    p.part = o, o += up(p.slots * rows * kQ4Lat * 4);
+    p.slot = o, o += p.listed ? up(p.slots * 16) : 0;
+    p.seq = o, o += p.listed ? up(B * 8) : 0;
     p.stats = o, o += weights ? up(B * rows * 8) : 0;
     p.wpart = o, o += weights ? up(static_cast<int64_t>(p.chunks) * B * npos * 4) : 0;
     p.total = o;
@@ -1101,31 +1200,32 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
 }
 
 template <int RG, int NT, int RT, int PT>
-int launch_attend(const AttendArgs &a, hipStream_t st) {
+int launch_attend(const AttendArgs &a, int slots, hipStream_t st) {
     constexpr int bytes = attend_lds(RG, RT, PT);
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(attend_kernel<RG, NT, RT, PT>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     const int rc = check_hip(attr, "mla q4: attention LDS size");
     if (rc) return rc;
-    attend_kernel<RG, NT, RT, PT><<<dim3(static_cast<unsigned>(a.B * a.NS * a.rblocks)), 512, bytes, st>>>(a);
+    attend_kernel<RG, NT, RT, PT><<<dim3(static_cast<unsigned>(slots * a.rblocks)), 512, bytes, st>>>(a);
     return check_hip(hipGetLastError(), "mla q4: attention launch");
 }
 
 template <int RG>
 int launch_attend_of(const AttendArgs &a, const Plan &p, hipStream_t st) {
-    if (p.NT == 3) return p.RT == 1 ? launch_attend<RG, 3, 1, 1>(a, st) : launch_attend<RG, 3, 2, 1>(a, st);
-    if (p.PT == 1) return p.RT == 1 ? launch_attend<RG, 5, 1, 1>(a, st) : launch_attend<RG, 5, 3, 1>(a, st);
-    return p.RT == 1 ? launch_attend<RG, 5, 1, 2>(a, st) : launch_attend<RG, 5, 3, 2>(a, st);
+    if (p.NT == 3) return p.RT == 1 ? launch_attend<RG, 3, 1, 1>(a, p.slots, st) : launch_attend<RG, 3, 2, 1>(a, p.slots, st);
+    if (p.PT == 1) return p.RT == 1 ? launch_attend<RG, 5, 1, 1>(a, p.slots, st) : launch_attend<RG, 5, 3, 1>(a, p.slots, st);
+    return p.RT == 1 ? launch_attend<RG, 5, 1, 2>(a, p.slots, st) : launch_attend<RG, 5, 3, 2>(a, p.slots, st);
 }
 
 template <typename QT, int NT, int RT, int MT>
 int launch_qa_of(const QaArgs &a, hipStream_t st) {
     const int bytes = std::max(((a.nope + 31) / 32) * 32 * kWLd, 16 * MT * kFLd * 4);
+    static_assert(32 * kWLd >= (2 * kMaxListed + 16) * 4, "the list of ranges fits");
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(qa_kernel<QT, NT, RT, MT>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 256 * kWLd);
     const int rc = check_hip(attr, "mla q4: query LDS size");
     if (rc) return rc;
-    qa_kernel<QT, NT, RT, MT><<<dim3(a.H, static_cast<unsigned>(cdiv(a.M, 16 * MT)), 4), 256, bytes, st>>>(a);
+    qa_kernel<QT, NT, RT, MT><<<dim3(a.H, static_cast<unsigned>(cdiv(a.M, 16 * MT)), a.ranges.seq ? 5 : 4), 256, bytes, st>>>(a);
     return check_hip(hipGetLastError(), "mla q4: query launch");
 }
 
@@ -1136,9 +1236,9 @@ int launch_qa(const QaArgs &a, hipStream_t st) {
 
 int launch_uv(const UvArgs &a, int many, hipStream_t st) {
     static const hipError_t few16 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_few_kernel<16, 8>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, few_lds(16, kMaxSplits));
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds);
     static const hipError_t few8 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_few_kernel<8, 4>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, few_lds(8, kFewSplits));
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds);
     static const hipError_t many2 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_many_kernel<2>),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 64 * 272 + 64 * kMaxSplits * 4);
     static const hipError_t many3 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_many_kernel<3>),
@@ -1147,13 +1247,15 @@ int launch_uv(const UvArgs &a, int many, hipStream_t st) {
     if (rc) return rc;
     const unsigned H = static_cast<unsigned>(a.order.H);
     if (!many) {
-        int per = static_cast<int>(std::min<int64_t>(16, a.M));     // fewer queries to a block until there are two blocks a CU
-        while (per > 1 && H * cdiv(a.M, per) < 512) per = (per + 1) / 2;
+        // the fewest queries to a block with which all blocks run at once (one a CU, for its LDS)
+        const int z = a.NS <= kFewSplits ? 2 : 1;
+        int per = static_cast<int>(std::min<int64_t>(16, a.M));
+        while (per > 1 && z * H * cdiv(a.M, per - 1) <= 256) --per;
         const unsigned tiles = static_cast<unsigned>(cdiv(a.M, per));
         if (a.NS <= kFewSplits)
-            uv_few_kernel<8, 4><<<dim3(H, tiles, 2), 512, few_lds(8, a.NS), st>>>(a, per);
+            uv_few_kernel<8, 4><<<dim3(H, tiles, z), 512, kFewLds, st>>>(a, per);
         else
-            uv_few_kernel<16, 8><<<dim3(H, tiles), 1024, few_lds(16, a.NS), st>>>(a, per);
+            uv_few_kernel<16, 8><<<dim3(H, tiles), 1024, kFewLds, st>>>(a, per);
     }
     if (many && a.out_bf16)
         uv_many_kernel<2><<<dim3(H, static_cast<unsigned>(cdiv(a.M, 64))), 256, 2 * 64 * 272 + 64 * a.NS * 4, st>>>(a);
@@ -1221,8 +1323,10 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
     const Plan p = plan_of(B, T, H, v_dim, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weight != nullptr, lengths != nullptr);
     if (workspace_bytes < p.total)
         return set_error(K3_ERR_WORKSPACE, "mla q4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.total);
-    if (static_cast<int64_t>(p.Ts) * std::max({p_row, s_row, 2 * rot_row}) >= (1ll << 31))
-        return set_error(K3_ERR_SHAPE, "mla q4: a split of %d positions spans 2 GiB", p.Ts);
+    // (a range of a list is at most as long as all positions shared out)
+    const int64_t longest = p.listed ? std::max<int64_t>(p.Ts, B * max_length / p.spread * 1.01 + 128) : p.Ts;
+    if (longest * std::max({p_row, s_row, 2 * rot_row}) >= (1ll << 31))
+        return set_error(K3_ERR_SHAPE, "mla q4: a split of %lld positions spans 2 GiB", (long long)longest);
     auto st = static_cast<hipStream_t>(stream);
     char *ws = static_cast<char *>(workspace);
     for (int64_t t0 = 0; t0 < T; t0 += p.order.T) {
@@ -1231,7 +1335,10 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         const int rows = order.count(), M = static_cast<int>(B * order.T);
         const int64_t q_seq = static_cast<int64_t>(p.tiles) * q4_tile_bytes(p.NT, p.RT);
         QaArgs qa{q_nope, q_rot, qn_batch, qn_token, qn_head, qr_batch, qr_token, qr_head, static_cast<const uint16_t *>(w_uk),
-                  ws + p.qop, q_seq, static_cast<int>(H), static_cast<int>(nope_dim), M, static_cast<int>(t0), order};
+                  ws + p.qop, q_seq, static_cast<int>(H), static_cast<int>(nope_dim), M, static_cast<int>(t0), order, {}};
+        if (p.listed)
+            qa.ranges = Ranges{lengths, reinterpret_cast<int4 *>(ws + p.slot), reinterpret_cast<int2 *>(ws + p.seq), static_cast<int>(B),
+                               static_cast<int>(max_length), p.slots, p.spread, p.Ts};
         int rc;
         if (q_dtype == K3_BF16)
             rc = p.NT == 5 ? launch_qa<uint16_t, 5, 1>(qa, st) : launch_qa<uint16_t, 3, 1>(qa, st);
@@ -1245,18 +1352,20 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         a.p_b = p_batch, a.p_t = p_row, a.s_b = s_batch, a.s_t = s_row, a.r_b = 2 * rot_batch, a.r_t = 2 * rot_row;
         a.lengths = lengths, a.counts = counts;
         a.length = static_cast<int>(max_length), a.cap = a.length, a.count = static_cast<int>(T);
+        a.slot = qa.ranges.slot;
         a.part = reinterpret_cast<float *>(ws + p.part), a.ml = reinterpret_cast<float2 *>(ws + p.ml);
         a.order = order, a.t0 = static_cast<int>(t0), a.rows = rows, a.Ts = p.Ts, a.NS = p.NS;
         a.rblocks = static_cast<int>(cdiv(rows, 16 * p.RG)), a.B = static_cast<int>(B), a.c = scale * 1.4426950408889634f;
         // blocks b % 8 run on one XCD: with several ranges its blocks get neighbouring ones (one L2 reads them); with one range the blocks
         // that see most, which come first, are to be spread
-        a.swizzle = p.NS > 1 && (a.B * a.NS * a.rblocks) % 8 == 0;
+        a.swizzle = p.NS > 1 && (p.slots * a.rblocks) % 8 == 0;
         rc = p.RG == 4 ? launch_attend_of<4>(a, p, st) : p.RG == 2 ? launch_attend_of<2>(a, p, st) : launch_attend_of<1>(a, p, st);
         if (rc) return rc;
         UvArgs u{};
         u.part = a.part, u.ml = a.ml, u.w_uv = static_cast<const uint16_t *>(w_uv);
         u.out = out, u.out_bf16 = out_dtype == K3_BF16, u.gate = gate;
         u.stats = weight ? reinterpret_cast<float2 *>(ws + p.stats) : nullptr;
+        u.seq = qa.ranges.seq;
         u.order = order, u.M = M, u.V = static_cast<int>(v_dim), u.rows = rows, u.NS = p.NS;
         u.Tall = static_cast<int>(T), u.t0 = a.t0;
         rc = launch_uv(u, p.many, st);

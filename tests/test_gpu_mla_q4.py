@@ -161,6 +161,26 @@ def test_sequences_of_unequal_length(T, lengths, counts, weight):
                 assert bool((o[b, t] == 0).all())
 
 
+def _lengths(kind, B, cap):
+    g = torch.Generator().manual_seed(B)
+    if kind == "one long":
+        return [cap if b == B // 2 else b % 4 for b in range(B)]
+    if kind == "none":
+        return [0] * B
+    if kind == "full":
+        return [cap] * B
+    return [int(cap ** float(torch.rand(1, generator=g))) if b % 7 else 0 for b in range(B)]
+
+
+@pytest.mark.parametrize("kind", ["one long", "none", "full", "spread"])
+@pytest.mark.parametrize("B,T,H,cap,out", [(2, 1, 64, 1500, F32), (32, 1, 64, 700, BF16), (33, 2, 16, 900, F32), (130, 1, 3, 300, BF16),
+                                           (511, 1, 2, 70, F32), (3, 40, 8, 260, F32)])
+def test_batches_of_unequal_length(kind, B, T, H, cap, out):
+    """Batches that share the card out over the positions there are: one long sequence among empty ones, nothing, all of
+    the capacity, lengths of every size; as many sequences as such a batch may have."""
+    _check(_problem(B, T, H, cap, 170), _lengths(kind, B, cap), out=out, weight=H == 16)
+
+
 @pytest.mark.parametrize("nope,v", [(8, 8), (40, 24), (128, 64), (192, 128), (256, 256), (64, 1024)])
 def test_head_widths(nope, v):
     _check(_problem(2, 2, 6, 50, 40, nope, v), weight=True)
@@ -367,6 +387,22 @@ def test_output_gate():
 
 
 # ------------------------------------------------------------------------------- streams, graphs, threads
+def test_captured_batch_replays_with_other_lengths():
+    """The sharing out is made anew from the lengths at every replay."""
+    from k3hip.mla_q4 import mla_q4_attention
+    B, cap = 20, 900
+    args, n = _problem(B, 1, 64, cap, 190), _ints(_lengths("spread", B, cap))
+    mla_q4_attention(*args, SCALE, lengths=n)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = mla_q4_attention(*args, SCALE, lengths=n)
+    for kind in ("full", "one long", "none", "spread", "full"):
+        n.copy_(_ints(_lengths(kind, B, cap)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, mla_q4_attention(*args, SCALE, lengths=n)), kind
+
+
 def test_another_stream():
     from k3hip.mla_q4 import mla_q4_attention
     args = _problem(1, 2, 32, 400, 170)
