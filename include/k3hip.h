@@ -499,7 +499,7 @@ int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim,
  * values enter exactly; the absorbed queries to 2^-12 of a unit under their group's largest for a bf16 out without weight,
  * else 2^-22; the probabilities to 2^-11 for a bf16 out, 2^-22 for fp32; sums and softmax in fp32.
  * nope a multiple of 8 up to 256, v one up to 1024, H <= 4096, B H <= 65536, max_length <= 2^24.  Pointers 16-byte
- * aligned; p_row and p_batch multiples of 16, rot pitches of 8.
+ * aligned (scales 4-byte); p_row and p_batch multiples of 16, rot pitches of 8, scale pitches of 4.
  * Counterpart of MLAAttention.__call__ over a QuantLatent cache (air_llm/models/kimi_k3/attention_mla.py:193-212). */
 int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t qn_token, int64_t qn_head, const void *q_rot,
                         int64_t qr_batch, int64_t qr_token, int64_t qr_head, int q_dtype, const void *w_uk,
@@ -516,7 +516,7 @@ int64_t k3_mla_step_q4_workspace_size(int64_t q_lora_rank, int64_t heads, int64_
 
 /* k3_mla_step_decode over the 4-bit cache: row pos gets rmsnorm(ckv[:r], kv_a_norm) as k3_mla_q4_append rounds it
  * and bf16(ckv[r:]); the core is k3_mla_q4_attention's over rows 0..pos.  packed, scales, rot: one sequence's
- * cache_rows rows, pitches in elements (packed and rot rows whole 16 bytes); weight: fp32 [cache_rows], to which the step's
+ * cache_rows rows, pitches in elements (packed and rot rows whole 16 bytes, scale rows whole 4); weight: fp32 [cache_rows], to which the step's
  * attention weights are added (row pos starts at zero), or null.  kv_lora_rank 512, rope_dim 64, nope_dim and v_dim multiples of 8 up to 256 and 1024; the
  * rest as there. */
 int k3_mla_step_decode_q4(const void *x, int x_dtype, const void *q_a, const float *q_a_norm, const void *q_b, const void *kv_a,

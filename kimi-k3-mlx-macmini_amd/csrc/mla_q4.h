@@ -92,6 +92,18 @@ __device__ __forceinline__ float q4_rows_max(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// Sum over the 16 lanes of a row, in every lane of it.
+__device__ __forceinline__ float q4_row16_sum(float v) {
+    auto turned = [&](auto ctrl) __attribute__((always_inline)) {
+        return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    v += turned(std::integral_constant<int, 0xb1>{});    // quad_perm [1,0,3,2]
+    v += turned(std::integral_constant<int, 0x4e>{});    // quad_perm [2,3,0,1]
+    v += turned(std::integral_constant<int, 0x124>{});   // row_ror:4
+    v += turned(std::integral_constant<int, 0x128>{});   // row_ror:8
+    return v;
+}
+
 // bf16 pair (RNE, hardware conversion) of (a, b): low half a
 __device__ __forceinline__ uint32_t q4_pack_bf16(float a, float b) {
     const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};

@@ -41,13 +41,17 @@ typedef __attribute__((address_space(3))) i32x2 *lds_i2;
 // launches, which takes one head's matrix, writes and reads whole tiles).
 struct Rows {
     int T, H, Tp;                           // Tp 0: by query
+    uint32_t inverse;                       // ceil(2^32 / d), d = Tp or H (0: d is 1): exact for the rows of a pass, row d < 2^32
     __host__ __device__ int count() const { return Tp ? H * Tp : T * H; }
     __device__ int of(int t, int h) const { return Tp ? h * Tp + t : t * H + h; }
-    __device__ int query(int row) const { return Tp ? row % Tp : row / H; }       // may be >= T: no row
+    // row / d by a multiplication (the weight sums divide several times a tile)
+    __device__ int major(int row) const { return inverse ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), inverse)) : row; }
+    __device__ int query(int row) const { return Tp ? row - major(row) * Tp : major(row); }       // may be >= T: no row
     // the last query of rows row0 .. row1
     __device__ int last_query(int row0, int row1) const {
-        if (!Tp) return row1 / H;
-        return row0 / Tp != row1 / Tp ? T - 1 : min(row1 % Tp, T - 1);
+        const int last = major(row1);
+        if (!Tp) return last;
+        return major(row0) != last ? T - 1 : min(row1 - last * Tp, T - 1);
     }
 };
 
@@ -470,17 +474,25 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         // round rd's scores; their maximum over the wave's tiles
         auto scores = [&](int rd, f32x4 (&out)[NTILE]) __attribute__((always_inline)) {
             float top = -INFINITY;
+            struct Keys {
+                u32x4 c[kQ4Steps], o[2];
+                int scale;
+            } keys[2];                                      // a tile's are read while the one's before are multiplied
+            auto read = [&](int u, Keys &t) __attribute__((always_inline)) {
+                const int at = (tg * NTILE + u) * 16;
+                const char *k = kbuf + rd % kSlots * kKBytes + (at + r16) * kKLd, *o = rbuf + (rd & 1) * kRBytes + (at + r16) * kRLd + q4 * 16;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) t.o[x] = *reinterpret_cast<const u32x4 *>(o + x * 64);
+                t.scale = *reinterpret_cast<const int *>(k + 256 + q4 * 4);
+#pragma unroll
+                for (int s = 0; s < kQ4Steps; ++s) t.c[s] = *reinterpret_cast<const u32x4 *>(k + q4 * 64 + s * 16);
+            };
+            read(0, keys[0]);
 #pragma unroll
             for (int u = 0; u < NTILE; ++u) {
                 const int at = (tg * NTILE + u) * 16;
-                const char *k = kbuf + rd % kSlots * kKBytes + (at + r16) * kKLd, *o = rbuf + (rd & 1) * kRBytes + (at + r16) * kRLd + q4 * 16;
-                const int ks = *reinterpret_cast<const int *>(k + 256 + q4 * 4);
-                u32x4 kc[kQ4Steps];
-#pragma unroll
-                for (int s = 0; s < kQ4Steps; ++s) kc[s] = *reinterpret_cast<const u32x4 *>(k + q4 * 64 + s * 16);
-                u32x4 oc[2];
-#pragma unroll
-                for (int x = 0; x < 2; ++x) oc[x] = *reinterpret_cast<const u32x4 *>(o + x * 64);
+                const Keys &t = keys[u & 1];
+                if (u + 1 < NTILE) read(u + 1, keys[(u + 1) & 1]);
                 f32x4 d[4];                                 // the terms in chains of their own
 #pragma unroll
                 for (int x = 0; x < 4; ++x) d[x] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -488,14 +500,14 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
                     for (int x = RT - 1; x >= 0; --x)
-                        d[3] = q4_mfma_bf16(oc[s], *reinterpret_cast<const u32x4 *>(qr + (2 * x + s) * 1024), d[3]);
+                        d[3] = q4_mfma_bf16(t.o[s], *reinterpret_cast<const u32x4 *>(qr + (2 * x + s) * 1024), d[3]);
 #pragma unroll
                 for (int x = NT - 1; x >= 0; --x) {
                     f32x4 &c = d[x < 3 ? x : 3];
-                    c = q4_mfma<0>(kc[0], ks, qlo[x][0], qhi[x][0], qs[x], c);
-                    c = q4_mfma<1>(kc[1], ks, qlo[x][1], qhi[x][1], qs[x], c);
-                    c = q4_mfma<2>(kc[2], ks, qlo[x][2], qhi[x][2], qs[x], c);
-                    c = q4_mfma<3>(kc[3], ks, qlo[x][3], qhi[x][3], qs[x], c);
+                    c = q4_mfma<0>(t.c[0], t.scale, qlo[x][0], qhi[x][0], qs[x], c);
+                    c = q4_mfma<1>(t.c[1], t.scale, qlo[x][1], qhi[x][1], qs[x], c);
+                    c = q4_mfma<2>(t.c[2], t.scale, qlo[x][2], qhi[x][2], qs[x], c);
+                    c = q4_mfma<3>(t.c[3], t.scale, qlo[x][3], qhi[x][3], qs[x], c);
                 }
                 const f32x4 s = d[0] + ((d[3] + d[2]) + d[1]);
 #pragma unroll
@@ -613,13 +625,31 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
             for (int c = 0; c < 8; ++c)
                 code[c] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i2)(k + c * 8)));
             float f[RG];
-            bool any = false;
-            stage();
 #pragma unroll
-            for (int r = 0; r < RG; ++r) {
-                f[r] = xf[rd & 1][r * 16 + r16];
-                any = any || f[r] != 1.f;
+            for (int r = 0; r < RG; ++r) f[r] = xf[rd & 1][r * 16 + r16];
+            // 8 of the lane's 16 positions a step: their probabilities, and a scale for every 32 columns.  With up to 32 rows all of them
+            // are read before the next round is stored (the stores would hold them up: 19.9 us for 18.6 over 32,768 positions).
+            constexpr bool kFirst = RG <= 2;
+            u32x4 pf[kFirst ? 2 : 1][RG][N], h[kFirst ? 2 : 1][4];
+            auto probabilities = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+                for (int r = 0; r < RG; ++r)
+#pragma unroll
+                    for (int x = 0; x < N; ++x) pf[kFirst ? s : 0][r][x] = *reinterpret_cast<const u32x4 *>(p + r * kPLd + x * 2048 + s * 256);
+            };
+            auto scale = [&](int s, int g) __attribute__((always_inline)) { h[kFirst ? s : 0][g] = *reinterpret_cast<const u32x4 *>(t + g * (2 * kRound) + s * 16); };
+            if (kFirst) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    probabilities(s);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) scale(s, g);
+                }
             }
+            stage();
+            bool any = false;
+#pragma unroll
+            for (int r = 0; r < RG; ++r) any = any || f[r] != 1.f;
             if (__any(any)) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
@@ -627,22 +657,19 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                     for (int r = 0; r < RG; ++r) acc[c][r] *= f[r];
             }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {                   // 8 of the lane's 16 positions
-                u32x4 pf[RG][N];
+            for (int s = 0; s < 2; ++s) {
+                const int b = kFirst ? s : 0;
+                if (!kFirst) probabilities(s);
 #pragma unroll
-                for (int r = 0; r < RG; ++r)
-#pragma unroll
-                    for (int x = 0; x < N; ++x) pf[r][x] = *reinterpret_cast<const u32x4 *>(p + r * kPLd + x * 2048 + s * 256);
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {               // 32 columns: one scale a position
-                    const u32x4 h = *reinterpret_cast<const u32x4 *>(t + g * (2 * kRound) + s * 16);
+                for (int g = 0; g < 4; ++g) {               // 32 columns
+                    if (!kFirst) scale(s, g);
 #pragma unroll
                     for (int c = 2 * g; c < 2 * g + 2; ++c) {
-                        const u32x4 v = kBf ? q4_values_bf16(code[c][s], h) : q4_values_f16(code[c][s], h);
+                        const u32x4 v = kBf ? q4_values_bf16(code[c][s], h[b][g]) : q4_values_f16(code[c][s], h[b][g]);
 #pragma unroll
                         for (int x = N - 1; x >= 0; --x)
 #pragma unroll
-                            for (int r = 0; r < RG; ++r) acc[c][r] = kBf ? q4_mfma_bf16(v, pf[r][x], acc[c][r]) : q4_mfma_f16(v, pf[r][x], acc[c][r]);
+                            for (int r = 0; r < RG; ++r) acc[c][r] = kBf ? q4_mfma_bf16(v, pf[b][r][x], acc[c][r]) : q4_mfma_f16(v, pf[b][r][x], acc[c][r]);
                     }
                     if (RG == 4) __builtin_amdgcn_sched_barrier(0);
                 }
@@ -702,7 +729,7 @@ struct UvArgs {
     void *out;               // [B, Tall, H, V]
     int out_bf16;
     const float *gate;       // [B, Tall, H, V] or null
-    float2 *stats;           // [B][rows]: maximum less kLift, 1 / sum (which is lifted); or null
+    float *stats;            // [B][rows]: log2 of what a probability's exponential is divided by; or null
     const int2 *seq;         // the sequences' records, or null: NS each
     Rows order;
     int M, V, rows, NS, Tall, t0;
@@ -747,7 +774,8 @@ __device__ __forceinline__ void record_weights(const UvArgs &a, int b, int row, 
     const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
     for (int u = 0; u < kMaxSplits / 64; ++u) w[u] = v[u].y == 0.f ? 0.f : w[u] * inv;
-    if (stats && a.stats && lane == 0) a.stats[static_cast<int64_t>(b) * a.rows + row] = make_float2(mx - kLift, inv);
+    // (the sum is lifted by kLift; a row that sees nothing has no probabilities)
+    if (stats && a.stats && lane == 0) a.stats[static_cast<int64_t>(b) * a.rows + row] = l == 0.f ? 0.f : mx - kLift + __log2f(l);
 }
 
 // Few queries: grid (H, ceil(M / per), Z), WAVES waves, queries per y .. +per (at most 16) of head x, VT tiles of 16 output columns
@@ -965,31 +993,38 @@ __global__ __launch_bounds__(256, 2) void uv_many_kernel(UvArgs a) {
 // ------------------------------------------------------------------ weights
 struct WeightArgs {
     AttendArgs a;
-    const float2 *stats;     // [B][rows]
-    float *part;             // [chunks][B][npos]
+    const float *stats;      // [B][rows]
+    float *part;             // [chunks][B][pitch]
     float *weight;           // [B] rows of w_b floats
     int64_t w_b;
-    int tiles, chunk, chunks, npos;
+    int tiles, chunk, chunks;
+    int64_t pitch;           // npos in whole blocks
 };
 constexpr int kWTiles = 4;   // tiles of 16 positions per wave
 
 // grid (ceil(npos / 512), chunks, B): a wave keeps 64 positions' codes in registers; the block takes the row tiles
 // chunk y .. of its sequence one after the other, each staged in LDS for its eight waves while the last one is worked on, and adds
-// their probabilities; part[chunk][b][position].  Bound by the matrix cores and, with few rows, by the first loads.
+// their probabilities, exp2(c s - log2 of the row's divisor); part[chunk][b][position].  One block a CU: 4000 tiles of 1000 queries of 64 heads
+// over as many positions take 100 us, 6000 cycles a tile where its products need 2800 (the rest: exponentials, and the products'
+// operands from LDS, 34 KB a wave); one tile over 20,001 positions 9 us, most of it the first loads.
 template <int NT, int RT>
 __global__ __launch_bounds__(512, 1) void weights_kernel(WeightArgs wa) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int kBytes = q4_tile_bytes(NT, RT), kLoads = (kBytes + 8191) / 8192;
     const AttendArgs &a = wa.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
-    const int b = blockIdx.z, jb = blockIdx.x * (8 * 16 * kWTiles), j0 = jb + wave * (16 * kWTiles);
+    // the blocks of one chunk on one XCD (blocks b % 8), so that its L2 reads the tiles once
+    const int id = blockIdx.y * gridDim.x + blockIdx.x, turn = id / (8 * gridDim.x), place = id % (8 * gridDim.x);
+    const bool whole = 8 * (turn + 1) <= static_cast<int>(gridDim.y);
+    const int chunk = whole ? 8 * turn + (place & 7) : blockIdx.y, pos = whole ? place >> 3 : blockIdx.x;
+    const int b = blockIdx.z, jb = pos * (8 * 16 * kWTiles), j0 = jb + wave * (16 * kWTiles);
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.cap) : a.length;
     const int cnt = a.counts ? min(max(a.counts[b], 0), a.count) : a.count;
     const int n = min(len - j0, 16 * kWTiles);     // positions there are from j0 on
     f32x4 sum[kWTiles];
 #pragma unroll
     for (int u = 0; u < kWTiles; ++u) sum[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int last = min(wa.tiles, (static_cast<int>(blockIdx.y) + 1) * wa.chunk);
+    const int last = min(wa.tiles, (chunk + 1) * wa.chunk);
     // positions that the rows of tile i see
     auto seen = [&](int i) __attribute__((always_inline)) {
         const int t = min(a.t0 + a.order.last_query(16 * i, min(16 * i + 16, a.rows) - 1), cnt - 1);
@@ -999,119 +1034,126 @@ __global__ __launch_bounds__(512, 1) void weights_kernel(WeightArgs wa) {
         while (i < last && seen(i) <= jb) ++i;
         return i;
     };
-    u32x4 stage[kLoads];
-    auto load = [&](int i) __attribute__((always_inline)) {
-        const char *tile = a.qop + b * a.q_seq + static_cast<int64_t>(min(i, wa.tiles - 1)) * kBytes;
+    struct Stage {          // the next tile, loaded before this one's products and stored after them
+        u32x4 q[kLoads];
+        float st;
+    };
+    auto load = [&](int i, Stage &g) __attribute__((always_inline)) {
+        i = min(i, wa.tiles - 1);
+        g.st = wa.stats[static_cast<int64_t>(b) * a.rows + min(i * 16 + r16, a.rows - 1)];
+        const char *tile = a.qop + b * a.q_seq + static_cast<int64_t>(i) * kBytes;
 #pragma unroll
         for (int u = 0; u < kLoads; ++u)
-            stage[u] = *reinterpret_cast<const u32x4 *>(tile + min(u * 8192 + tid * 16, kBytes - 16));
+            g.q[u] = *reinterpret_cast<const u32x4 *>(tile + min(u * 8192 + tid * 16, kBytes - 16));
     };
-    auto store = [&](int buf) __attribute__((always_inline)) {
+    auto store = [&](int buf, const Stage &g) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kLoads; ++u)
-            if (u * 8192 + tid * 16 < kBytes) *reinterpret_cast<u32x4 *>(lds + buf * kBytes + u * 8192 + tid * 16) = stage[u];
+            if (u * 8192 + tid * 16 < kBytes) *reinterpret_cast<u32x4 *>(lds + buf * kBytes + u * 8192 + tid * 16) = g.q[u];
     };
-    int i = next(blockIdx.y * wa.chunk);
-    load(i);
+    Stage g;
+    int i = next(chunk * wa.chunk);
+    load(i, g);
+    // The wave's positions.  Their codes come in as whole rows, sixteen lanes a row, and take their lanes' order through LDS (a row
+    // quarter to a lane, they took 9.5 us of a launch's 15 for one tile of queries over 20,001 positions), where the second tile will be.
     u32x4 kc[kWTiles][kQ4Steps], ro[kWTiles][2];
     int ks[kWTiles];
-    if (n > 0) {
-        const auto rp = make_rsrc(a.packed + b * a.p_b + j0 * a.p_t, static_cast<uint32_t>((n - 1) * a.p_t + 256));
-        const auto rs = make_rsrc(a.scales + b * a.s_b + j0 * a.s_t, static_cast<uint32_t>((n - 1) * a.s_t + 16));
-        const auto rr = make_rsrc(a.rot + b * a.r_b + j0 * a.r_t, static_cast<uint32_t>((n - 1) * a.r_t + 128));
+    {
+        const int64_t there = max(n, 0), first = n > 0 ? j0 : 0;
+        const auto rp = make_rsrc(a.packed + b * a.p_b + first * a.p_t, static_cast<uint32_t>(there ? (there - 1) * a.p_t + 256 : 0));
+        const auto rs = make_rsrc(a.scales + b * a.s_b + first * a.s_t, static_cast<uint32_t>(there ? (there - 1) * a.s_t + 16 : 0));
+        const auto rr = make_rsrc(a.rot + b * a.r_b + first * a.r_t, static_cast<uint32_t>(there ? (there - 1) * a.r_t + 128 : 0));
+        const uint32_t pt = static_cast<uint32_t>(a.p_t), rt = static_cast<uint32_t>(a.r_t), st = static_cast<uint32_t>(a.s_t);
 #pragma unroll
-        for (int u = 0; u < kWTiles; ++u) {
-            const int j = u * 16 + r16;
-            const bool ok = j < n;
+        for (int u = 0; u < kWTiles; ++u) {         // (rows past the last are outside and load zeros)
 #pragma unroll
             for (int s = 0; s < kQ4Steps; ++s)
-                kc[u][s] = __builtin_bit_cast(u32x4, buf_load16(rp, ok ? static_cast<uint32_t>(j) * static_cast<uint32_t>(a.p_t) + q4 * 64u + s * 16u : kOobOffset));
+                kc[u][s] = __builtin_bit_cast(u32x4, buf_load16(rp, static_cast<uint32_t>(u * 16 + 4 * s + q4) * pt + r16 * 16u));
 #pragma unroll
             for (int s = 0; s < 2; ++s)
-                ro[u][s] = __builtin_bit_cast(u32x4, buf_load16(rr, ok ? static_cast<uint32_t>(j) * static_cast<uint32_t>(a.r_t) + s * 64u + q4 * 16u : kOobOffset));
-            uint32_t k4 = 0;
-#pragma unroll
-            for (int s = 0; s < kQ4Steps; ++s)
-                k4 |= static_cast<uint32_t>(__builtin_amdgcn_raw_buffer_load_b8(
-                          rs, ok ? static_cast<uint32_t>(j) * static_cast<uint32_t>(a.s_t) + q4 * 4u + s : kOobOffset, 0, 0)) << (8 * s);
-            ks[u] = static_cast<int>(k4);
+                ro[u][s] = __builtin_bit_cast(u32x4, buf_load16(rr, static_cast<uint32_t>(u * 16 + r16) * rt + s * 64u + q4 * 16u));
+            ks[u] = static_cast<int>(buf_load4(rs, static_cast<uint32_t>(u * 16 + r16) * st + q4 * 4u));
         }
-    } else {
+        char *const x = lds + kBytes + wave * (16 * kKLd);
 #pragma unroll
         for (int u = 0; u < kWTiles; ++u) {
-            ks[u] = 0;
 #pragma unroll
-            for (int s = 0; s < kQ4Steps; ++s) kc[u][s] = u32x4{0u, 0u, 0u, 0u};
-            ro[u][0] = ro[u][1] = u32x4{0u, 0u, 0u, 0u};
+            for (int s = 0; s < kQ4Steps; ++s) *reinterpret_cast<u32x4 *>(x + (4 * s + q4) * kKLd + r16 * 16) = kc[u][s];
+#pragma unroll
+            for (int s = 0; s < kQ4Steps; ++s) kc[u][s] = *reinterpret_cast<const u32x4 *>(x + r16 * kKLd + q4 * 64 + s * 16);
         }
     }
-    int buf = 0;
-    store(0);
+    store(0, g);
+    __builtin_amdgcn_s_waitcnt(0x0f70);     // vmcnt(0): all is here (else every tile's first product would wait for the next tile's loads)
     __syncthreads();
+    int buf = 0;
     while (i < last) {
-        const int following = next(i + 1);
-        if (following < last) load(following);
+        const float st = g.st;
+        const int ahead = next(i + 1);
+        if (ahead < last) load(ahead, g);
         const char *tile = lds + buf * kBytes + lane * 16;
         if (n > 0 && seen(i) > j0) {
             const int row = i * 16 + r16, tq = a.order.query(row);
-            const bool there = row < a.rows && tq < a.order.T;
-            const int limit = (there ? q4_sees(a.t0 + tq, cnt, len) : 0) - j0;
-            const float2 st = there ? wa.stats[static_cast<int64_t>(b) * a.rows + row] : make_float2(0.f, 0.f);
-            f32x4 hi[kWTiles], lo[kWTiles];
+            const int limit = (row < a.rows && tq < a.order.T ? q4_sees(a.t0 + tq, cnt, len) : 0) - j0;
+            struct Term {
+                u32x4 lo[kQ4Steps];
+                u32x2 hi[kQ4Steps];
+                int scale;
+            } q[2];                         // a term's operands are read while the one's before are multiplied
+            auto operands = [&](int x, Term &t) __attribute__((always_inline)) {
+                t.scale = *reinterpret_cast<const int *>(tile + q4_scale_at(NT, x) - lane * 12);
 #pragma unroll
-            for (int u = 0; u < kWTiles; ++u) hi[u] = lo[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int s = 0; s < kQ4Steps; ++s) {
+                    t.lo[s] = *reinterpret_cast<const u32x4 *>(tile + q4_code_at(x, s));
+                    t.hi[s] = *reinterpret_cast<const u32x2 *>(tile + q4_code_at(x, s) + 1024 - lane * 8);
+                }
+            };
+            f32x4 d[kWTiles];               // the smallest terms first
+#pragma unroll
+            for (int u = 0; u < kWTiles; ++u) d[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            operands(NT - 1, q[(NT - 1) & 1]);
 #pragma unroll
             for (int x = RT - 1; x >= 0; --x)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const u32x4 qr = *reinterpret_cast<const u32x4 *>(tile + q4_rope_at(NT, x, s));
 #pragma unroll
-                    for (int u = 0; u < kWTiles; ++u) lo[u] = q4_mfma_bf16(ro[u][s], qr, lo[u]);
+                    for (int u = 0; u < kWTiles; ++u) d[u] = q4_mfma_bf16(ro[u][s], qr, d[u]);
                 }
 #pragma unroll
             for (int x = NT - 1; x >= 0; --x) {
-                const int qs = *reinterpret_cast<const int *>(tile + q4_scale_at(NT, x) - lane * 12);
-                u32x4 qlo[kQ4Steps];
-                u32x2 qhi[kQ4Steps];
+                if (x > 0) operands(x - 1, q[(x - 1) & 1]);
+                const Term &t = q[x & 1];
 #pragma unroll
-                for (int s = 0; s < kQ4Steps; ++s) {
-                    qlo[s] = *reinterpret_cast<const u32x4 *>(tile + q4_code_at(x, s));
-                    qhi[s] = *reinterpret_cast<const u32x2 *>(tile + q4_code_at(x, s) + 1024 - lane * 8);
-                }
+                for (int u = 0; u < kWTiles; ++u) d[u] = q4_mfma<0>(kc[u][0], ks[u], t.lo[0], t.hi[0], t.scale, d[u]);
 #pragma unroll
-                for (int u = 0; u < kWTiles; ++u) {
-                    f32x4 &d = x < 2 ? hi[u] : lo[u];
-                    d = q4_mfma<0>(kc[u][0], ks[u], qlo[0], qhi[0], qs, d);
-                    d = q4_mfma<1>(kc[u][1], ks[u], qlo[1], qhi[1], qs, d);
-                    d = q4_mfma<2>(kc[u][2], ks[u], qlo[2], qhi[2], qs, d);
-                    d = q4_mfma<3>(kc[u][3], ks[u], qlo[3], qhi[3], qs, d);
-                }
+                for (int u = 0; u < kWTiles; ++u) d[u] = q4_mfma<1>(kc[u][1], ks[u], t.lo[1], t.hi[1], t.scale, d[u]);
+#pragma unroll
+                for (int u = 0; u < kWTiles; ++u) d[u] = q4_mfma<2>(kc[u][2], ks[u], t.lo[2], t.hi[2], t.scale, d[u]);
+#pragma unroll
+                for (int u = 0; u < kWTiles; ++u) d[u] = q4_mfma<3>(kc[u][3], ks[u], t.lo[3], t.hi[3], t.scale, d[u]);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int u = 0; u < kWTiles; ++u)
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
-                    const float p = __builtin_amdgcn_exp2f((hi[u][v] + lo[u][v]) * a.c - st.x) * st.y;
+                    const float p = __builtin_amdgcn_exp2f(fmaf(d[u][v], a.c, -st));
                     sum[u][v] += u * 16 + 4 * q4 + v < limit ? p : 0.f;
                 }
         }
-        if (following < last) store(buf ^ 1);
+        if (ahead < last) store(buf ^ 1, g);
         __syncthreads();
-        buf ^= 1, i = following;
+        buf ^= 1, i = ahead;
     }
     // over the 16 rows of the tiles (lanes of a DPP row), in a fixed order
-    if (j0 >= wa.npos) return;
-    float *out = wa.part + (static_cast<int64_t>(blockIdx.y) * a.B + b) * wa.npos + j0;
+    float *out = wa.part + (static_cast<int64_t>(chunk) * a.B + b) * wa.pitch + j0 + 4 * q4;
 #pragma unroll
-    for (int u = 0; u < kWTiles; ++u)
+    for (int u = 0; u < kWTiles; ++u) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            float p = sum[u][v];
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) p += __shfl_xor(p, o);
-            const int j = u * 16 + 4 * q4 + v;
-            if (r16 == 0 && j0 + j < wa.npos) out[j] = p;
-        }
+        for (int v = 0; v < 4; ++v) sum[u][v] = q4_row16_sum(sum[u][v]);
+        if (r16 == 0) *reinterpret_cast<f32x4 *>(out + u * 16) = sum[u];
+    }
 }
 
 // weight[b][j] += the chunks' sums: four threads a position, each every fourth chunk, added in order
@@ -1119,8 +1161,8 @@ __global__ __launch_bounds__(256) void weights_add_kernel(WeightArgs wa) {
     __shared__ float part[4][64];
     const int c = threadIdx.x & 63, g = threadIdx.x >> 6, j = blockIdx.x * 64 + c, b = blockIdx.y;
     const int len = wa.a.lengths ? min(max(wa.a.lengths[b], 0), wa.a.cap) : wa.a.length;
-    const float *src = wa.part + static_cast<int64_t>(b) * wa.npos + j;
-    const int64_t pitch = static_cast<int64_t>(wa.a.B) * wa.npos;
+    const float *src = wa.part + b * wa.pitch + j;
+    const int64_t pitch = wa.a.B * wa.pitch;
     float s = 0.f;
     if (j < len) {
 #pragma unroll 8
@@ -1143,7 +1185,8 @@ constexpr int kByHead = 32;               // queries of a sequence from which ro
 constexpr int kManyQueries = 48;          // queries (all sequences) from which uv_many takes less than uv_few
 
 Rows rows_of(int64_t T, int64_t H) {
-    return Rows{static_cast<int>(T), static_cast<int>(H), T >= kByHead ? static_cast<int>(cdiv(T, 16) * 16) : 0};
+    const int64_t Tp = T >= kByHead ? cdiv(T, 16) * 16 : 0, d = Tp ? Tp : H;
+    return Rows{static_cast<int>(T), static_cast<int>(H), static_cast<int>(Tp), d == 1 ? 0u : static_cast<uint32_t>(cdiv(1ll << 32, d))};
 }
 
 // What the launches are cut into; a function of its arguments alone.
@@ -1183,7 +1226,7 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
     p.Ts = static_cast<int>(ts);
     p.many = !p.listed && B * p.order.T >= kManyQueries;
     const int64_t pos_blocks = std::max<int64_t>(1, cdiv(npos, 128 * kWTiles));
-    p.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.tiles, 512 / (pos_blocks * B))));
+    p.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.tiles, 256 / (pos_blocks * B))));
     p.chunk = static_cast<int>(cdiv(p.tiles, p.chunks));
     p.chunks = static_cast<int>(cdiv(p.tiles, p.chunk));
     auto up = [](int64_t v) { return (v + 255) & ~int64_t(255); };
@@ -1193,8 +1236,8 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
     p.part = o, o += up(p.slots * rows * kQ4Lat * 4);
     p.slot = o, o += p.listed ? up(p.slots * 16) : 0;
     p.seq = o, o += p.listed ? up(B * 8) : 0;
-    p.stats = o, o += weights ? up(B * rows * 8) : 0;
-    p.wpart = o, o += weights ? up(static_cast<int64_t>(p.chunks) * B * npos * 4) : 0;
+    p.stats = o, o += weights ? up(B * rows * 4) : 0;
+    p.wpart = o, o += weights ? up(p.chunks * B * pos_blocks * (128 * kWTiles) * 4) : 0;
     p.total = o;
     return p;
 }
@@ -1234,48 +1277,55 @@ int launch_qa(const QaArgs &a, hipStream_t st) {
     return a.M > 32 ? launch_qa_of<QT, NT, RT, 4>(a, st) : launch_qa_of<QT, NT, RT, 1>(a, st);
 }
 
-int launch_uv(const UvArgs &a, int many, hipStream_t st) {
-    static const hipError_t few16 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_few_kernel<16, 8>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds);
-    static const hipError_t few8 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_few_kernel<8, 4>),
+template <int WAVES, int VT>
+int launch_few(const UvArgs &a, int per, unsigned tiles, hipStream_t st) {
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_few_kernel<WAVES, VT>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds);
+    const int rc = check_hip(attr, "mla q4: output LDS size");
+    if (rc) return rc;
+    uv_few_kernel<WAVES, VT><<<dim3(static_cast<unsigned>(a.order.H), tiles, 8 / VT), 64 * WAVES, kFewLds, st>>>(a, per);
+    return check_hip(hipGetLastError(), "mla q4: join and W_UV launch");
+}
+
+int launch_uv(const UvArgs &a, int many, hipStream_t st) {
+    const unsigned H = static_cast<unsigned>(a.order.H);
+    if (!many) {
+        // The fewest queries to a block with which all blocks run at once (one a CU, for its LDS); then the output columns in as many
+        // parts (8 waves hold half of them), which join the same records (1 token of 64 heads with 64 records: 40.7 us in all in one part, 37.7 in two, 37.2 in four;
+        // 32 tokens, in one part a block a CU: 42.3, 47.4, 57.6).
+        const int least = a.NS <= kFewSplits ? 2 : 1;
+        int per = static_cast<int>(std::min<int64_t>(16, a.M));
+        while (per > 1 && least * H * cdiv(a.M, per - 1) <= 256) --per;
+        const unsigned tiles = static_cast<unsigned>(cdiv(a.M, per)), blocks = H * tiles;
+        if (a.NS <= kFewSplits) return blocks <= 64 ? launch_few<8, 2>(a, per, tiles, st) : launch_few<8, 4>(a, per, tiles, st);
+        return blocks <= 64 ? launch_few<16, 2>(a, per, tiles, st) : blocks <= 128 ? launch_few<16, 4>(a, per, tiles, st)
+                                                                                  : launch_few<16, 8>(a, per, tiles, st);
+    }
     static const hipError_t many2 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_many_kernel<2>),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 64 * 272 + 64 * kMaxSplits * 4);
     static const hipError_t many3 = hipFuncSetAttribute(reinterpret_cast<const void *>(uv_many_kernel<3>),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 3 * 64 * 272 + 64 * kMaxSplits * 4);
-    const int rc = check_hip(!many ? (few8 != hipSuccess ? few8 : few16) : a.out_bf16 ? many2 : many3, "mla q4: output LDS size");
+    const int rc = check_hip(a.out_bf16 ? many2 : many3, "mla q4: output LDS size");
     if (rc) return rc;
-    const unsigned H = static_cast<unsigned>(a.order.H);
-    if (!many) {
-        // the fewest queries to a block with which all blocks run at once (one a CU, for its LDS)
-        const int z = a.NS <= kFewSplits ? 2 : 1;
-        int per = static_cast<int>(std::min<int64_t>(16, a.M));
-        while (per > 1 && z * H * cdiv(a.M, per - 1) <= 256) --per;
-        const unsigned tiles = static_cast<unsigned>(cdiv(a.M, per));
-        if (a.NS <= kFewSplits)
-            uv_few_kernel<8, 4><<<dim3(H, tiles, z), 512, kFewLds, st>>>(a, per);
-        else
-            uv_few_kernel<16, 8><<<dim3(H, tiles), 1024, kFewLds, st>>>(a, per);
-    }
-    if (many && a.out_bf16)
+    if (a.out_bf16)
         uv_many_kernel<2><<<dim3(H, static_cast<unsigned>(cdiv(a.M, 64))), 256, 2 * 64 * 272 + 64 * a.NS * 4, st>>>(a);
-    else if (many)
+    else
         uv_many_kernel<3><<<dim3(H, static_cast<unsigned>(cdiv(a.M, 64))), 256, 3 * 64 * 272 + 64 * a.NS * 4, st>>>(a);
     return check_hip(hipGetLastError(), "mla q4: join and W_UV launch");
 }
 
 template <int RT>
 int launch_weights(const WeightArgs &wa, hipStream_t st) {
-    constexpr int bytes = 2 * q4_tile_bytes(5, RT);
+    constexpr int bytes = q4_tile_bytes(5, RT) + std::max(q4_tile_bytes(5, RT), 8 * 16 * kKLd);     // (the second tile's place also turns the codes)
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(weights_kernel<5, RT>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     int rc = check_hip(attr, "mla q4: weights LDS size");
     if (rc) return rc;
     const unsigned B = static_cast<unsigned>(wa.a.B);
-    weights_kernel<5, RT><<<dim3(static_cast<unsigned>(cdiv(wa.npos, 128 * kWTiles)), static_cast<unsigned>(wa.chunks), B), 512, bytes, st>>>(wa);
+    weights_kernel<5, RT><<<dim3(static_cast<unsigned>(wa.pitch / (128 * kWTiles)), static_cast<unsigned>(wa.chunks), B), 512, bytes, st>>>(wa);
     rc = check_hip(hipGetLastError(), "mla q4: weights launch");
     if (rc) return rc;
-    weights_add_kernel<<<dim3(static_cast<unsigned>(cdiv(wa.npos, 64)), B), 256, 0, st>>>(wa);
+    weights_add_kernel<<<dim3(static_cast<unsigned>(wa.pitch / 64), B), 256, 0, st>>>(wa);
     return check_hip(hipGetLastError(), "mla q4: weight sum launch");
 }
 
@@ -1314,12 +1364,12 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
                          (long long)H, (long long)max_length);
     if (qn_batch % 4 || qn_token % 4 || qn_head % 4 || qr_batch % 4 || qr_token % 4 || qr_head % 4)
         return set_error(K3_ERR_SHAPE, "mla q4: query strides must be multiples of 4 elements");
-    if (max_length > 0 && (p_row < 256 || p_row % 16 || p_batch % 16 || s_row < 16 || rot_row < kQ4Rope || rot_row % 8 ||
+    if (max_length > 0 && (p_row < 256 || p_row % 16 || p_batch % 16 || s_row < 16 || s_row % 4 || s_batch % 4 || rot_row < kQ4Rope || rot_row % 8 ||
                            rot_batch % 8 || p_row > (1 << 16) || s_row > (1 << 16) || rot_row > (1 << 15)))
-        return set_error(K3_ERR_SHAPE, "mla q4: cache row pitches too small, too large or not multiples of 16 bytes");
+        return set_error(K3_ERR_SHAPE, "mla q4: cache row pitches too small, too large or not multiples of 16 bytes (scales: 4)");
     if (!aligned16(q_nope) || !aligned16(q_rot) || !aligned16(w_uk) || !aligned16(w_uv) || !aligned16(out) || !aligned16(workspace) ||
-        !aligned16(packed) || !aligned16(rot) || (gate && !aligned16(gate)))
-        return set_error(K3_ERR_ALIGN, "mla q4: queries, weights, cache, output and workspace must be 16-byte aligned");
+        !aligned16(packed) || !aligned16(rot) || (reinterpret_cast<uintptr_t>(scales) & 3u) || (gate && !aligned16(gate)))
+        return set_error(K3_ERR_ALIGN, "mla q4: queries, weights, cache, output and workspace must be 16-byte (scales 4-byte) aligned");
     const Plan p = plan_of(B, T, H, v_dim, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weight != nullptr, lengths != nullptr);
     if (workspace_bytes < p.total)
         return set_error(K3_ERR_WORKSPACE, "mla q4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.total);
@@ -1364,7 +1414,7 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         UvArgs u{};
         u.part = a.part, u.ml = a.ml, u.w_uv = static_cast<const uint16_t *>(w_uv);
         u.out = out, u.out_bf16 = out_dtype == K3_BF16, u.gate = gate;
-        u.stats = weight ? reinterpret_cast<float2 *>(ws + p.stats) : nullptr;
+        u.stats = weight ? reinterpret_cast<float *>(ws + p.stats) : nullptr;
         u.seq = qa.ranges.seq;
         u.order = order, u.M = M, u.V = static_cast<int>(v_dim), u.rows = rows, u.NS = p.NS;
         u.Tall = static_cast<int>(T), u.t0 = a.t0;
@@ -1372,7 +1422,7 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         if (rc) return rc;
         if (weight && max_length > 0) {
             WeightArgs wa{a, u.stats, reinterpret_cast<float *>(ws + p.wpart), weight, w_batch, static_cast<int>(cdiv(rows, 16)), p.chunk,
-                          0, static_cast<int>(max_length)};
+                          0, cdiv(max_length, 128 * kWTiles) * (128 * kWTiles)};
             wa.chunks = static_cast<int>(cdiv(wa.tiles, wa.chunk));
             rc = p.RT == 1 ? launch_weights<1>(wa, st) : launch_weights<3>(wa, st);
             if (rc) return rc;

@@ -149,6 +149,8 @@ def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor
     capacity); ``counts`` int32 [B]: sequence b has only counts[b] queries, the first ones of its T.  A query that
     sees nothing gives zeros.
 
+    The cache's rows are read as they lie: ``packed`` and ``rot`` 16-byte aligned with pitches of whole 16 bytes, ``scales`` 4.
+
     ``weight`` fp32 [B, cap], changed in place: every position's attention weight, summed over the queries and heads, is
     added to it.  ``gate`` [B, T, H * v] fp32: the output times sigmoid(gate).
     """

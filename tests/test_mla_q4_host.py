@@ -149,11 +149,12 @@ def test_entry_points_check_their_arguments():
         assert attend(**{f"_{i}": n}) == _lib.K3_ERR_NULL, i
     assert attend(_8=4) == _lib.K3_ERR_DTYPE and attend(_33=9) == _lib.K3_ERR_DTYPE
     for at in ({"_26": 256}, {"_27": 32}, {"_28": 120 + 4}, {"_28": 264}, {"_28": 0}, {"_29": 1032}, {"_29": 92}, {"_25": 0}, {"_25": 5000},
-               {"_23": 40000}, {"_22": -1}, {"_22": (1 << 24) + 1}, {"_1": 1538}, {"_7": 63}, {"_13": 248}, {"_13": 264}, {"_16": 8},
+               {"_23": 40000}, {"_22": -1}, {"_22": (1 << 24) + 1}, {"_1": 1538}, {"_7": 63}, {"_13": 248}, {"_13": 264}, {"_16": 8}, {"_16": 18}, {"_15": 130},
                {"_19": 60}, {"_24": 1 << 25}):
         assert attend(**at) == _lib.K3_ERR_SHAPE, at
     for i in (0, 4, 9, 10, 11, 17, 32, 36):
         assert attend(**{f"_{i}": ctypes.c_void_p(4104)}) == _lib.K3_ERR_ALIGN, i
+    assert attend(_14=ctypes.c_void_p(4098)) == _lib.K3_ERR_ALIGN
     assert attend(_37=size - 1) == _lib.K3_ERR_WORKSPACE
     assert attend(_23=0) == _lib.K3_OK and attend(_24=0) == _lib.K3_OK
 
@@ -306,9 +307,10 @@ def test_step_entry_point_checks_its_arguments():
     for i in (0, 2, 3, 4, 5, 6, 7, 8, 10, 11, 13, 15, 22, 31):
         assert step(**{f"_{i}": n}) == _lib.K3_ERR_NULL, i
     assert step(_1=3) == _lib.K3_ERR_DTYPE and step(_23=3) == _lib.K3_ERR_DTYPE
-    for at in ({"_12": 255}, {"_12": 264}, {"_14": 15}, {"_16": 63}, {"_16": 68}, {"_18": 5}, {"_19": -1}, {"_19": 8}, {"_24": 60}, {"_25": 0},
+    for at in ({"_12": 255}, {"_12": 264}, {"_14": 15}, {"_14": 18}, {"_16": 63}, {"_16": 68}, {"_18": 5}, {"_19": -1}, {"_19": 8}, {"_24": 60}, {"_25": 0},
                {"_27": 264}, {"_28": 32}, {"_29": 1032}, {"_30": 256}, {"_18": (1 << 24) + 1}):
         assert step(**at) == _lib.K3_ERR_SHAPE, at
     for i in (0, 2, 3, 4, 5, 6, 7, 8, 10, 11, 15, 31):
         assert step(**{f"_{i}": ctypes.c_void_p(4104)}) == _lib.K3_ERR_ALIGN, i
+    assert step(_13=ctypes.c_void_p(4097)) == _lib.K3_ERR_ALIGN
     assert step(_32=size - 1) == _lib.K3_ERR_WORKSPACE
