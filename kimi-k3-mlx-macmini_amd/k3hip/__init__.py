@@ -7,6 +7,8 @@ Host-side mirror of the reference interfaces, backed by hand-written HIP kernels
                            mxfp4_matvec        (air_llm/models/kimi_k3/mxfp4.py)
 * ``k3hip.mxfp4_matvec``   mxfp4_matvec_fused / expert_projection
                            (air_llm/kernels/metal/mxfp4_matvec.py)
+* ``k3hip.mla_q4``         the 4-bit latent cache and its attention  (air_llm/models/kimi_k3/mla_quant.py)
+* ``k3hip.evict``          eviction by accumulated attention weight
 """
 from __future__ import annotations
 
