@@ -516,7 +516,7 @@ int64_t k3_mla_step_q4_workspace_size(int64_t q_lora_rank, int64_t heads, int64_
 
 /* k3_mla_step_decode over the 4-bit cache: row pos gets rmsnorm(ckv[:r], kv_a_norm) as k3_mla_q4_append rounds it
  * and bf16(ckv[r:]); the core is k3_mla_q4_attention's over rows 0..pos.  packed, scales, rot: one sequence's
- * cache_rows rows, pitches in elements (packed and rot rows whole 16 bytes, scale rows whole 4); weight: fp32 [cache_rows], to which the step's
+ * cache_rows rows, pitches in elements (packed and rot rows whole 16 bytes, scale rows whole 4, all up to 1 KB); weight: fp32 [cache_rows], to which the step's
  * attention weights are added (row pos starts at zero), or null.  kv_lora_rank 512, rope_dim 64, nope_dim and v_dim multiples of 8 up to 256 and 1024; the
  * rest as there. */
 int k3_mla_step_decode_q4(const void *x, int x_dtype, const void *q_a, const float *q_a_norm, const void *q_b, const void *kv_a,

@@ -185,7 +185,8 @@ extern "C" int k3_mla_step_decode_q4(const void *x, int x_dtype, const void *q_a
     if (kv_lora_rank != 512 || rope_dim != 64 || nope_dim % 8 || nope_dim <= 0 || nope_dim > 256 || v_dim % 8 || v_dim > 1024 ||
         heads > 4096 || cache_rows > (1 << 24))
         return set_error(K3_ERR_SHAPE, "mla step: the 4-bit cache takes kv_lora_rank 512, rope 64, nope up to 256, v up to 1024");
-    if (p_row < 256 || p_row % 16 || p_row > (1 << 16) || s_row < 16 || s_row % 4 || s_row > (1 << 16) || rot_row < 64 || rot_row % 8 || rot_row > (1 << 15))
+    // (pitches up to 1 KB: then no range of positions that the core takes spans 2 GiB, which it would refuse)
+    if (p_row < 256 || p_row % 16 || p_row > 1024 || s_row < 16 || s_row % 4 || s_row > 1024 || rot_row < 64 || rot_row % 8 || rot_row > 512)
         return set_error(K3_ERR_SHAPE, "mla step: cache row pitches too small, too large or not multiples of 16 bytes");
     if (!aligned16(packed) || !aligned16(rot) || (reinterpret_cast<uintptr_t>(scales) & 3u) || !aligned16(w_uk) || !aligned16(w_uv))
         return set_error(K3_ERR_ALIGN, "mla step: cache and weights must be 16-byte (scales 4-byte) aligned");

@@ -245,9 +245,8 @@ class MLAAttention:
             raise ValueError(f"mla_cache_bits {self.cache_bits}: the latent cache is held in 4 bits, or in mla_cache_dtype (None)")
         if self.cache_bits == 4 and getattr(cfg, "mla_cache_group_size", None) not in (None, 32):
             raise ValueError(f"mla_cache_group_size {cfg.mla_cache_group_size}: the 4-bit cache has a scale for every 32 values")
-        if self.cache_bits == 4 and (cfg.kv_lora_rank, cfg.qk_rope_head_dim) != (KV_LORA_RANK, ROPE_DIM):
-            raise ValueError(f"the 4-bit cache takes kv_lora_rank {KV_LORA_RANK} and qk_rope_head_dim {ROPE_DIM}; got "
-                             f"{cfg.kv_lora_rank}, {cfg.qk_rope_head_dim}")
+        if self.cache_bits == 4:
+            self._check_q4()
         mats = [self.q_a, self.q_b, self.kv_a, self.o_w] + ([self.g_w] if self.g_w is not None else [])
         self.fused_step = (all(m.dtype == torch.bfloat16 and m.is_cuda for m in mats)
                            and (self.cache_dtype == torch.bfloat16 or self.cache_bits == 4)
@@ -258,6 +257,15 @@ class MLAAttention:
             self._mats["g"] = T.contiguous_aligned(self.g_w) if self.g_w is not None else None
             self._q_an32 = T.contiguous_aligned(self.q_an.to(torch.float32))
             self._kv_an32 = T.contiguous_aligned(self.kv_an.to(torch.float32))
+
+    def _check_q4(self) -> None:
+        """Refuses head sizes that the 4-bit cache's kernels do not take."""
+        c = self.cfg
+        if ((c.kv_lora_rank, c.qk_rope_head_dim) != (KV_LORA_RANK, ROPE_DIM) or c.qk_nope_head_dim % 8 or c.qk_nope_head_dim > 256
+                or c.v_head_dim % 8 or c.v_head_dim > 1024 or c.num_attention_heads > 4096):
+            raise ValueError(f"the 4-bit cache takes kv_lora_rank {KV_LORA_RANK}, qk_rope_head_dim {ROPE_DIM}, qk_nope_head_dim and "
+                             f"v_head_dim multiples of 8 up to 256 and 1024, 4096 heads; got {c.kv_lora_rank}, {c.qk_rope_head_dim}, "
+                             f"{c.qk_nope_head_dim}, {c.v_head_dim}, {c.num_attention_heads}")
 
     @staticmethod
     def _mm(a: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
@@ -278,6 +286,8 @@ class MLAAttention:
         if cache is None and self.cache_bits == 4:
             cache = new_cache_q4(B, Tn, bool(getattr(c, "mla_cache_weights", False)), x.device)
         q4 = isinstance(cache, MLACacheQ4)
+        if q4:
+            self._check_q4()
         if q4 and T.tracked(x, self.q_a, self.q_an, self.q_b, self.kv_a, self.kv_an, self.kv_b, self.g_w, self.o_w):
             raise ValueError("the 4-bit cache carries no gradient: call the layer under no_grad or on detached tensors")
         if q4 and cache.weight is not None and self.kv_b.dtype != torch.bfloat16:
@@ -419,10 +429,12 @@ class MLAAttention:
         if isinstance(cache, MLACacheQ4):
             packed, scales, rot, weight = cache.packed, cache.scales, cache.rot, cache.weight
             T.require_device(xin, packed, scales, rot, weight)
+            p_row, s_row, rot_row = cache.row_pitches()
             nbytes = _lib.size("k3_mla_step_q4_workspace_size", ql, nh, nope, rope, vhd, klr, pos + 1, int(weight is not None))
-            ws = _workspace.get(x.device, nbytes, "mla_step")
-            _lib.call("k3_mla_step_decode_q4", *front, T.ptr(packed), packed.stride(1), T.ptr(scales), scales.stride(1), T.ptr(rot),
-                      rot.stride(1), T.ptr(weight), *back, T.ptr(ws), ws.numel(), T.stream(xin))
+            with T.current(x.device):
+                ws = _workspace.get(x.device, nbytes, "mla_step")
+                _lib.call("k3_mla_step_decode_q4", *front, T.ptr(packed), p_row, T.ptr(scales), s_row, T.ptr(rot), rot_row, T.ptr(weight), *back,
+                          T.ptr(ws), ws.numel(), T.stream(xin))
         else:
             lat, rot = cache.latent[0], cache.rot[0]
             nbytes = int(_lib.lib().k3_mla_step_workspace_size(hidden, ql, nh, nope, rope, vhd, klr, pos + 1))

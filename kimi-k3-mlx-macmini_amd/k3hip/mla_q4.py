@@ -111,6 +111,8 @@ def mla_q4_append(c_new: torch.Tensor, r_new: torch.Tensor, packed: torch.Tensor
     if starts is None and not 0 <= start0 <= start0 + n <= cap:
         raise ValueError(f"{n} tokens at position {start0} do not fit a capacity of {cap}")
     T.require_device(c_new, r_new, packed, scales, rot, starts, counts, weight)
+    if T.tracked(c_new, r_new):
+        raise ValueError("mla_q4_append carries no gradient: call it under no_grad or on detached tensors")
     if B == 0 or n == 0 or cap == 0:
         return
     if not c_ok or c_new.data_ptr() % 16:
@@ -230,7 +232,7 @@ class MLACacheQ4:
     def capacity(self) -> int:
         return self.packed.shape[1]
 
-    def _buffers(self) -> list[torch.Tensor]:
+    def buffers(self) -> list[torch.Tensor]:
         return [self.packed, self.scales, self.rot] + ([] if self.weight is None else [self.weight])
 
     def _take(self, buffers: list[torch.Tensor], length: int) -> "MLACacheQ4":
@@ -238,6 +240,14 @@ class MLACacheQ4:
         self.weight = buffers[3] if self.weight is not None else None
         self.length = length
         return self
+
+    def row_pitches(self) -> tuple[int, int, int]:
+        """The rows' pitches of a single sequence's buffers, in elements; refuses buffers of another form."""
+        B, cap = _buffers(self.packed, self.scales, self.rot)
+        if B != 1:
+            raise ValueError(f"a cache of {B} sequences for one sequence's token")
+        _weight_pitch(self.weight, B, cap)
+        return _pitches(self.packed)[1], _pitches(self.scales)[1], _pitches(self.rot)[1]
 
     def view(self) -> tuple[torch.Tensor, torch.Tensor]:
         """The valid prefix: latents decoded to fp32, rotary rows as they are (the kernels read the codes directly)."""
@@ -254,8 +264,8 @@ class MLACacheQ4:
         if need > self.capacity:
             from .mla import grown_capacity
             cap = grown_capacity(need, self.capacity)
-            new = [x.new_zeros((x.shape[0], cap, *x.shape[2:])) for x in self._buffers()]
-            for x, y in zip(self._buffers(), new):
+            new = [x.new_zeros((x.shape[0], cap, *x.shape[2:])) for x in self.buffers()]
+            for x, y in zip(self.buffers(), new):
                 y[:, :self.length] = x[:, :self.length]
             self._take(new, self.length)
         return self
@@ -280,7 +290,7 @@ class MLACacheQ4:
         if self.weight is None:
             raise ValueError("the cache keeps no attention weights (new_cache_q4(.., weights=True))")
         from .evict import cache_evict
-        new, index, _ = cache_evict(self.weight, self._buffers(), keep, lengths=self.length, sink=sink, recent=recent,
+        new, index, _ = cache_evict(self.weight, self.buffers(), keep, lengths=self.length, sink=sink, recent=recent,
                                     capacity=max(self.capacity, keep))
         self._take(new, min(self.length, keep))
         return index

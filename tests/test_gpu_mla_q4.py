@@ -95,6 +95,16 @@ def test_append_writes_only_its_positions(B, T, cap, start, counts):
                 assert bool((packed[b, j] == 7).all()) and bool((scales[b, j] == 7).all()) and bool((rot[b, j] == 7).all())
 
 
+def test_append_zeroes_the_weight_of_what_it_writes():
+    from k3hip.mla_q4 import mla_q4_append
+    B, T, cap = 4, 3, 10
+    w = torch.ones(B, 2 * cap, device="cuda")[:, 3:3 + cap]
+    mla_q4_append(_rand(1, B, T, 512).cuda(), _rand(2, B, T, 64).cuda(), *_cache(B, cap), start=_ints([0, 8, -1, 4]), counts=_ints([3, 3, 3, 1]),
+                  weight=w)
+    zero = [(w[b] == 0).nonzero().flatten().tolist() for b in range(B)]
+    assert zero == [[0, 1, 2], [8, 9], [0, 1], [4]] and int((w == 1).sum()) == B * cap - 8
+
+
 def test_append_nothing():
     from k3hip.mla_q4 import mla_q4_append
     packed, scales, rot = _cache(2, 4, 3)

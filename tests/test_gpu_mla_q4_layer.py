@@ -107,11 +107,11 @@ def test_prompt_decode_evict_decode(mats, heads, gate, dtype):
         total = torch.nn.functional.pad(total, (0, T)) + mass
         assert bool(((cache.weight[:, :cache.length].double() - total).abs() <= WEIGHT_TOL * total).all())
     assert cache.capacity == 512 and not cache.weight[:, cache.length:].any()
-    n, old = cache.length, [t.clone() for t in cache._buffers()]
+    n, old = cache.length, [t.clone() for t in cache.buffers()]
     index = cache.evict(100, sink=4, recent=32)
     assert index[0].tolist() == oracle.evict(old[3][0, :n].tolist(), n, 100, 4, 32)
     assert cache.length == 100 and cache.capacity == 512
-    for a, b in zip(cache._buffers(), old):
+    for a, b in zip(cache.buffers(), old):
         assert torch.equal(a[0, :100], b[0, index[0].long()]) and not a[:, 100:].any()
     total = total[:, index[0].long()]
     for i in range(3):
@@ -184,14 +184,43 @@ def test_masked_form_over_the_decoded_latents():
 def test_refusals_leave_the_cache(T):
     layer, w = _layer(4)
     _, cache = layer(_x(3, 1, 10))
-    before = [t.clone() for t in cache._buffers()]
+    before = [t.clone() for t in cache.buffers()]
     with pytest.raises(ValueError, match="no gradient"):
         layer(_x(4, 1, T).requires_grad_(), cache)
     layer, w = _layer(4, kv_b=F32, mats=F32)
     cache.weight = torch.zeros(1, cache.capacity, device="cuda")
     with pytest.raises(ValueError, match="no attention weights"):
         layer(_x(4, 1, T), cache)
-    assert cache.length == 10 and all(torch.equal(a, b) for a, b in zip(cache._buffers(), before))
+    assert cache.length == 10 and all(torch.equal(a, b) for a, b in zip(cache.buffers(), before))
+
+
+def test_another_batch_is_refused():
+    layer, w = _layer(4)
+    _, cache = layer(_x(3, 2, 10))
+    for T in (1, 2):
+        with pytest.raises(ValueError):
+            layer(_x(4, 1, T), cache)
+    assert cache.length == 10
+
+
+def test_a_callers_cache_and_layers_without_the_option():
+    """The cache decides: a 4-bit one runs in a layer made without the option, and a bf16 one in a layer made with it."""
+    from k3hip.mla import new_cache
+    from k3hip.mla_q4 import new_cache_q4
+    layer, w = _layer(8)
+    layer.cfg.mla_cache_bits = None
+    plain = type(layer)(layer.cfg, w)
+    cache, x = new_cache_q4(1, 50), _x(1, 1, 40)
+    out, same = plain(x, cache)
+    assert same is cache and cache.length == 40
+    _close(out, _want(w, 8, x, cache)[0])
+    out, _ = plain(_x(2, 1, 1), cache)
+    _close(out, _want(w, 8, _x(2, 1, 1), cache)[0])
+    a, b = new_cache(1, 512, 64, 50), new_cache(1, 512, 64, 50)
+    for t in (x, _x(2, 1, 1)):
+        y, _ = layer(t, a)
+        z, _ = plain(t, b)
+        assert torch.equal(y, z)
 
 
 def test_step_equals_the_calls_it_is_made_of():
@@ -206,7 +235,7 @@ def test_step_equals_the_calls_it_is_made_of():
     layer.fused_step, x = True, _x(2, 1, 1)
     a, _ = layer(x, strided)
     b, _ = layer(x, cache)
-    assert torch.equal(a, b) and all(torch.equal(s, t) for s, t in zip(strided._buffers(), cache._buffers()))
+    assert torch.equal(a, b) and all(torch.equal(s, t) for s, t in zip(strided.buffers(), cache.buffers()))
     cache.length -= 1
     layer.fused_step = False
     c, _ = layer(x, cache)

@@ -232,13 +232,14 @@ def _layer(cfg):
     from k3hip.mla import MLAAttention
     z = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
     klr, rope = cfg.kv_lora_rank, cfg.qk_rope_head_dim
-    return MLAAttention(cfg, {"q_a_proj.weight": z(64, 64), "q_a_layernorm.weight": z(64), "q_b_proj.weight": z(2 * 192, 64),
+    v = cfg.v_head_dim
+    return MLAAttention(cfg, {"q_a_proj.weight": z(64, 64), "q_a_layernorm.weight": z(64), "q_b_proj.weight": z(2 * cfg.q_head_dim, 64),
                               "kv_a_proj_with_mqa.weight": z(klr + rope, 64), "kv_a_layernorm.weight": z(klr),
-                              "kv_b_proj.weight": z(2 * 256, klr), "o_proj.weight": z(64, 256)})
+                              "kv_b_proj.weight": z(2 * (cfg.qk_nope_head_dim + v), klr), "o_proj.weight": z(64, 2 * v)})
 
 
 @pytest.mark.parametrize("kw", [{"mla_cache_bits": 8}, {"mla_cache_bits": 3}, {"mla_cache_group_size": 64}, {"kv_lora_rank": 256},
-                                {"qk_rope_head_dim": 32}])
+                                {"qk_rope_head_dim": 32}, {"qk_nope_head_dim": 264, "q_head_dim": 328}, {"v_head_dim": 1032}])
 def test_layer_refuses_other_quantised_caches(kw):
     with pytest.raises(ValueError):
         _layer(_cfg(**kw))
@@ -257,14 +258,14 @@ def test_cache_grows_by_doubling(weights):
     from k3hip.mla_q4 import new_cache_q4
     cache = new_cache_q4(2, 1, weights, "cpu")
     assert cache.capacity == 256 and cache.bytes_per_token() == 400 and cache.nbytes_used() == 0
-    for x in cache._buffers():
+    for x in cache.buffers():
         x.copy_(torch.randint(1, 100, x.shape).to(x.dtype))
-    before = [x.clone() for x in cache._buffers()]
+    before = [x.clone() for x in cache.buffers()]
     cache.length = 250
     assert cache.reserve(6).capacity == 256 and cache.packed is not None
     cache.reserve(7)
     assert cache.capacity == 512 and cache.length == 250 and cache.nbytes_used() == 2 * 250 * 400
-    for x, y in zip(cache._buffers(), before):
+    for x, y in zip(cache.buffers(), before):
         assert torch.equal(x[:, :250], y[:, :250]) and not x[:, 250:].any() and x.dtype == y.dtype
     cache.length = 512
     assert cache.reserve(1000).capacity == 1536
@@ -275,6 +276,32 @@ def test_cache_without_weights_cannot_evict():
     from k3hip.mla_q4 import new_cache_q4
     with pytest.raises(ValueError, match="no attention weights"):
         new_cache_q4(1, 1, device="cpu").evict(4)
+
+
+@pytest.mark.parametrize("change", [
+    lambda c: setattr(c, "rot", c.rot.float()), lambda c: setattr(c, "packed", c.packed[:, :100]),
+    lambda c: setattr(c, "scales", c.scales[..., :8]), lambda c: setattr(c, "weight", torch.zeros(1, 255)),
+    lambda c: setattr(c, "weight", torch.zeros(1, 256, dtype=torch.float64)),
+])
+def test_step_refuses_buffers_of_another_form(change):
+    from k3hip.mla_q4 import new_cache_q4
+    cache = new_cache_q4(1, 1, True, "cpu")
+    assert cache.row_pitches() == (256, 16, 64)
+    change(cache)
+    with pytest.raises((ValueError, TypeError)):
+        cache.row_pitches()
+    with pytest.raises(ValueError, match="2 sequences"):
+        new_cache_q4(2, 1, device="cpu").row_pitches()
+
+
+def test_append_refuses_gradients(monkeypatch):
+    from k3hip.mla_q4 import mla_q4_append
+    calls = _launches(monkeypatch)
+    with pytest.raises(ValueError, match="no gradient"):
+        mla_q4_append(torch.zeros(2, 1, 512, requires_grad=True), torch.zeros(2, 1, 64), *_cache())
+    with torch.no_grad():
+        mla_q4_append(torch.zeros(2, 1, 512, requires_grad=True), torch.zeros(2, 1, 64), *_cache())
+    assert len(calls) == 1
 
 
 def test_cache_passes_its_buffers_and_length(monkeypatch):
@@ -307,7 +334,7 @@ def test_step_entry_point_checks_its_arguments():
     for i in (0, 2, 3, 4, 5, 6, 7, 8, 10, 11, 13, 15, 22, 31):
         assert step(**{f"_{i}": n}) == _lib.K3_ERR_NULL, i
     assert step(_1=3) == _lib.K3_ERR_DTYPE and step(_23=3) == _lib.K3_ERR_DTYPE
-    for at in ({"_12": 255}, {"_12": 264}, {"_14": 15}, {"_14": 18}, {"_16": 63}, {"_16": 68}, {"_18": 5}, {"_19": -1}, {"_19": 8}, {"_24": 60}, {"_25": 0},
+    for at in ({"_12": 255}, {"_12": 264}, {"_14": 15}, {"_14": 18}, {"_12": 1040}, {"_14": 1028}, {"_16": 520}, {"_16": 63}, {"_16": 68}, {"_18": 5}, {"_19": -1}, {"_19": 8}, {"_24": 60}, {"_25": 0},
                {"_27": 264}, {"_28": 32}, {"_29": 1032}, {"_30": 256}, {"_18": (1 << 24) + 1}):
         assert step(**at) == _lib.K3_ERR_SHAPE, at
     for i in (0, 2, 3, 4, 5, 6, 7, 8, 10, 11, 15, 31):
