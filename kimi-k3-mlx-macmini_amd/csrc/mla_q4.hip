@@ -36,16 +36,24 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s4_t *lds_s4;
 typedef __attribute__((address_space(3))) i32x2 *lds_i2;
 
+// n / d by a multiplication: ceil(2^32 / d) (0: d is 1) is exact where n d < 2^32, as for the rows, queries and blocks of a pass (a
+// division is some 40 dependent instructions, and most kernels here make several before their first load).
+inline uint32_t inverse_of(int64_t d) { return d == 1 ? 0u : static_cast<uint32_t>(cdiv(1ll << 32, d)); }
+__device__ __forceinline__ int quotient(int n, uint32_t inverse) {
+    return inverse ? static_cast<int>(__umulhi(static_cast<uint32_t>(n), inverse)) : n;
+}
+
 // The order of a sequence's rows: by query (row = t H + h: the heads of one query are neighbours, few queries fill the tiles)
 // or by head (row = h Tp + t, Tp = T rounded up to 16: a tile is 16 queries of one head, so a block of the query and output
 // launches, which takes one head's matrix, writes and reads whole tiles).
 struct Rows {
     int T, H, Tp;                           // Tp 0: by query
-    uint32_t inverse;                       // ceil(2^32 / d), d = Tp or H (0: d is 1): exact for the rows of a pass, row d < 2^32
+    uint32_t inverse, inverse_t;            // of d = Tp or H, and of T
     __host__ __device__ int count() const { return Tp ? H * Tp : T * H; }
     __device__ int of(int t, int h) const { return Tp ? h * Tp + t : t * H + h; }
-    // row / d by a multiplication (the weight sums divide several times a tile)
-    __device__ int major(int row) const { return inverse ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), inverse)) : row; }
+    __device__ int major(int row) const { return quotient(row, inverse); }
+    __device__ int seq(int m) const { return quotient(m, inverse_t); }      // of query m of all sequences
+    __device__ int token(int m) const { return m - seq(m) * T; }
     __device__ int query(int row) const { return Tp ? row - major(row) * Tp : major(row); }       // may be >= T: no row
     // the last query of rows row0 .. row1
     __device__ int last_query(int row0, int row1) const {
@@ -191,7 +199,8 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     const uint16_t *w = a.w_uk + static_cast<int64_t>(h) * a.nope * kQ4Lat + quarter * 128;
     const int qt = MT == 1 ? 0 : wave, col = MT == 1 ? wave * 32 : 0, mine = m0 + 16 * qt + r16;   // the wave's queries and columns
     const bool live = mine < a.M;
-    const QT *q = static_cast<const QT *>(a.q_nope) + (live ? mine / T : 0) * a.n_b + (live ? a.t0 + mine % T : 0) * a.n_t + h * a.n_h + 4 * q4;
+    const int qb = live ? a.rows.seq(mine) : 0, qt0 = live ? a.t0 + mine - qb * T : 0;
+    const QT *q = static_cast<const QT *>(a.q_nope) + qb * a.n_b + qt0 * a.n_t + h * a.n_h + 4 * q4;
     QueryRaw<QT> ahead[kAhead];
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) ahead[s].load(q, 32 * s, a.nope - 4 * q4, live);
@@ -245,8 +254,8 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     __syncthreads();
     if (tid < 64 * MT && m0 + (tid >> 2) < a.M) {
         // one group of 32 columns of one query: its terms
-        const int i = tid >> 2, g = tid & 3, m = m0 + i, row = a.rows.of(m % T, h), at = quarter * 16 + (row & 15);
-        char *tile = a.qop + m / T * a.q_seq + static_cast<int64_t>(row >> 4) * q4_tile_bytes(NT, RT);
+        const int i = tid >> 2, g = tid & 3, m = m0 + i, row = a.rows.of(a.rows.token(m), h), at = quarter * 16 + (row & 15);
+        char *tile = a.qop + a.rows.seq(m) * a.q_seq + static_cast<int64_t>(row >> 4) * q4_tile_bytes(NT, RT);
         const float *src = fs + i * kFLd + g * 32;
         float v[32];
         uint32_t top = 0;
@@ -284,9 +293,9 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     for (int j = MT == 1 ? tid - 64 : tid; j < 128 * MT; j += 256) {
         const int i = j >> 3, m = m0 + i, c = j & 7;
         if (j < 0 || m >= a.M) continue;
-        const int row = a.rows.of(m % T, h), at = (c & 3) * 16 + (row & 15);
-        char *tile = a.qop + m / T * a.q_seq + static_cast<int64_t>(row >> 4) * q4_tile_bytes(NT, RT);
-        const QT *qr = static_cast<const QT *>(a.q_rot) + m / T * a.r_b + (a.t0 + m % T) * a.r_t + h * a.r_h + c * 8;
+        const int b = a.rows.seq(m), t = m - b * T, row = a.rows.of(t, h), at = (c & 3) * 16 + (row & 15);
+        char *tile = a.qop + b * a.q_seq + static_cast<int64_t>(row >> 4) * q4_tile_bytes(NT, RT);
+        const QT *qr = static_cast<const QT *>(a.q_rot) + b * a.r_b + (a.t0 + t) * a.r_t + h * a.r_h + c * 8;
         u32x4 f[3] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
         if constexpr (std::is_same<QT, float>::value) {
             const f32x4 x = *reinterpret_cast<const f32x4 *>(qr), y = *reinterpret_cast<const f32x4 *>(qr + 4);
@@ -314,6 +323,7 @@ struct AttendArgs {
     float2 *ml;                                 // [slots][rows]
     Rows order;
     int t0, rows, Ts, NS, rblocks, B;           // rows: order.count()
+    uint32_t inverse_rblocks, inverse_ns;
     float c;                                    // scale * log2(e)
     int swizzle;
 };
@@ -349,8 +359,8 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     const int r16 = lane & 15, q4 = lane >> 4;
     const int nb = gridDim.x;
     const int w = a.swizzle ? (blockIdx.x & 7) * (nb >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-    int rb = w % a.rblocks;
-    const int slot = w / a.rblocks;
+    const int slot = quotient(w, a.inverse_rblocks);
+    int rb = w - slot * a.rblocks;
     int4 range;                                 // sequence, first position, last + 1, length
     if (a.slot) {
         const int4 r = a.slot[slot];
@@ -358,7 +368,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                           __builtin_amdgcn_readfirstlane(r.w));
         if (range.x < 0) return;
     } else {
-        range.x = slot / a.NS, range.y = slot % a.NS * a.Ts, range.z = range.y + a.Ts;
+        range.x = quotient(slot, a.inverse_ns), range.y = (slot - range.x * a.NS) * a.Ts, range.z = range.y + a.Ts;
         range.w = a.lengths ? min(max(a.lengths[range.x], 0), a.cap) : a.length;
     }
     const int b = range.x, len = range.w;
@@ -449,6 +459,11 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         // ================= score waves
         const int rg = wave % RG, tg = wave / RG;
         const char *tile = a.qop + b * a.q_seq + static_cast<int64_t>((row0 >> 4) + rg) * q4_tile_bytes(NT, RT);
+        // (the rotary operands first: they go to LDS before the first barrier, which need not wait for the others)
+        u32x4 qo[2 * RT];
+#pragma unroll
+        for (int x = 0; x < 2 * RT; ++x) qo[x] = *reinterpret_cast<const u32x4 *>(tile + q4_rope_at(NT, 0, x) + lane * 16);
+        __builtin_amdgcn_sched_barrier(0);
         u32x4 qlo[NT][kQ4Steps];
         u32x2 qhi[NT][kQ4Steps];
         int qs[NT];
@@ -464,7 +479,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         // (the score waves of a row group write the same)
         char *const qr = qbuf + rg * RT * 2048 + lane * 16;
 #pragma unroll
-        for (int x = 0; x < 2 * RT; ++x) *reinterpret_cast<u32x4 *>(qr + x * 1024) = *reinterpret_cast<const u32x4 *>(tile + q4_rope_at(NT, 0, x) + lane * 16);
+        for (int x = 0; x < 2 * RT; ++x) *reinterpret_cast<u32x4 *>(qr + x * 1024) = qo[x];
         const int row = row0 + rg * 16 + r16;
         const int tq = a.order.query(row), sees = row < a.rows && tq < a.order.T ? q4_sees(a.t0 + tq, cnt, len) : 0;
         const int limit = min(sees, t_end) - t_begin;       // positions of this split that the row sees
@@ -738,7 +753,7 @@ struct UvArgs {
 constexpr int kMaxSplits = 256;
 
 __device__ __forceinline__ void store_out4(const UvArgs &a, int m, int h, int v, f32x4 o) {
-    const int64_t at = ((static_cast<int64_t>(m / a.order.T) * a.Tall + a.t0 + m % a.order.T) * a.order.H + h) * a.V + v;
+    const int64_t at = ((static_cast<int64_t>(a.order.seq(m)) * a.Tall + a.t0 + a.order.token(m)) * a.order.H + h) * a.V + v;
     if (a.gate) {
         const f32x4 g = *reinterpret_cast<const f32x4 *>(a.gate + at);
 #pragma unroll
@@ -814,7 +829,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void uv_few_kernel(UvArgs a, int per
     const int g = (wave >> 1) & (pairs - 1);
     constexpr int kBatch = 8;
     for (int i = (wave >> 1) / pairs; i < nv; i += kPairs / pairs) {
-        const int m = m0 + i, b = m / a.order.T, row = a.order.of(m % a.order.T, h);
+        const int m = m0 + i, b = a.order.seq(m), row = a.order.of(m - b * a.order.T, h);
         int2 there = a.records(b);
         there.x = __builtin_amdgcn_readfirstlane(there.x), there.y = __builtin_amdgcn_readfirstlane(there.y);
         const int n = there.y;
@@ -910,9 +925,9 @@ __global__ __launch_bounds__(256, 2) void uv_many_kernel(UvArgs a) {
     const int h = blockIdx.x, m0 = blockIdx.y * 64, nv = min(64, a.M - m0);
     for (int i = wave; i < nv; i += 4) {
         const int m = m0 + i;
-        const int b = m / a.order.T;
+        const int b = a.order.seq(m);
         float f[kMaxSplits / 64];
-        record_weights(a, b, a.order.of(m % a.order.T, h), a.records(b), true, f);
+        record_weights(a, b, a.order.of(m - b * a.order.T, h), a.records(b), true, f);
 #pragma unroll
         for (int u = 0; u < kMaxSplits / 64; ++u)
             if (64 * u + lane < a.NS) wsp[i * a.NS + 64 * u + lane] = f[u];
@@ -924,7 +939,7 @@ __global__ __launch_bounds__(256, 2) void uv_many_kernel(UvArgs a) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
         const int m = m0 + min(8 * u + i8, nv - 1);
-        at[u] = static_cast<uint32_t>(m / a.order.T * a.NS) * pitch + static_cast<uint32_t>(a.order.of(m % a.order.T, h) * kQ4Lat + 4 * c4);
+        at[u] = static_cast<uint32_t>(a.order.seq(m) * a.NS) * pitch + static_cast<uint32_t>(a.order.of(a.order.token(m), h) * kQ4Lat + 4 * c4);
     }
     for (int v0 = 0; v0 < a.V; v0 += 128) {
         f32x4 acc[2][4];
@@ -1185,8 +1200,8 @@ constexpr int kByHead = 32;               // queries of a sequence from which ro
 constexpr int kManyQueries = 48;          // queries (all sequences) from which uv_many takes less than uv_few
 
 Rows rows_of(int64_t T, int64_t H) {
-    const int64_t Tp = T >= kByHead ? cdiv(T, 16) * 16 : 0, d = Tp ? Tp : H;
-    return Rows{static_cast<int>(T), static_cast<int>(H), static_cast<int>(Tp), d == 1 ? 0u : static_cast<uint32_t>(cdiv(1ll << 32, d))};
+    const int64_t Tp = T >= kByHead ? cdiv(T, 16) * 16 : 0;
+    return Rows{static_cast<int>(T), static_cast<int>(H), static_cast<int>(Tp), inverse_of(Tp ? Tp : H), inverse_of(T)};
 }
 
 // What the launches are cut into; a function of its arguments alone.
@@ -1405,7 +1420,8 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         a.slot = qa.ranges.slot;
         a.part = reinterpret_cast<float *>(ws + p.part), a.ml = reinterpret_cast<float2 *>(ws + p.ml);
         a.order = order, a.t0 = static_cast<int>(t0), a.rows = rows, a.Ts = p.Ts, a.NS = p.NS;
-        a.rblocks = static_cast<int>(cdiv(rows, 16 * p.RG)), a.B = static_cast<int>(B), a.c = scale * 1.4426950408889634f;
+        a.inverse_ns = inverse_of(p.NS);
+        a.rblocks = static_cast<int>(cdiv(rows, 16 * p.RG)), a.inverse_rblocks = inverse_of(a.rblocks), a.B = static_cast<int>(B), a.c = scale * 1.4426950408889634f;
         // blocks b % 8 run on one XCD: with several ranges its blocks get neighbouring ones (one L2 reads them); with one range the blocks
         // that see most, which come first, are to be spread
         a.swizzle = p.NS > 1 && (p.slots * a.rblocks) % 8 == 0;
