@@ -812,13 +812,14 @@ __global__ __launch_bounds__(64 * WAVES, 1) void uv_few_kernel(UvArgs a, int per
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
     float *const x = sm, *const d = sm + 16 * kXLd;
     const int h = blockIdx.x, m0 = blockIdx.y * per, col0 = wave * kCols, nv = min(per, a.M - m0);
+    const auto rw = make_rsrc(a.w_uv + static_cast<int64_t>(h) * a.V * kQ4Lat, static_cast<uint32_t>(a.V) * (2 * kQ4Lat));
     auto weights_of = [&](int v0, u32x4 (&w)[VT][kSteps]) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < VT; ++t) {
-            const int v = v0 + t * 16 + r16;
-            const uint16_t *wr = a.w_uv + (static_cast<int64_t>(h) * a.V + v) * kQ4Lat + col0 + 8 * q4;
+            // (rows past the head's last are outside and load zeros)
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) w[t][k] = v < a.V ? *reinterpret_cast<const u32x4 *>(wr + 32 * k) : u32x4{0u, 0u, 0u, 0u};
+            for (int k = 0; k < kSteps; ++k)
+                w[t][k] = __builtin_bit_cast(u32x4, buf_load16(rw, static_cast<uint32_t>(v0 + t * 16 + r16) * (2 * kQ4Lat) + 2 * (col0 + 8 * q4 + 32 * k)));
         }
     };
     u32x4 w[VT][kSteps];
@@ -923,17 +924,30 @@ __global__ __launch_bounds__(256, 2) void uv_many_kernel(UvArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
     float *const wsp = reinterpret_cast<float *>(lds + TERMS * kTerm);
     const int h = blockIdx.x, m0 = blockIdx.y * 64, nv = min(64, a.M - m0);
-    for (int i = wave; i < nv; i += 4) {
-        const int m = m0 + i;
-        const int b = a.order.seq(m);
-        float f[kMaxSplits / 64];
-        record_weights(a, b, a.order.of(m - b * a.order.T, h), a.records(b), true, f);
-#pragma unroll
-        for (int u = 0; u < kMaxSplits / 64; ++u)
-            if (64 * u + lane < a.NS) wsp[i * a.NS + 64 * u + lane] = f[u];
+    {
+        // The records' weights (as record_weights) of all 64 queries at once, four lanes each: a wave a query waited for sixteen loads one
+        // after the other, 18 of the launch's 52 us at 1000 queries of 64 heads.
+        const int i = tid >> 2, part = tid & 3, m = m0 + min(i, nv - 1), b = a.order.seq(m), row = a.order.of(m - b * a.order.T, h);
+        const float2 *ml = a.ml + static_cast<int64_t>(b) * a.NS * a.rows + row;
+        float mx = -INFINITY, l = 0.f;
+        for (int s = part; s < a.NS; s += 4) mx = fmaxf(mx, ml[static_cast<int64_t>(s) * a.rows].x);
+        mx = fmaxf(mx, __shfl_xor(mx, 1));
+        mx = fmaxf(mx, __shfl_xor(mx, 2));
+        for (int s = part; s < a.NS; s += 4) {
+            const float2 v = ml[static_cast<int64_t>(s) * a.rows];
+            const float w = v.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v.x - mx);
+            wsp[i * a.NS + s] = w;
+            l = fmaf(w, v.y, l);
+        }
+        l += __shfl_xor(l, 1);
+        l += __shfl_xor(l, 2);
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        for (int s = part; s < a.NS; s += 4) wsp[i * a.NS + s] = wsp[i * a.NS + s] == 0.f ? 0.f : wsp[i * a.NS + s] * inv;
+        if (a.stats && part == 0 && i < nv) a.stats[static_cast<int64_t>(b) * a.rows + row] = l == 0.f ? 0.f : mx - kLift + __log2f(l);
     }
     __syncthreads();
     const uint32_t pitch = static_cast<uint32_t>(a.rows) * kQ4Lat;
+    const auto rw = make_rsrc(a.w_uv + static_cast<int64_t>(h) * a.V * kQ4Lat, static_cast<uint32_t>(a.V) * (2 * kQ4Lat));
     const int c4 = tid & 31, i8 = tid >> 5;
     uint32_t at[8];     // (a pass's records are at most 2^16 rows, so 2^27 bytes)
 #pragma unroll
@@ -952,10 +966,10 @@ __global__ __launch_bounds__(256, 2) void uv_many_kernel(UvArgs a) {
             u32x4 w[2][4];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int v = v0 + (2 * wave + t) * 16 + r16;
-                const uint16_t *wr = a.w_uv + (static_cast<int64_t>(h) * a.V + v) * kQ4Lat + col0 + 8 * q4;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w[t][k] = v < a.V ? *reinterpret_cast<const u32x4 *>(wr + k * 32) : u32x4{0u, 0u, 0u, 0u};
+                for (int k = 0; k < 4; ++k)         // (rows past the head's last are outside and load zeros)
+                    w[t][k] = __builtin_bit_cast(u32x4, buf_load16(rw, static_cast<uint32_t>(v0 + (2 * wave + t) * 16 + r16) * (2 * kQ4Lat) +
+                                                                           2 * (col0 + 8 * q4 + 32 * k)));
             }
             f32x4 s[8];
 #pragma unroll
@@ -1196,8 +1210,9 @@ struct Plan {
 };
 
 constexpr int64_t kChunkRows = 1 << 16;   // rows (heads x queries, all sequences) of one pass over the queries
-constexpr int kByHead = 32;               // queries of a sequence from which rows go by head
-constexpr int kManyQueries = 48;          // queries (all sequences) from which uv_many takes less than uv_few
+// Queries of a sequence from which rows go by head, by head / by query, us in all, 64 heads: 17 over 64 39.0 / 37.2, 32 over 1024 with
+// weights 54.0 / 56.7, 32 over 2048 42.9 / 43.3, 48 57.1 / 59.7.
+constexpr int kByHead = 32;
 
 Rows rows_of(int64_t T, int64_t H) {
     const int64_t Tp = T >= kByHead ? cdiv(T, 16) * 16 : 0;
@@ -1239,7 +1254,10 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
         p.slots = static_cast<int>(B * p.NS);
     }
     p.Ts = static_cast<int>(ts);
-    p.many = !p.listed && B * p.order.T >= kManyQueries;
+    // uv_many where uv_few's blocks (16 queries of a head) would not all run at once.  Measured, us in all, many / few: 256 queries of 16
+    // heads over 1024 (256 blocks) 51.5 / 49.6, 320 (320) 54.7 / 60.2; 64 of 64 over 2048 (256) 61.7 / 58.8, 72 (320) 64.1 / 67.5; 48 of 96
+    // (288) 63.2 / 68.5; 600 of 2 over 8000 (76) 73.9 / 55.6; 128 of 64 over 512 (512) 49.0 / 63.2.
+    p.many = !p.listed && H * cdiv(B * p.order.T, 16) > 256;
     const int64_t pos_blocks = std::max<int64_t>(1, cdiv(npos, 128 * kWTiles));
     p.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.tiles, 256 / (pos_blocks * B))));
     p.chunk = static_cast<int>(cdiv(p.tiles, p.chunks));
@@ -1289,6 +1307,7 @@ int launch_qa_of(const QaArgs &a, hipStream_t st) {
 
 template <typename QT, int NT, int RT>
 int launch_qa(const QaArgs &a, hipStream_t st) {
+    // (24 queries of 64 heads 41.5 us in all either way, 64 61.1 / 62.3)
     return a.M > 32 ? launch_qa_of<QT, NT, RT, 4>(a, st) : launch_qa_of<QT, NT, RT, 1>(a, st);
 }
 
