@@ -9,8 +9,7 @@
 //   qa       q_nope W_UK on the bf16 matrix cores (fp32 queries as three bf16 terms), rounded into the 6-bit terms
 //            that the scaled matrix product takes (mla_q4.h)
 //   attend   a block = 16 RG rows x a range of positions, eight waves: the maximum and sum run with the positions
-//   uv       the ranges' records joined, the context times W_UV
-//   out      (few rows) the four column quarters of that product added, and the output gate
+//   uv       the ranges' records joined, the context times W_UV, the output gate
 //   weights  (if asked for) p once more from the rows' final maxima and sums, added over the rows
 //
 // attend, per round of 64 positions: the codes go to LDS as they are, 256 bytes and 16 scale bytes a position, and both products

@@ -184,10 +184,10 @@ def _lengths(kind, B, cap):
 
 @pytest.mark.parametrize("kind", ["one long", "none", "full", "spread"])
 @pytest.mark.parametrize("B,T,H,cap,out", [(2, 1, 64, 1500, F32), (32, 1, 64, 700, BF16), (33, 2, 16, 900, F32), (130, 1, 3, 300, BF16),
-                                           (511, 1, 2, 70, F32), (3, 40, 8, 260, F32)])
+                                           (511, 1, 2, 70, F32), (3, 40, 8, 260, F32), (600, 1, 2, 50, F32), (16, 33, 64, 60, BF16)])
 def test_batches_of_unequal_length(kind, B, T, H, cap, out):
     """Batches that share the card out over the positions there are: one long sequence among empty ones, nothing, all of
-    the capacity, lengths of every size; as many sequences as such a batch may have."""
+    the capacity, lengths of every size; as many sequences as such a batch may have, and batches with rows enough without it."""
     _check(_problem(B, T, H, cap, 170), _lengths(kind, B, cap), out=out, weight=H == 16)
 
 
