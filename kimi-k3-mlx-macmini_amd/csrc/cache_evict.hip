@@ -5,10 +5,11 @@
 // Two launches.  select (a block per sequence): the weights become keys that order as whole numbers do (NaN below
 // all, -0 as 0) and stay in registers (up to 32,768 positions; beyond that every pass reads them again); the key of the
 // last one to stay is found 11, 11 and 10 bits at a time from a histogram of the keys that still match, in LDS (four
-// copies, by lane, for weights that are alike), and no further than a bin that stays whole.  Of the positions with exactly
-// that key the lowest stay.  A wave's ballot over 64 neighbours counts them in order, and one scan over those
+// copies, by lane, for weights that are alike; sixteen took 22.9 us for 21.3), and no further than a bin that stays whole.  Of the
+// positions with exactly that key the lowest stay.  A wave's ballot over 64 neighbours counts them in order, and one scan over those
 // counts gives each kept position its place: no atomics on the result.  gather: rows of every buffer, 16 bytes a thread.
-// Bound by the latency of a block's passes (select), by HBM or the launch (gather).
+// Bound by a block's passes (select: 5.8 us for 1025 positions, 20 for 32,768, of which loading and the first histogram 8, the
+// places 6), by HBM or the launch (gather: 53 MB in 10 us).
 #include <algorithm>
 
 #include "k3_common.h"
@@ -33,27 +34,38 @@ __device__ __forceinline__ uint32_t order_key(float f) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// inclusive prefix of v over the wave: within rows of 16 lanes, then across them
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);    // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);    // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);    // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 // exclusive prefix of v over the block's threads, and the total
-__device__ __forceinline__ int block_prefix(int v, int *sums, int &total) {
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *sums, uint32_t &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(s, o);
-        if (lane >= o) s += x;
-    }
+    const uint32_t s = wave_prefix(v);
     if (lane == 63) sums[wave] = s;
     __syncthreads();
-    int before = 0;
+    uint32_t before = 0;
     total = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 64; ++w) {
-        const int x = sums[w];
-        before += w < wave ? x : 0;
+        const uint32_t x = sums[w];
+        before += w < wave ? x : 0u;
         total += x;
     }
     __syncthreads();
     return before + s - v;
+}
+
+// lanes below this one whose bit is set
+__device__ __forceinline__ int below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
 }
 
 // VPT keys a thread, position (j * kWaves + wave) * 64 + lane of a chunk of kThreads * VPT
@@ -61,7 +73,7 @@ template <int VPT>
 __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
     __shared__ int hist[kBins * kCopies];
     __shared__ int2 counts[VPT * kWaves];   // of 64 neighbours: keys above the threshold, keys at it
-    __shared__ int sums[kWaves];
+    __shared__ uint32_t sums[kWaves];
     __shared__ int found[3];
     constexpr int kChunk = kThreads * VPT;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
@@ -81,13 +93,15 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
     for (int i = tid; i < a.recent; i += kThreads) index[a.keep - a.recent + i] = n - a.recent + i;
     if (need == 0) return;
     const float *w = a.weight + b * a.ld + a.sink;
+    // (Behind the last position keys of 0, the lowest there is: they come after all that are there, so wherever they are counted among
+    // the positions at the threshold, `need` are found before them.)
     uint32_t key[VPT];
     auto load = [&](int c0) {
         float f[VPT];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int i = c0 + j * kThreads + tid;
-            f[j] = i < mid ? w[i] : 0.f;
+            f[j] = i < mid ? w[i] : __builtin_nanf("");
         }
 #pragma unroll
         for (int j = 0; j < VPT; ++j) key[j] = order_key(f[j]);
@@ -105,8 +119,9 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
             if (mid > kChunk) load(c0);
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
+                if (c0 + j * kThreads >= mid) break;
                 const uint32_t k = key[j];
-                if (c0 + j * kThreads + tid < mid && (pass == 0 || (k >> (shift + bits)) == prefix))
+                if (pass == 0 || (k >> (shift + bits)) == prefix)
                     atomicAdd(&hist[((k >> shift) & ((1 << bits) - 1)) * kCopies + (tid & (kCopies - 1))], 1);
             }
         }
@@ -119,8 +134,8 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
             const int4 v = *reinterpret_cast<const int4 *>(&hist[(2 * top + x) * kCopies]);
             c[x] = (v.x + v.y) + (v.z + v.w);
         }
-        int total;
-        const int above = block_prefix(c[0] + c[1], sums, total);   // keys in higher bins
+        uint32_t total;
+        const int above = static_cast<int>(block_prefix(static_cast<uint32_t>(c[0] + c[1]), sums, total));   // keys in higher bins
 #pragma unroll
         for (int x = 1, over = above; x >= 0; over += c[x], --x)
             if (over < need && over + c[x] >= need) found[0] = 2 * top + x, found[1] = need - over, found[2] = c[x];
@@ -131,35 +146,37 @@ __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
         __syncthreads();
         if (whole) break;
     }
-    // keys whose leading bits are above the prefix stay, and the first `need` of those that match
+    // keys whose leading bits are above the prefix stay, and the first `need` of those that match (the largest key, +infinity's, leaves
+    // room above it)
+    const uint32_t low = prefix << shift, high = (prefix + 1) << shift;
     int at = a.sink, same_seen = 0;
     for (int c0 = 0; c0 < mid; c0 += kChunk) {
         if (mid > kChunk) load(c0);
+        // lane j: how many of the wave's j-th 64 neighbours are above (high half) and at the threshold (a chunk has 2^15 at most)
+        uint32_t mine = 0;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const bool there = c0 + j * kThreads + tid < mid;
-            const uint64_t more = __ballot(there && (key[j] >> shift) > prefix), same = __ballot(there && (key[j] >> shift) == prefix);
-            if (lane == 0) counts[j * kWaves + wave] = make_int2(__popcll(more), __popcll(same));
+            const uint64_t more = __ballot(key[j] >= high), same = __ballot(key[j] >= low) & ~more;
+            mine = lane == j ? (static_cast<uint32_t>(__popcll(more)) << 16) + static_cast<uint32_t>(__popcll(same)) : mine;
         }
+        if (lane < VPT) counts[lane * kWaves + wave].x = static_cast<int>(mine);
         __syncthreads();
-        const int2 v = tid < VPT * kWaves ? counts[tid] : make_int2(0, 0);
-        int total, all;
-        const int same_before = same_seen + block_prefix(v.y, sums, all);
-        const int place = at + block_prefix(v.x + min(max(need - same_before, 0), v.y), sums, total);
-        if (tid < VPT * kWaves) counts[tid] = make_int2(place, same_before);
+        const uint32_t v = tid < VPT * kWaves ? static_cast<uint32_t>(counts[tid].x) : 0u;
+        uint32_t total;
+        const uint32_t before = block_prefix(v, sums, total);
+        const int same_before = same_seen + static_cast<int>(before & 0xffffu), same_after = same_seen + static_cast<int>(total & 0xffffu);
+        // of the positions at the threshold the first `need` stay
+        const int stayed = min(same_seen, need);
+        if (tid < VPT * kWaves) counts[tid] = make_int2(at + static_cast<int>(before >> 16) + min(same_before, need) - stayed, same_before);
         __syncthreads();
-        const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const int i = c0 + j * kThreads + tid;
-            const bool same = i < mid && (key[j] >> shift) == prefix;
-            const uint64_t sames = __ballot(same);
+            const uint64_t more = __ballot(key[j] >= high), same = __ballot(key[j] >= low) & ~more;
             const int2 o = counts[j * kWaves + wave];
-            const bool stay = (i < mid && (key[j] >> shift) > prefix) || (same && o.y + __popcll(sames & below) < need);
-            const uint64_t stays = __ballot(stay);
-            if (stay) index[o.x + __popcll(stays & below)] = a.sink + i;
+            const uint64_t stays = more | (same & __ballot(o.y + below(same) < need));
+            if ((stays >> lane) & 1) index[o.x + below(stays)] = a.sink + c0 + j * kThreads + tid;
         }
-        at += total, same_seen += all;
+        at += static_cast<int>(total >> 16) + min(same_after, need) - stayed, same_seen = same_after;
         __syncthreads();
     }
 }

@@ -545,6 +545,21 @@ def test_evict(B, n, keep, sink, recent, lengths, kind):
             assert bool((bits(x[b, len(want):].cpu()) == 0).all())
 
 
+def test_evict_whole_chunks_above_and_at_the_threshold():
+    """Neighbourhoods of 32,768 positions that stay as a whole, that are all alike, and that go as a whole."""
+    from k3hip.evict import cache_evict
+    n, keep = 140000, 70000
+    w = torch.cat([torch.full((40000,), 3.0), torch.full((70000,), 2.0), torch.full((30000,), 1.0)])[None]
+    (x,), index, kept = cache_evict(w.cuda(), [torch.arange(n, device="cuda")[None, :, None].contiguous()], keep)
+    want = torch.arange(keep)
+    assert int(kept) == keep and torch.equal(index[0].cpu().long(), want) and torch.equal(x[0, :, 0].cpu(), want)
+    w = w.flip(1)
+    _, index, _ = cache_evict(w.cuda(), [], keep, sink=5, recent=100)
+    # the last 40,000 hold the 100 recent; 5 first; the rest are the first ones of weight 2 (from 30,000 on)
+    want = torch.cat([torch.arange(5), torch.arange(30000, 30000 + keep - 40000 - 5), torch.arange(100000, n)])
+    assert torch.equal(index[0].cpu().long(), want)
+
+
 def test_evict_strided_buffers_and_the_bf16_cache():
     from k3hip.evict import cache_evict
     from k3hip.mla import MLACache
