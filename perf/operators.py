@@ -14,7 +14,6 @@ weight and the rest little, as trained attention does.
 """
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -244,7 +243,6 @@ def _plain_evict(s: dict):
 
 
 # ------------------------------------------------------------------------------- one pass
-@functools.cache     # a program imports its package once, not every pass
 def _package():
     at = str(Path(__file__).resolve().parent.parent / "kimi-k3-mlx-macmini_amd")
     if at not in sys.path:
