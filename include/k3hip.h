@@ -471,7 +471,8 @@ int k3_mla_step_decode(const void *x, int x_dtype, const void *q_a, const float 
  * A group of 32 with largest magnitude m gets the scale 2^e, e = floor(log2 m) - 2, one more if
  * m > 7 * 2^e, its byte e + 127 held to 2..252; codes round to nearest, ties to even.  A group of
  * zeros gets byte 127, one with a NaN or an infinity 255: the position is NaN to every query that sees it.
- * c 16-byte aligned with pitches of whole 16 bytes; packed 4-byte aligned, pitches multiples of 4. */
+ * c 16-byte aligned with pitches of whole 16 bytes; packed 4-byte aligned, pitches multiples of 4.
+ * Pitches by which two sequences share memory of packed, scales, rot or weight are refused. */
 int k3_mla_q4_append(const void *c, int64_t c_batch, int64_t c_row, int c_dtype, const void *r, int64_t r_batch,
                      int64_t r_row, int r_dtype, void *packed, int64_t p_batch, int64_t p_row, void *scales,
                      int64_t s_batch, int64_t s_row, void *rot, int64_t rot_batch, int64_t rot_row,
@@ -493,8 +494,8 @@ int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim,
  * lengths int32 [B] on the device (taken as 0 .. max_length) or null: max_length for all; counts int32 [B] on
  *   the device (taken as 0 .. T) or null: T.  Every sequence has max_length readable rows;
  * gate [B, T, H, v] fp32 logits or null: o times sigmoid(gate);
- * out [B, T, H, v] contiguous, out_dtype; weight fp32 rows w_batch floats apart, positions past lengths[b] left as
- *   they are.
+ * out [B, T, H, v] contiguous, out_dtype; weight fp32 rows w_batch >= max_length floats apart, positions past
+ *   lengths[b] left as they are.
  * A query that sees nothing (also: t >= counts[b]) gets zeros and adds nothing to weight.  Deterministic.  The cache's
  * values enter exactly; the absorbed queries to 2^-12 of a unit under their group's largest for a bf16 out without weight,
  * else 2^-22; the probabilities to 2^-11 for a bf16 out, 2^-22 for fp32; sums and softmax in fp32.
@@ -533,7 +534,8 @@ int k3_mla_step_decode_q4(const void *x, int x_dtype, const void *q_a, const flo
  * <= keep; ties: the lowest position; NaN counts below all).  index [B, keep] int32: the kept positions in ascending order, then -1;
  * kept [B] int32: how many.  Then row i of every dst buffer is row index[i] of its src, and rows kept[b] .. dst_rows - 1
  * are zeroed.  buffers <= 8; the six arrays are host arrays of one entry per buffer: pointers, and batch and row pitches and row
- * sizes in bytes.  weight rows are w_batch floats apart.  src and dst must not overlap.  No counterpart in the
+ * sizes in bytes.  weight rows are w_batch floats apart.  src and dst must not overlap, nor
+ * (refused) two sequences of a dst.  No counterpart in the
  * reference, whose cache only grows. */
 int k3_cache_evict(const float *weight, int64_t w_batch, const int32_t *lengths, int64_t max_length, int64_t B,
                    int64_t keep, int64_t sink, int64_t recent, int32_t *index, int32_t *kept, int64_t buffers,

@@ -248,6 +248,8 @@ extern "C" int k3_cache_evict(const float *weight, int64_t w_batch, const int32_
             return set_error(K3_ERR_SHAPE, "cache evict: buffer %lld", (long long)x);
         if (src_row[x] < row_bytes[x] || dst_row[x] < row_bytes[x])
             return set_error(K3_ERR_SHAPE, "cache evict: rows of buffer %lld overlap", (long long)x);
+        if (!blocks_apart(B, dst_batch[x], dst_rows, dst_row[x], row_bytes[x]))
+            return set_error(K3_ERR_SHAPE, "cache evict: sequences of buffer %lld's result overlap", (long long)x);
         const int64_t all = row_bytes[x] | src_batch[x] | src_row[x] | dst_batch[x] | dst_row[x] |
                             static_cast<int64_t>(reinterpret_cast<uintptr_t>(src[x]) | reinterpret_cast<uintptr_t>(dst[x]));
         g.unit[x] = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;

@@ -138,6 +138,14 @@ __device__ __forceinline__ float wave_max_all(float v) {
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Whether B blocks, `batch` apart, of `rows` rows, `row` apart, of `width` elements share none: whole blocks one after the other, or
+// the blocks' rows side by side.  (Rows of one block are the caller's to check.)  Blocks that are written by workgroups of their own have to be.
+inline bool blocks_apart(int64_t B, int64_t batch, int64_t rows, int64_t row, int64_t width) {
+    if (B <= 1 || rows <= 0 || width <= 0) return true;
+    return batch >= static_cast<__int128>(rows - 1) * row + width ||
+           (batch >= width && (rows == 1 || row >= static_cast<__int128>(B - 1) * batch + width));
+}
+
 // ---------------------------------------------------------------- buffer loads
 // Raw buffer resource over [base, base + bytes): loads whose byte offset falls outside
 // return zeros, which lets tails and invalid rows load without branches.

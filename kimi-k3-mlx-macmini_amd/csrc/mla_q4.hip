@@ -1400,6 +1400,8 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
     if (max_length > 0 && (p_row < 256 || p_row % 16 || p_batch % 16 || s_row < 16 || s_row % 4 || s_batch % 4 || rot_row < kQ4Rope || rot_row % 8 ||
                            rot_batch % 8 || p_row > (1 << 16) || s_row > (1 << 16) || rot_row > (1 << 15)))
         return set_error(K3_ERR_SHAPE, "mla q4: cache row pitches too small, too large or not multiples of 16 bytes (scales: 4)");
+    if (weight && !blocks_apart(B, w_batch, 1, max_length, max_length))
+        return set_error(K3_ERR_SHAPE, "mla q4: the sequences' weights overlap, %lld apart", (long long)w_batch);
     if (!aligned16(q_nope) || !aligned16(q_rot) || !aligned16(w_uk) || !aligned16(w_uv) || !aligned16(out) || !aligned16(workspace) ||
         !aligned16(packed) || !aligned16(rot) || (reinterpret_cast<uintptr_t>(scales) & 3u) || (gate && !aligned16(gate)))
         return set_error(K3_ERR_ALIGN, "mla q4: queries, weights, cache, output and workspace must be 16-byte (scales 4-byte) aligned");

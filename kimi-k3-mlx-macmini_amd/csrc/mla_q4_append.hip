@@ -134,6 +134,9 @@ extern "C" int k3_mla_q4_append(const void *c, int64_t c_batch, int64_t c_row, i
     if (c_batch % unit || c_row % unit || c_row < 0 || r_row < 0 || p_row < kQ4Lat / 2 || s_row < kQ4Lat / 32 || rot_row < kQ4Rope ||
         p_row % 4 || p_batch % 4)
         return set_error(K3_ERR_SHAPE, "mla q4 append: a row pitch is too small or not a multiple of 16 bytes");
+    if (!blocks_apart(B, p_batch, cap, p_row, kQ4Lat / 2) || !blocks_apart(B, s_batch, cap, s_row, kQ4Lat / 32) ||
+        !blocks_apart(B, rot_batch, cap, rot_row, kQ4Rope) || (weight && !blocks_apart(B, w_batch, 1, cap, cap)))
+        return set_error(K3_ERR_SHAPE, "mla q4 append: sequences overlap in a buffer that is written");
     if (!aligned16(c) || (reinterpret_cast<uintptr_t>(packed) & 3u))
         return set_error(K3_ERR_ALIGN, "mla q4 append: c must be 16-byte and packed 4-byte aligned");
     return mla_q4_append(c, c_batch, c_row, c_dtype, r, r_batch, r_row, r_dtype, nullptr, 0.f, packed, p_batch, p_row, scales, s_batch,

@@ -74,6 +74,16 @@ def _pitches(t: torch.Tensor) -> tuple[int, int]:
     return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else max(t.stride(1), t.shape[2]))
 
 
+def _apart(t: torch.Tensor, name: str) -> None:
+    """Refuses a buffer [B, cap, ...] to be written whose sequences share memory (an expanded one): they would race."""
+    B, cap = t.shape[:2]
+    if B < 2 or cap == 0:
+        return
+    batch, row, width = t.stride(0), t.stride(1), t.shape[2] if t.dim() == 3 else 1
+    if batch < (cap - 1) * row + width and (batch < width or (cap > 1 and row < (B - 1) * batch + width)):
+        raise ValueError(f"{name}: the sequences overlap in memory (strides {t.stride()}); they are written")
+
+
 def _weight_pitch(weight: torch.Tensor | None, B: int, cap: int) -> int:
     """The batch pitch of the accumulated attention, [B, cap] fp32 or None."""
     if weight is None:
@@ -82,6 +92,7 @@ def _weight_pitch(weight: torch.Tensor | None, B: int, cap: int) -> int:
         raise TypeError(f"weight must be float32; got {weight.dtype}")
     if tuple(weight.shape) != (B, cap) or (cap > 1 and weight.stride(1) != 1):
         raise ValueError(f"weight must be [{B}, {cap}] with contiguous rows; got {tuple(weight.shape)}")
+    _apart(weight, "weight")
     return weight.stride(0) if B > 1 else 0
 
 
@@ -133,6 +144,8 @@ def _append_plan(c_new, r_new, packed, scales, rot, starts, counts, weight) -> t
         raise ValueError(f"c_new [B, T, {LATENT}] and r_new [B, T, {ROPE}] with B = {B} expected; got {tuple(c_new.shape)}, "
                          f"{tuple(r_new.shape)}")
     cdt, rdt = T.dtype_code(c_new.dtype), T.dtype_code(r_new.dtype)
+    for t, name in ((packed, "packed"), (scales, "scales"), (rot, "rot")):
+        _apart(t, name)
     _per_sequence(starts, B, "start")
     _per_sequence(counts, B, "counts")
     return (B, c_new.shape[1], cap, _rows_ok(c_new, 16 // c_new.element_size()), r_new.stride(2) == 1, cdt, rdt, _pitches(packed),

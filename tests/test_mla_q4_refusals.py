@@ -1,0 +1,82 @@
+"""Calls of the 4-bit cache that would write where another sequence writes: refused before anything is launched (no GPU)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from test_mla_q4_host import BF16, U8, _cache, _launches
+
+
+# ------------------------------------------------------------------------------- sequences that share memory
+def _append(cache, **kw):
+    from k3hip.mla_q4 import mla_q4_append
+    B = cache[0].shape[0]
+    mla_q4_append(torch.zeros(B, 1, 512), torch.zeros(B, 1, 64), *cache, **kw)
+
+
+def _attend(cache, **kw):
+    from k3hip.mla_q4 import mla_q4_attention
+    B = cache[0].shape[0]
+    w = torch.zeros(4, 128, 512, dtype=BF16)
+    return mla_q4_attention(torch.zeros(B, 1, 4, 128), torch.zeros(B, 1, 4, 64), w, w, *cache, 0.1, **kw)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("share", [
+    lambda t: t[:1].expand(2, -1, -1),                                                                      # one buffer for both
+    lambda t: t.as_strided(t.shape, (t.shape[2] * (t.shape[1] - 1), t.shape[2], 1)),                        # the last row is the next one's first
+    lambda t: t.as_strided(t.shape, (t.shape[2] // 2, 2 * t.shape[2], 1)),                                  # rows that overlap side by side
+])
+def test_append_refuses_sequences_that_share_rows(monkeypatch, which, share):
+    calls = _launches(monkeypatch)
+    cache = list(_cache())
+    cache[which] = share(cache[which])
+    with pytest.raises(ValueError, match="overlap"):
+        _append(cache)
+    assert not calls
+    _attend(cache)                          # reading them is in order
+    assert len(calls) == 1
+
+
+@pytest.mark.parametrize("weight", [torch.zeros(8).expand(2, 8), torch.zeros(15).as_strided((2, 8), (7, 1))])
+def test_summed_weights_of_sequences_that_share_memory(monkeypatch, weight):
+    calls = _launches(monkeypatch)
+    for f in (_append, _attend):
+        with pytest.raises(ValueError, match="overlap"):
+            f(_cache(), weight=weight)
+    assert not calls
+    from k3hip.evict import cache_evict
+    cache_evict(weight, [], 4)              # which reads them
+    assert len(calls) == 1
+
+
+@pytest.mark.parametrize("B,cap", [(1, 8), (2, 8), (3, 1), (2, 0)])
+def test_sequences_that_lie_apart_pass(monkeypatch, B, cap):
+    calls = _launches(monkeypatch)
+    for cache in (_cache(B, cap), tuple(t.transpose(0, 1) for t in _cache(cap, B)),       # batch first, position first
+                  tuple(torch.cat((t, t), 2)[..., :t.shape[2]] for t in _cache(B, cap))):
+        _append(cache, start=0 if cap else torch.zeros(B, dtype=torch.int32), weight=torch.zeros(B, cap + 3)[:, :cap])
+    assert len(calls) == (3 if cap else 0)
+
+
+def test_entry_points_refuse_sequences_that_share_memory():
+    from k3hip import _lib
+    lib = _lib.lib()
+    p, n = ctypes.c_void_p(4096), None
+    app = [p, 1536, 512, 0, p, 192, 64, 0, p, 2048, 256, p, 128, 16, p, 512, 64, n, 0, n, p, 8, 2, 3, 8, 512, 64, n]
+    att = [p, 1536, 512, 128, p, 768, 256, 64, 0, p, p, p, 2048, 256, p, 128, 16, p, 512, 64, n, n, 8, 2, 3, 4, 512, 64, 128, 96,
+           0.1, n, p, 0, p, 8, p, 0, n]
+    longs, ptrs = (ctypes.c_int64 * 2), (ctypes.c_void_p * 2)
+    one, big = longs(64, 16), longs(512, 128)
+    ev = [p, 8, n, 8, 2, 4, 1, 2, p, p, 2, ptrs(4096, 8192), big, one, ptrs(16384, 32768), big, one, one, 4, n]
+    for call, base, at in (
+            (lib.k3_mla_q4_append, app, {9: 2044}), (lib.k3_mla_q4_append, app, {9: 0}), (lib.k3_mla_q4_append, app, {9: -2048}),
+            (lib.k3_mla_q4_append, app, {12: 127}), (lib.k3_mla_q4_append, app, {15: 511}), (lib.k3_mla_q4_append, app, {21: 7}),
+            (lib.k3_mla_q4_append, app, {21: 0}), (lib.k3_mla_q4_attention, att, {35: 7}), (lib.k3_mla_q4_attention, att, {35: 0}),
+            (lib.k3_cache_evict, ev, {15: longs(512, 63)}), (lib.k3_cache_evict, ev, {15: longs(0, 128)})):
+        args = list(base)
+        for i, v in at.items():
+            args[i] = v
+        assert call(*args) == _lib.K3_ERR_SHAPE and b"overlap" in lib.k3_last_error(), (call.__name__, at)
