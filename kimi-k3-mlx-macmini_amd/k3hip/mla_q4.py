@@ -122,8 +122,8 @@ def mla_q4_append(c_new: torch.Tensor, r_new: torch.Tensor, packed: torch.Tensor
     if starts is None and not 0 <= start0 <= start0 + n <= cap:
         raise ValueError(f"{n} tokens at position {start0} do not fit a capacity of {cap}")
     T.require_device(c_new, r_new, packed, scales, rot, starts, counts, weight)
-    if T.tracked(c_new, r_new):
-        raise ValueError("mla_q4_append carries no gradient: call it under no_grad or on detached tensors")
+    if T.tracked(c_new, r_new, rot, weight):
+        raise ValueError("mla_q4_append carries no gradient, nor into the buffers it writes: call it under no_grad or on detached tensors")
     if B == 0 or n == 0 or cap == 0:
         return
     if not c_ok or c_new.data_ptr() % 16:
@@ -181,7 +181,7 @@ def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor
     if not 0 <= most <= cap:
         raise ValueError(f"length {most} outside the capacity {cap}")
     T.require_device(q_nope, q_rot, wk, wv, packed, scales, rot, weight, gate, lengths, counts)
-    if T.tracked(q_nope, q_rot, wk, wv, rot, gate):
+    if T.tracked(q_nope, q_rot, wk, wv, rot, gate, weight):
         raise ValueError("mla_q4_attention carries no gradient: call it under no_grad or on detached tensors")
     device = packed.device
     out = torch.empty((B, Tq, H, V), dtype=out_dtype, device=device)
@@ -260,6 +260,8 @@ class MLACacheQ4:
         if B != 1:
             raise ValueError(f"a cache of {B} sequences for one sequence's token")
         _weight_pitch(self.weight, B, cap)
+        if T.tracked(self.rot, self.weight):
+            raise ValueError("the cache is written in place and carries no gradient: its buffers must be detached")
         return _pitches(self.packed)[1], _pitches(self.scales)[1], _pitches(self.rot)[1]
 
     def view(self) -> tuple[torch.Tensor, torch.Tensor]:

@@ -1,4 +1,4 @@
-"""Calls of the 4-bit cache that would write where another sequence writes: refused before anything is launched (no GPU)."""
+"""Calls of the 4-bit cache that would write where they must not: refused before anything is launched (no GPU)."""
 from __future__ import annotations
 
 import ctypes
@@ -80,3 +80,27 @@ def test_entry_points_refuse_sequences_that_share_memory():
         for i, v in at.items():
             args[i] = v
         assert call(*args) == _lib.K3_ERR_SHAPE and b"overlap" in lib.k3_last_error(), (call.__name__, at)
+
+
+# ------------------------------------------------------------------------------- buffers of an autograd graph
+def test_buffers_that_are_written_carry_no_gradient(monkeypatch):
+    """As torch refuses to write into a leaf; under no_grad it is in order, as there."""
+    from k3hip.mla_q4 import new_cache_q4
+    calls = _launches(monkeypatch)
+    weight, rot = torch.zeros(2, 8, requires_grad=True), _cache()[2].requires_grad_()
+    for f in (lambda: _append(_cache(), weight=weight), lambda: _attend(_cache(), weight=weight),
+              lambda: _append(_cache()[:2] + (rot,)), lambda: _attend(_cache()[:2] + (rot,))):
+        with pytest.raises(ValueError, match="no gradient"):
+            f()
+        assert not calls
+        with torch.no_grad():
+            f()
+        assert len(calls) == 1
+        calls.clear()
+    for name in ("weight", "rot"):          # the one-call decode step asks for the pitches before it launches anything
+        cache = new_cache_q4(1, 1, True, "cpu")
+        getattr(cache, name).requires_grad_()
+        with pytest.raises(ValueError, match="no gradient"):
+            cache.row_pitches()
+        with torch.no_grad():
+            assert cache.row_pitches() == (256, 16, 64)
