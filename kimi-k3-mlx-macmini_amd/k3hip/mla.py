@@ -292,7 +292,7 @@ class MLAAttention:
             raise ValueError("the 4-bit cache carries no gradient: call the layer under no_grad or on detached tensors")
         if q4 and cache.weight is not None and self.kv_b.dtype != torch.bfloat16:
             raise ValueError("the masked form (fp32 kv_b) sums no attention weights: the cache must keep none")
-        if self.fused_step and B == 1 and Tn == 1 and (cache is None or q4 or cache.latent.dtype == torch.bfloat16):
+        if self.fused_step and B == 1 and Tn == 1 and (cache is None or (self.kv_b if q4 else cache.latent).dtype == torch.bfloat16):
             return self.decode_step(x, cache)
         nh, qhd, vhd = c.num_attention_heads, c.q_head_dim, c.v_head_dim
         nope, rope, klr = c.qk_nope_head_dim, c.qk_rope_head_dim, c.kv_lora_rank
@@ -414,6 +414,8 @@ class MLAAttention:
             cache = new_cache_q4(1, 1, bool(getattr(c, "mla_cache_weights", False)), x.device)
         elif cache is None:
             cache = new_cache(1, klr, rope, 1, self.cache_dtype, x.device)
+        if isinstance(cache, MLACacheQ4) and self.kv_b.dtype != torch.bfloat16:
+            raise ValueError("the one-call step over a 4-bit cache takes bf16 kv_b; call the layer for the fp32 masked form")
         cache.reserve(1)
         pos = cache.length
         xin = T.contiguous_aligned(x.reshape(hidden))

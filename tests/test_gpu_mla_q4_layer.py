@@ -240,3 +240,18 @@ def test_step_equals_the_calls_it_is_made_of():
     layer.fused_step = False
     c, _ = layer(x, cache)
     assert float((b - c).norm() / b.norm()) <= 2 * TOL
+
+
+@pytest.mark.parametrize("mats", [BF16, F32])
+def test_fp32_kv_b_is_not_rounded_for_one_token(mats):
+    """kv_b with values between bf16's (which are up to 2^-9 apart from them): a prompt, one token and a few, all by the masked
+    form, whatever the projections' dtype."""
+    layer, w = _layer(4, mats=mats, kv_b=F32)
+    w = {**w, "kv_b_proj.weight": w["kv_b_proj.weight"] * (1 + 2.0 ** -9)}
+    layer = type(layer)(layer.cfg, w)
+    assert layer.fused_step == (mats == BF16)
+    cache = None
+    for i, T in enumerate((20, 1, 1, 3)):
+        x = _x(70 + i, 1, T)
+        out, cache = layer(x, cache)
+        _close(out, _want(w, 4, x, cache)[0])

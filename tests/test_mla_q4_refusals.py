@@ -104,3 +104,21 @@ def test_buffers_that_are_written_carry_no_gradient(monkeypatch):
             cache.row_pitches()
         with torch.no_grad():
             assert cache.row_pitches() == (256, 16, 64)
+
+
+# ------------------------------------------------------------------------------- fp32 kv_b
+def test_one_token_with_fp32_kv_b_stays_on_the_masked_form(monkeypatch):
+    """The one-call step takes W_UK and W_UV in bf16; fp32 ones are not rounded to it because a call has one token."""
+    from k3hip.mla_q4 import MLACacheQ4, new_cache_q4
+    from test_mla_q4_host import _cfg, _layer
+    calls = _launches(monkeypatch)
+    monkeypatch.setattr(MLACacheQ4, "view", lambda c: (torch.zeros(1, c.length, 512), c.rot[:, :c.length]))
+    layer, x = _layer(_cfg()), torch.zeros(1, 1, 64)
+    layer.fused_step = True
+    layer.kv_b = layer.kv_b.float()
+    cache = new_cache_q4(1, 1, device="cpu")
+    layer(x, cache)
+    assert [name for name, _ in calls] == ["k3_mla_q4_append"] and cache.length == 1
+    with pytest.raises(ValueError, match="bf16 kv_b"):
+        layer.decode_step(x, cache)
+    assert len(calls) == 1 and cache.length == 1
