@@ -24,6 +24,7 @@ from . import _torch as T
 LATENT, ROPE, GROUP = 512, 64, 32
 # Scratch up to this size is kept per stream (a decode step's); larger scratch, a prompt's, is the call's own.
 KEPT_WORKSPACE = 1 << 26
+MAX_ROWS = 1 << 16      # heads x sequences of one k3_mla_q4_attention
 
 
 # What a call's layout (shapes, strides, dtypes; no addresses) comes to, once its checks are passed: the checks cost
@@ -162,7 +163,7 @@ def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor
     rot [B, cap, .].  Causal: the queries are each sequence's last T positions, query t sees positions 0 ..
     length - T + t.  ``lengths``: the sequences' lengths, a whole number for all or an int32 [B] device tensor (default: the
     capacity); ``counts`` int32 [B]: sequence b has only counts[b] queries, the first ones of its T.  A query that
-    sees nothing gives zeros.
+    sees nothing gives zeros.  A batch of more than 65,536 rows (sequences x heads) goes out in parts.
 
     The cache's rows are read as they lie: ``packed`` and ``rot`` 16-byte aligned with pitches of whole 16 bytes, ``scales`` 4.
 
@@ -186,6 +187,13 @@ def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor
     device = packed.device
     out = torch.empty((B, Tq, H, V), dtype=out_dtype, device=device)
     if B == 0 or Tq == 0:
+        return out
+    if B * H > MAX_ROWS and B > 1:
+        for b in range(0, B, max(1, MAX_ROWS // H)):
+            part = slice(b, min(B, b + max(1, MAX_ROWS // H)))
+            cut = [None if t is None else t[part] for t in (lengths, counts, weight, gate)]
+            out[part] = mla_q4_attention(q_nope[part], q_rot[part], wk, wv, packed[part], scales[part], rot[part], scale,
+                                         most if lengths is None else cut[0], *cut[1:], out_dtype)
         return out
     if gate is not None:
         gate = T.contiguous_aligned(gate.to(torch.float32))

@@ -376,6 +376,18 @@ def test_prompt_in_several_passes(monkeypatch):
     assert abs(float(weight.double().sum()) - T * H) < 2 ** -16 * T * H
 
 
+def test_a_batch_past_65536_rows():
+    """900 sequences of 80 heads, 72,000 rows, in two launches of the kernels; a gate, lengths of every size."""
+    from k3hip.mla_q4 import mla_q4_attention
+    B, H, cap = 900, 80, 24
+    args, lengths = _problem(B, 1, H, cap, 400, v=32), [b % (cap + 1) for b in range(B)]
+    o, _ = _check(args, lengths, weight=True)
+    gate = _rand(401, B, 1, H * 32).cuda()
+    gated = mla_q4_attention(*args, SCALE, lengths=_ints(lengths), weight=torch.zeros(B, cap, device="cuda"), gate=gate)
+    want = o.double() * torch.sigmoid(gate.double()).view_as(o)
+    assert bool(((gated.double() - want).abs() <= 2 ** -21 * want.abs()).all())
+
+
 def test_repeated_calls_give_the_same_bits():
     from k3hip.mla_q4 import mla_q4_attention
     args = _problem(3, 2, 48, 900, 150)

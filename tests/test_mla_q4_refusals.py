@@ -1,4 +1,5 @@
-"""Calls of the 4-bit cache that would write where they must not: refused before anything is launched (no GPU)."""
+"""Calls of the 4-bit cache that would write where they must not, refused before anything is launched, and calls that are not to be
+refused (no GPU)."""
 from __future__ import annotations
 
 import ctypes
@@ -122,3 +123,40 @@ def test_one_token_with_fp32_kv_b_stays_on_the_masked_form(monkeypatch):
     with pytest.raises(ValueError, match="bf16 kv_b"):
         layer.decode_step(x, cache)
     assert len(calls) == 1 and cache.length == 1
+
+
+# ------------------------------------------------------------------------------- large batches
+@pytest.mark.parametrize("lengths", [None, 5, torch.arange(700, dtype=torch.int32) % 9])
+def test_a_batch_past_65536_rows_goes_out_in_parts(monkeypatch, lengths):
+    """700 sequences of 96 heads: two calls, each with its own part of everything that is per sequence."""
+    from k3hip.mla_q4 import mla_q4_attention
+    calls = _launches(monkeypatch)
+    B, H, cap = 700, 96, 8
+    q, w = torch.zeros(1, 1, 1, 192).expand(B, 1, H, 192), torch.zeros(H, 128, 512, dtype=BF16)
+    cache, weight, gate = _cache(B, cap), torch.zeros(B, cap + 2)[:, :cap], torch.zeros(B, 1, H * 128)
+    counts = torch.ones(B, dtype=torch.int32)
+    o = mla_q4_attention(q[..., :128], q[..., 128:], w, w, *cache, 0.1, lengths=lengths, counts=counts, weight=weight, gate=gate)
+    assert o.shape == (B, 1, H, 128) and len(calls) == 2
+    first = 0
+    for (name, a), n in zip(calls, (682, 18)):
+        assert name == "k3_mla_q4_attention" and a[23] == n and a[25] == H
+        for i, t in ((11, cache[0]), (14, cache[1]), (17, cache[2]), (21, counts), (31, gate), (34, weight)):
+            assert a[i] == t[first].data_ptr(), i
+        assert a[35] == cap + 2 and a[22] == (lengths if isinstance(lengths, int) else cap)
+        assert a[20] == (lengths[first].data_ptr() if isinstance(lengths, torch.Tensor) else 0)
+        first += n
+
+
+def test_layer_takes_a_batch_past_65536_rows(monkeypatch):
+    from types import SimpleNamespace
+
+    from k3hip.mla import MLAAttention
+    from test_mla_q4_host import _cfg
+    calls = _launches(monkeypatch)
+    z = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
+    layer = MLAAttention(SimpleNamespace(**{**vars(_cfg()), "num_attention_heads": 96}), {
+        "q_a_proj.weight": z(64, 64), "q_a_layernorm.weight": z(64), "q_b_proj.weight": z(96 * 192, 64), "kv_a_proj_with_mqa.weight": z(576, 64),
+        "kv_a_layernorm.weight": z(512), "kv_b_proj.weight": z(96 * 256, 512), "o_proj.weight": z(64, 96 * 128)})
+    out, cache = layer(torch.zeros(700, 1, 64))
+    assert out.shape == (700, 1, 64) and cache.length == 1
+    assert [name for name, _ in calls] == ["k3_mla_q4_append"] + ["k3_mla_q4_attention"] * 2
