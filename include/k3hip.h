@@ -501,6 +501,7 @@ int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim,
  * else 2^-22; the probabilities to 2^-11 for a bf16 out, 2^-22 for fp32; sums and softmax in fp32.
  * nope a multiple of 8 up to 256, v one up to 1024, H <= 4096, B H <= 65536, max_length <= 2^24.  Pointers 16-byte
  * aligned (scales 4-byte); p_row and p_batch multiples of 16, rot pitches of 8, scale pitches of 4.
+ * Row pitches up to 64 KB; from 2 KB on the rows of one range, up to 2^20 positions, must span less than 2 GiB.
  * Counterpart of MLAAttention.__call__ over a QuantLatent cache (air_llm/models/kimi_k3/attention_mla.py:193-212). */
 int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t qn_token, int64_t qn_head, const void *q_rot,
                         int64_t qr_batch, int64_t qr_token, int64_t qr_head, int q_dtype, const void *w_uk,

@@ -948,7 +948,7 @@ __global__ __launch_bounds__(256, 2) void uv_many_kernel(UvArgs a) {
     const uint32_t pitch = static_cast<uint32_t>(a.rows) * kQ4Lat;
     const auto rw = make_rsrc(a.w_uv + static_cast<int64_t>(h) * a.V * kQ4Lat, static_cast<uint32_t>(a.V) * (2 * kQ4Lat));
     const int c4 = tid & 31, i8 = tid >> 5;
-    uint32_t at[8];     // (a pass's records are at most 2^16 rows, so 2^27 bytes)
+    uint32_t at[8];     // (a pass has fewer than 1.5 x 2^16 rows, and more than one record a row for 2^14 of them or 2^20 positions: 2^30 floats)
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
         const int m = m0 + min(8 * u + i8, nv - 1);
@@ -1208,7 +1208,8 @@ struct Plan {
     int64_t qop, ml, part, stats, wpart, slot, seq, total;
 };
 
-constexpr int64_t kChunkRows = 1 << 16;   // rows (heads x queries, all sequences) of one pass over the queries
+constexpr int64_t kChunkRows = 1 << 16;   // rows (heads x queries, all sequences) of one pass over the queries, before a head's are padded
+constexpr int64_t kLongest = 1 << 20;     // positions of a range: byte offsets in it take 32 bits, 2^30 at a pitch of 1 KB
 // Queries of a sequence from which rows go by head, by head / by query, us in all, 64 heads: 17 over 64 39.0 / 37.2, 32 over 1024 with
 // weights 54.0 / 56.7, 32 over 2048 42.9 / 43.3, 48 57.1 / 59.7.
 constexpr int kByHead = 32;
@@ -1240,12 +1241,13 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf1
     const int64_t base = B * p.rblocks;
     // One block a CU, and at least two rounds to a block: 4096 positions in ranges of 64 took 29.2 us for 27.0.
     int64_t ns = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, 256 / base));
-    int64_t ts = std::max<int64_t>(2 * kRound, cdiv(cdiv(std::max<int64_t>(npos, 1), ns), kRound) * kRound);
+    int64_t ts = std::min(kLongest, std::max<int64_t>(2 * kRound, cdiv(cdiv(std::max<int64_t>(npos, 1), ns), kRound) * kRound));
     p.NS = static_cast<int>(cdiv(std::max<int64_t>(npos, 1), ts));
     p.listed = varied && B > 1 && base < 512;
     if (p.listed) {
-        // a range that is not full for every sequence, so that many fewer for the rest, but as many as there are sequences at least
-        const int64_t spread = std::max<int64_t>(256 / p.rblocks - B, B);
+        // a range that is not full for every sequence, so that many fewer for the rest, but as many as there are sequences at least,
+        // and as it takes to hold all of the capacity
+        const int64_t spread = std::max({256 / p.rblocks - B, B, cdiv(B * npos, kLongest)});
         ts = std::max<int64_t>(2 * kRound, cdiv(cdiv(npos, kMaxSplits), kRound) * kRound);
         p.NS = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(cdiv(npos, ts), spread + 1)));
         p.spread = static_cast<int>(spread), p.slots = static_cast<int>(spread + B);
@@ -1408,10 +1410,10 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
     const Plan p = plan_of(B, T, H, v_dim, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weight != nullptr, lengths != nullptr);
     if (workspace_bytes < p.total)
         return set_error(K3_ERR_WORKSPACE, "mla q4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.total);
-    // (a range of a list is at most as long as all positions shared out)
+    // (a range of a list is at most as long as all positions shared out: 1.01 kLongest + 128 positions, 1.02 2^30 bytes at pitches of 1 KB)
     const int64_t longest = p.listed ? std::max<int64_t>(p.Ts, B * max_length / p.spread * 1.01 + 128) : p.Ts;
     if (longest * std::max({p_row, s_row, 2 * rot_row}) >= (1ll << 31))
-        return set_error(K3_ERR_SHAPE, "mla q4: a split of %lld positions spans 2 GiB", (long long)longest);
+        return set_error(K3_ERR_SHAPE, "mla q4: a range of %lld positions spans 2 GiB at these row pitches", (long long)longest);
     auto st = static_cast<hipStream_t>(stream);
     char *ws = static_cast<char *>(workspace);
     for (int64_t t0 = 0; t0 < T; t0 += p.order.T) {

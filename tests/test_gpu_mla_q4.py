@@ -358,6 +358,37 @@ def test_a_cache_past_four_gigabytes():
     assert abs(float(weight.double().sum()) - H) < float(rel.max()) * H
 
 
+@pytest.mark.parametrize("B,T", [(1, 80), (2, 64)])
+def test_many_queries_past_eight_million_positions(B, T):
+    """Rows enough to fill the card with one range a sequence, which would span 2 GiB of codes: cut into ranges that do not, for all
+    sequences and in the list of unequal ones.  All positions are zero but a few at the ends and at 2^20, so the sums are known."""
+    from k3hip.mla_q4 import mla_q4_attention
+    n, H = (1 << 23) + 5000, 128
+    packed, scales, rot = _cache(B, n)
+    scales.fill_(127)
+    q_nope, q_rot, wk, wv, p, s, r = _problem(B, T, H, 8, 410, std=8.0)
+    at = torch.tensor([0, (1 << 20) - 1, 1 << 20, n // 2, n - 2 * T, n - 40, n - 2, n - 1], device="cuda")
+    packed[0, at], scales[0, at], rot[0, at] = p[0], s[0], r[0]
+    o = mla_q4_attention(q_nope, q_rot, wk, wv, packed, scales, rot, SCALE, lengths=None if B == 1 else _ints([n, 3]))
+    qa = torch.matmul(q_nope[0].transpose(0, 1).double(), wk.double())                          # [H, T, 512]
+    lat, rows = oracle.values(p[0], s[0]), r[0].double()
+    qr = q_rot[0].transpose(0, 1).double()
+    sees = n - T + 1 + torch.arange(T, device="cuda")
+    z = (torch.matmul(qa, lat.T.contiguous()) + torch.matmul(qr, rows.T.contiguous())) * SCALE  # [H, T, 8]
+    z = z.masked_fill(at >= sees[:, None], -math.inf)
+    m = z.amax(-1, keepdim=True).clamp(min=0)
+    e = torch.exp(z - m)
+    zeros = (sees - (at < sees[:, None]).sum(1))[:, None]
+    prob = e / (e.sum(-1, keepdim=True) + zeros * torch.exp(-m))
+    want = torch.matmul(torch.matmul(prob, lat), wv.double().transpose(1, 2).contiguous())
+    # a probability: as over 2^24 positions, a lane's longest run being 16 a round over a range of 2^20: 2^18 additions, 2^-6
+    mags = (torch.matmul(qa.abs(), lat.abs().T.contiguous()) + torch.matmul(qr.abs(), rows.abs().T.contiguous())).amax(-1, keepdim=True) * SCALE
+    rel = 2 * 2.0 ** -18 * mags + 2.0 ** -6
+    mag = torch.matmul(torch.matmul(prob, lat.abs()), wv.double().abs().transpose(1, 2).contiguous())
+    assert bool(((o[0].transpose(0, 1).double() - want).abs() <= rel * mag).all())
+    assert float(mag.mean()) > 1e-3 and not o[1:].any()
+
+
 def test_prompt_in_several_passes(monkeypatch):
     """More rows than one pass over the queries takes (65,536): the same as its parts."""
     from k3hip.mla_q4 import mla_q4_attention
