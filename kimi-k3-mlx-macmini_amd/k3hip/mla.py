@@ -322,7 +322,11 @@ class MLAAttention:
         cache.append(c_new, r_new)
         scale = qhd ** -0.5
         if q4 and self.kv_b.dtype == torch.bfloat16:
-            o = cache.attend(q[..., :nope], q[..., nope:], self.wk, self.wv, scale, gate)
+            try:
+                o = cache.attend(q[..., :nope], q[..., nope:], self.wk, self.wv, scale, gate)
+            except BaseException:
+                cache.length -= Tn      # (refused, or no memory: a caller that tries again appends the same tokens)
+                raise
             return mm(o.reshape(B, Tn, nh * vhd), self.o_w), cache
         lat, rot = cache.view()
         # one query token: the HIP core, over a bf16 cache or the reference's default fp32

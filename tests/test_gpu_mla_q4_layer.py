@@ -194,6 +194,23 @@ def test_refusals_leave_the_cache(T):
     assert cache.length == 10 and all(torch.equal(a, b) for a, b in zip(cache.buffers(), before))
 
 
+def test_a_misaligned_buffer_leaves_the_cache_at_its_length():
+    """Scale rows at an odd address: the append writes them, the attention refuses them, and a sound buffer goes on from there."""
+    layer, w = _layer(4)
+    _, cache = layer(_x(3, 1, 10))
+    scales = cache.scales
+    cache.scales = torch.zeros(1, 256, 17, dtype=torch.uint8, device="cuda")[..., 1:]
+    before = [t[:, :10].clone() for t in cache.buffers()]
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            layer(_x(4, 1, 3), cache)
+        assert cache.length == 10 and all(torch.equal(a[:, :10], b) for a, b in zip(cache.buffers(), before))
+    cache.scales = scales
+    out, _ = layer(_x(4, 1, 3), cache)
+    assert cache.length == 13
+    _close(out, _want(w, 4, _x(4, 1, 3), cache)[0])
+
+
 def test_another_batch_is_refused():
     layer, w = _layer(4)
     _, cache = layer(_x(3, 2, 10))

@@ -160,3 +160,25 @@ def test_layer_takes_a_batch_past_65536_rows(monkeypatch):
     out, cache = layer(torch.zeros(700, 1, 64))
     assert out.shape == (700, 1, 64) and cache.length == 1
     assert [name for name, _ in calls] == ["k3_mla_q4_append"] + ["k3_mla_q4_attention"] * 2
+
+
+# ------------------------------------------------------------------------------- a refusal after the append
+@pytest.mark.parametrize("B,T", [(1, 3), (2, 1)])
+def test_layer_takes_back_positions_that_are_not_attended_to(monkeypatch, B, T):
+    """Append takes buffers that attention refuses (a misaligned view, say): then the cache is as long as it was."""
+    from k3hip import _lib
+    from k3hip.mla_q4 import new_cache_q4
+    from test_mla_q4_host import _cfg, _layer
+    calls = _launches(monkeypatch)
+    layer, cache, x = _layer(_cfg()), new_cache_q4(B, 1, device="cpu"), torch.zeros(B, T, 64)
+    layer(x, cache)
+
+    def refuse(name, *a):
+        calls.append((name, a))
+        if name == "k3_mla_q4_attention":
+            raise ValueError("must be 16-byte (scales 4-byte) aligned")
+    monkeypatch.setattr(_lib, "call", refuse)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="aligned"):
+            layer(x, cache)
+        assert cache.length == T and calls[-2][0] == "k3_mla_q4_append" and calls[-2][1][18] == T
