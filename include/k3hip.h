@@ -498,7 +498,10 @@ int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim,
  *   lengths[b] left as they are.
  * A query that sees nothing (also: t >= counts[b]) gets zeros and adds nothing to weight.  Deterministic.  The cache's
  * values enter exactly; the absorbed queries to 2^-12 of a unit under their group's largest for a bf16 out without weight,
- * else 2^-22; the probabilities to 2^-11 for a bf16 out, 2^-22 for fp32; sums and softmax in fp32.
+ * else 2^-22; the probabilities, for the context, to 2^-11 for a bf16 out, 2^-22 for fp32, and none closer than 2^-35 of the
+ * largest in its range (fp16's smallest step: n positions under that beside one lose up to n 2^-35 of the output; the divisor
+ * and weight count them); the context before W_UV to 2^-17 for a bf16 out of many queries (more than
+ * 256 tiles of 16 queries of a head), else 2^-24; sums and softmax in fp32.  A score of -infinity counts as hidden.
  * nope a multiple of 8 up to 256, v one up to 1024, H <= 4096, B H <= 65536, max_length <= 2^24.  Pointers 16-byte
  * aligned (scales 4-byte); p_row and p_batch multiples of 16, rot pitches of 8, scale pitches of 4.
  * Row pitches up to 64 KB; from 2 KB on the rows of one range, up to 2^20 positions, must span less than 2 GiB.

@@ -20,7 +20,9 @@
 // Values.  The second product's operands are fp16: E2M1 times 2^-23 .. 2^13 (scale bytes 104 .. 140) is exact in it,
 // and its 11 bits make one term of a probability enough for a bf16 result (2^-11 each, independent, below the
 // result's own 2^-8) and two for fp32 (2^-22), where bf16 would need two and three.  Probabilities are 2^kLift times those of the
-// row's reference maximum, so fp16's last bit, 2^-24, is 2^-34 of the largest.  A block that has come upon a scale
+// row's reference maximum, so fp16's last bit, 2^-24, is 2^-34 of the largest, and a probability is off by up to half of that whatever
+// its size: n positions below 2^-35 beside one that takes all lose n 2^-35 of the context at most (2^-20 over 32,768; the divisor, in
+// fp32, counts them).  A block that has come upon a scale
 // byte outside that range goes over its positions again with bf16 operands, exact for every byte, and one term more.
 //
 // Query operands of 16 rows (a row: one head of one query), `terms` latent and `rterms` rotary terms:

@@ -110,8 +110,8 @@ def mla_q4_append(c_new: torch.Tensor, r_new: torch.Tensor, packed: torch.Tensor
     ``start``: a whole number (positions past the capacity are a ValueError), or an int32 [B] device tensor, every
     sequence its own; ``counts`` int32 [B]: only sequence b's first counts[b] tokens are written.  Positions
     that a tensor puts outside the capacity are left out.  A group's scale is the power of two that puts its
-    largest magnitude at 4 to 7 times itself (above 7 the next one); codes round to nearest even.  A position with a NaN or an
-    infinity is NaN to every query that sees it.  ``weight`` fp32 [B, cap]: the attention that positions have received, zeroed where one
+    largest magnitude at 4 to 7 times itself (above 7 the next one); codes round to nearest even.  A position whose latent holds a NaN
+    or an infinity is NaN to every query that sees it.  ``weight`` fp32 [B, cap]: the attention that positions have received, zeroed where one
     is written.
     """
     starts = start if isinstance(start, torch.Tensor) else None

@@ -314,6 +314,37 @@ def test_growing_scores_move_the_reference():
     _check((q_nope, q_rot, wk, wv, packed, scales, rot), weight=True)
 
 
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("T,H,n", [(129, 64, 4096), (1, 16, 700)])
+@pytest.mark.parametrize("k", [10, 20, 28, 33, 36])
+def test_a_long_flat_tail_beside_one_large_position(k, T, H, n, out):
+    """Position 0 has 2^k times the weight of any other and no values, so the output is the tail's alone: 129 queries run over all
+    positions as one range.  Bounds, u = 2^-24: scores of up to 25 (72 u of them, twice, for a probability and the divisor: 2^-12), the sums
+    (v / 8 + 300) u < 2^-14, W_UV 66 u, the rotary query's terms 2^-25 of a score (bf16: 2^-17, twice: 2^-11.3), a probability's 2^-22
+    (bf16: 2^-11): 2^-11 in all, for bf16 2^-10 more and the output's rounding; and, whatever a probability's size, fp16's half step, 2^-35 of the largest, for each position."""
+    from k3hip.mla_q4 import mla_q4_attention
+    wk, wv = (t.cuda() for t in (_rand(420, H, 128, 512, std=512 ** -0.5, dtype=BF16), _rand(421, H, 128, 512, std=512 ** -0.5, dtype=BF16)))
+    packed, scales, rot = _cache(1, n)
+    packed[0, 1:], rot[0, 0, 0] = 0x22, 1.0                    # the tail's values are all 1
+    scales.fill_(127)
+    q_nope, q_rot = torch.zeros(1, T, H, 128, device="cuda"), torch.zeros(1, T, H, 64, device="cuda")
+    q_rot[..., 0] = k * math.log(2) / SCALE
+    weight = torch.zeros(1, n, device="cuda")
+    o = mla_q4_attention(q_nope, q_rot, wk, wv, packed, scales, rot, SCALE, out_dtype=out)
+    mla_q4_attention(q_nope, q_rot, wk, wv, packed, scales, rot, SCALE, out_dtype=out, weight=weight)
+    tail = (n - T + torch.arange(T, device="cuda")).double()   # positions of it that query t sees
+    p = 1 / (2.0 ** k + tail)
+    rows, mags = wv.double().sum(2), wv.double().abs().sum(2)  # [H, v]
+    want = (p * tail)[:, None, None] * rows
+    tol = 2.0 ** -11 * (p * tail)[:, None, None] * mags + (tail * 2.0 ** -35 * 2.0 ** k * p)[:, None, None] * mags
+    if out == BF16:
+        tol += 2.0 ** -10 * (p * tail)[:, None, None] * mags + 2.0 ** -8 * want.abs()
+    assert bool(((o[0].double() - want).abs() <= tol).all()), float(((o[0].double() - want).abs() / tol).max())
+    # the summed weights count every position, however small
+    got, one = weight[0, 1:n - T + 1].double(), H * float(p.sum())
+    assert bool(((got - one).abs() <= 2.0 ** -11 * one).all())
+
+
 @pytest.mark.parametrize("T,H,n,out", [(1, 64, 20000, F32), (1, 64, 20000, BF16), (4, 96, 6000, BF16), (128, 16, 1024, F32)])
 def test_long_caches(T, H, n, out):
     args = _problem(1, T, H, n, 120)
