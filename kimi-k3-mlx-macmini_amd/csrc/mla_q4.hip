@@ -1220,7 +1220,7 @@ Rows rows_of(int64_t T, int64_t H) {
 }
 
 // What the launches are cut into; a function of its arguments alone.
-Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t V, int64_t npos, int q_bf16, int out_bf16, int weights, int varied) {
+Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t npos, int q_bf16, int out_bf16, int weights, int varied) {
     Plan p{};
     const bool fine = !out_bf16 || weights;
     p.NT = fine ? 5 : 3, p.RT = q_bf16 ? 1 : fine ? 3 : 2, p.PT = out_bf16 ? 1 : 2;
@@ -1372,7 +1372,7 @@ using namespace k3;
 extern "C" int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim, int64_t max_length, int q_dtype,
                                             int out_dtype, int weights, int varied) {
     if (B <= 0 || T <= 0 || H <= 0 || v_dim <= 0 || max_length < 0) return 0;
-    return plan_of(B, T, H, v_dim, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weights != 0, varied != 0).total;
+    return plan_of(B, T, H, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weights != 0, varied != 0).total;
 }
 
 extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t qn_token, int64_t qn_head, const void *q_rot,
@@ -1407,7 +1407,7 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
     if (!aligned16(q_nope) || !aligned16(q_rot) || !aligned16(w_uk) || !aligned16(w_uv) || !aligned16(out) || !aligned16(workspace) ||
         !aligned16(packed) || !aligned16(rot) || (reinterpret_cast<uintptr_t>(scales) & 3u) || (gate && !aligned16(gate)))
         return set_error(K3_ERR_ALIGN, "mla q4: queries, weights, cache, output and workspace must be 16-byte (scales 4-byte) aligned");
-    const Plan p = plan_of(B, T, H, v_dim, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weight != nullptr, lengths != nullptr);
+    const Plan p = plan_of(B, T, H, max_length, q_dtype == K3_BF16, out_dtype == K3_BF16, weight != nullptr, lengths != nullptr);
     if (workspace_bytes < p.total)
         return set_error(K3_ERR_WORKSPACE, "mla q4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.total);
     // (a range of a list is at most as long as all positions shared out: 1.01 kLongest + 128 positions, 1.02 2^30 bytes at pitches of 1 KB)
@@ -1417,7 +1417,7 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
     auto st = static_cast<hipStream_t>(stream);
     char *ws = static_cast<char *>(workspace);
     for (int64_t t0 = 0; t0 < T; t0 += p.order.T) {
-        // (the last pass may have fewer queries; its order stays that of the others, whose room it has)
+        // (the last pass may have fewer queries, so few that its rows go by query; it has the others' room, block height and join)
         Rows order = rows_of(std::min<int64_t>(p.order.T, T - t0), H);
         const int rows = order.count(), M = static_cast<int>(B * order.T);
         const int64_t q_seq = static_cast<int64_t>(p.tiles) * q4_tile_bytes(p.NT, p.RT);

@@ -438,6 +438,50 @@ def test_prompt_in_several_passes(monkeypatch):
     assert abs(float(weight.double().sum()) - T * H) < 2 ** -16 * T * H
 
 
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_a_last_pass_of_few_queries(out):
+    """1024 queries of 64 heads and 5 more, whose rows go by query where the others' go by head: outputs under a gate on both sides
+    of the boundary, and the weights of both passes together."""
+    from k3hip.mla_q4 import mla_q4_attention
+    T, H = 1029, 64
+    args = _problem(1, T, H, T, 430, x=BF16)
+    gate = _rand(434, 1, T, H * 128).cuda()
+    weight = torch.zeros(1, T, device="cuda")
+    o = mla_q4_attention(*args, SCALE, weight=weight, gate=gate, out_dtype=out)
+    for t in (0, 1022, 1023, 1024, 1025, 1028):
+        part = (args[0][:, t:t + 1], args[1][:, t:t + 1], *args[2:])
+        want, tol, _, _ = oracle.attention(*part, SCALE, [t + 1], [1], True, out == F32, torch.finfo(out).eps / 2)
+        open_by = torch.sigmoid(gate[0, t].double()).view(1, 1, H, 128)      # (in fp32 to 2^-21)
+        assert bool(((o[:, t:t + 1].double() - want * open_by).abs() <= tol * open_by + 2.0 ** -21 * want.abs()).all())
+    parts = torch.zeros(1, T, device="cuda")
+    mla_q4_attention(args[0][:, :1000], args[1][:, :1000], *args[2:], SCALE, lengths=1000, weight=parts)
+    mla_q4_attention(args[0][:, 1000:], args[1][:, 1000:], *args[2:], SCALE, weight=parts)
+    assert bool(((weight - parts).abs() <= 2 ** -16 * parts).all())
+    assert abs(float(weight.double().sum()) - T * H) < 2 ** -16 * T * H
+
+
+def test_several_passes_of_several_sequences():
+    """Three sequences of 346 queries of 64 heads, 341 and 5 a pass, with lengths and counts of their own."""
+    from k3hip.mla_q4 import mla_q4_attention
+    B, T, H, cap = 3, 346, 64, 400
+    args, lengths, counts = _problem(B, T, H, cap, 440), [400, 346, 150], [346, 344, 345]
+    weight = torch.zeros(B, cap, device="cuda")
+    o = mla_q4_attention(*args, SCALE, lengths=_ints(lengths), counts=_ints(counts), weight=weight)
+    for b in range(B):
+        one = [t[b:b + 1] for t in (args[0], args[1], *args[4:])]
+        for t in (0, 194, 195, 196, 340, 341, 343, 344, 345):
+            sees = max(0, lengths[b] - counts[b] + t + 1) if t < counts[b] else 0
+            if sees == 0:
+                assert not o[b, t].any()
+                continue
+            part = (one[0][:, t:t + 1], one[1][:, t:t + 1], *args[2:4], *one[2:])
+            want, tol, _, _ = oracle.attention(*part, SCALE, [sees], [1], True, True, 2.0 ** -24)
+            assert bool(((o[b:b + 1, t:t + 1].double() - want).abs() <= tol).all()), (b, t)
+        alone, n = torch.zeros(1, cap, device="cuda"), counts[b]
+        mla_q4_attention(one[0][:, :n], one[1][:, :n], *args[2:4], *one[2:], SCALE, lengths=lengths[b], weight=alone)
+        assert bool(((weight[b:b + 1] - alone).abs() <= 2 ** -16 * alone).all()) and not weight[b, lengths[b]:].any()
+
+
 def test_a_batch_past_65536_rows():
     """900 sequences of 80 heads, 72,000 rows, in two launches of the kernels; a gate, lengths of every size."""
     from k3hip.mla_q4 import mla_q4_attention
