@@ -1034,7 +1034,8 @@ constexpr int kWTiles = 4;   // tiles of 16 positions per wave
 // chunk y .. of its sequence one after the other, each staged in LDS for its eight waves while the last one is worked on, and adds
 // their probabilities, exp2(c s - log2 of the row's divisor); part[chunk][b][position].  One block a CU: 4000 tiles of 1000 queries of 64 heads
 // over as many positions take 100 us, 6000 cycles a tile where its products need 2800 (the rest: exponentials, and the products'
-// operands from LDS, 34 KB a wave); one tile over 20,001 positions 9 us, most of it the first loads.
+// operands from LDS, 34 KB a wave), and the chunks are uneven there: the first 512 positions are seen by all of their 32 tiles, the others by
+// half; one tile over 20,001 positions 9 us, most of it the first loads.
 template <int NT, int RT>
 __global__ __launch_bounds__(512, 1) void weights_kernel(WeightArgs wa) {
     extern __shared__ __attribute__((aligned(16))) char lds[];

@@ -10,7 +10,9 @@
 // With norm weights the row is RMS-normalised first, in fp32 (the decode step's latent).
 //
 // A wave takes one position: 64 lanes x 8 values, a group is four lanes, its maximum two lane swaps, and a lane's eight
-// codes are one dword, so loads and stores are whole lines.  Bound by HBM on a prompt, by the launch for one token.
+// codes are one dword, so loads and stores are whole lines.  One token 1.9 us: the launch.  Four
+// sequences of 1024 to 8192 tokens, bf16: 21 MB in 9.4 us, 2.3 TB/s, where a copy reaches 5.1: blocks of four positions, many of them past
+// their sequence's end, and one row's load in flight a wave.
 #include "mla_q4.h"
 
 namespace k3 {
