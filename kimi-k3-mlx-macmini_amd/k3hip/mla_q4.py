@@ -24,7 +24,7 @@ from . import _torch as T
 LATENT, ROPE, GROUP = 512, 64, 32
 # Scratch up to this size is kept per stream (a decode step's); larger scratch, a prompt's, is the call's own.
 KEPT_WORKSPACE = 1 << 26
-MAX_ROWS = 1 << 16      # heads x sequences of one k3_mla_q4_attention
+MAX_ROWS, MAX_SEQUENCES = 1 << 16, (1 << 16) - 1      # heads x sequences, and sequences, of one k3_mla_q4_attention
 
 
 # What a call's layout (shapes, strides, dtypes; no addresses) comes to, once its checks are passed: the checks cost
@@ -188,9 +188,10 @@ def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor
     out = torch.empty((B, Tq, H, V), dtype=out_dtype, device=device)
     if B == 0 or Tq == 0:
         return out
-    if B * H > MAX_ROWS and B > 1:
-        for b in range(0, B, max(1, MAX_ROWS // H)):
-            part = slice(b, min(B, b + max(1, MAX_ROWS // H)))
+    if B > MAX_SEQUENCES or (B * H > MAX_ROWS and B > 1):
+        most_at_once = max(1, min(MAX_SEQUENCES, MAX_ROWS // max(1, H)))
+        for b in range(0, B, most_at_once):
+            part = slice(b, min(B, b + most_at_once))
             cut = [None if t is None else t[part] for t in (lengths, counts, weight, gate)]
             out[part] = mla_q4_attention(q_nope[part], q_rot[part], wk, wv, packed[part], scales[part], rot[part], scale,
                                          most if lengths is None else cut[0], *cut[1:], out_dtype)

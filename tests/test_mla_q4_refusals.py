@@ -147,6 +147,15 @@ def test_a_batch_past_65536_rows_goes_out_in_parts(monkeypatch, lengths):
         first += n
 
 
+@pytest.mark.parametrize("B,H,parts", [(65536, 1, [65535, 1]), (65535, 1, [65535]), (16, 4096, [16]), (17, 4096, [16, 1])])
+def test_parts_keep_within_what_one_call_takes(monkeypatch, B, H, parts):
+    from k3hip.mla_q4 import mla_q4_attention
+    calls = _launches(monkeypatch)
+    q, w = torch.zeros(1, 1, 1, 72).expand(B, 1, H, 72), torch.zeros(1, 8, 1).to(BF16).expand(H, 8, 512)
+    mla_q4_attention(q[..., :8], q[..., 8:], w, w, *(t.expand(B, -1, -1) for t in _cache(1, 2)), 0.1)
+    assert [a[23] for _, a in calls] == parts
+
+
 def test_layer_takes_a_batch_past_65536_rows(monkeypatch):
     from types import SimpleNamespace
 
