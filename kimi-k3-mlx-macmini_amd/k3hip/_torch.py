@@ -50,6 +50,11 @@ def current(device: torch.device):
     return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def capturing() -> bool:
+    """Whether the current stream is being captured into a graph."""
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 def require_device(*ts: torch.Tensor) -> None:
     dev = None
     for t in ts:

@@ -46,7 +46,7 @@ import torch
 
 from . import _blas, _lib, _workspace
 from . import _torch as T
-from .mla_q4 import MLACacheQ4, new_cache_q4
+from .mla_q4 import MLACacheQ4, new_cache_q4, scratch
 
 CACHE_STEP = 256
 KV_LORA_RANK = 512
@@ -438,7 +438,7 @@ class MLAAttention:
             p_row, s_row, rot_row = cache.row_pitches()
             nbytes = _lib.size("k3_mla_step_q4_workspace_size", ql, nh, nope, rope, vhd, klr, pos + 1, int(weight is not None))
             with T.current(x.device):
-                ws = _workspace.get(x.device, nbytes, "mla_step")
+                ws = scratch(x.device, nbytes, "mla_step")
                 _lib.call("k3_mla_step_decode_q4", *front, T.ptr(packed), p_row, T.ptr(scales), s_row, T.ptr(rot), rot_row, T.ptr(weight), *back,
                           T.ptr(ws), ws.numel(), T.stream(xin))
         else:

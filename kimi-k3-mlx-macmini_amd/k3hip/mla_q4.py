@@ -22,7 +22,7 @@ from . import _lib, _workspace
 from . import _torch as T
 
 LATENT, ROPE, GROUP = 512, 64, 32
-# Scratch up to this size is kept per stream (a decode step's); larger scratch, a prompt's, is the call's own.
+# Scratch up to this size is kept per stream (a decode step's); larger scratch, a prompt's, is the call's own, and so is a captured call's.
 KEPT_WORKSPACE = 1 << 26
 MAX_ROWS, MAX_SEQUENCES = 1 << 16, (1 << 16) - 1      # heads x sequences, and sequences, of one k3_mla_q4_attention
 
@@ -95,6 +95,14 @@ def _weight_pitch(weight: torch.Tensor | None, B: int, cap: int) -> int:
         raise ValueError(f"weight must be [{B}, {cap}] with contiguous rows; got {tuple(weight.shape)}")
     _apart(weight, "weight")
     return weight.stride(0) if B > 1 else 0
+
+
+def scratch(device: torch.device, nbytes: int, tag: str) -> torch.Tensor:
+    """Workspace of a call on device, the current one.  A captured call's is its graph's, also where the stream has a kept one: two graphs
+    captured after a call there may replay side by side, and one would take the other's list of ranges."""
+    if nbytes > KEPT_WORKSPACE or T.capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _workspace.get(device, nbytes, tag)
 
 
 def _rows_ok(t: torch.Tensor, per: int) -> bool:
@@ -206,8 +214,7 @@ def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor
     ns, rs = q_nope.stride(), q_rot.stride()
     nbytes = _lib.size("k3_mla_q4_workspace_size", *sizes[:4], most, *sizes[4:])
     with T.current(device):
-        ws = (_workspace.get(device, nbytes, "mla_q4") if nbytes <= KEPT_WORKSPACE
-              else torch.empty(nbytes, dtype=torch.uint8, device=device))
+        ws = scratch(device, nbytes, "mla_q4")
         _lib.call("k3_mla_q4_attention", q_nope.data_ptr(), ns[0], ns[1], ns[2], q_rot.data_ptr(), rs[0], rs[1], rs[2], code,
                   wk.data_ptr(), wv.data_ptr(), packed.data_ptr(), *pp, scales.data_ptr(), *sp, rot.data_ptr(), *rp, T.ptr(lengths),
                   T.ptr(counts), most, B, Tq, H, LATENT, ROPE, nope, V, scale, T.ptr(gate), out.data_ptr(), out_code, T.ptr(weight),

@@ -603,6 +603,39 @@ def test_two_captured_graphs_do_not_share_scratch():
             assert torch.equal(o, y)
 
 
+def test_graphs_captured_on_a_stream_in_use_replay_side_by_side():
+    """A stream with a workspace of its own from eager calls, and two graphs captured on it, batches of other sizes whose lists of
+    ranges do not fit each other: replayed at once on two streams, beside eager calls on the first."""
+    from k3hip.mla_q4 import mla_q4_attention
+    a, b = _problem(20, 1, 64, 900, 450), _problem(3, 2, 32, 500, 460)
+    calls = [(a, _ints(_lengths("spread", 20, 900))), (b, _ints([500, 0, 77]))]
+    want = [mla_q4_attention(*x, SCALE, lengths=n) for x, n in calls]
+    stream, graphs, outs = torch.cuda.Stream(), [], []
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for x, n in calls:
+            mla_q4_attention(*x, SCALE, lengths=n)
+    torch.cuda.synchronize()
+    for x, n in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            outs.append(mla_q4_attention(*x, SCALE, lengths=n))
+        graphs.append(g)
+    others = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, others):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(stream):
+            eager = [mla_q4_attention(*x, SCALE, lengths=n) for x, n in calls]
+        torch.cuda.synchronize()
+        for o, e, y in zip(outs, eager, want):
+            assert torch.equal(o, y) and torch.equal(e, y)
+
+
 def test_two_threads_on_one_stream():
     import threading
 

@@ -191,3 +191,24 @@ def test_layer_takes_back_positions_that_are_not_attended_to(monkeypatch, B, T):
         with pytest.raises(ValueError, match="aligned"):
             layer(x, cache)
         assert cache.length == T and calls[-2][0] == "k3_mla_q4_append" and calls[-2][1][18] == T
+
+
+# ------------------------------------------------------------------------------- scratch of captured calls
+def test_a_captured_call_takes_no_kept_workspace(monkeypatch):
+    """Not even one that its stream has: another graph captured there would have the same."""
+    from k3hip import _torch as T
+    from k3hip import _workspace
+    from k3hip.mla_q4 import new_cache_q4
+    from test_mla_q4_host import _cfg, _layer
+    calls, kept = _launches(monkeypatch), []
+    monkeypatch.setattr(_workspace, "get", lambda d, n, tag="": kept.append(tag) or torch.empty(n, dtype=U8))
+    layer, cache, x = _layer(_cfg()), new_cache_q4(1, 4, device="cpu"), torch.zeros(1, 1, 64)
+    layer._mats = {k: m for k, m in (("q_a", layer.q_a), ("q_b", layer.q_b), ("kv_a", layer.kv_a), ("g", None), ("o", layer.o_w))}
+    layer._q_an32, layer._kv_an32 = layer.q_an.float(), layer.kv_an.float()
+    for captured, want in ((False, ["mla_q4", "mla_step"]), (True, [])):
+        monkeypatch.setattr(T, "capturing", lambda: captured, raising=False)
+        _attend(_cache(), lengths=torch.ones(2, dtype=torch.int32))
+        layer.decode_step(x, cache)
+        assert kept == want
+        kept.clear()
+    assert [name for name, _ in calls] == ["k3_mla_q4_attention", "k3_mla_step_decode_q4"] * 2
