@@ -35,6 +35,7 @@ extern "C" {
 /* ---- dtype enums ------------------------------------------------------------------- */
 #define K3_F32   0
 #define K3_BF16  1
+#define K3_F16   2   /* pages of the paged latent cache only */
 
 /* ---- activation enums (expert FFN) ------------------------------------------------- */
 #define K3_ACT_SILU  0   /* silu(g) * u                         (air_llm/models/kimi_k3/ops.py:42-43) */
@@ -546,6 +547,67 @@ int k3_cache_evict(const float *weight, int64_t w_batch, const int32_t *lengths,
                    const void *const *src, const int64_t *src_batch, const int64_t *src_row, void *const *dst,
                    const int64_t *dst_batch, const int64_t *dst_row, const int64_t *row_bytes, int64_t dst_rows,
                    void *stream);
+
+/* ---- the paged latent cache -------------------------------------------------------------- */
+
+/* Workspace bytes of k3_page_tables for B requests.  No initialisation. */
+int64_t k3_page_tables_workspace_size(int64_t B);
+
+/* Changes the lengths of B requests whose cache lies in pages of page_size positions (a power of two up to 65536), and gives
+ * their new tokens' rows.  Request b holds lengths[b] positions (taken as 0 .. blocks * page_size), its pages the first entries
+ * of row b of table [B, blocks] (rows table_row entries apart); it is to hold target[b] (negative: 0).  free_list [pages]: its
+ * entries from used[0] on (taken as 0 .. pages) are the pages that nobody holds.
+ *   - A request that shrinks gives back its pages from the target's on, but none of its first shared[b] (shared null: none): all,
+ *     in the batch's order, are written before entry `used` of the list, whose free entries begin at base = used - returned (never
+ *     below 0; more than `used` pages given back are dropped).  Its row of the table stays.
+ *   - A request that grows takes its pages from base on, one request after the other, and they are written into its row; from the first
+ *     one on that the list has not enough for, requests that need pages stay as they are.  So does one whose target does not fit `blocks`.
+ *   - new_lengths [B], new_used [1]: what came of it; slots [B, tokens]: the row of request b's i-th new token in the pool, page *
+ *     page_size + position % page_size, -1 past its new length (tokens 0: slots may be null).
+ * new_lengths may be lengths (or target), and new_used may be used; other buffers must not overlap.  One launch up to 4096 tokens (B *
+ * tokens) of up to 2048 requests, else two.  blocks * page_size < 2^31.  No counterpart in the reference, whose cache is one sequence's. */
+int k3_page_tables(int32_t *table, int64_t table_row, int64_t blocks, const int32_t *lengths, const int32_t *target,
+                   const int32_t *shared, int32_t *free_list, int64_t pages, const int32_t *used, int64_t page_size, int64_t B,
+                   int64_t tokens, int32_t *new_lengths, int32_t *new_used, int32_t *slots, void *workspace,
+                   int64_t workspace_bytes, void *stream);
+
+/* Rounds c [B, T, 512] and r [B, T, 64] (bf16 or fp32; pitches in elements, c's whole 16 bytes) into rows slots [B, T] int32 of a pool
+ * of pages: row s is row s % page_size of page s / page_size, lat rows of 512 and rot rows of 64 elements of cache_dtype (K3_F16 or
+ * K3_BF16), lat_row and rot_row apart, pages lat_page and rot_page apart (elements; lat's whole 16 bytes).  norm [512] fp32 or null: c is
+ * RMS-normed first, norm * c / sqrt(mean(c^2) + eps).  One rounding to nearest (above fp16's largest: infinity).  Slots outside the pool
+ * are left out; a call's others must differ.  Counterpart of MLACache.append (air_llm/models/kimi_k3/attention_mla.py:89-108). */
+int k3_mla_paged_append(const void *c, int64_t c_batch, int64_t c_row, int c_dtype, const void *r, int64_t r_batch, int64_t r_row,
+                        int r_dtype, const float *norm, float eps, const int32_t *slots, void *lat, int64_t lat_page,
+                        int64_t lat_row, void *rot, int64_t rot_page, int64_t rot_row, int cache_dtype, int64_t pages,
+                        int64_t page_size, int64_t B, int64_t T, int64_t kv_lora_rank, int64_t rope_dim, void *stream);
+
+/* Workspace bytes of k3_mla_paged_attention for the same sizes (shared: positions of the common prefix).  No initialisation. */
+int64_t k3_mla_paged_workspace_size(int64_t B, int64_t T, int64_t H, int64_t max_length, int64_t shared, int cache_dtype, int out_dtype);
+
+/* The absorbed attention of T queries of each of B sequences over a paged cache, causal: query t of sequence b's first counts[b] sees
+ * positions 0 .. lengths[b] - counts[b] + t.
+ *   o[b,t,h] = W_UV[h] (softmax_j(scale (q_nope[b,t,h] W_UK[h] . lat_j + q_rot[b,t,h] . rot_j)) lat_j)
+ * Positions below prefix_pages * page_size lie in the pages prefix [prefix_pages], read and multiplied once for all sequences; position j of
+ * the others in page table[b][j / page_size] (rows of the table table_row >= blocks entries apart).  A position whose page is not one of
+ * 0 .. pages - 1 counts as not there.
+ * q_nope [B, T, H, nope], q_rot [B, T, H, 64]: bf16 or fp32 (both the same), pitches in elements, multiples of 4; w_uk [H, nope, 512],
+ *   w_uv [H, v, 512] bf16; lat, rot: as k3_mla_paged_append's, all pitches whole 16 bytes; page_size a power of two, 32 .. 65536;
+ * lengths int32 [B] on the device (taken as 0 .. max_length, at most blocks * page_size), counts int32 [B] on the device (taken as 0 .. T) or
+ *   null: T; gate [B, T, H, v] fp32 logits or null: o times sigmoid(gate); out [B, T, H, v] contiguous, out_dtype.
+ * A query that sees nothing (also: t >= counts[b]) gets zeros.  Deterministic.  fp16 pages: the absorbed queries enter as one fp16 term
+ * for a bf16 out (2^-11, and none closer than 2^-38 of the largest of its 128 columns), two for fp32 (2^-22); probabilities as one (2^-11) or two
+ * (2^-22), none closer than 2^-32 of the row's largest.  bf16 pages: two bf16 terms of both (2^-16).  The context before W_UV: two bf16 terms
+ * for a bf16 out (2^-16), else three; sums and softmax in fp32.  A masked position's values do not matter, whatever they are.
+ * nope a multiple of 8 up to 256, v one up to 1024, H <= 4096, B H <= 65536, max_length <= 2^24.  Pointers 16-byte aligned.
+ * Counterpart of MLAAttention.__call__'s core for a batch (air_llm/models/kimi_k3/attention_mla.py:193-212). */
+int k3_mla_paged_attention(const void *q_nope, int64_t qn_batch, int64_t qn_token, int64_t qn_head, const void *q_rot,
+                           int64_t qr_batch, int64_t qr_token, int64_t qr_head, int q_dtype, const void *w_uk, const void *w_uv,
+                           const void *lat, int64_t lat_page, int64_t lat_row, const void *rot, int64_t rot_page, int64_t rot_row,
+                           int cache_dtype, int64_t pages, int64_t page_size, const int32_t *table, int64_t table_row, int64_t blocks,
+                           const int32_t *prefix, int64_t prefix_pages, const int32_t *lengths, const int32_t *counts,
+                           int64_t max_length, int64_t B, int64_t T, int64_t H, int64_t kv_lora_rank, int64_t rope_dim,
+                           int64_t nope_dim, int64_t v_dim, float scale, const float *gate, void *out, int out_dtype,
+                           void *workspace, int64_t workspace_bytes, void *stream);
 
 /* ---- Kimi Delta Attention recurrent step (one token) -------------------------------------- */
 

@@ -1,0 +1,901 @@
+// Latent (MLA) attention of a batch over a paged cache, in the absorbed form: one token or several of each of B sequences, the
+// positions of a common prefix read and multiplied once for all of them.
+//
+//     qa[b,t,h]  = q_nope[b,t,h] W_UK[h]                                             [512]
+//     s[b,t,h,j] = scale (qa[b,t,h] . lat_j + q_rot[b,t,h] . rot_j)                   j < sees(b, t)
+//     p = softmax_j(s);   o[b,t,h] = W_UV[h] (sum_j p[b,t,h,j] lat_j)
+//
+// A row is one head of one query.  Every row reads the same 1152 bytes of a position, so a set of rows over a range of positions is two
+// matrix products, 2176 flops a pair: for a sequence its own T x H rows, for the prefix the rows of all sequences.  Launches:
+//   qa       q_nope W_UK on the bf16 matrix cores (fp32 queries as three bf16 terms), rounded into the terms that attend multiplies; a block
+//            more makes the list of items
+//   attend   an item a block: a tile of rows x a range of positions; the maximum and sum run with the positions
+//   uv       the items' records joined (prefix ranges and own ranges alike), the context times W_UV, the output gate
+//
+// Numerics.  fp16 pages multiply as fp16: 11 bits make one term of a query or probability enough for a bf16 result (off by 2^-11 at most, independent
+// errors below the result's own 2^-8) and two for fp32 (2^-22); bf16 terms would need two and three.  The absorbed query's 128 columns
+// of a quarter, and its rotary columns, are scaled by a power of two of their own that puts the largest at 2^13 .. 2^14, so fp16's range is no
+// question of the queries' size; the five partial products of a score meet in fp32 with their scales.  Probabilities are 2^kLift times
+// those of the row's reference, which moves when a score exceeds it by kSlack (log2): at most 2^15, so fp16 holds them, and its last bit is
+// 2^-31 of the largest.  bf16 pages multiply as bf16, exact, against two terms of both (2^-16), as the core over one sequence's cache
+// does.
+#include <algorithm>
+#include <type_traits>
+
+#include "mla_q4.h"
+
+namespace k3 {
+namespace {
+
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4_t *lds_s4;
+
+constexpr int kLat = 512, kRot = 64;
+constexpr int kSteps = (kLat + kRot) / 32;      // 18 steps of 32 columns of a score
+constexpr int kParts = 5;                       // scales of a row: four quarters of 128 columns, the rotary columns
+constexpr int kFrag = 1024;                     // bytes of an operand of 16 rows and 32 columns: 64 lanes x 16
+constexpr float kLiftP = 7.f, kSlackP = 8.f;
+
+// ------------------------------------------------------------------ items
+// Rows in groups of 16: group g of sequence b holds its rows 16 g .. of t H + h.  A block takes GT groups: of one sequence over a range of
+// its own positions, or any GT neighbours over a range of the prefix.
+struct Item {
+    int seq;            // the sequence, or -1: the prefix
+    int tile;           // the first group is GT tile (of the sequence, or of all)
+    int begin, end;     // positions
+};
+struct Head {           // of the list
+    int used;           // items
+    int ranges;         // of the prefix: its items are range r of tile i at r tiles + i
+};
+struct Lists {
+    const int32_t *lengths, *counts;
+    Head *head;
+    int2 *seq;          // [B]: first item, ranges of each of its tiles
+    Item *item;
+    int B, T, t0, Tall, cap, prefix;        // prefix: positions
+    int tiles, ptiles;  // of a sequence, of the prefix
+    int most;           // items there is room for
+    int turns;          // items a CU may have
+};
+
+// what query t (of its sequence's first n = counts[b]) sees
+__device__ __forceinline__ int sees_of(const Lists &a, int b, int t) {
+    const int len = min(max(a.lengths[b], 0), a.cap), n = a.counts ? min(max(a.counts[b], 0), a.Tall) : a.Tall;
+    return q4_sees(t, n, len);
+}
+// .. the last query of the pass
+__device__ __forceinline__ int sees_last(const Lists &a, int b) {
+    const int n = a.counts ? min(max(a.counts[b], 0), a.Tall) : a.Tall, t = min(a.t0 + a.T, n) - 1;
+    return t < a.t0 ? 0 : sees_of(a, b, t);
+}
+
+constexpr int kSearched = 1024;         // sequences up to which the ranges' length is searched for
+constexpr int kCandidates = 64;
+constexpr int kRound = 32;              // positions of a round of the attention
+
+// By one block of 256 threads.  Ranges are all of one length, the one of 64 candidates (one to two shares of one to four turns of
+// the card's 256 CUs) for which turns x (length + kStart) is least; kStart: what an item's start and end cost, in positions.
+constexpr int kStart = 192;
+__device__ __forceinline__ void list_items(const Lists &a, int *lds) {
+    int *const own = lds, *const sh = lds + kSearched;      // own: positions of a sequence's own
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int lp = 0;
+    float sum = 0.f;
+    for (int b = tid; b < a.B; b += 256) {
+        const int n = sees_last(a, b), o = max(n - a.prefix, 0);
+        if (b < kSearched) own[b] = o;
+        lp = max(lp, min(n, a.prefix));
+        sum += static_cast<float>(o);
+    }
+    lp = static_cast<int>(wave_max_all(static_cast<float>(lp)));        // (below 2^24: exact)
+    sum = wave_sum_all(sum);
+    if (lane == 0) sh[wave] = lp, sh[4 + wave] = __float_as_int(sum);
+    __syncthreads();
+    lp = max(max(sh[0], sh[1]), max(sh[2], sh[3]));
+    sum = (__int_as_float(sh[4]) + __int_as_float(sh[5])) + (__int_as_float(sh[6]) + __int_as_float(sh[7]));
+    const float work = static_cast<float>(a.ptiles) * lp + static_cast<float>(a.tiles) * sum;
+    int best = 1 << 24;                 // (all of a sequence: what always fits)
+    if (a.B <= kSearched) {
+        float least = INFINITY;
+        for (int i = wave; i < kCandidates; i += 4) {
+            const int turns = 1 + i / 16;
+            const float want = work / (256.f * turns) * (1.f + (i % 16) * (1.f / 16));
+            const int Ts = (static_cast<int>(fminf(want, 16777216.f)) / kRound + 1) * kRound;
+            const float inv = 1.0f / Ts;
+            int n = 0;
+            for (int b = lane; b < a.B; b += 64) {
+                const int o = own[b];
+                int c = static_cast<int>(o * inv);      // (within one of o / Ts: made exact)
+                c += (c + 1) * Ts <= o ? 1 : c * Ts > o ? -1 : 0;
+                n += c + (c * Ts < o);
+            }
+            const int all = static_cast<int>(wave_sum_all(static_cast<float>(n))) * a.tiles + (lp + Ts - 1) / Ts * a.ptiles;
+            const float cost = static_cast<float>((all + 255) / 256) * static_cast<float>(Ts + kStart);
+            if (turns <= a.turns && all <= a.most && cost < least) least = cost, best = Ts;
+        }
+        if (lane == 0) sh[8 + wave] = best, sh[12 + wave] = __float_as_int(least);
+        __syncthreads();
+        best = sh[8], least = __int_as_float(sh[12]);
+        for (int i = 1; i < 4; ++i)
+            if (__int_as_float(sh[12 + i]) < least) least = __int_as_float(sh[12 + i]), best = sh[8 + i];
+    }
+    const int Ts = best, ranges = (lp + Ts - 1) / Ts;
+    for (int j = tid; j < ranges * a.ptiles; j += 256) {
+        const int r = j / a.ptiles;
+        a.item[j] = Item{-1, j - r * a.ptiles, r * Ts, min((r + 1) * Ts, lp)};
+    }
+    // the sequences' items, 256 sequences at a time
+    int done = ranges * a.ptiles;
+    for (int b0 = 0; b0 < a.B; b0 += 256) {
+        const int b = b0 + tid;
+        const int o = b >= a.B ? 0 : b < kSearched ? own[b] : max(sees_last(a, b) - a.prefix, 0);
+        const int c = (o + Ts - 1) / Ts, n = c * a.tiles;
+        int at = n;
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) {
+            const int x = __shfl_up(at, k);
+            if (lane >= k) at += x;
+        }
+        __syncthreads();                // sh is free
+        if (lane == 63) sh[wave] = at;
+        __syncthreads();
+        at -= n;
+        for (int i = 0; i < wave; ++i) at += sh[i];
+        at += done;
+        if (b < a.B) a.seq[b] = make_int2(at, c);
+        for (int j = 0; j < n; ++j) {
+            const int r = j / a.tiles;
+            a.item[at + j] = Item{b, j - r * a.tiles, a.prefix + r * Ts, a.prefix + min((r + 1) * Ts, o)};
+        }
+        done += sh[0] + sh[1] + sh[2] + sh[3];
+    }
+    if (tid == 0) *a.head = Head{done, ranges};
+}
+
+// ------------------------------------------------------------------ qa
+struct QaArgs {
+    const void *q_nope, *q_rot;
+    int64_t n_b, n_t, n_h, r_b, r_t, r_h;       // strides in elements (batch, query, head)
+    const uint16_t *w_uk;                       // [H, nope, 512]
+    char *qop;                                  // [group][term][step] operands
+    float *scales;                              // [group][kParts][16]
+    int H, nope, M, T, t0, G;                   // M = B T queries of the pass; G groups a sequence
+    Lists lists;
+};
+
+constexpr int kWLd = 272;                       // LDS bytes per staged weight row (128 columns + 16 bytes)
+constexpr int kFLd = 132;                       // floats per staged result row
+
+__device__ __forceinline__ void three_terms(const float (&v)[8], u32x4 (&f)[3]) {
+    uint32_t t[3][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split3_near<false>(v[i], t[0][i], t[1][i], t[2][i]);
+#pragma unroll
+    for (int x = 0; x < 3; ++x)
+        f[x] = u32x4{hi16x2(t[x][0], t[x][1]), hi16x2(t[x][2], t[x][3]), hi16x2(t[x][4], t[x][5]), hi16x2(t[x][6], t[x][7])};
+}
+
+// 8 query values of a lane: slots 8 q4 .. +8 of a step of 32 hold n = 4 q4 + {0..3} and 16 + 4 q4 + {0..3}, the order in which
+// the transposed reads of the weights give theirs
+template <typename QT>
+struct Query {
+    typedef typename std::conditional<std::is_same<QT, float>::value, f32x4, u32x2>::type V;
+    V x[2];
+    __device__ __forceinline__ void load(const QT *q, int n, int nope, bool live) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[i] = live && n + 16 * i < nope ? *reinterpret_cast<const V *>(q + n + 16 * i) : V{};
+    }
+    __device__ __forceinline__ void terms(u32x4 (&f)[3]) const {
+        if constexpr (std::is_same<QT, float>::value) {
+            const float v[8] = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+            three_terms(v, f);
+        } else {
+            f[0] = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
+        }
+    }
+};
+
+// the operand terms of 8 neighbouring columns, scaled by s
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    return F16 ? q4_pack_f16(a, b) : q4_pack_bf16(a, b);
+}
+template <bool F16>
+__device__ __forceinline__ void unpack2(uint32_t p, float &a, float &b) {
+    if constexpr (F16) {
+        const f16x2 v = __builtin_bit_cast(f16x2, p);
+        a = static_cast<float>(v[0]), b = static_cast<float>(v[1]);
+    } else {
+        a = q4_lo(p), b = q4_hi(p);
+    }
+}
+template <bool F16, int NT>
+__device__ __forceinline__ void store_terms(float (&v)[8], float s, char *at) {     // at: the first term's operand, the lane's 16 bytes
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= s;
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+        u32x4 p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            p[i] = pack2<F16>(v[2 * i], v[2 * i + 1]);
+            if (x + 1 < NT) {
+                float a, b;
+                unpack2<F16>(p[i], a, b);
+                v[2 * i] -= a, v[2 * i + 1] -= b;
+            }
+        }
+        *reinterpret_cast<u32x4 *>(at + x * (kSteps * kFrag)) = p;
+    }
+}
+// the power of two that puts a magnitude (its bits) at 2^13 .. 2^14, and its inverse; 1 for zeros, infinities and NaNs
+__device__ __forceinline__ void scale_of(uint32_t top, float &s, float &inverse) {
+    const int e = top == 0u || top >= 0x7f800000u ? 13 : min(max(static_cast<int>(top >> 23) - 127, -100), 120);
+    s = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
+    inverse = __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
+}
+
+// grid (H, ceil(M / (16 MT)), 4 or 5): queries 16 MT y .. of head x, latent columns 128 z .. +128; z = 4: the list of items.
+// MT 1: few queries, a wave to 32 of the columns; MT 4: a wave to 16 of the queries.
+template <typename QT, bool F16, int NT, int MT>
+__global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float *const fs = reinterpret_cast<float *>(lds);                   // [16 MT][kFLd], after the products
+    constexpr int kTerms = std::is_same<QT, float>::value ? 3 : 1, kAhead = 4, kTiles = MT == 1 ? 2 : 8;    // column tiles of a wave
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
+    const int h = blockIdx.x, m0 = blockIdx.y * 16 * MT, quarter = blockIdx.z;
+    if (quarter == 4) {
+        if (h == 0 && m0 == 0) list_items(a.lists, reinterpret_cast<int *>(lds));
+        return;
+    }
+    const int steps = (a.nope + 31) >> 5;
+    const uint16_t *w = a.w_uk + static_cast<int64_t>(h) * a.nope * kLat + quarter * 128;
+    const int qt = MT == 1 ? 0 : wave, col = MT == 1 ? wave * 32 : 0, mine = m0 + 16 * qt + r16;    // the wave's queries and columns
+    const bool live = mine < a.M;
+    const int qb = live ? mine / a.T : 0, qt0 = live ? a.t0 + mine - qb * a.T : 0;
+    const QT *q = static_cast<const QT *>(a.q_nope) + qb * a.n_b + qt0 * a.n_t + h * a.n_h + 4 * q4;
+    Query<QT> ahead[kAhead];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) ahead[s].load(q, 32 * s, a.nope - 4 * q4, live);
+    for (int i0 = 0; i0 < 2 * steps; i0 += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = (i0 + u) * 256 + tid, n = i >> 4;
+            v[u] = n < a.nope ? *reinterpret_cast<const uint4 *>(w + static_cast<int64_t>(n) * kLat + (i & 15) * 8) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = (i0 + u) * 256 + tid, n = i >> 4;
+            if (n < 32 * steps) *reinterpret_cast<uint4 *>(lds + n * kWLd + (i & 15) * 16) = v[u];
+        }
+    }
+    f32x4 acc[kTiles];
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+    auto step = [&](int s, const Query<QT> &raw) __attribute__((always_inline)) {
+        const char *wr = lds + (32 * s + 4 * q4 + (r16 >> 2)) * kWLd + (r16 & 3) * 8 + col * 2;
+        u32x4 qf[3];
+        raw.terms(qf);
+#pragma unroll
+        for (int j0 = 0; j0 < kTiles; j0 += 2) {
+            u32x4 wf[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + (j0 + j) * 32));
+                const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + (j0 + j) * 32 + 16 * kWLd));
+                wf[j] = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+#pragma unroll
+            for (int k = kTerms - 1; k >= 0; --k)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[j0 + j] = q4_mfma_bf16(wf[j], qf[k], acc[j0 + j]);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+        if (s < steps) step(s, ahead[s]);
+    for (int s = kAhead; s < steps; ++s) {
+        Query<QT> raw;
+        raw.load(q, 32 * s, a.nope - 4 * q4, live);
+        step(s, raw);
+    }
+    __syncthreads();   // the weights are read
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) *reinterpret_cast<f32x4 *>(fs + (16 * qt + r16) * kFLd + col + j * 16 + 4 * q4) = acc[j];
+    __syncthreads();
+    // where row (query m, head h)'s operands are
+    auto place = [&](int m, int &r) -> int64_t {
+        const int b = m / a.T, row = (m - b * a.T) * a.H + h;
+        r = row & 15;
+        return static_cast<int64_t>(b) * a.G + (row >> 4);
+    };
+    if (tid < 64 * MT) {                // four threads to a query, a step of 32 columns each
+        const int i = tid >> 2, k = tid & 3, m = m0 + i;
+        float v[4][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(fs + i * kFLd + k * 32 + 4 * j);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[j >> 1][(j & 1) * 4 + y] = x[y], top = max(top, __float_as_uint(x[y]) & 0x7fffffffu);
+        }
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
+        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
+        if (m < a.M) {
+            float s, inverse;
+            scale_of(top, s, inverse);
+            int r;
+            const int64_t g = place(m, r);
+            char *const at = a.qop + (g * (NT * kSteps) + quarter * 4 + k) * kFrag + r * 16;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) store_terms<F16, NT>(v[c], s, at + c * 256);
+            if (k == 0) a.scales[(g * kParts + quarter) * 16 + r] = inverse;
+        }
+    }
+    if (quarter != 0) return;
+    // rotary columns 8 c .. +8 of a query, eight threads a query
+    for (int j = tid; j < 128 * MT; j += 256) {
+        const int i = j >> 3, m = m0 + i, c = j & 7;
+        float v[8];
+        uint32_t top = 0;
+        const int b = min(m, a.M - 1) / a.T, t = min(m, a.M - 1) - b * a.T;
+        const QT *qr = static_cast<const QT *>(a.q_rot) + b * a.r_b + (a.t0 + t) * a.r_t + h * a.r_h + c * 8;
+        if constexpr (std::is_same<QT, float>::value) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(qr), y = *reinterpret_cast<const f32x4 *>(qr + 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = x[k], v[4 + k] = y[k];
+        } else {
+            const u32x2 x = *reinterpret_cast<const u32x2 *>(qr), y = *reinterpret_cast<const u32x2 *>(qr + 4);
+            const uint32_t p[4] = {x.x, x.y, y.x, y.y};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[2 * k] = q4_lo(p[k]), v[2 * k + 1] = q4_hi(p[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+#pragma unroll
+        for (int k = 1; k < 8; k <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), k)));
+        if (m >= a.M) continue;
+        float s, inverse;
+        scale_of(top, s, inverse);
+        int r;
+        const int64_t g = place(m, r);
+        store_terms<F16, NT>(v, s, a.qop + (g * (NT * kSteps) + 16 + (c >> 2)) * kFrag + ((c & 3) * 16 + r) * 16);
+        if (c == 0) a.scales[(g * kParts + 4) * 16 + r] = inverse;
+    }
+}
+
+// ------------------------------------------------------------------ attend
+struct AttendArgs {
+    const char *qop;
+    const float *scales;
+    const char *lat, *rot;
+    int64_t lat_page, rot_page;                 // bytes
+    uint32_t lat_row, rot_row;
+    const int32_t *table, *prefix;
+    int64_t table_row;
+    int pages, shift;
+    Lists lists;
+    float *part;                                // [item][Mrec][512]
+    float2 *ml;                                 // [item][Mrec]
+    int H, G, groups, Mrec;                     // groups: of all sequences
+    float c;                                    // scale * log2(e)
+};
+
+constexpr int kLatLd = 1056;                    // LDS bytes of a staged latent row: 1024 + 32
+constexpr int kSlotBytes = kRound * (kLatLd + 128);
+constexpr int kSlots = 4;
+constexpr int kPBytes = 4 * kFrag;              // probabilities of 64 (row, term)s and a round
+constexpr int attend_lds() { return kSlots * kSlotBytes + 2 * kPBytes; }
+
+template <bool F16>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return F16 ? q4_mfma_f16(a, b, c) : q4_mfma_bf16(a, b, c);
+}
+
+// Infinities and NaNs of a pair to zero.
+template <bool F16>
+__device__ __forceinline__ uint32_t finite2(uint32_t p) {
+    constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
+    if ((p & e) == e) p &= 0xffff0000u;
+    if ((p & (e << 16)) == (e << 16)) p &= 0xffffu;
+    return p;
+}
+
+// An item a block: eight waves, two to a SIMD.  Rounds of 32 positions are staged in LDS as they lie in the pages (latent rows 1024
+// bytes of 1056, rotary rows 128 with the 16-byte columns of row r at c ^ (r & 7)).
+//   score waves (0 .. 3): S^T[position][row] of 16 (row, term)s each; the queries' operands stay in registers.  A lane (row r16, q4) has positions
+//           4 q4 .. +4 and 16 + 4 q4 .. +4, just what it holds as an operand of the second product.
+//   context waves (4 .. 7): ctx^T[column][row] += rows^T P^T, 128 columns each, from transposed reads of the staged rows.
+// GT = 4 / NT groups of 16 rows: with two terms the probabilities' second terms are rows of their own for the context waves, and the context
+// is their sum.
+template <bool F16, int NT>
+__global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
+    constexpr int GT = 4 / NT, kRows = 16 * GT;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int limits[64];
+    __shared__ float xf[2][64];                 // rescale factors [parity][16 x group + row]
+    char *const pbuf = lds + kSlots * kSlotBytes;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, q4 = lane >> 4;
+    // blocks b % 8 share an XCD and its L2: neighbours in the list, which read the same positions, go to one
+    const Head head = *a.lists.head;
+    const int used = __builtin_amdgcn_readfirstlane(head.used), each = (used + 7) >> 3;
+    const int at = static_cast<int>(blockIdx.x & 7) * each + static_cast<int>(blockIdx.x >> 3);
+    if (static_cast<int>(blockIdx.x >> 3) >= each || at >= used) return;
+    const Item it = a.lists.item[at];
+    const int seq = __builtin_amdgcn_readfirstlane(it.seq), tile = __builtin_amdgcn_readfirstlane(it.tile);
+    const int t_begin = __builtin_amdgcn_readfirstlane(it.begin), end = __builtin_amdgcn_readfirstlane(it.end);
+    // ---- what the rows see
+    if (tid < kRows) {
+        const int g = tile * GT + (tid >> 4);
+        const int b = seq >= 0 ? seq : g / a.G, row = (g - (seq >= 0 ? 0 : b * a.G)) * 16 + (tid & 15), t = row / a.H;
+        const bool there = b < a.lists.B && t < a.lists.T && (seq < 0 || g < a.G);
+        limits[tid] = there ? min(sees_of(a.lists, b, a.lists.t0 + t), end) : 0;
+    }
+    __syncthreads();
+    const int mine = lane < kRows ? limits[lane] : 0;
+    const int t_end = static_cast<int>(wave_max_all(static_cast<float>(mine)));
+    const int t_all = -static_cast<int>(wave_max_all(-static_cast<float>(mine > t_begin ? mine : 1 << 24)));     // what every row sees (of those that see any)
+    float2 *const ml = a.ml + static_cast<int64_t>(at) * a.Mrec;
+    if (t_end <= t_begin) {
+        if (tid < a.Mrec) ml[tid] = make_float2(-INFINITY, 0.f);
+        return;
+    }
+    const int nr = (t_end - t_begin + kRound - 1) / kRound;
+    const int32_t *const pages = seq < 0 ? a.prefix : a.table + seq * a.table_row;
+    // the pool's page of a round (a range and a round begin where 32 positions of one page do), -1: none
+    auto page_of = [&](int rd) -> int {
+        const int pos = t_begin + rd * kRound;
+        const int p = rd < nr ? pages[pos >> a.shift] : -1;
+        return p >= 0 && p < a.pages ? p : -1;
+    };
+
+    if (wave < 4) {
+        // ================= score waves
+        const int grp = wave % GT;
+        const int gidx = min((seq >= 0 ? seq * a.G : 0) + tile * GT + grp, a.groups - 1);
+        const char *qp = a.qop + static_cast<int64_t>(gidx) * (NT * kSteps * kFrag) + lane * 16;
+        u32x4 q[NT][kSteps];
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) q[x][k] = *reinterpret_cast<const u32x4 *>(qp + (x * kSteps + k) * kFrag);
+        float fac[kParts];
+#pragma unroll
+        for (int j = 0; j < kParts; ++j) fac[j] = a.scales[(static_cast<int64_t>(gidx) * kParts + j) * 16 + r16] * a.c;
+        const int limit = limits[grp * 16 + r16];
+        float ref = -INFINITY, l_run = 0.f;
+        for (int rd = 0; rd < nr; ++rd) {
+            __syncthreads();                    // staged
+            const char *slot = lds;
+            f32x4 acc[2][kParts];
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int j = 0; j < kParts; ++j) acc[p][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const int row = p * 16 + r16;
+                    const char *src = k < 16 ? slot + row * kLatLd + k * 64 + q4 * 16
+                                             : slot + kRound * kLatLd + row * 128 + ((((k - 16) * 4 + q4) ^ (row & 7)) * 16);
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(src);
+#pragma unroll
+                    for (int y = 0; y < NT; ++y) acc[p][k / 4] = mfma<F16>(x, q[y][k], acc[p][k / 4]);
+                }
+            if (wave < GT) {
+                const int base = t_begin + rd * kRound + 4 * q4;
+                const bool ok = page_of(rd) >= 0, mixed = !ok || t_begin + (rd + 1) * kRound > t_all;
+                float s[8], mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int p = i >> 2, v = i & 3;
+                    float x = acc[p][0][v] * fac[0];
+#pragma unroll
+                    for (int j = 1; j < kParts; ++j) x = fmaf(acc[p][j][v], fac[j], x);
+                    // (where values are cleaned for the sake of rows that do not see them, an infinite score has to make its row NaN by itself)
+                    if (mixed && !(fabsf(x) < INFINITY)) x = NAN;
+                    s[i] = ok && base + 16 * p + v < limit ? x : -INFINITY;
+                    mx = fmaxf(mx, s[i]);
+                }
+                mx = q4_rows_max(mx);
+                float f = 1.f;
+                if (__any(mx > ref + kSlackP)) {
+                    if (mx > ref + kSlackP) {
+                        f = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - mx);
+                        l_run *= f;
+                        ref = mx;
+                    }
+                }
+                const float from = ref == -INFINITY ? 0.f : ref - kLiftP;
+                float pr[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(s[i] - from), l_run += pr[i];
+                char *const to = pbuf + grp * NT * kFrag + lane * 16;
+#pragma unroll
+                for (int y = 0; y < NT; ++y) {
+                    u32x4 o;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[i] = pack2<F16>(pr[2 * i], pr[2 * i + 1]);
+                        if (y + 1 < NT) {
+                            float u, w;
+                            unpack2<F16>(o[i], u, w);
+                            pr[2 * i] -= u, pr[2 * i + 1] -= w;
+                        }
+                    }
+                    *reinterpret_cast<u32x4 *>(to + y * kFrag) = o;
+                }
+                if (q4 == 0) xf[0][grp * 16 + r16] = f;
+            }
+            __syncthreads();                    // probabilities written
+            __syncthreads();                    // all is read
+        }
+        l_run = q4_rows_sum(l_run);
+        if (wave < GT && q4 == 0 && grp * 16 + r16 < a.Mrec) ml[grp * 16 + r16] = make_float2(ref, l_run);
+    } else {
+        // ================= context waves
+        const int cw = wave - 4, st = tid - 256;
+        f32x4 acc[8][4];                        // [16 columns][16 (row, term)s]
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) acc[n][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int rd = 0; rd < nr; ++rd) {
+            const int page = page_of(rd), off = (t_begin + rd * kRound) & ((1 << a.shift) - 1), rows = t_end - t_begin - rd * kRound;
+            const char *lat = a.lat + page * a.lat_page + static_cast<int64_t>(off) * a.lat_row;
+            const char *rot = a.rot + page * a.rot_page + static_cast<int64_t>(off) * a.rot_row;
+            for (int i = 0; i < 8; ++i) {
+                const int row = i * 4 + (st >> 6), c = st & 63;
+                const u32x4 x = page >= 0 && row < rows ? *reinterpret_cast<const u32x4 *>(lat + static_cast<int64_t>(row) * a.lat_row + c * 16) : u32x4{0, 0, 0, 0};
+                *reinterpret_cast<u32x4 *>(lds + row * kLatLd + c * 16) = x;
+            }
+            {
+                const int row = st >> 3, c = st & 7;
+                const u32x4 x = page >= 0 && row < rows ? *reinterpret_cast<const u32x4 *>(rot + static_cast<int64_t>(row) * a.rot_row + c * 16) : u32x4{0, 0, 0, 0};
+                *reinterpret_cast<u32x4 *>(lds + kRound * kLatLd + row * 128 + (c ^ (row & 7)) * 16) = x;
+            }
+            __syncthreads();                    // staged
+            __syncthreads();                    // probabilities written
+            if (page < 0 || t_begin + (rd + 1) * kRound > t_all) {
+                // some row does not see all of this round: what it does not see must not reach it, not even as 0 x infinity
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    u32x4 *const x = reinterpret_cast<u32x4 *>(lds + (4 * i + q4) * kLatLd + cw * 256 + r16 * 16);
+                    u32x4 v = *x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = finite2<F16>(v[j]);
+                    *x = v;
+                }
+            }
+            u32x4 p[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                p[g] = *reinterpret_cast<const u32x4 *>(pbuf + g * kFrag + lane * 16);
+                const float f = xf[0][g / NT * 16 + r16];
+                if (__any(f != 1.f)) {
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) acc[n][g] *= f;
+                }
+            }
+            const char *src = lds + (4 * q4 + (r16 >> 2)) * kLatLd + cw * 256 + (r16 & 3) * 8;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32));
+                const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32 + 16 * kLatLd));
+                const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int g = 0; g < 4; ++g) acc[n][g] = mfma<F16>(v, p[g], acc[n][g]);
+            }
+            __syncthreads();                    // all is read
+        }
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+            const int row = g * 16 + r16;
+            if (row >= a.Mrec) continue;
+            float *to = a.part + (static_cast<int64_t>(at) * a.Mrec + row) * kLat + cw * 128 + 4 * q4;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                f32x4 o = acc[n][g * NT];
+                if constexpr (NT == 2) o += acc[n][g * NT + 1];
+                *reinterpret_cast<f32x4 *>(to + n * 16) = o;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ uv
+struct UvArgs {
+    const float *part;
+    const float2 *ml;
+    const Head *head;
+    const int2 *seq;
+    const uint16_t *w_uv;       // [H, V, 512]
+    void *out;                  // [B, Tall, H, V]
+    const float *gate;          // the same, or null
+    int H, V, M, T, t0, Tall, G, GT, tiles, ptiles, Mrec, out_bf16;
+};
+
+constexpr int kCLd = 1040;      // LDS bytes of a context row's term: 1024 + 16
+
+// grid (H, ceil(M / PER), Z): PER queries of head x, the z-th part of the V / 16 tiles of output columns.  256 / PER threads join a query's
+// records, sixteen to a record (32 columns each), 16 / PER records side by side; the sums meet in LDS and are left there as TERMS bf16 terms.  Then
+// a wave takes output tiles, its rows of W_UV as they lie.
+template <int TERMS, int PER>
+__global__ __launch_bounds__(256) void uv_kernel(UvArgs a) {
+    static_assert(PER == 1 || PER >= 4, "a query's threads are the block, whose one query is there, or within a wave");
+    constexpr int kSide = 16 / PER;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float *const sums = reinterpret_cast<float *>(lds);         // [PER][kSide][512]
+    char *const ctx = lds + 16 * kLat * 4;                      // [TERMS][16][kCLd]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
+    const int h = blockIdx.x, m0 = blockIdx.y * PER;
+    {
+        const int i = tid / (256 / PER), side = tid / 16 % kSide, c = tid & 15, m = m0 + i;
+        f32x4 s[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (m < a.M) {
+            const int b = m / a.T, row = (m - b * a.T) * a.H + h, g = row >> 4, pg = b * a.G + g;
+            const int2 mine = a.seq[b];
+            const int np = a.head->ranges, n = np + mine.y;
+            // record k of the row: ranges of the prefix, then its own
+            auto record = [&](int k) -> int64_t {
+                const int64_t item = k < np ? static_cast<int64_t>(k) * a.ptiles + pg / a.GT : mine.x + static_cast<int64_t>(k - np) * a.tiles + g / a.GT;
+                return item * a.Mrec + (k < np ? pg % a.GT : g % a.GT) * 16 + (row & 15);
+            };
+            float mx = -INFINITY, l = 0.f;
+            for (int k = tid % (256 / PER); k < n; k += 256 / PER) mx = fmaxf(mx, a.ml[record(k)].x);
+            // (over the query's threads, within a wave here and over the block's waves below)
+#pragma unroll
+            for (int o = 1; o < (256 / PER < 64 ? 256 / PER : 64); o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+            if constexpr (PER == 1) {
+                if (lane == 0) sums[wave] = mx;
+                __syncthreads();
+                mx = fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3]));
+                __syncthreads();
+            }
+            for (int k = side; k < n; k += kSide) {
+                const int64_t at = record(k);
+                const float2 v = a.ml[at];
+                if (v.y == 0.f) continue;       // (it sees nothing there, and what is written there does not matter)
+                const float w = __builtin_amdgcn_exp2f(v.x - mx);
+                l = fmaf(w, v.y, l);
+                const float *from = a.part + at * kLat + 4 * c;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) s[u] += w * *reinterpret_cast<const f32x4 *>(from + 64 * u);
+            }
+            // l: the same in a record's sixteen threads; over the records side by side
+            float all = l;
+            if constexpr (kSide > 1) {
+#pragma unroll
+                for (int o = 16; o < (256 / PER < 64 ? 256 / PER : 64); o <<= 1) all += __shfl_xor(all, o);
+                if constexpr (PER == 1) {
+                    if (lane == 0) sums[wave] = all;
+                    __syncthreads();
+                    all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                    __syncthreads();
+                }
+            }
+            const float inv = all == 0.f ? 0.f : 1.0f / all;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s[u] *= inv;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) *reinterpret_cast<f32x4 *>(sums + (i * kSide + side) * kLat + 4 * c + 64 * u) = s[u];
+    }
+    __syncthreads();
+    for (int j = tid; j < PER * 128; j += 256) {
+        const int i = j >> 7, c = j & 127;
+        f32x4 x = *reinterpret_cast<const f32x4 *>(sums + i * kSide * kLat + 4 * c);
+#pragma unroll
+        for (int k = 1; k < kSide; ++k) x += *reinterpret_cast<const f32x4 *>(sums + (i * kSide + k) * kLat + 4 * c);
+#pragma unroll
+        for (int y = 0; y < TERMS; ++y) {
+            const u32x2 p = {q4_pack_bf16(x[0], x[1]), q4_pack_bf16(x[2], x[3])};
+            *reinterpret_cast<u32x2 *>(ctx + (y * 16 + i) * kCLd + c * 8) = p;
+            x -= f32x4{q4_lo(p.x), q4_hi(p.x), q4_lo(p.y), q4_hi(p.y)};
+        }
+    }
+    __syncthreads();
+    const int vtiles = (a.V + 15) / 16, per_z = (vtiles + gridDim.z - 1) / gridDim.z, v_last = min(vtiles, (static_cast<int>(blockIdx.z) + 1) * per_z);
+    const auto rw = make_rsrc(a.w_uv + static_cast<int64_t>(h) * a.V * kLat, static_cast<uint32_t>(a.V) * (2 * kLat));
+    for (int vt = blockIdx.z * per_z + wave; vt < v_last; vt += 4) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        u32x4 w[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k)            // (rows past the head's last are outside and load zeros)
+            w[k] = __builtin_bit_cast(u32x4, buf_load16(rw, static_cast<uint32_t>(vt * 16 + r16) * (2 * kLat) + k * 64 + q4 * 16));
+#pragma unroll
+        for (int y = TERMS - 1; y >= 0; --y)
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                o = q4_mfma_bf16(w[k], *reinterpret_cast<const u32x4 *>(ctx + (y * 16 + r16 % PER) * kCLd + k * 64 + q4 * 16), o);
+        const int m = m0 + r16, v = vt * 16 + 4 * q4;
+        if (r16 < PER && m < a.M && v < a.V) {
+            const int b = m / a.T, t = a.t0 + m - b * a.T;
+            const int64_t to = ((static_cast<int64_t>(b) * a.Tall + t) * a.H + h) * a.V + v;
+            if (a.gate) {
+                const f32x4 g = *reinterpret_cast<const f32x4 *>(a.gate + to);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = o[i] / (1.0f + expf(-g[i]));
+            }
+            if (a.out_bf16)
+                *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + to) = u32x2{q4_pack_bf16(o[0], o[1]), q4_pack_bf16(o[2], o[3])};
+            else
+                *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + to) = o;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+constexpr int64_t kPassRows = 1 << 16;      // rows (heads x queries, all sequences) of one pass over the queries
+
+struct Plan {
+    int NT, GT, T, G, tiles, ptiles, Mrec, most, turns;     // T: queries of a sequence in a pass
+    int64_t groups, qop, scales, part, ml, head, seq, item, total;
+};
+
+// What the launches are cut into; a function of its arguments alone.
+Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t max_length, int64_t prefix, int cache_dtype, int out_dtype) {
+    Plan p{};
+    p.NT = cache_dtype == K3_F16 && out_dtype == K3_BF16 ? 1 : 2;
+    p.GT = 4 / p.NT;
+    p.T = static_cast<int>(std::max<int64_t>(1, std::min(T, kPassRows / (B * H))));
+    p.G = static_cast<int>(cdiv(p.T * H, 16));
+    p.tiles = static_cast<int>(cdiv(p.G, p.GT));
+    p.groups = B * p.G;
+    p.ptiles = prefix > 0 ? static_cast<int>(cdiv(p.groups, p.GT)) : 0;
+    p.Mrec = 16 * static_cast<int>(std::min<int64_t>(p.GT, prefix > 0 ? p.groups : p.G));
+    const int64_t base = B * p.tiles + p.ptiles;
+    const int64_t positions = p.ptiles * std::min(prefix, max_length) + B * p.tiles * std::max<int64_t>(max_length - prefix, 0);
+    p.turns = static_cast<int>(std::min<int64_t>(4, std::max<int64_t>(1, positions / (256 * 1024))));
+    p.most = static_cast<int>(base + std::min<int64_t>(256 * p.turns, positions / kRound + 1));
+    auto up = [](int64_t v) { return (v + 255) & ~int64_t(255); };
+    int64_t o = 0;
+    p.qop = o, o += up(p.groups * p.NT * kSteps * kFrag);
+    p.scales = o, o += up(p.groups * kParts * 16 * 4);
+    p.ml = o, o += up(static_cast<int64_t>(p.most) * p.Mrec * 8);
+    p.part = o, o += up(static_cast<int64_t>(p.most) * p.Mrec * kLat * 4);
+    p.head = o, o += 256;
+    p.seq = o, o += up(B * 8);
+    p.item = o, o += up(static_cast<int64_t>(p.most) * static_cast<int64_t>(sizeof(Item)));
+    p.total = o;
+    return p;
+}
+
+template <typename QT, bool F16, int NT, int MT>
+int launch_qa_of(const QaArgs &a, hipStream_t st) {
+    const int bytes = std::max({((a.nope + 31) / 32) * 32 * kWLd, 16 * MT * kFLd * 4, (kSearched + 64) * 4});
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(qa_kernel<QT, F16, NT, MT>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, 256 * kWLd);
+    const int rc = check_hip(attr, "mla paged: query LDS size");
+    if (rc) return rc;
+    qa_kernel<QT, F16, NT, MT><<<dim3(static_cast<unsigned>(a.H), static_cast<unsigned>(cdiv(a.M, 16 * MT)), 5), 256, bytes, st>>>(a);
+    return check_hip(hipGetLastError(), "mla paged: query launch");
+}
+template <typename QT>
+int launch_qa(const QaArgs &a, bool f16, int NT, hipStream_t st) {
+    if (!f16) return a.M > 32 ? launch_qa_of<QT, false, 2, 4>(a, st) : launch_qa_of<QT, false, 2, 1>(a, st);
+    if (NT == 1) return a.M > 32 ? launch_qa_of<QT, true, 1, 4>(a, st) : launch_qa_of<QT, true, 1, 1>(a, st);
+    return a.M > 32 ? launch_qa_of<QT, true, 2, 4>(a, st) : launch_qa_of<QT, true, 2, 1>(a, st);
+}
+
+template <bool F16, int NT>
+int launch_attend(const AttendArgs &a, int most, hipStream_t st) {
+    static const hipError_t attr =
+        hipFuncSetAttribute(reinterpret_cast<const void *>(attend_kernel<F16, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, attend_lds());
+    const int rc = check_hip(attr, "mla paged: attention LDS size");
+    if (rc) return rc;
+    attend_kernel<F16, NT><<<dim3(static_cast<unsigned>(cdiv(most, 8) * 8)), 512, attend_lds(), st>>>(a);
+    return check_hip(hipGetLastError(), "mla paged: attention launch");
+}
+
+template <int TERMS, int PER>
+int launch_uv_of(const UvArgs &a, unsigned parts, hipStream_t st) {
+    constexpr int bytes = 16 * kLat * 4 + TERMS * 16 * kCLd;
+    static const hipError_t attr =
+        hipFuncSetAttribute(reinterpret_cast<const void *>(uv_kernel<TERMS, PER>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const int rc = check_hip(attr, "mla paged: output LDS size");
+    if (rc) return rc;
+    uv_kernel<TERMS, PER><<<dim3(static_cast<unsigned>(a.H), static_cast<unsigned>(cdiv(a.M, PER)), parts), 256, bytes, st>>>(a);
+    return check_hip(hipGetLastError(), "mla paged: join and W_UV launch");
+}
+template <int TERMS>
+int launch_uv(const UvArgs &a, hipStream_t st) {
+    // the most queries to a block with which there are blocks for every CU
+    const unsigned parts = static_cast<unsigned>(std::min<int64_t>(cdiv(a.V, 64), std::max<int64_t>(1, 256 / (a.H * cdiv(a.M, 16)))));
+    if (a.M >= 16 || a.H * cdiv(a.M, 4) >= 512) return launch_uv_of<TERMS, 16>(a, parts, st);
+    if (a.M >= 4) return launch_uv_of<TERMS, 4>(a, parts, st);
+    return launch_uv_of<TERMS, 1>(a, parts, st);
+}
+
+}  // namespace
+}  // namespace k3
+
+using namespace k3;
+
+extern "C" int64_t k3_mla_paged_workspace_size(int64_t B, int64_t T, int64_t H, int64_t max_length, int64_t shared, int cache_dtype,
+                                               int out_dtype) {
+    if (B <= 0 || T <= 0 || H <= 0 || max_length < 0 || shared < 0) return 0;
+    return plan_of(B, T, H, max_length, shared, cache_dtype, out_dtype).total;
+}
+
+extern "C" int k3_mla_paged_attention(const void *q_nope, int64_t qn_batch, int64_t qn_token, int64_t qn_head, const void *q_rot,
+                                      int64_t qr_batch, int64_t qr_token, int64_t qr_head, int q_dtype, const void *w_uk,
+                                      const void *w_uv, const void *lat, int64_t lat_page, int64_t lat_row, const void *rot,
+                                      int64_t rot_page, int64_t rot_row, int cache_dtype, int64_t pages, int64_t page_size,
+                                      const int32_t *table, int64_t table_row, int64_t blocks, const int32_t *prefix,
+                                      int64_t prefix_pages, const int32_t *lengths, const int32_t *counts, int64_t max_length, int64_t B,
+                                      int64_t T, int64_t H, int64_t kv_lora_rank, int64_t rope_dim, int64_t nope_dim, int64_t v_dim,
+                                      float scale, const float *gate, void *out, int out_dtype, void *workspace, int64_t workspace_bytes,
+                                      void *stream) {
+    if (B == 0 || T == 0) return K3_OK;
+    if (!q_nope || !q_rot || !w_uk || !w_uv || !out || !workspace || !lengths || (pages > 0 && (!lat || !rot)) || (blocks > 0 && !table) ||
+        (prefix_pages > 0 && !prefix))
+        return set_error(K3_ERR_NULL, "mla paged: null pointer");
+    if (q_dtype != K3_F32 && q_dtype != K3_BF16) return set_error(K3_ERR_DTYPE, "mla paged: q_dtype %d", q_dtype);
+    if (out_dtype != K3_F32 && out_dtype != K3_BF16) return set_error(K3_ERR_DTYPE, "mla paged: out_dtype %d", out_dtype);
+    if (cache_dtype != K3_F16 && cache_dtype != K3_BF16) return set_error(K3_ERR_DTYPE, "mla paged: cache dtype %d", cache_dtype);
+    if (kv_lora_rank != kLat || rope_dim != kRot)
+        return set_error(K3_ERR_SHAPE, "mla paged: kv_lora_rank=%lld rope=%lld; the kernels take 512 and 64", (long long)kv_lora_rank,
+                         (long long)rope_dim);
+    if (nope_dim <= 0 || nope_dim > 256 || nope_dim % 8 || v_dim <= 0 || v_dim > 1024 || v_dim % 8)
+        return set_error(K3_ERR_SHAPE, "mla paged: nope=%lld must be a multiple of 8 up to 256 and v=%lld one up to 1024",
+                         (long long)nope_dim, (long long)v_dim);
+    if (page_size < kRound || page_size > (1 << 16) || (page_size & (page_size - 1)))
+        return set_error(K3_ERR_SHAPE, "mla paged: page_size=%lld must be a power of two, 32 to 65536", (long long)page_size);
+    if (B < 0 || B > 65535 || T < 0 || T > (1 << 24) || H <= 0 || H > 4096 || B * H > kPassRows || pages < 0 || pages >= (1ll << 31) || blocks < 0 ||
+        prefix_pages < 0 || max_length < 0 || max_length > (1 << 24) || blocks > (1 << 24) || prefix_pages > (1 << 24) || max_length > blocks * page_size)
+        return set_error(K3_ERR_SHAPE, "mla paged: B=%lld, T=%lld, H=%lld, %lld pages, max_length=%lld of %lld blocks or prefix of %lld pages out of range",
+                         (long long)B, (long long)T, (long long)H, (long long)pages, (long long)max_length, (long long)blocks, (long long)prefix_pages);
+    if (B > 1 && table_row < blocks) return set_error(K3_ERR_SHAPE, "mla paged: the table's rows overlap, %lld apart", (long long)table_row);
+    if (qn_batch % 4 || qn_token % 4 || qn_head % 4 || qr_batch % 4 || qr_token % 4 || qr_head % 4)
+        return set_error(K3_ERR_SHAPE, "mla paged: query strides must be multiples of 4 elements");
+    if (lat_row < kLat || rot_row < kRot || lat_row % 8 || rot_row % 8 || lat_page % 8 || rot_page % 8 || lat_row > (1 << 20) || rot_row > (1 << 20))
+        return set_error(K3_ERR_SHAPE, "mla paged: cache row pitches too small, too large or not multiples of 16 bytes");
+    if (!aligned16(q_nope) || !aligned16(q_rot) || !aligned16(w_uk) || !aligned16(w_uv) || !aligned16(out) || !aligned16(workspace) ||
+        !aligned16(lat) || !aligned16(rot) || (gate && !aligned16(gate)))
+        return set_error(K3_ERR_ALIGN, "mla paged: queries, weights, cache, output and workspace must be 16-byte aligned");
+    const Plan p = plan_of(B, T, H, max_length, prefix_pages * page_size, cache_dtype, out_dtype);
+    if (workspace_bytes < p.total)
+        return set_error(K3_ERR_WORKSPACE, "mla paged: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)p.total);
+    int shift = 0;
+    while ((1ll << shift) < page_size) ++shift;
+    auto st = static_cast<hipStream_t>(stream);
+    char *ws = static_cast<char *>(workspace);
+    const bool f16 = cache_dtype == K3_F16;
+    for (int64_t t0 = 0; t0 < T; t0 += p.T) {
+        // (the last pass may have fewer queries; it has the others' room)
+        const int Tp = static_cast<int>(std::min<int64_t>(p.T, T - t0)), G = static_cast<int>(cdiv(Tp * H, 16)), M = static_cast<int>(B * Tp);
+        const int tiles = static_cast<int>(cdiv(G, p.GT)), groups = static_cast<int>(B * G);
+        const int ptiles = prefix_pages > 0 ? static_cast<int>(cdiv(groups, p.GT)) : 0;
+        const Lists lists{lengths, counts, reinterpret_cast<Head *>(ws + p.head), reinterpret_cast<int2 *>(ws + p.seq),
+                          reinterpret_cast<Item *>(ws + p.item), static_cast<int>(B), Tp, static_cast<int>(t0), static_cast<int>(T),
+                          static_cast<int>(max_length), static_cast<int>(std::min<int64_t>(prefix_pages * page_size, 1 << 24)), tiles, ptiles, p.most, p.turns};
+        const QaArgs qa{q_nope, q_rot, qn_batch, qn_token, qn_head, qr_batch, qr_token, qr_head, static_cast<const uint16_t *>(w_uk),
+                        ws + p.qop, reinterpret_cast<float *>(ws + p.scales), static_cast<int>(H), static_cast<int>(nope_dim), M, Tp,
+                        static_cast<int>(t0), G, lists};
+        int rc = q_dtype == K3_BF16 ? launch_qa<uint16_t>(qa, f16, p.NT, st) : launch_qa<float>(qa, f16, p.NT, st);
+        if (rc) return rc;
+        AttendArgs a{};
+        a.qop = qa.qop, a.scales = qa.scales, a.lat = static_cast<const char *>(lat), a.rot = static_cast<const char *>(rot);
+        a.lat_page = 2 * lat_page, a.rot_page = 2 * rot_page;
+        a.lat_row = static_cast<uint32_t>(2 * lat_row), a.rot_row = static_cast<uint32_t>(2 * rot_row);
+        a.table = table, a.prefix = prefix, a.table_row = table_row, a.pages = static_cast<int>(pages), a.shift = shift;
+        a.lists = lists;
+        a.part = reinterpret_cast<float *>(ws + p.part), a.ml = reinterpret_cast<float2 *>(ws + p.ml);
+        a.H = static_cast<int>(H), a.G = G, a.groups = groups, a.Mrec = p.Mrec, a.c = scale * 1.4426950408889634f;
+        rc = !f16 ? launch_attend<false, 2>(a, p.most, st) : p.NT == 1 ? launch_attend<true, 1>(a, p.most, st) : launch_attend<true, 2>(a, p.most, st);
+        if (rc) return rc;
+        const UvArgs u{a.part, a.ml, lists.head, lists.seq, static_cast<const uint16_t *>(w_uv), out, gate, a.H, static_cast<int>(v_dim), M, Tp,
+                       static_cast<int>(t0), static_cast<int>(T), G, p.GT, tiles, ptiles, p.Mrec, out_dtype == K3_BF16};
+        rc = u.out_bf16 ? launch_uv<2>(u, st) : launch_uv<3>(u, st);
+        if (rc) return rc;
+    }
+    return K3_OK;
+}

@@ -18,7 +18,7 @@ LIB_PATH = Path(__file__).resolve().with_name("libk3hip.so")
 K3_OK, K3_ERR_SHAPE, K3_ERR_DTYPE, K3_ERR_ALIGN, K3_ERR_SCALE_RANGE = 0, 1, 2, 3, 4
 K3_ERR_WORKSPACE, K3_ERR_HIP, K3_ERR_NULL = 5, 6, 7
 
-K3_F32, K3_BF16 = 0, 1
+K3_F32, K3_BF16, K3_F16 = 0, 1, 2
 K3_ACT_SILU, K3_ACT_SITU = 0, 1
 K3_ROUTE_SOFTMAX, K3_ROUTE_SIGMOID_BIAS = 0, 1
 
@@ -57,6 +57,14 @@ SIGNATURES: dict[str, list] = {
     "k3_mla_step_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64],
     "k3_mla_step_decode": [_P, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _F32,
                            _F32, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P],
+    "k3_page_tables_workspace_size": [_I64],
+    "k3_page_tables": [_P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P],
+    "k3_mla_paged_append": [_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _F32, _P, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64,
+                            _I64, _I64, _I64, _I64, _I64, _P],
+    "k3_mla_paged_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I32, _I32],
+    "k3_mla_paged_attention": [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I32, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64,
+                               _I64, _P, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F32, _P,
+                               _P, _I32, _P, _I64, _P],
     "k3_mla_step_q4_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I32],
     "k3_mla_step_decode_q4": [_P, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _F32, _F32,
                               _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P],
@@ -112,6 +120,7 @@ _RESTYPE = {"k3_last_error": ctypes.c_char_p, "k3_version": ctypes.c_char_p,
             "k3_dense_workspace_size": ctypes.c_int64,
             "k3_mla_prefill_workspace_size": ctypes.c_int64,
             "k3_moe_grouped_workspace_size": ctypes.c_int64,
+            "k3_page_tables_workspace_size": ctypes.c_int64, "k3_mla_paged_workspace_size": ctypes.c_int64,
             "k3_moe_routed_workspace_size": ctypes.c_int64,
             "k3_moe_layer_multi_workspace_size": ctypes.c_int64,
             "k3_moe_latent_layer_multi_workspace_size": ctypes.c_int64}
