@@ -404,6 +404,19 @@ __device__ __forceinline__ uint32_t finite2(uint32_t p) {
     return p;
 }
 
+// 16 bytes a lane from offset `off` of a buffer straight into LDS, lane l's at to + 16 l; what lies outside the buffer arrives as zeros.  Not
+// tracked by the compiler (nor is m0, which nothing else here uses): a wave waits for its own loads (arrived) and meets the others at a barrier before anything is read.  (As an
+// instruction of the compiler's it made every read of LDS wait for all loads in flight.  No register is written, so none can be reused
+// under it; its operands are read as it issues.)
+__device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(to) : "memory");
+}
+// All but the last LEFT loads have arrived, LDS is written and read; then all waves of the block are here.
+template <int LEFT>
+__device__ __forceinline__ void arrived_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
 // An item a block: eight waves, two to a SIMD.  Rounds of 32 positions are staged in LDS as they lie in the pages (latent rows 1024
 // bytes of 1056, rotary rows 128 with the 16-byte columns of row r at c ^ (r & 7)).
 //   score waves (0 .. 3): S^T[position][row] of 16 (row, term)s each; the queries' operands stay in registers.  A lane (row r16, q4) has positions
@@ -445,14 +458,41 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         return;
     }
     const int nr = (t_end - t_begin + kRound - 1) / kRound;
-    const int32_t *const pages = seq < 0 ? a.prefix : a.table + seq * a.table_row;
-    // the pool's page of a round (a range and a round begin where 32 positions of one page do), -1: none
-    auto page_of = [&](int rd) -> int {
-        const int pos = t_begin + rd * kRound;
-        const int p = rd < nr ? pages[pos >> a.shift] : -1;
-        return p >= 0 && p < a.pages ? p : -1;
-    };
 
+    // ---- staging: round rd into slot rd % kSlots, by all waves: four latent rows each, the context waves eight rotary rows as well.
+    // A lane keeps the page of one of 64 rounds (a round lies in one page; -1: outside the pool, or no such round).
+    const int32_t *const pages = seq < 0 ? a.prefix : a.table + seq * a.table_row;
+    int mypage = -1;
+    auto look_up = [&](int first) __attribute__((always_inline)) {
+        const int rd = first + lane;
+        const int p = rd < nr ? pages[(t_begin + rd * kRound) >> a.shift] : -1;
+        mypage = p < a.pages ? p : -1;
+    };
+    auto page_of = [&](int rd) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(mypage, rd & 63); };
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds));
+    const int rrow = 8 * (wave & 3) + (lane >> 3);
+    const uint32_t lat_off = static_cast<uint32_t>(4 * wave) * a.lat_row + lane * 16u;
+    const uint32_t rot_off = static_cast<uint32_t>(rrow) * a.rot_row + ((lane & 7) ^ (rrow & 7)) * 16u;
+    auto rsrc_of = [&](const char *base, uint32_t bytes) __attribute__((always_inline)) {
+        const uint64_t at = reinterpret_cast<uint64_t>(base);
+        return u32x4{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xffffu, bytes, 0x00020000u};
+    };
+    auto stage = [&](int rd, int page, bool context) __attribute__((always_inline)) {
+        const int off = (t_begin + rd * kRound) & ((1 << a.shift) - 1), rows = page >= 0 ? min(t_end - t_begin - rd * kRound, kRound) : 0;
+        const uint32_t to = lds0 + (rd & (kSlots - 1)) * kSlotBytes;
+        const int64_t p = page >= 0 ? page : 0;
+        const u32x4 rl = rsrc_of(a.lat + p * a.lat_page + static_cast<int64_t>(off) * a.lat_row, rows > 0 ? (rows - 1) * a.lat_row + 1024u : 0u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_to_lds(rl, lat_off + i * a.lat_row, to + (4 * wave + i) * kLatLd);
+        if (context) {
+            const u32x4 rr = rsrc_of(a.rot + p * a.rot_page + static_cast<int64_t>(off) * a.rot_row, rows > 0 ? (rows - 1) * a.rot_row + 128u : 0u);
+            load_to_lds(rr, rot_off, to + kRound * kLatLd + (wave & 3) * 1024);
+        }
+    };
+    look_up(0);
+
+    // Iteration t = -1 .. nr - 1: round t + 3 is sent for, the score waves take round t + 1, the context waves round t; then round t + 2 is
+    // waited for.  A slot is written again three iterations after its scores, two after its context.
     if (wave < 4) {
         // ================= score waves
         const int grp = wave % GT;
@@ -468,28 +508,40 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         for (int j = 0; j < kParts; ++j) fac[j] = a.scales[(static_cast<int64_t>(gidx) * kParts + j) * 16 + r16] * a.c;
         const int limit = limits[grp * 16 + r16];
         float ref = -INFINITY, l_run = 0.f;
-        for (int rd = 0; rd < nr; ++rd) {
-            __syncthreads();                    // staged
-            const char *slot = lds;
-            f32x4 acc[2][kParts];
+        // (all of it is here before the first round is sent for: a wait for it in the loop would wait for the rounds in flight)
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
-                for (int j = 0; j < kParts; ++j) acc[p][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(q[x][k]));
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k)
+        for (int j = 0; j < kParts; ++j) asm volatile("" : "+v"(fac[j]));
+        stage(0, page_of(0), false);
+        stage(1, page_of(1), false);
+        arrived_barrier<4>();
+        for (int rd = 0; rd <= nr; ++rd) {
+            const bool ok = page_of(rd) >= 0;
+            if (((rd + 2) & 63) == 0) look_up(rd + 2);      // (rounds rd + 2 .. of the next 64: this round's page is taken)
+            stage(rd + 2, page_of(rd + 2), false);
+            if (rd < nr && wave < GT) {
+                const char *slot = lds + (rd & (kSlots - 1)) * kSlotBytes;
+                f32x4 acc[2][kParts];
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const int row = p * 16 + r16;
-                    const char *src = k < 16 ? slot + row * kLatLd + k * 64 + q4 * 16
-                                             : slot + kRound * kLatLd + row * 128 + ((((k - 16) * 4 + q4) ^ (row & 7)) * 16);
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(src);
+                for (int p = 0; p < 2; ++p)
 #pragma unroll
-                    for (int y = 0; y < NT; ++y) acc[p][k / 4] = mfma<F16>(x, q[y][k], acc[p][k / 4]);
-                }
-            if (wave < GT) {
+                    for (int j = 0; j < kParts; ++j) acc[p][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const int row = p * 16 + r16;
+                        const char *src = k < 16 ? slot + row * kLatLd + k * 64 + q4 * 16
+                                                 : slot + kRound * kLatLd + row * 128 + ((((k - 16) * 4 + q4) ^ (row & 7)) * 16);
+                        const u32x4 x = *reinterpret_cast<const u32x4 *>(src);
+#pragma unroll
+                        for (int y = 0; y < NT; ++y) acc[p][k / 4] = mfma<F16>(x, q[y][k], acc[p][k / 4]);
+                    }
                 const int base = t_begin + rd * kRound + 4 * q4;
-                const bool ok = page_of(rd) >= 0, mixed = !ok || t_begin + (rd + 1) * kRound > t_all;
+                const bool mixed = !ok || t_begin + (rd + 1) * kRound > t_all;
                 float s[8], mx = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -497,11 +549,18 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                     float x = acc[p][0][v] * fac[0];
 #pragma unroll
                     for (int j = 1; j < kParts; ++j) x = fmaf(acc[p][j][v], fac[j], x);
-                    // (where values are cleaned for the sake of rows that do not see them, an infinite score has to make its row NaN by itself)
-                    if (mixed && !(fabsf(x) < INFINITY)) x = NAN;
-                    s[i] = ok && base + 16 * p + v < limit ? x : -INFINITY;
-                    mx = fmaxf(mx, s[i]);
+                    s[i] = x;
                 }
+                if (mixed) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        // (where values are cleaned for the sake of rows that do not see them, an infinite score has to make its row NaN by itself)
+                        if (!(fabsf(s[i]) < INFINITY)) s[i] = NAN;
+                        s[i] = ok && base + 16 * (i >> 2) + (i & 3) < limit ? s[i] : -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i]);
                 mx = q4_rows_max(mx);
                 float f = 1.f;
                 if (__any(mx > ref + kSlackP)) {
@@ -515,7 +574,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 float pr[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(s[i] - from), l_run += pr[i];
-                char *const to = pbuf + grp * NT * kFrag + lane * 16;
+                char *const to = pbuf + (rd & 1) * kPBytes + grp * NT * kFrag + lane * 16;
 #pragma unroll
                 for (int y = 0; y < NT; ++y) {
                     u32x4 o;
@@ -530,68 +589,66 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                     }
                     *reinterpret_cast<u32x4 *>(to + y * kFrag) = o;
                 }
-                if (q4 == 0) xf[0][grp * 16 + r16] = f;
+                if (q4 == 0) xf[rd & 1][grp * 16 + r16] = f;
             }
-            __syncthreads();                    // probabilities written
-            __syncthreads();                    // all is read
+            arrived_barrier<4>();
         }
         l_run = q4_rows_sum(l_run);
-        if (wave < GT && q4 == 0 && grp * 16 + r16 < a.Mrec) ml[grp * 16 + r16] = make_float2(ref, l_run);
+        // (a row that sees nothing of the range was not masked where all others see all: its record counts for nothing)
+        if (wave < GT && q4 == 0 && grp * 16 + r16 < a.Mrec)
+            ml[grp * 16 + r16] = limit > t_begin ? make_float2(ref, l_run) : make_float2(-INFINITY, 0.f);
     } else {
         // ================= context waves
-        const int cw = wave - 4, st = tid - 256;
+        const int cw = wave - 4;
         f32x4 acc[8][4];                        // [16 columns][16 (row, term)s]
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int g = 0; g < 4; ++g) acc[n][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int rd = 0; rd < nr; ++rd) {
-            const int page = page_of(rd), off = (t_begin + rd * kRound) & ((1 << a.shift) - 1), rows = t_end - t_begin - rd * kRound;
-            const char *lat = a.lat + page * a.lat_page + static_cast<int64_t>(off) * a.lat_row;
-            const char *rot = a.rot + page * a.rot_page + static_cast<int64_t>(off) * a.rot_row;
-            for (int i = 0; i < 8; ++i) {
-                const int row = i * 4 + (st >> 6), c = st & 63;
-                const u32x4 x = page >= 0 && row < rows ? *reinterpret_cast<const u32x4 *>(lat + static_cast<int64_t>(row) * a.lat_row + c * 16) : u32x4{0, 0, 0, 0};
-                *reinterpret_cast<u32x4 *>(lds + row * kLatLd + c * 16) = x;
-            }
-            {
-                const int row = st >> 3, c = st & 7;
-                const u32x4 x = page >= 0 && row < rows ? *reinterpret_cast<const u32x4 *>(rot + static_cast<int64_t>(row) * a.rot_row + c * 16) : u32x4{0, 0, 0, 0};
-                *reinterpret_cast<u32x4 *>(lds + kRound * kLatLd + row * 128 + (c ^ (row & 7)) * 16) = x;
-            }
-            __syncthreads();                    // staged
-            __syncthreads();                    // probabilities written
-            if (page < 0 || t_begin + (rd + 1) * kRound > t_all) {
-                // some row does not see all of this round: what it does not see must not reach it, not even as 0 x infinity
+        stage(0, page_of(0), true);
+        stage(1, page_of(1), true);
+        arrived_barrier<5>();
+        int before = -1, now = page_of(0);      // the pages of rounds rd - 1 and rd
+        for (int rd = 0; rd <= nr; ++rd) {      // (as the score waves count: round rd - 1 is taken here)
+            const int after = page_of(rd + 1);
+            if (((rd + 2) & 63) == 0) look_up(rd + 2);
+            stage(rd + 2, page_of(rd + 2), true);
+            if (rd > 0) {
+                char *const slot = lds + ((rd - 1) & (kSlots - 1)) * kSlotBytes;
+                const char *const pb = pbuf + ((rd - 1) & 1) * kPBytes + lane * 16;
+                if (before < 0 || t_begin + rd * kRound > t_all) {
+                    // some row does not see all of this round: what it does not see must not reach it, not even as 0 x infinity
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    u32x4 *const x = reinterpret_cast<u32x4 *>(lds + (4 * i + q4) * kLatLd + cw * 256 + r16 * 16);
-                    u32x4 v = *x;
+                    for (int i = 0; i < 8; ++i) {
+                        u32x4 *const x = reinterpret_cast<u32x4 *>(slot + (4 * i + q4) * kLatLd + cw * 256 + r16 * 16);
+                        u32x4 v = *x;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = finite2<F16>(v[j]);
-                    *x = v;
+                        for (int j = 0; j < 4; ++j) v[j] = finite2<F16>(v[j]);
+                        *x = v;
+                    }
+                }
+                u32x4 p[4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    p[g] = *reinterpret_cast<const u32x4 *>(pb + g * kFrag);
+                    const float f = xf[(rd - 1) & 1][g / NT * 16 + r16];
+                    if (__any(f != 1.f)) {
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) acc[n][g] *= f;
+                    }
+                }
+                const char *src = slot + (4 * q4 + (r16 >> 2)) * kLatLd + cw * 256 + (r16 & 3) * 8;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32));
+                    const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32 + 16 * kLatLd));
+                    const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) acc[n][g] = mfma<F16>(v, p[g], acc[n][g]);
                 }
             }
-            u32x4 p[4];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                p[g] = *reinterpret_cast<const u32x4 *>(pbuf + g * kFrag + lane * 16);
-                const float f = xf[0][g / NT * 16 + r16];
-                if (__any(f != 1.f)) {
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) acc[n][g] *= f;
-                }
-            }
-            const char *src = lds + (4 * q4 + (r16 >> 2)) * kLatLd + cw * 256 + (r16 & 3) * 8;
-#pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32));
-                const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32 + 16 * kLatLd));
-                const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                for (int g = 0; g < 4; ++g) acc[n][g] = mfma<F16>(v, p[g], acc[n][g]);
-            }
-            __syncthreads();                    // all is read
+            before = now, now = after;
+            arrived_barrier<5>();
         }
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
@@ -606,6 +663,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
             }
         }
     }
+    arrived_barrier<0>();       // (nothing may arrive in LDS after the block has left it)
 }
 
 // ------------------------------------------------------------------ uv
