@@ -14,9 +14,10 @@
 //
 // Numerics.  fp16 pages multiply as fp16: 11 bits make one term of a query or probability enough for a bf16 result (off by 2^-11 at most, independent
 // errors below the result's own 2^-8) and two for fp32 (2^-22); bf16 terms would need two and three.  The absorbed query's 128 columns
-// of a quarter, and its rotary columns, are scaled by a power of two of their own that puts the largest at 2^13 .. 2^14, so fp16's range is no
-// question of the queries' size; the five partial products of a score meet in fp32 with their scales.  Probabilities are 2^kLift times
-// those of the row's reference, which moves when a score exceeds it by kSlack (log2): at most 2^15, so fp16 holds them, and its last bit is
+// of a quarter, and its rotary columns, are scaled by a power of two of their own that puts the largest at 2^13 .. 2^14 (a block of the query
+// launch has one of them), and all to the row's largest scale as attend takes them in, so fp16's range is no question of the queries' size: what
+// falls below fp16's last bit then is 2^-38 of the row's largest.  Probabilities are 2^kLift times
+// those of the row's reference, which moves when one would exceed 2^kTop: so fp16 holds them, and its last bit is
 // 2^-31 of the largest.  bf16 pages multiply as bf16, exact, against two terms of both (2^-16), as the core over one sequence's cache
 // does.
 #include <algorithm>
@@ -34,7 +35,7 @@ constexpr int kLat = 512, kRot = 64;
 constexpr int kSteps = (kLat + kRot) / 32;      // 18 steps of 32 columns of a score
 constexpr int kParts = 5;                       // scales of a row: four quarters of 128 columns, the rotary columns
 constexpr int kFrag = 1024;                     // bytes of an operand of 16 rows and 32 columns: 64 lanes x 16
-constexpr float kLiftP = 7.f, kSlackP = 8.f;
+constexpr float kLiftP = 7.f, kTop = 15.f;     // log2 of a probability at the row's reference, and of the largest there may be
 
 // ------------------------------------------------------------------ items
 // Rows in groups of 16: group g of sequence b holds its rows 16 g .. of t H + h.  A block takes GT groups: of one sequence over a range of
@@ -229,11 +230,17 @@ __device__ __forceinline__ void store_terms(float (&v)[8], float s, char *at) { 
         *reinterpret_cast<u32x4 *>(at + x * (kSteps * kFrag)) = p;
     }
 }
-// the power of two that puts a magnitude (its bits) at 2^13 .. 2^14, and its inverse; 1 for zeros, infinities and NaNs
+// the power of two that puts a magnitude (its bits) at 2^13 .. 2^14, and its inverse; 1 for infinities and NaNs, and for zeros, whose
+// inverse is given as 0: they have no part in the row's scale
+template <bool F16>
 __device__ __forceinline__ void scale_of(uint32_t top, float &s, float &inverse) {
+    if constexpr (!F16) {               // (bf16 terms need none)
+        s = inverse = 1.f;
+        return;
+    }
     const int e = top == 0u || top >= 0x7f800000u ? 13 : min(max(static_cast<int>(top >> 23) - 127, -100), 120);
     s = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
-    inverse = __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
+    inverse = top == 0u ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
 }
 
 // grid (H, ceil(M / (16 MT)), 4 or 5): queries 16 MT y .. of head x, latent columns 128 z .. +128; z = 4: the list of items.
@@ -326,7 +333,7 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
         top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
         if (m < a.M) {
             float s, inverse;
-            scale_of(top, s, inverse);
+            scale_of<F16>(top, s, inverse);
             int r;
             const int64_t g = place(m, r);
             char *const at = a.qop + (g * (NT * kSteps) + quarter * 4 + k) * kFrag + r * 16;
@@ -359,7 +366,7 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
         for (int k = 1; k < 8; k <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), k)));
         if (m >= a.M) continue;
         float s, inverse;
-        scale_of(top, s, inverse);
+        scale_of<F16>(top, s, inverse);
         int r;
         const int64_t g = place(m, r);
         store_terms<F16, NT>(v, s, a.qop + (g * (NT * kSteps) + 16 + (c >> 2)) * kFrag + ((c & 3) * 16 + r) * 16);
@@ -412,24 +419,40 @@ __device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t off, uint32_t t
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(to) : "memory");
 }
 // All but the last LEFT loads have arrived, LDS is written and read; then all waves of the block are here.
-template <int LEFT>
+template <int LEFT, bool LDS = true>
 __device__ __forceinline__ void arrived_barrier() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+    if constexpr (LDS)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
+
+// the largest of three, a NaN aside (fmaxf makes its operands canonical first)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
+__device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // An item a block: eight waves, two to a SIMD.  Rounds of 32 positions are staged in LDS as they lie in the pages (latent rows 1024
 // bytes of 1056, rotary rows 128 with the 16-byte columns of row r at c ^ (r & 7)).
-//   score waves (0 .. 3): S^T[position][row] of 16 (row, term)s each; the queries' operands stay in registers.  A lane (row r16, q4) has positions
-//           4 q4 .. +4 and 16 + 4 q4 .. +4, just what it holds as an operand of the second product.
+//   score waves (0 .. 3): S^T[position][row], 16 positions of a round and two operands each (two groups of 16 rows, or a group's two terms), so
+//           every row of keys is read from LDS twice; the queries' operands stay in registers.  A lane has four positions of a row, half of what
+//           it holds as an operand of the second product.  The two waves of a row keep one reference: a wave that finds a score too far above
+//           it says so, and at the start of the next round all waves know, and wait while the round's probabilities are formed again.
 //   context waves (4 .. 7): ctx^T[column][row] += rows^T P^T, 128 columns each, from transposed reads of the staged rows.
 // GT = 4 / NT groups of 16 rows: with two terms the probabilities' second terms are rows of their own for the context waves, and the context
 // is their sum.
 template <bool F16, int NT>
 __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
-    constexpr int GT = 4 / NT, kRows = 16 * GT;
+    constexpr int GT = 4 / NT, kRows = 16 * GT, GR = 2 / NT;     // GR: groups of rows of a score wave
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int limits[64];
-    __shared__ float xf[2][64];                 // rescale factors [parity][16 x group + row]
+    __shared__ float xm[2][2][64];              // largest exponents [parity][half of the round][row], where a reference has to move
+    __shared__ float xf[64];                    // factors of the rows whose reference moved
+    __shared__ __attribute__((aligned(16))) int need[4][4];     // [round % 4][score wave]: a reference has to move
     char *const pbuf = lds + kSlots * kSlotBytes;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, q4 = lane >> 4;
@@ -460,126 +483,128 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     const int nr = (t_end - t_begin + kRound - 1) / kRound;
 
     // ---- staging: round rd into slot rd % kSlots, by all waves: four latent rows each, the context waves eight rotary rows as well.
-    // A lane keeps the page of one of 64 rounds (a round lies in one page; -1: outside the pool, or no such round).
+    // A lane keeps, for one of 64 rounds, where its rows are (a round lies in one page) and how many bytes there are from there on: none for
+    // a page outside the pool.
     const int32_t *const pages = seq < 0 ? a.prefix : a.table + seq * a.table_row;
-    int mypage = -1;
+    uint64_t my_lat, my_rot;
+    uint32_t my_latb, my_rotb;
     auto look_up = [&](int first) __attribute__((always_inline)) {
-        const int rd = first + lane;
-        const int p = rd < nr ? pages[(t_begin + rd * kRound) >> a.shift] : -1;
-        mypage = p < a.pages ? p : -1;
+        const int rd = first + lane, pos = t_begin + rd * kRound, off = pos & ((1 << a.shift) - 1);
+        int p = rd < nr ? pages[pos >> a.shift] : -1;
+        const bool in = p >= 0 && p < a.pages;
+        const uint32_t rows = static_cast<uint32_t>(min(t_end - pos, kRound)) - 1u;
+        p = in ? p : 0;
+        my_lat = reinterpret_cast<uint64_t>(a.lat) + p * a.lat_page + static_cast<uint64_t>(off) * a.lat_row;
+        my_rot = reinterpret_cast<uint64_t>(a.rot) + p * a.rot_page + static_cast<uint64_t>(off) * a.rot_row;
+        my_latb = in ? rows * a.lat_row + 1024u : 0u;
+        my_rotb = in ? rows * a.rot_row + 128u : 0u;
     };
-    auto page_of = [&](int rd) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(mypage, rd & 63); };
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds));
     const int rrow = 8 * (wave & 3) + (lane >> 3);
     const uint32_t lat_off = static_cast<uint32_t>(4 * wave) * a.lat_row + lane * 16u;
     const uint32_t rot_off = static_cast<uint32_t>(rrow) * a.rot_row + ((lane & 7) ^ (rrow & 7)) * 16u;
-    auto rsrc_of = [&](const char *base, uint32_t bytes) __attribute__((always_inline)) {
-        const uint64_t at = reinterpret_cast<uint64_t>(base);
-        return u32x4{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xffffu, bytes, 0x00020000u};
+    auto rsrc_of = [&](uint64_t at, uint32_t bytes, int rd) __attribute__((always_inline)) {
+        const int l = rd & 63;
+        return u32x4{static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at), l)),
+                     static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at >> 32), l)) & 0xffffu,
+                     static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(bytes), l)), 0x00020000u};
     };
-    auto stage = [&](int rd, int page, bool context) __attribute__((always_inline)) {
-        const int off = (t_begin + rd * kRound) & ((1 << a.shift) - 1), rows = page >= 0 ? min(t_end - t_begin - rd * kRound, kRound) : 0;
-        const uint32_t to = lds0 + (rd & (kSlots - 1)) * kSlotBytes;
-        const int64_t p = page >= 0 ? page : 0;
-        const u32x4 rl = rsrc_of(a.lat + p * a.lat_page + static_cast<int64_t>(off) * a.lat_row, rows > 0 ? (rows - 1) * a.lat_row + 1024u : 0u);
+    // prepare(rd), then a row at a time: a load takes 16 cycles of the CU's path to LDS, so they are spread over a round
+    u32x4 r_lat, r_rot;
+    uint32_t to_slot;
+    auto prepare = [&](int rd, bool context) __attribute__((always_inline)) {
+        to_slot = lds0 + (rd & (kSlots - 1)) * kSlotBytes;
+        r_lat = rsrc_of(my_lat, my_latb, rd);
+        if (context) r_rot = rsrc_of(my_rot, my_rotb, rd);
+    };
+    auto stage_row = [&](int i) __attribute__((always_inline)) { load_to_lds(r_lat, lat_off + i * a.lat_row, to_slot + (4 * wave + i) * kLatLd); };
+    auto stage_rot = [&]() __attribute__((always_inline)) { load_to_lds(r_rot, rot_off, to_slot + kRound * kLatLd + (wave & 3) * 1024); };
+    auto stage = [&](int rd, bool context) __attribute__((always_inline)) {
+        prepare(rd, context);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load_to_lds(rl, lat_off + i * a.lat_row, to + (4 * wave + i) * kLatLd);
-        if (context) {
-            const u32x4 rr = rsrc_of(a.rot + p * a.rot_page + static_cast<int64_t>(off) * a.rot_row, rows > 0 ? (rows - 1) * a.rot_row + 128u : 0u);
-            load_to_lds(rr, rot_off, to + kRound * kLatLd + (wave & 3) * 1024);
-        }
+        for (int i = 0; i < 4; ++i) stage_row(i);
+        if (context) stage_rot();
     };
+    bool in0, in1;              // whether the pages of this round and the next are in the pool; r_lat says it of the one after that
     look_up(0);
 
     // Iteration t = -1 .. nr - 1: round t + 3 is sent for, the score waves take round t + 1, the context waves round t; then round t + 2 is
     // waited for.  A slot is written again three iterations after its scores, two after its context.
+    // The score waves leave in need[round % 4] whether a row's reference has to move for it: then its probabilities are formed again, by all
+    // score waves, before they are used, and the block waits for it.  (One reading lane's word for the usual answer, that none has.)
+    if (tid < 16) need[tid >> 2][tid & 3] = 0;
+    auto needed = [&](int rd) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4 *>(need[rd & 3]); };
+    auto any_of = [&](u32x4 n) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(n.x | n.y | n.z | n.w) != 0; };
+
     if (wave < 4) {
         // ================= score waves
-        const int grp = wave % GT;
-        const int gidx = min((seq >= 0 ? seq * a.G : 0) + tile * GT + grp, a.groups - 1);
-        const char *qp = a.qop + static_cast<int64_t>(gidx) * (NT * kSteps * kFrag) + lane * 16;
-        u32x4 q[NT][kSteps];
+        constexpr int kAhead = 6;
+        const int rg = wave & 1, pt = wave >> 1;            // operands 2 rg and 2 rg + 1; positions 16 pt .. +16 of a round
+        u32x4 q[2][kSteps];                                 // [operand]: two groups of rows, or a group's two terms
+        float fac[GR];
+        int limit[GR];
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int o = 0; o < 2; ++o) {
+            const int grp = (2 * rg + o) / NT, term = NT == 2 ? o : 0;
+            const int gidx = min((seq >= 0 ? seq * a.G : 0) + tile * GT + grp, a.groups - 1);
+            const char *qp = a.qop + (static_cast<int64_t>(gidx) * NT + term) * (kSteps * kFrag) + lane * 16;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) q[x][k] = *reinterpret_cast<const u32x4 *>(qp + (x * kSteps + k) * kFrag);
-        float fac[kParts];
+            for (int k = 0; k < kSteps; ++k) q[o][k] = *reinterpret_cast<const u32x4 *>(qp + k * kFrag);
+            float top = 1.f;
+            if constexpr (F16) {        // to the row's one scale: exact, but for what comes below fp16's last bit
+                float part[kParts];
+                top = 0.f;
 #pragma unroll
-        for (int j = 0; j < kParts; ++j) fac[j] = a.scales[(static_cast<int64_t>(gidx) * kParts + j) * 16 + r16] * a.c;
-        const int limit = limits[grp * 16 + r16];
-        float ref = -INFINITY, l_run = 0.f;
+                for (int j = 0; j < kParts; ++j) {
+                    part[j] = a.scales[(static_cast<int64_t>(gidx) * kParts + j) * 16 + r16];
+                    top = fmaxf(top, part[j]);
+                }
+                const float inv = top > 0.f ? 1.0f / top : 0.f;     // (a power of two)
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    const _Float16 d = static_cast<_Float16>(part[k / 4] * inv);
+                    const f16x2 d2 = {d, d};
+                    const uint32_t w[4] = {q[o][k].x, q[o][k].y, q[o][k].z, q[o][k].w};
+                    uint32_t v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, w[i]) * d2);
+                    q[o][k] = u32x4{v[0], v[1], v[2], v[3]};
+                }
+            }
+            fac[o % GR] = top * a.c;
+            limit[o % GR] = limits[grp * 16 + r16];
+        }
         // (all of it is here before the first round is sent for: a wait for it in the loop would wait for the rounds in flight)
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int o = 0; o < 2; ++o)
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(q[x][k]));
+            for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(q[o][k]));
 #pragma unroll
-        for (int j = 0; j < kParts; ++j) asm volatile("" : "+v"(fac[j]));
-        stage(0, page_of(0), false);
-        stage(1, page_of(1), false);
-        arrived_barrier<4>();
-        for (int rd = 0; rd <= nr; ++rd) {
-            const bool ok = page_of(rd) >= 0;
-            if (((rd + 2) & 63) == 0) look_up(rd + 2);      // (rounds rd + 2 .. of the next 64: this round's page is taken)
-            stage(rd + 2, page_of(rd + 2), false);
-            if (rd < nr && wave < GT) {
-                const char *slot = lds + (rd & (kSlots - 1)) * kSlotBytes;
-                f32x4 acc[2][kParts];
+        for (int g = 0; g < GR; ++g) asm volatile("" : "+v"(fac[g]));
+        // exponents of the last round's probabilities, 2^e with e = score - from (a row's reference less kLiftP); top: above it the reference
+        // moves (kTop, or anything for a row that has none yet)
+        float e[GR][4], from[GR], top[GR], l_run[GR], l_new[GR];
 #pragma unroll
-                for (int p = 0; p < 2; ++p)
+        for (int g = 0; g < GR; ++g) from[g] = 0.f, top[g] = -INFINITY, l_run[g] = l_new[g] = 0.f;
+        const char *const krow = lds + (pt * 16 + r16) * kLatLd + q4 * 16;
+        const char *const rrow0 = lds + kRound * kLatLd + (pt * 16 + r16) * 128;
+        auto frag = [&](int slot, int k) __attribute__((always_inline)) {
+            return *reinterpret_cast<const u32x4 *>(k < 16 ? krow + slot + k * 64 : rrow0 + slot + ((((k - 16) * 4 + q4) ^ (r16 & 7)) * 16));
+        };
+        // probabilities of a round, as operands of the second product
+        auto publish = [&](int rd) __attribute__((always_inline)) {
+            char *const to = pbuf + (rd & 1) * kPBytes + 2 * rg * kFrag + lane * 16 + pt * 8;
 #pragma unroll
-                    for (int j = 0; j < kParts; ++j) acc[p][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int g = 0; g < GR; ++g) {
+                float pr[4];
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        const int row = p * 16 + r16;
-                        const char *src = k < 16 ? slot + row * kLatLd + k * 64 + q4 * 16
-                                                 : slot + kRound * kLatLd + row * 128 + ((((k - 16) * 4 + q4) ^ (row & 7)) * 16);
-                        const u32x4 x = *reinterpret_cast<const u32x4 *>(src);
-#pragma unroll
-                        for (int y = 0; y < NT; ++y) acc[p][k / 4] = mfma<F16>(x, q[y][k], acc[p][k / 4]);
-                    }
-                const int base = t_begin + rd * kRound + 4 * q4;
-                const bool mixed = !ok || t_begin + (rd + 1) * kRound > t_all;
-                float s[8], mx = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int p = i >> 2, v = i & 3;
-                    float x = acc[p][0][v] * fac[0];
-#pragma unroll
-                    for (int j = 1; j < kParts; ++j) x = fmaf(acc[p][j][v], fac[j], x);
-                    s[i] = x;
-                }
-                if (mixed) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        // (where values are cleaned for the sake of rows that do not see them, an infinite score has to make its row NaN by itself)
-                        if (!(fabsf(s[i]) < INFINITY)) s[i] = NAN;
-                        s[i] = ok && base + 16 * (i >> 2) + (i & 3) < limit ? s[i] : -INFINITY;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i]);
-                mx = q4_rows_max(mx);
-                float f = 1.f;
-                if (__any(mx > ref + kSlackP)) {
-                    if (mx > ref + kSlackP) {
-                        f = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - mx);
-                        l_run *= f;
-                        ref = mx;
-                    }
-                }
-                const float from = ref == -INFINITY ? 0.f : ref - kLiftP;
-                float pr[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) pr[i] = __builtin_amdgcn_exp2f(s[i] - from), l_run += pr[i];
-                char *const to = pbuf + (rd & 1) * kPBytes + grp * NT * kFrag + lane * 16;
+                for (int i = 0; i < 4; ++i) pr[i] = __builtin_amdgcn_exp2f(e[g][i]);
+                if constexpr (!F16 || NT == 2) l_new[g] = (pr[0] + pr[1]) + (pr[2] + pr[3]);
 #pragma unroll
                 for (int y = 0; y < NT; ++y) {
-                    u32x4 o;
+                    u32x2 o;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 2; ++i) {
                         o[i] = pack2<F16>(pr[2 * i], pr[2 * i + 1]);
                         if (y + 1 < NT) {
                             float u, w;
@@ -587,69 +612,199 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                             pr[2 * i] -= u, pr[2 * i + 1] -= w;
                         }
                     }
-                    *reinterpret_cast<u32x4 *>(to + y * kFrag) = o;
+                    *reinterpret_cast<u32x2 *>(to + (NT == 2 ? y : g) * kFrag) = o;
+                    if constexpr (F16 && NT == 1) {     // (the sum of what is multiplied: the roundings of a probability that takes all cancel)
+                        const f16x2 one = {1, 1};
+                        l_new[g] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, static_cast<uint32_t>(o.x)), one,
+                                                          __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, static_cast<uint32_t>(o.y)), one, 0.f, false), false);
+                    }
                 }
-                if (q4 == 0) xf[rd & 1][grp * 16 + r16] = f;
             }
+        };
+        stage(0, false);
+        in0 = r_lat.z != 0;
+        stage(1, false);
+        in1 = r_lat.z != 0;
+        arrived_barrier<4>();
+        for (int rd = 0; rd <= nr; ++rd) {
+            if (((rd + 2) & 63) == 0) look_up(rd + 2);
+            const int slot = (rd & (kSlots - 1)) * kSlotBytes;
+            u32x4 ring[kAhead];                             // operands on their way (of a round too many: of an old slot)
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) ring[k] = frag(slot, k);
+            const u32x4 raw = needed(rd - 1);
+            f32x4 acc[2];                                   // [operand]
+            bool again = false;
+            if (rd == nr) {
+                again = any_of(raw);
+            } else {
+                __builtin_amdgcn_s_setprio(2);
+                acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    const u32x4 x = ring[k % kAhead];
+#pragma unroll
+                    for (int o = 0; o < 2; ++o) acc[o] = mfma<F16>(x, q[o][k], acc[o]);
+                    if (k + kAhead < kSteps) ring[k % kAhead] = frag(slot, k + kAhead);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (k == 0) prepare(rd + 2, false);
+                    if (k == 2) again = rd > 0 && any_of(raw);
+                    if (k >= 4 && k % 3 == 1 && k < 16) stage_row(k / 3 - 1);
+                }
+            }
+            {
+                if (again) {
+                    const u32x4 n = needed(rd - 1);
+                    const bool me = (pt ? (rg ? n.w : n.z) : (rg ? n.y : n.x)) != 0, other = (pt ? (rg ? n.y : n.x) : (rg ? n.w : n.z)) != 0;
+#pragma unroll
+                    for (int g = 0; g < GR; ++g) {
+                        const int row = (GR * rg + g) * 16 + r16;
+                        float t = other ? xm[(rd - 1) & 1][1 - pt][row] : -INFINITY, f = 1.f;
+                        if (me) t = fmaxf(t, xm[(rd - 1) & 1][pt][row]);
+                        if (t > top[g]) {
+                            const float d = t - kLiftP;
+                            f = top[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(-d);
+                            from[g] += d, top[g] = kTop;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) e[g][i] -= d;
+                        }
+                        l_run[g] *= f;
+                        if (pt == 0 && q4 == 0) xf[row] = f;
+                    }
+                    publish(rd - 1);
+                    block_barrier();
+                }
+#pragma unroll
+                for (int g = 0; g < GR; ++g) l_run[g] += l_new[g];
+            }
+            if (rd < nr) {
+                const int base = t_begin + rd * kRound + 16 * pt + 4 * q4;
+                const bool mixed = !in0 || t_begin + (rd + 1) * kRound > t_all;
+#pragma unroll
+                for (int g = 0; g < GR; ++g)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[g][i] = fmaf(NT == 2 ? acc[0][i] + acc[1][i] : acc[g][i], fac[g], -from[g]);
+                if (mixed) {
+#pragma unroll
+                    for (int g = 0; g < GR; ++g)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            // (where values are cleaned for the sake of rows that do not see them, an infinite score has to make its row NaN by itself)
+                            if (!(fabsf(e[g][i]) < INFINITY)) e[g][i] = NAN;
+                            e[g][i] = in0 && base + i < limit[g] ? e[g][i] : -INFINITY;
+                        }
+                }
+                bool above = false;
+#pragma unroll
+                for (int g = 0; g < GR; ++g) above |= max3(max3(e[g][0], e[g][1], e[g][2]), e[g][3], top[g]) > top[g];
+                if (__any(above)) {
+                    if (lane == 0) need[rd & 3][wave] = 1;
+#pragma unroll
+                    for (int g = 0; g < GR; ++g) {
+                        const float t = q4_rows_max(fmaxf(fmaxf(e[g][0], e[g][1]), fmaxf(e[g][2], e[g][3])));
+                        if (q4 == 0) xm[rd & 1][pt][(GR * rg + g) * 16 + r16] = t;
+                    }
+                }
+                publish(rd);
+                __builtin_amdgcn_s_setprio(0);
+            }
+            in0 = in1, in1 = r_lat.z != 0;
             arrived_barrier<4>();
         }
-        l_run = q4_rows_sum(l_run);
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+            const float l = q4_rows_sum(l_run[g]);
+            if (pt == 1 && q4 == 0) xf[(GR * rg + g) * 16 + r16] = l;
+            l_run[g] = l;
+        }
+        block_barrier();
         // (a row that sees nothing of the range was not masked where all others see all: its record counts for nothing)
-        if (wave < GT && q4 == 0 && grp * 16 + r16 < a.Mrec)
-            ml[grp * 16 + r16] = limit > t_begin ? make_float2(ref, l_run) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+            const int row = (GR * rg + g) * 16 + r16;
+            if (pt == 0 && q4 == 0 && row < a.Mrec)
+                ml[row] = limit[g] > t_begin ? make_float2(from[g], l_run[g] + xf[row]) : make_float2(-INFINITY, 0.f);
+        }
     } else {
         // ================= context waves
+        constexpr int kAhead = 5;
         const int cw = wave - 4;
         f32x4 acc[8][4];                        // [16 columns][16 (row, term)s]
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int g = 0; g < 4; ++g) acc[n][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-        stage(0, page_of(0), true);
-        stage(1, page_of(1), true);
+        stage(0, true);
+        in0 = r_lat.z != 0;
+        stage(1, true);
+        in1 = r_lat.z != 0;
         arrived_barrier<5>();
-        int before = -1, now = page_of(0);      // the pages of rounds rd - 1 and rd
+        s4_t ring[kAhead][2];                   // operands on their way: 16 columns of the positions 0 .. 16 and 16 .. 32
+        const char *const src0 = lds + (4 * q4 + (r16 >> 2)) * kLatLd + cw * 256 + (r16 & 3) * 8;
+        auto columns = [&](int rd, int n, s4_t (&x)[2]) __attribute__((always_inline)) {
+            const char *src = src0 + (rd & (kSlots - 1)) * kSlotBytes;
+            x[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32));
+            x[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32 + 16 * kLatLd));
+        };
         for (int rd = 0; rd <= nr; ++rd) {      // (as the score waves count: round rd - 1 is taken here)
-            const int after = page_of(rd + 1);
             if (((rd + 2) & 63) == 0) look_up(rd + 2);
-            stage(rd + 2, page_of(rd + 2), true);
-            if (rd > 0) {
-                char *const slot = lds + ((rd - 1) & (kSlots - 1)) * kSlotBytes;
+            if (rd == 0) {
+                stage(2, true);
+            } else {
                 const char *const pb = pbuf + ((rd - 1) & 1) * kPBytes + lane * 16;
-                if (before < 0 || t_begin + rd * kRound > t_all) {
-                    // some row does not see all of this round: what it does not see must not reach it, not even as 0 x infinity
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        u32x4 *const x = reinterpret_cast<u32x4 *>(slot + (4 * i + q4) * kLatLd + cw * 256 + r16 * 16);
-                        u32x4 v = *x;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) v[j] = finite2<F16>(v[j]);
-                        *x = v;
-                    }
-                }
+                const u32x4 raw = needed(rd - 1);
                 u32x4 p[4];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    p[g] = *reinterpret_cast<const u32x4 *>(pb + g * kFrag);
-                    const float f = xf[(rd - 1) & 1][g / NT * 16 + r16];
-                    if (__any(f != 1.f)) {
+                for (int g = 0; g < 4; ++g) p[g] = *reinterpret_cast<const u32x4 *>(pb + g * kFrag);
+                if (any_of(raw)) {
+                    block_barrier();
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) p[g] = *reinterpret_cast<const u32x4 *>(pb + g * kFrag);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float f = xf[g / NT * 16 + r16];
 #pragma unroll
                         for (int n = 0; n < 8; ++n) acc[n][g] *= f;
                     }
                 }
-                const char *src = slot + (4 * q4 + (r16 >> 2)) * kLatLd + cw * 256 + (r16 & 3) * 8;
+                if (wave == 4 && lane == 0) *reinterpret_cast<u32x4 *>(need[(rd + 1) & 3]) = u32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32));
-                    const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(src + n * 32 + 16 * kLatLd));
+                    const s4_t x = ring[n % kAhead][0], y = ring[n % kAhead][1];
+                    if (n + kAhead < 8) columns(rd - 1, n + kAhead, ring[n % kAhead]);
                     const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
                     for (int g = 0; g < 4; ++g) acc[n][g] = mfma<F16>(v, p[g], acc[n][g]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (n == 0) prepare(rd + 2, true);
+                    if (n >= 1 && n < 5) stage_row(n - 1);
+                    if (n == 5) stage_rot();
                 }
             }
-            before = now, now = after;
-            arrived_barrier<5>();
+            // round rd's rows, which the score waves have: their first operands, while this wave would wait
+            if (rd < nr && (!in0 || t_begin + (rd + 1) * kRound > t_all)) {
+                // some row does not see all of it: what it does not see must not reach it, not even as 0 x infinity
+                arrived_barrier<5>();           // (the scores are taken from the values as they are)
+                char *const slot = lds + (rd & (kSlots - 1)) * kSlotBytes;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    u32x4 *const x = reinterpret_cast<u32x4 *>(slot + (4 * i + q4) * kLatLd + cw * 256 + r16 * 16);
+                    u32x4 v = *x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = finite2<F16>(v[j]);
+                    *x = v;
+                }
+#pragma unroll
+                for (int n = 0; n < kAhead; ++n) columns(rd, n, ring[n]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < kAhead; ++n) columns(rd, n, ring[n]);
+                // (nothing that this wave wrote is waited for but need[], which its reads since then came after)
+                arrived_barrier<5, false>();
+            }
+            in0 = in1, in1 = r_lat.z != 0;
         }
+        block_barrier();
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
             const int row = g * 16 + r16;

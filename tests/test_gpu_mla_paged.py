@@ -161,3 +161,18 @@ def test_attention_with_counts_and_gate(pages, out):
     got = _run(case, counts=counts, gate=gate, out_dtype=out)
     _check(got, want, bound)
     assert not bool(got[2].any()) and not bool(got[0, 3:].any())
+
+
+@pytest.mark.parametrize("pages,out", [(F16, BF16), (BF16, F32)])
+def test_attention_over_ranges_of_more_than_64_rounds(pages, out):
+    # so many requests that a block takes all 4416 positions of the prefix, 138 rounds
+    case = oracle.make(_gen(9), 150, 1, 64, [4416 + b % 3 for b in range(150)], pages_dtype=pages, prefix=4416)
+    got = _run(case, out_dtype=out)
+    for b in (0, 1, 77, 149):
+        one = {k: v[b:b + 1] if k in ("q_nope", "q_rot", "table", "lengths") else v for k, v in case.items()}
+        _check(got[b:b + 1], *oracle.attention(**one, out_dtype=out))
+    # a page of the prefix that is none: its positions count as not there
+    case["prefix"][40] = case["lat"].shape[0]
+    got = _run(case, out_dtype=out)
+    one = {k: v[5:6] if k in ("q_nope", "q_rot", "table", "lengths") else v for k, v in case.items()}
+    _check(got[5:6], *oracle.attention(**one, out_dtype=out))
