@@ -10,7 +10,7 @@
 //   qa       q_nope W_UK on the bf16 matrix cores (fp32 queries as three bf16 terms), rounded into the terms that attend multiplies; a block
 //            more makes the list of items
 //   attend   an item a block: a tile of rows x a range of positions; the maximum and sum run with the positions
-//   uv       the items' records joined (prefix ranges and own ranges alike), the context times W_UV, the output gate
+//   uv       the items' records joined (those of the prefix and the sequence's own alike), the context times W_UV, the output gate
 //
 // Numerics.  fp16 pages multiply as fp16: 11 bits make one term of a query or probability enough for a bf16 result (off by 2^-11 at most, independent
 // errors below the result's own 2^-8) and two for fp32 (2^-22); bf16 terms would need two and three.  The absorbed query's 128 columns
@@ -38,26 +38,30 @@ constexpr int kFrag = 1024;                     // bytes of an operand of 16 row
 constexpr float kLiftP = 7.f, kTop = 15.f;     // log2 of a probability at the row's reference, and of the largest there may be
 
 // ------------------------------------------------------------------ items
-// Rows in groups of 16: group g of sequence b holds its rows 16 g .. of t H + h.  A block takes GT groups: of one sequence over a range of
-// its own positions, or any GT neighbours over a range of the prefix.
+// Rows in groups of 16: group g of sequence b holds its rows 16 g .. of t H + h.  A block takes an item: a tile of GT groups over a range of
+// positions.  Positions below `split`, all of the prefix, are taken by tiles of any GT neighbours (ranges of one length, every tile's first range,
+// then every tile's second ..), those from there on by tiles of one sequence (its ranges one after the other).  Where a sequence's groups fill whole
+// tiles both are the same tiles, and the split may lie before the prefix's end: no range is cut there.
 struct Item {
-    int seq;            // the sequence, or -1: the prefix
+    int seq;            // the sequence, or -1: of all
     int tile;           // the first group is GT tile (of the sequence, or of all)
     int begin, end;     // positions
 };
 struct Head {           // of the list
-    int used;           // items
-    int ranges;         // of the prefix: its items are range r of tile i at r tiles + i
+    int ranges;         // below the split: its items are range r of tile i at r tiles + i
+    int low, high;      // items below and above the split
+    int pad;
 };
 struct Lists {
     const int32_t *lengths, *counts;
     Head *head;
-    int2 *seq;          // [B]: first item, ranges of each of its tiles
+    int2 *seq;          // [B]: first item above the split, ranges of each of its tiles
     Item *item;
     int B, T, t0, Tall, cap, prefix;        // prefix: positions
-    int tiles, ptiles;  // of a sequence, of the prefix
+    int tiles, ptiles;  // of a sequence, of all
     int most;           // items there is room for
     int turns;          // items a CU may have
+    int aligned;        // a sequence's groups fill whole tiles
 };
 
 // what query t (of its sequence's first n = counts[b]) sees
@@ -72,86 +76,117 @@ __device__ __forceinline__ int sees_last(const Lists &a, int b) {
 }
 
 constexpr int kSearched = 1024;         // sequences up to which the ranges' length is searched for
-constexpr int kCandidates = 64;
+constexpr int kCandidates = 64;         // lengths: one to two shares of one to kTurns turns of the card's 256 CUs
+constexpr int kTurns = 8;
 constexpr int kRound = 32;              // positions of a round of the attention
+constexpr int kStart = 256;             // what an item's start and end cost, in positions
+constexpr int kListLds = (kSearched + 4 * kCandidates + 16) * 4;
 
-// By one block of 256 threads.  Ranges are all of one length, the one of 64 candidates (one to two shares of one to four turns of
-// the card's 256 CUs) for which turns x (length + kStart) is least; kStart: what an item's start and end cost, in positions.
-constexpr int kStart = 192;
+// n / d, 1 / d given: exact for n < 2^23
+__device__ __forceinline__ int divide(int n, int d, float inverse) {
+    int c = static_cast<int>(static_cast<float>(n) * inverse);
+    return c + ((c + 1) * d <= n ? 1 : c * d > n ? -1 : 0);
+}
+
+// By one block of 256 threads.  All ranges are of one length, the candidate that costs least by this account: the full ones in whole turns of
+// the 256 CUs, the others where there is room in these, else in turns of their own; and no less than all there is to do shared out.
 __device__ __forceinline__ void list_items(const Lists &a, int *lds) {
-    int *const own = lds, *const sh = lds + kSearched;      // own: positions of a sequence's own
+    int *const own = lds, *const part = lds + kSearched, *const sh = part + 4 * kCandidates;    // own: what a sequence's last query sees
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int lp = 0;
     float sum = 0.f;
     for (int b = tid; b < a.B; b += 256) {
-        const int n = sees_last(a, b), o = max(n - a.prefix, 0);
-        if (b < kSearched) own[b] = o;
+        const int n = sees_last(a, b);
+        if (b < kSearched) own[b] = n;
         lp = max(lp, min(n, a.prefix));
-        sum += static_cast<float>(o);
+        sum += static_cast<float>(a.aligned ? n : max(n - a.prefix, 0));
     }
-    lp = static_cast<int>(wave_max_all(static_cast<float>(lp)));        // (below 2^24: exact)
+    lp = static_cast<int>(wave_max_all(static_cast<float>(lp)));        // (at most 2^24: exact)
     sum = wave_sum_all(sum);
     if (lane == 0) sh[wave] = lp, sh[4 + wave] = __float_as_int(sum);
     __syncthreads();
     lp = max(max(sh[0], sh[1]), max(sh[2], sh[3]));
     sum = (__int_as_float(sh[4]) + __int_as_float(sh[5])) + (__int_as_float(sh[6]) + __int_as_float(sh[7]));
-    const float work = static_cast<float>(a.ptiles) * lp + static_cast<float>(a.tiles) * sum;
-    int best = 1 << 24;                 // (all of a sequence: what always fits)
+    const float work = static_cast<float>(a.tiles) * sum + (a.aligned ? 0.f : static_cast<float>(a.ptiles) * lp);
+    int Ts = 1 << 24;                   // (all of a sequence: what always fits)
+    // (a candidate a lane, a quarter of the sequences a wave)
     if (a.B <= kSearched) {
-        float least = INFINITY;
-        for (int i = wave; i < kCandidates; i += 4) {
-            const int turns = 1 + i / 16;
-            const float want = work / (256.f * turns) * (1.f + (i % 16) * (1.f / 16));
-            const int Ts = (static_cast<int>(fminf(want, 16777216.f)) / kRound + 1) * kRound;
-            const float inv = 1.0f / Ts;
-            int n = 0;
-            for (int b = lane; b < a.B; b += 64) {
-                const int o = own[b];
-                int c = static_cast<int>(o * inv);      // (within one of o / Ts: made exact)
-                c += (c + 1) * Ts <= o ? 1 : c * Ts > o ? -1 : 0;
-                n += c + (c * Ts < o);
-            }
-            const int all = static_cast<int>(wave_sum_all(static_cast<float>(n))) * a.tiles + (lp + Ts - 1) / Ts * a.ptiles;
-            const float cost = static_cast<float>((all + 255) / 256) * static_cast<float>(Ts + kStart);
-            if (turns <= a.turns && all <= a.most && cost < least) least = cost, best = Ts;
+        constexpr int kFractions = kCandidates / kTurns;
+        const int k = 1 + lane / kFractions;
+        const float want = work / (256.f * k) * (1.f + (lane % kFractions) * (1.f / kFractions));
+        const int T1 = (static_cast<int>(fminf(want, 8388608.f)) / kRound + 1) * kRound;
+        const float inv = 1.0f / T1;
+        const int r0 = a.aligned ? lp / T1 : (lp + T1 - 1) / T1, split = a.aligned ? r0 * T1 : a.prefix;
+        int full = 0, all = 0;
+        for (int b = wave; b < a.B; b += 4) {
+            const int o = max(own[b] - split, 0), c = divide(o, T1, inv);
+            full += c, all += c + (c * T1 < o);
         }
-        if (lane == 0) sh[8 + wave] = best, sh[12 + wave] = __float_as_int(least);
+        part[wave * kCandidates + lane] = full;
         __syncthreads();
-        best = sh[8], least = __int_as_float(sh[12]);
-        for (int i = 1; i < 4; ++i)
-            if (__int_as_float(sh[12 + i]) < least) least = __int_as_float(sh[12 + i]), best = sh[8 + i];
+        full = (part[lane] + part[kCandidates + lane]) + (part[2 * kCandidates + lane] + part[3 * kCandidates + lane]);
+        __syncthreads();
+        part[wave * kCandidates + lane] = all;
+        __syncthreads();
+        all = (part[lane] + part[kCandidates + lane]) + (part[2 * kCandidates + lane] + part[3 * kCandidates + lane]);
+        const int items = all * a.tiles + r0 * a.ptiles, whole = full * a.tiles + r0 * a.ptiles;
+        const int turns = (whole + 255) >> 8, left = items - whole - (turns * 256 - whole);
+        float cost = static_cast<float>(turns) * (T1 + kStart) + static_cast<float>((max(left, 0) + 255) >> 8) * (T1 / 2 + kStart);
+        cost = fmaxf(cost, (work + static_cast<float>(items) * kStart) * (1.0f / 256.f));
+        if (k > a.turns || items > a.most) cost = INFINITY;
+        // (cost, lane) least
+        float least = cost;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) least = fminf(least, __shfl_xor(least, o));
+        if (least < INFINITY) Ts = __builtin_amdgcn_readlane(T1, __builtin_ctzll(__ballot(cost == least)));
     }
-    const int Ts = best, ranges = (lp + Ts - 1) / Ts;
-    for (int j = tid; j < ranges * a.ptiles; j += 256) {
-        const int r = j / a.ptiles;
+    const int ranges = a.ptiles == 0 ? 0 : a.aligned ? lp / Ts : (lp + Ts - 1) / Ts, split = a.aligned ? ranges * Ts : a.prefix;
+    const int low = ranges * a.ptiles;
+    const float inv_p = 1.0f / max(a.ptiles, 1), inv_t = 1.0f / a.tiles, inv_T = 1.0f / Ts;
+    for (int j = tid; j < low; j += 256) {
+        const int r = divide(j, a.ptiles, inv_p);
         a.item[j] = Item{-1, j - r * a.ptiles, r * Ts, min((r + 1) * Ts, lp)};
     }
-    // the sequences' items, 256 sequences at a time
-    int done = ranges * a.ptiles;
+    // the sequences' items, 256 sequences at a time: their first items' places, then their items, a thread each
+    int done = low;
     for (int b0 = 0; b0 < a.B; b0 += 256) {
-        const int b = b0 + tid;
-        const int o = b >= a.B ? 0 : b < kSearched ? own[b] : max(sees_last(a, b) - a.prefix, 0);
-        const int c = (o + Ts - 1) / Ts, n = c * a.tiles;
+        const int b = b0 + tid, nb = min(a.B - b0, 256);
+        const int o = b >= a.B ? 0 : max((b < kSearched ? own[b] : sees_last(a, b)) - split, 0);
+        const int c = divide(o + Ts - 1, Ts, inv_T), n = c * a.tiles;
         int at = n;
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) {
             const int x = __shfl_up(at, k);
             if (lane >= k) at += x;
         }
-        __syncthreads();                // sh is free
+        __syncthreads();                // sh and part are free
         if (lane == 63) sh[wave] = at;
         __syncthreads();
         at -= n;
         for (int i = 0; i < wave; ++i) at += sh[i];
-        at += done;
-        if (b < a.B) a.seq[b] = make_int2(at, c);
-        for (int j = 0; j < n; ++j) {
-            const int r = j / a.tiles;
-            a.item[at + j] = Item{b, j - r * a.tiles, a.prefix + r * Ts, a.prefix + min((r + 1) * Ts, o)};
+        if (b < a.B) a.seq[b] = make_int2(done + at, c);
+        const int total = sh[0] + sh[1] + sh[2] + sh[3];
+        part[tid] = at;                 // (kCandidates x 4 = 256)
+        if (b0 < kSearched) {
+            __syncthreads();
+            for (int j = tid; j < total; j += 256) {
+                int q = 0;              // the last sequence that starts at or before j (one of several that start there has items: the last)
+#pragma unroll
+                for (int step = 128; step; step >>= 1)
+                    if (q + step < nb && part[q + step] <= j) q += step;
+                const int x = j - part[q], r = divide(x, a.tiles, inv_t), len = own[b0 + q];
+                a.item[done + j] = Item{b0 + q, x - r * a.tiles, split + r * Ts, min(split + (r + 1) * Ts, len)};
+            }
+            __syncthreads();
+        } else {
+            for (int j = 0; j < n; ++j) {
+                const int r = divide(j, a.tiles, inv_t);
+                a.item[done + at + j] = Item{b, j - r * a.tiles, split + r * Ts, min(split + (r + 1) * Ts, split + o)};
+            }
         }
-        done += sh[0] + sh[1] + sh[2] + sh[3];
+        done += total;
     }
-    if (tid == 0) *a.head = Head{done, ranges};
+    if (tid == 0) *a.head = Head{ranges, low, done - low, 0};
 }
 
 // ------------------------------------------------------------------ qa
@@ -456,11 +491,14 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     char *const pbuf = lds + kSlots * kSlotBytes;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, q4 = lane >> 4;
-    // blocks b % 8 share an XCD and its L2: neighbours in the list, which read the same positions, go to one
+    // blocks b % 8 share an XCD and its L2: neighbours in the list, which read the same positions, go to one, and an eighth of both kinds to each
     const Head head = *a.lists.head;
-    const int used = __builtin_amdgcn_readfirstlane(head.used), each = (used + 7) >> 3;
-    const int at = static_cast<int>(blockIdx.x & 7) * each + static_cast<int>(blockIdx.x >> 3);
-    if (static_cast<int>(blockIdx.x >> 3) >= each || at >= used) return;
+    const int low = __builtin_amdgcn_readfirstlane(head.low), high = __builtin_amdgcn_readfirstlane(head.high);
+    const int x = static_cast<int>(blockIdx.x & 7), j = static_cast<int>(blockIdx.x >> 3);
+    const int l0 = static_cast<int>(static_cast<int64_t>(low) * x >> 3), l1 = static_cast<int>(static_cast<int64_t>(low) * (x + 1) >> 3);
+    const int h0 = static_cast<int>(static_cast<int64_t>(high) * x >> 3), h1 = static_cast<int>(static_cast<int64_t>(high) * (x + 1) >> 3);
+    if (j >= l1 - l0 + h1 - h0) return;
+    const int at = j < l1 - l0 ? l0 + j : low + h0 + j - (l1 - l0);
     const Item it = a.lists.item[at];
     const int seq = __builtin_amdgcn_readfirstlane(it.seq), tile = __builtin_amdgcn_readfirstlane(it.tile);
     const int t_begin = __builtin_amdgcn_readfirstlane(it.begin), end = __builtin_amdgcn_readfirstlane(it.end);
@@ -485,12 +523,12 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     // ---- staging: round rd into slot rd % kSlots, by all waves: four latent rows each, the context waves eight rotary rows as well.
     // A lane keeps, for one of 64 rounds, where its rows are (a round lies in one page) and how many bytes there are from there on: none for
     // a page outside the pool.
-    const int32_t *const pages = seq < 0 ? a.prefix : a.table + seq * a.table_row;
+    const int32_t *const pages = a.table + max(seq, 0) * a.table_row;
     uint64_t my_lat, my_rot;
     uint32_t my_latb, my_rotb;
     auto look_up = [&](int first) __attribute__((always_inline)) {
         const int rd = first + lane, pos = t_begin + rd * kRound, off = pos & ((1 << a.shift) - 1);
-        int p = rd < nr ? pages[pos >> a.shift] : -1;
+        int p = rd < nr ? (pos < a.lists.prefix ? a.prefix : pages)[pos >> a.shift] : -1;
         const bool in = p >= 0 && p < a.pages;
         const uint32_t rows = static_cast<uint32_t>(min(t_end - pos, kRound)) - 1u;
         p = in ? p : 0;
@@ -835,112 +873,135 @@ struct UvArgs {
 
 constexpr int kCLd = 1040;      // LDS bytes of a context row's term: 1024 + 16
 
-// grid (H, ceil(M / PER), Z): PER queries of head x, the z-th part of the V / 16 tiles of output columns.  256 / PER threads join a query's
-// records, sixteen to a record (32 columns each), 16 / PER records side by side; the sums meet in LDS and are left there as TERMS bf16 terms.  Then
-// a wave takes output tiles, its rows of W_UV as they lie.
+// A row's records: those of its tile below the split, then its sequence's.
+struct Records {
+    int first, low, n, step, tiles, in, pin, Mrec;
+    __device__ __forceinline__ Records(const UvArgs &a, int m, int h) {
+        const int b = m / a.T, row = (m - b * a.T) * a.H + h, g = row >> 4, pg = b * a.G + g;
+        const int2 mine = a.seq[b];
+        low = a.head->ranges, n = low + mine.y;
+        first = mine.x + g / a.GT, step = a.ptiles, tiles = a.tiles, Mrec = a.Mrec;
+        in = (g % a.GT) * 16 + (row & 15), pin = pg / a.GT * a.Mrec + (pg % a.GT) * 16 + (row & 15);
+    }
+    // the place of record k (at most 2^31 rows: of items of at least 1 KB a row, 2 TB)
+    __device__ __forceinline__ int at(int k) const { return k < low ? k * step * Mrec + pin : (first + (k - low) * tiles) * Mrec + in; }
+};
+
+// grid (H, ceil(M / PER)), eight waves: PER queries of head x.  A wave joins the records of a query (PER 1: eight waves every eighth record of 64), eight
+// columns a lane, and leaves the context in LDS as TERMS bf16 terms; then a wave takes 16 output columns of all queries, its rows of W_UV as they lie
+// (the first of them loaded before anything else).
 template <int TERMS, int PER>
-__global__ __launch_bounds__(256) void uv_kernel(UvArgs a) {
-    static_assert(PER == 1 || PER >= 4, "a query's threads are the block, whose one query is there, or within a wave");
-    constexpr int kSide = 16 / PER;
+__global__ __launch_bounds__(512) void uv_kernel(UvArgs a) {
+    static_assert(PER == 1 || PER % 8 == 0, "waves to a query, or queries to a wave");
+    constexpr int kTiles = (PER + 15) / 16, kRows = PER < 16 ? PER : 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    float *const sums = reinterpret_cast<float *>(lds);         // [PER][kSide][512]
-    char *const ctx = lds + 16 * kLat * 4;                      // [TERMS][16][kCLd]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
+    char *const ctx = lds;                                      // [TERMS][PER][kCLd]
+    float *const sums = reinterpret_cast<float *>(lds + TERMS * PER * kCLd);    // PER 1: [8][512], then maxima and sums [8]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
     const int h = blockIdx.x, m0 = blockIdx.y * PER;
-    {
-        const int i = tid / (256 / PER), side = tid / 16 % kSide, c = tid & 15, m = m0 + i;
-        f32x4 s[8];
+    const int vtiles = (a.V + 15) / 16;
+    const auto rw = make_rsrc(a.w_uv + static_cast<int64_t>(h) * a.V * kLat, static_cast<uint32_t>(a.V) * (2 * kLat));
+    u32x4 w[16];
+    auto weights = [&](int vt) __attribute__((always_inline)) {         // (rows past the head's last are outside and load zeros)
 #pragma unroll
-        for (int u = 0; u < 8; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 16; ++k)
+            w[k] = __builtin_bit_cast(u32x4, buf_load16(rw, static_cast<uint32_t>(vt * 16 + r16) * (2 * kLat) + k * 64 + q4 * 16));
+    };
+    weights(wave);
+    // the context of columns 4 lane .. +4 and 256 + 4 lane .. +4
+    auto store = [&](int i, f32x4 x, f32x4 y) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+            const u32x2 p = {q4_pack_bf16(x[0], x[1]), q4_pack_bf16(x[2], x[3])}, o = {q4_pack_bf16(y[0], y[1]), q4_pack_bf16(y[2], y[3])};
+            *reinterpret_cast<u32x2 *>(ctx + (t * PER + i) * kCLd + lane * 8) = p;
+            *reinterpret_cast<u32x2 *>(ctx + (t * PER + i) * kCLd + 512 + lane * 8) = o;
+            x -= f32x4{q4_lo(p.x), q4_hi(p.x), q4_lo(p.y), q4_hi(p.y)};
+            y -= f32x4{q4_lo(o.x), q4_hi(o.x), q4_lo(o.y), q4_hi(o.y)};
+        }
+    };
+#pragma unroll 1
+    for (int i = PER == 1 ? 0 : wave; i < PER; i += 8) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+        float mx = -INFINITY, l = 0.f;
+        const int m = m0 + i;
         if (m < a.M) {
-            const int b = m / a.T, row = (m - b * a.T) * a.H + h, g = row >> 4, pg = b * a.G + g;
-            const int2 mine = a.seq[b];
-            const int np = a.head->ranges, n = np + mine.y;
-            // record k of the row: ranges of the prefix, then its own
-            auto record = [&](int k) -> int64_t {
-                const int64_t item = k < np ? static_cast<int64_t>(k) * a.ptiles + pg / a.GT : mine.x + static_cast<int64_t>(k - np) * a.tiles + g / a.GT;
-                return item * a.Mrec + (k < np ? pg % a.GT : g % a.GT) * 16 + (row & 15);
-            };
-            float mx = -INFINITY, l = 0.f;
-            for (int k = tid % (256 / PER); k < n; k += 256 / PER) mx = fmaxf(mx, a.ml[record(k)].x);
-            // (over the query's threads, within a wave here and over the block's waves below)
+            const Records rec(a, m, h);
+            // (the weight of a record that the row sees nothing of is zero, and what is written there does not matter)
+            auto stats = [&](int k) __attribute__((always_inline)) { return k < rec.n ? a.ml[rec.at(k)] : make_float2(-INFINITY, 0.f); };
+            float2 v = stats(lane);             // the first 64
+            mx = v.x;
+            for (int k0 = 64; k0 < rec.n; k0 += 64) mx = fmaxf(mx, stats(k0 + lane).x);
+            mx = wave_max_all(mx);
+            for (int k0 = 0; k0 < rec.n; k0 += 64) {
+                if (k0) v = stats(k0 + lane);
+                const int at = rec.at(min(k0 + lane, rec.n - 1)), n = min(rec.n - k0, 64);
+                const float f = v.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v.x - mx);
+                if (PER > 1 || wave == 0) l = fmaf(f, v.y, l);
+                constexpr int kSide = 8;                        // records on their way
+                for (int j0 = PER == 1 ? wave * kSide : 0; j0 < n; j0 += PER == 1 ? 8 * kSide : kSide) {
+                    f32x4 c[kSide][2];
+                    float g[kSide];
 #pragma unroll
-            for (int o = 1; o < (256 / PER < 64 ? 256 / PER : 64); o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-            if constexpr (PER == 1) {
-                if (lane == 0) sums[wave] = mx;
-                __syncthreads();
-                mx = fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3]));
-                __syncthreads();
-            }
-            for (int k = side; k < n; k += kSide) {
-                const int64_t at = record(k);
-                const float2 v = a.ml[at];
-                if (v.y == 0.f) continue;       // (it sees nothing there, and what is written there does not matter)
-                const float w = __builtin_amdgcn_exp2f(v.x - mx);
-                l = fmaf(w, v.y, l);
-                const float *from = a.part + at * kLat + 4 * c;
+                    for (int j = 0; j < kSide; ++j) {
+                        const int from = __builtin_amdgcn_readlane(at, min(j0 + j, n - 1));
+                        g[j] = j0 + j < n ? readlane_f(f, j0 + j) : 0.f;
+                        const float *p = a.part + static_cast<int64_t>(from) * kLat + 4 * lane;
+                        c[j][0] = *reinterpret_cast<const f32x4 *>(p), c[j][1] = *reinterpret_cast<const f32x4 *>(p + 256);
+                    }
 #pragma unroll
-                for (int u = 0; u < 8; ++u) s[u] += w * *reinterpret_cast<const f32x4 *>(from + 64 * u);
-            }
-            // l: the same in a record's sixteen threads; over the records side by side
-            float all = l;
-            if constexpr (kSide > 1) {
-#pragma unroll
-                for (int o = 16; o < (256 / PER < 64 ? 256 / PER : 64); o <<= 1) all += __shfl_xor(all, o);
-                if constexpr (PER == 1) {
-                    if (lane == 0) sums[wave] = all;
-                    __syncthreads();
-                    all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-                    __syncthreads();
+                    for (int j = 0; j < kSide; ++j)
+                        if (g[j] != 0.f) x += g[j] * c[j][0], y += g[j] * c[j][1];
                 }
             }
-            const float inv = all == 0.f ? 0.f : 1.0f / all;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) s[u] *= inv;
+            l = wave_sum_all(l);
         }
+        if constexpr (PER > 1) {
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            store(i, x * inv, y * inv);
+        } else {
+            *reinterpret_cast<f32x4 *>(sums + wave * kLat + 4 * lane) = x;
+            *reinterpret_cast<f32x4 *>(sums + wave * kLat + 256 + 4 * lane) = y;
+            if (wave == 0 && lane == 0) sums[8 * kLat] = l;
+            __syncthreads();
+            if (wave == 0) {
+                const float all = sums[8 * kLat], inv = all == 0.f ? 0.f : 1.0f / all;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) *reinterpret_cast<f32x4 *>(sums + (i * kSide + side) * kLat + 4 * c + 64 * u) = s[u];
+                for (int k = 1; k < 8; ++k) {
+                    x += *reinterpret_cast<const f32x4 *>(sums + k * kLat + 4 * lane);
+                    y += *reinterpret_cast<const f32x4 *>(sums + k * kLat + 256 + 4 * lane);
+                }
+                store(0, x * inv, y * inv);
+            }
+        }
     }
     __syncthreads();
-    for (int j = tid; j < PER * 128; j += 256) {
-        const int i = j >> 7, c = j & 127;
-        f32x4 x = *reinterpret_cast<const f32x4 *>(sums + i * kSide * kLat + 4 * c);
+    for (int vt = wave; vt < vtiles; vt += 8) {
+        if (vt != wave) weights(vt);
+        f32x4 o[kTiles];
 #pragma unroll
-        for (int k = 1; k < kSide; ++k) x += *reinterpret_cast<const f32x4 *>(sums + (i * kSide + k) * kLat + 4 * c);
-#pragma unroll
-        for (int y = 0; y < TERMS; ++y) {
-            const u32x2 p = {q4_pack_bf16(x[0], x[1]), q4_pack_bf16(x[2], x[3])};
-            *reinterpret_cast<u32x2 *>(ctx + (y * 16 + i) * kCLd + c * 8) = p;
-            x -= f32x4{q4_lo(p.x), q4_hi(p.x), q4_lo(p.y), q4_hi(p.y)};
-        }
-    }
-    __syncthreads();
-    const int vtiles = (a.V + 15) / 16, per_z = (vtiles + gridDim.z - 1) / gridDim.z, v_last = min(vtiles, (static_cast<int>(blockIdx.z) + 1) * per_z);
-    const auto rw = make_rsrc(a.w_uv + static_cast<int64_t>(h) * a.V * kLat, static_cast<uint32_t>(a.V) * (2 * kLat));
-    for (int vt = blockIdx.z * per_z + wave; vt < v_last; vt += 4) {
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        u32x4 w[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k)            // (rows past the head's last are outside and load zeros)
-            w[k] = __builtin_bit_cast(u32x4, buf_load16(rw, static_cast<uint32_t>(vt * 16 + r16) * (2 * kLat) + k * 64 + q4 * 16));
-#pragma unroll
+        for (int t = 0; t < kTiles; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
         for (int y = TERMS - 1; y >= 0; --y)
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-                o = q4_mfma_bf16(w[k], *reinterpret_cast<const u32x4 *>(ctx + (y * 16 + r16 % PER) * kCLd + k * 64 + q4 * 16), o);
-        const int m = m0 + r16, v = vt * 16 + 4 * q4;
-        if (r16 < PER && m < a.M && v < a.V) {
-            const int b = m / a.T, t = a.t0 + m - b * a.T;
-            const int64_t to = ((static_cast<int64_t>(b) * a.Tall + t) * a.H + h) * a.V + v;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+                    o[t] = q4_mfma_bf16(w[k], *reinterpret_cast<const u32x4 *>(ctx + (y * PER + t * 16 + r16 % kRows) * kCLd + k * 64 + q4 * 16), o[t]);
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const int m = m0 + t * 16 + r16, v = vt * 16 + 4 * q4;
+            if (r16 >= kRows || m >= a.M || v >= a.V) continue;
+            const int b = m / a.T, tq = a.t0 + m - b * a.T;
+            const int64_t to = ((static_cast<int64_t>(b) * a.Tall + tq) * a.H + h) * a.V + v;
             if (a.gate) {
                 const f32x4 g = *reinterpret_cast<const f32x4 *>(a.gate + to);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = o[i] / (1.0f + expf(-g[i]));
+                for (int i = 0; i < 4; ++i) o[t][i] = o[t][i] / (1.0f + expf(-g[i]));
             }
             if (a.out_bf16)
-                *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + to) = u32x2{q4_pack_bf16(o[0], o[1]), q4_pack_bf16(o[2], o[3])};
+                *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + to) = u32x2{q4_pack_bf16(o[t][0], o[t][1]), q4_pack_bf16(o[t][2], o[t][3])};
             else
-                *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + to) = o;
+                *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + to) = o[t];
         }
     }
 }
@@ -964,9 +1025,10 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t max_length, int64_t prefix
     p.groups = B * p.G;
     p.ptiles = prefix > 0 ? static_cast<int>(cdiv(p.groups, p.GT)) : 0;
     p.Mrec = 16 * static_cast<int>(std::min<int64_t>(p.GT, prefix > 0 ? p.groups : p.G));
+    // every range that is not full, a tile and sequence one at most, and the others: at most 256 a turn, and of a round at least
     const int64_t base = B * p.tiles + p.ptiles;
     const int64_t positions = p.ptiles * std::min(prefix, max_length) + B * p.tiles * std::max<int64_t>(max_length - prefix, 0);
-    p.turns = static_cast<int>(std::min<int64_t>(4, std::max<int64_t>(1, positions / (256 * 1024))));
+    p.turns = static_cast<int>(std::min<int64_t>(kTurns, std::max<int64_t>(1, positions / (256 * 1024))));
     p.most = static_cast<int>(base + std::min<int64_t>(256 * p.turns, positions / kRound + 1));
     auto up = [](int64_t v) { return (v + 255) & ~int64_t(255); };
     int64_t o = 0;
@@ -983,7 +1045,7 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t max_length, int64_t prefix
 
 template <typename QT, bool F16, int NT, int MT>
 int launch_qa_of(const QaArgs &a, hipStream_t st) {
-    const int bytes = std::max({((a.nope + 31) / 32) * 32 * kWLd, 16 * MT * kFLd * 4, (kSearched + 64) * 4});
+    const int bytes = std::max({((a.nope + 31) / 32) * 32 * kWLd, 16 * MT * kFLd * 4, kListLds});
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(qa_kernel<QT, F16, NT, MT>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 256 * kWLd);
     const int rc = check_hip(attr, "mla paged: query LDS size");
@@ -1004,27 +1066,26 @@ int launch_attend(const AttendArgs &a, int most, hipStream_t st) {
         hipFuncSetAttribute(reinterpret_cast<const void *>(attend_kernel<F16, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, attend_lds());
     const int rc = check_hip(attr, "mla paged: attention LDS size");
     if (rc) return rc;
-    attend_kernel<F16, NT><<<dim3(static_cast<unsigned>(cdiv(most, 8) * 8)), 512, attend_lds(), st>>>(a);
+    attend_kernel<F16, NT><<<dim3(static_cast<unsigned>(cdiv(most, 8) * 8 + 8)), 512, attend_lds(), st>>>(a);   // (an eighth of both kinds of item: one more at most)
     return check_hip(hipGetLastError(), "mla paged: attention launch");
 }
 
 template <int TERMS, int PER>
-int launch_uv_of(const UvArgs &a, unsigned parts, hipStream_t st) {
-    constexpr int bytes = 16 * kLat * 4 + TERMS * 16 * kCLd;
+int launch_uv_of(const UvArgs &a, hipStream_t st) {
+    constexpr int bytes = TERMS * PER * kCLd + (PER == 1 ? (8 * kLat + 16) * 4 : 0);
     static const hipError_t attr =
         hipFuncSetAttribute(reinterpret_cast<const void *>(uv_kernel<TERMS, PER>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     const int rc = check_hip(attr, "mla paged: output LDS size");
     if (rc) return rc;
-    uv_kernel<TERMS, PER><<<dim3(static_cast<unsigned>(a.H), static_cast<unsigned>(cdiv(a.M, PER)), parts), 256, bytes, st>>>(a);
+    uv_kernel<TERMS, PER><<<dim3(static_cast<unsigned>(a.H), static_cast<unsigned>(cdiv(a.M, PER))), 512, bytes, st>>>(a);
     return check_hip(hipGetLastError(), "mla paged: join and W_UV launch");
 }
 template <int TERMS>
 int launch_uv(const UvArgs &a, hipStream_t st) {
-    // the most queries to a block with which there are blocks for every CU
-    const unsigned parts = static_cast<unsigned>(std::min<int64_t>(cdiv(a.V, 64), std::max<int64_t>(1, 256 / (a.H * cdiv(a.M, 16)))));
-    if (a.M >= 16 || a.H * cdiv(a.M, 4) >= 512) return launch_uv_of<TERMS, 16>(a, parts, st);
-    if (a.M >= 4) return launch_uv_of<TERMS, 4>(a, parts, st);
-    return launch_uv_of<TERMS, 1>(a, parts, st);
+    // the most queries to a block, which reads its head's W_UV, with which there are blocks for every CU
+    if (a.H * cdiv(a.M, 32) >= 512) return launch_uv_of<TERMS, 32>(a, st);
+    if (a.M > 4) return launch_uv_of<TERMS, 8>(a, st);
+    return launch_uv_of<TERMS, 1>(a, st);
 }
 
 }  // namespace
@@ -1089,7 +1150,8 @@ extern "C" int k3_mla_paged_attention(const void *q_nope, int64_t qn_batch, int6
         const int ptiles = prefix_pages > 0 ? static_cast<int>(cdiv(groups, p.GT)) : 0;
         const Lists lists{lengths, counts, reinterpret_cast<Head *>(ws + p.head), reinterpret_cast<int2 *>(ws + p.seq),
                           reinterpret_cast<Item *>(ws + p.item), static_cast<int>(B), Tp, static_cast<int>(t0), static_cast<int>(T),
-                          static_cast<int>(max_length), static_cast<int>(std::min<int64_t>(prefix_pages * page_size, 1 << 24)), tiles, ptiles, p.most, p.turns};
+                          static_cast<int>(max_length), static_cast<int>(std::min(prefix_pages * page_size, max_length)), tiles, ptiles, p.most, p.turns,
+                          ptiles > 0 && G % p.GT == 0};
         const QaArgs qa{q_nope, q_rot, qn_batch, qn_token, qn_head, qr_batch, qr_token, qr_head, static_cast<const uint16_t *>(w_uk),
                         ws + p.qop, reinterpret_cast<float *>(ws + p.scales), static_cast<int>(H), static_cast<int>(nope_dim), M, Tp,
                         static_cast<int>(t0), G, lists};
