@@ -18,7 +18,7 @@
 // launch has one of them), and all to the row's largest scale as attend takes them in, so fp16's range is no question of the queries' size: what
 // falls below fp16's last bit then is 2^-38 of the row's largest.  Probabilities are 2^kLift times
 // those of the row's reference, which moves when one would exceed 2^kTop: so fp16 holds them, and its last bit is
-// 2^-31 of the largest.  bf16 pages multiply as bf16, exact, against two terms of both (2^-16), as the core over one sequence's cache
+// 2^-31 of the largest; an item's context, over its sum, goes to the join as fp16 (2^-11).  Two terms: as fp32.  bf16 pages multiply as bf16, exact, against two terms of both (2^-16), as the core over one sequence's cache
 // does.
 #include <algorithm>
 #include <type_traits>
@@ -37,8 +37,17 @@ constexpr int kParts = 5;                       // scales of a row: four quarter
 constexpr int kFrag = 1024;                     // bytes of an operand of 16 rows and 32 columns: 64 lanes x 16
 constexpr float kLiftP = 7.f, kTop = 15.f;     // log2 of a probability at the row's reference, and of the largest there may be
 
+// The order of a sequence's rows: by query (row = t H + h: few queries fill the groups of 16) or by head (row = h Tp + t, Tp = T rounded up
+// to 16: a group is 16 queries of one head, so a block of the query launch, which takes one head's matrix, writes whole operands).
+struct Rows {
+    int T, H, Tp;                   // Tp 0: by query
+    __host__ __device__ int count() const { return Tp ? H * Tp : T * H; }
+    __device__ __forceinline__ int of(int t, int h) const { return Tp ? h * Tp + t : t * H + h; }
+    __device__ __forceinline__ int query(int row) const { return Tp ? row % Tp : row / H; }     // may be >= T: no row
+};
+
 // ------------------------------------------------------------------ items
-// Rows in groups of 16: group g of sequence b holds its rows 16 g .. of t H + h.  A block takes an item: a tile of GT groups over a range of
+// Rows in groups of 16: group g of sequence b holds its rows 16 g .. +16.  A block takes an item: a tile of GT groups over a range of
 // positions.  Positions below `split`, all of the prefix, are taken by tiles of any GT neighbours (ranges of one length, every tile's first range,
 // then every tile's second ..), those from there on by tiles of one sequence (its ranges one after the other).  Where a sequence's groups fill whole
 // tiles both are the same tiles, and the split may lie before the prefix's end: no range is cut there.
@@ -197,6 +206,7 @@ struct QaArgs {
     char *qop;                                  // [group][term][step] operands
     float *scales;                              // [group][kParts][16]
     int H, nope, M, T, t0, G;                   // M = B T queries of the pass; G groups a sequence
+    Rows rows;
     Lists lists;
 };
 
@@ -350,7 +360,7 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     __syncthreads();
     // where row (query m, head h)'s operands are
     auto place = [&](int m, int &r) -> int64_t {
-        const int b = m / a.T, row = (m - b * a.T) * a.H + h;
+        const int b = m / a.T, row = a.rows.of(m - b * a.T, h);
         r = row & 15;
         return static_cast<int64_t>(b) * a.G + (row >> 4);
     };
@@ -420,9 +430,10 @@ struct AttendArgs {
     int64_t table_row;
     int pages, shift;
     Lists lists;
-    float *part;                                // [item][Mrec][512]
+    void *part;                                 // [item][Mrec][512]: contexts (fp32), or contexts over their sums (fp16: with one term)
     float2 *ml;                                 // [item][Mrec]
-    int H, G, groups, Mrec;                     // groups: of all sequences
+    int G, groups, Mrec;                        // groups: of all sequences
+    Rows rows;
     float c;                                    // scale * log2(e)
 };
 
@@ -483,6 +494,8 @@ __device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcn
 template <bool F16, int NT>
 __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     constexpr int GT = 4 / NT, kRows = 16 * GT, GR = 2 / NT;     // GR: groups of rows of a score wave
+    constexpr int kRecRow = kLat * (NT == 1 ? 2 : 4), kRecLd = kRecRow + 16;    // bytes of a record's row
+    static_assert(kRows * kRecLd <= kSlots * kSlotBytes && kRows * kRecRow == 64 * 1024, "the records fit the rounds' room");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int limits[64];
     __shared__ float xm[2][2][64];              // largest exponents [parity][half of the round][row], where a reference has to move
@@ -505,8 +518,8 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     // ---- what the rows see
     if (tid < kRows) {
         const int g = tile * GT + (tid >> 4);
-        const int b = seq >= 0 ? seq : g / a.G, row = (g - (seq >= 0 ? 0 : b * a.G)) * 16 + (tid & 15), t = row / a.H;
-        const bool there = b < a.lists.B && t < a.lists.T && (seq < 0 || g < a.G);
+        const int b = seq >= 0 ? seq : g / a.G, row = (g - (seq >= 0 ? 0 : b * a.G)) * 16 + (tid & 15), t = a.rows.query(row);
+        const bool there = b < a.lists.B && row < a.rows.count() && t < a.lists.T && (seq < 0 || g < a.G);
         limits[tid] = there ? min(sees_of(a.lists, b, a.lists.t0 + t), end) : 0;
     }
     __syncthreads();
@@ -749,10 +762,11 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
             in0 = in1, in1 = r_lat.z != 0;
             arrived_barrier<4>();
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
             const float l = q4_rows_sum(l_run[g]);
-            if (pt == 1 && q4 == 0) xf[(GR * rg + g) * 16 + r16] = l;
+            if (q4 == 0) (pt ? xf : xm[0][0])[(GR * rg + g) * 16 + r16] = l;
             l_run[g] = l;
         }
         block_barrier();
@@ -842,33 +856,49 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
             }
             in0 = in1, in1 = r_lat.z != 0;
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // (what still arrives must not fall into the records, nor into LDS that the block has left)
         block_barrier();
+        // the rows go through LDS (the rounds are done), so that they leave it as whole rows
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
             const int row = g * 16 + r16;
-            if (row >= a.Mrec) continue;
-            float *to = a.part + (static_cast<int64_t>(at) * a.Mrec + row) * kLat + cw * 128 + 4 * q4;
+            char *const to = lds + row * kRecLd + (cw * 128 + 4 * q4) * (NT == 1 ? 2 : 4);
+            if constexpr (NT == 1) {
+                const float l = xm[0][0][row] + xf[row], inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                f32x4 o = acc[n][g * NT];
-                if constexpr (NT == 2) o += acc[n][g * NT + 1];
-                *reinterpret_cast<f32x4 *>(to + n * 16) = o;
+                for (int n = 0; n < 8; ++n) {
+                    const f32x4 o = acc[n][g] * inv;
+                    *reinterpret_cast<u32x2 *>(to + n * 32) = u32x2{q4_pack_f16(o[0], o[1]), q4_pack_f16(o[2], o[3])};
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) *reinterpret_cast<f32x4 *>(to + n * 64) = acc[n][g * NT] + acc[n][g * NT + 1];
             }
         }
     }
-    arrived_barrier<0>();       // (nothing may arrive in LDS after the block has left it)
+    block_barrier();
+    {
+        char *const to = static_cast<char *>(a.part) + static_cast<int64_t>(at) * a.Mrec * kRecRow;
+        constexpr int kOf = kRecRow / 1024;         // 1 KB a wave and store
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int piece = i * 8 + wave, row = piece / kOf, off = piece % kOf * 1024 + lane * 16;
+            if (row < a.Mrec) *reinterpret_cast<u32x4 *>(to + static_cast<int64_t>(row) * kRecRow + off) = *reinterpret_cast<const u32x4 *>(lds + row * kRecLd + off);
+        }
+    }
 }
 
 // ------------------------------------------------------------------ uv
 struct UvArgs {
-    const float *part;
+    const void *part;
     const float2 *ml;
     const Head *head;
     const int2 *seq;
     const uint16_t *w_uv;       // [H, V, 512]
     void *out;                  // [B, Tall, H, V]
     const float *gate;          // the same, or null
-    int H, V, M, T, t0, Tall, G, GT, tiles, ptiles, Mrec, out_bf16;
+    int H, V, M, T, t0, Tall, G, GT, tiles, ptiles, Mrec, out_bf16, half;       // half: the records are fp16
+    Rows rows;
 };
 
 constexpr int kCLd = 1040;      // LDS bytes of a context row's term: 1024 + 16
@@ -877,7 +907,7 @@ constexpr int kCLd = 1040;      // LDS bytes of a context row's term: 1024 + 16
 struct Records {
     int first, low, n, step, tiles, in, pin, Mrec;
     __device__ __forceinline__ Records(const UvArgs &a, int m, int h) {
-        const int b = m / a.T, row = (m - b * a.T) * a.H + h, g = row >> 4, pg = b * a.G + g;
+        const int b = m / a.T, row = a.rows.of(m - b * a.T, h), g = row >> 4, pg = b * a.G + g;
         const int2 mine = a.seq[b];
         low = a.head->ranges, n = low + mine.y;
         first = mine.x + g / a.GT, step = a.ptiles, tiles = a.tiles, Mrec = a.Mrec;
@@ -888,12 +918,11 @@ struct Records {
 };
 
 // grid (H, ceil(M / PER)), eight waves: PER queries of head x.  A wave joins the records of a query (PER 1: eight waves every eighth record of 64), eight
-// columns a lane, and leaves the context in LDS as TERMS bf16 terms; then a wave takes 16 output columns of all queries, its rows of W_UV as they lie
-// (the first of them loaded before anything else).
+// columns a lane, and leaves the context in LDS as TERMS bf16 terms; then a wave takes 16 output columns of all queries, its rows of W_UV as they lie.
 template <int TERMS, int PER>
-__global__ __launch_bounds__(512) void uv_kernel(UvArgs a) {
+__global__ __launch_bounds__(512, PER > 8 ? 4 : 2) void uv_kernel(UvArgs a) {
     static_assert(PER == 1 || PER % 8 == 0, "waves to a query, or queries to a wave");
-    constexpr int kTiles = (PER + 15) / 16, kRows = PER < 16 ? PER : 16;
+    constexpr int kTiles = (PER + 15) / 16, kRows = PER < 16 ? PER : 16, kSide = PER > 8 ? 4 : 12;   // kSide: records on their way
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char *const ctx = lds;                                      // [TERMS][PER][kCLd]
     float *const sums = reinterpret_cast<float *>(lds + TERMS * PER * kCLd);    // PER 1: [8][512], then maxima and sums [8]
@@ -907,7 +936,6 @@ __global__ __launch_bounds__(512) void uv_kernel(UvArgs a) {
         for (int k = 0; k < 16; ++k)
             w[k] = __builtin_bit_cast(u32x4, buf_load16(rw, static_cast<uint32_t>(vt * 16 + r16) * (2 * kLat) + k * 64 + q4 * 16));
     };
-    weights(wave);
     // the context of columns 4 lane .. +4 and 256 + 4 lane .. +4
     auto store = [&](int i, f32x4 x, f32x4 y) __attribute__((always_inline)) {
 #pragma unroll
@@ -919,38 +947,66 @@ __global__ __launch_bounds__(512) void uv_kernel(UvArgs a) {
             y -= f32x4{q4_lo(o.x), q4_hi(o.x), q4_lo(o.y), q4_hi(o.y)};
         }
     };
+    // the row's records, and the maxima and sums of its first 64: sent for while the query before is joined
+    auto stats = [&](const Records &rec, int k) __attribute__((always_inline)) { return k < rec.n ? a.ml[rec.at(k)] : make_float2(-INFINITY, 0.f); };
+    auto query = [&](int i) __attribute__((always_inline)) { return Records(a, min(m0 + i, a.M - 1), h); };
+    Records next = query(PER == 1 ? 0 : wave);
+    float2 v_next = stats(next, lane);
+    if constexpr (PER <= 8) weights(wave);      // (behind what the join waits for; with more queries, two blocks a CU: the registers are the joins')
 #pragma unroll 1
     for (int i = PER == 1 ? 0 : wave; i < PER; i += 8) {
         f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-        float mx = -INFINITY, l = 0.f;
-        const int m = m0 + i;
-        if (m < a.M) {
-            const Records rec(a, m, h);
+        float l = 0.f;
+        const Records rec = next;
+        float2 v = v_next;
+        if (PER > 8 && i + 8 < PER) next = query(i + 8), v_next = stats(next, lane);
+        if (m0 + i < a.M) {
             // (the weight of a record that the row sees nothing of is zero, and what is written there does not matter)
-            auto stats = [&](int k) __attribute__((always_inline)) { return k < rec.n ? a.ml[rec.at(k)] : make_float2(-INFINITY, 0.f); };
-            float2 v = stats(lane);             // the first 64
-            mx = v.x;
-            for (int k0 = 64; k0 < rec.n; k0 += 64) mx = fmaxf(mx, stats(k0 + lane).x);
+            float mx = v.x;
+            for (int k0 = 64; k0 < rec.n; k0 += 64) mx = fmaxf(mx, stats(rec, k0 + lane).x);
             mx = wave_max_all(mx);
             for (int k0 = 0; k0 < rec.n; k0 += 64) {
-                if (k0) v = stats(k0 + lane);
+                if (k0) v = stats(rec, k0 + lane);
                 const int at = rec.at(min(k0 + lane, rec.n - 1)), n = min(rec.n - k0, 64);
                 const float f = v.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v.x - mx);
                 if (PER > 1 || wave == 0) l = fmaf(f, v.y, l);
-                constexpr int kSide = 8;                        // records on their way
+                // (fp16 records are contexts over their sums)
+                const float weight = TERMS == 2 && a.half ? f * v.y : f;
                 for (int j0 = PER == 1 ? wave * kSide : 0; j0 < n; j0 += PER == 1 ? 8 * kSide : kSide) {
-                    f32x4 c[kSide][2];
                     float g[kSide];
+                    int from[kSide];
 #pragma unroll
                     for (int j = 0; j < kSide; ++j) {
-                        const int from = __builtin_amdgcn_readlane(at, min(j0 + j, n - 1));
-                        g[j] = j0 + j < n ? readlane_f(f, j0 + j) : 0.f;
-                        const float *p = a.part + static_cast<int64_t>(from) * kLat + 4 * lane;
-                        c[j][0] = *reinterpret_cast<const f32x4 *>(p), c[j][1] = *reinterpret_cast<const f32x4 *>(p + 256);
+                        from[j] = __builtin_amdgcn_readlane(at, (j0 + j) & 63);
+                        g[j] = j0 + j < n ? readlane_f(weight, (j0 + j) & 63) : 0.f;
                     }
+                    if (TERMS == 2 && a.half) {
+                        u32x2 c[kSide][2] = {};
 #pragma unroll
-                    for (int j = 0; j < kSide; ++j)
-                        if (g[j] != 0.f) x += g[j] * c[j][0], y += g[j] * c[j][1];
+                        for (int j = 0; j < kSide; ++j) {
+                            const uint16_t *p = static_cast<const uint16_t *>(a.part) + static_cast<int64_t>(from[j]) * kLat + 4 * lane;
+                            if (j0 + j < n) c[j][0] = *reinterpret_cast<const u32x2 *>(p), c[j][1] = *reinterpret_cast<const u32x2 *>(p + 256);
+                        }
+#pragma unroll
+                        for (int j = 0; j < kSide; ++j)
+                            if (g[j] != 0.f) {
+                                float u[8];
+                                unpack2<true>(c[j][0].x, u[0], u[1]), unpack2<true>(c[j][0].y, u[2], u[3]);
+                                unpack2<true>(c[j][1].x, u[4], u[5]), unpack2<true>(c[j][1].y, u[6], u[7]);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) x[k] = fmaf(g[j], u[k], x[k]), y[k] = fmaf(g[j], u[4 + k], y[k]);
+                            }
+                    } else {
+                        f32x4 c[kSide][2] = {};
+#pragma unroll
+                        for (int j = 0; j < kSide; ++j) {
+                            const float *p = static_cast<const float *>(a.part) + static_cast<int64_t>(from[j]) * kLat + 4 * lane;
+                            if (j0 + j < n) c[j][0] = *reinterpret_cast<const f32x4 *>(p), c[j][1] = *reinterpret_cast<const f32x4 *>(p + 256);
+                        }
+#pragma unroll
+                        for (int j = 0; j < kSide; ++j)
+                            if (g[j] != 0.f) x += g[j] * c[j][0], y += g[j] * c[j][1];
+                    }
                 }
             }
             l = wave_sum_all(l);
@@ -976,17 +1032,21 @@ __global__ __launch_bounds__(512) void uv_kernel(UvArgs a) {
     }
     __syncthreads();
     for (int vt = wave; vt < vtiles; vt += 8) {
-        if (vt != wave) weights(vt);
-        f32x4 o[kTiles];
+        if (PER > 8 || vt != wave) weights(vt);
+        f32x4 o[kTiles], o2[kTiles];
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < kTiles; ++t) o[t] = o2[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int y = TERMS - 1; y >= 0; --y)
 #pragma unroll
             for (int k = 0; k < 16; ++k)
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t)
-                    o[t] = q4_mfma_bf16(w[k], *reinterpret_cast<const u32x4 *>(ctx + (y * PER + t * 16 + r16 % kRows) * kCLd + k * 64 + q4 * 16), o[t]);
+                for (int t = 0; t < kTiles; ++t) {
+                    f32x4 &to = k & 1 ? o2[t] : o[t];
+                    to = q4_mfma_bf16(w[k], *reinterpret_cast<const u32x4 *>(ctx + (y * PER + t * 16 + r16 % kRows) * kCLd + k * 64 + q4 * 16), to);
+                }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) o[t] += o2[t];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
             const int m = m0 + t * 16 + r16, v = vt * 16 + 4 * q4;
@@ -1011,8 +1071,15 @@ constexpr int64_t kPassRows = 1 << 16;      // rows (heads x queries, all sequen
 
 struct Plan {
     int NT, GT, T, G, tiles, ptiles, Mrec, most, turns;     // T: queries of a sequence in a pass
+    Rows rows;
     int64_t groups, qop, scales, part, ml, head, seq, item, total;
 };
+
+// By head where that adds a tenth of rows at most.
+Rows rows_of(int64_t T, int64_t H) {
+    const int64_t Tp = cdiv(T, 16) * 16;
+    return Rows{static_cast<int>(T), static_cast<int>(H), 10 * Tp <= 11 * T ? static_cast<int>(Tp) : 0};
+}
 
 // What the launches are cut into; a function of its arguments alone.
 Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t max_length, int64_t prefix, int cache_dtype, int out_dtype) {
@@ -1020,7 +1087,8 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t max_length, int64_t prefix
     p.NT = cache_dtype == K3_F16 && out_dtype == K3_BF16 ? 1 : 2;
     p.GT = 4 / p.NT;
     p.T = static_cast<int>(std::max<int64_t>(1, std::min(T, kPassRows / (B * H))));
-    p.G = static_cast<int>(cdiv(p.T * H, 16));
+    p.rows = rows_of(p.T, H);
+    p.G = static_cast<int>(cdiv(p.rows.count(), 16));
     p.tiles = static_cast<int>(cdiv(p.G, p.GT));
     p.groups = B * p.G;
     p.ptiles = prefix > 0 ? static_cast<int>(cdiv(p.groups, p.GT)) : 0;
@@ -1035,7 +1103,7 @@ Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t max_length, int64_t prefix
     p.qop = o, o += up(p.groups * p.NT * kSteps * kFrag);
     p.scales = o, o += up(p.groups * kParts * 16 * 4);
     p.ml = o, o += up(static_cast<int64_t>(p.most) * p.Mrec * 8);
-    p.part = o, o += up(static_cast<int64_t>(p.most) * p.Mrec * kLat * 4);
+    p.part = o, o += up(static_cast<int64_t>(p.most) * p.Mrec * kLat * (p.NT == 1 ? 2 : 4));
     p.head = o, o += 256;
     p.seq = o, o += up(B * 8);
     p.item = o, o += up(static_cast<int64_t>(p.most) * static_cast<int64_t>(sizeof(Item)));
@@ -1145,7 +1213,9 @@ extern "C" int k3_mla_paged_attention(const void *q_nope, int64_t qn_batch, int6
     const bool f16 = cache_dtype == K3_F16;
     for (int64_t t0 = 0; t0 < T; t0 += p.T) {
         // (the last pass may have fewer queries; it has the others' room)
-        const int Tp = static_cast<int>(std::min<int64_t>(p.T, T - t0)), G = static_cast<int>(cdiv(Tp * H, 16)), M = static_cast<int>(B * Tp);
+        const int Tp = static_cast<int>(std::min<int64_t>(p.T, T - t0)), M = static_cast<int>(B * Tp);
+        const Rows rows = Tp == p.T ? p.rows : Rows{Tp, static_cast<int>(H), 0};
+        const int G = static_cast<int>(cdiv(rows.count(), 16));
         const int tiles = static_cast<int>(cdiv(G, p.GT)), groups = static_cast<int>(B * G);
         const int ptiles = prefix_pages > 0 ? static_cast<int>(cdiv(groups, p.GT)) : 0;
         const Lists lists{lengths, counts, reinterpret_cast<Head *>(ws + p.head), reinterpret_cast<int2 *>(ws + p.seq),
@@ -1154,7 +1224,7 @@ extern "C" int k3_mla_paged_attention(const void *q_nope, int64_t qn_batch, int6
                           ptiles > 0 && G % p.GT == 0};
         const QaArgs qa{q_nope, q_rot, qn_batch, qn_token, qn_head, qr_batch, qr_token, qr_head, static_cast<const uint16_t *>(w_uk),
                         ws + p.qop, reinterpret_cast<float *>(ws + p.scales), static_cast<int>(H), static_cast<int>(nope_dim), M, Tp,
-                        static_cast<int>(t0), G, lists};
+                        static_cast<int>(t0), G, rows, lists};
         int rc = q_dtype == K3_BF16 ? launch_qa<uint16_t>(qa, f16, p.NT, st) : launch_qa<float>(qa, f16, p.NT, st);
         if (rc) return rc;
         AttendArgs a{};
@@ -1163,12 +1233,12 @@ extern "C" int k3_mla_paged_attention(const void *q_nope, int64_t qn_batch, int6
         a.lat_row = static_cast<uint32_t>(2 * lat_row), a.rot_row = static_cast<uint32_t>(2 * rot_row);
         a.table = table, a.prefix = prefix, a.table_row = table_row, a.pages = static_cast<int>(pages), a.shift = shift;
         a.lists = lists;
-        a.part = reinterpret_cast<float *>(ws + p.part), a.ml = reinterpret_cast<float2 *>(ws + p.ml);
-        a.H = static_cast<int>(H), a.G = G, a.groups = groups, a.Mrec = p.Mrec, a.c = scale * 1.4426950408889634f;
+        a.part = ws + p.part, a.ml = reinterpret_cast<float2 *>(ws + p.ml);
+        a.rows = rows, a.G = G, a.groups = groups, a.Mrec = p.Mrec, a.c = scale * 1.4426950408889634f;
         rc = !f16 ? launch_attend<false, 2>(a, p.most, st) : p.NT == 1 ? launch_attend<true, 1>(a, p.most, st) : launch_attend<true, 2>(a, p.most, st);
         if (rc) return rc;
-        const UvArgs u{a.part, a.ml, lists.head, lists.seq, static_cast<const uint16_t *>(w_uv), out, gate, a.H, static_cast<int>(v_dim), M, Tp,
-                       static_cast<int>(t0), static_cast<int>(T), G, p.GT, tiles, ptiles, p.Mrec, out_dtype == K3_BF16};
+        const UvArgs u{a.part, a.ml, lists.head, lists.seq, static_cast<const uint16_t *>(w_uv), out, gate, static_cast<int>(H), static_cast<int>(v_dim), M, Tp,
+                       static_cast<int>(t0), static_cast<int>(T), G, p.GT, tiles, ptiles, p.Mrec, out_dtype == K3_BF16, p.NT == 1, rows};
         rc = u.out_bf16 ? launch_uv<2>(u, st) : launch_uv<3>(u, st);
         if (rc) return rc;
     }

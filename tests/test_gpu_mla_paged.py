@@ -136,7 +136,7 @@ FORMS = [(F16, BF16, BF16), (F16, F32, F32), (BF16, BF16, BF16), (BF16, F32, F32
 @pytest.mark.parametrize("T,H,lens,prefix,page", [
     (1, 64, [1], 0, 64), (1, 16, [31, 32, 33], 0, 32), (1, 96, [700, 0, 65], 0, 64), (1, 8, [200] * 9, 0, 64), (3, 20, [130, 3, 2], 0, 64),
     (1, 64, [300, 257, 256, 0, 100], 256, 64), (2, 12, [64, 65, 66, 190, 1], 64, 32), (40, 16, [40, 100], 0, 128), (17, 5, [145, 141], 128, 32),
-    (1, 1, [1000], 0, 32), (1, 128, [2500, 2049], 2048, 1024),
+    (1, 1, [1000], 0, 32), (1, 128, [2500, 2049], 2048, 1024), (32, 3, [32, 100], 0, 32), (79, 5, [200, 150, 80], 64, 64), (64, 16, [64, 129], 0, 64),
 ])
 def test_attention(T, H, lens, prefix, page, pages, x, out):
     case = oracle.make(_gen(T * H + len(lens)), len(lens), T, H, lens, page=page, pages_dtype=pages, x=x, prefix=prefix)
