@@ -37,6 +37,10 @@ other call ``k3_mla_q4_attention`` on the codes, for all sequences of a batch at
 masked form over the decoded latents, and calls that a gradient is asked of are refused.  ``cfg.mla_cache_weights``
 (not the reference's) makes a new cache of this kind sum the attention its positions receive, which ``MLACacheQ4.evict``
 goes by.
+
+A caller's ``k3hip.mla_paged.MLACachePaged`` is the cache of a batch of requests in pages: the layer writes the step's tokens to
+the slots that ``PageTable.extend`` gave them and attends with ``k3_mla_paged_attention`` (fp16 or bf16 pages, bf16 ``kv_b``, no
+gradients), a common prefix read and multiplied once for the batch.
 """
 from __future__ import annotations
 
@@ -46,6 +50,7 @@ import torch
 
 from . import _blas, _lib, _workspace
 from . import _torch as T
+from .mla_paged import MLACachePaged
 from .mla_q4 import MLACacheQ4, new_cache_q4, scratch
 
 CACHE_STEP = 256
@@ -258,12 +263,12 @@ class MLAAttention:
             self._q_an32 = T.contiguous_aligned(self.q_an.to(torch.float32))
             self._kv_an32 = T.contiguous_aligned(self.kv_an.to(torch.float32))
 
-    def _check_q4(self) -> None:
-        """Refuses head sizes that the 4-bit cache's kernels do not take."""
+    def _check_q4(self, what: str = "4-bit") -> None:
+        """Refuses head sizes that the kernels of the 4-bit cache, or the paged one, do not take."""
         c = self.cfg
         if ((c.kv_lora_rank, c.qk_rope_head_dim) != (KV_LORA_RANK, ROPE_DIM) or c.qk_nope_head_dim % 8 or c.qk_nope_head_dim > 256
                 or c.v_head_dim % 8 or c.v_head_dim > 1024 or c.num_attention_heads > 4096):
-            raise ValueError(f"the 4-bit cache takes kv_lora_rank {KV_LORA_RANK}, qk_rope_head_dim {ROPE_DIM}, qk_nope_head_dim and "
+            raise ValueError(f"the {what} cache takes kv_lora_rank {KV_LORA_RANK}, qk_rope_head_dim {ROPE_DIM}, qk_nope_head_dim and "
                              f"v_head_dim multiples of 8 up to 256 and 1024, 4096 heads; got {c.kv_lora_rank}, {c.qk_rope_head_dim}, "
                              f"{c.qk_nope_head_dim}, {c.v_head_dim}, {c.num_attention_heads}")
 
@@ -280,9 +285,22 @@ class MLAAttention:
                 pass
         return a.to(torch.float32) @ w.to(torch.float32).T
 
-    def __call__(self, x: torch.Tensor, cache: MLACache | None = None):
+    def _check_paged(self, x: torch.Tensor, cache: MLACachePaged) -> None:
+        """Refuses what the paged cache's calls do not take, before any of them is made."""
+        self._check_q4("paged")
+        if self.kv_b.dtype != torch.bfloat16:
+            raise ValueError("the paged cache takes bf16 kv_b (the checkpoint dtype)")
+        if T.tracked(x, self.q_a, self.q_an, self.q_b, self.kv_a, self.kv_an, self.kv_b, self.g_w, self.o_w, cache.latent, cache.rot):
+            raise ValueError("the paged cache carries no gradient: call the layer under no_grad or on detached tensors")
+        if x.shape[:2] != cache.pages.slots.shape:
+            raise ValueError(f"{tuple(x.shape[:2])} tokens for slots of {tuple(cache.pages.slots.shape)}: call pages.extend for the step first")
+
+    def __call__(self, x: torch.Tensor, cache: MLACache | MLACacheQ4 | MLACachePaged | None = None):
         c = self.cfg
         B, Tn, _ = x.shape
+        paged = isinstance(cache, MLACachePaged)
+        if paged:
+            self._check_paged(x, cache)
         if cache is None and self.cache_bits == 4:
             cache = new_cache_q4(B, Tn, bool(getattr(c, "mla_cache_weights", False)), x.device)
         q4 = isinstance(cache, MLACacheQ4)
@@ -292,7 +310,7 @@ class MLAAttention:
             raise ValueError("the 4-bit cache carries no gradient: call the layer under no_grad or on detached tensors")
         if q4 and cache.weight is not None and self.kv_b.dtype != torch.bfloat16:
             raise ValueError("the masked form (fp32 kv_b) sums no attention weights: the cache must keep none")
-        if self.fused_step and B == 1 and Tn == 1 and (cache is None or (self.kv_b if q4 else cache.latent).dtype == torch.bfloat16):
+        if self.fused_step and B == 1 and Tn == 1 and not paged and (cache is None or (self.kv_b if q4 else cache.latent).dtype == torch.bfloat16):
             return self.decode_step(x, cache)
         nh, qhd, vhd = c.num_attention_heads, c.q_head_dim, c.v_head_dim
         nope, rope, klr = c.qk_nope_head_dim, c.qk_rope_head_dim, c.kv_lora_rank
@@ -301,13 +319,13 @@ class MLAAttention:
         mats = [self.q_a, self.kv_a] + ([self.g_w] if gated else [])
         xf = x.reshape(B * Tn, x.shape[-1])
         # (a gradient or tangent of anything the call reads takes the tensor form throughout)
-        rest = [self.q_an, self.kv_an, self.kv_b] + ([] if cache is None else [cache.rot] if q4 else [cache.latent, cache.rot])
+        rest = [self.q_an, self.kv_an, self.kv_b] + ([] if cache is None or paged else [cache.rot] if q4 else [cache.latent, cache.rot])
         if (B * Tn > 1 and _blas.dense_ok(xf, *mats) and _blas.weights_ok(self.q_b, self.o_w)
                 and not T.tracked(*rest)):
             qa, ckv, *g = _blas.project(xf, mats, checked=True)
             qa = _rmsnorm_rows(qa, self.q_an, eps)
             q = _blas.project(qa, [self.q_b], checked=True)[0].reshape(B, Tn, nh, qhd)
-            c_new = _rmsnorm_rows(ckv[:, :klr], self.kv_an, eps).reshape(B, Tn, klr)
+            c_new = ckv[:, :klr].reshape(B, Tn, klr) if paged else _rmsnorm_rows(ckv[:, :klr], self.kv_an, eps).reshape(B, Tn, klr)
             r_new = ckv[:, klr:].reshape(B, Tn, -1)
             gate = g[0].reshape(B, Tn, nh * vhd) if gated else None
             mm = lambda a, w: _blas.project(a.reshape(B * Tn, -1), [w])[0].reshape(B, Tn, -1)  # noqa: E731
@@ -315,8 +333,12 @@ class MLAAttention:
             mm = self._mm
             q = mm(_rmsnorm(mm(x, self.q_a), self.q_an, eps), self.q_b).reshape(B, Tn, nh, qhd)
             ckv = mm(x, self.kv_a)
-            c_new, r_new = _rmsnorm(ckv[..., :klr], self.kv_an, eps), ckv[..., klr:]
+            c_new, r_new = ckv[..., :klr] if paged else _rmsnorm(ckv[..., :klr], self.kv_an, eps), ckv[..., klr:]
             gate = mm(x, self.g_w) if gated else None
+        if paged:
+            cache.append(c_new, r_new, norm=self.kv_an, eps=eps)
+            o = cache.attend(q[..., :nope], q[..., nope:], self.wk, self.wv, qhd ** -0.5, gate)
+            return mm(o.reshape(B, Tn, nh * vhd), self.o_w), cache
         if cache is None:
             cache = new_cache(B, klr, rope, Tn, self.cache_dtype, x.device)
         cache.append(c_new, r_new)

@@ -45,7 +45,9 @@ def attention(q_nope, q_rot, wk, wv, lat, rot, table, lengths, scale, counts=Non
     The bound counts, with u a type's half step: the result's own rounding; six standard deviations of a score's error, whose terms
     (one for each column: u of the query terms times the product, independent) add as a root of squares, and of the probabilities'
     roundings, which add so over the positions; 2^-19 of the sum of magnitudes for the fp32 sums (576 and more products, 2^-24 each, and the
-    context's terms before W_UV, 2^-16 at a bf16 result)."""
+    context's terms before W_UV, 2^-16 at a bf16 result).  At a bf16 result over fp16 pages the contexts of ranges are fp16, over their sums: every
+    column of range i off by 2^-11 |c_i| at most, independently, weighed with the range's share w_i; sum_i w_i |c_i| is at most sum_j p_j |lat_j|, so
+    six deviations are 6 2^-11 of the root of the squares of W_UV times that."""
     f64 = torch.float64
     B, T, H, nope = q_nope.shape
     V, page, pool = wv.shape[1], lat.shape[1], lat.shape[0]
@@ -79,6 +81,8 @@ def attention(q_nope, q_rot, wk, wv, lat, rot, table, lengths, scale, counts=Non
             spread = torch.einsum("hj,hjv->hv", p * sigma, v.abs()) + (p * sigma).sum(-1, keepdim=True) * out.abs()
             weight = u_q * torch.einsum("hj,hjv->hv", p.square(), v.square()).sqrt()
             sums = torch.einsum("hj,hjr,hvr->hv", p, Ls.abs().expand(H, -1, -1), wv.to(f64).abs())
+            if not fine and lat.dtype == torch.float16:
+                weight = weight + u_q * torch.einsum("hr,hvr->hv", (p @ Ls.abs()).square(), wv.to(f64).square()).sqrt()
             bound[b, t] = 6 * (spread + weight) + sums * (2.0 ** -19 if fine else 2.0 ** -15)
             if gate is not None:
                 g = torch.sigmoid(gate[b, t].to(f64).reshape(H, V))

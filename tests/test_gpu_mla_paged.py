@@ -176,3 +176,265 @@ def test_attention_over_ranges_of_more_than_64_rounds(pages, out):
     got = _run(case, out_dtype=out)
     one = {k: v[5:6] if k in ("q_nope", "q_rot", "table", "lengths") else v for k, v in case.items()}
     _check(got[5:6], *oracle.attention(**one, out_dtype=out))
+
+
+# ------------------------------------------------------------------------------- what is masked, what is infinite
+@pytest.mark.parametrize("pages,out", [(F16, BF16), (F16, F32), (BF16, F32)])
+def test_what_is_masked_does_not_matter(pages, out):
+    # drafts: the first query does not see the last position, whatever it holds; a short request beside longer ones in the same tiles
+    case = oracle.make(_gen(3), 3, 4, 16, [100, 67, 66], pages_dtype=pages, prefix=64)
+    clean = _run(case, out_dtype=out)
+    _check(clean, *oracle.attention(**case, out_dtype=out))
+    for value in (math.nan, math.inf, -math.inf):
+        lat, rot = case["lat"].clone(), case["rot"].clone()
+        last = int(case["lengths"][0]) - 1
+        lat[case["table"][0, last // 64].long(), last % 64, ::7] = value
+        rot[case["table"][0, last // 64].long(), last % 64] = value
+        got = _run({**case, "lat": lat, "rot": rot}, out_dtype=out)
+        assert bool(got[0, 3].isnan().all()) and bool((got[0, :3] == clean[0, :3]).all()) and bool((got[1:] == clean[1:]).all())
+    # a position of the common prefix: every query that sees it, and none that does not (the third request, cut to 20)
+    case["lengths"][2] = 20
+    clean = _run(case, out_dtype=out)
+    lat = case["lat"].clone()
+    lat[case["prefix"][0].long(), 40, 5] = math.inf
+    got = _run({**case, "lat": lat}, out_dtype=out)
+    assert bool(got[:2].isnan().all()) and bool((got[2] == clean[2]).all())
+
+
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_a_query_that_is_not_finite_is_alone(out):
+    case = oracle.make(_gen(4), 2, 2, 20, [90, 40], x=F32)
+    clean = _run(case, out_dtype=out)
+    q = case["q_nope"].clone()
+    q[0, 1, 3, 17], q[1, 0, 0, 0] = math.nan, math.inf
+    got = _run({**case, "q_nope": q}, out_dtype=out)
+    assert bool(got[0, 1, 3].isnan().all()) and bool(got[1, 0, 0].isnan().all())
+    got[0, 1, 3], got[1, 0, 0] = clean[0, 1, 3], clean[1, 0, 0]
+    assert bool((got == clean).all())
+
+
+def test_queries_that_see_nothing_are_zero():
+    case = oracle.make(_gen(5), 4, 3, 8, [40, 5, 2, 64])
+    case["lengths"][0] = 0
+    case["lengths"][3] = -9
+    got = _run(case, counts=torch.tensor([3, 3, 3, 3], dtype=I32, device="cuda"))
+    assert not bool(got[0].any()) and not bool(got[3].any()) and not bool(got[2, 0].any()) and bool(got[2, 1:].all())
+    none = _run(case, counts=torch.zeros(4, dtype=I32, device="cuda"))
+    assert not bool(none.any())
+    empty = {**case, "table": case["table"][:, :0].contiguous()}
+    assert not bool(_run(empty).any())
+
+
+@pytest.mark.parametrize("pages,out", [(F16, BF16), (F16, F32), (BF16, BF16)])
+def test_pages_outside_the_pool_count_as_not_there(pages, out):
+    case = oracle.make(_gen(6), 3, 1, 16, [200, 130, 64], pages_dtype=pages)
+    for b, k, p in ((0, 0, -1), (0, 2, case["lat"].shape[0]), (1, 1, -2 ** 31), (2, 0, 2 ** 31 - 1)):
+        case["table"][b, k] = p
+    want, bound = oracle.attention(**case, out_dtype=out)
+    got = _run(case, out_dtype=out)
+    _check(got, want, bound)
+    assert not bool(got[2].any())
+
+
+# ------------------------------------------------------------------------------- sizes of the values
+@pytest.mark.parametrize("out", [BF16, F32])
+@pytest.mark.parametrize("size", [1e-30, 1e-4, 1e25])
+def test_queries_of_any_size(size, out):
+    # the scale takes the size back, so scores are as ever
+    case = oracle.make(_gen(7), 2, 1, 16, [150, 33], x=F32)
+    case["q_nope"], case["q_rot"], case["scale"] = case["q_nope"] * size, case["q_rot"] * size, case["scale"] / size
+    want, bound = oracle.attention(**case, out_dtype=out)
+    _check(_run(case, out_dtype=out), want, bound)
+
+
+def test_parts_of_a_query_of_unequal_size():
+    # no rotary part, or one that is 2^20 times the rest: each has its scale
+    case = oracle.make(_gen(8), 2, 1, 16, [150, 33], x=F32)
+    for nope, rot in ((1.0, 0.0), (0.0, 1.0), (2.0 ** -20, 1.0), (1.0, 2.0 ** -20)):
+        c = {**case, "q_nope": case["q_nope"] * nope, "q_rot": case["q_rot"] * rot}
+        for out in (BF16, F32):
+            want, bound = oracle.attention(**c, out_dtype=out)
+            # (a part below 2^-38 of the row's largest is not there: here 2^-20 of it stays, with 2^-18 of its own accuracy)
+            _check(_run(c, out_dtype=out), want, bound)
+
+
+@pytest.mark.parametrize("pages,out", [(F16, BF16), (F16, F32), (BF16, BF16)])
+def test_scores_that_keep_growing(pages, out):
+    # every round exceeds all before it by far, in either half of it, so the reference moves again and again; and the other way round
+    case = oracle.make(_gen(9), 2, 1, 20, [640, 639], pages_dtype=pages, x=F32)
+    ramp = torch.linspace(0, 400, 640, device="cuda")
+    for order in (ramp, ramp.flip(0), ramp.roll(17)):
+        rot = case["rot"].clone()
+        for b in range(2):
+            pos = torch.arange(int(case["lengths"][b]), device="cuda")
+            rot[case["table"][b, pos // 64].long(), pos % 64, 0] = order[pos].to(pages)
+        q_rot = case["q_rot"].clone()
+        q_rot[..., 0] = 192 ** 0.5
+        c = {**case, "rot": rot, "q_rot": q_rot}
+        want, bound = oracle.attention(**c, out_dtype=out)
+        _check(_run(c, out_dtype=out), want, bound)
+
+
+# ------------------------------------------------------------------------------- layouts
+def test_layouts_and_strides():
+    case = oracle.make(_gen(10), 3, 2, 12, [100, 31, 65], x=F32)
+    want = _run(case)
+    P = case["lat"].shape[0]
+    both = torch.cat((case["lat"], case["rot"], case["rot"]), -1)                # one pool of wider rows
+    wide = torch.full((3, 9), 77, dtype=I32, device="cuda")
+    wide[:, 3:3 + case["table"].shape[1]] = case["table"]
+    across = torch.stack((case["lat"], case["lat"]), 1)[:, 1]                    # pages further apart
+    q = torch.cat((case["q_nope"], case["q_rot"]), -1)
+    for c in (dict(lat=both[..., :512], rot=both[..., 512:576]), dict(table=wide[:, 3:3 + case["table"].shape[1]]), dict(lat=across),
+              dict(q_nope=case["q_nope"].transpose(1, 2).contiguous().transpose(1, 2)),
+              dict(q_nope=torch.cat((q[..., :1], q[..., :128]), -1)[..., 1:], q_rot=q.flip(-1).flip(-1)[..., 128:]),
+              dict(wk=case["wk"].transpose(0, 1).contiguous().transpose(0, 1)), dict(max_length=int(case["lengths"].max()))):
+        assert bool((_run({**case, **c}) == want).all()), list(c)
+    assert P == across.shape[0]
+    # a first half of the queries that is cut from a larger batch
+    part = {**case, **{k: case[k][1:] for k in ("q_nope", "q_rot", "table", "lengths")}}
+    _check(_run(part), *oracle.attention(**part))
+
+
+def test_max_length_cuts():
+    case = oracle.make(_gen(11), 2, 1, 8, [100, 50])
+    cut = {**case, "lengths": case["lengths"].clamp(max=70)}
+    assert bool((_run(case, max_length=70) == _run(cut)).all())
+    long = {**case, "lengths": torch.tensor([10 ** 9, 50], dtype=I32, device="cuda"), "table": case["table"][:, :1].contiguous()}
+    assert bool((_run(long) == _run({**long, "lengths": torch.tensor([64, 50], dtype=I32, device="cuda")})).all())
+
+
+def test_a_pool_of_more_than_4_gib():
+    # the pages in use lie behind 2^31 and 2^32 bytes
+    pages = (1 << 32) // (64 * 1024) + 40
+    case = oracle.make(_gen(12), 2, 1, 16, [130, 64], spare=0)
+    lat = torch.empty(pages, 64, 512, dtype=F16, device="cuda")
+    rot = torch.empty(pages, 64, 64, dtype=F16, device="cuda")
+    n = case["lat"].shape[0]
+    to = torch.tensor([pages - 1, (1 << 31) // (64 * 1024) + 1, pages - 20, 7, pages - 3][:n], device="cuda")
+    lat[to], rot[to] = case["lat"], case["rot"]
+    moved = {**case, "lat": lat, "rot": rot, "table": torch.where(case["table"] >= 0, to[case["table"].clamp(min=0).long()].to(I32), case["table"])}
+    assert bool((_run(moved) == _run(case)).all())
+    from k3hip.mla_paged import mla_paged_append
+    slot = torch.tensor([[(pages - 1) * 64 + 63]], dtype=I32, device="cuda")
+    mla_paged_append(torch.full((1, 1, 512), 3.0, device="cuda"), torch.full((1, 1, 64), 4.0, device="cuda"), slot, lat, rot)
+    assert bool((lat[-1, 63] == 3).all()) and bool((rot[-1, 63] == 4).all()) and bool((lat[-1, 62] == case["lat"][0, 62]).all())
+
+
+# ------------------------------------------------------------------------------- many
+def _sampled(case, got, which, out, **kw):
+    for b in which:
+        one = {k: v[b:b + 1] if k in ("q_nope", "q_rot", "table", "lengths") else v for k, v in case.items()}
+        _check(got[b:b + 1], *oracle.attention(**one, out_dtype=out, **kw), label=b)
+
+
+@pytest.mark.parametrize("B,H,T,out", [(1100, 64, 1, BF16), (1500, 8, 1, F32), (40, 64, 33, BF16), (3, 96, 300, BF16), (2, 64, 70, F32)])
+def test_many_rows(B, H, T, out):
+    # batches in parts, more sequences than the list's lengths are searched for, queries in passes (and a last pass of few)
+    g = _gen(B)
+    lens = [int(n) for n in torch.randint(0, 3 * T + 90, (B,), generator=g)]
+    lens[0], lens[-1] = 3 * T + 90, 1
+    case = oracle.make(g, B, T, H, lens, page=32)
+    got = _run(case, out_dtype=out)
+    _sampled(case, got, {0, 1, B // 2, B - 1}, out)
+
+
+def test_many_rows_behind_a_prefix():
+    g = _gen(2)
+    case = oracle.make(g, 700, 1, 24, [96 + b % 70 for b in range(700)], page=32, prefix=96)
+    case["lengths"][5] = 0
+    for out in (BF16, F32):
+        got = _run(case, out_dtype=out)
+        _sampled(case, got, (0, 5, 6, 350, 699), out)
+
+
+def test_the_same_bits_every_time():
+    for out in (BF16, F32):
+        case = oracle.make(_gen(14), 24, 2, 16, [600 + 40 * b for b in range(24)], prefix=512)
+        first = _run(case, out_dtype=out)
+        for _ in range(3):
+            assert bool((_run(case, out_dtype=out) == first).all())
+
+
+# ------------------------------------------------------------------------------- streams and graphs
+def test_another_stream():
+    case = oracle.make(_gen(15), 8, 1, 16, [500 + b for b in range(8)])
+    want = _run(case)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [_run(case) for _ in range(3)]
+    assert all(bool((_run(case) == want).all()) for _ in range(3))
+    side.synchronize()
+    assert all(bool((g == want).all()) for g in got)
+
+
+def test_a_captured_step_follows_the_lengths():
+    """Tables, append and attention of a step in one graph, replayed while requests grow, with eager work between."""
+    from k3hip.mla_paged import new_cache_paged
+    from k3hip.pages import PageTable
+    g = _gen(16)
+    H, B = 16, 5
+    case = oracle.make(g, B, 1, H, [1] * B, x=F32)
+    start = torch.tensor([0, 63, 64, 100, 31], dtype=I32, device="cuda")
+
+    def fresh():
+        t = PageTable(B, 512, 30, page_size=64)
+        c = new_cache_paged(t, F16)
+        t.extend(start, tokens=100)
+        data = torch.Generator().manual_seed(3)
+        c.append(torch.randn(B, 100, 512, generator=data).cuda(), torch.randn(B, 100, 64, generator=data).cuda())
+        return t, c
+
+    def step(t, c, new, q):
+        t.extend(1)
+        c.append(new[..., :512], new[..., 512:], norm=torch.ones(512, device="cuda"))
+        return c.attend(q[..., :128], q[..., 128:], case["wk"], case["wv"], 192 ** -0.5)
+
+    news = [torch.randn(B, 1, 576, generator=g).cuda() for _ in range(7)]
+    qs = [torch.randn(B, 1, H, 192, generator=g).cuda() for _ in range(7)]
+    t, c = fresh()
+    eager = [step(t, c, n, q).clone() for n, q in zip(news, qs)]
+    lengths = t.lengths.clone()
+
+    t2, c2 = fresh()
+    new, q = news[0].clone(), qs[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                       # (a warm-up on tables of its own)
+        step(*fresh(), new, q)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t2.extend(1)
+        c2.append(new[..., :512], new[..., 512:], norm=torch.ones(512, device="cuda"))
+        out = c2.attend(q[..., :128], q[..., 128:], case["wk"], case["wv"], 192 ** -0.5)
+    for i in range(7):
+        new.copy_(news[i]), q.copy_(qs[i])
+        graph.replay()
+        other = _run(case)                              # (eager work on the same stream, with a workspace of its own)
+        torch.cuda.synchronize()
+        assert bool((out == eager[i]).all()), i
+        assert bool(torch.isfinite(other).all())
+    assert bool((t2.lengths == lengths).all()) and bool((t2.table == t.table).all())
+
+
+def test_two_captured_calls_have_scratch_of_their_own():
+    a = oracle.make(_gen(17), 6, 1, 16, [900 + b for b in range(6)])
+    b = oracle.make(_gen(18), 6, 1, 16, [100 + 80 * b for b in range(6)])
+    want = _run(a), _run(b)
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for c in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = _run(c)
+        graphs.append(g), outs.append(o)
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(bool((o == w).all()) for o, w in zip(outs, want))
+        for o in outs:
+            o.zero_()
