@@ -18,8 +18,7 @@
 // launch has one of them), and all to the row's largest scale as attend takes them in, so fp16's range is no question of the queries' size: what
 // falls below fp16's last bit then is 2^-38 of the row's largest.  Probabilities are 2^kLift times
 // those of the row's reference, which moves when one would exceed 2^kTop: so fp16 holds them, and its last bit is
-// 2^-31 of the largest; an item's context, over its sum, goes to the join as fp16 (2^-11).  Two terms: as fp32.  bf16 pages multiply as bf16, exact, against two terms of both (2^-16), as the core over one sequence's cache
-// does.
+// 2^-31 of the largest; an item's context, over its sum, goes to the join as fp16 (2^-11).  Two terms: as fp32.  bf16 pages multiply as bf16, exact, against two terms of both for a bf16 result (2^-16), three for fp32 (2^-24).
 #include <algorithm>
 #include <type_traits>
 
@@ -489,16 +488,17 @@ __device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcn
 //           it holds as an operand of the second product.  The two waves of a row keep one reference: a wave that finds a score too far above
 //           it says so, and at the start of the next round all waves know, and wait while the round's probabilities are formed again.
 //   context waves (4 .. 7): ctx^T[column][row] += rows^T P^T, 128 columns each, from transposed reads of the staged rows.
-// GT = 4 / NT groups of 16 rows: with two terms the probabilities' second terms are rows of their own for the context waves, and the context
-// is their sum.
+// GT = 4 / NT groups of 16 rows: with more terms the probabilities' further terms are rows of their own for the context waves, and the context
+// is their sum.  With three, the scores of the queries' third terms are formed by the other two score waves and join the others through LDS.
 template <bool F16, int NT>
 __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
-    constexpr int GT = 4 / NT, kRows = 16 * GT, GR = 2 / NT;     // GR: groups of rows of a score wave
+    constexpr int GT = 4 / NT, VG = GT * NT, kRows = 16 * GT, GR = NT == 1 ? 2 : 1;      // GR: groups of rows of a score wave
     constexpr int kRecRow = kLat * (NT == 1 ? 2 : 4), kRecLd = kRecRow + 16;    // bytes of a record's row
-    static_assert(kRows * kRecLd <= kSlots * kSlotBytes && kRows * kRecRow == 64 * 1024, "the records fit the rounds' room");
+    static_assert(kRows * kRecLd <= kSlots * kSlotBytes && kRows * kRecRow % (8 * 1024) == 0, "the records fit the rounds' room");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int limits[64];
     __shared__ float xm[2][2][64];              // largest exponents [parity][half of the round][row], where a reference has to move
+    __shared__ f32x4 xs[NT == 3 ? 2 : 1][64];   // the third terms' scores [half of the round][lane]
     __shared__ float xf[64];                    // factors of the rows whose reference moved
     __shared__ __attribute__((aligned(16))) int need[4][4];     // [round % 4][score wave]: a reference has to move
     char *const pbuf = lds + kSlots * kSlotBytes;
@@ -591,16 +591,21 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         // ================= score waves
         constexpr int kAhead = 6;
         const int rg = wave & 1, pt = wave >> 1;            // operands 2 rg and 2 rg + 1; positions 16 pt .. +16 of a round
+        const bool main = NT < 3 || rg == 0;                // (three terms: the third's waves give their scores to the others')
         u32x4 q[2][kSteps];                                 // [operand]: two groups of rows, or a group's two terms
         float fac[GR];
         int limit[GR];
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
-            const int grp = (2 * rg + o) / NT, term = NT == 2 ? o : 0;
+            const int grp = NT == 3 ? 0 : (2 * rg + o) / NT, term = NT == 3 ? 2 * rg + o : NT == 2 ? o : 0;
             const int gidx = min((seq >= 0 ? seq * a.G : 0) + tile * GT + grp, a.groups - 1);
-            const char *qp = a.qop + (static_cast<int64_t>(gidx) * NT + term) * (kSteps * kFrag) + lane * 16;
+            const char *qp = a.qop + (static_cast<int64_t>(gidx) * NT + min(term, NT - 1)) * (kSteps * kFrag) + lane * 16;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) q[o][k] = *reinterpret_cast<const u32x4 *>(qp + k * kFrag);
+            if (NT == 3 && term == 3) {
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) q[o][k] = u32x4{0, 0, 0, 0};
+            }
             float top = 1.f;
             if constexpr (F16) {        // to the row's one scale: exact, but for what comes below fp16's last bit
                 float part[kParts];
@@ -663,7 +668,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                             pr[2 * i] -= u, pr[2 * i + 1] -= w;
                         }
                     }
-                    *reinterpret_cast<u32x2 *>(to + (NT == 2 ? y : g) * kFrag) = o;
+                    *reinterpret_cast<u32x2 *>(to + (NT == 1 ? g : y) * kFrag) = o;
                     if constexpr (F16 && NT == 1) {     // (the sum of what is multiplied: the roundings of a probability that takes all cancel)
                         const f16x2 one = {1, 1};
                         l_new[g] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, static_cast<uint32_t>(o.x)), one,
@@ -704,7 +709,9 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 }
             }
             {
-                if (again) {
+                if (again && !main) {
+                    block_barrier();
+                } else if (again) {
                     const u32x4 n = needed(rd - 1);
                     const bool me = (pt ? (rg ? n.w : n.z) : (rg ? n.y : n.x)) != 0, other = (pt ? (rg ? n.y : n.x) : (rg ? n.w : n.z)) != 0;
 #pragma unroll
@@ -729,12 +736,18 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 for (int g = 0; g < GR; ++g) l_run[g] += l_new[g];
             }
             if (rd < nr) {
+                if constexpr (NT == 3) {
+                    if (!main) xs[pt][lane] = acc[0];
+                    block_barrier();
+                    if (main) acc[1] += xs[pt][lane];
+                }
+                if (main) {
                 const int base = t_begin + rd * kRound + 16 * pt + 4 * q4;
                 const bool mixed = !in0 || t_begin + (rd + 1) * kRound > t_all;
 #pragma unroll
                 for (int g = 0; g < GR; ++g)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) e[g][i] = fmaf(NT == 2 ? acc[0][i] + acc[1][i] : acc[g][i], fac[g], -from[g]);
+                    for (int i = 0; i < 4; ++i) e[g][i] = fmaf(NT > 1 ? acc[0][i] + acc[1][i] : acc[g][i], fac[g], -from[g]);
                 if (mixed) {
 #pragma unroll
                     for (int g = 0; g < GR; ++g)
@@ -757,6 +770,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                     }
                 }
                 publish(rd);
+                }
                 __builtin_amdgcn_s_setprio(0);
             }
             in0 = in1, in1 = r_lat.z != 0;
@@ -766,7 +780,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
             const float l = q4_rows_sum(l_run[g]);
-            if (q4 == 0) (pt ? xf : xm[0][0])[(GR * rg + g) * 16 + r16] = l;
+            if (main && q4 == 0) (pt ? xf : xm[0][0])[(GR * rg + g) * 16 + r16] = l;
             l_run[g] = l;
         }
         block_barrier();
@@ -774,18 +788,18 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
             const int row = (GR * rg + g) * 16 + r16;
-            if (pt == 0 && q4 == 0 && row < a.Mrec)
+            if (main && pt == 0 && q4 == 0 && row < a.Mrec)
                 ml[row] = limit[g] > t_begin ? make_float2(from[g], l_run[g] + xf[row]) : make_float2(-INFINITY, 0.f);
         }
     } else {
         // ================= context waves
         constexpr int kAhead = 5;
         const int cw = wave - 4;
-        f32x4 acc[8][4];                        // [16 columns][16 (row, term)s]
+        f32x4 acc[8][VG];                       // [16 columns][16 (row, term)s]
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) acc[n][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int g = 0; g < VG; ++g) acc[n][g] = f32x4{0.f, 0.f, 0.f, 0.f};
         stage(0, true);
         in0 = r_lat.z != 0;
         stage(1, true);
@@ -805,15 +819,15 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
             } else {
                 const char *const pb = pbuf + ((rd - 1) & 1) * kPBytes + lane * 16;
                 const u32x4 raw = needed(rd - 1);
-                u32x4 p[4];
+                u32x4 p[VG];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) p[g] = *reinterpret_cast<const u32x4 *>(pb + g * kFrag);
+                for (int g = 0; g < VG; ++g) p[g] = *reinterpret_cast<const u32x4 *>(pb + g * kFrag);
                 if (any_of(raw)) {
                     block_barrier();
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) p[g] = *reinterpret_cast<const u32x4 *>(pb + g * kFrag);
+                    for (int g = 0; g < VG; ++g) p[g] = *reinterpret_cast<const u32x4 *>(pb + g * kFrag);
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
+                    for (int g = 0; g < VG; ++g) {
                         const float f = xf[g / NT * 16 + r16];
 #pragma unroll
                         for (int n = 0; n < 8; ++n) acc[n][g] *= f;
@@ -826,13 +840,14 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                     if (n + kAhead < 8) columns(rd - 1, n + kAhead, ring[n % kAhead]);
                     const u32x4 v = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) acc[n][g] = mfma<F16>(v, p[g], acc[n][g]);
+                    for (int g = 0; g < VG; ++g) acc[n][g] = mfma<F16>(v, p[g], acc[n][g]);
                     __builtin_amdgcn_sched_barrier(0);
                     if (n == 0) prepare(rd + 2, true);
                     if (n >= 1 && n < 5) stage_row(n - 1);
                     if (n == 5) stage_rot();
                 }
             }
+            if (NT == 3 && rd < nr) block_barrier();        // (the third terms' scores)
             // round rd's rows, which the score waves have: their first operands, while this wave would wait
             if (rd < nr && (!in0 || t_begin + (rd + 1) * kRound > t_all)) {
                 // some row does not see all of it: what it does not see must not reach it, not even as 0 x infinity
@@ -872,7 +887,11 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 }
             } else {
 #pragma unroll
-                for (int n = 0; n < 8; ++n) *reinterpret_cast<f32x4 *>(to + n * 64) = acc[n][g * NT] + acc[n][g * NT + 1];
+                for (int n = 0; n < 8; ++n) {
+                    f32x4 o = acc[n][g * NT] + acc[n][g * NT + 1];
+                    if constexpr (NT == 3) o += acc[n][2];
+                    *reinterpret_cast<f32x4 *>(to + n * 64) = o;
+                }
             }
         }
     }
@@ -881,7 +900,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         char *const to = static_cast<char *>(a.part) + static_cast<int64_t>(at) * a.Mrec * kRecRow;
         constexpr int kOf = kRecRow / 1024;         // 1 KB a wave and store
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kRows * kOf / 8; ++i) {
             const int piece = i * 8 + wave, row = piece / kOf, off = piece % kOf * 1024 + lane * 16;
             if (row < a.Mrec) *reinterpret_cast<u32x4 *>(to + static_cast<int64_t>(row) * kRecRow + off) = *reinterpret_cast<const u32x4 *>(lds + row * kRecLd + off);
         }
@@ -1084,7 +1103,7 @@ Rows rows_of(int64_t T, int64_t H) {
 // What the launches are cut into; a function of its arguments alone.
 Plan plan_of(int64_t B, int64_t T, int64_t H, int64_t max_length, int64_t prefix, int cache_dtype, int out_dtype) {
     Plan p{};
-    p.NT = cache_dtype == K3_F16 && out_dtype == K3_BF16 ? 1 : 2;
+    p.NT = (cache_dtype == K3_F16 ? 1 : 2) + (out_dtype == K3_F32);
     p.GT = 4 / p.NT;
     p.T = static_cast<int>(std::max<int64_t>(1, std::min(T, kPassRows / (B * H))));
     p.rows = rows_of(p.T, H);
@@ -1123,6 +1142,7 @@ int launch_qa_of(const QaArgs &a, hipStream_t st) {
 }
 template <typename QT>
 int launch_qa(const QaArgs &a, bool f16, int NT, hipStream_t st) {
+    if (NT == 3) return a.M > 32 ? launch_qa_of<QT, false, 3, 4>(a, st) : launch_qa_of<QT, false, 3, 1>(a, st);
     if (!f16) return a.M > 32 ? launch_qa_of<QT, false, 2, 4>(a, st) : launch_qa_of<QT, false, 2, 1>(a, st);
     if (NT == 1) return a.M > 32 ? launch_qa_of<QT, true, 1, 4>(a, st) : launch_qa_of<QT, true, 1, 1>(a, st);
     return a.M > 32 ? launch_qa_of<QT, true, 2, 4>(a, st) : launch_qa_of<QT, true, 2, 1>(a, st);
@@ -1235,7 +1255,7 @@ extern "C" int k3_mla_paged_attention(const void *q_nope, int64_t qn_batch, int6
         a.lists = lists;
         a.part = ws + p.part, a.ml = reinterpret_cast<float2 *>(ws + p.ml);
         a.rows = rows, a.G = G, a.groups = groups, a.Mrec = p.Mrec, a.c = scale * 1.4426950408889634f;
-        rc = !f16 ? launch_attend<false, 2>(a, p.most, st) : p.NT == 1 ? launch_attend<true, 1>(a, p.most, st) : launch_attend<true, 2>(a, p.most, st);
+        rc = p.NT == 3 ? launch_attend<false, 3>(a, p.most, st) : !f16 ? launch_attend<false, 2>(a, p.most, st) : p.NT == 1 ? launch_attend<true, 1>(a, p.most, st) : launch_attend<true, 2>(a, p.most, st);
         if (rc) return rc;
         const UvArgs u{a.part, a.ml, lists.head, lists.seq, static_cast<const uint16_t *>(w_uv), out, gate, static_cast<int>(H), static_cast<int>(v_dim), M, Tp,
                        static_cast<int>(t0), static_cast<int>(T), G, p.GT, tiles, ptiles, p.Mrec, out_dtype == K3_BF16, p.NT == 1, rows};

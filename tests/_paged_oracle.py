@@ -52,7 +52,7 @@ def attention(q_nope, q_rot, wk, wv, lat, rot, table, lengths, scale, counts=Non
     B, T, H, nope = q_nope.shape
     V, page, pool = wv.shape[1], lat.shape[1], lat.shape[0]
     fine = out_dtype == torch.float32
-    u_q = 2.0 ** -16 if lat.dtype == torch.bfloat16 else 2.0 ** -22 if fine else 2.0 ** -11
+    u_q = (2.0 ** -24 if fine else 2.0 ** -16) if lat.dtype == torch.bfloat16 else 2.0 ** -22 if fine else 2.0 ** -11
     o, bound = (torch.zeros(B, T, H, V, dtype=f64, device=lat.device) for _ in range(2))
     n_prefix = 0 if prefix is None else len(prefix)
     for b in range(B):

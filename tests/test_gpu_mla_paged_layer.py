@@ -4,7 +4,7 @@ against the layer over a cache of its own (tests/test_gpu_mla.py checks that one
 What the layer computes around the core are fp32 sums of at most 1024 products, three of them one after the other, whose errors are independent:
 sqrt(1024) 2^-24 = 2e-6 each, normwise.  The core, fp32 result: fp16 pages hold latents and rotary values to 2^-11, bf16 pages to 2^-8, and each position's
 rounding is its own; a result is a mean of positions and its scores (of size 8 at most) take 2^-11 x 8 / sqrt(576) of it, so what a page's type makes of
-a result is below 4 roundings: 4 x 2^-11 and 4 x 2^-8 against unrounded caches.  Over the pages' own values: 2^-16 (bf16: two terms) x 8."""
+a result is below 4 roundings: 4 x 2^-11 and 4 x 2^-8 against unrounded caches.  Over the pages' own values: 2^-22 x 8."""
 from __future__ import annotations
 
 from types import SimpleNamespace
@@ -85,7 +85,7 @@ def test_a_batch_of_requests(dtype, x_dtype, heads, gate):
                 continue
             alone, own[b] = layer(x[b:b + 1, :n], own[b])
             want = _want(w, heads, x[b, :n], *_rows(cache, b), gate)
-            assert _rel(out[b, :n], want) < 2e-5 + 8 * (2.0 ** -16 if dtype == BF16 else 2.0 ** -22)
+            assert _rel(out[b, :n], want) < 2e-5
             assert _rel(out[b, :n], alone[0].double()) < page_tol
             assert not bool(out[b, n:].any())
 
