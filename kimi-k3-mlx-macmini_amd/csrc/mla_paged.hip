@@ -287,7 +287,9 @@ __device__ __forceinline__ void scale_of(uint32_t top, float &s, float &inverse)
     inverse = top == 0u ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
 }
 
-// grid (H, ceil(M / (16 MT)), 4 or 5): queries 16 MT y .. of head x, latent columns 128 z .. +128; z = 4: the list of items.
+// A block: queries 16 MT y .. of head h, latent columns 128 z .. +128, all heads of a (y, z) after one another; and before them all
+// one for the list of items.  Blocks b % 8 run on one XCD.  Rows by query: an eighth of the blocks in a row goes to each, so the heads that share an
+// operand's 128-byte lines meet in one L2 (64 requests of 64 heads 10.7 -> 9.0 us, 120 16.0 -> 13.9); by head every head is on one XCD, with its matrix.
 // MT 1: few queries, a wave to 32 of the columns; MT 4: a wave to 16 of the queries.
 template <typename QT, bool F16, int NT, int MT>
 __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
@@ -295,11 +297,13 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     float *const fs = reinterpret_cast<float *>(lds);                   // [16 MT][kFLd], after the products
     constexpr int kTerms = std::is_same<QT, float>::value ? 3 : 1, kAhead = 4, kTiles = MT == 1 ? 2 : 8;    // column tiles of a wave
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q4 = lane >> 4;
-    const int h = blockIdx.x, m0 = blockIdx.y * 16 * MT, quarter = blockIdx.z;
-    if (quarter == 4) {
-        if (h == 0 && m0 == 0) list_items(a.lists, reinterpret_cast<int *>(lds));
+    const int blocks = gridDim.x - 1;
+    if (blockIdx.x == 0) {
+        list_items(a.lists, reinterpret_cast<int *>(lds));
         return;
     }
+    const int id = static_cast<int>(blockIdx.x) - 1, b = blocks % 8 || a.rows.Tp ? id : (id & 7) * (blocks >> 3) + (id >> 3);
+    const int h = b % a.H, m0 = b / a.H / 4 * 16 * MT, quarter = b / a.H % 4;
     const int steps = (a.nope + 31) >> 5;
     const uint16_t *w = a.w_uk + static_cast<int64_t>(h) * a.nope * kLat + quarter * 128;
     const int qt = MT == 1 ? 0 : wave, col = MT == 1 ? wave * 32 : 0, mine = m0 + 16 * qt + r16;    // the wave's queries and columns
@@ -939,9 +943,9 @@ struct Records {
 // grid (H, ceil(M / PER)), eight waves: PER queries of head x.  A wave joins the records of a query (PER 1: eight waves every eighth record of 64), eight
 // columns a lane, and leaves the context in LDS as TERMS bf16 terms; then a wave takes 16 output columns of all queries, its rows of W_UV as they lie.
 template <int TERMS, int PER>
-__global__ __launch_bounds__(512, PER > 8 ? 4 : 2) void uv_kernel(UvArgs a) {
+__global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
     static_assert(PER == 1 || PER % 8 == 0, "waves to a query, or queries to a wave");
-    constexpr int kTiles = (PER + 15) / 16, kRows = PER < 16 ? PER : 16, kSide = PER > 8 ? 4 : 12;   // kSide: records on their way
+    constexpr int kTiles = (PER + 15) / 16, kRows = PER < 16 ? PER : 16, kSide = PER == 8 ? 12 : 4;  // kSide: records on their way
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char *const ctx = lds;                                      // [TERMS][PER][kCLd]
     float *const sums = reinterpret_cast<float *>(lds + TERMS * PER * kCLd);    // PER 1: [8][512], then maxima and sums [8]
@@ -1137,7 +1141,7 @@ int launch_qa_of(const QaArgs &a, hipStream_t st) {
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 256 * kWLd);
     const int rc = check_hip(attr, "mla paged: query LDS size");
     if (rc) return rc;
-    qa_kernel<QT, F16, NT, MT><<<dim3(static_cast<unsigned>(a.H), static_cast<unsigned>(cdiv(a.M, 16 * MT)), 5), 256, bytes, st>>>(a);
+    qa_kernel<QT, F16, NT, MT><<<dim3(static_cast<unsigned>(4 * a.H * cdiv(a.M, 16 * MT) + 1)), 256, bytes, st>>>(a);
     return check_hip(hipGetLastError(), "mla paged: query launch");
 }
 template <typename QT>
@@ -1170,9 +1174,13 @@ int launch_uv_of(const UvArgs &a, hipStream_t st) {
 }
 template <int TERMS>
 int launch_uv(const UvArgs &a, hipStream_t st) {
-    // the most queries to a block, which reads its head's W_UV, with which there are blocks for every CU
-    if (a.H * cdiv(a.M, 32) >= 512) return launch_uv_of<TERMS, 32>(a, st);
-    if (a.M > 4) return launch_uv_of<TERMS, 8>(a, st);
+    // The most queries to a block, which reads its head's W_UV, with which there are blocks for every CU (of 32 and 16 queries two a CU, of 8 one).
+    // Measured, us, 8 / 16 / 32 queries: 32 requests of 64 heads 15.0 / 17.8 / -, 25 of 96 16.0 / 11.5 / -, 64 of 64 16.6 / 10.6 / 16.6 (8), 120 of 64
+    // 32.4 / 16.6 / 16.0, 800 of 64 - / 60 / 53.  Few queries have waves enough for all a query's records: 6 of 64 heads, some 80 records each, 18.1 for
+    // a wave a query, 17.5 for eight.
+    if (a.H * cdiv(a.M, 16) > 512) return launch_uv_of<TERMS, 32>(a, st);
+    if (a.H * cdiv(a.M, 8) > 256) return launch_uv_of<TERMS, 16>(a, st);
+    if (a.M > 8) return launch_uv_of<TERMS, 8>(a, st);
     return launch_uv_of<TERMS, 1>(a, st);
 }
 
