@@ -596,6 +596,10 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         constexpr int kAhead = 6;
         const int rg = wave & 1, pt = wave >> 1;            // operands 2 rg and 2 rg + 1; positions 16 pt .. +16 of a round
         const bool main = NT < 3 || rg == 0;                // (three terms: the third's waves give their scores to the others')
+        stage(0, false);
+        in0 = r_lat.z != 0;
+        stage(1, false);
+        in1 = r_lat.z != 0;
         u32x4 q[2][kSteps];                                 // [operand]: two groups of rows, or a group's two terms
         float fac[GR];
         int limit[GR];
@@ -634,7 +638,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
             fac[o % GR] = top * a.c;
             limit[o % GR] = limits[grp * 16 + r16];
         }
-        // (all of it is here before the first round is sent for: a wait for it in the loop would wait for the rounds in flight)
+        // (all of it is here before the loop: a wait for it there would wait for the rounds in flight)
 #pragma unroll
         for (int o = 0; o < 2; ++o)
 #pragma unroll
@@ -681,10 +685,6 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                 }
             }
         };
-        stage(0, false);
-        in0 = r_lat.z != 0;
-        stage(1, false);
-        in1 = r_lat.z != 0;
         arrived_barrier<4>();
         for (int rd = 0; rd <= nr; ++rd) {
             if (((rd + 2) & 63) == 0) look_up(rd + 2);
