@@ -792,8 +792,11 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int g = 0; g < GR; ++g) {
             const int row = (GR * rg + g) * 16 + r16;
-            if (main && pt == 0 && q4 == 0 && row < a.Mrec)
-                ml[row] = limit[g] > t_begin ? make_float2(from[g], l_run[g] + xf[row]) : make_float2(-INFINITY, 0.f);
+            if (main && pt == 0 && q4 == 0 && row < a.Mrec) {
+                // (nor does one whose positions are all on pages outside the pool: it has no reference, and 0 might be far above the others')
+                const float l = l_run[g] + xf[row];
+                ml[row] = limit[g] > t_begin && l != 0.f ? make_float2(from[g], l) : make_float2(-INFINITY, 0.f);
+            }
         }
     } else {
         // ================= context waves

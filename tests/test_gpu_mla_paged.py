@@ -236,6 +236,21 @@ def test_pages_outside_the_pool_count_as_not_there(pages, out):
     assert not bool(got[2].any())
 
 
+@pytest.mark.parametrize("pages,out", [(F16, BF16), (F16, F32), (BF16, BF16), (BF16, F32)])
+def test_ranges_without_a_page_beside_scores_far_below_zero(pages, out):
+    # whole ranges lie on pages outside the pool (the first, the last, some between); the scores of the others are about -300
+    case = oracle.make(_gen(16), 2, 1, 16, [640, 300], pages_dtype=pages, x=F32)
+    case["rot"] = case["rot"].clone()
+    case["rot"][..., 0] = -300.0
+    case["q_rot"] = case["q_rot"].clone()
+    case["q_rot"][..., 0] = 192 ** 0.5
+    for b, k in ((0, 0), (0, 3), (0, 4), (0, 9), (1, 1)):
+        case["table"][b, k] = -1
+    want, bound = oracle.attention(**case, out_dtype=out)
+    assert float(want.abs().mean()) > 1e-2
+    _check(_run(case, out_dtype=out), want, bound)
+
+
 # ------------------------------------------------------------------------------- sizes of the values
 @pytest.mark.parametrize("out", [BF16, F32])
 @pytest.mark.parametrize("size", [1e-30, 1e-4, 1e25])
@@ -258,7 +273,7 @@ def test_parts_of_a_query_of_unequal_size():
             _check(_run(c, out_dtype=out), want, bound)
 
 
-@pytest.mark.parametrize("pages,out", [(F16, BF16), (F16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("pages,out", [(F16, BF16), (F16, F32), (BF16, BF16), (BF16, F32)])
 def test_scores_that_keep_growing(pages, out):
     # every round exceeds all before it by far, in either half of it, so the reference moves again and again; and the other way round
     case = oracle.make(_gen(9), 2, 1, 20, [640, 639], pages_dtype=pages, x=F32)
