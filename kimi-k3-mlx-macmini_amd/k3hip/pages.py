@@ -32,7 +32,7 @@ def page_tables(table: torch.Tensor, lengths: torch.Tensor, target: torch.Tensor
     All int32 device tensors.  ``table`` [B, blocks]: request b's pages, in order, ceil(lengths[b] / page_size) of them; changed in
     place.  ``target`` [B]: the lengths to come to (negative: 0).  ``free`` [pages]: its entries from ``used`` [1] on are the pages that nobody
     holds; changed in place, where pages are given back.  ``shared`` [B]: so many of a request's first pages are not its own and are never
-    given back.  ``inplace``: ``lengths`` and ``used`` are written over instead of new tensors.
+    given back (a request that comes below them and grows again takes pages of its own in their places).  ``inplace``: ``lengths`` and ``used`` are written over instead of new tensors.
 
     Pages given back come in front of the list's free entries, in the batch's order, and can be taken in the same call.  Pages are taken
     in the batch's order; from the first request on that there are not enough for, requests that need pages stay at their length, as does one whose
@@ -102,16 +102,20 @@ class PageTable:
         return self.table.shape[1] * self.page_size
 
     def resize(self, target: torch.Tensor, tokens: int = 0) -> torch.Tensor:
-        """All requests to ``target`` [batch] int32 positions -> slots of up to ``tokens`` new tokens each (``page_tables``)."""
+        """All requests to ``target`` [batch] int32 positions -> slots of up to ``tokens`` new tokens each (``page_tables``).  None goes below
+        a common prefix."""
+        _per_sequence(target, self.batch, "target")
+        if self.prefix is not None:
+            target = target.clamp(min=len(self.prefix) * self.page_size)
         before = self.lengths.clone()
         _, _, self.slots = page_tables(self.table, self.lengths, target, self.free, self.used, self.page_size, tokens, self.shared, inplace=True)
         self.counts = (self.lengths - before).clamp_(min=0)
         return self.slots
 
     def extend(self, counts: int | torch.Tensor, tokens: int | None = None) -> torch.Tensor:
-        """Room for ``counts`` more tokens of every request (a number, or int32 [batch], 0 for a request that rests) -> slots
-        [batch, tokens] (``tokens``: the most that a request gets; needed for a tensor).  A request for which there is no page left gets none:
-        its ``counts`` entry is 0, its slots are -1."""
+        """Room for ``counts`` more tokens of every request (a number, or int32 [batch], 0 for a request that rests, below 0 for one that gives
+        so many back) -> slots [batch, tokens] (``tokens``: the most that a request gets; needed for a tensor).  A request for which there
+        is no page left gets none: its ``counts`` entry is 0, its slots are -1."""
         if isinstance(counts, torch.Tensor):
             _per_sequence(counts, self.batch, "counts")
             if tokens is None:
@@ -123,10 +127,7 @@ class PageTable:
     def truncate(self, lengths: torch.Tensor) -> None:
         """No request longer than ``lengths`` [batch] int32; pages behind that are given back.  A common prefix stays."""
         _per_sequence(lengths, self.batch, "lengths")
-        target = torch.minimum(self.lengths, lengths)
-        if self.prefix is not None:
-            target = target.clamp(min=len(self.prefix) * self.page_size)
-        self.resize(target)
+        self.resize(torch.minimum(self.lengths, lengths))
 
     def release(self, ended: torch.Tensor) -> None:
         """The requests where ``ended`` [batch] bool is true give back all pages of their own: they hold nothing, or the common prefix."""

@@ -245,6 +245,22 @@ def test_page_table_with_a_common_prefix(on_cpu):
     _held(t)
 
 
+@pytest.mark.parametrize("call,first", [
+    (lambda t: t.extend(torch.tensor([-10, -200, 0], dtype=I32), tokens=1), 65), (lambda t: t.resize(torch.tensor([0, -3, 69], dtype=I32)), 64),
+])
+def test_no_request_goes_below_a_common_prefix(on_cpu, call, first):
+    t = on_cpu.PageTable(3, 256, 12, page_size=32, device="cpu")
+    t.extend(torch.tensor([70, 0, 0], dtype=I32), tokens=70)
+    t.share(64)
+    t.extend(5)
+    call(t)
+    assert t.lengths.tolist() == [first, 64, 69] and t.counts.tolist() == [0] * 3
+    t.extend(40)
+    # the rows still begin with the prefix, and what follows is nobody else's
+    assert t.table[:, :2].tolist() == [t.prefix.tolist()] * 3
+    _held(t)
+
+
 def test_share_wants_the_others_empty(on_cpu):
     t = on_cpu.PageTable(2, 64, 4, page_size=32, device="cpu")
     t.extend(32)
@@ -254,7 +270,7 @@ def test_share_wants_the_others_empty(on_cpu):
 
 @pytest.mark.parametrize("call", [
     lambda t: t.extend(torch.zeros(2, dtype=I32)), lambda t: t.extend(torch.zeros(3, dtype=I32), tokens=1), lambda t: t.truncate(torch.zeros(3, dtype=I32)),
-    lambda t: t.release(torch.zeros(3, dtype=torch.bool)), lambda t: t.release(torch.zeros(2, dtype=I32)),
+    lambda t: t.resize(torch.zeros(3, dtype=I32)), lambda t: t.resize(torch.zeros(2)), lambda t: t.release(torch.zeros(3, dtype=torch.bool)), lambda t: t.release(torch.zeros(2, dtype=I32)),
 ])
 def test_page_table_refuses(on_cpu, call):
     with pytest.raises((ValueError, TypeError)):
