@@ -12,13 +12,17 @@
 //   attend   an item a block: a tile of rows x a range of positions; the maximum and sum run with the positions
 //   uv       the items' records joined (those of the prefix and the sequence's own alike), the context times W_UV, the output gate
 //
-// Numerics.  fp16 pages multiply as fp16: 11 bits make one term of a query or probability enough for a bf16 result (off by 2^-11 at most, independent
-// errors below the result's own 2^-8) and two for fp32 (2^-22); bf16 terms would need two and three.  The absorbed query's 128 columns
-// of a quarter, and its rotary columns, are scaled by a power of two of their own that puts the largest at 2^13 .. 2^14 (a block of the query
-// launch has one of them), and all to the row's largest scale as attend takes them in, so fp16's range is no question of the queries' size: what
-// falls below fp16's last bit then is 2^-38 of the row's largest.  Probabilities are 2^kLift times
-// those of the row's reference, which moves when one would exceed 2^kTop: so fp16 holds them, and its last bit is
-// 2^-31 of the largest; an item's context, over its sum, goes to the join as fp16 (2^-11).  Two terms: as fp32.  bf16 pages multiply as bf16, exact, against two terms of both for a bf16 result (2^-16), three for fp32 (2^-24).
+// Numerics.  fp16 pages multiply as fp16: 11 bits make one term of a query or probability enough for a bf16 result (off by 2^-11 at most,
+// independent errors below the result's own 2^-8) and two for fp32 (2^-22); bf16 terms would need two and three.  The absorbed query's 128
+// columns of a quarter, and its rotary columns, are scaled by a power of two of their own that puts the largest at 2^13 .. 2^14 (a block
+// of the query launch has one of them), and all to the row's largest scale as attend takes them in, so fp16's range is no question of the
+// queries' size: what falls below fp16's last bit then is 2^-38 of the row's largest.  Probabilities are 2^kLiftP times those of the row's
+// reference, which moves when one would exceed 2^kTop: so fp16 holds them, and its last bit is 2^-31 of the largest.  With one term an item's
+// context, over its sum, goes to the join as fp16 (2^-11, and no finer than 2^-25, as the pages' own values), else as fp32.  bf16 pages multiply
+// as bf16, exact, against two terms of both for a bf16 result (2^-16), three for fp32 (2^-24).
+//
+// Measured, us (qa + attend + uv):  1 request over 17 positions, 96 heads 6 + 10 + 8; 32 over up to 8192, 64 heads 9 + 19 + 14; 64 behind a prefix
+// of 8192 and up to 1024 of their own 9 + 80 + 11; 120 behind 32,768 14 + 480 + 17 (550 when the card is warm).
 #include <algorithm>
 #include <type_traits>
 
@@ -58,7 +62,6 @@ struct Item {
 struct Head {           // of the list
     int ranges;         // below the split: its items are range r of tile i at r tiles + i
     int low, high;      // items below and above the split
-    int pad;
 };
 struct Lists {
     const int32_t *lengths, *counts;
@@ -97,7 +100,9 @@ __device__ __forceinline__ int divide(int n, int d, float inverse) {
 }
 
 // By one block of 256 threads.  All ranges are of one length, the candidate that costs least by this account: the full ones in whole turns of
-// the 256 CUs, the others where there is room in these, else in turns of their own; and no less than all there is to do shared out.
+// the 256 CUs, the others where there is room in these, else in turns of their own; and no less than all there is to do shared out.  The list
+// takes 4 to 7 us beside the queries' blocks, which take 6 and more.  (Equal shares of all positions to every block, items cut where a share ends:
+// slower, 120 requests behind 32,768 positions by a fifth.  Blocks that are at different places of the prefix miss in L2.)
 __device__ __forceinline__ void list_items(const Lists &a, int *lds) {
     int *const own = lds, *const part = lds + kSearched, *const sh = part + 4 * kCandidates;    // own: what a sequence's last query sees
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -194,7 +199,7 @@ __device__ __forceinline__ void list_items(const Lists &a, int *lds) {
         }
         done += total;
     }
-    if (tid == 0) *a.head = Head{ranges, low, done - low, 0};
+    if (tid == 0) *a.head = Head{ranges, low, done - low};
 }
 
 // ------------------------------------------------------------------ qa
@@ -290,7 +295,9 @@ __device__ __forceinline__ void scale_of(uint32_t top, float &s, float &inverse)
 // A block: queries 16 MT y .. of head h, latent columns 128 z .. +128, all heads of a (y, z) after one another; and before them all
 // one for the list of items.  Blocks b % 8 run on one XCD.  Rows by query: an eighth of the blocks in a row goes to each, so the heads that share an
 // operand's 128-byte lines meet in one L2 (64 requests of 64 heads 10.7 -> 9.0 us, 120 16.0 -> 13.9); by head every head is on one XCD, with its matrix.
-// MT 1: few queries, a wave to 32 of the columns; MT 4: a wave to 16 of the queries.
+// MT 1: few queries, a wave to 32 of the columns; MT 4: a wave to 16 of the queries.  A block's 32 KB of weights are read and turned once
+// for its queries; 64 heads' take 8.4 MB, 1.8 us at a copy's rate, and the launch 9 us for 32 and 64 queries: the first loads, one barrier,
+// the products, another, the stores, one after the other, and no second block on the CU to hide them behind.
 template <typename QT, bool F16, int NT, int MT>
 __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -461,9 +468,9 @@ __device__ __forceinline__ uint32_t finite2(uint32_t p) {
 }
 
 // 16 bytes a lane from offset `off` of a buffer straight into LDS, lane l's at to + 16 l; what lies outside the buffer arrives as zeros.  Not
-// tracked by the compiler (nor is m0, which nothing else here uses): a wave waits for its own loads (arrived) and meets the others at a barrier before anything is read.  (As an
-// instruction of the compiler's it made every read of LDS wait for all loads in flight.  No register is written, so none can be reused
-// under it; its operands are read as it issues.)
+// tracked by the compiler (nor is m0, which nothing else here uses): a wave waits for its own loads (arrived) and meets the others at a barrier
+// before anything is read.  (As an instruction of the compiler's it made every read of LDS wait for all loads in flight.  No register is
+// written, so none can be reused under it; its operands are read as it issues.)
 __device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t off, uint32_t to) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rsrc), "s"(to) : "memory");
 }
@@ -492,6 +499,11 @@ __device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcn
 //           it holds as an operand of the second product.  The two waves of a row keep one reference: a wave that finds a score too far above
 //           it says so, and at the start of the next round all waves know, and wait while the round's probabilities are formed again.
 //   context waves (4 .. 7): ctx^T[column][row] += rows^T P^T, 128 columns each, from transposed reads of the staged rows.
+// What bounds it: at 64 (row, term)s a round's products take 1088 cycles of a SIMD's matrix unit and the round 1960, 55 %: 960 to 1100 TFLOP/s
+// (a large library product reaches 1205 in fp16).  No one part does: 120 requests behind 32,768 positions take 489 us, without the context's products 446,
+// without the scores' 409, without the loads 461, without the exponentials 466; a round of nothing but its barrier, address and flag reads takes 890 cycles, and
+// products keep the card near its power limit (the same call 550 to 650 us when repeated on random data).  Waves' priorities, operands
+// read further ahead and other item costs than kStart are within the noise.
 // GT = 4 / NT groups of 16 rows: with more terms the probabilities' further terms are rows of their own for the context waves, and the context
 // is their sum.  With three, the scores of the queries' third terms are formed by the other two score waves and join the others through LDS.
 template <bool F16, int NT>
@@ -746,34 +758,34 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
                     if (main) acc[1] += xs[pt][lane];
                 }
                 if (main) {
-                const int base = t_begin + rd * kRound + 16 * pt + 4 * q4;
-                const bool mixed = !in0 || t_begin + (rd + 1) * kRound > t_all;
-#pragma unroll
-                for (int g = 0; g < GR; ++g)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) e[g][i] = fmaf(NT > 1 ? acc[0][i] + acc[1][i] : acc[g][i], fac[g], -from[g]);
-                if (mixed) {
+                    const int base = t_begin + rd * kRound + 16 * pt + 4 * q4;
+                    const bool mixed = !in0 || t_begin + (rd + 1) * kRound > t_all;
 #pragma unroll
                     for (int g = 0; g < GR; ++g)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            // (where values are cleaned for the sake of rows that do not see them, an infinite score has to make its row NaN by itself)
-                            if (!(fabsf(e[g][i]) < INFINITY)) e[g][i] = NAN;
-                            e[g][i] = in0 && base + i < limit[g] ? e[g][i] : -INFINITY;
-                        }
-                }
-                bool above = false;
+                        for (int i = 0; i < 4; ++i) e[g][i] = fmaf(NT > 1 ? acc[0][i] + acc[1][i] : acc[g][i], fac[g], -from[g]);
+                    if (mixed) {
 #pragma unroll
-                for (int g = 0; g < GR; ++g) above |= max3(max3(e[g][0], e[g][1], e[g][2]), e[g][3], top[g]) > top[g];
-                if (__any(above)) {
-                    if (lane == 0) need[rd & 3][wave] = 1;
+                        for (int g = 0; g < GR; ++g)
 #pragma unroll
-                    for (int g = 0; g < GR; ++g) {
-                        const float t = q4_rows_max(fmaxf(fmaxf(e[g][0], e[g][1]), fmaxf(e[g][2], e[g][3])));
-                        if (q4 == 0) xm[rd & 1][pt][(GR * rg + g) * 16 + r16] = t;
+                            for (int i = 0; i < 4; ++i) {
+                                // (where values are cleaned for the sake of rows that do not see them, an infinite score has to make its row NaN by itself)
+                                if (!(fabsf(e[g][i]) < INFINITY)) e[g][i] = NAN;
+                                e[g][i] = in0 && base + i < limit[g] ? e[g][i] : -INFINITY;
+                            }
                     }
-                }
-                publish(rd);
+                    bool above = false;
+#pragma unroll
+                    for (int g = 0; g < GR; ++g) above |= max3(max3(e[g][0], e[g][1], e[g][2]), e[g][3], top[g]) > top[g];
+                    if (__any(above)) {
+                        if (lane == 0) need[rd & 3][wave] = 1;
+#pragma unroll
+                        for (int g = 0; g < GR; ++g) {
+                            const float t = q4_rows_max(fmaxf(fmaxf(e[g][0], e[g][1]), fmaxf(e[g][2], e[g][3])));
+                            if (q4 == 0) xm[rd & 1][pt][(GR * rg + g) * 16 + r16] = t;
+                        }
+                    }
+                    publish(rd);
                 }
                 __builtin_amdgcn_s_setprio(0);
             }
@@ -909,7 +921,8 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int i = 0; i < kRows * kOf / 8; ++i) {
             const int piece = i * 8 + wave, row = piece / kOf, off = piece % kOf * 1024 + lane * 16;
-            if (row < a.Mrec) *reinterpret_cast<u32x4 *>(to + static_cast<int64_t>(row) * kRecRow + off) = *reinterpret_cast<const u32x4 *>(lds + row * kRecLd + off);
+            if (row < a.Mrec)
+                *reinterpret_cast<u32x4 *>(to + static_cast<int64_t>(row) * kRecRow + off) = *reinterpret_cast<const u32x4 *>(lds + row * kRecLd + off);
         }
     }
 }
@@ -943,6 +956,7 @@ struct Records {
     __device__ __forceinline__ int at(int k) const { return k < low ? k * step * Mrec + pin : (first + (k - low) * tiles) * Mrec + in; }
 };
 
+// Bound by the records, 64 KB an item, and W_UV, behind the launch itself: 64 queries of 64 heads behind a prefix read 40 MB in 11 us.
 // grid (H, ceil(M / PER)), eight waves: PER queries of head x.  A wave joins the records of a query (PER 1: eight waves every eighth record of 64), eight
 // columns a lane, and leaves the context in LDS as TERMS bf16 terms; then a wave takes 16 output columns of all queries, its rows of W_UV as they lie.
 template <int TERMS, int PER>
@@ -1161,7 +1175,8 @@ int launch_attend(const AttendArgs &a, int most, hipStream_t st) {
         hipFuncSetAttribute(reinterpret_cast<const void *>(attend_kernel<F16, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, attend_lds());
     const int rc = check_hip(attr, "mla paged: attention LDS size");
     if (rc) return rc;
-    attend_kernel<F16, NT><<<dim3(static_cast<unsigned>(cdiv(most, 8) * 8 + 8)), 512, attend_lds(), st>>>(a);   // (an eighth of both kinds of item: one more at most)
+    // (an eighth of both kinds of item to an XCD: one more than an eighth of all at most)
+    attend_kernel<F16, NT><<<dim3(static_cast<unsigned>(cdiv(most, 8) * 8 + 8)), 512, attend_lds(), st>>>(a);
     return check_hip(hipGetLastError(), "mla paged: attention launch");
 }
 
@@ -1266,7 +1281,10 @@ extern "C" int k3_mla_paged_attention(const void *q_nope, int64_t qn_batch, int6
         a.lists = lists;
         a.part = ws + p.part, a.ml = reinterpret_cast<float2 *>(ws + p.ml);
         a.rows = rows, a.G = G, a.groups = groups, a.Mrec = p.Mrec, a.c = scale * 1.4426950408889634f;
-        rc = p.NT == 3 ? launch_attend<false, 3>(a, p.most, st) : !f16 ? launch_attend<false, 2>(a, p.most, st) : p.NT == 1 ? launch_attend<true, 1>(a, p.most, st) : launch_attend<true, 2>(a, p.most, st);
+        rc = p.NT == 3   ? launch_attend<false, 3>(a, p.most, st)
+             : !f16      ? launch_attend<false, 2>(a, p.most, st)
+             : p.NT == 1 ? launch_attend<true, 1>(a, p.most, st)
+                         : launch_attend<true, 2>(a, p.most, st);
         if (rc) return rc;
         const UvArgs u{a.part, a.ml, lists.head, lists.seq, static_cast<const uint16_t *>(w_uv), out, gate, static_cast<int>(H), static_cast<int>(v_dim), M, Tp,
                        static_cast<int>(t0), static_cast<int>(T), G, p.GT, tiles, ptiles, p.Mrec, out_dtype == K3_BF16, p.NT == 1, rows};

@@ -13,7 +13,8 @@
 //
 // One block plans: a thread takes neighbouring requests, a prefix sum over the block's 1024 threads orders them.  Few tokens
 // (kAlone) are then done by the same block, more by a second launch.  Both are bound by latency: dependent loads of lengths, table
-// and list (about 1 us each) and the launch itself.
+// and list (about 1 us each) and the launch itself.  64 requests of a token each 4.4 us; 48 prompts of up to 8192 tokens 3.4 + 6.8, where a copy
+// would write the 1.6 MB of slots in 0.3.
 #include <algorithm>
 
 #include "k3_common.h"

@@ -8,6 +8,8 @@ Host-side mirror of the reference interfaces, backed by hand-written HIP kernels
 * ``k3hip.mxfp4_matvec``   mxfp4_matvec_fused / expert_projection
                            (air_llm/kernels/metal/mxfp4_matvec.py)
 * ``k3hip.mla_q4``         the 4-bit latent cache and its attention  (air_llm/models/kimi_k3/mla_quant.py)
+* ``k3hip.pages``          page tables of a batch of requests
+* ``k3hip.mla_paged``      the paged latent cache and its attention  (air_llm/models/kimi_k3/attention_mla.py:62-117, :193-212)
 * ``k3hip.evict``          eviction by accumulated attention weight
 """
 from __future__ import annotations

@@ -47,7 +47,8 @@ def attention(q_nope, q_rot, wk, wv, lat, rot, table, lengths, scale, counts=Non
     roundings, which add so over the positions; 2^-19 of the sum of magnitudes for the fp32 sums (576 and more products, 2^-24 each, and the
     context's terms before W_UV, 2^-16 at a bf16 result).  At a bf16 result over fp16 pages the contexts of ranges are fp16, over their sums: every
     column of range i off by 2^-11 |c_i| at most, independently, weighed with the range's share w_i; sum_i w_i |c_i| is at most sum_j p_j |lat_j|, so
-    six deviations are 6 2^-11 of the root of the squares of W_UV times that."""
+    six deviations are 6 2^-11 of the root of the squares of W_UV times that.  Below 2^-14 fp16's values are 2^-24 apart whatever their size, so
+    a column of a range is off by 2^-25 at least there, as the pages' own values are: 6 2^-25 of the root of the squares of W_UV."""
     f64 = torch.float64
     B, T, H, nope = q_nope.shape
     V, page, pool = wv.shape[1], lat.shape[1], lat.shape[0]
@@ -83,6 +84,7 @@ def attention(q_nope, q_rot, wk, wv, lat, rot, table, lengths, scale, counts=Non
             sums = torch.einsum("hj,hjr,hvr->hv", p, Ls.abs().expand(H, -1, -1), wv.to(f64).abs())
             if not fine and lat.dtype == torch.float16:
                 weight = weight + u_q * torch.einsum("hr,hvr->hv", (p @ Ls.abs()).square(), wv.to(f64).square()).sqrt()
+                weight = weight + 2.0 ** -25 * wv.to(f64).square().sum(-1).sqrt()
             bound[b, t] = 6 * (spread + weight) + sums * (2.0 ** -19 if fine else 2.0 ** -15)
             if gate is not None:
                 g = torch.sigmoid(gate[b, t].to(f64).reshape(H, V))

@@ -130,6 +130,7 @@ def _run(case, **kw):
 
 
 FORMS = [(F16, BF16, BF16), (F16, F32, F32), (BF16, BF16, BF16), (BF16, F32, F32), (F16, F32, BF16), (F16, BF16, F32)]
+FORMS_PO = [(F16, BF16), (F16, F32), (BF16, BF16), (BF16, F32)]      # pages, result: one, two, two and three terms
 
 
 @pytest.mark.parametrize("pages,x,out", FORMS)
@@ -236,7 +237,7 @@ def test_pages_outside_the_pool_count_as_not_there(pages, out):
     assert not bool(got[2].any())
 
 
-@pytest.mark.parametrize("pages,out", [(F16, BF16), (F16, F32), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("pages,out", FORMS_PO)
 def test_ranges_without_a_page_beside_scores_far_below_zero(pages, out):
     # whole ranges lie on pages outside the pool (the first, the last, some between); the scores of the others are about -300
     case = oracle.make(_gen(16), 2, 1, 16, [640, 300], pages_dtype=pages, x=F32)
@@ -262,6 +263,17 @@ def test_queries_of_any_size(size, out):
     _check(_run(case, out_dtype=out), want, bound)
 
 
+@pytest.mark.parametrize("pages,out", FORMS_PO)
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -12, 2.0 ** 11])
+def test_latents_of_any_size(size, pages, out):
+    # (2^-20: fp16's last bits, below its smallest normal value)
+    case = oracle.make(_gen(17), 2, 1, 16, [150, 33], pages_dtype=pages, x=F32)
+    case["lat"] = (case["lat"].float() * size).clamp(-6e4, 6e4).to(pages)
+    case["q_nope"] = case["q_nope"] * min(1.0, 1 / size)
+    want, bound = oracle.attention(**case, out_dtype=out)
+    _check(_run(case, out_dtype=out), want, bound)
+
+
 def test_parts_of_a_query_of_unequal_size():
     # no rotary part, or one that is 2^20 times the rest: each has its scale
     case = oracle.make(_gen(8), 2, 1, 16, [150, 33], x=F32)
@@ -273,7 +285,7 @@ def test_parts_of_a_query_of_unequal_size():
             _check(_run(c, out_dtype=out), want, bound)
 
 
-@pytest.mark.parametrize("pages,out", [(F16, BF16), (F16, F32), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("pages,out", FORMS_PO)
 def test_scores_that_keep_growing(pages, out):
     # every round exceeds all before it by far, in either half of it, so the reference moves again and again; and the other way round
     case = oracle.make(_gen(9), 2, 1, 20, [640, 639], pages_dtype=pages, x=F32)
