@@ -956,6 +956,18 @@ struct Records {
     __device__ __forceinline__ int at(int k) const { return k < low ? k * step * Mrec + pin : (first + (k - low) * tiles) * Mrec + in; }
 };
 
+// The lanes of a whose bit is set, and those of b whose bit is not, change places; CTRL pairs the lanes (xor 1: 0xb1, xor 2: 0x4e).
+template <int CTRL>
+__device__ __forceinline__ void exchange(u32x4 &a, u32x4 &b, bool set) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const uint32_t x = a[d], y = b[d];
+        const uint32_t to_a = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(y), CTRL, 0xf, 0xf, true));
+        const uint32_t to_b = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xf, 0xf, true));
+        a[d] = set ? to_a : x, b[d] = set ? y : to_b;
+    }
+}
+
 // Bound by the records, 64 KB an item, and W_UV, behind the launch itself: 64 queries of 64 heads behind a prefix read 40 MB in 11 us.
 // grid (H, ceil(M / PER)), eight waves: PER queries of head x.  A wave joins the records of a query (PER 1: eight waves every eighth record of 64), eight
 // columns a lane, and leaves the context in LDS as TERMS bf16 terms; then a wave takes 16 output columns of all queries, its rows of W_UV as they lie.
@@ -970,11 +982,22 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
     const int h = blockIdx.x, m0 = blockIdx.y * PER;
     const int vtiles = (a.V + 15) / 16;
     const auto rw = make_rsrc(a.w_uv + static_cast<int64_t>(h) * a.V * kLat, static_cast<uint32_t>(a.V) * (2 * kLat));
+    // An operand's 16 neighbouring lanes are 16 rows of W_UV, and loaded like that take the load path three to four times as long as 64 bytes of
+    // four rows do.  So load 4 J + i is of rows i, 4 + i, 8 + i and 12 + i, 256 bytes of each, and turned() exchanges the lanes of a quad with
+    // the four loads: then operand 4 J + i is columns 128 J + 32 q4 + 8 i .. +8 of row r16.
     u32x4 w[16];
     auto weights = [&](int vt) __attribute__((always_inline)) {         // (rows past the head's last are outside and load zeros)
+        const uint32_t at = static_cast<uint32_t>(vt * 16 + (r16 & 12)) * (2 * kLat) + q4 * 64 + (r16 & 3) * 16;
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-            w[k] = __builtin_bit_cast(u32x4, buf_load16(rw, static_cast<uint32_t>(vt * 16 + r16) * (2 * kLat) + k * 64 + q4 * 16));
+        for (int k = 0; k < 16; ++k) w[k] = __builtin_bit_cast(u32x4, buf_load16(rw, at + (k & 3) * (2 * kLat) + (k >> 2) * 256));
+    };
+    auto turned = [&]() __attribute__((always_inline)) {
+        const bool odd = lane & 1, high = lane & 2;
+#pragma unroll
+        for (int J = 0; J < 16; J += 4) {
+            exchange<0xb1>(w[J], w[J + 1], odd), exchange<0xb1>(w[J + 2], w[J + 3], odd);
+            exchange<0x4e>(w[J], w[J + 2], high), exchange<0x4e>(w[J + 1], w[J + 3], high);
+        }
     };
     // the context of columns 4 lane .. +4 and 256 + 4 lane .. +4
     auto store = [&](int i, f32x4 x, f32x4 y) __attribute__((always_inline)) {
@@ -1073,6 +1096,7 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
     __syncthreads();
     for (int vt = wave; vt < vtiles; vt += 8) {
         if (PER > 8 || vt != wave) weights(vt);
+        turned();
         f32x4 o[kTiles], o2[kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) o[t] = o2[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1083,7 +1107,7 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
                     f32x4 &to = k & 1 ? o2[t] : o[t];
-                    to = q4_mfma_bf16(w[k], *reinterpret_cast<const u32x4 *>(ctx + (y * PER + t * 16 + r16 % kRows) * kCLd + k * 64 + q4 * 16), to);
+                    to = q4_mfma_bf16(w[k], *reinterpret_cast<const u32x4 *>(ctx + (y * PER + t * 16 + r16 % kRows) * kCLd + (k >> 2) * 256 + q4 * 64 + (k & 3) * 16), to);
                 }
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) o[t] += o2[t];
