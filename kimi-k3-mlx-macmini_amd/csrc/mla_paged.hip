@@ -87,11 +87,11 @@ __device__ __forceinline__ int sees_last(const Lists &a, int b) {
 }
 
 constexpr int kSearched = 1024;         // sequences up to which the ranges' length is searched for
-constexpr int kCandidates = 64;         // lengths: one to two shares of one to kTurns turns of the card's 256 CUs
+constexpr int kCandidates = 64;         // lengths: from a share of the most turns of the card's 256 CUs to 1.6 shares of one, evenly by their logarithm
 constexpr int kTurns = 8;
 constexpr int kRound = 32;              // positions of a round of the attention
 constexpr int kStart = 256;             // what an item's start and end cost, in positions
-constexpr int kListLds = (kSearched + 4 * kCandidates + 16) * 4;
+constexpr int kListLds = (kSearched + 4 * 4 * kCandidates + 16) * 4;
 
 // n / d, 1 / d given: exact for n < 2^23
 __device__ __forceinline__ int divide(int n, int d, float inverse) {
@@ -99,12 +99,15 @@ __device__ __forceinline__ int divide(int n, int d, float inverse) {
     return c + ((c + 1) * d <= n ? 1 : c * d > n ? -1 : 0);
 }
 
-// By one block of 256 threads.  All ranges are of one length, the candidate that costs least by this account: the full ones in whole turns of
-// the 256 CUs, the others where there is room in these, else in turns of their own; and no less than all there is to do shared out.  The list
-// takes 4 to 7 us beside the queries' blocks, which take 6 and more.  (Equal shares of all positions to every block, items cut where a share ends:
-// slower, 120 requests behind 32,768 positions by a fifth.  Blocks that are at different places of the prefix miss in L2.)
+// By one block of 256 threads.  All ranges are of one length, the candidate that costs least by this account of an XCD's 32 CUs and its eighth of the
+// items: the full ranges in whole turns; the others (m positions at a mean, mx at most) where there is room in these, several to a CU if none but the
+// prefix's ranges are full, else in turns of their own; and no less than all there is to do shared out.  (The schedule that the card then runs,
+// worked out on the host for 120 draws of batches, prefixes and lengths, takes 0.8 % longer than at the best candidate, 38 % at worst; with
+// half a range for mx and m and no account of XCDs 2.8 and 64 %.)  The list takes 4 to 7 us beside the queries' blocks, which take 6 and
+// more.  (Equal shares of all positions to every block, items cut where a share ends: slower, 120 requests behind 32,768 positions by a fifth.
+// Blocks that are at different places of the prefix miss in L2.)
 __device__ __forceinline__ void list_items(const Lists &a, int *lds) {
-    int *const own = lds, *const part = lds + kSearched, *const sh = part + 4 * kCandidates;    // own: what a sequence's last query sees
+    int *const own = lds, *const part = lds + kSearched, *const sh = part + 4 * 4 * kCandidates;    // own: what a sequence's last query sees
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int lp = 0;
     float sum = 0.f;
@@ -124,29 +127,32 @@ __device__ __forceinline__ void list_items(const Lists &a, int *lds) {
     int Ts = 1 << 24;                   // (all of a sequence: what always fits)
     // (a candidate a lane, a quarter of the sequences a wave)
     if (a.B <= kSearched) {
-        constexpr int kFractions = kCandidates / kTurns;
-        const int k = 1 + lane / kFractions;
-        const float want = work / (256.f * k) * (1.f + (lane % kFractions) * (1.f / kFractions));
+        const float least_want = 0.97f * work / (256.f * a.turns), step = log2f(1.6f / 0.97f * a.turns) / (kCandidates - 1);
+        const float want = least_want * exp2f(step * lane);
         const int T1 = (static_cast<int>(fminf(want, 8388608.f)) / kRound + 1) * kRound;
         const float inv = 1.0f / T1;
         const int r0 = a.aligned ? lp / T1 : (lp + T1 - 1) / T1, split = a.aligned ? r0 * T1 : a.prefix;
-        int full = 0, all = 0;
+        int full = 0, rest = 0, mx = 0;         // full ranges, others, the longest of these
+        float spent = 0.f;                      // positions of the others
         for (int b = wave; b < a.B; b += 4) {
-            const int o = max(own[b] - split, 0), c = divide(o, T1, inv);
-            full += c, all += c + (c * T1 < o);
+            const int o = max(own[b] - split, 0), c = divide(o, T1, inv), left = o - c * T1;
+            full += c, rest += left > 0, mx = max(mx, left), spent += static_cast<float>(left);
         }
-        part[wave * kCandidates + lane] = full;
+        reinterpret_cast<int4 *>(part)[wave * kCandidates + lane] = make_int4(full, rest, mx, __float_as_int(spent));
         __syncthreads();
-        full = (part[lane] + part[kCandidates + lane]) + (part[2 * kCandidates + lane] + part[3 * kCandidates + lane]);
-        __syncthreads();
-        part[wave * kCandidates + lane] = all;
-        __syncthreads();
-        all = (part[lane] + part[kCandidates + lane]) + (part[2 * kCandidates + lane] + part[3 * kCandidates + lane]);
-        const int items = all * a.tiles + r0 * a.ptiles, whole = full * a.tiles + r0 * a.ptiles;
-        const int turns = (whole + 255) >> 8, left = items - whole - (turns * 256 - whole);
-        float cost = static_cast<float>(turns) * (T1 + kStart) + static_cast<float>((max(left, 0) + 255) >> 8) * (T1 / 2 + kStart);
+        full = rest = mx = 0, spent = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int4 v = reinterpret_cast<const int4 *>(part)[i * kCandidates + lane];
+            full += v.x, rest += v.y, mx = max(mx, v.z), spent += __int_as_float(v.w);
+        }
+        const int whole = full * a.tiles + r0 * a.ptiles, others = rest * a.tiles, items = whole + others;
+        const float L = static_cast<float>(T1 + kStart), M = static_cast<float>(mx + kStart), m = spent / max(rest, 1) + kStart;
+        const int mine = (whole + 7) >> 3, turns = (mine + 31) >> 5, room = (turns * 32 - mine) * (full ? 1 : max(1, static_cast<int>(L / M)));
+        const int more = (max(((others + 7) >> 3) - room, 0) + 31) >> 5;
+        float cost = turns * L + (more ? (more - 1) * m + M : 0.f);
         cost = fmaxf(cost, (work + static_cast<float>(items) * kStart) * (1.0f / 256.f));
-        if (k > a.turns || items > a.most) cost = INFINITY;
+        if (items > a.most) cost = INFINITY;
         // (cost, lane) least
         float least = cost;
 #pragma unroll
@@ -179,7 +185,7 @@ __device__ __forceinline__ void list_items(const Lists &a, int *lds) {
         for (int i = 0; i < wave; ++i) at += sh[i];
         if (b < a.B) a.seq[b] = make_int2(done + at, c);
         const int total = sh[0] + sh[1] + sh[2] + sh[3];
-        part[tid] = at;                 // (kCandidates x 4 = 256)
+        part[tid] = at;
         if (b0 < kSearched) {
             __syncthreads();
             for (int j = tid; j < total; j += 256) {
@@ -531,6 +537,13 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     const Item it = a.lists.item[at];
     const int seq = __builtin_amdgcn_readfirstlane(it.seq), tile = __builtin_amdgcn_readfirstlane(it.tile);
     const int t_begin = __builtin_amdgcn_readfirstlane(it.begin), end = __builtin_amdgcn_readfirstlane(it.end);
+    // the page of a lane's round of 64 (a round lies in one page): positions below `to` are in the table
+    const int32_t *const pages = a.table + max(seq, 0) * a.table_row;
+    auto page_of = [&](int rd, int to) __attribute__((always_inline)) {
+        const int pos = t_begin + rd * kRound;
+        return pos < to ? (pos < a.lists.prefix ? a.prefix : pages)[pos >> a.shift] : -1;
+    };
+    const int first_page = page_of(lane, end);      // (asked for beside the lengths)
     // ---- what the rows see
     if (tid < kRows) {
         const int g = tile * GT + (tid >> 4);
@@ -550,15 +563,12 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
     const int nr = (t_end - t_begin + kRound - 1) / kRound;
 
     // ---- staging: round rd into slot rd % kSlots, by all waves: four latent rows each, the context waves eight rotary rows as well.
-    // A lane keeps, for one of 64 rounds, where its rows are (a round lies in one page) and how many bytes there are from there on: none for
-    // a page outside the pool.
-    const int32_t *const pages = a.table + max(seq, 0) * a.table_row;
+    // A lane keeps, for one of 64 rounds, where its rows are and how many bytes there are from there on: none for a page outside the pool.
     uint64_t my_lat, my_rot;
     uint32_t my_latb, my_rotb;
-    auto look_up = [&](int first) __attribute__((always_inline)) {
-        const int rd = first + lane, pos = t_begin + rd * kRound, off = pos & ((1 << a.shift) - 1);
-        int p = rd < nr ? (pos < a.lists.prefix ? a.prefix : pages)[pos >> a.shift] : -1;
-        const bool in = p >= 0 && p < a.pages;
+    auto place = [&](int rd, int p) __attribute__((always_inline)) {
+        const int pos = t_begin + rd * kRound, off = pos & ((1 << a.shift) - 1);
+        const bool in = rd < nr && p >= 0 && p < a.pages;
         const uint32_t rows = static_cast<uint32_t>(min(t_end - pos, kRound)) - 1u;
         p = in ? p : 0;
         my_lat = reinterpret_cast<uint64_t>(a.lat) + p * a.lat_page + static_cast<uint64_t>(off) * a.lat_row;
@@ -566,6 +576,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         my_latb = in ? rows * a.lat_row + 1024u : 0u;
         my_rotb = in ? rows * a.rot_row + 128u : 0u;
     };
+    auto look_up = [&](int first) __attribute__((always_inline)) { place(first + lane, page_of(first + lane, t_end)); };
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds));
     const int rrow = 8 * (wave & 3) + (lane >> 3);
     const uint32_t lat_off = static_cast<uint32_t>(4 * wave) * a.lat_row + lane * 16u;
@@ -593,7 +604,7 @@ __global__ __launch_bounds__(512, 1) void attend_kernel(AttendArgs a) {
         if (context) stage_rot();
     };
     bool in0, in1;              // whether the pages of this round and the next are in the pool; r_lat says it of the one after that
-    look_up(0);
+    place(lane, first_page);
 
     // Iteration t = -1 .. nr - 1: round t + 3 is sent for, the score waves take round t + 1, the context waves round t; then round t + 2 is
     // waited for.  A slot is written again three iterations after its scores, two after its context.
@@ -999,13 +1010,14 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
             exchange<0x4e>(w[J], w[J + 2], high), exchange<0x4e>(w[J + 1], w[J + 3], high);
         }
     };
-    // the context of columns 4 lane .. +4 and 256 + 4 lane .. +4
+    // the context of columns 8 lane .. +8 (fp16 records: 16 bytes a lane), or of 4 lane .. +4 and 256 + 4 lane .. +4
+    const bool half = TERMS == 2 && a.half;
     auto store = [&](int i, f32x4 x, f32x4 y) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < TERMS; ++t) {
             const u32x2 p = {q4_pack_bf16(x[0], x[1]), q4_pack_bf16(x[2], x[3])}, o = {q4_pack_bf16(y[0], y[1]), q4_pack_bf16(y[2], y[3])};
-            *reinterpret_cast<u32x2 *>(ctx + (t * PER + i) * kCLd + lane * 8) = p;
-            *reinterpret_cast<u32x2 *>(ctx + (t * PER + i) * kCLd + 512 + lane * 8) = o;
+            *reinterpret_cast<u32x2 *>(ctx + (t * PER + i) * kCLd + lane * (half ? 16 : 8)) = p;
+            *reinterpret_cast<u32x2 *>(ctx + (t * PER + i) * kCLd + (half ? lane * 16 + 8 : 512 + lane * 8)) = o;
             x -= f32x4{q4_lo(p.x), q4_hi(p.x), q4_lo(p.y), q4_hi(p.y)};
             y -= f32x4{q4_lo(o.x), q4_hi(o.x), q4_lo(o.y), q4_hi(o.y)};
         }
@@ -1034,7 +1046,7 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
                 const float f = v.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(v.x - mx);
                 if (PER > 1 || wave == 0) l = fmaf(f, v.y, l);
                 // (fp16 records are contexts over their sums)
-                const float weight = TERMS == 2 && a.half ? f * v.y : f;
+                const float weight = half ? f * v.y : f;
                 for (int j0 = PER == 1 ? wave * kSide : 0; j0 < n; j0 += PER == 1 ? 8 * kSide : kSide) {
                     float g[kSide];
                     int from[kSide];
@@ -1043,19 +1055,19 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
                         from[j] = __builtin_amdgcn_readlane(at, (j0 + j) & 63);
                         g[j] = j0 + j < n ? readlane_f(weight, (j0 + j) & 63) : 0.f;
                     }
-                    if (TERMS == 2 && a.half) {
-                        u32x2 c[kSide][2] = {};
+                    if (half) {
+                        u32x4 c[kSide] = {};
 #pragma unroll
                         for (int j = 0; j < kSide; ++j) {
-                            const uint16_t *p = static_cast<const uint16_t *>(a.part) + static_cast<int64_t>(from[j]) * kLat + 4 * lane;
-                            if (j0 + j < n) c[j][0] = *reinterpret_cast<const u32x2 *>(p), c[j][1] = *reinterpret_cast<const u32x2 *>(p + 256);
+                            const uint16_t *p = static_cast<const uint16_t *>(a.part) + static_cast<int64_t>(from[j]) * kLat + 8 * lane;
+                            if (j0 + j < n) c[j] = *reinterpret_cast<const u32x4 *>(p);
                         }
 #pragma unroll
                         for (int j = 0; j < kSide; ++j)
                             if (g[j] != 0.f) {
                                 float u[8];
-                                unpack2<true>(c[j][0].x, u[0], u[1]), unpack2<true>(c[j][0].y, u[2], u[3]);
-                                unpack2<true>(c[j][1].x, u[4], u[5]), unpack2<true>(c[j][1].y, u[6], u[7]);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) unpack2<true>(c[j][k], u[2 * k], u[2 * k + 1]);
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) x[k] = fmaf(g[j], u[k], x[k]), y[k] = fmaf(g[j], u[4 + k], y[k]);
                             }
