@@ -1060,17 +1060,16 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
 #pragma unroll
                         for (int j = 0; j < kSide; ++j) {
                             const uint16_t *p = static_cast<const uint16_t *>(a.part) + static_cast<int64_t>(from[j]) * kLat + 8 * lane;
-                            if (j0 + j < n) c[j] = *reinterpret_cast<const u32x4 *>(p);
+                            if (g[j] != 0.f) c[j] = *reinterpret_cast<const u32x4 *>(p);
                         }
 #pragma unroll
-                        for (int j = 0; j < kSide; ++j)
-                            if (g[j] != 0.f) {
-                                float u[8];
+                        for (int j = 0; j < kSide; ++j) {
+                            float u[8];
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) unpack2<true>(c[j][k], u[2 * k], u[2 * k + 1]);
+                            for (int k = 0; k < 4; ++k) unpack2<true>(c[j][k], u[2 * k], u[2 * k + 1]);
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) x[k] = fmaf(g[j], u[k], x[k]), y[k] = fmaf(g[j], u[4 + k], y[k]);
-                            }
+                            for (int k = 0; k < 4; ++k) x[k] = fmaf(g[j], u[k], x[k]), y[k] = fmaf(g[j], u[4 + k], y[k]);
+                        }
                     } else {
                         f32x4 c[kSide][2] = {};
 #pragma unroll
@@ -1080,7 +1079,7 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
                         }
 #pragma unroll
                         for (int j = 0; j < kSide; ++j)
-                            if (g[j] != 0.f) x += g[j] * c[j][0], y += g[j] * c[j][1];
+                            if (g[j] != 0.f) x += g[j] * c[j][0], y += g[j] * c[j][1]; 
                     }
                 }
             }
