@@ -232,22 +232,28 @@ __device__ __forceinline__ void three_terms(const float (&v)[8], u32x4 (&f)[3]) 
         f[x] = u32x4{hi16x2(t[x][0], t[x][1]), hi16x2(t[x][2], t[x][3]), hi16x2(t[x][4], t[x][5]), hi16x2(t[x][6], t[x][7])};
 }
 
-// 8 query values of a lane: slots 8 q4 .. +8 of a step of 32 hold n = 4 q4 + {0..3} and 16 + 4 q4 + {0..3}, the order in which
-// the transposed reads of the weights give theirs
+// 8 query values of a lane, columns 8 q4 .. +8 of a step of 32 of query r16.  They are loaded four lanes to a query (neighbouring lanes that read from
+// 16 queries take the load path four times as long: 4 x 200 tokens 32 us for 28.5) and change lanes as they are used.
+typedef u32x4 __attribute__((aligned(8))) u32x4_8;
 template <typename QT>
 struct Query {
-    typedef typename std::conditional<std::is_same<QT, float>::value, f32x4, u32x2>::type V;
-    V x[2];
-    __device__ __forceinline__ void load(const QT *q, int n, int nope, bool live) {
+    static constexpr int kWords = sizeof(QT) * 2;   // of 4 bytes
+    u32x4 x[kWords / 4];
+    __device__ __forceinline__ void load(const QT *q, bool there) {     // q: columns 8 (lane % 4) of query lane / 4
 #pragma unroll
-        for (int i = 0; i < 2; ++i) x[i] = live && n + 16 * i < nope ? *reinterpret_cast<const V *>(q + n + 16 * i) : V{};
+        for (int i = 0; i < kWords / 4; ++i) x[i] = there ? reinterpret_cast<const u32x4_8 *>(q)[i] : u32x4{};
     }
-    __device__ __forceinline__ void terms(u32x4 (&f)[3]) const {
+    __device__ __forceinline__ void terms(int from, u32x4 (&f)[3]) const {     // from: 4 times the lane that holds this lane's
+        uint32_t v[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) v[i] = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(from, static_cast<int>(x[i / 4][i % 4])));
         if constexpr (std::is_same<QT, float>::value) {
-            const float v[8] = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
-            three_terms(v, f);
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __uint_as_float(v[i]);
+            three_terms(w, f);
         } else {
-            f[0] = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
+            f[0] = u32x4{v[0], v[1], v[2], v[3]};
         }
     }
 };
@@ -319,13 +325,14 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     const int h = b % a.H, m0 = b / a.H / 4 * 16 * MT, quarter = b / a.H % 4;
     const int steps = (a.nope + 31) >> 5;
     const uint16_t *w = a.w_uk + static_cast<int64_t>(h) * a.nope * kLat + quarter * 128;
-    const int qt = MT == 1 ? 0 : wave, col = MT == 1 ? wave * 32 : 0, mine = m0 + 16 * qt + r16;    // the wave's queries and columns
+    const int qt = MT == 1 ? 0 : wave, col = MT == 1 ? wave * 32 : 0, mine = m0 + 16 * qt + (lane >> 2);    // the wave's queries and columns
     const bool live = mine < a.M;
     const int qb = live ? mine / a.T : 0, qt0 = live ? a.t0 + mine - qb * a.T : 0;
-    const QT *q = static_cast<const QT *>(a.q_nope) + qb * a.n_b + qt0 * a.n_t + h * a.n_h + 4 * q4;
+    const QT *q = static_cast<const QT *>(a.q_nope) + qb * a.n_b + qt0 * a.n_t + h * a.n_h + 8 * (lane & 3);
+    const int own = a.nope - 8 * (lane & 3), from = 16 * r16 + 4 * q4;
     Query<QT> ahead[kAhead];
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) ahead[s].load(q, 32 * s, a.nope - 4 * q4, live);
+    for (int s = 0; s < kAhead; ++s) ahead[s].load(q + 32 * s, live && 32 * s < own);
     for (int i0 = 0; i0 < 2 * steps; i0 += 8) {
         uint4 v[8];
 #pragma unroll
@@ -344,16 +351,16 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
     for (int j = 0; j < kTiles; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     __syncthreads();
     auto step = [&](int s, const Query<QT> &raw) __attribute__((always_inline)) {
-        const char *wr = lds + (32 * s + 4 * q4 + (r16 >> 2)) * kWLd + (r16 & 3) * 8 + col * 2;
+        const char *wr = lds + (32 * s + 8 * q4 + (r16 >> 2)) * kWLd + (r16 & 3) * 8 + col * 2;
         u32x4 qf[3];
-        raw.terms(qf);
+        raw.terms(from, qf);
 #pragma unroll
         for (int j0 = 0; j0 < kTiles; j0 += 2) {
             u32x4 wf[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + (j0 + j) * 32));
-                const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + (j0 + j) * 32 + 16 * kWLd));
+                const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(wr + (j0 + j) * 32 + 4 * kWLd));
                 wf[j] = __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
             }
 #pragma unroll
@@ -367,7 +374,7 @@ __global__ __launch_bounds__(256) void qa_kernel(QaArgs a) {
         if (s < steps) step(s, ahead[s]);
     for (int s = kAhead; s < steps; ++s) {
         Query<QT> raw;
-        raw.load(q, 32 * s, a.nope - 4 * q4, live);
+        raw.load(q + 32 * s, live && 32 * s < own);
         step(s, raw);
     }
     __syncthreads();   // the weights are read

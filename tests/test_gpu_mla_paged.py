@@ -323,6 +323,16 @@ def test_layouts_and_strides():
     _check(_run(part), *oracle.attention(**part))
 
 
+@pytest.mark.parametrize("T,out", [(1, BF16), (20, BF16), (3, F32)])
+def test_bf16_queries_whose_rows_lie_8_bytes_off(T, out):
+    # (pitches of 196 and more elements: read as they are, every second row off a multiple of 16 bytes)
+    case = oracle.make(_gen(18), 3, T, 12, [100, 31, 65], nope=136)
+    q = torch.cat((case["q_nope"], case["q_rot"], case["q_rot"][..., :4]), -1)
+    wide = {**case, "q_nope": q[..., :136], "q_rot": torch.cat((case["q_rot"], case["q_rot"][..., :4]), -1)[..., :64]}
+    assert q.stride(2) % 8 == 4
+    assert bool((_run(wide, out_dtype=out) == _run({**case, "q_nope": case["q_nope"].contiguous(), "q_rot": case["q_rot"].contiguous()}, out_dtype=out)).all())
+
+
 def test_max_length_cuts():
     case = oracle.make(_gen(11), 2, 1, 8, [100, 50])
     cut = {**case, "lengths": case["lengths"].clamp(max=70)}
