@@ -21,8 +21,8 @@
 // context, over its sum, goes to the join as fp16 (2^-11, and no finer than 2^-25, as the pages' own values), else as fp32.  bf16 pages multiply
 // as bf16, exact, against two terms of both for a bf16 result (2^-16), three for fp32 (2^-24).
 //
-// Measured, us (qa + attend + uv):  1 request over 17 positions, 96 heads 6 + 10 + 8; 32 over up to 8192, 64 heads 9 + 19 + 14; 64 behind a prefix
-// of 8192 and up to 1024 of their own 9 + 80 + 11; 120 behind 32,768 14 + 480 + 17 (550 when the card is warm).
+// Measured, us (qa + attend + uv):  1 request over 17 positions, 96 heads 7 + 9 + 6; 32 over up to 8192, 64 heads 9 + 20 + 13; 64 behind a prefix
+// of 8192 and up to 1024 of their own 9 + 80 + 9; 120 behind 32,768 14 + 480 + 12 (535 when the card is warm).
 #include <algorithm>
 #include <type_traits>
 
@@ -986,7 +986,7 @@ __device__ __forceinline__ void exchange(u32x4 &a, u32x4 &b, bool set) {
     }
 }
 
-// Bound by the records, 64 KB an item, and W_UV, behind the launch itself: 64 queries of 64 heads behind a prefix read 40 MB in 11 us.
+// Bound by the records, 64 KB an item, and W_UV, behind the launch itself: 64 queries of 64 heads behind a prefix read 40 MB in 9 us.
 // grid (H, ceil(M / PER)), eight waves: PER queries of head x.  A wave joins the records of a query (PER 1: eight waves every eighth record of 64), eight
 // columns a lane, and leaves the context in LDS as TERMS bf16 terms; then a wave takes 16 output columns of all queries, its rows of W_UV as they lie.
 template <int TERMS, int PER>
@@ -1001,8 +1001,8 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
     const int vtiles = (a.V + 15) / 16;
     const auto rw = make_rsrc(a.w_uv + static_cast<int64_t>(h) * a.V * kLat, static_cast<uint32_t>(a.V) * (2 * kLat));
     // An operand's 16 neighbouring lanes are 16 rows of W_UV, and loaded like that take the load path three to four times as long as 64 bytes of
-    // four rows do.  So load 4 J + i is of rows i, 4 + i, 8 + i and 12 + i, 256 bytes of each, and turned() exchanges the lanes of a quad with
-    // the four loads: then operand 4 J + i is columns 128 J + 32 q4 + 8 i .. +8 of row r16.
+    // four rows do (4 x 200 tokens 54 us for 44, 6 long requests 15 for 11).  So load 4 J + i is of rows i, 4 + i, 8 + i and 12 + i, 256 bytes of
+    // each, and turned() exchanges the lanes of a quad with the four loads: then operand 4 J + i is columns 128 J + 32 q4 + 8 i .. +8 of row r16.
     u32x4 w[16];
     auto weights = [&](int vt) __attribute__((always_inline)) {         // (rows past the head's last are outside and load zeros)
         const uint32_t at = static_cast<uint32_t>(vt * 16 + (r16 & 12)) * (2 * kLat) + q4 * 64 + (r16 & 3) * 16;
@@ -1125,7 +1125,8 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
                     f32x4 &to = k & 1 ? o2[t] : o[t];
-                    to = q4_mfma_bf16(w[k], *reinterpret_cast<const u32x4 *>(ctx + (y * PER + t * 16 + r16 % kRows) * kCLd + (k >> 2) * 256 + q4 * 64 + (k & 3) * 16), to);
+                    const char *c = ctx + (y * PER + t * 16 + r16 % kRows) * kCLd + (k >> 2) * 256 + q4 * 64 + (k & 3) * 16;
+                    to = q4_mfma_bf16(w[k], *reinterpret_cast<const u32x4 *>(c), to);
                 }
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) o[t] += o2[t];
@@ -1235,9 +1236,9 @@ int launch_uv_of(const UvArgs &a, hipStream_t st) {
 template <int TERMS>
 int launch_uv(const UvArgs &a, hipStream_t st) {
     // The most queries to a block, which reads its head's W_UV, with which there are blocks for every CU (of 32 and 16 queries two a CU, of 8 one).
-    // Measured, us, 8 / 16 / 32 queries: 32 requests of 64 heads 15.0 / 17.8 / -, 25 of 96 16.0 / 11.5 / -, 64 of 64 16.6 / 10.6 / 16.6 (8), 120 of 64
-    // 32.4 / 16.6 / 16.0, 800 of 64 - / 60 / 53.  Few queries have waves enough for all a query's records: 6 of 64 heads, some 80 records each, 18.1 for
-    // a wave a query, 17.5 for eight.
+    // Measured, us, 8 / 16 / 32 queries: 32 requests of 64 heads 12.7 / 17.1 / 25.8, 25 of 96 13.4 / 10.2 / 13.4, 64 of 64 13.2 / 9.3 / 12.8, 120 of 64
+    // 24.4 / 12.6 / 13.8, 800 of 64 119 / 51.6 / 45.3.  Few queries have waves enough for all a query's records: 6 of 64 heads, some 80 records each,
+    // 16.4 for a wave a query, 11.6 for eight.
     if (a.H * cdiv(a.M, 16) > 512) return launch_uv_of<TERMS, 32>(a, st);
     if (a.H * cdiv(a.M, 8) > 256) return launch_uv_of<TERMS, 16>(a, st);
     if (a.M > 8) return launch_uv_of<TERMS, 8>(a, st);
