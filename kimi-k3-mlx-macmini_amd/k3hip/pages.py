@@ -103,7 +103,8 @@ class PageTable:
 
     def resize(self, target: torch.Tensor, tokens: int = 0) -> torch.Tensor:
         """All requests to ``target`` [batch] int32 positions -> slots of up to ``tokens`` new tokens each (``page_tables``).  None goes below
-        a common prefix."""
+        a common prefix.  One that grows by more than ``tokens`` has slots of the first ones only: the rest, on the pages of its row, is
+        the caller's to write before anything attends (``extend`` gives none more than it has slots)."""
         _per_sequence(target, self.batch, "target")
         if self.prefix is not None:
             target = target.clamp(min=len(self.prefix) * self.page_size)
@@ -114,14 +115,17 @@ class PageTable:
 
     def extend(self, counts: int | torch.Tensor, tokens: int | None = None) -> torch.Tensor:
         """Room for ``counts`` more tokens of every request (a number, or int32 [batch], 0 for a request that rests, below 0 for one that gives
-        so many back) -> slots [batch, tokens] (``tokens``: the most that a request gets; needed for a tensor).  A request for which there
-        is no page left gets none: its ``counts`` entry is 0, its slots are -1."""
+        so many back) -> slots [batch, tokens] (``tokens``: the most that a request gets; needed for a tensor, whose larger entries are cut to
+        it).  A request for which there is no page left gets none: its ``counts`` entry is 0, its slots are -1."""
         if isinstance(counts, torch.Tensor):
             _per_sequence(counts, self.batch, "counts")
             if tokens is None:
                 raise ValueError("tokens: the most new tokens of a request, where counts is a tensor")
+            counts = counts.clamp(max=int(tokens))
         else:
-            tokens = int(counts) if tokens is None else tokens
+            tokens = int(counts) if tokens is None else int(tokens)
+            if counts > tokens:
+                raise ValueError(f"{counts} new tokens of every request for {tokens} slots of each")
         return self.resize(self.lengths + counts, tokens)
 
     def truncate(self, lengths: torch.Tensor) -> None:

@@ -1,0 +1,27 @@
+"""What a batch's tables may be asked for: more tokens than there are slots, numbers that do not fit 32 bits, tokens given back by a number.  The
+tables' class over the definition of its one launch, without a GPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_mla_paged_host import _held, on_cpu  # noqa: F401
+
+I32 = torch.int32
+
+
+def _counts(*n):
+    return torch.tensor(n, dtype=I32)
+
+
+def test_no_request_gets_more_tokens_than_slots(on_cpu):
+    t = on_cpu.PageTable(3, 256, 12, page_size=32, device="cpu")
+    slots = t.extend(_counts(5, 2, 3), tokens=3)
+    assert t.lengths.tolist() == t.counts.tolist() == [3, 2, 3] == (slots >= 0).sum(1).tolist()
+    slots = t.extend(_counts(100, -1, 0), tokens=2)
+    assert t.lengths.tolist() == [5, 1, 3] and t.counts.tolist() == [2, 0, 0] == (slots >= 0).sum(1).tolist()
+    assert [len(r) for r in _held(t)] == [1, 1, 1]
+    with pytest.raises(ValueError, match="tokens"):
+        t.extend(4, tokens=2)
+    assert t.lengths.tolist() == [5, 1, 3]
+    assert t.extend(2, tokens=4).shape == (3, 4) and t.counts.tolist() == [2, 2, 2]
