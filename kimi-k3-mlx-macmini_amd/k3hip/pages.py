@@ -123,7 +123,7 @@ class PageTable:
                 raise ValueError("tokens: the most new tokens of a request, where counts is a tensor")
             counts = counts.clamp(max=int(tokens))
         else:
-            tokens = int(counts) if tokens is None else int(tokens)
+            tokens = max(int(counts), 0) if tokens is None else int(tokens)
             if counts > tokens:
                 raise ValueError(f"{counts} new tokens of every request for {tokens} slots of each")
         return self.resize(self.lengths + counts, tokens)

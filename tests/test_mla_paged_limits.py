@@ -25,3 +25,12 @@ def test_no_request_gets_more_tokens_than_slots(on_cpu):
         t.extend(4, tokens=2)
     assert t.lengths.tolist() == [5, 1, 3]
     assert t.extend(2, tokens=4).shape == (3, 4) and t.counts.tolist() == [2, 2, 2]
+
+
+def test_a_number_below_zero_gives_tokens_back(on_cpu):
+    t = on_cpu.PageTable(2, 256, 12, page_size=32, device="cpu")
+    t.extend(_counts(70, 3), tokens=70)
+    assert t.extend(-5).shape == (2, 0)
+    assert t.lengths.tolist() == [65, 0] and t.counts.tolist() == [0, 0] and [len(r) for r in _held(t)] == [3, 0]
+    assert t.extend(-2, tokens=1).tolist() == [[-1], [-1]] and t.lengths.tolist() == [63, 0] and [len(r) for r in _held(t)] == [2, 0]
+    assert t.extend(0).shape == (2, 0)
