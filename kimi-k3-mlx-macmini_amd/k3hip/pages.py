@@ -121,11 +121,14 @@ class PageTable:
             _per_sequence(counts, self.batch, "counts")
             if tokens is None:
                 raise ValueError("tokens: the most new tokens of a request, where counts is a tensor")
-            counts = counts.clamp(max=int(tokens))
+            tokens = int(tokens)
+            counts = counts.clamp(max=tokens)
         else:
             tokens = max(int(counts), 0) if tokens is None else int(tokens)
             if counts > tokens:
                 raise ValueError(f"{counts} new tokens of every request for {tokens} slots of each")
+        if tokens >= (1 << 31) - self.capacity:         # (lengths are int32)
+            raise ValueError(f"{tokens} new tokens of a request and the {self.capacity} it may hold do not fit 32 bits")
         return self.resize(self.lengths + counts, tokens)
 
     def truncate(self, lengths: torch.Tensor) -> None:

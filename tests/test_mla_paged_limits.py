@@ -34,3 +34,19 @@ def test_a_number_below_zero_gives_tokens_back(on_cpu):
     assert t.lengths.tolist() == [65, 0] and t.counts.tolist() == [0, 0] and [len(r) for r in _held(t)] == [3, 0]
     assert t.extend(-2, tokens=1).tolist() == [[-1], [-1]] and t.lengths.tolist() == [63, 0] and [len(r) for r in _held(t)] == [2, 0]
     assert t.extend(0).shape == (2, 0)
+
+
+@pytest.mark.parametrize("most", [2 ** 31 - 1, 2 ** 31 - 256])
+def test_lengths_do_not_wrap(on_cpu, monkeypatch, most):
+    """``lengths + counts`` is int32: past 2^31 it would be below zero, and the request would give all its pages back."""
+    t = on_cpu.PageTable(2, 256, 12, page_size=32, device="cpu")
+    t.extend(_counts(70, 3), tokens=70)
+    seen = []
+    monkeypatch.setattr(t, "resize", lambda target, tokens: seen.append(target.tolist()))
+    for counts in (_counts(most, 0), _counts(0, most), most):
+        with pytest.raises(ValueError, match="tokens"):
+            t.extend(counts, tokens=most)
+    assert not seen
+    t.extend(_counts(most, -2 ** 31), tokens=2 ** 31 - 257)
+    t.extend(2 ** 31 - 257)
+    assert seen == [[70 + 2 ** 31 - 257, 3 - 2 ** 31], [70 + 2 ** 31 - 257, 3 + 2 ** 31 - 257]]
