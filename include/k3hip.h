@@ -557,17 +557,18 @@ int64_t k3_page_tables_workspace_size(int64_t B);
  * their new tokens' rows.  Request b holds lengths[b] positions (taken as 0 .. blocks * page_size), its pages the first entries
  * of row b of table [B, blocks] (rows table_row entries apart); it is to hold target[b] (negative: 0).  free_list [pages]: its
  * entries from used[0] on (taken as 0 .. pages) are the pages that nobody holds.
- *   - A request that shrinks gives back its pages from the target's on, but none of its first shared[b] (shared null: none): all,
- *     in the batch's order, are written before entry `used` of the list, whose free entries begin at base = used - returned (never
+ *   - A request that shrinks gives back its pages from the target's on, but none of its first shared[b], which are not its own (shared
+ *     null: none): all, in the batch's order, are written before entry `used` of the list, whose free entries begin at base = used - returned (never
  *     below 0; more than `used` pages given back are dropped).  Its row of the table stays.
  *   - A request that grows takes its pages from base on, one request after the other, and they are written into its row; from the first
  *     one on that the list has not enough for, requests that need pages stay as they are.  So does one whose target does not fit `blocks`.
+ *     Pages that it takes in the places of shared ones, having come below them, are its own: shared[b] is written, the pages before those.
  *   - new_lengths [B], new_used [1]: what came of it; slots [B, tokens]: the row of request b's i-th new token in the pool, page *
  *     page_size + position % page_size, -1 past its new length (tokens 0: slots may be null).
  * new_lengths may be lengths (or target), and new_used may be used; other buffers must not overlap.  One launch up to 4096 tokens (B *
  * tokens) of up to 2048 requests, else two.  blocks * page_size < 2^31.  No counterpart in the reference, whose cache is one sequence's. */
 int k3_page_tables(int32_t *table, int64_t table_row, int64_t blocks, const int32_t *lengths, const int32_t *target,
-                   const int32_t *shared, int32_t *free_list, int64_t pages, const int32_t *used, int64_t page_size, int64_t B,
+                   int32_t *shared, int32_t *free_list, int64_t pages, const int32_t *used, int64_t page_size, int64_t B,
                    int64_t tokens, int32_t *new_lengths, int32_t *new_used, int32_t *slots, void *workspace,
                    int64_t workspace_bytes, void *stream);
 

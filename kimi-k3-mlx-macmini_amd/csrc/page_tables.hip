@@ -7,6 +7,7 @@
 //   takes    a request that grows takes its pages from base on, one request after the other; the first that the list does not
 //            hold enough for, and every later one that needs pages, stays as it is (so the ones that get theirs are those whose running
 //            sum of needs fits: one prefix sum answers for all of them)
+//            Pages that it takes in the places of shared ones are its own: shared[b] comes down to the pages before them
 //   slots    new token i of request b -> its row in the pool, page * page_size + position % page_size, or -1
 // A page taken from below `used` is one that was just given back: it is looked up in the giver's own row (by a binary search of the
 // running sums), so nothing waits for the list to be written.
@@ -22,7 +23,9 @@
 namespace k3 {
 namespace {
 
+constexpr int64_t kMaxRequests = 65535;
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+static_assert((kMaxRequests + kPlanThreads - 1) / kPlanThreads <= 64, "a bit for each of a thread's requests");
 constexpr int kLdsRequests = 2048;      // the plan's records of so many requests fit in LDS
 constexpr int64_t kAlone = 4096;        // tokens (requests x new tokens) that the planning block does itself
 
@@ -35,8 +38,8 @@ struct Record {
 struct TablesArgs {
     int32_t *table;
     int64_t ld;
-    const int32_t *lengths, *target, *shared;
-    int32_t *free_list;
+    const int32_t *lengths, *target;
+    int32_t *shared, *free_list;
     const int32_t *used;
     int32_t *new_lengths, *new_used, *slots;
     Record *records;                    // [B], and behind them base and used
@@ -110,13 +113,15 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(TablesArgs a) {
     const int most = a.W << a.shift;
     const int used = min(max(a.used[0], 0), a.N);
     if (tid == 0) granted = 0;
+    uint64_t below = 0;                 // of this thread's requests (64 at most): those that grow from below their shared pages
     Sum2 own{0, 0};                     // given back, needed
     for (int b = first; b < last; ++b) {
         const int len = min(max(a.lengths[b], 0), most), target = max(a.target[b], 0);
         const int have = pages_of(len, a.shift);
         const bool fits = target <= most;
         const int want = fits ? pages_of(target, a.shift) : have;
-        const int keep = a.shared ? max(want, a.shared[b]) : want;
+        const int shared = a.shared ? a.shared[b] : 0, keep = max(want, shared);
+        if (want > have && shared > have) below |= 1ull << (b - first);
         const int give = want < have ? max(have - keep, 0) : 0;
         rec[b] = Record{len, fits ? target : len, own.x, give, own.y};
         own.x += give, own.y += max(want - have, 0);
@@ -130,6 +135,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(TablesArgs a) {
         const int need = max(pages_of(r.to, a.shift) - pages_of(r.len, a.shift), 0), at = before.y + r.at;
         if (need && at + need > left) r.to = r.len;
         else got = max(got, need ? at + need : 0);
+        if ((below >> (b - first) & 1) && r.to != r.len) a.shared[b] = pages_of(r.len, a.shift);
         r.before += before.x, r.at = base + at;
         rec[b] = r;
         a.new_lengths[b] = r.to;
@@ -170,7 +176,7 @@ using namespace k3;
 extern "C" int64_t k3_page_tables_workspace_size(int64_t B) { return B <= 0 ? 0 : (B + 1) * static_cast<int64_t>(sizeof(Record)); }
 
 extern "C" int k3_page_tables(int32_t *table, int64_t table_row, int64_t blocks, const int32_t *lengths, const int32_t *target,
-                              const int32_t *shared, int32_t *free_list, int64_t pages, const int32_t *used, int64_t page_size, int64_t B,
+                              int32_t *shared, int32_t *free_list, int64_t pages, const int32_t *used, int64_t page_size, int64_t B,
                               int64_t tokens, int32_t *new_lengths, int32_t *new_used, int32_t *slots, void *workspace,
                               int64_t workspace_bytes, void *stream) {
     if (B == 0) return K3_OK;
@@ -179,7 +185,7 @@ extern "C" int k3_page_tables(int32_t *table, int64_t table_row, int64_t blocks,
         return set_error(K3_ERR_NULL, "page tables: null pointer");
     if (page_size < 1 || page_size > (1 << 16) || (page_size & (page_size - 1)))
         return set_error(K3_ERR_SHAPE, "page tables: page_size=%lld must be a power of two up to 65536", (long long)page_size);
-    if (B < 0 || B > 65535 || blocks < 0 || blocks * page_size >= (1ll << 31) || B * blocks >= (1ll << 31) || pages < 0 || pages >= (1ll << 31) ||
+    if (B < 0 || B > kMaxRequests || blocks < 0 || blocks * page_size >= (1ll << 31) || B * blocks >= (1ll << 31) || pages < 0 || pages >= (1ll << 31) ||
         tokens < 0 || tokens >= (1ll << 31) || B * tokens >= (1ll << 40))
         return set_error(K3_ERR_SHAPE, "page tables: B=%lld, %lld blocks of %lld, %lld pages or %lld tokens out of range", (long long)B,
                          (long long)blocks, (long long)page_size, (long long)pages, (long long)tokens);

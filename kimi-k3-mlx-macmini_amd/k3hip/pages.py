@@ -32,7 +32,8 @@ def page_tables(table: torch.Tensor, lengths: torch.Tensor, target: torch.Tensor
     All int32 device tensors.  ``table`` [B, blocks]: request b's pages, in order, ceil(lengths[b] / page_size) of them; changed in
     place.  ``target`` [B]: the lengths to come to (negative: 0).  ``free`` [pages]: its entries from ``used`` [1] on are the pages that nobody
     holds; changed in place, where pages are given back.  ``shared`` [B]: so many of a request's first pages are not its own and are never
-    given back (a request that comes below them and grows again takes pages of its own in their places).  ``inplace``: ``lengths`` and ``used`` are written over instead of new tensors.
+    given back; changed in place: a request that has come below them and grows again takes pages of its own in their places, and its entry comes down to
+    what is left of them.  ``inplace``: ``lengths`` and ``used`` are written over instead of new tensors.
 
     Pages given back come in front of the list's free entries, in the batch's order, and can be taken in the same call.  Pages are taken
     in the batch's order; from the first request on that there are not enough for, requests that need pages stay at their length, as does one whose

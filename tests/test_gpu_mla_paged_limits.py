@@ -31,3 +31,52 @@ def test_counts_above_the_slots_are_cut():
         assert t.counts.tolist() == [3, 2, 0] and t.lengths.tolist() == [43, 33, 7]
         outs.append(layer(x[:, :3], cache)[0])
     assert bool((outs[0] == outs[1]).all()) and bool(outs[0][0].any()) and not bool(outs[0][2].any())
+
+
+# ------------------------------------------------------------------------------- pages that a request shares
+def _account(table, lengths, shared, free, used, page, common):
+    """Every page is common, in one request's row behind its shared ones, or free; none is in two of these, none in none."""
+    held = [p for row, n, s in zip(table.tolist(), lengths.tolist(), shared.tolist()) for p in row[max(s, 0):-(-n // page)]]
+    flat = held + list(common) + free.tolist()[int(used):]
+    assert sorted(flat) == list(range(len(free))), (held, flat)
+
+
+@pytest.mark.parametrize("tokens", [0, 5000])         # (one launch, two)
+def test_a_request_below_its_shared_pages_loses_none(tokens):
+    from k3hip.pages import page_tables
+    page = 32
+    table, free, used = _whole([[0, 1, -1, -1]]), _whole([0, 1, 2, 3, 4, 5]), _whole([2])
+    lengths, shared = _whole([64]), _whole([2])
+    for target, held, its in ((0, 0, 2), (96, 96, 0), (0, 0, 0), (128, 128, 0), (128, 128, 0), (40, 40, 0), (0, 0, 0), (96, 96, 0)):
+        page_tables(table, lengths, _whole([target]), free, used, page, tokens=tokens, shared=shared, inplace=True)
+        assert lengths.tolist() == [held] and shared.tolist() == [its], target
+        _account(table, lengths, shared, free, used, page, (0, 1))
+    # one that comes below some of them only; one that gets no page keeps its account
+    table, free, used = _whole([[0, 1, 2, 3, -1, -1], [0, 1, 2, -1, -1, -1]]), _whole(list(range(8))), _whole([4])
+    lengths, shared = _whole([128, 0]), _whole([3, 3])
+    for target, held, its in (([40, 0], [40, 0], [3, 3]), ([65, 192], [65, 0], [2, 3]), ([160, 0], [160, 0], [2, 3]), ([0, 1], [0, 1], [2, 0])):
+        page_tables(table, lengths, _whole(target), free, used, page, tokens=tokens, shared=shared, inplace=True)
+        assert lengths.tolist() == held and shared.tolist() == its, target
+        _account(table, lengths, shared, free, used, page, (0, 1, 2))
+
+
+@pytest.mark.parametrize("B,page,tokens", [(6, 32, 3), (300, 16, 1), (2500, 8, 2)])
+def test_no_page_is_lost_on_the_way(B, page, tokens):
+    """Requests that begin with common pages, below them and above them again, in any order."""
+    import random
+
+    from k3hip.pages import page_tables
+    rng = random.Random(B)
+    width, common = 7, [5, 0, 3]
+    pool = 3 + 4 * B
+    rest = [p for p in range(pool) if p not in common]
+    rng.shuffle(rest)
+    table = _whole([common + [-1] * (width - 3) for _ in range(B)])
+    free, used = _whole(common + rest), _whole([3])
+    lengths, shared = torch.full((B,), 3 * page, dtype=I32, device="cuda"), torch.full((B,), 3, dtype=I32, device="cuda")
+    for step in range(25):
+        now = lengths.tolist()
+        to = [rng.choice([0, n, n + 1, n - page, n + page, rng.randint(0, width * page)]) for n in now]
+        page_tables(table, lengths, _whole(to), free, used, page, tokens=tokens, shared=shared, inplace=True)
+        _account(table, lengths, shared, free, used, page, common)
+    assert min(shared.tolist()) == 0
