@@ -595,7 +595,7 @@ int64_t k3_mla_paged_workspace_size(int64_t B, int64_t T, int64_t H, int64_t max
  *   w_uv [H, v, 512] bf16; lat, rot: as k3_mla_paged_append's, all pitches whole 16 bytes; page_size a power of two, 32 .. 65536;
  * lengths int32 [B] on the device (taken as 0 .. max_length, at most blocks * page_size), counts int32 [B] on the device (taken as 0 .. T) or
  *   null: T; gate [B, T, H, v] fp32 logits or null: o times sigmoid(gate); out [B, T, H, v] contiguous, out_dtype.
- * A query that sees nothing (also: t >= counts[b]) gets zeros.  Deterministic.  fp16 pages: the absorbed queries enter as one fp16 term
+ * A query that sees nothing (also: t >= counts[b]) gets zeros, whatever its gate.  Deterministic.  fp16 pages: the absorbed queries enter as one fp16 term
  * for a bf16 out (2^-11, and none closer than 2^-38 of the largest of its 128 columns), two for fp32 (2^-22); probabilities as one (2^-11) or two
  * (2^-22), none closer than 2^-32 of the row's largest; for a bf16 out the contexts of ranges of positions as fp16 (2^-11, and no finer than
  * 2^-25, as the pages).  bf16 pages: two bf16 terms of both for a bf16 out (2^-16), three for fp32 (2^-24).  The context before W_UV: two

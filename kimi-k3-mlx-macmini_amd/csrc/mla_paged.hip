@@ -994,8 +994,9 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
     static_assert(PER == 1 || PER % 8 == 0, "waves to a query, or queries to a wave");
     constexpr int kTiles = (PER + 15) / 16, kRows = PER < 16 ? PER : 16, kSide = PER == 8 ? 12 : 4;  // kSide: records on their way
     extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ float seen[PER];                                 // a query's sum: 0 where it sees nothing
     char *const ctx = lds;                                      // [TERMS][PER][kCLd]
-    float *const sums = reinterpret_cast<float *>(lds + TERMS * PER * kCLd);    // PER 1: [8][512], then maxima and sums [8]
+    float *const sums = reinterpret_cast<float *>(lds + TERMS * PER * kCLd);    // PER 1: [8][512]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, q4 = lane >> 4;
     const int h = blockIdx.x, m0 = blockIdx.y * PER;
     const int vtiles = (a.V + 15) / 16;
@@ -1094,14 +1095,15 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
         }
         if constexpr (PER > 1) {
             const float inv = l == 0.f ? 0.f : 1.0f / l;
+            if (lane == 0) seen[i] = l;
             store(i, x * inv, y * inv);
         } else {
             *reinterpret_cast<f32x4 *>(sums + wave * kLat + 4 * lane) = x;
             *reinterpret_cast<f32x4 *>(sums + wave * kLat + 256 + 4 * lane) = y;
-            if (wave == 0 && lane == 0) sums[8 * kLat] = l;
+            if (wave == 0 && lane == 0) seen[0] = l;
             __syncthreads();
             if (wave == 0) {
-                const float all = sums[8 * kLat], inv = all == 0.f ? 0.f : 1.0f / all;
+                const float all = seen[0], inv = all == 0.f ? 0.f : 1.0f / all;
 #pragma unroll
                 for (int k = 1; k < 8; ++k) {
                     x += *reinterpret_cast<const f32x4 *>(sums + k * kLat + 4 * lane);
@@ -1138,8 +1140,9 @@ __global__ __launch_bounds__(512, PER == 8 ? 2 : 4) void uv_kernel(UvArgs a) {
             const int64_t to = ((static_cast<int64_t>(b) * a.Tall + tq) * a.H + h) * a.V + v;
             if (a.gate) {
                 const f32x4 g = *reinterpret_cast<const f32x4 *>(a.gate + to);
+                const bool any = seen[t * 16 + r16] != 0.f;     // (the gate of a query that sees nothing may be anything: a row of padding's)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[t][i] = o[t][i] / (1.0f + expf(-g[i]));
+                for (int i = 0; i < 4; ++i) o[t][i] = any ? o[t][i] / (1.0f + expf(-g[i])) : 0.f;
             }
             if (a.out_bf16)
                 *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + to) = u32x2{q4_pack_bf16(o[t][0], o[t][1]), q4_pack_bf16(o[t][2], o[t][3])};
@@ -1225,7 +1228,7 @@ int launch_attend(const AttendArgs &a, int most, hipStream_t st) {
 
 template <int TERMS, int PER>
 int launch_uv_of(const UvArgs &a, hipStream_t st) {
-    constexpr int bytes = TERMS * PER * kCLd + (PER == 1 ? (8 * kLat + 16) * 4 : 0);
+    constexpr int bytes = TERMS * PER * kCLd + (PER == 1 ? 8 * kLat * 4 : 0);
     static const hipError_t attr =
         hipFuncSetAttribute(reinterpret_cast<const void *>(uv_kernel<TERMS, PER>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     const int rc = check_hip(attr, "mla paged: output LDS size");

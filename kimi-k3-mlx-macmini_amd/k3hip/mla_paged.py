@@ -105,7 +105,7 @@ def mla_paged_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Ten
     size from 32 on; table int32 [B, blocks]: position j of sequence b lies in page table[b, j // page_size].  Causal: the queries are each
     sequence's last positions; with n = counts[b] (int32 [B], default T) query t < n sees positions 0 .. lengths[b] - n + t, and
     later ones see nothing.  ``lengths`` int32 [B] on the device; ``max_length``: none is longer (default: what the table holds; longer ones
-    are cut).  A query that sees nothing gives zeros; a position on a page outside the pool counts as not there.
+    are cut).  A query that sees nothing gives zeros, whatever its gate; a position on a page outside the pool counts as not there.
 
     ``prefix`` int32 [n]: the pages of the first n * page_size positions of every sequence, read and multiplied once for the whole batch;
     ``table`` counts from position 0 all the same, its first n columns are not read.

@@ -80,3 +80,47 @@ def test_no_page_is_lost_on_the_way(B, page, tokens):
         page_tables(table, lengths, _whole(to), free, used, page, tokens=tokens, shared=shared, inplace=True)
         _account(table, lengths, shared, free, used, page, common)
     assert min(shared.tolist()) == 0
+
+
+# ------------------------------------------------------------------------------- rows of no query
+@pytest.mark.parametrize("out", [BF16, F32])
+@pytest.mark.parametrize("B,T,H", [(3, 2, 8), (5, 4, 16), (6, 40, 24), (9, 80, 32)])       # (one to 32 queries a block of the last launch)
+def test_a_gate_that_is_no_number_leaves_zeros_where_nothing_is_seen(B, T, H, out):
+    import _paged_oracle as oracle
+    from k3hip.mla_paged import mla_paged_attention
+    g = torch.Generator().manual_seed(B)
+    case = oracle.make(g, B, T, H, [T + 30 + 7 * b for b in range(B)], page=32, x=F32)
+    counts = _whole([T // 2] + [T] * (B - 1))
+    case["lengths"][1] = 0
+    case["table"][2] = -1                                           # (no page of it is in the pool)
+    gate = torch.randn(B, T, H * 128, generator=g).cuda()
+    clean = mla_paged_attention(**case, counts=counts, gate=gate, out_dtype=out)
+    nothing = torch.zeros(B, T, dtype=torch.bool, device="cuda")
+    nothing[0, T // 2:] = nothing[1] = nothing[2] = True
+    for value in (float("nan"), float("-inf"), float("inf")):
+        bad = torch.where(nothing[..., None], torch.full_like(gate, value), gate)
+        got = mla_paged_attention(**case, counts=counts, gate=bad, out_dtype=out)
+        assert not bool(got[nothing].any()) and bool((got == clean).all()) and bool(got[~nothing].any())
+
+
+@pytest.mark.parametrize("gate", [True, False])
+@pytest.mark.parametrize("heads,T", [(4, 3), (16, 40)])
+def test_padding_that_is_no_number_stays_out_of_a_step(heads, T, gate):
+    """Rows past a request's tokens hold whatever the caller's buffer does: their outputs are zeros, the others' and the cache as with zeros there."""
+    from k3hip.mla_paged import new_cache_paged
+    from k3hip.pages import PageTable
+    layer, _ = _layer(heads, gate)
+    x = torch.randn(3, T, HID, generator=torch.Generator().manual_seed(2)).cuda()
+    counts = [T, 1, 0]
+    outs, pools = [], []
+    for padding in (0.0, float("nan"), float("inf")):
+        t = PageTable(3, 128, 12, page_size=32)
+        cache = new_cache_paged(t)
+        t.extend(_whole(counts), tokens=T)
+        x = x.clone()
+        for b, n in enumerate(counts):
+            x[b, n:] = padding
+        outs.append(layer(x, cache)[0])
+        pools.append(torch.cat((cache.latent, cache.rot), -1))
+    for out, pool in zip(outs, pools):
+        assert not bool(out[1, 1:].any()) and not bool(out[2].any()) and bool((out == outs[0]).all()) and bool((pool == pools[0]).all())
