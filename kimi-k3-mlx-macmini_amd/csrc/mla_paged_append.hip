@@ -14,6 +14,7 @@ namespace k3 {
 namespace {
 
 constexpr int kLat = 512, kRot = 64;
+constexpr int64_t kMaxRow = 1 << 23;         // blocks of a row of the grid
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct AppendArgs {
@@ -48,7 +49,7 @@ __device__ __forceinline__ uint16_t rounded(float v) {
 template <typename CT, typename RT, bool F16>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     const int lane = threadIdx.x & 63;
-    const int64_t m = blockIdx.x * 4ll + (threadIdx.x >> 6);
+    const int64_t m = (blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (m >= a.M) return;
     const int64_t slot = a.slots[m];
     if (slot < 0 || slot >= a.rows) return;
@@ -83,11 +84,13 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 
 template <typename CT, typename RT>
 int launch(const AppendArgs &a, bool f16, hipStream_t st) {
-    const unsigned blocks = static_cast<unsigned>(cdiv(a.M, 4));
+    // (a row of blocks has at most 2^32 - 1 threads, and a launch of more goes out short without an error)
+    const int64_t blocks = cdiv(a.M, 4), rows = cdiv(blocks, kMaxRow);
+    const dim3 grid(static_cast<unsigned>(cdiv(blocks, rows)), static_cast<unsigned>(rows));
     if (f16)
-        paged_append_kernel<CT, RT, true><<<blocks, 256, 0, st>>>(a);
+        paged_append_kernel<CT, RT, true><<<grid, 256, 0, st>>>(a);
     else
-        paged_append_kernel<CT, RT, false><<<blocks, 256, 0, st>>>(a);
+        paged_append_kernel<CT, RT, false><<<grid, 256, 0, st>>>(a);
     return check_hip(hipGetLastError(), "mla paged append: launch");
 }
 

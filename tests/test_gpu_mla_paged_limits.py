@@ -124,3 +124,21 @@ def test_padding_that_is_no_number_stays_out_of_a_step(heads, T, gate):
         pools.append(torch.cat((cache.latent, cache.rot), -1))
     for out, pool in zip(outs, pools):
         assert not bool(out[1, 1:].any()) and not bool(out[2].any()) and bool((out == outs[0]).all()) and bool((pool == pools[0]).all())
+
+
+# ------------------------------------------------------------------------------- more than a launch's row of blocks
+def test_append_of_more_tokens_than_a_row_of_blocks():
+    """2^26 tokens are 2^32 threads; most slots are outside the pool, so only a few of them are written."""
+    from k3hip.mla_paged import mla_paged_append
+    M = (1 << 26) + 5
+    row = torch.randn(2, 1, 576, generator=torch.Generator().manual_seed(1)).cuda()
+    c, r = row[:1, :, :512].expand(1, M, 512), row[:1, :, 512:].expand(1, M, 64)        # (one row, M times)
+    slots = torch.full((1, M), -1, dtype=I32, device="cuda")
+    written = {0: 3, 7: 40, (1 << 26) - 1: 31, 1 << 26: 0, M - 1: 63}
+    for m, s in written.items():
+        slots[0, m] = s
+    lat, rot = torch.zeros(2, 32, 512, dtype=F16, device="cuda"), torch.zeros(2, 32, 64, dtype=F16, device="cuda")
+    mla_paged_append(c, r, slots, lat, rot)
+    want = torch.zeros(64, 576, dtype=F16, device="cuda")
+    want[list(written.values())] = row[0].to(F16)
+    assert bool((torch.cat((lat, rot), -1).view(64, 576) == want).all())
