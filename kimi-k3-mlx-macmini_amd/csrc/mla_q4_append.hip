@@ -54,7 +54,7 @@ __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
 template <typename CT, typename RT>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const int lane = threadIdx.x & 63, b = blockIdx.y;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t i = (static_cast<int64_t>(blockIdx.z) * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
     const int64_t n = a.counts ? min(static_cast<int64_t>(a.counts[b]), a.T) : a.T;
     const int64_t at = (a.start ? a.start[b] : a.start0) + i;
     if (i >= n || at < 0 || at >= a.cap) return;
@@ -104,7 +104,9 @@ int mla_q4_append(const void *c, int64_t c_b, int64_t c_t, int c_dtype, const vo
                   float *weight, int64_t w_b, int64_t B, int64_t T, int64_t cap, hipStream_t st) {
     const AppendArgs a{c,   r,   c_b, c_t, r_b, r_t,   static_cast<uint8_t *>(packed), static_cast<uint8_t *>(scales),
                        static_cast<uint16_t *>(rot), p_b, p_t, s_b, s_t, o_b, o_t, start, counts, start0, weight, w_b, norm, eps, T, cap};
-    const dim3 grid(static_cast<unsigned>(cdiv(T, 4)), static_cast<unsigned>(B));
+    // (a row of blocks has at most 2^32 - 1 threads, and a launch of more goes out short without an error)
+    const int64_t blocks = cdiv(T, 4), rows = cdiv(blocks, 1 << 23);
+    const dim3 grid(static_cast<unsigned>(cdiv(blocks, rows)), static_cast<unsigned>(B), static_cast<unsigned>(rows));
     if (c_dtype == K3_F32)
         r_dtype == K3_F32 ? append_kernel<float, float><<<grid, 256, 0, st>>>(a) : append_kernel<float, uint16_t><<<grid, 256, 0, st>>>(a);
     else
