@@ -497,7 +497,7 @@ int64_t k3_mla_q4_workspace_size(int64_t B, int64_t T, int64_t H, int64_t v_dim,
  * gate [B, T, H, v] fp32 logits or null: o times sigmoid(gate);
  * out [B, T, H, v] contiguous, out_dtype; weight fp32 rows w_batch >= max_length floats apart, positions past
  *   lengths[b] left as they are.
- * A query that sees nothing (also: t >= counts[b]) gets zeros and adds nothing to weight.  Deterministic.  The cache's
+ * A query that sees nothing (also: t >= counts[b]) gets zeros, whatever its gate, and adds nothing to weight.  Deterministic.  The cache's
  * values enter exactly; the absorbed queries to 2^-12 of a unit under their group's largest for a bf16 out without weight,
  * else 2^-22; the probabilities, for the context, to 2^-11 for a bf16 out, 2^-22 for fp32, and none closer than 2^-35 of the
  * largest in its range (fp16's smallest step: n positions under that beside one lose up to n 2^-35 of the output; the divisor

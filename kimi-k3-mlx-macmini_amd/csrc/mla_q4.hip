@@ -745,18 +745,22 @@ struct UvArgs {
     const float *gate;       // [B, Tall, H, V] or null
     float *stats;            // [B][rows]: log2 of what a probability's exponential is divided by; or null
     const int2 *seq;         // the sequences' records, or null: NS each
+    const int32_t *lengths, *counts;    // [B] or null: length, and Tall
     Rows order;
-    int M, V, rows, NS, Tall, t0;
+    int M, V, rows, NS, Tall, t0, length;
     __device__ __forceinline__ int2 records(int b) const { return seq ? seq[b] : make_int2(b * NS, NS); }  // first, number (at most NS)
 };
 constexpr int kMaxSplits = 256;
 
 __device__ __forceinline__ void store_out4(const UvArgs &a, int m, int h, int v, f32x4 o) {
-    const int64_t at = ((static_cast<int64_t>(a.order.seq(m)) * a.Tall + a.t0 + a.order.token(m)) * a.order.H + h) * a.V + v;
+    const int b = a.order.seq(m), tq = a.t0 + a.order.token(m);
+    const int64_t at = ((static_cast<int64_t>(b) * a.Tall + tq) * a.order.H + h) * a.V + v;
     if (a.gate) {
         const f32x4 g = *reinterpret_cast<const f32x4 *>(a.gate + at);
+        // (the gate of a query that sees nothing may be anything: a row of padding's)
+        const bool any = q4_sees(tq, a.counts ? min(a.counts[b], a.Tall) : a.Tall, a.lengths ? min(a.lengths[b], a.length) : a.length) > 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = o[i] / (1.0f + expf(-g[i]));
+        for (int i = 0; i < 4; ++i) o[i] = any ? o[i] / (1.0f + expf(-g[i])) : 0.f;
     }
     if (a.out_bf16)
         *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + at) = u32x2{q4_pack_bf16(o[0], o[1]), q4_pack_bf16(o[2], o[3])};
@@ -1456,7 +1460,7 @@ extern "C" int k3_mla_q4_attention(const void *q_nope, int64_t qn_batch, int64_t
         u.stats = weight ? reinterpret_cast<float *>(ws + p.stats) : nullptr;
         u.seq = qa.ranges.seq;
         u.order = order, u.M = M, u.V = static_cast<int>(v_dim), u.rows = rows, u.NS = p.NS;
-        u.Tall = static_cast<int>(T), u.t0 = a.t0;
+        u.Tall = static_cast<int>(T), u.t0 = a.t0, u.lengths = lengths, u.counts = counts, u.length = a.length;
         rc = launch_uv(u, p.many, st);
         if (rc) return rc;
         if (weight && max_length > 0) {

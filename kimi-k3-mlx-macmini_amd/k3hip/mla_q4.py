@@ -171,7 +171,7 @@ def mla_q4_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Tensor
     rot [B, cap, .].  Causal: the queries are each sequence's last T positions, query t sees positions 0 ..
     length - T + t.  ``lengths``: the sequences' lengths, a whole number for all or an int32 [B] device tensor (default: the
     capacity); ``counts`` int32 [B]: sequence b has only counts[b] queries, the first ones of its T.  A query that
-    sees nothing gives zeros.  A batch of more than 65,536 rows (sequences x heads) goes out in parts.
+    sees nothing gives zeros, whatever its gate.  A batch of more than 65,536 rows (sequences x heads) goes out in parts.
 
     The cache's rows are read as they lie: ``packed`` and ``rot`` 16-byte aligned with pitches of whole 16 bytes, ``scales`` 4.
 
