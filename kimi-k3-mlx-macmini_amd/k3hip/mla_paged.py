@@ -125,7 +125,7 @@ def mla_paged_attention(q_nope: torch.Tensor, q_rot: torch.Tensor, wk: torch.Ten
     if B == 0 or Tq == 0:
         return out
     if B > MAX_SEQUENCES or (B * H > MAX_ROWS and B > 1):
-        most_at_once = max(1, min(MAX_SEQUENCES, MAX_ROWS // H))
+        most_at_once = max(1, min(MAX_SEQUENCES, MAX_ROWS // max(1, H)))
         for b in range(0, B, most_at_once):
             part = slice(b, min(B, b + most_at_once))
             out[part] = mla_paged_attention(q_nope[part], q_rot[part], wk, wv, lat, rot, table[part], lengths[part], scale,

@@ -50,3 +50,13 @@ def test_lengths_do_not_wrap(on_cpu, monkeypatch, most):
     t.extend(_counts(most, -2 ** 31), tokens=2 ** 31 - 257)
     t.extend(2 ** 31 - 257)
     assert seen == [[70 + 2 ** 31 - 257, 3 - 2 ** 31], [70 + 2 ** 31 - 257, 3 + 2 ** 31 - 257]]
+
+
+def test_a_large_batch_without_heads_is_refused_as_a_small_one_is(monkeypatch):
+    import test_mla_paged_host as host
+    calls = host._launches(monkeypatch)
+    w = torch.zeros(0, 128, 512, dtype=torch.bfloat16)
+    for B in (2, 70000):
+        host._attend(q_nope=torch.zeros(B, 1, 0, 128), q_rot=torch.zeros(B, 1, 0, 64), wk=w, wv=w, table=torch.zeros(B, 1, dtype=I32),
+                     lengths=torch.zeros(B, dtype=I32))
+    assert [c[1][28] for c in calls] == [2, 65535, 4465] and {c[1][30] for c in calls} == {0}       # (the entry point refuses 0 heads)
