@@ -436,6 +436,8 @@ class MLAAttention:
         nh, nope, rope, vhd, klr = (c.num_attention_heads, c.qk_nope_head_dim, c.qk_rope_head_dim,
                                     c.v_head_dim, c.kv_lora_rank)
         hidden, ql = x.shape[-1], self.q_a.shape[0]
+        if isinstance(cache, MLACachePaged):
+            raise ValueError("the one-call step takes a cache of one sequence; call the layer for the paged cache")
         if cache is None and self.cache_bits == 4:
             cache = new_cache_q4(1, 1, bool(getattr(c, "mla_cache_weights", False)), x.device)
         elif cache is None:

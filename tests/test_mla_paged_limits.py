@@ -60,3 +60,19 @@ def test_a_large_batch_without_heads_is_refused_as_a_small_one_is(monkeypatch):
         host._attend(q_nope=torch.zeros(B, 1, 0, 128), q_rot=torch.zeros(B, 1, 0, 64), wk=w, wv=w, table=torch.zeros(B, 1, dtype=I32),
                      lengths=torch.zeros(B, dtype=I32))
     assert [c[1][28] for c in calls] == [2, 65535, 4465] and {c[1][30] for c in calls} == {0}       # (the entry point refuses 0 heads)
+
+
+def test_the_one_call_step_refuses_a_paged_cache(on_cpu):
+    from types import SimpleNamespace
+
+    from k3hip.mla import MLAAttention
+    from k3hip.mla_paged import new_cache_paged
+    cfg = SimpleNamespace(num_attention_heads=2, q_lora_rank=16, kv_lora_rank=512, qk_nope_head_dim=8, qk_rope_head_dim=64, v_head_dim=8, q_head_dim=72,
+                          rms_norm_eps=1e-5)
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    layer = MLAAttention(cfg, {"q_a_proj.weight": z(16, 32), "q_a_layernorm.weight": z(16), "q_b_proj.weight": z(144, 16), "o_proj.weight": z(32, 16),
+                               "kv_a_proj_with_mqa.weight": z(576, 32), "kv_a_layernorm.weight": z(512), "kv_b_proj.weight": z(32, 512)})
+    t = on_cpu.PageTable(1, 64, 4, page_size=32, device="cpu")
+    t.extend(1)
+    with pytest.raises(ValueError, match="paged"):
+        layer.decode_step(torch.zeros(1, 1, 32), new_cache_paged(t))
