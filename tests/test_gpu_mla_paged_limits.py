@@ -142,3 +142,74 @@ def test_append_of_more_tokens_than_a_row_of_blocks():
     want = torch.zeros(64, 576, dtype=F16, device="cuda")
     want[list(written.values())] = row[0].to(F16)
     assert bool((torch.cat((lat, rot), -1).view(64, 576) == want).all())
+
+
+# ------------------------------------------------------------------------------- batches and queries in parts
+def _sampled(case, got, which, out, **kw):
+    import _paged_oracle as oracle
+    from test_gpu_mla_paged import _check
+    for b in which:
+        part = {k: v[b:b + 1] if k in ("q_nope", "q_rot", "table", "lengths") else v for k, v in case.items()}
+        _check(got[b:b + 1], *oracle.attention(**part, out_dtype=out, **{k: v[b:b + 1] for k, v in kw.items()}), label=b)
+
+
+@pytest.mark.parametrize("H,pages,out", [(60, F16, BF16), (16, F16, BF16), (32, F16, F32), (40, BF16, BF16), (16, BF16, F32), (24, F16, F32)])
+def test_more_than_1024_sequences_behind_a_prefix(H, pages, out):
+    """(whose ranges' length is not searched for), one of them long; groups that fill whole tiles and groups that do not."""
+    import _paged_oracle as oracle
+    from k3hip.mla_paged import mla_paged_attention
+    B = 1030
+    lens = [96 + b % 70 for b in range(B)]
+    lens[3], lens[700], lens[1029] = 96 + 3000, 20, 0
+    case = oracle.make(torch.Generator().manual_seed(H), B, 1, H, lens, page=32, pages_dtype=pages, x=BF16, prefix=96)
+    got = mla_paged_attention(**case, out_dtype=out)
+    _sampled(case, got, (0, 3, 4, 256, 700, 1028), out)
+    assert not bool(got[1029].any())
+
+
+@pytest.mark.parametrize("pages,out", [(F16, BF16), (F16, F32), (BF16, BF16), (BF16, F32)])
+def test_passes_with_counts_gate_and_prefix(pages, out):
+    """86,400 rows: 227 queries of each, then 73 (of requests that have 300, 228, 150 and none)."""
+    import _paged_oracle as oracle
+    from k3hip.mla_paged import mla_paged_attention
+    B, T, H = 4, 300, 72
+    g = torch.Generator().manual_seed(5)
+    case = oracle.make(g, B, T, H, [128 + 320, 228, 128 + 190, 128 + 64], page=64, pages_dtype=pages, x=F32, prefix=128)
+    counts, gate = _whole([999, 228, 150, 0]), 2 * torch.randn(B, T, H * 128, generator=g).cuda()
+    gate[1, 228:] = gate[2, 150:] = gate[3] = float("nan")
+    got = mla_paged_attention(**case, counts=counts, gate=gate, out_dtype=out)
+    _sampled(case, got, range(3), out, counts=counts, gate=gate.nan_to_num())
+    assert not bool(got[1, 228:].any()) and not bool(got[2, 150:].any()) and not bool(got[3].any())
+
+
+@pytest.mark.parametrize("pages", [F16, BF16])
+def test_counts_and_gate_at_an_fp32_result(pages):
+    """What the layer calls: fp32 queries and results, counts and a gate; few queries and many, behind a prefix and without."""
+    import _paged_oracle as oracle
+    from k3hip.mla_paged import mla_paged_attention
+    for T, H, prefix, lens in ((1, 96, 0, [1, 700, 0]), (5, 12, 64, [90, 70, 69]), (40, 16, 0, [64, 40, 300])):
+        g = torch.Generator().manual_seed(T)
+        case = oracle.make(g, 3, T, H, lens, page=32, pages_dtype=pages, x=F32, prefix=prefix)
+        counts, gate = _whole([1, T, T // 2]), 2 * torch.randn(3, T, H * 128, generator=g).cuda()
+        _sampled(case, mla_paged_attention(**case, counts=counts, gate=gate), range(3), F32, counts=counts, gate=gate)
+
+
+@pytest.mark.parametrize("dtype,x_dtype", [(F16, F32), (F16, BF16), (BF16, F32), (BF16, BF16)])
+def test_a_batch_of_one_place(dtype, x_dtype):
+    """One request, one token a step (tolerances: tests/test_gpu_mla_paged_layer.py)."""
+    from k3hip.mla import new_cache
+    from k3hip.mla_paged import new_cache_paged
+    from k3hip.pages import PageTable
+    from test_gpu_mla_paged_layer import _rel, _rows, _want
+    layer, w = _layer(16)
+    g = torch.Generator().manual_seed(3)
+    t, own = PageTable(1, 256, 8, page_size=32), new_cache(1, 512, 64, 1, dtype=F32)
+    cache = new_cache_paged(t, dtype)
+    for T in (1, 1, 70, 1, 1):
+        x = torch.randn(1, T, HID, generator=g).to(x_dtype).cuda()
+        t.extend(T)
+        out = layer(x, cache)[0]
+        alone, own = layer(x, own)
+        assert out.shape == (1, T, HID) and out.dtype == F32
+        assert _rel(out[0], _want(w, 16, x[0], *_rows(cache, 0), True)) < 2e-5
+        assert _rel(out[0], alone[0].double()) < 4 * (2.0 ** -11 if dtype == F16 else 2.0 ** -8)
