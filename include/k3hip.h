@@ -596,10 +596,11 @@ int64_t k3_mla_paged_workspace_size(int64_t B, int64_t T, int64_t H, int64_t max
  * lengths int32 [B] on the device (taken as 0 .. max_length, at most blocks * page_size), counts int32 [B] on the device (taken as 0 .. T) or
  *   null: T; gate [B, T, H, v] fp32 logits or null: o times sigmoid(gate); out [B, T, H, v] contiguous, out_dtype.
  * A query that sees nothing (also: t >= counts[b]) gets zeros, whatever its gate.  Deterministic.  fp16 pages: the absorbed queries enter as one fp16 term
- * for a bf16 out (2^-11, and none closer than 2^-38 of the largest of its 128 columns), two for fp32 (2^-22); probabilities as one (2^-11) or two
+ * for a bf16 out (2^-11, and none closer than 2^-38 of the row's largest), two for fp32 (2^-22); probabilities as one (2^-11) or two
  * (2^-22), none closer than 2^-32 of the row's largest; for a bf16 out the contexts of ranges of positions as fp16 (2^-11, and no finer than
  * 2^-25, as the pages).  bf16 pages: two bf16 terms of both for a bf16 out (2^-16), three for fp32 (2^-24).  The context before W_UV: two
- * bf16 terms for a bf16 out (2^-16), else three; sums and softmax in fp32.  A masked position's values do not matter, whatever they are.
+ * bf16 terms for a bf16 out (2^-16), else three; sums and softmax in fp32.  A masked position's values do not matter, whatever they are;
+ * one that is seen and holds an infinity or a NaN makes the result NaN, or, where its score is -infinity, may be left out instead.
  * nope a multiple of 8 up to 256, v one up to 1024, H <= 4096, B H <= 65536, max_length <= 2^24.  Pointers 16-byte aligned.
  * Counterpart of MLAAttention.__call__'s core for a batch (air_llm/models/kimi_k3/attention_mla.py:193-212). */
 int k3_mla_paged_attention(const void *q_nope, int64_t qn_batch, int64_t qn_token, int64_t qn_head, const void *q_rot,

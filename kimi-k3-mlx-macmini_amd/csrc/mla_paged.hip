@@ -93,7 +93,8 @@ constexpr int kRound = 32;              // positions of a round of the attention
 constexpr int kStart = 256;             // what an item's start and end cost, in positions
 constexpr int kListLds = (kSearched + 4 * 4 * kCandidates + 16) * 4;
 
-// n / d, 1 / d given: exact for n < 2^23
+// n / d, 1 / d given.  Exact for n < 2^25 (a length and a range's, both up to 2^24) with n / d < 2^21 (ranges are of 32 positions at least,
+// items fewer): n, 1 / d and the product are rounded, 2^-24 each, so the estimate is off by less than 1/2 and one step puts it right.
 __device__ __forceinline__ int divide(int n, int d, float inverse) {
     int c = static_cast<int>(static_cast<float>(n) * inverse);
     return c + ((c + 1) * d <= n ? 1 : c * d > n ? -1 : 0);
@@ -1238,10 +1239,13 @@ int launch_uv_of(const UvArgs &a, hipStream_t st) {
 }
 template <int TERMS>
 int launch_uv(const UvArgs &a, hipStream_t st) {
-    // The most queries to a block, which reads its head's W_UV, with which there are blocks for every CU (of 32 and 16 queries two a CU, of 8 one).
+    // A block reads its head's W_UV: the fewest queries to a block with which all blocks are on the card at once (of 32 and 16 queries two a CU, of 8
+    // one), else 32.
     // Measured, us, 8 / 16 / 32 queries: 32 requests of 64 heads 12.7 / 17.1 / 25.8, 25 of 96 13.4 / 10.2 / 13.4, 64 of 64 13.2 / 9.3 / 12.8, 120 of 64
     // 24.4 / 12.6 / 13.8, 800 of 64 119 / 51.6 / 45.3.  Few queries have waves enough for all a query's records: 6 of 64 heads, some 80 records each,
-    // 16.4 for a wave a query, 11.6 for eight.
+    // 16.4 for a wave a query, 11.6 for eight.  Whole calls, eight waves a query / a wave (8 queries a block): requests of up to 16,384, 64 heads, 4 of
+    // them 32.6 / 45.7, 8 34.0 / 40.3, 12 38.9 / 39.0, 16 42.6 / 40.2; of up to 500 20.3 / 21.1, 23.8 / 22.7, 27.6 / 22.5, 30.1 / 23.7.  With 16 heads
+    // eight waves are the shorter at 16 queries too (30.0 / 37.2), with 96 the longer from 6 on (40.1 / 39.6, 27.7 / 24.3).
     if (a.H * cdiv(a.M, 16) > 512) return launch_uv_of<TERMS, 32>(a, st);
     if (a.H * cdiv(a.M, 8) > 256) return launch_uv_of<TERMS, 16>(a, st);
     if (a.M > 8) return launch_uv_of<TERMS, 8>(a, st);

@@ -16,6 +16,9 @@
 // (kAlone) are then done by the same block, more by a second launch.  Both are bound by latency: dependent loads of lengths, table
 // and list (about 1 us each) and the launch itself.  64 requests of a token each 4.4 us; 48 prompts of up to 8192 tokens 3.4 + 6.8, where a copy
 // would write the 1.6 MB of slots in 0.3.
+// One launch / two, us a call in a graph: 1 request of 2048 tokens 4.0 / 5.8, 4096 4.8 / 5.8, 8192 6.4 / 5.9; 16 of 256 6.0 / 6.5, of 512 7.1 / 6.9; 64 of one
+// 4.8 / 6.5, of 16 5.1 / 6.8.  The rule counts tokens alone: where many requests have few each one launch is the longer (its sixteen waves move
+// the requests' pages one after the other): 64 of 64 12.1 / 8.7, 512 of one 10.3 / 7.8, 2048 of one 26.3 / 11.7.
 #include <algorithm>
 
 #include "k3_common.h"

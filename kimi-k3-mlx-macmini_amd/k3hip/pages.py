@@ -145,7 +145,8 @@ class PageTable:
 
     def share(self, length: int, source: int = 0) -> None:
         """Make the first ``length`` positions of request ``source``, whole pages, the common prefix of the batch: all others, which must
-        hold nothing yet, and whatever takes their places later, begin with them.  The pages stay taken."""
+        hold nothing yet, and whatever takes their places later, begin with them.  The pages stay taken.
+        Reads the lengths on the host.  A graph that was captured before does not know of the prefix: capture its steps anew."""
         n, left = divmod(int(length), self.page_size)
         if left or not 0 < n <= self.table.shape[1]:
             raise ValueError(f"a prefix of {length} positions is not 1 to {self.table.shape[1]} whole pages of {self.page_size}")
